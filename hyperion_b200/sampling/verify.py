@@ -1,0 +1,81 @@
+"""Verification of drafted tokens against the target model's logits, from given random numbers (csrc/verify.cu), and a slow host reference of
+the same rule for tests.
+
+A request brings n drafted tokens and n + 1 rows of logits (row i was computed behind draft i - 1).  With p_i = softmax(row_i / temperature) and
+the drafter's q_i, draft x_i stands when ``uniform_i * q_i(x_i) < p_i(x_i)``; the first that does not is replaced by a draw from max(p_i - q_i, 0),
+and when all stand one more token is drawn from p_n, so that the tokens are distributed as the target's own.  A draw from weights w is
+``argmax_v w_v / noise_v`` with exponentially distributed noise.  Temperature 0: a draft stands when it is its row's largest logit, which follows.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from ..ops.basic import status_word
+from ..ops.native import KernelError, check, is_bf16, library, ptr, require_cuda, stream_ptr
+
+
+CHUNK = 4096  # entries of the vocabulary a block looks through (csrc/verify.cu)
+
+
+def _stride(matrix: Optional[torch.Tensor]) -> ctypes.c_longlong:
+    return ctypes.c_longlong(matrix.stride(0) if matrix is not None else 0)
+
+
+def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.Tensor, uniform: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor, *,
+                  most: int, probabilities: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """How many of each request's drafts stand, [requests] int32, and its tokens, [requests, most] int32: the drafts that stand, the token that
+    follows them, then -1.
+
+    ``logits`` [rows, vocab] float32 or bfloat16; request r has the rows ``row_start[r]`` to ``row_start[r + 1] - 1`` (int32 [requests + 1]), one more
+    than it has drafts; ``most`` is at least the largest such number of rows.  ``drafts`` [rows] int32: the token drafted at each row (a request's
+    last one is not read); ``probabilities`` [rows, vocab] float32: the drafter's at that row, or None where it gave none (its token then counts
+    with probability 1); ``uniform`` [rows] float32 in [0, 1); ``noise`` [requests, vocab] float32, exponentially distributed, above 0;
+    ``temperature`` [requests] float32, 0 for greedy.  A draft outside the vocabulary does not stand and is reported (``raise_on_status``)."""
+    require_cuda(logits, row_start, drafts, uniform, noise, temperature, probabilities)
+    if logits.dim() != 2 or row_start.dim() != 1 or row_start.shape[0] < 1:
+        raise KernelError("verify_drafts: logits [rows, vocab] and row_start [requests + 1]")
+    rows, vocab = logits.shape
+    requests = row_start.shape[0] - 1
+    if logits.stride(1) != 1 or noise.shape != (requests, vocab) or noise.dtype != torch.float32 or noise.stride(1) != 1:
+        raise KernelError("verify_drafts: logits [rows, vocab] and float32 noise [requests, vocab], both with unit inner stride")
+    if probabilities is not None and (probabilities.shape != (rows, vocab) or probabilities.dtype != torch.float32 or probabilities.stride(1) != 1):
+        raise KernelError("verify_drafts: the drafter's probabilities are float32 [rows, vocab] with unit inner stride")
+    for name, t, dtype, count in (("row_start", row_start, torch.int32, requests + 1), ("drafts", drafts, torch.int32, rows), ("uniform", uniform, torch.float32, rows),
+                                  ("temperature", temperature, torch.float32, requests)):
+        if t.dtype != dtype or t.shape != (count,) or not t.is_contiguous():
+            raise KernelError(f"verify_drafts: {name} is a dense {dtype} vector of {count}")
+    if most < 1:
+        raise KernelError("verify_drafts: most counts a request's drafts and the token that follows them")
+    lib = library("verify")
+    answer = torch.empty((requests, 1 + most), dtype=torch.int32, device=logits.device).view(-1)
+    accepted, tokens = answer[:requests], answer[requests:].view(requests, most)
+    workspace = torch.empty(rows * -(-vocab // CHUNK) + 3 * requests, dtype=torch.int64, device=logits.device)
+    check(lib.hb_verify_drafts(ptr(logits), is_bf16(logits), _stride(logits), ptr(row_start), requests, rows, vocab, ptr(drafts), ptr(probabilities),
+                               _stride(probabilities), ptr(uniform), ptr(noise), _stride(noise), ptr(temperature), ptr(workspace), ptr(accepted), ptr(tokens), most,
+                               ptr(status_word(logits.device)), stream_ptr()), "verify_drafts")
+    return accepted, tokens
+
+
+def reference_verify(logits: np.ndarray, drafts: Sequence[int], uniform: Sequence[float], noise: np.ndarray, temperature: float,
+                     probabilities: Optional[np.ndarray] = None) -> tuple[int, list[int]]:
+    """One request by the same rule in float64: (how many drafts stand, those and the token that follows them)."""
+    z = np.asarray(logits, dtype=np.float64).copy()
+    z[np.isnan(z)] = -np.inf
+    z = np.minimum(z, np.finfo(np.float32).max)
+    if temperature == 0:
+        best = z.argmax(1)
+        accepted = next((i for i, x in enumerate(drafts) if x != best[i]), len(drafts))
+        return accepted, [int(x) for x in drafts[:accepted]] + [int(best[accepted])]
+    top = z.max(1, keepdims=True)
+    p = np.where(np.isfinite(top), np.exp((z - np.where(np.isfinite(top), top, 0.0)) / temperature), 0.0)
+    p = p / np.maximum(p.sum(1, keepdims=True), np.finfo(np.float64).tiny)
+    for i, x in enumerate(drafts):
+        q = probabilities[i].astype(np.float64) if probabilities is not None else np.eye(z.shape[1])[x]
+        if not uniform[i] * q[x] < p[i, x]:
+            rest = np.maximum(p[i] - q, 0.0)
+            return i, [int(y) for y in drafts[:i]] + [int(((rest if rest.max() > 0 else p[i]) / noise).argmax())]
+    return len(drafts), [int(x) for x in drafts] + [int((p[len(drafts)] / noise).argmax())]
