@@ -28,6 +28,8 @@ enum : int {
     HB_STATUS_IN_ATTENTION_TMA_TOKENS = 0x800,
     HB_STATUS_IN_ATTENTION_TCGEN05 = 0x1000,
     HB_STATUS_IN_CHUNKED_WALK = 0x2000,
+    HB_STATUS_IN_ATTENTION_STRIPS = 0x4000,
+    HB_STATUS_IN_ATTENTION_SHARED = 0x8000,
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }

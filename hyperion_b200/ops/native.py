@@ -27,6 +27,11 @@ def ptr(tensor: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(tensor.data_ptr())
 
 
+def address(value: int) -> ctypes.c_void_p:
+    """A device address that is no tensor's own start."""
+    return ctypes.c_void_p(value)
+
+
 _bound_stream: list = [None]  # the stream a step has bound for its launches, or None
 
 
