@@ -1,0 +1,684 @@
+// Attention behind shared positions on the 5th-generation tensor cores: items of many rows (attention_shared.cu has the items, the pieces they leave and the kernel
+// for few rows), over paged caches of bfloat16 and of 8-bit records (cache8.cu), head sizes 64 and 128 (HB_HEAD_DIM), pages of 8 to 64 tokens.
+//
+// An item is up to 256 (token, head) rows of one key/value head and a range of keys: all of a group's tokens over a share of the positions that they
+// hold in common, or a portion of a prompt over its own.  One persistent block per SM holds all of the SM's tensor memory and takes every gridDim-th item; two
+// halves of 128 rows (H and L) walk the same tiles of 128 keys, so that the tensor core runs one half's products under the other half's softmax:
+//   warp 0       fetches: one cp.async.bulk.tensor per page (and 128-byte panel) of K and of V, the queries as one 3-D box per 64-column panel;
+//   warp 1       issues S_x = Q_x K^T (M 128, N 128) and O_x += P_x V (P from tensor memory, V MN-major), each half's next S right behind its last product;
+//   warps 2-9    softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by more than 2^8;
+//   warps 10-13  8-bit records only: two warps turn each K tile into bfloat16 (which holds code * 2^e exactly) in the swizzled layout that the products
+//                read, two each V tile; the records' bytes come once from memory and the tensor core sees what it sees over a bfloat16 cache.
+// Weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as much as its own
+// rounding does.  A row of S is 128 float columns of tensor memory and the two parts of its P are 2 x 64, so P takes exactly the place of the S it was
+// made from, 32 keys at a time; the softmax reads S twice (for the maximum, then for the weights), 32 columns under way while it works on 32, which lets 14 warps share
+// the register file (128 registers a thread).
+//
+// Slots beyond an item's range may hold anything: their scores are replaced, and their values are zeros before a product reads them (the warps that convert write
+// them so; over bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded; a wait that runs out sets
+// HB_STATUS_WAIT_EXPIRED, all roles leave their loops, tensor memory is freed and the block returns.
+#include <cuda.h>
+
+#include "common.cuh"
+
+#ifndef HB_HEAD_DIM
+#define HB_HEAD_DIM 128
+#endif
+
+namespace {
+typedef __nv_bfloat16 bf16;
+constexpr int D = HB_HEAD_DIM;
+static_assert(D == 64 || D == 128, "head sizes 64 and 128");
+constexpr int BM = 128;                       // rows of one half = tensor-memory lanes
+constexpr int ROWS = 2 * BM;                  // rows of an item
+constexpr int BN = 128;                       // keys per tile
+constexpr int PANELS = D / 64;
+constexpr int KV_PANEL = BN * 64;             // elements of a 128-key x 64-column panel (16 KB)
+constexpr int Q_PANEL = ROWS * 64;            // elements of a 256-row x 64-column panel of Q (32 KB)
+constexpr int TILE_BYTES = PANELS * KV_PANEL * 2;
+constexpr int RAW_BYTES = BN * D;             // a tile of codes
+constexpr int K_STAGES = 2, RAW_STAGES = 2;
+constexpr int TMEM_COLS = 512;                // S_H [0,128) S_L [128,256) O_H [256,256+D) O_L [384,384+D); P_x over S_x
+constexpr int O_COL = 256;
+constexpr int ITEM_WORDS = 6;                 // first token, tokens, table row, first key, last key + 1, number of the piece
+constexpr unsigned WAIT_LIMIT = 1u << 24;
+constexpr float RESCALE_THRESHOLD = 8.0f;     // in the exp2 domain
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
+    const unsigned addr = smem_u32(bar);
+    for (unsigned spin = 0; spin < WAIT_LIMIT; ++spin) {
+        unsigned done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+        if (done) return true;
+        if ((spin & 1023) == 1023 && *failed) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// The lane that issues the products is one thread, and a lone thread runs a few cycles per instruction: descriptor
+// arithmetic between two products is time the tensor cores stand idle. So descriptors are kept as 32-bit low words that
+// are only added to (the high word is the same for K-major and MN-major tiles with the 128-byte swizzle and 8-row groups
+// 1,024 bytes apart), and four products are issued from one statement.
+constexpr unsigned DESC_HIGH = (unsigned)(1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ unsigned low_k_major(const void* tile) { return ((smem_u32(tile) & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ unsigned low_mn_major(const void* tile, unsigned panel_bytes) { return ((smem_u32(tile) & 0x3FFFFu) >> 4) | ((panel_bytes >> 4) << 16); }
+
+// S = Q K^T over one 64-column panel of the head (4 products of 16 columns); `first` = 0 starts a new S.
+__device__ __forceinline__ void umma_s_panel(unsigned tmem_d, unsigned q_low, unsigned k_low, unsigned idesc, unsigned first) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 al, bl;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
+        "add.u32 al, %1, 2;\n\t"
+        "add.u32 bl, %2, 2;\n\t"
+        "mov.b64 da, {al, %5};\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t"
+        "add.u32 al, %1, 4;\n\t"
+        "add.u32 bl, %2, 4;\n\t"
+        "mov.b64 da, {al, %5};\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t"
+        "add.u32 al, %1, 6;\n\t"
+        "add.u32 bl, %2, 6;\n\t"
+        "mov.b64 da, {al, %5};\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t}"
+        ::"r"(tmem_d), "r"(q_low), "r"(k_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
+}
+// O += P V over 32 keys: the upper parts of P (8 columns per 16 keys), then the lower ones, V MN-major (16 keys = two 8-key groups = 2,048 bytes = 128 units of
+// the descriptor's address field).
+__device__ __forceinline__ void umma_pv_32(unsigned tmem_o, unsigned tmem_p, unsigned v_low, unsigned idesc, unsigned first) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 bl, pa;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 da, {%2, %5};\n\t"
+        "add.u32 bl, %2, 128;\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], da, %3, p;\n\t"
+        "add.u32 pa, %1, 8;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %3, q;\n\t"
+        "add.u32 pa, %1, 16;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], da, %3, q;\n\t"
+        "add.u32 pa, %1, 24;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %3, q;\n\t}"
+        ::"r"(tmem_o), "r"(tmem_p), "r"(v_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
+}
+__device__ __forceinline__ void umma_commit_at(unsigned bar_addr) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr) : "memory");
+}
+// float accumulator, bfloat16 operands, A K-major, M 128, N n; B MN-major when b_mn.
+__device__ __forceinline__ unsigned idesc_for(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(BM >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
+    unsigned r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 32 consecutive columns of this thread's lane, on their way; arrived() says that they are there, and nothing that reads them can stand before it.
+__device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void arrived(unsigned (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void tmem_st32(unsigned taddr, const unsigned (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+                 : "memory");
+}
+// 2^x by the hardware approximation (inputs are <= 8 here; -inf gives 0).
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack_bf16x2(float lo, float hi) {
+    unsigned w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+__device__ __forceinline__ void tmem_st16(unsigned taddr, const float (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+                   "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+                   "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+                   "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
+                 : "memory");
+}
+__device__ __forceinline__ float value_of_half(unsigned short h) {
+    float f;
+    asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(h));
+    return f;
+}
+
+struct Args {
+    const signed char* exponents;  // of an 8-bit cache
+    bf16* out; int out_stride;
+    const int* block_table; int table_width;
+    const int* items; int n_items;  // of each key/value head and head chunk
+    const int* last;                // [tokens]: the last position a token sees, -1 for none
+    const int* piece_start;         // [tokens + 1]
+    float* pieces;                  // [pieces, heads, D], or null: rows have one piece each and are stored at once
+    float2* sums;                   // [pieces, heads]: (m, l)
+    int heads, kv_heads, page_size, pages;
+    int gc, chunks;                 // heads of an item, items of a key/value head's group
+    float scale_log2;
+    int* status;
+};
+
+template <bool E8>
+struct Shape {
+    static constexpr int V_STAGES = E8 ? 1 : 2;
+    static constexpr int WARPS = E8 ? 14 : 10, THREADS = 32 * WARPS;
+    static constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
+    static constexpr int RAW = E8 ? RAW_STAGES * (2 * RAW_BYTES + 2 * BN) : 0;  // codes of K and of V, and their exponents
+    static constexpr size_t USED = 1024 + (size_t)Q_BYTES + (size_t)(K_STAGES + V_STAGES) * TILE_BYTES + RAW + 256;
+    // more than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory
+    static constexpr size_t SMEM = USED > 120 * 1024 ? USED : 120 * 1024;
+    static_assert(USED <= 227 * 1024, "an SM's shared memory");
+};
+
+struct Item {
+    int tok0, ntok, key_lo, key_hi, piece, kvh, first_head, heads_here, start, n_tiles, halves;
+    const int* table;
+};
+
+template <bool E8>
+__global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
+    typedef Shape<E8> S;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* k_ring = base;
+    unsigned char* v_ring = k_ring + (size_t)K_STAGES * TILE_BYTES;
+    unsigned char* qs = v_ring + (size_t)S::V_STAGES * TILE_BYTES;
+    unsigned char* raw_ring = qs + S::Q_BYTES;                      // [RAW_STAGES][K, V] codes
+    unsigned char* exps = raw_ring + (E8 ? RAW_STAGES * 2 * RAW_BYTES : 0);  // [RAW_STAGES][K, V][BN]
+    unsigned long long* k_full = reinterpret_cast<unsigned long long*>(exps + (E8 ? RAW_STAGES * 2 * BN : 0));
+    unsigned long long* k_empty = k_full + 2;
+    unsigned long long* v_full = k_empty + 2;
+    unsigned long long* v_empty = v_full + 2;
+    unsigned long long* raw_full = v_empty + 2;    // [2][K, V]
+    unsigned long long* raw_empty = raw_full + 4;  // [2][K, V]
+    unsigned long long* s_full = raw_empty + 4;    // [2]: per half
+    unsigned long long* p_full = s_full + 2;       // [2]
+    unsigned long long* o_done = p_full + 2;       // [2]
+    unsigned long long* q_full = o_done + 2;
+    unsigned long long* q_empty = q_full + 1;
+    unsigned long long* edge_full = q_empty + 1;   // bfloat16: a V tile whose slots beyond the range are cleared before it is announced
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(edge_full + 1);
+    volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&k_full[s], E8 ? 2 : 1);  // two converting warps, or the copies' bytes
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], E8 ? 2 : 1);
+            mbar_init(&v_empty[s], 1);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 4);
+            mbar_init(&o_done[s], 1);
+        }
+        for (int s = 0; s < 4; ++s) { mbar_init(&raw_full[s], 33); mbar_init(&raw_empty[s], 2); }  // the codes' bytes and 32 lanes' exponents
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(edge_full, 1);
+        *failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // rows of Q that no copy writes (beyond tokens x heads of an item) are computed like the others and never stored
+    for (int e = tid; e < S::Q_BYTES / 16; e += S::THREADS) reinterpret_cast<uint4*>(qs)[e] = make_uint4(0, 0, 0, 0);
+    let_next_kernel_start();
+    wait_for_previous_kernels();
+    // All of the SM's tensor memory, and only now: a block of a kernel further back in the stream that has yet to start on this SM can no longer want any.
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = *tmem_slot;
+    const int shift = 31 - __clz(a.page_size);
+    const int group = a.heads / a.kv_heads, ys = a.kv_heads * a.chunks, total = a.n_items * ys;
+
+    // The roles run through the block's items each at its own pace, held together by the barriers of the data alone.  A wait by parity tells "this phase is over"
+    // only to a thread that is at most one phase behind: every barrier's waiter is the one whose own arrival, on the barrier's counterpart, lets the next
+    // phase begin, or it looks at the barrier once per phase.
+    auto read_item = [&](int index) {
+        Item it;
+        const int* words = a.items + (size_t)(index / ys) * ITEM_WORDS;
+        const int y = index % ys;
+        it.tok0 = words[0], it.ntok = words[1], it.key_lo = words[3], it.key_hi = words[4], it.piece = words[5];
+        it.table = a.block_table + (size_t)words[2] * a.table_width;
+        it.kvh = y / a.chunks;
+        const int chunk = y - it.kvh * a.chunks;
+        it.first_head = it.kvh * group + chunk * a.gc;
+        it.heads_here = min(a.gc, group - chunk * a.gc);
+        it.start = it.key_lo / BN * BN;
+        it.n_tiles = it.key_hi > it.key_lo ? (it.key_hi - it.start + BN - 1) / BN : 0;
+        it.halves = it.ntok * a.gc > BM ? 2 : 1;
+        return it;
+    };
+    auto fail = [&] { *failed = 1; };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ producer (the whole warp)
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+        }
+        const int pages_per_tile = BN >> shift, tokens_per_item = ROWS / a.gc;
+        bool alive = true;
+        int g = 0, edges = 0, round = 0;  // g: tiles so far
+        for (int index = blockIdx.x; index < total && alive; index += gridDim.x, ++round) {
+            const Item it = read_item(index);
+            if (lane == 0) {  // the queries: tokens beyond the item's own come along, or are filled with zeros
+                if (!mbar_wait(q_empty, (round & 1) ^ 1, failed)) alive = false;
+                if (alive) {
+                    mbar_expect_tx(q_full, (unsigned)(PANELS * 128 * a.gc * tokens_per_item));
+                    for (int h = 0; h < PANELS; ++h) tma_load_3d(qs + h * Q_PANEL * 2, &q_map, q_full, h * 64, it.first_head, it.tok0);
+                }
+            }
+            alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
+            for (int t = 0; t < it.n_tiles && alive; ++t, ++g) {
+                const int tile_base = it.start + t * BN;
+                int my_page = -1;
+                const int k0 = tile_base + lane * a.page_size;
+                if (lane < pages_per_tile && k0 < it.key_hi && k0 + a.page_size > it.key_lo) {
+                    const int block = k0 >> shift;
+                    const int id = block < a.table_width ? __ldg(it.table + block) : -1;
+                    if (id >= 0 && id < a.pages) my_page = id;
+                    else atomicOr(a.status, HB_STATUS_BAD_PAGE);
+                }
+                const unsigned valid = __popc(__ballot_sync(0xffffffffu, my_page >= 0));
+                const bool edge = tile_base < it.key_lo || tile_base + BN > it.key_hi;
+                for (int which = 0; which < 2 && alive; ++which) {  // the K tile, then the V tile
+                    const int s = g & 1, turn = g >> 1;
+                    unsigned long long* empty = E8 ? &raw_empty[2 * s + which] : (which ? &v_empty[s] : &k_empty[s]);
+                    unsigned long long* full = E8 ? &raw_full[2 * s + which] : (which ? (edge ? edge_full : &v_full[s]) : &k_full[s]);
+                    int ok = 1;
+                    if (lane == 0) ok = mbar_wait(empty, (turn & 1) ^ 1, failed) ? 1 : 0;
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) { alive = false; break; }
+                    if (lane == 0) {
+                        const unsigned page_bytes = (unsigned)a.page_size * D * (E8 ? 1u : 2u);
+                        if (valid) mbar_expect_tx(full, valid * page_bytes); else mbar_arrive(full);
+                    }
+                    __syncwarp();
+                    if constexpr (E8) {
+                        const int key = lane * 4, from = __shfl_sync(0xffffffffu, my_page, key >> shift);
+                        if (from >= 0) {
+                            const signed char* src = a.exponents + (((size_t)from * 2 + which) * a.kv_heads + it.kvh) * a.page_size + (key & (a.page_size - 1));
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + (2 * s + which) * BN + key)), "l"(src) : "memory");
+                        }
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
+                        if (my_page >= 0)
+                            tma_load_2d(raw_ring + (2 * s + which) * RAW_BYTES + lane * a.page_size * D, &kv_map, full, 0, ((my_page * 2 + which) * a.kv_heads + it.kvh) * a.page_size);
+                    } else {
+                        unsigned char* stage = which ? v_ring + (size_t)s * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
+                        const int ops = pages_per_tile * PANELS;
+                        for (int op0 = 0; op0 < ops; op0 += 32) {
+                            const int op = op0 + lane, p = min(op, ops - 1) / PANELS, h = op % PANELS;
+                            const int from = __shfl_sync(0xffffffffu, my_page, p);
+                            if (op < ops && from >= 0)
+                                tma_load_2d(stage + h * KV_PANEL * 2 + p * a.page_size * 128, &kv_map, full, h * 64, ((from * 2 + which) * a.kv_heads + it.kvh) * a.page_size);
+                        }
+                        if (which && edge) {
+                            ok = mbar_wait(edge_full, edges & 1, failed) ? 1 : 0;
+                            ++edges;
+                            if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+                            for (int e = lane; e < BN * 8 * PANELS; e += 32) {
+                                const int row = (e >> 3) & (BN - 1), pos = tile_base + row;
+                                if (pos < it.key_lo || pos >= it.key_hi) reinterpret_cast<uint4*>(stage)[e] = make_uint4(0, 0, 0, 0);
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&v_full[s]);
+                        }
+                    }
+                }
+            }
+        }
+        if (!alive) fail();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ tensor-core issuer (one lane)
+        if (lane == 0) {
+            const unsigned idesc_s = idesc_for(BN, false), idesc_o = idesc_for(D, true);
+            const unsigned q_low0 = low_k_major(qs), k_low0 = low_k_major(k_ring), v_low0 = low_mn_major(v_ring, KV_PANEL * 2);
+            auto issue_s = [&](int x, int g) {  // S_x = Q_x K(g)^T
+                const unsigned k_low = k_low0 + (unsigned)(g & 1) * (TILE_BYTES >> 4), q_low = q_low0 + (unsigned)x * (BM * 128 >> 4);
+                umma_s_panel(tmem + x * BN, q_low, k_low, idesc_s, 0u);
+#pragma unroll
+                for (int h = 1; h < PANELS; ++h) umma_s_panel(tmem + x * BN, q_low + h * (Q_PANEL * 2 >> 4), k_low + h * (KV_PANEL * 2 >> 4), idesc_s, 1u);
+                umma_commit_at(smem_u32(&s_full[x]));
+            };
+            auto issue_pv = [&](int x, int g, unsigned accumulate) {  // O_x (+)= P_x V(g), both parts of P
+                const unsigned v_low = v_low0 + (unsigned)(g % S::V_STAGES) * (TILE_BYTES >> 4), o = tmem + O_COL + x * BM, p = tmem + x * BN;
+                umma_pv_32(o, p, v_low, idesc_o, accumulate);
+                umma_pv_32(o, p + 32, v_low + 256, idesc_o, 1u);
+                umma_pv_32(o, p + 64, v_low + 512, idesc_o, 1u);
+                umma_pv_32(o, p + 96, v_low + 768, idesc_o, 1u);
+                umma_commit_at(smem_u32(&o_done[x]));
+            };
+            bool ok = true;
+            int g0 = 0, h0[2] = {0, 0}, round = 0;
+            for (int index = blockIdx.x; index < total && ok; index += gridDim.x, ++round) {
+                const Item it = read_item(index);
+                if (!mbar_wait(q_full, round & 1, failed)) { ok = false; break; }
+                if (it.n_tiles == 0) { umma_commit_at(smem_u32(q_empty)); continue; }
+                if (!mbar_wait(&k_full[g0 & 1], (g0 >> 1) & 1, failed)) { ok = false; break; }
+                tc_fence_after();
+                // S_x of the first tile lands in the columns that the last product of the item before read its P from: products of one thread run in the
+                // order of their issue
+                for (int x = 0; x < it.halves; ++x) issue_s(x, g0);
+                umma_commit_at(smem_u32(&k_empty[g0 & 1]));
+                if (it.n_tiles == 1) umma_commit_at(smem_u32(q_empty));
+                for (int j = 0; j < it.n_tiles && ok; ++j) {
+                    const int g = g0 + j;
+                    const bool more = j + 1 < it.n_tiles;
+                    for (int x = 0; x < it.halves && ok; ++x) {
+                        if (!mbar_wait(&p_full[x], (h0[x] + j) & 1, failed)) { ok = false; break; }
+                        if (x == 0 && !mbar_wait(&v_full[g % S::V_STAGES], (g / S::V_STAGES) & 1, failed)) { ok = false; break; }
+                        tc_fence_after();
+                        issue_pv(x, g, j > 0 ? 1u : 0u);
+                        if (x == it.halves - 1) umma_commit_at(smem_u32(&v_empty[g % S::V_STAGES]));
+                        if (more) {
+                            if (x == 0) {
+                                if (!mbar_wait(&k_full[(g + 1) & 1], ((g + 1) >> 1) & 1, failed)) { ok = false; break; }
+                                tc_fence_after();
+                            }
+                            issue_s(x, g + 1);
+                            if (x == it.halves - 1) {
+                                umma_commit_at(smem_u32(&k_empty[(g + 1) & 1]));
+                                if (j + 2 == it.n_tiles) umma_commit_at(smem_u32(q_empty));
+                            }
+                        }
+                    }
+                }
+                g0 += it.n_tiles;
+                h0[0] += it.n_tiles;
+                if (it.halves == 2) h0[1] += it.n_tiles;
+            }
+            if (!ok) fail();
+        }
+    } else if (warp < 10) {
+        // ------------------------------------------------------------------ softmax: thread = row = tensor-memory lane of its half
+        const int x = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane, v = x * BM + r;
+        const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
+        const unsigned s_addr = lane_addr + x * BN, o_addr = lane_addr + O_COL + x * BM;
+        const float scale = a.scale_log2;
+        int hx = 0;  // tiles this half has seen
+        bool ok = true;
+        for (int index = blockIdx.x; index < total && ok; index += gridDim.x) {
+            const Item it = read_item(index);
+            if (x >= it.halves) continue;
+            const int tok = v / a.gc, hh = v - tok * a.gc;
+            const bool row_valid = tok < it.ntok && hh < it.heads_here;
+            // a row that is no one's is computed like the item's last token and never stored: it takes the same way through the code as its neighbours
+            const int token = it.tok0 + min(tok, it.ntok - 1), hi = min(it.key_hi - 1, a.last[token]);
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < it.n_tiles; ++j) {
+                const int h = hx + j;
+                if (!mbar_wait(&s_full[x], h & 1, failed)) { ok = false; break; }
+                tc_fence_after();
+                const int tile_base = it.start + j * BN, last_visible = hi - tile_base, first_visible = it.key_lo - tile_base;
+                const bool masked = !__all_sync(0xffffffffu, last_visible >= BN - 1 && first_visible <= 0);  // one way for the whole warp
+                unsigned s0[32], s1[32];  // of this row's S, 32 columns at hand and 32 on their way
+                auto hide = [&](unsigned (&s)[32], int c) {  // what the row does not see
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[i] = (c + i <= last_visible && c + i >= first_visible) ? s[i] : 0xff800000u;
+                    }
+                };
+                float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto look = [&](unsigned (&s)[32], int c) {
+                    hide(s, c);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(s[i]));
+                };
+                tmem_ld32(s_addr, s0), arrived(s0);
+                tmem_ld32(s_addr + 32, s1), look(s0, 0), arrived(s1);
+                tmem_ld32(s_addr + 64, s0), look(s1, 32), arrived(s0);
+                tmem_ld32(s_addr + 96, s1), look(s0, 64), arrived(s1);
+                tmem_ld32(s_addr + 64, s0), look(s1, 96);
+                const float tmax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * scale;  // the scale is positive: the largest score stays the largest
+                const float m_new = fmaxf(m, tmax);
+                float alpha = 1.f;
+                if (m == -INFINITY) {
+                    m = m_new;  // nothing seen so far: the row of O holds zeros (or is overwritten by the first product)
+                } else if (m_new - m > RESCALE_THRESHOLD) {
+                    alpha = exp2f(m - m_new);
+                    m = m_new;
+                }
+                const float minus_m = m == -INFINITY ? 0.f : -m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                auto weigh = [&](unsigned (&s)[32], int c) {  // P of 32 columns, in two parts, over the columns that they came from
+                    unsigned w[32];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p0 = fast_exp2(fmaf(__uint_as_float(s[2 * i]), scale, minus_m)), p1 = fast_exp2(fmaf(__uint_as_float(s[2 * i + 1]), scale, minus_m));
+                        sum[i & 3] += p0 + p1;
+                        w[i] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+                        w[16 + i] = pack_bf16x2(p0 - __uint_as_float(__float_as_uint(p0) & 0xffff0000u), p1 - __uint_as_float(__float_as_uint(p1) & 0xffff0000u));
+                    }
+                    tmem_st32(s_addr + c, w);
+                };
+                weigh(s1, 96), arrived(s0), hide(s0, 64);
+                tmem_ld32(s_addr + 32, s1), weigh(s0, 64), arrived(s1), hide(s1, 32);
+                tmem_ld32(s_addr, s0), weigh(s1, 32), arrived(s0), hide(s0, 0);
+                weigh(s0, 0);
+                l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                // Every thread sees every phase of o_done go by, tile by tile; the product of tile j - 1 was issued a whole tile ago.
+                if (j > 0 && !mbar_wait(&o_done[x], (h - 1) & 1, failed)) { ok = false; break; }
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    tc_fence_after();  // O may be rescaled only between two products
+#pragma unroll
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        tmem_ld16(o_addr + c, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] *= alpha;
+                        tmem_st16(o_addr + c, o);
+                    }
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
+            }
+            if (ok && it.n_tiles > 0) ok = mbar_wait(&o_done[x], (hx + it.n_tiles - 1) & 1, failed);  // every phase but the item's last was seen in the loop
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            if (ok) {
+                const size_t slot = row_valid && a.pieces ? (size_t)(a.piece_start[token] + it.piece) * a.heads + it.first_head + hh : 0;
+                const float inv = a.pieces ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
+#pragma unroll
+                for (int c = 0; c < D; c += 16) {
+                    float o[16];
+                    if (it.n_tiles > 0) {
+                        tmem_ld16(o_addr + c, o);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = 0.f;
+                    }
+                    if (row_valid && a.pieces) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(a.pieces + slot * D + c + i), "r"(__float_as_uint(o[i])), "r"(__float_as_uint(o[i + 1])),
+                                         "r"(__float_as_uint(o[i + 2])), "r"(__float_as_uint(o[i + 3])), "r"(__float_as_uint(o[i + 4])), "r"(__float_as_uint(o[i + 5])),
+                                         "r"(__float_as_uint(o[i + 6])), "r"(__float_as_uint(o[i + 7])) : "memory");
+                    } else if (row_valid) {
+                        uint2* dst = reinterpret_cast<uint2*>(a.out + (size_t)token * a.out_stride + (size_t)(it.first_head + hh) * D + c);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) dst[i] = make_uint2(pack_bf16x2(o[4 * i] * inv, o[4 * i + 1] * inv), pack_bf16x2(o[4 * i + 2] * inv, o[4 * i + 3] * inv));
+                    }
+                }
+                if (row_valid && a.pieces) a.sums[slot] = make_float2(m, l);
+                // the row is out of tensor memory before this thread hands over the next item's first P, and only then is O written anew
+                tc_fence_before();
+            }
+            hx += it.n_tiles;
+        }
+        if (!ok) fail();
+    } else if constexpr (E8) {
+        // ------------------------------------------------------------------ codes into bfloat16: warps 10 and 11 the K tiles, 12 and 13 the V tiles
+        const int which = (warp - 10) >> 1, w = warp & 1;
+        constexpr int CHUNKS = D / 16;  // 16 codes each, of a row
+        bool ok = true;
+        int g = 0;
+        for (int index = blockIdx.x; index < total && ok; index += gridDim.x) {
+            const Item it = read_item(index);
+            for (int t = 0; t < it.n_tiles; ++t, ++g) {
+                const int s = g & 1, turn = g >> 1, tile_base = it.start + t * BN;
+                const int vs = g % S::V_STAGES, v_turn = g / S::V_STAGES;
+                ok = mbar_wait(&raw_full[2 * s + which], turn & 1, failed) && mbar_wait(which ? &v_empty[vs] : &k_empty[s], ((which ? v_turn : turn) & 1) ^ 1, failed);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const unsigned char* raw = raw_ring + (2 * s + which) * RAW_BYTES;
+                const signed char* e8 = reinterpret_cast<const signed char*>(exps + (2 * s + which) * BN);
+                unsigned char* tile = which ? v_ring + (size_t)vs * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
+                // eight lanes take a 16-byte chunk of eight rows: the swizzles of both layouts put those in different banks
+#pragma unroll 4
+                for (int i = 0; i < BN / 8 * CHUNKS / 8; ++i) {
+                    const int octet = (i * 2 + w) * 4 + (lane >> 3), chunk = octet % CHUNKS, row = octet / CHUNKS * 8 + (lane & 7);
+                    const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+                    const int e = min(max((int)e8[row], -40), 40);
+                    const float factor = __uint_as_float((unsigned)(127 + e) << 23);
+                    const bool keep = which == 0 || (tile_base + row >= it.key_lo && tile_base + row < it.key_hi);
+                    const unsigned* words = reinterpret_cast<const unsigned*>(&codes);
+                    unsigned wide[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        unsigned h0, h1;
+                        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
+                        wide[2 * k] = pack_bf16x2(value_of_half((unsigned short)h0) * factor, value_of_half((unsigned short)(h0 >> 16)) * factor);
+                        wide[2 * k + 1] = pack_bf16x2(value_of_half((unsigned short)h1) * factor, value_of_half((unsigned short)(h1 >> 16)) * factor);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int oc = 2 * chunk + half;
+                        uint4 out = make_uint4(wide[4 * half], wide[4 * half + 1], wide[4 * half + 2], wide[4 * half + 3]);
+                        if (!keep) out = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(tile + (oc >> 3) * (KV_PANEL * 2) + row * 128 + (((oc & 7) ^ (row & 7)) << 4)) = out;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(which ? &v_full[vs] : &k_full[s]);
+                    mbar_arrive(&raw_empty[2 * s + which]);
+                }
+            }
+        }
+        if (!ok) fail();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && *failed) atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_SHARED);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = nullptr;
+    if (!fn) {
+        void* found = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &found, cudaEnableDefault, &result) == cudaSuccess &&
+            result == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(found);
+    }
+    return fn;
+}
+
+template <bool E8>
+int launch(const Args& a, const void* q, int q_stride, int n_tokens, const void* cache, cudaStream_t stream) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return HB_BAD_ARGUMENT;
+    // the cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and up to 128 bytes
+    CUtensorMap map, q_map;
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)a.pages * 2 * a.kv_heads * a.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * (E8 ? 1 : 2)};
+    const cuuint32_t box[2] = {(cuuint32_t)(E8 ? D : 64), (cuuint32_t)a.page_size};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    if (encode(&map, E8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               E8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return HB_BAD_ARGUMENT;
+    // the queries as (column, head, token): an item's box is 64 columns of gc heads of its tokens
+    const cuuint64_t q_dims[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)n_tokens};
+    const cuuint64_t q_strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)q_stride * 2};
+    const cuuint32_t q_box[3] = {64, (cuuint32_t)a.gc, (cuuint32_t)(ROWS / a.gc)};
+    if (encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), q_dims, q_strides, q_box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return HB_BAD_ARGUMENT;
+    static const cudaError_t configured = cudaFuncSetAttribute(attention_shared_kernel<E8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8>::SMEM);
+    if (configured != cudaSuccess) return (int)configured;
+    int device = 0, sms = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return HB_BAD_ARGUMENT;
+    const long long total = (long long)a.n_items * a.kv_heads * a.chunks;
+    if (total > 0x7fffffffLL - sms) return HB_UNSUPPORTED_SIZE;
+    return launch_after_previous(attention_shared_kernel<E8>, dim3((unsigned)(total < sms ? total : sms)), dim3(Shape<E8>::THREADS), Shape<E8>::SMEM, stream, map, q_map, a);
+}
+}  // namespace
+
+// cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
+// items [n_items, 6]: see ITEM_WORDS; an item has at most 256 / min(heads / kv_heads, 256) tokens.  pieces, sums null: one piece a row.
+HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_tokens, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table,
+                                        int table_width, const int* items, int n_items, const int* last, const int* piece_start, float* pieces, float* sums, int heads,
+                                        int kv_heads, int page_size, int pages, float scale, int* status, cudaStream_t stream) {
+    if (n_items <= 0) return 0;
+    if (!q || !out || !cache || !block_table || !items || !last || !piece_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || n_tokens <= 0 || q_stride % 8 || out_stride % 4) return HB_BAD_ARGUMENT;
+    if (!(scale > 0.f)) return HB_BAD_ARGUMENT;  // the row maximum is taken before the scores are scaled
+    if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
+    if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)pieces & 31) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
+    if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
+    const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
+    const Args a{(const signed char*)exponents, (bf16*)out, out_stride, block_table, table_width, items, n_items, last, piece_start, pieces, (float2*)sums,
+                 heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
+    return exponents ? launch<true>(a, q, q_stride, n_tokens, cache, stream) : launch<false>(a, q, q_stride, n_tokens, cache, stream);
+}

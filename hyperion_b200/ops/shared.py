@@ -19,9 +19,12 @@ from .cache8 import Cache8, check_cache8
 from .native import KernelError, check, f32, library, ptr, require_cuda, sm_count, stream_ptr
 
 STRIP_ROWS = 16    # (token, head) rows of a strip
-KEY_TILE = 64      # keys of a strip kernel's stage
-LEAST_TILES = 3    # of a range that is cut further
-BLOCKS_PER_SM = 2  # of the strip kernel
+TILE_ROWS = 256    # of an item of the tile kernel
+STRIP_KEYS, TILE_KEYS = 64, 128  # keys of a stage
+LEAST_KEYS = 192   # of a range that is cut further
+STRIPS_PER_SM = 2  # blocks of the strip kernel that share an SM
+MOST_STRIP_ROWS = 64
+ITEM_WORDS = 6
 
 
 def supported(head_dim: int, page_size: int) -> bool:
@@ -31,20 +34,52 @@ def supported(head_dim: int, page_size: int) -> bool:
 class SharedPlan:
     """What the launches of a step need: the items, the last position each token sees and the first piece of each token, in one int32 tensor."""
 
-    __slots__ = ("tokens", "rows", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strips", "data", "strips_at", "last_at", "starts_at")
+    __slots__ = ("tokens", "rows", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strips", "tiles", "data", "strips_at", "tiles_at", "last_at", "starts_at")
 
 
-def _cut(first, last, tiles_each):
-    """Ranges [first, last) cut into shares of about ``tiles_each`` key tiles on tile boundaries: (source range, share's number, first key, last key + 1)."""
-    base = first // KEY_TILE
-    tiles = -(-last // KEY_TILE) - base
-    shares = np.maximum(1, -(-tiles // tiles_each))
+def _tiles_of(first, last, keys):
+    return -(-last // keys) - first // keys
+
+
+def _strip_share(ranges, cuts, across, sms) -> int:
+    """Key tiles of a strip's share: so many that the blocks fill the device once."""
+    work = int((cuts * _tiles_of(ranges[:, 3], ranges[:, 4], STRIP_KEYS)).sum()) * across
+    return max(LEAST_KEYS // STRIP_KEYS, -(-work // (STRIPS_PER_SM * sms)))
+
+
+ITEM_OVERHEAD = 3  # what an item of the tile kernel costs beside its key tiles, in key tiles: its queries' way in, its rows' way out, the first tile's latency
+
+
+def _tile_share(ranges, cuts, across, sms) -> int:
+    """Key tiles of a tile item's share: the longest that lets the items fill the device in one to four turns, whichever is soonest done."""
+    tiles = _tiles_of(ranges[:, 3], ranges[:, 4], TILE_KEYS)
+    longest = int(tiles.max())
+    best = None
+    for turns in range(1, 5):
+        low, high = 1, longest  # the smallest share with no more items than that
+        while low < high:
+            middle = (low + high) // 2
+            if int((cuts * -(-tiles // middle)).sum()) * across <= turns * sms:
+                high = middle
+            else:
+                low = middle + 1
+        items = int((cuts * -(-tiles // low)).sum()) * across
+        time = -(-items // sms) * (low + ITEM_OVERHEAD)
+        if best is None or time < best[0]:
+            best = time, low
+    return max(2, best[1])
+
+
+def _cut(first, last, keys, share):
+    """Ranges [first, last) cut on tile boundaries into shares of about ``share`` tiles of ``keys``: (shares of each, source range, share's number, first key, last key + 1)."""
+    base, tiles = first // keys, _tiles_of(first, last, keys)
+    shares = np.maximum(1, -(-tiles // share))
     each = -(-tiles // shares)
     shares = -(-tiles // each)  # no share is empty
     source = np.repeat(np.arange(len(first)), shares)
     number = np.arange(len(source)) - np.repeat(np.cumsum(shares) - shares, shares)
-    low = np.maximum(first[source], (base[source] + number * each[source]) * KEY_TILE)
-    high = np.minimum(last[source], (base[source] + (number + 1) * each[source]) * KEY_TILE)
+    low = np.maximum(first[source], (base[source] + number * each[source]) * keys)
+    high = np.minimum(last[source], (base[source] + (number + 1) * each[source]) * keys)
     return shares, source, number, low, high
 
 
@@ -60,7 +95,7 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
         raise KernelError(f"plan_shared: {heads} query heads do not divide over {kv_heads} key/value heads")
     requests, total = len(n), int(n.sum())
-    if length.size and int(length.max()) > 2**31 - 1 - KEY_TILE:
+    if length.size and int(length.max()) > 2**31 - 1 - TILE_KEYS:
         raise KernelError("plan_shared: a position fits 32 bits")
     start = np.concatenate([[0], np.cumsum(n)])
     own_from = np.zeros(requests, dtype=np.int64)
@@ -81,39 +116,52 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     # ranges: (first token, tokens, table row, first key, last key + 1)
     ranges = np.concatenate([np.stack([group_ranges[:, 0], group_ranges[:, 1], group_ranges[:, 2], 0 * group_ranges[:, 3], group_ranges[:, 3]], 1),
                              np.stack([start[live], n[live], live, own_from[live], length[live]], 1)])
-    group = heads // kv_heads
-    per, across = max(1, STRIP_ROWS // group), kv_heads * -(-group // STRIP_ROWS)  # tokens of a strip, strips beside one another
-    cuts = -(-ranges[:, 1] // per)
-    tiles = -(-ranges[:, 4] // KEY_TILE) - ranges[:, 3] // KEY_TILE
-    work = int((cuts * tiles).sum()) * across
-    share = max(LEAST_TILES, -(-work // (BLOCKS_PER_SM * (sms or sm_count(device)))))
-    shares, source, number, low, high = _cut(ranges[:, 3], ranges[:, 4], share)
+    group, sms = heads // kv_heads, sms or sm_count(device)
+    shares, kinds = np.ones(len(ranges), dtype=np.int64), []
+    wide = ranges[:, 1] * group > MOST_STRIP_ROWS
+    for chosen, rows, keys, choose in ((np.flatnonzero(~wide), STRIP_ROWS, STRIP_KEYS, _strip_share), (np.flatnonzero(wide), TILE_ROWS, TILE_KEYS, _tile_share)):
+        of_kind, per = ranges[chosen], max(1, rows // group)  # tokens of an item
+        cuts = -(-of_kind[:, 1] // per)
+        if len(chosen):
+            parts, source, number, low, high = _cut(of_kind[:, 3], of_kind[:, 4], keys, choose(of_kind, cuts, kv_heads * -(-group // rows), sms))
+            shares[chosen] = parts
+            kinds.append((of_kind, chosen, per, cuts, source, number, low, high))
+        else:
+            kinds.append(None)
     # a token's pieces: its group's shares, then its own request's
     of_group = np.zeros(requests, dtype=np.int64)
     for k, (*_, first, members) in enumerate(groups):
         of_group[first: first + members] = shares[k]
     of_own = np.zeros(requests, dtype=np.int64)
     of_own[live] = shares[len(groups):]
-    number = number + np.concatenate([np.zeros(len(groups), dtype=np.int64), of_group[live]])[source]
+    before = np.concatenate([np.zeros(len(groups), dtype=np.int64), of_group[live]])
     token_pieces = np.repeat(of_group + of_own, n)
     starts = np.concatenate([[0], np.cumsum(token_pieces)])
-    # strips: every share of a range for every run of `per` tokens of it
-    times = cuts[source]
-    at = np.repeat(np.arange(len(source)), times)
-    run = np.arange(len(at)) - np.repeat(np.cumsum(times) - times, times)
-    tok = ranges[source[at], 0] + run * per
-    items = np.stack([tok, np.minimum(per, ranges[source[at], 0] + ranges[source[at], 1] - tok), ranges[source[at], 2], low[at], high[at], number[at]], 1)
+    # items: every share of a range for every run of `per` tokens of it, the longest first
+    items = []
+    for kind in kinds:
+        if kind is None:
+            items.append(np.zeros((0, ITEM_WORDS), dtype=np.int64))
+            continue
+        of_kind, chosen, per, cuts, source, number, low, high = kind
+        times = cuts[source]
+        at = np.repeat(np.arange(len(source)), times)
+        run = np.arange(len(at)) - np.repeat(np.cumsum(times) - times, times)
+        of = of_kind[source[at]]
+        tok = of[:, 0] + run * per
+        made = np.stack([tok, np.minimum(per, of[:, 0] + of[:, 1] - tok), of[:, 2], low[at], high[at], (number + before[chosen][source])[at]], 1)
+        items.append(made[np.argsort(made[:, 3] - made[:, 4], kind="stable")])
     last = np.arange(total) - np.repeat(start[:-1], n) + np.repeat(length - n, n)
 
     plan = SharedPlan()
     plan.tokens, plan.rows, plan.heads, plan.kv_heads, plan.head_dim = total, requests, heads, kv_heads, head_dim
     plan.longest = int(length[n > 0].max()) if total else 0
     plan.pieces, plan.joined = int(starts[-1]), bool((token_pieces != 1).any())
-    plan.strips = len(items)
-    flat = np.concatenate([items.ravel(), last, starts]).astype(np.int32)
-    plan.data = torch.from_numpy(flat).to(device)
-    base = plan.data.data_ptr()
-    plan.strips_at, plan.last_at, plan.starts_at = base, base + 4 * items.size, base + 4 * (items.size + total)
+    plan.strips, plan.tiles = len(items[0]), len(items[1])
+    parts = [items[0].ravel(), items[1].ravel(), last, starts]
+    plan.data = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device)
+    at = plan.data.data_ptr() + 4 * np.concatenate([[0], np.cumsum([len(part) for part in parts])])
+    plan.strips_at, plan.tiles_at, plan.last_at, plan.starts_at = (int(x) for x in at[:4])
     return plan
 
 
@@ -156,6 +204,11 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
         workspace = torch.empty(max(1, plan.pieces * heads * (head_dim + 2)), dtype=torch.float32, device=q.device)
         pieces = workspace.data_ptr()
         sums = pieces + 4 * plan.pieces * heads * head_dim
+    if plan.tiles:
+        check(library("attention_shared_tiles", HB_HEAD_DIM=head_dim).hb_attention_shared_tiles(
+            ptr(q), q.stride(0), plan.tokens, ptr(out), out.stride(0), ptr(entries), ptr(exponents), ptr(block_table), block_table.shape[1], native.address(plan.tiles_at),
+            plan.tiles, native.address(plan.last_at), native.address(plan.starts_at), native.address(pieces), native.address(sums), heads, kv_heads, page_size, pages, f32(scale),
+            ptr(status_word(q.device)), stream), "attention_shared")
     if plan.strips:
         check(lib.hb_attention_strips(ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(entries), ptr(exponents), ptr(block_table), block_table.shape[1],
                                       native.address(plan.strips_at), plan.strips, native.address(plan.last_at), native.address(plan.starts_at), native.address(pieces),

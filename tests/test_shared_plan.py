@@ -9,7 +9,7 @@ from hyperion_b200.ops import KernelError, plan_shared
 
 def items_of(plan):
     flat = plan.data.numpy()
-    n = plan.strips * 6
+    n = (plan.strips + plan.tiles) * 6
     return flat[:n].reshape(-1, 6), flat[n: n + plan.tokens], flat[n + plan.tokens: n + 2 * plan.tokens + 1]
 
 
@@ -21,8 +21,9 @@ def covered(counts, lengths, heads, kv, groups, sms):
         shared[first: first + n] = positions
     owner = np.repeat(np.arange(len(counts)), counts)
     seen, pieces = [set() for _ in owner], [[] for _ in owner]
-    for tok, n, row, low, high, number in items:
-        assert n >= 1 and high > low and n * min(16, heads // kv) <= 16
+    for i, (tok, n, row, low, high, number) in enumerate(items):
+        rows = 16 if i < plan.strips else 256
+        assert n >= 1 and high > low and n * min(rows, heads // kv) <= rows
         for t in range(tok, tok + n):
             assert row == owner[t] or (high <= shared[owner[t]] == shared[row])  # another request's table for shared positions only
             assert not seen[t] & set(range(low, high))
