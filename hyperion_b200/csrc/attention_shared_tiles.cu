@@ -6,13 +6,16 @@
 // halves of 128 rows (H and L) walk the same tiles of 128 keys, so that the tensor core runs one half's products under the other half's softmax:
 //   warp 0       fetches: one cp.async.bulk.tensor per page (and 128-byte panel) of K and of V, the queries as one 3-D box per 64-column panel;
 //   warp 1       issues S_x = Q_x K^T (M 128, N 128) and O_x += P_x V (P from tensor memory, V MN-major), each half's next S right behind its last product;
-//   warps 2-9    softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by more than 2^8;
-//   warps 10-13  8-bit records only: two warps turn each K tile into bfloat16 (which holds code * 2^e exactly) in the swizzled layout that the products
-//                read, two each V tile; the records' bytes come once from memory and the tensor core sees what it sees over a bfloat16 cache.
-// Weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as much as its own
-// rounding does.  A row of S is 128 float columns of tensor memory and the two parts of its P are 2 x 64, so P takes exactly the place of the S it was
-// made from, 32 keys at a time; the softmax reads S twice (for the maximum, then for the weights), 32 columns under way while it works on 32, which lets 14 warps share
-// the register file (128 registers a thread).
+//   warps 4-11   softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by much;
+//   warps 12-19  8-bit records only: four warps turn each K tile into bfloat16 (which holds code * 2^e exactly) in the swizzled layout that the products
+//                read, four each V tile; the records' bytes come once from memory.
+// Over bfloat16 values, weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as
+// much as its own rounding does.  8-bit values go as float16, which holds code * 2^(e - e0) exactly for exponents from e0 - 12 to e0 + 7 (e0: the largest of
+// the item's first tile; the result is scaled back at the end), and so do the weights, whose rounding then does not show and whose second part is not
+// needed.  A tile with exponents beyond that range goes the way of bfloat16 values.
+// A row of S is 128 float columns of tensor memory and the two parts of its P are 2 x 64, so P takes exactly the place of the S it was made from, 32 keys at a
+// time; the softmax reads S twice (for the maximum, then for the weights), 32 columns under way while it works on 32, which lets 20 warps share the register
+// file.  P is handed over in two halves of the tile's keys, so that the product of the first runs under the making of the second.
 //
 // Slots beyond an item's range may hold anything: their scores are replaced, and their values are zeros before a product reads them (the warps that convert write
 // them so; over bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded; a wait that runs out sets
@@ -37,12 +40,11 @@ constexpr int KV_PANEL = BN * 64;             // elements of a 128-key x 64-colu
 constexpr int Q_PANEL = ROWS * 64;            // elements of a 256-row x 64-column panel of Q (32 KB)
 constexpr int TILE_BYTES = PANELS * KV_PANEL * 2;
 constexpr int RAW_BYTES = BN * D;             // a tile of codes
-constexpr int K_STAGES = 2, RAW_STAGES = 2;
+constexpr int STAGES = 2;                     // of K tiles and of V tiles as the products read them; one tile of codes of each is under way
 constexpr int TMEM_COLS = 512;                // S_H [0,128) S_L [128,256) O_H [256,256+D) O_L [384,384+D); P_x over S_x
 constexpr int O_COL = 256;
 constexpr int ITEM_WORDS = 6;                 // first token, tokens, table row, first key, last key + 1, number of the piece
 constexpr unsigned WAIT_LIMIT = 1u << 24;
-constexpr float RESCALE_THRESHOLD = 8.0f;     // in the exp2 domain
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
@@ -131,12 +133,26 @@ __device__ __forceinline__ void umma_pv_32(unsigned tmem_o, unsigned tmem_p, uns
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %3, q;\n\t}"
         ::"r"(tmem_o), "r"(tmem_p), "r"(v_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
 }
+// The same with P in one part.
+__device__ __forceinline__ void umma_pv_32_whole(unsigned tmem_o, unsigned tmem_p, unsigned v_low, unsigned idesc, unsigned first) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t.reg .b32 bl, pa;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t"
+        "add.u32 bl, %2, 128;\n\t"
+        "add.u32 pa, %1, 8;\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %3, q;\n\t}"
+        ::"r"(tmem_o), "r"(tmem_p), "r"(v_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
+}
 __device__ __forceinline__ void umma_commit_at(unsigned bar_addr) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr) : "memory");
 }
-// float accumulator, bfloat16 operands, A K-major, M 128, N n; B MN-major when b_mn.
-__device__ __forceinline__ unsigned idesc_for(int n, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(BM >> 4) << 24);
+// float accumulator, both operands bfloat16 or both float16, A K-major, M 128, N n; B MN-major when b_mn.
+__device__ __forceinline__ unsigned idesc_for(int n, bool b_mn, bool f16) {
+    return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(BM >> 4) << 24);
 }
 __device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
     unsigned r[16];
@@ -174,12 +190,38 @@ __device__ __forceinline__ unsigned pack_bf16x2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
     return w;
 }
-__device__ __forceinline__ void tmem_st16(unsigned taddr, const float (&v)[16]) {
+__device__ __forceinline__ unsigned pack_f16x2(float lo, float hi) {
+    unsigned w;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+// Two floats at a time.
+struct Pair { float x, y; };
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("{.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void tmem_st16_words(unsigned taddr, const unsigned (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(taddr), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
-                   "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
-                   "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
-                   "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
 __device__ __forceinline__ float value_of_half(unsigned short h) {
@@ -205,15 +247,22 @@ struct Args {
 
 template <bool E8>
 struct Shape {
-    static constexpr int V_STAGES = E8 ? 1 : 2;
-    static constexpr int WARPS = E8 ? 14 : 10, THREADS = 32 * WARPS;
+    static constexpr int WARPS = E8 ? 20 : 12, THREADS = 32 * WARPS;
+    // Registers a thread, by groups of four warps, of the 96 that 640 threads are launched with (128 * 56 + 256 * 152 + 256 * 56 = 60,416 of 61,440)
+    [[maybe_unused]] static constexpr int FEW = 56, MANY = 152, CONVERTING = 56;
     static constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
-    static constexpr int RAW = E8 ? RAW_STAGES * (2 * RAW_BYTES + 2 * BN) : 0;  // codes of K and of V, and their exponents
-    static constexpr size_t USED = 1024 + (size_t)Q_BYTES + (size_t)(K_STAGES + V_STAGES) * TILE_BYTES + RAW + 256;
+    // How far (in powers of two) a maximum may be outgrown before the row is rescaled.  A stale maximum changes no result (numerator and denominator use the same
+    // one) as long as nothing overflows: weights are float16 up to 2^15, or bfloat16 and their sums float.
+    static constexpr float OUTGROWN = E8 ? 13.f : 32.f;
+    static constexpr int RAW = E8 ? 2 * RAW_BYTES + 2 * BN : 0;  // codes of K and of V, and their exponents
+    static constexpr size_t USED = 1024 + (size_t)Q_BYTES + (size_t)2 * STAGES * TILE_BYTES + RAW + 256;
     // more than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory
     static constexpr size_t SMEM = USED > 120 * 1024 ? USED : 120 * 1024;
     static_assert(USED <= 227 * 1024, "an SM's shared memory");
 };
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 struct Item {
     int tok0, ntok, key_lo, key_hi, piece, kvh, first_head, heads_here, start, n_tiles, halves;
@@ -226,37 +275,42 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* k_ring = base;
-    unsigned char* v_ring = k_ring + (size_t)K_STAGES * TILE_BYTES;
-    unsigned char* qs = v_ring + (size_t)S::V_STAGES * TILE_BYTES;
-    unsigned char* raw_ring = qs + S::Q_BYTES;                      // [RAW_STAGES][K, V] codes
-    unsigned char* exps = raw_ring + (E8 ? RAW_STAGES * 2 * RAW_BYTES : 0);  // [RAW_STAGES][K, V][BN]
-    unsigned long long* k_full = reinterpret_cast<unsigned long long*>(exps + (E8 ? RAW_STAGES * 2 * BN : 0));
+    unsigned char* v_ring = k_ring + (size_t)STAGES * TILE_BYTES;
+    unsigned char* qs = v_ring + (size_t)STAGES * TILE_BYTES;
+    unsigned char* raw_tiles = qs + S::Q_BYTES;              // [K, V] codes
+    unsigned char* exps = raw_tiles + (E8 ? 2 * RAW_BYTES : 0);  // [K, V][BN]
+    unsigned long long* k_full = reinterpret_cast<unsigned long long*>(exps + (E8 ? 2 * BN : 0));
     unsigned long long* k_empty = k_full + 2;
     unsigned long long* v_full = k_empty + 2;
     unsigned long long* v_empty = v_full + 2;
-    unsigned long long* raw_full = v_empty + 2;    // [2][K, V]
-    unsigned long long* raw_empty = raw_full + 4;  // [2][K, V]
-    unsigned long long* s_full = raw_empty + 4;    // [2]: per half
-    unsigned long long* p_full = s_full + 2;       // [2]
-    unsigned long long* o_done = p_full + 2;       // [2]
-    unsigned long long* q_full = o_done + 2;
+    unsigned long long* raw_full = v_empty + 2;    // [K, V]
+    unsigned long long* raw_empty = raw_full + 2;  // [K, V]
+    unsigned long long* s_full = raw_empty + 2;    // [2]: per half
+    unsigned long long* p_full = s_full + 2;       // [2][2]: the P of the tile's upper keys, then of its lower ones
+    unsigned long long* o_done = p_full + 4;       // [2]: the item's last product
+    unsigned long long* kind_full = o_done + 2;    // [2]: 8-bit: what the V tile will be is known
+    unsigned long long* q_full = kind_full + 2;
     unsigned long long* q_empty = q_full + 1;
     unsigned long long* edge_full = q_empty + 1;   // bfloat16: a V tile whose slots beyond the range are cleared before it is announced
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(edge_full + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* kinds = failed + 1;  // [2]: 2 * (e0 + 64) + whether the tile's values are float16
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&k_full[s], E8 ? 2 : 1);  // two converting warps, or the copies' bytes
+            mbar_init(&k_full[s], E8 ? 4 : 1);  // four converting warps, or the copies' bytes
             mbar_init(&k_empty[s], 1);
-            mbar_init(&v_full[s], E8 ? 2 : 1);
+            mbar_init(&v_full[s], E8 ? 4 : 1);
+            mbar_init(&raw_full[s], 33);        // the codes' bytes and 32 lanes' exponents
+            mbar_init(&raw_empty[s], 4);
             mbar_init(&v_empty[s], 1);
             mbar_init(&s_full[s], 1);
-            mbar_init(&p_full[s], 4);
+            mbar_init(&p_full[2 * s], 4);
+            mbar_init(&p_full[2 * s + 1], 4);
             mbar_init(&o_done[s], 1);
+            mbar_init(&kind_full[s], 1);
         }
-        for (int s = 0; s < 4; ++s) { mbar_init(&raw_full[s], 33); mbar_init(&raw_empty[s], 2); }  // the codes' bytes and 32 lanes' exponents
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(edge_full, 1);
@@ -300,7 +354,9 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
     };
     auto fail = [&] { *failed = 1; };
 
-    if (warp == 0) {
+    if (warp < 4) {
+      if constexpr (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::FEW));
+      if (warp == 0) {
         // ------------------------------------------------------------------ producer (the whole warp)
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
@@ -333,10 +389,10 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                 const bool edge = tile_base < it.key_lo || tile_base + BN > it.key_hi;
                 for (int which = 0; which < 2 && alive; ++which) {  // the K tile, then the V tile
                     const int s = g & 1, turn = g >> 1;
-                    unsigned long long* empty = E8 ? &raw_empty[2 * s + which] : (which ? &v_empty[s] : &k_empty[s]);
-                    unsigned long long* full = E8 ? &raw_full[2 * s + which] : (which ? (edge ? edge_full : &v_full[s]) : &k_full[s]);
+                    unsigned long long* empty = E8 ? &raw_empty[which] : (which ? &v_empty[s] : &k_empty[s]);
+                    unsigned long long* full = E8 ? &raw_full[which] : (which ? (edge ? edge_full : &v_full[s]) : &k_full[s]);
                     int ok = 1;
-                    if (lane == 0) ok = mbar_wait(empty, (turn & 1) ^ 1, failed) ? 1 : 0;
+                    if (lane == 0) ok = mbar_wait(empty, ((E8 ? g : turn) & 1) ^ 1, failed) ? 1 : 0;
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) { alive = false; break; }
                     if (lane == 0) {
@@ -348,11 +404,11 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                         const int key = lane * 4, from = __shfl_sync(0xffffffffu, my_page, key >> shift);
                         if (from >= 0) {
                             const signed char* src = a.exponents + (((size_t)from * 2 + which) * a.kv_heads + it.kvh) * a.page_size + (key & (a.page_size - 1));
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + (2 * s + which) * BN + key)), "l"(src) : "memory");
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + which * BN + key)), "l"(src) : "memory");
                         }
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
                         if (my_page >= 0)
-                            tma_load_2d(raw_ring + (2 * s + which) * RAW_BYTES + lane * a.page_size * D, &kv_map, full, 0, ((my_page * 2 + which) * a.kv_heads + it.kvh) * a.page_size);
+                            tma_load_2d(raw_tiles + which * RAW_BYTES + lane * a.page_size * D, &kv_map, full, 0, ((my_page * 2 + which) * a.kv_heads + it.kvh) * a.page_size);
                     } else {
                         unsigned char* stage = which ? v_ring + (size_t)s * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
                         const int ops = pages_per_tile * PANELS;
@@ -379,10 +435,10 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             }
         }
         if (!alive) fail();
-    } else if (warp == 1) {
+      } else if (warp == 1) {
         // ------------------------------------------------------------------ tensor-core issuer (one lane)
         if (lane == 0) {
-            const unsigned idesc_s = idesc_for(BN, false), idesc_o = idesc_for(D, true);
+            const unsigned idesc_s = idesc_for(BN, false, false), idesc_o = idesc_for(D, true, false), idesc_half = idesc_for(D, true, true);
             const unsigned q_low0 = low_k_major(qs), k_low0 = low_k_major(k_ring), v_low0 = low_mn_major(v_ring, KV_PANEL * 2);
             auto issue_s = [&](int x, int g) {  // S_x = Q_x K(g)^T
                 const unsigned k_low = k_low0 + (unsigned)(g & 1) * (TILE_BYTES >> 4), q_low = q_low0 + (unsigned)x * (BM * 128 >> 4);
@@ -391,13 +447,15 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                 for (int h = 1; h < PANELS; ++h) umma_s_panel(tmem + x * BN, q_low + h * (Q_PANEL * 2 >> 4), k_low + h * (KV_PANEL * 2 >> 4), idesc_s, 1u);
                 umma_commit_at(smem_u32(&s_full[x]));
             };
-            auto issue_pv = [&](int x, int g, unsigned accumulate) {  // O_x (+)= P_x V(g), both parts of P
-                const unsigned v_low = v_low0 + (unsigned)(g % S::V_STAGES) * (TILE_BYTES >> 4), o = tmem + O_COL + x * BM, p = tmem + x * BN;
-                umma_pv_32(o, p, v_low, idesc_o, accumulate);
-                umma_pv_32(o, p + 32, v_low + 256, idesc_o, 1u);
-                umma_pv_32(o, p + 64, v_low + 512, idesc_o, 1u);
-                umma_pv_32(o, p + 96, v_low + 768, idesc_o, 1u);
-                umma_commit_at(smem_u32(&o_done[x]));
+            auto issue_pv = [&](int x, int g, int part, bool halves, unsigned accumulate) {  // O_x (+)= P_x V(g) over the upper (part 0) or the lower 64 keys
+                const unsigned at = part ? 0u : 64u, v_low = v_low0 + (unsigned)(g % STAGES) * (TILE_BYTES >> 4) + at * 8, o = tmem + O_COL + x * BM, p = tmem + x * BN + at;
+                if (halves) {
+                    umma_pv_32_whole(o, p, v_low, idesc_half, accumulate);
+                    umma_pv_32_whole(o, p + 32, v_low + 256, idesc_half, 1u);
+                } else {
+                    umma_pv_32(o, p, v_low, idesc_o, accumulate);
+                    umma_pv_32(o, p + 32, v_low + 256, idesc_o, 1u);
+                }
             };
             bool ok = true;
             int g0 = 0, h0[2] = {0, 0}, round = 0;
@@ -415,12 +473,21 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                 for (int j = 0; j < it.n_tiles && ok; ++j) {
                     const int g = g0 + j;
                     const bool more = j + 1 < it.n_tiles;
+                    bool halves = false;
+                    if constexpr (E8) {
+                        if (!mbar_wait(&kind_full[g & 1], (g >> 1) & 1, failed)) { ok = false; break; }
+                        halves = kinds[g & 1] & 1;
+                    }
                     for (int x = 0; x < it.halves && ok; ++x) {
-                        if (!mbar_wait(&p_full[x], (h0[x] + j) & 1, failed)) { ok = false; break; }
-                        if (x == 0 && !mbar_wait(&v_full[g % S::V_STAGES], (g / S::V_STAGES) & 1, failed)) { ok = false; break; }
-                        tc_fence_after();
-                        issue_pv(x, g, j > 0 ? 1u : 0u);
-                        if (x == it.halves - 1) umma_commit_at(smem_u32(&v_empty[g % S::V_STAGES]));
+                        for (int part = 0; part < 2 && ok; ++part) {
+                            if (!mbar_wait(&p_full[2 * x + part], (h0[x] + j) & 1, failed)) { ok = false; break; }
+                            if (x == 0 && part == 0 && !mbar_wait(&v_full[g % STAGES], (g / STAGES) & 1, failed)) { ok = false; break; }
+                            tc_fence_after();
+                            issue_pv(x, g, part, halves, j > 0 || part > 0 ? 1u : 0u);
+                        }
+                        if (!ok) break;
+                        if (!more) umma_commit_at(smem_u32(&o_done[x]));
+                        if (x == it.halves - 1) umma_commit_at(smem_u32(&v_empty[g % STAGES]));
                         if (more) {
                             if (x == 0) {
                                 if (!mbar_wait(&k_full[(g + 1) & 1], ((g + 1) >> 1) & 1, failed)) { ok = false; break; }
@@ -440,22 +507,26 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             }
             if (!ok) fail();
         }
-    } else if (warp < 10) {
+      }
+    } else if (warp < 12) {
         // ------------------------------------------------------------------ softmax: thread = row = tensor-memory lane of its half
-        const int x = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane, v = x * BM + r;
+        if constexpr (E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::MANY));
+        const int x = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane, v = x * BM + r;
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
         const unsigned s_addr = lane_addr + x * BN, o_addr = lane_addr + O_COL + x * BM;
         const float scale = a.scale_log2;
-        int hx = 0;  // tiles this half has seen
+        const Pair scale2{scale, scale}, minus_one{-1.f, -1.f};
+        int hx = 0, g0 = 0, mine = 0;  // tiles this half has seen; the block's tiles; items this half has had a part in
         bool ok = true;
         for (int index = blockIdx.x; index < total && ok; index += gridDim.x) {
             const Item it = read_item(index);
-            if (x >= it.halves) continue;
+            if (x >= it.halves) { g0 += it.n_tiles; continue; }
             const int tok = v / a.gc, hh = v - tok * a.gc;
             const bool row_valid = tok < it.ntok && hh < it.heads_here;
             // a row that is no one's is computed like the item's last token and never stored: it takes the same way through the code as its neighbours
             const int token = it.tok0 + min(tok, it.ntok - 1), hi = min(it.key_hi - 1, a.last[token]);
             float m = -INFINITY, l = 0.f;
+            int kind = 2 * 64;
             for (int j = 0; j < it.n_tiles; ++j) {
                 const int h = hx + j;
                 if (!mbar_wait(&s_full[x], h & 1, failed)) { ok = false; break; }
@@ -463,73 +534,119 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                 const int tile_base = it.start + j * BN, last_visible = hi - tile_base, first_visible = it.key_lo - tile_base;
                 const bool masked = !__all_sync(0xffffffffu, last_visible >= BN - 1 && first_visible <= 0);  // one way for the whole warp
                 unsigned s0[32], s1[32];  // of this row's S, 32 columns at hand and 32 on their way
-                auto hide = [&](unsigned (&s)[32], int c) {  // what the row does not see
-                    if (masked) {
+                // The loops below are kept short on purpose: the roles of a block run different code on the same schedulers, and straight-line code is bound by
+                // the fetching of instructions (8-bit, 256 requests behind 16,384 positions: 163 us with every loop unrolled and masks in each of them).
+                if (masked) {  // what the row does not see is replaced where it stands
+#pragma unroll 1
+                    for (int c = 0; c < BN; c += 32) {
+                        tmem_ld32(s_addr + c, s0), arrived(s0);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = (c + i <= last_visible && c + i >= first_visible) ? s[i] : 0xff800000u;
+                        for (int i = 0; i < 32; ++i) s0[i] = (c + i <= last_visible && c + i >= first_visible) ? s0[i] : 0xff800000u;
+                        tmem_st32(s_addr + c, s0);
                     }
-                };
-                float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                auto look = [&](unsigned (&s)[32], int c) {
-                    hide(s, c);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                float part[2] = {-INFINITY, -INFINITY};
+                auto look = [&](unsigned (&s)[32]) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(s[i]));
+                    for (int i = 0; i < 16; ++i) part[i & 1] = max3(part[i & 1], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
                 };
                 tmem_ld32(s_addr, s0), arrived(s0);
-                tmem_ld32(s_addr + 32, s1), look(s0, 0), arrived(s1);
-                tmem_ld32(s_addr + 64, s0), look(s1, 32), arrived(s0);
-                tmem_ld32(s_addr + 96, s1), look(s0, 64), arrived(s1);
-                tmem_ld32(s_addr + 64, s0), look(s1, 96);
-                const float tmax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * scale;  // the scale is positive: the largest score stays the largest
-                const float m_new = fmaxf(m, tmax);
+#pragma unroll 1
+                for (int c = 0; c < BN; c += 64) {
+                    tmem_ld32(s_addr + c + 32, s1), look(s0), arrived(s1);
+                    if (c == 0) tmem_ld32(s_addr + 64, s0);
+                    look(s1);
+                    if (c == 0) arrived(s0);
+                }
+                const float m_new = fmaxf(m, fmaxf(part[0], part[1]) * scale);  // the scale is positive: the largest score stays the largest
                 float alpha = 1.f;
                 if (m == -INFINITY) {
                     m = m_new;  // nothing seen so far: the row of O holds zeros (or is overwritten by the first product)
-                } else if (m_new - m > RESCALE_THRESHOLD) {
+                } else if (m_new - m > S::OUTGROWN) {
                     alpha = exp2f(m - m_new);
                     m = m_new;
                 }
+                // The products of the tiles before were issued before this S was, and this S has arrived: O stands still.
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        tmem_ld32(o_addr + c, s0), arrived(s0);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s0[i] = __float_as_uint(__uint_as_float(s0[i]) * alpha);
+                        tmem_st32(o_addr + c, s0);
+                    }
+                }
                 const float minus_m = m == -INFINITY ? 0.f : -m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                auto weigh = [&](unsigned (&s)[32], int c) {  // P of 32 columns, in two parts, over the columns that they came from
+                const Pair minus_m2{minus_m, minus_m};
+                Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                auto weights = [&](const unsigned (&s)[32], int i) {
+                    const Pair z = fma2(Pair{__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, scale2, minus_m2), p{fast_exp2(z.x), fast_exp2(z.y)};
+                    sum[i & 1] = add2(sum[i & 1], p);
+                    return p;
+                };
+                auto weigh_halves = [&](const unsigned (&s)[32], int c) {  // P of 32 columns as float16, over the first half of the columns that they came from
+                    unsigned w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const Pair p = weights(s, i);
+                        w[i] = pack_f16x2(p.x, p.y);
+                    }
+                    tmem_st16_words(s_addr + c, w);
+                };
+                auto weigh = [&](const unsigned (&s)[32], int c) {  // as bfloat16 in two parts, over all of them
                     unsigned w[32];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float p0 = fast_exp2(fmaf(__uint_as_float(s[2 * i]), scale, minus_m)), p1 = fast_exp2(fmaf(__uint_as_float(s[2 * i + 1]), scale, minus_m));
-                        sum[i & 3] += p0 + p1;
-                        w[i] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
-                        w[16 + i] = pack_bf16x2(p0 - __uint_as_float(__float_as_uint(p0) & 0xffff0000u), p1 - __uint_as_float(__float_as_uint(p1) & 0xffff0000u));
+                        const Pair p = weights(s, i);
+                        w[i] = __byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x7632);
+                        const Pair rest = fma2(Pair{__uint_as_float(__float_as_uint(p.x) & 0xffff0000u), __uint_as_float(__float_as_uint(p.y) & 0xffff0000u)}, minus_one, p);
+                        w[16 + i] = pack_bf16x2(rest.x, rest.y);
                     }
                     tmem_st32(s_addr + c, w);
                 };
-                weigh(s1, 96), arrived(s0), hide(s0, 64);
-                tmem_ld32(s_addr + 32, s1), weigh(s0, 64), arrived(s1), hide(s1, 32);
-                tmem_ld32(s_addr, s0), weigh(s1, 32), arrived(s0), hide(s0, 0);
-                weigh(s0, 0);
-                l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                // Every thread sees every phase of o_done go by, tile by tile; the product of tile j - 1 was issued a whole tile ago.
-                if (j > 0 && !mbar_wait(&o_done[x], (h - 1) & 1, failed)) { ok = false; break; }
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    tc_fence_after();  // O may be rescaled only between two products
-#pragma unroll
-                    for (int c = 0; c < D; c += 16) {
-                        float o[16];
-                        tmem_ld16(o_addr + c, o);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] *= alpha;
-                        tmem_st16(o_addr + c, o);
+                auto hand_over = [&](int which) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * x + which]);
+                };
+                // columns 96 to 127 are still at hand
+                auto walk = [&](auto&& weigh_32) {
+#pragma unroll 1
+                    for (int c = 64; c >= 0; c -= 64) {
+                        tmem_ld32(s_addr + c, s0), weigh_32(s1, c + 32), arrived(s0);
+                        if (c) tmem_ld32(s_addr + c - 32, s1);
+                        weigh_32(s0, c);
+                        hand_over(c ? 0 : 1);
+                        if (c) arrived(s1);
                     }
+                };
+                if constexpr (E8) {
+                    if (!mbar_wait(&kind_full[(g0 + j) & 1], ((g0 + j) >> 1) & 1, failed)) { ok = false; break; }
+                    kind = kinds[(g0 + j) & 1];
+                    if (kind & 1) {
+                        walk(weigh_halves);
+                    } else {
+#pragma unroll 1
+                        for (int c = 96; c >= 0; c -= 32) {
+                            tmem_ld32(s_addr + c, s0), arrived(s0);
+                            weigh(s0, c);
+                            if (c == 64) hand_over(0);
+                        }
+                        hand_over(1);
+                    }
+                } else {
+                    walk(weigh);
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[x]);
+                l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             }
-            if (ok && it.n_tiles > 0) ok = mbar_wait(&o_done[x], (hx + it.n_tiles - 1) & 1, failed);  // every phase but the item's last was seen in the loop
+            if (ok && it.n_tiles > 0) ok = mbar_wait(&o_done[x], mine++ & 1, failed);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             if (ok) {
                 const size_t slot = row_valid && a.pieces ? (size_t)(a.piece_start[token] + it.piece) * a.heads + it.first_head + hh : 0;
+                const float back = E8 ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
                 const float inv = a.pieces ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
 #pragma unroll
                 for (int c = 0; c < D; c += 16) {
@@ -540,6 +657,8 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = 0.f;
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] *= back;
                     if (row_valid && a.pieces) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 8)
@@ -556,56 +675,90 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                 // the row is out of tensor memory before this thread hands over the next item's first P, and only then is O written anew
                 tc_fence_before();
             }
-            hx += it.n_tiles;
+            hx += it.n_tiles, g0 += it.n_tiles;
         }
         if (!ok) fail();
     } else if constexpr (E8) {
-        // ------------------------------------------------------------------ codes into bfloat16: warps 10 and 11 the K tiles, 12 and 13 the V tiles
-        const int which = (warp - 10) >> 1, w = warp & 1;
+        // ------------------------------------------------------------------ codes into operands: warps 12 to 15 the K tiles, 16 to 19 the V tiles
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CONVERTING));
+        const int which = (warp - 12) >> 2, w = warp & 3;
         constexpr int CHUNKS = D / 16;  // 16 codes each, of a row
+        constexpr int LOWEST = -12, HIGHEST = 7;  // of e - e0, for float16
         bool ok = true;
         int g = 0;
         for (int index = blockIdx.x; index < total && ok; index += gridDim.x) {
             const Item it = read_item(index);
+            int e0 = 0;
             for (int t = 0; t < it.n_tiles; ++t, ++g) {
                 const int s = g & 1, turn = g >> 1, tile_base = it.start + t * BN;
-                const int vs = g % S::V_STAGES, v_turn = g / S::V_STAGES;
-                ok = mbar_wait(&raw_full[2 * s + which], turn & 1, failed) && mbar_wait(which ? &v_empty[vs] : &k_empty[s], ((which ? v_turn : turn) & 1) ^ 1, failed);
+                ok = mbar_wait(&raw_full[which], g & 1, failed);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const unsigned char* raw = raw_ring + (2 * s + which) * RAW_BYTES;
-                const signed char* e8 = reinterpret_cast<const signed char*>(exps + (2 * s + which) * BN);
-                unsigned char* tile = which ? v_ring + (size_t)vs * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
-                // eight lanes take a 16-byte chunk of eight rows: the swizzles of both layouts put those in different banks
-#pragma unroll 4
-                for (int i = 0; i < BN / 8 * CHUNKS / 8; ++i) {
-                    const int octet = (i * 2 + w) * 4 + (lane >> 3), chunk = octet % CHUNKS, row = octet / CHUNKS * 8 + (lane & 7);
-                    const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
-                    const int e = min(max((int)e8[row], -40), 40);
-                    const float factor = __uint_as_float((unsigned)(127 + e) << 23);
-                    const bool keep = which == 0 || (tile_base + row >= it.key_lo && tile_base + row < it.key_hi);
-                    const unsigned* words = reinterpret_cast<const unsigned*>(&codes);
-                    unsigned wide[8];
+                const unsigned char* raw = raw_tiles + which * RAW_BYTES;
+                const signed char* e8 = reinterpret_cast<const signed char*>(exps + which * BN);
+                unsigned char* tile = (which ? v_ring : k_ring) + (size_t)s * TILE_BYTES;
+                bool halves = false;
+                if (which) {  // what the tile will be, for those who make its weights and its products
+                    int low = 127, high = -128;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        unsigned h0, h1;
-                        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
-                        wide[2 * k] = pack_bf16x2(value_of_half((unsigned short)h0) * factor, value_of_half((unsigned short)(h0 >> 16)) * factor);
-                        wide[2 * k + 1] = pack_bf16x2(value_of_half((unsigned short)h1) * factor, value_of_half((unsigned short)(h1 >> 16)) * factor);
+                        const int pos = tile_base + lane * 4 + k, e = min(max((int)e8[lane * 4 + k], -40), 40);
+                        if (pos >= it.key_lo && pos < it.key_hi) low = min(low, e), high = max(high, e);
                     }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int oc = 2 * chunk + half;
-                        uint4 out = make_uint4(wide[4 * half], wide[4 * half + 1], wide[4 * half + 2], wide[4 * half + 3]);
-                        if (!keep) out = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(tile + (oc >> 3) * (KV_PANEL * 2) + row * 128 + (((oc & 7) ^ (row & 7)) << 4)) = out;
-                    }
+                    low = __reduce_min_sync(0xffffffffu, low), high = __reduce_max_sync(0xffffffffu, high);
+                    if (t == 0) e0 = high;
+                    halves = low - e0 >= LOWEST && high - e0 <= HIGHEST;
                 }
+                ok = mbar_wait(which ? &v_empty[s] : &k_empty[s], (turn & 1) ^ 1, failed);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (which && w == 0 && lane == 0) {  // only now: the products of the tile that had this slot, and its word in `kinds`, are done
+                    kinds[s] = 2 * (e0 + 64) + (halves ? 1 : 0);
+                    mbar_arrive(&kind_full[s]);
+                }
+                // eight lanes take a 16-byte chunk of eight rows: the swizzles of both layouts put those in different banks
+                auto convert = [&](auto as_halves) {
+#pragma unroll 2
+                    for (int i = 0; i < BN / 8 * CHUNKS / 16; ++i) {
+                        const int octet = (i * 4 + w) * 4 + (lane >> 3), chunk = octet % CHUNKS, row = octet / CHUNKS * 8 + (lane & 7);
+                        const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
+                        const int e = min(max((int)e8[row], -40), 40) - e0;
+                        const bool keep = which == 0 || (tile_base + row >= it.key_lo && tile_base + row < it.key_hi);
+                        const unsigned* words = reinterpret_cast<const unsigned*>(&codes);
+                        unsigned wide[8];
+                        if constexpr (as_halves.value) {
+                            const unsigned half = (unsigned)(15 + min(max(e, LOWEST), HIGHEST)) << 10, factor = half | half << 16;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                asm("{.reg .b16 lo, hi;\n\t.reg .b32 a, b;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 a, lo;\n\tcvt.rn.f16x2.e4m3x2 b, hi;\n\t"
+                                    "mul.rn.f16x2 %0, a, %3;\n\tmul.rn.f16x2 %1, b, %3;\n\t}" : "=r"(wide[2 * k]), "=r"(wide[2 * k + 1]) : "r"(words[k]), "r"(factor));
+                        } else {
+                            const float f = __uint_as_float((unsigned)(127 + e) << 23);
+                            const Pair factor{f, f};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                unsigned h0, h1;
+                                asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
+                                const Pair v0 = mul2(Pair{value_of_half((unsigned short)h0), value_of_half((unsigned short)(h0 >> 16))}, factor);
+                                const Pair v1 = mul2(Pair{value_of_half((unsigned short)h1), value_of_half((unsigned short)(h1 >> 16))}, factor);
+                                wide[2 * k] = pack_bf16x2(v0.x, v0.y), wide[2 * k + 1] = pack_bf16x2(v1.x, v1.y);
+                            }
+                        }
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int oc = 2 * chunk + half;
+                            uint4 out = make_uint4(wide[4 * half], wide[4 * half + 1], wide[4 * half + 2], wide[4 * half + 3]);
+                            if (!keep) out = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(tile + (oc >> 3) * (KV_PANEL * 2) + row * 128 + (((oc & 7) ^ (row & 7)) << 4)) = out;
+                        }
+                    }
+                };
+                if (halves) convert(Yes{}); else convert(No{});
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(which ? &v_full[vs] : &k_full[s]);
-                    mbar_arrive(&raw_empty[2 * s + which]);
+                    mbar_arrive(which ? &v_full[s] : &k_full[s]);
+                    mbar_arrive(&raw_empty[which]);
                 }
             }
         }

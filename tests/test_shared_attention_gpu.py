@@ -234,3 +234,23 @@ def test_refusals():
         with pytest.raises(ops.KernelError):
             attention_shared(**{**good, **bad})
     assert attention_shared(q[:0], 4, cache, table, plan_shared([0, 0], [100, 100], 4, 2, 64), 0.1).shape == (0, 256)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (16, 4, 128)])
+def test_blocks_of_several_items(heads, kv, dim, bits):
+    """More items than the device has multiprocessors, of many key tiles and of both heights, one behind the other in a block."""
+    counts, lengths = [1500, 9, 70, 260], [5000, 300, 3000, 2000]
+    q, cache, table = step(counts, lengths, heads, kv, dim, 16, bits, seed=9)
+    plan = plan_shared(counts, lengths, heads, kv, dim)
+    got = attention_shared(q, heads, cache, table, plan, 0.1)
+    ops.raise_on_status(q.device)
+    dense, first = values(cache), 0
+    for r, (n, length) in enumerate(zip(counts, lengths)):
+        k, v = dense[table[r, : -(-length // 16)].long()].permute(1, 2, 0, 3, 4).reshape(2, kv, 1, -1, dim)[:, :, :, :length]
+        x = q[first: first + n].double().view(n, kv, heads // kv, dim).permute(1, 2, 0, 3)
+        hidden = torch.arange(length, device="cuda") > torch.arange(length - n, length, device="cuda")[:, None]
+        p = torch.softmax((x @ k.transpose(2, 3) * 0.1).masked_fill(hidden, -float("inf")), -1)
+        want, size = ((p @ y).permute(2, 0, 1, 3).reshape(n, -1) for y in (v, v.abs()))
+        agree(got[first: first + n], want, size)
+        first += n
