@@ -9,15 +9,19 @@
 // A step whose rows have one piece each is stored at once.
 //
 // This file has the strip kernel, for items of few rows: it is bound by the bytes of the keys and values.  One lane of a producer warp per
-// page fetches K and V by TMA (one box a page and 128-byte panel, no multicast) into a ring of 64-key stages; each of four warps takes 16 of a
-// stage's keys for all 16 rows, S = Q K^T and O += P V by mma.sync m16n8k16, and at the end the warps' results are put together in shared memory.
+// page fetches K and V by TMA (one box a page and 128-byte panel, no multicast) into a ring of stages; each of four warps takes a quarter of a
+// stage's keys for all rows, and at the end the warps' results are put together in shared memory.  The products are S^T = K Q^T and O^T = V^T P^T
+// (mma.sync m16n8k16): keys and entries stand where the instruction has 16 rows, the few (token, head) rows where it has 8 columns, so that a decoded token of 7 heads a
+// key/value head wastes one column of 8 and not 9 rows of 16, and O takes half the registers.  P^T is turned from the one's result into the other's operand by movmatrix.
 //
-// 8-bit records meet the tensor cores as float16, which holds every e4m3 code: one conversion instruction for two codes and nothing else per
-// entry.  The exponents are kept out of the entries: a key's multiplies its score, and a value's goes into the softmax's exponent,
+// 8-bit records become float16, which holds every e4m3 code: one conversion instruction for two codes and nothing else per entry.  (mma.sync takes
+// e4m3 as it is, too, but on this architecture each such product costs the conversions and four additions besides: 42 us against 46 here.)  The exponents
+// are kept out of the entries: a key's
+// multiplies its score, and a value's goes into the softmax's exponent,
 //     z_j = y_j + e_j,  P_j = 2^(z_j - m),  o = sum P_j code_j,  l = sum P_j 2^-e_j,
 // with m the maximum of z.  Which entry of a head a lane's fragment holds does not matter to Q K^T as long as it is the same one in Q and K, so a
-// lane takes 16 bytes of a key at once (entries 16 c to 16 c + 15 of chunk c), and Q's fragments are loaded to match; the columns of P V come
-// out in another order than they are stored in, and are stored where they belong.
+// lane takes 16 bytes of a key at once, and Q's fragments are loaded to match; the columns of P V come out in another order than they are stored in, and are
+// stored where they belong.
 //
 // Where the values' exponents lie far apart (a value 2^12 times smaller than another one of its range), a weight that counts can be too small for float16
 // beside the other's: such a stage's weights are multiplied in lots by their size.
@@ -40,8 +44,7 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int D = HB_HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
-constexpr int BN = 64;          // keys of a stage
-constexpr int ROWS = 16;        // (token, head) rows of a strip
+constexpr int MOST_ROWS = 16;   // (token, head) rows of a strip: 8 or 16
 constexpr int WARPS = 4;        // that compute; one more fetches
 constexpr int THREADS = 32 * (WARPS + 1);
 constexpr int ITEM_WORDS = 6;   // first token, tokens, table row, first key, last key + 1, number of the piece
@@ -78,6 +81,11 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ unsigned turned(unsigned w) {  // an 8 x 8 matrix of 16-bit entries, two of a row a lane, transposed
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
+}
 __device__ __forceinline__ void ldmatrix_x4_trans(unsigned (&r)[4], const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
@@ -108,6 +116,11 @@ __device__ __forceinline__ unsigned upper_halves_of(unsigned codes) {
     asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(w) : "r"(codes));
     return w;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -115,18 +128,22 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // -126 <= e <= 127
 
-template <bool E8>
+template <bool E8, int NQ>  // NQ: eights of rows
 struct Shape {
+    static constexpr int ROWS = 8 * NQ;
+    static constexpr int BLOCKS = NQ == 1 ? 3 : 2;            // an SM, by registers
     static constexpr int BYTES = E8 ? 1 : 2;                  // of an entry
+    static constexpr int BN = E8 ? 128 : 64;                  // keys of a stage
+    static constexpr int KEYS = BN / WARPS;                   // of which a warp takes so many
     static constexpr int TILE = BN * D * BYTES;               // one K or V tile
     static constexpr int PANEL_BYTES = D * BYTES < 128 ? D * BYTES : 128;  // of a row, in one box
     static constexpr int PANELS = D * BYTES / PANEL_BYTES;
-    static constexpr int STAGE = 2 * TILE + (E8 ? 128 : 0);   // K, V, and the exponents of both
-    static constexpr int STAGES = E8 ? (D == 128 ? 6 : 8) : (D == 128 ? 3 : 5);
-    static constexpr int PER_CHUNK = 16 / BYTES;              // entries of 16 bytes
-    static constexpr int CHUNKS = D / PER_CHUNK;              // of a row
-    static constexpr int STEPS = PER_CHUNK / 4;               // products of 16 entries that one chunk a lane feeds
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 2 * STAGES * 8 + 16;
+    static constexpr int EXPS = E8 ? 2 * BN : 0;              // the exponents of K and V
+    static constexpr int STAGES = (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
+    static constexpr int CHUNKS = D * BYTES / 16;             // 16-byte chunks of a row
+    static constexpr int STEPS = 4 / BYTES;                   // products of 16 entries that a chunk a lane feeds
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * (2 * TILE + EXPS) + (E8 ? WARPS * 3 * KEYS * 4 : 0) + 2 * STAGES * 8 + 16;
+    static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024 && WARPS * ROWS * (D + 2) * 4 <= STAGES * 2 * TILE, "shared memory");
     // 16-byte chunk cc of row `key` as TMA's swizzle has placed it: the panel's row of 128 bytes (of 64, in pairs) with its chunks permuted.
     static __device__ __forceinline__ int at(int key, int cc) {
         if constexpr (PANEL_BYTES == 64) return key * 64 + ((cc ^ ((key >> 1) & 3)) << 4);
@@ -150,14 +167,16 @@ struct Args {
     int* status;
 };
 
-template <bool E8>
-__global__ void __launch_bounds__(THREADS) attention_strip_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
-    typedef Shape<E8> S;
+template <bool E8, int NQ>
+__global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_strip_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
+    typedef Shape<E8, NQ> S;
+    constexpr int BN = S::BN, KEYS = S::KEYS, NK = KEYS / 16, ROWS = S::ROWS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    // the tiles of all stages, then the exponents of all stages
+    // the tiles of all stages, the exponents of all stages, and each warp's keys' factors
     unsigned char* exps = ring + (size_t)S::STAGES * 2 * S::TILE;
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(exps + (E8 ? S::STAGES * 128 : 0));
+    float* factors = reinterpret_cast<float*>(exps + (size_t)S::STAGES * S::EXPS);
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(factors + (E8 ? WARPS * 3 * S::KEYS : 0));
     unsigned long long* empty = full + S::STAGES;
     volatile int* failed = reinterpret_cast<volatile int*>(empty + S::STAGES);
 
@@ -209,12 +228,12 @@ __global__ void __launch_bounds__(THREADS) attention_strip_kernel(const __grid_c
             }
             __syncwarp();
             unsigned char* stage = ring + (size_t)s * 2 * S::TILE;
-            if constexpr (E8) {  // the exponents of four keys or values a lane
-                const int which = lane >> 4, key = (lane & 15) * 4;
-                const int from = __shfl_sync(0xffffffffu, page, key >> shift);
+            if constexpr (E8) {  // the exponents of four keys and of four values a lane
+                const int key = lane * 4, from = __shfl_sync(0xffffffffu, page, key >> shift);
                 if (from >= 0) {
-                    const signed char* src = a.exponents + (((size_t)from * 2 + which) * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1));
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * 128 + lane * 4)), "l"(src) : "memory");
+                    const signed char* src = a.exponents + ((size_t)from * 2 * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1));
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * S::EXPS + key)), "l"(src) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * S::EXPS + BN + key)), "l"(src + (size_t)a.kv_heads * a.page_size) : "memory");
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
             }
@@ -231,47 +250,56 @@ __global__ void __launch_bounds__(THREADS) attention_strip_kernel(const __grid_c
     }
     // ---------------------------------------------------------------------- consumers
     const int t = lane & 3, g = lane >> 2;
-    unsigned qf[D / 16][4];
-    float row_scale[2];
-    int hi[2];  // the last key a row sees
+    // Q's fragments: a lane's 16-byte chunk t + 4 j of a key feeds products STEPS j to STEPS j + STEPS - 1, four of its entries each, so a query's entries stand
+    // in the fragments likewise.
+    unsigned qf[NQ][D / 16][2];
+    float row_scale[NQ][2];
+    int hi[NQ][2];  // of columns 2 t and 2 t + 1: the last key a row sees; a row that is no one's sees what the others see, and is never stored
+    int sees_all_to = key_hi - 1;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int v = g + r * 8, tok = v / a.gc, hh = v - tok * a.gc;
+    for (int q = 0; q < NQ; ++q) {
+        const int v = q * 8 + g, tok = v / a.gc, hh = v - tok * a.gc;
         const bool valid = tok < ntok && hh < heads_here;
-        hi[r] = valid ? min(key_hi - 1, a.last[tok0 + tok]) : -1;
+        const int mine_sees = valid ? min(key_hi - 1, a.last[tok0 + tok]) : key_hi - 1;
         const bf16* src = a.q + (size_t)(tok0 + (valid ? tok : 0)) * a.q_stride + (size_t)(first_head + (valid ? hh : 0)) * D;
-        uint4 raw[D / 32];  // this lane's quarter of the row: chunks t, t + 4, ... of PER_CHUNK entries
-        constexpr int PIECES = S::PER_CHUNK / 8;
+        constexpr int PER_CHUNK = 16 / S::BYTES, PIECES = PER_CHUNK / 8;  // entries of a chunk; 16-byte pieces of them in bfloat16
+        uint4 raw[D / 32];  // this lane's quarter of the row: chunks t, t + 4, ...
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
-            raw[i] = valid ? *reinterpret_cast<const uint4*>(src + (t + 4 * (i / PIECES)) * S::PER_CHUNK + (i % PIECES) * 8) : make_uint4(0, 0, 0, 0);
+            raw[i] = valid ? *reinterpret_cast<const uint4*>(src + (t + 4 * (i / PIECES)) * PER_CHUNK + (i % PIECES) * 8) : make_uint4(0, 0, 0, 0);
         const unsigned* words = reinterpret_cast<const unsigned*>(raw);
-        float factor = 1.f;
+        float factor = 1.f, scale = a.scale_log2;
         if constexpr (E8) {
             // As float16 with the row's largest entry between 2^13 and 2^14: an entry of eight bits keeps them all down to 2^-27 of the largest.
             float largest = 0.f;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(words[i] << 16)), fabsf(__uint_as_float(words[i] & 0xffff0000u))));
+            for (int i = 0; i < D / 8; ++i) largest = max3(largest, fabsf(__uint_as_float(words[i] << 16)), fabsf(__uint_as_float(words[i] & 0xffff0000u)));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
             const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 13, -126), 126);
             factor = power_of_two(-e);
-            row_scale[r] = a.scale_log2 * power_of_two(e);
-        } else {
-            row_scale[r] = a.scale_log2;
+            scale *= power_of_two(e);
         }
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {  // word i: entries 2 i, 2 i + 1 of the quarter; product i / 2, fragment register (i & 1) * 2 + r
-            unsigned w = words[i];
-            if constexpr (E8) w = pack<true>(__uint_as_float(w << 16) * factor, __uint_as_float(w & 0xffff0000u) * factor);
-            qf[i >> 1][(i & 1) * 2 + r] = w;
+        for (int i = 0; i < D / 8; ++i)
+            qf[q][i >> 1][i & 1] = E8 ? pack<true>(__uint_as_float(words[i] << 16) * factor, __uint_as_float(words[i] & 0xffff0000u) * factor) : words[i];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            row_scale[q][e] = __shfl_sync(0xffffffffu, scale, (2 * t + e) * 4);
+            hi[q][e] = __shfl_sync(0xffffffffu, mine_sees, (2 * t + e) * 4);
         }
+        sees_all_to = min(sees_all_to, __reduce_min_sync(0xffffffffu, mine_sees));  // positions that every row sees
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float m[NQ][2], l[NQ][2];
     int top_e = -128;  // the largest exponent among the values so far
-    float o[D / 8][4];
+    float o[NQ][D / 16][4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int q = 0; q < NQ; ++q) {
+        m[q][0] = m[q][1] = -INFINITY, l[q][0] = l[q][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[q][i][0] = o[q][i][1] = o[q][i][2] = o[q][i][3] = 0.f;
+    }
+    float* mine = factors + warp * 3 * KEYS;  // of this warp's keys: 2^e of the key, e of the value, 2^-e of the value
 
     for (int it = 0; it < n_tiles; ++it) {
         const int s = it % S::STAGES, round = it / S::STAGES;
@@ -282,145 +310,178 @@ __global__ void __launch_bounds__(THREADS) attention_strip_kernel(const __grid_c
         }
         const unsigned char* ks = ring + (size_t)s * 2 * S::TILE;
         const unsigned char* vs = ks + S::TILE;
-        const int key0 = warp * 16, pos0 = start + it * BN + key0;  // this warp's keys
-        if (pos0 < key_hi && pos0 + 16 > key_lo) {
-            float sc[2][4];
+        const int key0 = warp * KEYS, pos0 = start + it * BN + key0;  // this warp's keys
+        if (pos0 < key_hi && pos0 + KEYS > key_lo) {
+            const bool whole = pos0 >= key_lo && pos0 + KEYS <= key_hi;  // all of them are in the item's range
+            bool far_apart = false;
+            if constexpr (E8) {  // a lane has one key; what was never stored is no exponent: kept in range, it meets only scores that are replaced
+                const signed char* ex = reinterpret_cast<const signed char*>(exps + s * S::EXPS + key0 + lane);
+                const int ke = min(max((int)ex[0], -40), 40), ve = min(max((int)ex[BN], -40), 40), pos = pos0 + lane;
+                mine[lane] = power_of_two(ke), mine[KEYS + lane] = (float)ve, mine[2 * KEYS + lane] = power_of_two(-ve);
+                const bool inside = pos >= key_lo && pos < key_hi;
+                top_e = __reduce_max_sync(0xffffffffu, inside ? max(top_e, ve) : top_e);
+                far_apart = top_e - __reduce_min_sync(0xffffffffu, inside ? ve : 127) > FAR_APART;
+                __syncwarp();
+            }
+            float sc[NQ][NK][4];  // of keys g and g + 8 of 16 and columns 2 t and 2 t + 1: [(key, column)]
 #pragma unroll
-            for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int j = 0; j < S::CHUNKS / 4; ++j) {
+                for (int k = 0; k < NK; ++k) sc[q][k][0] = sc[q][k][1] = sc[q][k][2] = sc[q][k][3] = 0.f;
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const uint4 raw = *reinterpret_cast<const uint4*>(ks + S::at(key0 + n * 8 + g, t + 4 * j));
-                    const unsigned* words = reinterpret_cast<const unsigned*>(&raw);
+            for (int j = 0; j < S::CHUNKS / 4; ++j)
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {
+                    const uint4 raw0 = *reinterpret_cast<const uint4*>(ks + S::at(key0 + k * 16 + g, t + 4 * j)), raw1 = *reinterpret_cast<const uint4*>(ks + S::at(key0 + k * 16 + 8 + g, t + 4 * j));
+                    const unsigned* w0 = reinterpret_cast<const unsigned*>(&raw0);
+                    const unsigned* w1 = reinterpret_cast<const unsigned*>(&raw1);
 #pragma unroll
                     for (int w = 0; w < S::STEPS; ++w) {
-                        if constexpr (E8) mma<true>(sc[n], qf[j * S::STEPS + w], halves_of(words[w]), upper_halves_of(words[w]));
-                        else mma<false>(sc[n], qf[j * S::STEPS + w], words[2 * w], words[2 * w + 1]);
+                        unsigned x[4];
+                        if constexpr (E8) x[0] = halves_of(w0[w]), x[1] = halves_of(w1[w]), x[2] = upper_halves_of(w0[w]), x[3] = upper_halves_of(w1[w]);
+                        else x[0] = w0[2 * w], x[1] = w1[2 * w], x[2] = w0[2 * w + 1], x[3] = w1[2 * w + 1];
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) mma<E8>(sc[q][k], x, qf[q][j * S::STEPS + w][0], qf[q][j * S::STEPS + w][1]);
                     }
                 }
-            }
-            float back[2][2];  // 2^-e of the values' exponents
-            bool far_apart = false;
-            float mx[2] = {-INFINITY, -INFINITY};
-            int low_e = 127;
+            float back[NK][2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                float key_scale[2] = {1.f, 1.f}, value_e[2] = {0.f, 0.f};
-                back[n][0] = back[n][1] = 1.f;
-                if constexpr (E8) {
-                    const unsigned char* ex = exps + s * 128 + key0 + n * 8 + t * 2;
-                    const char2 ke = *reinterpret_cast<const char2*>(ex), ve = *reinterpret_cast<const char2*>(ex + 64);
+            for (int k = 0; k < NK; ++k)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {  // what was never stored is no exponent: kept in range, it meets only scores that are replaced
-                        const int k = min(max((int)(c ? ke.y : ke.x), -40), 40), v = min(max((int)(c ? ve.y : ve.x), -40), 40);
-                        key_scale[c] = power_of_two(k);
-                        value_e[c] = (float)v;
-                        back[n][c] = power_of_two(-v);
-                        const int pos = pos0 + n * 8 + t * 2 + c;
-                        if (pos < key_hi && pos >= key_lo) low_e = min(low_e, v), top_e = max(top_e, v);
-                    }
+                for (int h = 0; h < 2; ++h) {  // key g + 8 h of 16
+                    float key_scale = 1.f, value_e = 0.f;
+                    if constexpr (E8) key_scale = mine[k * 16 + h * 8 + g], value_e = mine[KEYS + k * 16 + h * 8 + g], back[k][h] = mine[2 * KEYS + k * 16 + h * 8 + g];
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) sc[q][k][2 * h + e] = E8 ? fmaf(sc[q][k][2 * h + e] * key_scale, row_scale[q][e], value_e) : sc[q][k][2 * h + e] * row_scale[q][e];
                 }
+            if (pos0 < key_lo || pos0 + KEYS - 1 > sees_all_to) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int pos = pos0 + n * 8 + t * 2 + (e & 1);
-                    float z = -INFINITY;
-                    if (pos <= hi[e >> 1] && pos >= key_lo) z = fmaf(sc[n][e] * key_scale[e & 1], row_scale[e >> 1], value_e[e & 1]);
-                    sc[n][e] = z;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], z);
-                }
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int k = 0; k < NK; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int pos = pos0 + k * 16 + (e >> 1) * 8 + g;
+                            if (pos > hi[q][e & 1] || pos < key_lo) sc[q][k][e] = -INFINITY;
+                        }
             }
-            if constexpr (E8) {
-                top_e = __reduce_max_sync(0xffffffffu, top_e);
-                far_apart = top_e - __reduce_min_sync(0xffffffffu, low_e) > FAR_APART;
-            }
-            float alpha[2];
+            bool rescale = false;
+            float alpha[NQ][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                const float m_new = fmaxf(m[r], mx[r] - (E8 ? HEADROOM : 0.f));
-                alpha[r] = m_new == -INFINITY ? 1.f : fast_exp2(m[r] - m_new);
-                m[r] = m_new;
-                mx[r] = m_new == -INFINITY ? 0.f : m_new;
-            }
-            float sum[2] = {0.f, 0.f};
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+                for (int e = 0; e < 2; ++e) {
+                    float mx = fmaxf(sc[q][0][e], sc[q][0][2 + e]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = fast_exp2(sc[n][e] - mx[e >> 1]);
-                    sc[n][e] = p;
-                    sum[e >> 1] = E8 ? fmaf(p, back[n][e & 1], sum[e >> 1]) : sum[e >> 1] + p;
-                }
+                    for (int k = 1; k < NK; ++k) mx = max3(mx, sc[q][k][e], sc[q][k][2 + e]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float m_new = fmaxf(m[q][e], mx - (E8 ? HEADROOM : 0.f));
+                    alpha[q][e] = m_new == -INFINITY ? 1.f : fast_exp2(m[q][e] - m_new);
+                    m[q][e] = m_new;
+                    rescale |= alpha[q][e] != 1.f;
+                    const float base = m_new == -INFINITY ? 0.f : m_new;
+                    l[q][e] *= alpha[q][e];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) l[r] = fmaf(l[r], alpha[r], sum[r]);  // of this lane's keys; the quad's lanes are added up at the end
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) o[i][0] *= alpha[0], o[i][1] *= alpha[0], o[i][2] *= alpha[1], o[i][3] *= alpha[1];
-            }
-            const unsigned pf[4] = {pack<E8>(sc[0][0], sc[0][1]), pack<E8>(sc[0][2], sc[0][3]), pack<E8>(sc[1][0], sc[1][1]), pack<E8>(sc[1][2], sc[1][3])};
-            unsigned pr[4];  // bfloat16: what the weights lose by rounding, as weights of their own
-            if constexpr (!E8) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    pr[i] = pack<false>(sc[i >> 1][(i & 1) * 2] - __uint_as_float(pf[i] << 16), sc[i >> 1][(i & 1) * 2 + 1] - __uint_as_float(pf[i] & 0xffff0000u));
-            }
-            // Values beyond the range read as zeros, whatever their slots hold.  A fragment register holds keys 2 t and 2 t + 1 in its halves.
-            unsigned keep[2] = {0xffffffffu, 0xffffffffu};
-            const bool whole = pos0 >= key_lo && pos0 + 16 <= key_hi;
-            if (!whole) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int pos = pos0 + h * 8 + t * 2;
-                    keep[h] = (pos >= key_lo && pos < key_hi ? 0xffffu : 0u) | (pos + 1 >= key_lo && pos + 1 < key_hi ? 0xffff0000u : 0u);
-                }
-            }
-            if (E8 && far_apart) {
-                // Weights by size, 2^18 at a time, each lot scaled up to where float16 holds it and the products scaled back.
-#pragma unroll 1
-                for (int lot = 0; lot < 7; ++lot) {
-                    const float up = power_of_two(18 * lot), down = power_of_two(-18 * lot), from = lot < 6 ? down * 0x1p-10f : 0.f, to = lot ? down * 256.f : INFINITY;
-                    unsigned part[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p0 = sc[i >> 1][(i & 1) * 2], p1 = sc[i >> 1][(i & 1) * 2 + 1];
-                        part[i] = pack<true>(p0 <= from || p0 > to ? 0.f : p0 * up, p1 <= from || p1 > to ? 0.f : p1 * up);
-                    }
-                    if (!__any_sync(0xffffffffu, (part[0] | part[1] | part[2] | part[3]) != 0)) continue;
-#pragma unroll
-                    for (int c = 0; c < S::CHUNKS; c += 2) {
-                        unsigned b[4];
-                        ldmatrix_x4_trans(b, vs + S::at(key0 + (lane & 15), c + (lane >> 4)));
+                    for (int k = 0; k < NK; ++k)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const unsigned b0 = __byte_perm(b[2 * h] & keep[0], 0, 0x3120), b1 = __byte_perm(b[2 * h + 1] & keep[1], 0, 0x3120);
-                            float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma<true>(even, part, halves_of(b0), halves_of(b1));
-                            mma<true>(odd, part, upper_halves_of(b0), upper_halves_of(b1));
-                            if constexpr (E8)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[2 * (c + h)][e] = fmaf(even[e], down, o[2 * (c + h)][e]), o[2 * (c + h) + 1][e] = fmaf(odd[e], down, o[2 * (c + h) + 1][e]);
+                            const float p = fast_exp2(sc[q][k][2 * h + e] - base);
+                            sc[q][k][2 * h + e] = p;
+                            l[q][e] = E8 ? fmaf(p, back[k][h], l[q][e]) : l[q][e] + p;  // of this lane's keys; the lanes are added up at the end
                         }
+                }
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) o[q][i][0] *= alpha[q][0], o[q][i][1] *= alpha[q][1], o[q][i][2] *= alpha[q][0], o[q][i][3] *= alpha[q][1];
+            }
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {  // 16 keys
+                const int key = key0 + k * 16;
+                // Values beyond the range read as zeros, whatever their slots hold.  A fragment register holds keys 2 t and 2 t + 1 in its halves.
+                unsigned keep[2] = {0xffffffffu, 0xffffffffu};
+                if (!whole) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int pos = pos0 + k * 16 + h * 8 + t * 2;
+                        keep[h] = (pos >= key_lo && pos < key_hi ? 0xffffu : 0u) | (pos + 1 >= key_lo && pos + 1 < key_hi ? 0xffff0000u : 0u);
                     }
                 }
-            } else
-#pragma unroll
-            for (int c = 0; c < S::CHUNKS; c += 2) {
-                unsigned b[4];
-                ldmatrix_x4_trans(b, vs + S::at(key0 + (lane & 15), c + (lane >> 4)));
-                if (!whole) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {  // chunk c + h
+                auto values = [&](int c, unsigned (&x)[2][4]) {  // 16 keys of two 16-byte chunks: 16 entries each in 8 bits; together in bfloat16, in x[0]
+                    unsigned b[4];
+                    ldmatrix_x4_trans(b, vs + S::at(key + (lane & 15), c + (lane >> 4)));
+                    if (!whole) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
                     if constexpr (E8) {
-                        // bytes (key 2t: entries 2g, 2g + 1; key 2t + 1: the same) -> the two keys' even entries, and their odd ones
-                        const unsigned b0 = __byte_perm(b[2 * h], 0, 0x3120), b1 = __byte_perm(b[2 * h + 1], 0, 0x3120);
-                        mma<true>(o[2 * (c + h)], pf, halves_of(b0), halves_of(b1));
-                        mma<true>(o[2 * (c + h) + 1], pf, upper_halves_of(b0), upper_halves_of(b1));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            // bytes (key 2t: entries 2g, 2g + 1; key 2t + 1: the same) -> the two keys' even entries, rows g, and their odd ones, rows g + 8
+                            const unsigned b0 = __byte_perm(b[2 * h], 0, 0x3120), b1 = __byte_perm(b[2 * h + 1], 0, 0x3120);
+                            x[h][0] = halves_of(b0), x[h][1] = upper_halves_of(b0), x[h][2] = halves_of(b1), x[h][3] = upper_halves_of(b1);
+                        }
                     } else {
-                        mma<false>(o[c + h], pf, b[2 * h], b[2 * h + 1]);
-                        mma<false>(o[c + h], pr, b[2 * h], b[2 * h + 1]);
+                        x[0][0] = b[0], x[0][1] = b[2], x[0][2] = b[1], x[0][3] = b[3];
                     }
+                };
+                constexpr int TILES = E8 ? 2 : 1;  // of 16 entries, of two chunks
+                if (E8 && far_apart) {
+                    // Weights by size, 2^18 at a time, each lot scaled up to where float16 holds it and the products scaled back.
+#pragma unroll 1
+                    for (int lot = 0; lot < 7; ++lot) {
+                        const float up = power_of_two(18 * lot), down = power_of_two(-18 * lot), from = lot < 6 ? down * 0x1p-10f : 0.f, to = lot ? down * 256.f : INFINITY;
+                        auto scaled = [&](float p) { return p <= from || p > to ? 0.f : p * up; };
+                        unsigned part[NQ][2], any = 0;
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                part[q][h] = turned(pack<true>(scaled(sc[q][k][2 * h]), scaled(sc[q][k][2 * h + 1])));
+                                any |= part[q][h];
+                            }
+                        if (!__any_sync(0xffffffffu, any != 0)) continue;
+#pragma unroll
+                        for (int c = 0; c < S::CHUNKS; c += 2) {
+                            unsigned x[2][4];
+                            values(c, x);
+#pragma unroll
+                            for (int h = 0; h < TILES; ++h)
+#pragma unroll
+                                for (int q = 0; q < NQ; ++q) {
+                                    float more[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma<E8>(more, x[h], part[q][0], part[q][1]);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) o[q][(c / 2) * TILES + h][e] = fmaf(more[e], down, o[q][(c / 2) * TILES + h][e]);
+                                }
+                        }
+                    }
+                    continue;
+                }
+                unsigned pf[NQ][2];
+                [[maybe_unused]] unsigned pr[NQ][2];  // bfloat16: what the weights lose by rounding, as weights of their own
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float p0 = sc[q][k][2 * h], p1 = sc[q][k][2 * h + 1];
+                        const unsigned w = pack<E8>(p0, p1);
+                        pf[q][h] = turned(w);
+                        if constexpr (!E8) pr[q][h] = turned(pack<false>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
+                    }
+#pragma unroll
+                for (int c = 0; c < S::CHUNKS; c += 2) {
+                    unsigned x[2][4];
+                    values(c, x);
+#pragma unroll
+                    for (int h = 0; h < TILES; ++h)
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) {
+                            mma<E8>(o[q][(c / 2) * TILES + h], x[h], pf[q][0], pf[q][1]);
+                            if constexpr (!E8) mma<E8>(o[q][(c / 2) * TILES + h], x[h], pr[q][0], pr[q][1]);
+                        }
                 }
             }
         }
@@ -433,21 +494,22 @@ __global__ void __launch_bounds__(THREADS) attention_strip_kernel(const __grid_c
     float* wm = wo + WARPS * ROWS * D;           // [WARPS][ROWS]
     float* wl = wm + WARPS * ROWS;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int row = g + r * 8;
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (t == 0) wm[warp * ROWS + row] = m[r], wl[warp * ROWS + row] = l[r];
-        float* dst = wo + ((size_t)warp * ROWS + row) * D;
-        if constexpr (E8) {
+    for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c)
-                *reinterpret_cast<float4*>(dst + 16 * c + 4 * t) = make_float4(o[2 * c][2 * r], o[2 * c + 1][2 * r], o[2 * c][2 * r + 1], o[2 * c + 1][2 * r + 1]);
-        } else {
+        for (int e = 0; e < 2; ++e) {
+            const int row = q * 8 + 2 * t + e;
+            float sum = l[q][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            if (g == 0) wm[warp * ROWS + row] = m[q][e], wl[warp * ROWS + row] = sum;
+            float* dst = wo + ((size_t)warp * ROWS + row) * D;
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+            for (int i = 0; i < D / 16; ++i) {
+                if constexpr (E8) *reinterpret_cast<float2*>(dst + 16 * i + 2 * g) = make_float2(o[q][i][e], o[q][i][2 + e]);
+                else dst[16 * i + g] = o[q][i][e], dst[16 * i + 8 + g] = o[q][i][2 + e];
+            }
         }
-    }
     asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
     if (*failed) return;
     for (int e = tid; e < ROWS * (D / 4); e += 32 * WARPS) {
@@ -479,10 +541,14 @@ __global__ void __launch_bounds__(THREADS) attention_strip_kernel(const __grid_c
     }
 }
 
-__device__ __forceinline__ void load_floats(const float* p, float (&v)[4]) { load4(p, v); }
-__device__ __forceinline__ void load_floats(const float* p, float (&v)[2]) {
-    const float2 x = *reinterpret_cast<const float2*>(p);
-    v[0] = x.x, v[1] = x.y;
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
+    if constexpr (N == 4) {
+        load4(p, v);
+    } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] = x.x, v[1] = x.y;
+    }
 }
 
 // A warp puts a (token, head)'s pieces together.
@@ -541,34 +607,34 @@ EncodeTiled encode_tiled() {
 }
 
 // The cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and up to 128 bytes.
-template <bool E8>
+template <bool E8, int NQ>
 int cache_map(CUtensorMap* map, const void* cache, int pages, int kv_heads, int page_size) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return HB_BAD_ARGUMENT;
     const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)pages * 2 * kv_heads * page_size};
-    const cuuint64_t strides[1] = {(cuuint64_t)D * Shape<E8>::BYTES};
-    const cuuint32_t box[2] = {(cuuint32_t)(Shape<E8>::PANEL_BYTES / Shape<E8>::BYTES), (cuuint32_t)page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * Shape<E8, NQ>::BYTES};
+    const cuuint32_t box[2] = {(cuuint32_t)(Shape<E8, NQ>::PANEL_BYTES / Shape<E8, NQ>::BYTES), (cuuint32_t)page_size};
     const cuuint32_t elem[2] = {1, 1};
     const CUresult r = encode(map, E8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, elem,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, Shape<E8>::PANEL_BYTES == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, Shape<E8, NQ>::PANEL_BYTES == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
 }
 
-template <bool E8>
+template <bool E8, int NQ>
 int launch_strips(const Args& a, const void* cache, int n_items, cudaStream_t stream) {
     CUtensorMap map;
-    if (int code = cache_map<E8>(&map, cache, a.pages, a.kv_heads, a.page_size)) return code;
-    static const cudaError_t configured = cudaFuncSetAttribute(attention_strip_kernel<E8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8>::SMEM);
+    if (int code = cache_map<E8, NQ>(&map, cache, a.pages, a.kv_heads, a.page_size)) return code;
+    static const cudaError_t configured = cudaFuncSetAttribute(attention_strip_kernel<E8, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8, NQ>::SMEM);
     if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(attention_strip_kernel<E8>, dim3(n_items, a.kv_heads * a.chunks), dim3(THREADS), Shape<E8>::SMEM, stream, map, a);
+    return launch_after_previous(attention_strip_kernel<E8, NQ>, dim3(n_items, a.kv_heads * a.chunks), dim3(THREADS), Shape<E8, NQ>::SMEM, stream, map, a);
 }
 }  // namespace
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
-// strips [n_strips, 6]: see ITEM_WORDS; a strip has at most 16 / min(heads / kv_heads, 16) tokens.  pieces, sums null: one piece a row.
+// strips [n_strips, 6]: see ITEM_WORDS; a strip has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row.
 HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
-                                  const int* strips, int n_strips, const int* last, const int* piece_start, float* pieces, float* sums, int heads, int kv_heads,
+                                  const int* strips, int n_strips, int rows, const int* last, const int* piece_start, float* pieces, float* sums, int heads, int kv_heads,
                                   int page_size, int pages, float scale, int* status, cudaStream_t stream) {
     if (n_strips <= 0) return 0;
     if (!q || !out || !cache || !block_table || !strips || !last || !piece_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
@@ -576,11 +642,13 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)pieces) & 15) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
-    const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
+    if (rows != 8 && rows != MOST_ROWS) return HB_UNSUPPORTED_SIZE;
+    const int group = heads / kv_heads, gc = group < rows ? group : rows, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, strips, last, piece_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
-    return exponents ? launch_strips<true>(a, cache, n_strips, stream) : launch_strips<false>(a, cache, n_strips, stream);
+    if (rows == 8) return exponents ? launch_strips<true, 1>(a, cache, n_strips, stream) : launch_strips<false, 1>(a, cache, n_strips, stream);
+    return exponents ? launch_strips<true, 2>(a, cache, n_strips, stream) : launch_strips<false, 2>(a, cache, n_strips, stream);
 }
 
 // Puts the pieces [piece_start[tokens], heads, D] of every token together.  A token without a piece is zeros.

@@ -18,11 +18,13 @@ from .basic import status_word
 from .cache8 import Cache8, check_cache8
 from .native import KernelError, check, f32, library, ptr, require_cuda, sm_count, stream_ptr
 
-STRIP_ROWS = 16    # (token, head) rows of a strip
+STRIP_ROWS = 8, 16  # (token, head) rows of a strip: eight where no request has more
 TILE_ROWS = 256    # of an item of the tile kernel
-STRIP_KEYS, TILE_KEYS = 64, 128  # keys of a stage
-LEAST_KEYS = 192   # of a range that is cut further
-STRIPS_PER_SM = 2  # blocks of the strip kernel that share an SM
+STRIP_KEYS, TILE_KEYS = 128, 128  # keys that shares are counted in
+STRIPS_PER_SM = {8: 3, 16: 2}  # blocks of the strip kernel that share an SM
+# What an item costs beside its key tiles, in key tiles (its queries' way in, its rows' way out, the first tile's latency), and the least it is cut to.
+STRIP_OVERHEAD, LEAST_STRIP = 3, 2
+TILE_OVERHEAD, LEAST_TILES = 3, 2
 MOST_STRIP_ROWS = 64
 ITEM_WORDS = 6
 
@@ -34,40 +36,30 @@ def supported(head_dim: int, page_size: int) -> bool:
 class SharedPlan:
     """What the launches of a step need: the items, the last position each token sees and the first piece of each token, in one int32 tensor."""
 
-    __slots__ = ("tokens", "rows", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strips", "tiles", "data", "strips_at", "tiles_at", "last_at", "starts_at")
+    __slots__ = ("tokens", "rows", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strips", "strip_rows", "tiles", "data", "strips_at", "tiles_at", "last_at", "starts_at")
 
 
 def _tiles_of(first, last, keys):
     return -(-last // keys) - first // keys
 
 
-def _strip_share(ranges, cuts, across, sms) -> int:
-    """Key tiles of a strip's share: so many that the blocks fill the device once."""
-    work = int((cuts * _tiles_of(ranges[:, 3], ranges[:, 4], STRIP_KEYS)).sum()) * across
-    return max(LEAST_KEYS // STRIP_KEYS, -(-work // (STRIPS_PER_SM * sms)))
-
-
-ITEM_OVERHEAD = 3  # what an item of the tile kernel costs beside its key tiles, in key tiles: its queries' way in, its rows' way out, the first tile's latency
-
-
-def _tile_share(ranges, cuts, across, sms) -> int:
-    """Key tiles of a tile item's share: the longest that lets the items fill the device in one to four turns, whichever is soonest done."""
-    tiles = _tiles_of(ranges[:, 3], ranges[:, 4], TILE_KEYS)
-    longest = int(tiles.max())
+def _share(tiles, cuts, across, slots, overhead, least) -> int:
+    """Key tiles of an item's share: the longest that lets the items take the device's ``slots`` in one to four turns, whichever is soonest done.
+    An item costs ``overhead`` key tiles beside its own."""
     best = None
     for turns in range(1, 5):
-        low, high = 1, longest  # the smallest share with no more items than that
+        low, high = least, max(least, int(tiles.max()))  # the smallest share with no more items than that
         while low < high:
             middle = (low + high) // 2
-            if int((cuts * -(-tiles // middle)).sum()) * across <= turns * sms:
+            if int((cuts * -(-tiles // middle)).sum()) * across <= turns * slots:
                 high = middle
             else:
                 low = middle + 1
         items = int((cuts * -(-tiles // low)).sum()) * across
-        time = -(-items // sms) * (low + ITEM_OVERHEAD)
+        time = -(-items // slots) * (low + overhead)
         if best is None or time < best[0]:
             best = time, low
-    return max(2, best[1])
+    return best[1]
 
 
 def _cut(first, last, keys, share):
@@ -119,11 +111,14 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     group, sms = heads // kv_heads, sms or sm_count(device)
     shares, kinds = np.ones(len(ranges), dtype=np.int64), []
     wide = ranges[:, 1] * group > MOST_STRIP_ROWS
-    for chosen, rows, keys, choose in ((np.flatnonzero(~wide), STRIP_ROWS, STRIP_KEYS, _strip_share), (np.flatnonzero(wide), TILE_ROWS, TILE_KEYS, _tile_share)):
+    strip_rows = STRIP_ROWS[int((ranges[~wide, 1] * group > STRIP_ROWS[0]).any())]
+    for chosen, rows, keys, slots, overhead, least in ((np.flatnonzero(~wide), strip_rows, STRIP_KEYS, STRIPS_PER_SM[strip_rows] * sms, STRIP_OVERHEAD, LEAST_STRIP),
+                                                       (np.flatnonzero(wide), TILE_ROWS, TILE_KEYS, sms, TILE_OVERHEAD, LEAST_TILES)):
         of_kind, per = ranges[chosen], max(1, rows // group)  # tokens of an item
         cuts = -(-of_kind[:, 1] // per)
         if len(chosen):
-            parts, source, number, low, high = _cut(of_kind[:, 3], of_kind[:, 4], keys, choose(of_kind, cuts, kv_heads * -(-group // rows), sms))
+            parts, source, number, low, high = _cut(of_kind[:, 3], of_kind[:, 4], keys,
+                                                     _share(_tiles_of(of_kind[:, 3], of_kind[:, 4], keys), cuts, kv_heads * -(-group // rows), slots, overhead, least))
             shares[chosen] = parts
             kinds.append((of_kind, chosen, per, cuts, source, number, low, high))
         else:
@@ -157,7 +152,7 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     plan.tokens, plan.rows, plan.heads, plan.kv_heads, plan.head_dim = total, requests, heads, kv_heads, head_dim
     plan.longest = int(length[n > 0].max()) if total else 0
     plan.pieces, plan.joined = int(starts[-1]), bool((token_pieces != 1).any())
-    plan.strips, plan.tiles = len(items[0]), len(items[1])
+    plan.strips, plan.strip_rows, plan.tiles = len(items[0]), strip_rows, len(items[1])
     parts = [items[0].ravel(), items[1].ravel(), last, starts]
     plan.data = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device)
     at = plan.data.data_ptr() + 4 * np.concatenate([[0], np.cumsum([len(part) for part in parts])])
@@ -211,7 +206,7 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
             ptr(status_word(q.device)), stream), "attention_shared")
     if plan.strips:
         check(lib.hb_attention_strips(ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(entries), ptr(exponents), ptr(block_table), block_table.shape[1],
-                                      native.address(plan.strips_at), plan.strips, native.address(plan.last_at), native.address(plan.starts_at), native.address(pieces),
+                                      native.address(plan.strips_at), plan.strips, plan.strip_rows, native.address(plan.last_at), native.address(plan.starts_at), native.address(pieces),
                                       native.address(sums), heads, kv_heads, page_size, pages, f32(scale), ptr(status_word(q.device)), stream), "attention_shared")
     if plan.joined:
         check(lib.hb_attention_pieces(native.address(pieces), native.address(sums), native.address(plan.starts_at), ptr(out), out.stride(0), plan.tokens, heads, stream),
