@@ -1,7 +1,7 @@
 // Attention of a step's queries over paged caches in which groups of requests share their first positions, for caches of bfloat16 and of
 // 8-bit records (cache8.cu), head sizes 64 and 128 (HB_HEAD_DIM) and pages of 8 to 64 tokens.
 //
-// The host cuts the step into items: (tokens that stand together, a table row, a range of keys).  A group's shared positions are one range
+// The host (host/shared_plan.cpp) cuts the step into items: (tokens that stand together, a table row, a range of keys).  A group's shared positions are one range
 // for all of its tokens, so they are fetched once for all of them; what a request holds beyond them is a range for its own tokens; either may
 // be cut further so that the device is filled.  An item leaves for each of its (token, head) rows a piece
 //     m,  l = sum_j 2^(y_j - m),  o = sum_j 2^(y_j - m) v_j          y_j = score_j * scale * log2(e)
@@ -47,7 +47,8 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int MOST_ROWS = 16;   // (token, head) rows of a strip: 8 or 16
 constexpr int WARPS = 4;        // that compute; one more fetches
 constexpr int THREADS = 32 * (WARPS + 1);
-constexpr int ITEM_WORDS = 6;   // first token, tokens, table row, first key, last key + 1, number of the piece
+constexpr int ITEM_WORDS = 6;   // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of a request's own positions)
+constexpr int OWN_PIECE = 1 << 30;
 constexpr unsigned WAIT_LIMIT = 1u << 24;
 constexpr float HEADROOM = 8.f;  // m stands so far below the maximum: P up to 2^8 keeps float16's small weights further from its smallest number
 
@@ -142,8 +143,9 @@ struct Shape {
     static constexpr int STAGES = (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
     static constexpr int CHUNKS = D * BYTES / 16;             // 16-byte chunks of a row
     static constexpr int STEPS = 4 / BYTES;                   // products of 16 entries that a chunk a lane feeds
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * (2 * TILE + EXPS) + (E8 ? WARPS * 3 * KEYS * 4 : 0) + 2 * STAGES * 8 + 16;
-    static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024 && WARPS * ROWS * (D + 2) * 4 <= STAGES * 2 * TILE, "shared memory");
+    static constexpr int JOIN = 2 * ROWS * (D / 2 + 2) * 4;   // where the warps' results meet: of two warps, half of the entries at a time
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * (2 * TILE + EXPS) + (E8 ? WARPS * 3 * KEYS * 4 : 0) + JOIN + 2 * STAGES * 8 + 16;
+    static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "an SM's shared memory");
     // 16-byte chunk cc of row `key` as TMA's swizzle has placed it: the panel's row of 128 bytes (of 64, in pairs) with its chunks permuted.
     static __device__ __forceinline__ int at(int key, int cc) {
         if constexpr (PANEL_BYTES == 64) return key * 64 + ((cc ^ ((key >> 1) & 3)) << 4);
@@ -157,8 +159,10 @@ struct Args {
     const signed char* exponents;  // of an 8-bit cache
     const int* block_table; int table_width;
     const int* items;
+    const int* first_item;   // [blocks + 1]: block b takes items first_item[b] .. first_item[b + 1] - 1
     const int* last;         // [tokens]: the last position a token sees, -1 for none
     const int* piece_start;  // [tokens + 1]
+    const int* own_start;    // [tokens]
     float* pieces;           // [pieces, heads, D], or null: rows have one piece each and are stored at once
     float2* sums;            // [pieces, heads]: (m, l)
     int heads, kv_heads, page_size, pages;
@@ -176,25 +180,25 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
     // the tiles of all stages, the exponents of all stages, and each warp's keys' factors
     unsigned char* exps = ring + (size_t)S::STAGES * 2 * S::TILE;
     float* factors = reinterpret_cast<float*>(exps + (size_t)S::STAGES * S::EXPS);
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(factors + (E8 ? WARPS * 3 * S::KEYS : 0));
+    float* join = factors + (E8 ? WARPS * 3 * S::KEYS : 0);
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(join + S::JOIN / 4);
     unsigned long long* empty = full + S::STAGES;
     volatile int* failed = reinterpret_cast<volatile int*>(empty + S::STAGES);
+    volatile int* lost = failed + 1;  // a computing warp has given up
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full[s], E8 ? 33 : 1); mbar_init(&empty[s], WARPS); }
-        *failed = 0;
+        *failed = 0, *lost = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     let_next_kernel_start();
     wait_for_previous_kernels();
-    const int* item = a.items + (size_t)blockIdx.x * ITEM_WORDS;
-    const int tok0 = item[0], ntok = item[1], key_lo = item[3], key_hi = item[4], piece = item[5];
-    const int* table = a.block_table + (size_t)item[2] * a.table_width;
     const int kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
     const int group = a.heads / a.kv_heads, first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
-    const int start = key_lo / BN * BN, n_tiles = key_hi > key_lo ? (key_hi - start + BN - 1) / BN : 0;
+    const int first_item = a.first_item[blockIdx.x], end_item = a.first_item[blockIdx.x + 1];
+    int stage = 0;  // so far: the ring runs on across the block's items
 
     if (warp == WARPS) {
         // ------------------------------------------------------------------ producer (the whole warp)
@@ -203,340 +207,393 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
         const int ops = pages_per_tile * OPS_PER_PAGE;
         const unsigned page_bytes = 2u * a.page_size * D * S::BYTES;
         if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
-        int looked = -1;
-        for (int it = 0; it < n_tiles; ++it) {
-            const int s = it % S::STAGES, round = it / S::STAGES;
-            if (it % tiles_per_look == 0) {  // a page number per lane, for the next tiles
-                const int block = ((start + it * BN) >> shift) + lane;
-                looked = block < a.table_width ? __ldg(table + block) : -1;
-            }
-            int ok = 1;
-            if (lane == 0) ok = mbar_wait(&empty[s], (round & 1) ^ 1, failed) ? 1 : 0;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) {
-                if (lane == 0) { *failed = 1; atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_STRIPS); }
-                break;
-            }
-            const int base = start + it * BN, k0 = base + lane * a.page_size;
-            int page = __shfl_sync(0xffffffffu, looked, (it % tiles_per_look) * pages_per_tile + lane);
-            const bool wanted = lane < pages_per_tile && k0 < key_hi && k0 + a.page_size > key_lo;
-            if (wanted && (page < 0 || page >= a.pages)) atomicOr(a.status, HB_STATUS_BAD_PAGE);
-            if (!wanted || page >= a.pages) page = -1;
-            const unsigned valid = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            if (lane == 0) {
-                if (valid) mbar_expect_tx(&full[s], valid * page_bytes); else mbar_arrive(&full[s]);
-            }
-            __syncwarp();
-            unsigned char* stage = ring + (size_t)s * 2 * S::TILE;
-            if constexpr (E8) {  // the exponents of four keys and of four values a lane
-                const int key = lane * 4, from = __shfl_sync(0xffffffffu, page, key >> shift);
-                if (from >= 0) {
-                    const signed char* src = a.exponents + ((size_t)from * 2 * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1));
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * S::EXPS + key)), "l"(src) : "memory");
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * S::EXPS + BN + key)), "l"(src + (size_t)a.kv_heads * a.page_size) : "memory");
+        for (int index = first_item; index < end_item; ++index) {
+            const int* item = a.items + (size_t)index * ITEM_WORDS;
+            const int key_lo = item[3], key_hi = item[4], start = key_lo / BN * BN, n_tiles = (key_hi - start + BN - 1) / BN;
+            const int* table = a.block_table + (size_t)item[2] * a.table_width;
+            int looked = -1;
+            for (int it = 0; it < n_tiles; ++it, ++stage) {
+                const int s = stage % S::STAGES, round = stage / S::STAGES;
+                if (it % tiles_per_look == 0) {  // a page number per lane, for the next tiles
+                    const int block = ((start + it * BN) >> shift) + lane;
+                    looked = block < a.table_width ? __ldg(table + block) : -1;
                 }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
-            }
-            for (int op0 = 0; op0 < ops; op0 += 32) {
-                const int op = op0 + lane;
-                const int p = min(op, ops - 1) / OPS_PER_PAGE, rest = op % OPS_PER_PAGE, which = rest / S::PANELS, panel = rest - which * S::PANELS;
-                const int from = __shfl_sync(0xffffffffu, page, p);
-                if (op < ops && from >= 0)
-                    tma_load_2d(stage + which * S::TILE + panel * (BN * S::PANEL_BYTES) + p * a.page_size * S::PANEL_BYTES, &kv_map, &full[s],
-                                panel * (S::PANEL_BYTES / S::BYTES), ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
+                int ok = 1;
+                if (lane == 0) ok = mbar_wait(&empty[s], (round & 1) ^ 1, failed) ? 1 : 0;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) {
+                    if (lane == 0) { *failed = 1; atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_STRIPS); }
+                    return;
+                }
+                const int base = start + it * BN, k0 = base + lane * a.page_size;
+                int page = __shfl_sync(0xffffffffu, looked, (it % tiles_per_look) * pages_per_tile + lane);
+                const bool wanted = lane < pages_per_tile && k0 < key_hi && k0 + a.page_size > key_lo;
+                if (wanted && (page < 0 || page >= a.pages)) atomicOr(a.status, HB_STATUS_BAD_PAGE);
+                if (!wanted || page >= a.pages) page = -1;
+                const unsigned valid = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) {
+                    if (valid) mbar_expect_tx(&full[s], valid * page_bytes); else mbar_arrive(&full[s]);
+                }
+                __syncwarp();
+                unsigned char* tiles = ring + (size_t)s * 2 * S::TILE;
+                if constexpr (E8) {  // the exponents of four keys and of four values a lane
+                    const int key = lane * 4, from = __shfl_sync(0xffffffffu, page, key >> shift);
+                    if (from >= 0) {
+                        const signed char* src = a.exponents + ((size_t)from * 2 * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1));
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * S::EXPS + key)), "l"(src) : "memory");
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + s * S::EXPS + BN + key)), "l"(src + (size_t)a.kv_heads * a.page_size) : "memory");
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+                }
+                for (int op0 = 0; op0 < ops; op0 += 32) {
+                    const int op = op0 + lane;
+                    const int p = min(op, ops - 1) / OPS_PER_PAGE, rest = op % OPS_PER_PAGE, which = rest / S::PANELS, panel = rest - which * S::PANELS;
+                    const int from = __shfl_sync(0xffffffffu, page, p);
+                    if (op < ops && from >= 0)
+                        tma_load_2d(tiles + which * S::TILE + panel * (BN * S::PANEL_BYTES) + p * a.page_size * S::PANEL_BYTES, &kv_map, &full[s],
+                                    panel * (S::PANEL_BYTES / S::BYTES), ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
+                }
             }
         }
         return;
     }
     // ---------------------------------------------------------------------- consumers
     const int t = lane & 3, g = lane >> 2;
-    // Q's fragments: a lane's 16-byte chunk t + 4 j of a key feeds products STEPS j to STEPS j + STEPS - 1, four of its entries each, so a query's entries stand
-    // in the fragments likewise.
-    unsigned qf[NQ][D / 16][2];
-    float row_scale[NQ][2];
-    int hi[NQ][2];  // of columns 2 t and 2 t + 1: the last key a row sees; a row that is no one's sees what the others see, and is never stored
-    int sees_all_to = key_hi - 1;
+    [[maybe_unused]] float* mine = factors + warp * 3 * KEYS;  // of this warp's keys: 2^e of the key, e of the value, 2^-e of the value
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); };
+    for (int index = first_item; index < end_item; ++index) {
+        const int* item = a.items + (size_t)index * ITEM_WORDS;
+        const int tok0 = item[0], ntok = item[1], key_lo = item[3], key_hi = item[4], piece = item[5];
+        const int start = key_lo / BN * BN, n_tiles = (key_hi - start + BN - 1) / BN;
+        // Q's fragments: a lane's 16-byte chunk t + 4 j of a key feeds products STEPS j to STEPS j + STEPS - 1, four of its entries each, so a query's entries stand
+        // in the fragments likewise.
+        unsigned qf[NQ][D / 16][2];
+        float row_scale[NQ][2];
+        int hi[NQ][2];  // of columns 2 t and 2 t + 1: the last key a row sees; a row that is no one's sees what the others see, and is never stored
+        int sees_all_to = key_hi - 1;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const int v = q * 8 + g, tok = v / a.gc, hh = v - tok * a.gc;
-        const bool valid = tok < ntok && hh < heads_here;
-        const int mine_sees = valid ? min(key_hi - 1, a.last[tok0 + tok]) : key_hi - 1;
-        const bf16* src = a.q + (size_t)(tok0 + (valid ? tok : 0)) * a.q_stride + (size_t)(first_head + (valid ? hh : 0)) * D;
-        constexpr int PER_CHUNK = 16 / S::BYTES, PIECES = PER_CHUNK / 8;  // entries of a chunk; 16-byte pieces of them in bfloat16
-        uint4 raw[D / 32];  // this lane's quarter of the row: chunks t, t + 4, ...
+        for (int q = 0; q < NQ; ++q) {
+            const int v = q * 8 + g, tok = v / a.gc, hh = v - tok * a.gc;
+            const bool valid = tok < ntok && hh < heads_here;
+            const int mine_sees = valid ? min(key_hi - 1, a.last[tok0 + tok]) : key_hi - 1;
+            const bf16* src = a.q + (size_t)(tok0 + (valid ? tok : 0)) * a.q_stride + (size_t)(first_head + (valid ? hh : 0)) * D;
+            constexpr int PER_CHUNK = 16 / S::BYTES, PIECES = PER_CHUNK / 8;  // entries of a chunk; 16-byte pieces of them in bfloat16
+            uint4 raw[D / 32];  // this lane's quarter of the row: chunks t, t + 4, ...
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-            raw[i] = valid ? *reinterpret_cast<const uint4*>(src + (t + 4 * (i / PIECES)) * PER_CHUNK + (i % PIECES) * 8) : make_uint4(0, 0, 0, 0);
-        const unsigned* words = reinterpret_cast<const unsigned*>(raw);
-        float factor = 1.f, scale = a.scale_log2;
-        if constexpr (E8) {
-            // As float16 with the row's largest entry between 2^13 and 2^14: an entry of eight bits keeps them all down to 2^-27 of the largest.
-            float largest = 0.f;
+            for (int i = 0; i < D / 32; ++i)
+                raw[i] = valid ? *reinterpret_cast<const uint4*>(src + (t + 4 * (i / PIECES)) * PER_CHUNK + (i % PIECES) * 8) : make_uint4(0, 0, 0, 0);
+            const unsigned* words = reinterpret_cast<const unsigned*>(raw);
+            float factor = 1.f, scale = a.scale_log2;
+            if constexpr (E8) {
+                // As float16 with the row's largest entry between 2^13 and 2^14: an entry of eight bits keeps them all down to 2^-27 of the largest.
+                float largest = 0.f;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) largest = max3(largest, fabsf(__uint_as_float(words[i] << 16)), fabsf(__uint_as_float(words[i] & 0xffff0000u)));
-            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-            const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 13, -126), 126);
-            factor = power_of_two(-e);
-            scale *= power_of_two(e);
-        }
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-            qf[q][i >> 1][i & 1] = E8 ? pack<true>(__uint_as_float(words[i] << 16) * factor, __uint_as_float(words[i] & 0xffff0000u) * factor) : words[i];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            row_scale[q][e] = __shfl_sync(0xffffffffu, scale, (2 * t + e) * 4);
-            hi[q][e] = __shfl_sync(0xffffffffu, mine_sees, (2 * t + e) * 4);
-        }
-        sees_all_to = min(sees_all_to, __reduce_min_sync(0xffffffffu, mine_sees));  // positions that every row sees
-    }
-    float m[NQ][2], l[NQ][2];
-    int top_e = -128;  // the largest exponent among the values so far
-    float o[NQ][D / 16][4];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        m[q][0] = m[q][1] = -INFINITY, l[q][0] = l[q][1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) o[q][i][0] = o[q][i][1] = o[q][i][2] = o[q][i][3] = 0.f;
-    }
-    float* mine = factors + warp * 3 * KEYS;  // of this warp's keys: 2^e of the key, e of the value, 2^-e of the value
-
-    for (int it = 0; it < n_tiles; ++it) {
-        const int s = it % S::STAGES, round = it / S::STAGES;
-        if (!mbar_wait(&full[s], round & 1, failed)) {
-            *failed = 1;
-            atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_STRIPS);
-            break;
-        }
-        const unsigned char* ks = ring + (size_t)s * 2 * S::TILE;
-        const unsigned char* vs = ks + S::TILE;
-        const int key0 = warp * KEYS, pos0 = start + it * BN + key0;  // this warp's keys
-        if (pos0 < key_hi && pos0 + KEYS > key_lo) {
-            const bool whole = pos0 >= key_lo && pos0 + KEYS <= key_hi;  // all of them are in the item's range
-            bool far_apart = false;
-            if constexpr (E8) {  // a lane has one key; what was never stored is no exponent: kept in range, it meets only scores that are replaced
-                const signed char* ex = reinterpret_cast<const signed char*>(exps + s * S::EXPS + key0 + lane);
-                const int ke = min(max((int)ex[0], -40), 40), ve = min(max((int)ex[BN], -40), 40), pos = pos0 + lane;
-                mine[lane] = power_of_two(ke), mine[KEYS + lane] = (float)ve, mine[2 * KEYS + lane] = power_of_two(-ve);
-                const bool inside = pos >= key_lo && pos < key_hi;
-                top_e = __reduce_max_sync(0xffffffffu, inside ? max(top_e, ve) : top_e);
-                far_apart = top_e - __reduce_min_sync(0xffffffffu, inside ? ve : 127) > FAR_APART;
-                __syncwarp();
+                for (int i = 0; i < D / 8; ++i) largest = max3(largest, fabsf(__uint_as_float(words[i] << 16)), fabsf(__uint_as_float(words[i] & 0xffff0000u)));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 13, -126), 126);
+                factor = power_of_two(-e);
+                scale *= power_of_two(e);
             }
-            float sc[NQ][NK][4];  // of keys g and g + 8 of 16 and columns 2 t and 2 t + 1: [(key, column)]
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
+            for (int i = 0; i < D / 8; ++i)
+                qf[q][i >> 1][i & 1] = E8 ? pack<true>(__uint_as_float(words[i] << 16) * factor, __uint_as_float(words[i] & 0xffff0000u) * factor) : words[i];
 #pragma unroll
-                for (int k = 0; k < NK; ++k) sc[q][k][0] = sc[q][k][1] = sc[q][k][2] = sc[q][k][3] = 0.f;
+            for (int e = 0; e < 2; ++e) {
+                row_scale[q][e] = __shfl_sync(0xffffffffu, scale, (2 * t + e) * 4);
+                hi[q][e] = __shfl_sync(0xffffffffu, mine_sees, (2 * t + e) * 4);
+            }
+            sees_all_to = min(sees_all_to, __reduce_min_sync(0xffffffffu, mine_sees));  // positions that every row sees
+        }
+        float m[NQ][2], l[NQ][2];
+        int top_e = -128;  // the largest exponent among the values so far
+        float o[NQ][D / 16][4];
 #pragma unroll
-            for (int j = 0; j < S::CHUNKS / 4; ++j)
+        for (int q = 0; q < NQ; ++q) {
+            m[q][0] = m[q][1] = -INFINITY, l[q][0] = l[q][1] = 0.f;
 #pragma unroll
-                for (int k = 0; k < NK; ++k) {
-                    const uint4 raw0 = *reinterpret_cast<const uint4*>(ks + S::at(key0 + k * 16 + g, t + 4 * j)), raw1 = *reinterpret_cast<const uint4*>(ks + S::at(key0 + k * 16 + 8 + g, t + 4 * j));
-                    const unsigned* w0 = reinterpret_cast<const unsigned*>(&raw0);
-                    const unsigned* w1 = reinterpret_cast<const unsigned*>(&raw1);
-#pragma unroll
-                    for (int w = 0; w < S::STEPS; ++w) {
-                        unsigned x[4];
-                        if constexpr (E8) x[0] = halves_of(w0[w]), x[1] = halves_of(w1[w]), x[2] = upper_halves_of(w0[w]), x[3] = upper_halves_of(w1[w]);
-                        else x[0] = w0[2 * w], x[1] = w1[2 * w], x[2] = w0[2 * w + 1], x[3] = w1[2 * w + 1];
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q) mma<E8>(sc[q][k], x, qf[q][j * S::STEPS + w][0], qf[q][j * S::STEPS + w][1]);
-                    }
+            for (int i = 0; i < D / 16; ++i) o[q][i][0] = o[q][i][1] = o[q][i][2] = o[q][i][3] = 0.f;
+        }
+
+        for (int it = 0; it < n_tiles; ++it, ++stage) {
+            const int s = stage % S::STAGES, round = stage / S::STAGES;
+            if (!mbar_wait(&full[s], round & 1, failed)) {
+                *failed = 1, *lost = 1;
+                atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_STRIPS);
+                break;
+            }
+            const unsigned char* ks = ring + (size_t)s * 2 * S::TILE;
+            const unsigned char* vs = ks + S::TILE;
+            const int key0 = warp * KEYS, pos0 = start + it * BN + key0;  // this warp's keys
+            if (pos0 < key_hi && pos0 + KEYS > key_lo) {
+                const bool whole = pos0 >= key_lo && pos0 + KEYS <= key_hi;  // all of them are in the item's range
+                bool far_apart = false;
+                if constexpr (E8) {  // a lane has one key; what was never stored is no exponent: kept in range, it meets only scores that are replaced
+                    const signed char* ex = reinterpret_cast<const signed char*>(exps + s * S::EXPS + key0 + lane);
+                    const int ke = min(max((int)ex[0], -40), 40), ve = min(max((int)ex[BN], -40), 40), pos = pos0 + lane;
+                    mine[lane] = power_of_two(ke), mine[KEYS + lane] = (float)ve, mine[2 * KEYS + lane] = power_of_two(-ve);
+                    const bool inside = pos >= key_lo && pos < key_hi;
+                    top_e = __reduce_max_sync(0xffffffffu, inside ? max(top_e, ve) : top_e);
+                    far_apart = top_e - __reduce_min_sync(0xffffffffu, inside ? ve : 127) > FAR_APART;
+                    __syncwarp();
                 }
-            float back[NK][2];
-#pragma unroll
-            for (int k = 0; k < NK; ++k)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {  // key g + 8 h of 16
-                    float key_scale = 1.f, value_e = 0.f;
-                    if constexpr (E8) key_scale = mine[k * 16 + h * 8 + g], value_e = mine[KEYS + k * 16 + h * 8 + g], back[k][h] = mine[2 * KEYS + k * 16 + h * 8 + g];
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) sc[q][k][2 * h + e] = E8 ? fmaf(sc[q][k][2 * h + e] * key_scale, row_scale[q][e], value_e) : sc[q][k][2 * h + e] * row_scale[q][e];
-                }
-            if (pos0 < key_lo || pos0 + KEYS - 1 > sees_all_to) {
+                float sc[NQ][NK][4];  // of keys g and g + 8 of 16 and columns 2 t and 2 t + 1: [(key, column)]
 #pragma unroll
                 for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                    for (int k = 0; k < NK; ++k)
+                    for (int k = 0; k < NK; ++k) sc[q][k][0] = sc[q][k][1] = sc[q][k][2] = sc[q][k][3] = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int pos = pos0 + k * 16 + (e >> 1) * 8 + g;
-                            if (pos > hi[q][e & 1] || pos < key_lo) sc[q][k][e] = -INFINITY;
+                for (int j = 0; j < S::CHUNKS / 4; ++j)
+#pragma unroll
+                    for (int k = 0; k < NK; ++k) {
+                        const uint4 raw0 = *reinterpret_cast<const uint4*>(ks + S::at(key0 + k * 16 + g, t + 4 * j)), raw1 = *reinterpret_cast<const uint4*>(ks + S::at(key0 + k * 16 + 8 + g, t + 4 * j));
+                        const unsigned* w0 = reinterpret_cast<const unsigned*>(&raw0);
+                        const unsigned* w1 = reinterpret_cast<const unsigned*>(&raw1);
+#pragma unroll
+                        for (int w = 0; w < S::STEPS; ++w) {
+                            unsigned x[4];
+                            if constexpr (E8) x[0] = halves_of(w0[w]), x[1] = halves_of(w1[w]), x[2] = upper_halves_of(w0[w]), x[3] = upper_halves_of(w1[w]);
+                            else x[0] = w0[2 * w], x[1] = w1[2 * w], x[2] = w0[2 * w + 1], x[3] = w1[2 * w + 1];
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q) mma<E8>(sc[q][k], x, qf[q][j * S::STEPS + w][0], qf[q][j * S::STEPS + w][1]);
                         }
+                    }
+                float back[NK][2];
+#pragma unroll
+                for (int k = 0; k < NK; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {  // key g + 8 h of 16
+                        float key_scale = 1.f, value_e = 0.f;
+                        if constexpr (E8) key_scale = mine[k * 16 + h * 8 + g], value_e = mine[KEYS + k * 16 + h * 8 + g], back[k][h] = mine[2 * KEYS + k * 16 + h * 8 + g];
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) sc[q][k][2 * h + e] = E8 ? fmaf(sc[q][k][2 * h + e] * key_scale, row_scale[q][e], value_e) : sc[q][k][2 * h + e] * row_scale[q][e];
+                    }
+                if (pos0 < key_lo || pos0 + KEYS - 1 > sees_all_to) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int k = 0; k < NK; ++k)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int pos = pos0 + k * 16 + (e >> 1) * 8 + g;
+                                if (pos > hi[q][e & 1] || pos < key_lo) sc[q][k][e] = -INFINITY;
+                            }
+                }
+                bool rescale = false;
+                float alpha[NQ][2];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(sc[q][0][e], sc[q][0][2 + e]);
+#pragma unroll
+                        for (int k = 1; k < NK; ++k) mx = max3(mx, sc[q][k][e], sc[q][k][2 + e]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float m_new = fmaxf(m[q][e], mx - (E8 ? HEADROOM : 0.f));
+                        alpha[q][e] = m_new == -INFINITY ? 1.f : fast_exp2(m[q][e] - m_new);
+                        m[q][e] = m_new;
+                        rescale |= alpha[q][e] != 1.f;
+                        const float base = m_new == -INFINITY ? 0.f : m_new;
+                        l[q][e] *= alpha[q][e];
+#pragma unroll
+                        for (int k = 0; k < NK; ++k)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float p = fast_exp2(sc[q][k][2 * h + e] - base);
+                                sc[q][k][2 * h + e] = p;
+                                l[q][e] = E8 ? fmaf(p, back[k][h], l[q][e]) : l[q][e] + p;  // of this lane's keys; the lanes are added up at the end
+                            }
+                    }
+                if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) o[q][i][0] *= alpha[q][0], o[q][i][1] *= alpha[q][1], o[q][i][2] *= alpha[q][0], o[q][i][3] *= alpha[q][1];
+                }
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {  // 16 keys
+                    const int key = key0 + k * 16;
+                    // Values beyond the range read as zeros, whatever their slots hold.  A fragment register holds keys 2 t and 2 t + 1 in its halves.
+                    unsigned keep[2] = {0xffffffffu, 0xffffffffu};
+                    if (!whole) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int pos = pos0 + k * 16 + h * 8 + t * 2;
+                            keep[h] = (pos >= key_lo && pos < key_hi ? 0xffffu : 0u) | (pos + 1 >= key_lo && pos + 1 < key_hi ? 0xffff0000u : 0u);
+                        }
+                    }
+                    auto values = [&](int c, unsigned (&x)[2][4]) {  // 16 keys of two 16-byte chunks: 16 entries each in 8 bits; together in bfloat16, in x[0]
+                        unsigned b[4];
+                        ldmatrix_x4_trans(b, vs + S::at(key + (lane & 15), c + (lane >> 4)));
+                        if (!whole) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
+                        if constexpr (E8) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                // bytes (key 2t: entries 2g, 2g + 1; key 2t + 1: the same) -> the two keys' even entries, rows g, and their odd ones, rows g + 8
+                                const unsigned b0 = __byte_perm(b[2 * h], 0, 0x3120), b1 = __byte_perm(b[2 * h + 1], 0, 0x3120);
+                                x[h][0] = halves_of(b0), x[h][1] = upper_halves_of(b0), x[h][2] = halves_of(b1), x[h][3] = upper_halves_of(b1);
+                            }
+                        } else {
+                            x[0][0] = b[0], x[0][1] = b[2], x[0][2] = b[1], x[0][3] = b[3];
+                        }
+                    };
+                    constexpr int TILES = E8 ? 2 : 1;  // of 16 entries, of two chunks
+                    if (E8 && far_apart) {
+                        // Weights by size, 2^18 at a time, each lot scaled up to where float16 holds it and the products scaled back.
+#pragma unroll 1
+                        for (int lot = 0; lot < 7; ++lot) {
+                            const float up = power_of_two(18 * lot), down = power_of_two(-18 * lot), from = lot < 6 ? down * 0x1p-10f : 0.f, to = lot ? down * 256.f : INFINITY;
+                            auto scaled = [&](float p) { return p <= from || p > to ? 0.f : p * up; };
+                            unsigned part[NQ][2], any = 0;
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    part[q][h] = turned(pack<true>(scaled(sc[q][k][2 * h]), scaled(sc[q][k][2 * h + 1])));
+                                    any |= part[q][h];
+                                }
+                            if (!__any_sync(0xffffffffu, any != 0)) continue;
+#pragma unroll
+                            for (int c = 0; c < S::CHUNKS; c += 2) {
+                                unsigned x[2][4];
+                                values(c, x);
+#pragma unroll
+                                for (int h = 0; h < TILES; ++h)
+#pragma unroll
+                                    for (int q = 0; q < NQ; ++q) {
+                                        float more[4] = {0.f, 0.f, 0.f, 0.f};
+                                        mma<E8>(more, x[h], part[q][0], part[q][1]);
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e) o[q][(c / 2) * TILES + h][e] = fmaf(more[e], down, o[q][(c / 2) * TILES + h][e]);
+                                    }
+                            }
+                        }
+                        continue;
+                    }
+                    unsigned pf[NQ][2];
+                    [[maybe_unused]] unsigned pr[NQ][2];  // bfloat16: what the weights lose by rounding, as weights of their own
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float p0 = sc[q][k][2 * h], p1 = sc[q][k][2 * h + 1];
+                            const unsigned w = pack<E8>(p0, p1);
+                            pf[q][h] = turned(w);
+                            if constexpr (!E8) pr[q][h] = turned(pack<false>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
+                        }
+#pragma unroll
+                    for (int c = 0; c < S::CHUNKS; c += 2) {
+                        unsigned x[2][4];
+                        values(c, x);
+#pragma unroll
+                        for (int h = 0; h < TILES; ++h)
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q) {
+                                mma<E8>(o[q][(c / 2) * TILES + h], x[h], pf[q][0], pf[q][1]);
+                                if constexpr (!E8) mma<E8>(o[q][(c / 2) * TILES + h], x[h], pr[q][0], pr[q][1]);
+                            }
+                    }
+                }
             }
-            bool rescale = false;
-            float alpha[NQ][2];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+        // The warps' results meet: every warp brings its sums to the largest maximum, then 2 and 3 hand theirs to 0 and 1, and 1 to 0, lane by lane, half of the
+        // entries at a time.  Warp 0 stores.
+        float* tops = join + 2 * ROWS * (D / 2);  // [WARPS][ROWS]
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 4);
+                l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 8);
+                l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 16);
+                if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e];
+            }
+        meet();
+        if (*lost) return;  // all four warps see the same: they set it before they come here only
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = q * 8 + 2 * t + e;
+                float top = tops[row];
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) top = fmaxf(top, tops[w * ROWS + row]);
+                const float f = m[q][e] == -INFINITY ? 0.f : fast_exp2(m[q][e] - top);
+                m[q][e] = top;
+                l[q][e] *= f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[q][i][e] *= f, o[q][i][2 + e] *= f;
+            }
+        meet();
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int step = 2; step > 0; step >>= 1) {
+                float4* mine_o = reinterpret_cast<float4*>(join) + (warp & (step - 1)) * (NQ * (D / 32) * 32) + lane;
+                float2* mine_l = reinterpret_cast<float2*>(tops) + (warp & (step - 1)) * NQ * 4 + t;
+                if (warp >= step && warp < 2 * step) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) mine_o[(q * (D / 32) + i) * 32] = make_float4(o[q][half * (D / 32) + i][0], o[q][half * (D / 32) + i][1], o[q][half * (D / 32) + i][2], o[q][half * (D / 32) + i][3]);
+                        if (half == 0 && g == 0) mine_l[q * 4] = make_float2(l[q][0], l[q][1]);
+                    }
+                }
+                meet();
+                if (warp < step) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            const float4 more = mine_o[(q * (D / 32) + i) * 32];
+                            float (&into)[4] = o[q][half * (D / 32) + i];
+                            into[0] += more.x, into[1] += more.y, into[2] += more.z, into[3] += more.w;
+                        }
+                        if (half == 0) {
+                            const float2 more = mine_l[q * 4];
+                            l[q][0] += more.x, l[q][1] += more.y;
+                        }
+                    }
+                }
+                meet();
+            }
+        if (warp == 0) {
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float mx = fmaxf(sc[q][0][e], sc[q][0][2 + e]);
+                    const int v = q * 8 + 2 * t + e, tok = v / a.gc, hh = v - tok * a.gc;
+                    if (tok >= ntok || hh >= heads_here) continue;
+                    const int token = tok0 + tok, head = first_head + hh;
+                    if (a.pieces) {
+                        const size_t slot = (size_t)((piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (piece & (OWN_PIECE - 1))) * a.heads + head;
+                        float* dst = a.pieces + slot * D;
+                        if (g == 0) a.sums[slot] = make_float2(m[q][e], l[q][e]);
 #pragma unroll
-                    for (int k = 1; k < NK; ++k) mx = max3(mx, sc[q][k][e], sc[q][k][2 + e]);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float m_new = fmaxf(m[q][e], mx - (E8 ? HEADROOM : 0.f));
-                    alpha[q][e] = m_new == -INFINITY ? 1.f : fast_exp2(m[q][e] - m_new);
-                    m[q][e] = m_new;
-                    rescale |= alpha[q][e] != 1.f;
-                    const float base = m_new == -INFINITY ? 0.f : m_new;
-                    l[q][e] *= alpha[q][e];
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float p = fast_exp2(sc[q][k][2 * h + e] - base);
-                            sc[q][k][2 * h + e] = p;
-                            l[q][e] = E8 ? fmaf(p, back[k][h], l[q][e]) : l[q][e] + p;  // of this lane's keys; the lanes are added up at the end
-                        }
-                }
-            if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) o[q][i][0] *= alpha[q][0], o[q][i][1] *= alpha[q][1], o[q][i][2] *= alpha[q][0], o[q][i][3] *= alpha[q][1];
-            }
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {  // 16 keys
-                const int key = key0 + k * 16;
-                // Values beyond the range read as zeros, whatever their slots hold.  A fragment register holds keys 2 t and 2 t + 1 in its halves.
-                unsigned keep[2] = {0xffffffffu, 0xffffffffu};
-                if (!whole) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int pos = pos0 + k * 16 + h * 8 + t * 2;
-                        keep[h] = (pos >= key_lo && pos < key_hi ? 0xffffu : 0u) | (pos + 1 >= key_lo && pos + 1 < key_hi ? 0xffff0000u : 0u);
-                    }
-                }
-                auto values = [&](int c, unsigned (&x)[2][4]) {  // 16 keys of two 16-byte chunks: 16 entries each in 8 bits; together in bfloat16, in x[0]
-                    unsigned b[4];
-                    ldmatrix_x4_trans(b, vs + S::at(key + (lane & 15), c + (lane >> 4)));
-                    if (!whole) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
-                    if constexpr (E8) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            // bytes (key 2t: entries 2g, 2g + 1; key 2t + 1: the same) -> the two keys' even entries, rows g, and their odd ones, rows g + 8
-                            const unsigned b0 = __byte_perm(b[2 * h], 0, 0x3120), b1 = __byte_perm(b[2 * h + 1], 0, 0x3120);
-                            x[h][0] = halves_of(b0), x[h][1] = upper_halves_of(b0), x[h][2] = halves_of(b1), x[h][3] = upper_halves_of(b1);
+                        for (int i = 0; i < D / 16; ++i) {
+                            if constexpr (E8) *reinterpret_cast<float2*>(dst + 16 * i + 2 * g) = make_float2(o[q][i][e], o[q][i][2 + e]);
+                            else dst[16 * i + g] = o[q][i][e], dst[16 * i + 8 + g] = o[q][i][2 + e];
                         }
                     } else {
-                        x[0][0] = b[0], x[0][1] = b[2], x[0][2] = b[1], x[0][3] = b[3];
-                    }
-                };
-                constexpr int TILES = E8 ? 2 : 1;  // of 16 entries, of two chunks
-                if (E8 && far_apart) {
-                    // Weights by size, 2^18 at a time, each lot scaled up to where float16 holds it and the products scaled back.
-#pragma unroll 1
-                    for (int lot = 0; lot < 7; ++lot) {
-                        const float up = power_of_two(18 * lot), down = power_of_two(-18 * lot), from = lot < 6 ? down * 0x1p-10f : 0.f, to = lot ? down * 256.f : INFINITY;
-                        auto scaled = [&](float p) { return p <= from || p > to ? 0.f : p * up; };
-                        unsigned part[NQ][2], any = 0;
+                        const float inv = l[q][e] > 0.f ? 1.f / l[q][e] : (l[q][e] == 0.f ? 0.f : l[q][e]);  // a row that sees nothing is zeros; a NaN stays one
+                        bf16* dst = a.out + (size_t)token * a.out_stride + (size_t)head * D;
 #pragma unroll
-                        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                part[q][h] = turned(pack<true>(scaled(sc[q][k][2 * h]), scaled(sc[q][k][2 * h + 1])));
-                                any |= part[q][h];
+                        for (int i = 0; i < D / 16; ++i) {
+                            if constexpr (E8) {
+                                *reinterpret_cast<__nv_bfloat162*>(dst + 16 * i + 2 * g) = __floats2bfloat162_rn(o[q][i][e] * inv, o[q][i][2 + e] * inv);
+                            } else {
+                                dst[16 * i + g] = __float2bfloat16_rn(o[q][i][e] * inv);
+                                dst[16 * i + 8 + g] = __float2bfloat16_rn(o[q][i][2 + e] * inv);
                             }
-                        if (!__any_sync(0xffffffffu, any != 0)) continue;
-#pragma unroll
-                        for (int c = 0; c < S::CHUNKS; c += 2) {
-                            unsigned x[2][4];
-                            values(c, x);
-#pragma unroll
-                            for (int h = 0; h < TILES; ++h)
-#pragma unroll
-                                for (int q = 0; q < NQ; ++q) {
-                                    float more[4] = {0.f, 0.f, 0.f, 0.f};
-                                    mma<E8>(more, x[h], part[q][0], part[q][1]);
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[q][(c / 2) * TILES + h][e] = fmaf(more[e], down, o[q][(c / 2) * TILES + h][e]);
-                                }
                         }
                     }
-                    continue;
                 }
-                unsigned pf[NQ][2];
-                [[maybe_unused]] unsigned pr[NQ][2];  // bfloat16: what the weights lose by rounding, as weights of their own
-#pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float p0 = sc[q][k][2 * h], p1 = sc[q][k][2 * h + 1];
-                        const unsigned w = pack<E8>(p0, p1);
-                        pf[q][h] = turned(w);
-                        if constexpr (!E8) pr[q][h] = turned(pack<false>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
-                    }
-#pragma unroll
-                for (int c = 0; c < S::CHUNKS; c += 2) {
-                    unsigned x[2][4];
-                    values(c, x);
-#pragma unroll
-                    for (int h = 0; h < TILES; ++h)
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q) {
-                            mma<E8>(o[q][(c / 2) * TILES + h], x[h], pf[q][0], pf[q][1]);
-                            if constexpr (!E8) mma<E8>(o[q][(c / 2) * TILES + h], x[h], pr[q][0], pr[q][1]);
-                        }
-                }
-            }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
-    }
-    // The warps' results meet in the ring, which no copy targets any more once all of them have passed the last stage.
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
-    float* wo = reinterpret_cast<float*>(ring);  // [WARPS][ROWS][D]
-    float* wm = wo + WARPS * ROWS * D;           // [WARPS][ROWS]
-    float* wl = wm + WARPS * ROWS;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int row = q * 8 + 2 * t + e;
-            float sum = l[q][e];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            if (g == 0) wm[warp * ROWS + row] = m[q][e], wl[warp * ROWS + row] = sum;
-            float* dst = wo + ((size_t)warp * ROWS + row) * D;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                if constexpr (E8) *reinterpret_cast<float2*>(dst + 16 * i + 2 * g) = make_float2(o[q][i][e], o[q][i][2 + e]);
-                else dst[16 * i + g] = o[q][i][e], dst[16 * i + 8 + g] = o[q][i][2 + e];
-            }
-        }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
-    if (*failed) return;
-    for (int e = tid; e < ROWS * (D / 4); e += 32 * WARPS) {
-        const int row = e / (D / 4), c = (e - row * (D / 4)) * 4, tok = row / a.gc, hh = row - tok * a.gc;
-        if (tok >= ntok || hh >= heads_here) continue;
-        float top = -INFINITY, total = 0.f, value[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, wm[w * ROWS + row]);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float mw = wm[w * ROWS + row], f = mw == -INFINITY ? 0.f : fast_exp2(mw - top);
-            total = fmaf(f, wl[w * ROWS + row], total);
-            float part[4];
-            load4(wo + ((size_t)w * ROWS + row) * D + c, part);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) value[i] = fmaf(f, part[i], value[i]);
-        }
-        const int token = tok0 + tok, head = first_head + hh;
-        if (a.pieces) {
-            const size_t slot = (size_t)(a.piece_start[token] + piece) * a.heads + head;
-            store4(a.pieces + slot * D + c, value);
-            if (c == 0) a.sums[slot] = make_float2(top, total);
-        } else {
-            const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);  // a row that sees nothing is zeros; a NaN stays one
-#pragma unroll
-            for (int i = 0; i < 4; ++i) value[i] *= inv;
-            store4(a.out + (size_t)token * a.out_stride + (size_t)head * D + c, value);
         }
     }
 }
@@ -622,22 +679,22 @@ int cache_map(CUtensorMap* map, const void* cache, int pages, int kv_heads, int 
 }
 
 template <bool E8, int NQ>
-int launch_strips(const Args& a, const void* cache, int n_items, cudaStream_t stream) {
+int launch_strips(const Args& a, const void* cache, int blocks, cudaStream_t stream) {
     CUtensorMap map;
     if (int code = cache_map<E8, NQ>(&map, cache, a.pages, a.kv_heads, a.page_size)) return code;
     static const cudaError_t configured = cudaFuncSetAttribute(attention_strip_kernel<E8, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8, NQ>::SMEM);
     if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(attention_strip_kernel<E8, NQ>, dim3(n_items, a.kv_heads * a.chunks), dim3(THREADS), Shape<E8, NQ>::SMEM, stream, map, a);
+    return launch_after_previous(attention_strip_kernel<E8, NQ>, dim3(blocks, a.kv_heads * a.chunks), dim3(THREADS), Shape<E8, NQ>::SMEM, stream, map, a);
 }
 }  // namespace
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
-// strips [n_strips, 6]: see ITEM_WORDS; a strip has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row.
+// items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row.
 HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
-                                  const int* strips, int n_strips, int rows, const int* last, const int* piece_start, float* pieces, float* sums, int heads, int kv_heads,
+                                  const int* items, const int* first_item, int blocks, int rows, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
                                   int page_size, int pages, float scale, int* status, cudaStream_t stream) {
-    if (n_strips <= 0) return 0;
-    if (!q || !out || !cache || !block_table || !strips || !last || !piece_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
+    if (blocks <= 0) return 0;
+    if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || q_stride % 8 || out_stride % 4) return HB_BAD_ARGUMENT;
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)pieces) & 15) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
@@ -645,10 +702,10 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     if (rows != 8 && rows != MOST_ROWS) return HB_UNSUPPORTED_SIZE;
     const int group = heads / kv_heads, gc = group < rows ? group : rows, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
-    const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, strips, last, piece_start, pieces, (float2*)sums,
+    const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
-    if (rows == 8) return exponents ? launch_strips<true, 1>(a, cache, n_strips, stream) : launch_strips<false, 1>(a, cache, n_strips, stream);
-    return exponents ? launch_strips<true, 2>(a, cache, n_strips, stream) : launch_strips<false, 2>(a, cache, n_strips, stream);
+    if (rows == 8) return exponents ? launch_strips<true, 1>(a, cache, blocks, stream) : launch_strips<false, 1>(a, cache, blocks, stream);
+    return exponents ? launch_strips<true, 2>(a, cache, blocks, stream) : launch_strips<false, 2>(a, cache, blocks, stream);
 }
 
 // Puts the pieces [piece_start[tokens], heads, D] of every token together.  A token without a piece is zeros.

@@ -2,7 +2,7 @@
 // for few rows), over paged caches of bfloat16 and of 8-bit records (cache8.cu), head sizes 64 and 128 (HB_HEAD_DIM), pages of 8 to 64 tokens.
 //
 // An item is up to 256 (token, head) rows of one key/value head and a range of keys: all of a group's tokens over a share of the positions that they
-// hold in common, or a portion of a prompt over its own.  One persistent block per SM holds all of the SM's tensor memory and takes every gridDim-th item; two
+// hold in common, or a portion of a prompt over its own.  One block per SM holds all of the SM's tensor memory and takes its share of the items; two
 // halves of 128 rows (H and L) walk the same tiles of 128 keys, so that the tensor core runs one half's products under the other half's softmax:
 //   warp 0       fetches: one cp.async.bulk.tensor per page (and 128-byte panel) of K and of V, the queries as one 3-D box per 64-column panel;
 //   warp 1       issues S_x = Q_x K^T (M 128, N 128) and O_x += P_x V (P from tensor memory, V MN-major), each half's next S right behind its last product;
@@ -43,7 +43,8 @@ constexpr int RAW_BYTES = BN * D;             // a tile of codes
 constexpr int STAGES = 2;                     // of K tiles and of V tiles as the products read them; one tile of codes of each is under way
 constexpr int TMEM_COLS = 512;                // S_H [0,128) S_L [128,256) O_H [256,256+D) O_L [384,384+D); P_x over S_x
 constexpr int O_COL = 256;
-constexpr int ITEM_WORDS = 6;                 // first token, tokens, table row, first key, last key + 1, number of the piece
+constexpr int ITEM_WORDS = 6;                 // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of its own positions)
+constexpr int OWN_PIECE = 1 << 30;
 constexpr unsigned WAIT_LIMIT = 1u << 24;
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -234,9 +235,11 @@ struct Args {
     const signed char* exponents;  // of an 8-bit cache
     bf16* out; int out_stride;
     const int* block_table; int table_width;
-    const int* items; int n_items;  // of each key/value head and head chunk
+    const int* items;
+    const int* first_item;          // [blocks + 1]: block b takes items first_item[b] .. first_item[b + 1] - 1
     const int* last;                // [tokens]: the last position a token sees, -1 for none
     const int* piece_start;         // [tokens + 1]
+    const int* own_start;           // [tokens]
     float* pieces;                  // [pieces, heads, D], or null: rows have one piece each and are stored at once
     float2* sums;                   // [pieces, heads]: (m, l)
     int heads, kv_heads, page_size, pages;
@@ -249,7 +252,9 @@ template <bool E8>
 struct Shape {
     static constexpr int WARPS = E8 ? 20 : 12, THREADS = 32 * WARPS;
     // Registers a thread, by groups of four warps, of the 96 that 640 threads are launched with (128 * 56 + 256 * 152 + 256 * 56 = 60,416 of 61,440)
-    [[maybe_unused]] static constexpr int FEW = 56, MANY = 152, CONVERTING = 56;
+    [[maybe_unused]] static constexpr int FEW = 56;
+    [[maybe_unused]] static constexpr int MANY = 152;
+    [[maybe_unused]] static constexpr int CONVERTING = 56;
     static constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
     // How far (in powers of two) a maximum may be outgrown before the row is rescaled.  A stale maximum changes no result (numerator and denominator use the same
     // one) as long as nothing overflows: weights are float16 up to 2^15, or bfloat16 and their sums float.
@@ -265,7 +270,7 @@ struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
 struct Item {
-    int tok0, ntok, key_lo, key_hi, piece, kvh, first_head, heads_here, start, n_tiles, halves;
+    int tok0, ntok, key_lo, key_hi, piece, start, n_tiles, halves;
     const int* table;
 };
 
@@ -332,21 +337,18 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
     tc_fence_after();
     const unsigned tmem = *tmem_slot;
     const int shift = 31 - __clz(a.page_size);
-    const int group = a.heads / a.kv_heads, ys = a.kv_heads * a.chunks, total = a.n_items * ys;
+    const int group = a.heads / a.kv_heads, kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
+    const int first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
+    const int first_item = a.first_item[blockIdx.x], end_item = a.first_item[blockIdx.x + 1];
 
     // The roles run through the block's items each at its own pace, held together by the barriers of the data alone.  A wait by parity tells "this phase is over"
     // only to a thread that is at most one phase behind: every barrier's waiter is the one whose own arrival, on the barrier's counterpart, lets the next
     // phase begin, or it looks at the barrier once per phase.
     auto read_item = [&](int index) {
         Item it;
-        const int* words = a.items + (size_t)(index / ys) * ITEM_WORDS;
-        const int y = index % ys;
+        const int* words = a.items + (size_t)index * ITEM_WORDS;
         it.tok0 = words[0], it.ntok = words[1], it.key_lo = words[3], it.key_hi = words[4], it.piece = words[5];
         it.table = a.block_table + (size_t)words[2] * a.table_width;
-        it.kvh = y / a.chunks;
-        const int chunk = y - it.kvh * a.chunks;
-        it.first_head = it.kvh * group + chunk * a.gc;
-        it.heads_here = min(a.gc, group - chunk * a.gc);
         it.start = it.key_lo / BN * BN;
         it.n_tiles = it.key_hi > it.key_lo ? (it.key_hi - it.start + BN - 1) / BN : 0;
         it.halves = it.ntok * a.gc > BM ? 2 : 1;
@@ -365,13 +367,13 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
         const int pages_per_tile = BN >> shift, tokens_per_item = ROWS / a.gc;
         bool alive = true;
         int g = 0, edges = 0, round = 0;  // g: tiles so far
-        for (int index = blockIdx.x; index < total && alive; index += gridDim.x, ++round) {
+        for (int index = first_item; index < end_item && alive; ++index, ++round) {
             const Item it = read_item(index);
             if (lane == 0) {  // the queries: tokens beyond the item's own come along, or are filled with zeros
                 if (!mbar_wait(q_empty, (round & 1) ^ 1, failed)) alive = false;
                 if (alive) {
                     mbar_expect_tx(q_full, (unsigned)(PANELS * 128 * a.gc * tokens_per_item));
-                    for (int h = 0; h < PANELS; ++h) tma_load_3d(qs + h * Q_PANEL * 2, &q_map, q_full, h * 64, it.first_head, it.tok0);
+                    for (int h = 0; h < PANELS; ++h) tma_load_3d(qs + h * Q_PANEL * 2, &q_map, q_full, h * 64, first_head, it.tok0);
                 }
             }
             alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
@@ -403,12 +405,12 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                     if constexpr (E8) {
                         const int key = lane * 4, from = __shfl_sync(0xffffffffu, my_page, key >> shift);
                         if (from >= 0) {
-                            const signed char* src = a.exponents + (((size_t)from * 2 + which) * a.kv_heads + it.kvh) * a.page_size + (key & (a.page_size - 1));
+                            const signed char* src = a.exponents + (((size_t)from * 2 + which) * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1));
                             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + which * BN + key)), "l"(src) : "memory");
                         }
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
                         if (my_page >= 0)
-                            tma_load_2d(raw_tiles + which * RAW_BYTES + lane * a.page_size * D, &kv_map, full, 0, ((my_page * 2 + which) * a.kv_heads + it.kvh) * a.page_size);
+                            tma_load_2d(raw_tiles + which * RAW_BYTES + lane * a.page_size * D, &kv_map, full, 0, ((my_page * 2 + which) * a.kv_heads + kvh) * a.page_size);
                     } else {
                         unsigned char* stage = which ? v_ring + (size_t)s * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
                         const int ops = pages_per_tile * PANELS;
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                             const int op = op0 + lane, p = min(op, ops - 1) / PANELS, h = op % PANELS;
                             const int from = __shfl_sync(0xffffffffu, my_page, p);
                             if (op < ops && from >= 0)
-                                tma_load_2d(stage + h * KV_PANEL * 2 + p * a.page_size * 128, &kv_map, full, h * 64, ((from * 2 + which) * a.kv_heads + it.kvh) * a.page_size);
+                                tma_load_2d(stage + h * KV_PANEL * 2 + p * a.page_size * 128, &kv_map, full, h * 64, ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
                         }
                         if (which && edge) {
                             ok = mbar_wait(edge_full, edges & 1, failed) ? 1 : 0;
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             };
             bool ok = true;
             int g0 = 0, h0[2] = {0, 0}, round = 0;
-            for (int index = blockIdx.x; index < total && ok; index += gridDim.x, ++round) {
+            for (int index = first_item; index < end_item && ok; ++index, ++round) {
                 const Item it = read_item(index);
                 if (!mbar_wait(q_full, round & 1, failed)) { ok = false; break; }
                 if (it.n_tiles == 0) { umma_commit_at(smem_u32(q_empty)); continue; }
@@ -518,11 +520,11 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
         const Pair scale2{scale, scale}, minus_one{-1.f, -1.f};
         int hx = 0, g0 = 0, mine = 0;  // tiles this half has seen; the block's tiles; items this half has had a part in
         bool ok = true;
-        for (int index = blockIdx.x; index < total && ok; index += gridDim.x) {
+        for (int index = first_item; index < end_item && ok; ++index) {
             const Item it = read_item(index);
             if (x >= it.halves) { g0 += it.n_tiles; continue; }
             const int tok = v / a.gc, hh = v - tok * a.gc;
-            const bool row_valid = tok < it.ntok && hh < it.heads_here;
+            const bool row_valid = tok < it.ntok && hh < heads_here;
             // a row that is no one's is computed like the item's last token and never stored: it takes the same way through the code as its neighbours
             const int token = it.tok0 + min(tok, it.ntok - 1), hi = min(it.key_hi - 1, a.last[token]);
             float m = -INFINITY, l = 0.f;
@@ -645,7 +647,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             if (ok) {
-                const size_t slot = row_valid && a.pieces ? (size_t)(a.piece_start[token] + it.piece) * a.heads + it.first_head + hh : 0;
+                const size_t slot = row_valid && a.pieces ? (size_t)((it.piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (it.piece & (OWN_PIECE - 1))) * a.heads + first_head + hh : 0;
                 const float back = E8 ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
                 const float inv = a.pieces ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
 #pragma unroll
@@ -666,7 +668,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                                          "r"(__float_as_uint(o[i + 2])), "r"(__float_as_uint(o[i + 3])), "r"(__float_as_uint(o[i + 4])), "r"(__float_as_uint(o[i + 5])),
                                          "r"(__float_as_uint(o[i + 6])), "r"(__float_as_uint(o[i + 7])) : "memory");
                     } else if (row_valid) {
-                        uint2* dst = reinterpret_cast<uint2*>(a.out + (size_t)token * a.out_stride + (size_t)(it.first_head + hh) * D + c);
+                        uint2* dst = reinterpret_cast<uint2*>(a.out + (size_t)token * a.out_stride + (size_t)(first_head + hh) * D + c);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) dst[i] = make_uint2(pack_bf16x2(o[4 * i] * inv, o[4 * i + 1] * inv), pack_bf16x2(o[4 * i + 2] * inv, o[4 * i + 3] * inv));
                     }
@@ -686,7 +688,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
         constexpr int LOWEST = -12, HIGHEST = 7;  // of e - e0, for float16
         bool ok = true;
         int g = 0;
-        for (int index = blockIdx.x; index < total && ok; index += gridDim.x) {
+        for (int index = first_item; index < end_item && ok; ++index) {
             const Item it = read_item(index);
             int e0 = 0;
             for (int t = 0; t < it.n_tiles; ++t, ++g) {
@@ -789,7 +791,7 @@ EncodeTiled encode_tiled() {
 }
 
 template <bool E8>
-int launch(const Args& a, const void* q, int q_stride, int n_tokens, const void* cache, cudaStream_t stream) {
+int launch(const Args& a, int blocks, const void* q, int q_stride, int n_tokens, const void* cache, cudaStream_t stream) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return HB_BAD_ARGUMENT;
     // the cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and up to 128 bytes
@@ -810,28 +812,25 @@ int launch(const Args& a, const void* q, int q_stride, int n_tokens, const void*
         return HB_BAD_ARGUMENT;
     static const cudaError_t configured = cudaFuncSetAttribute(attention_shared_kernel<E8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8>::SMEM);
     if (configured != cudaSuccess) return (int)configured;
-    int device = 0, sms = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return HB_BAD_ARGUMENT;
-    const long long total = (long long)a.n_items * a.kv_heads * a.chunks;
-    if (total > 0x7fffffffLL - sms) return HB_UNSUPPORTED_SIZE;
-    return launch_after_previous(attention_shared_kernel<E8>, dim3((unsigned)(total < sms ? total : sms)), dim3(Shape<E8>::THREADS), Shape<E8>::SMEM, stream, map, q_map, a);
+    return launch_after_previous(attention_shared_kernel<E8>, dim3(blocks, a.kv_heads * a.chunks), dim3(Shape<E8>::THREADS), Shape<E8>::SMEM, stream, map, q_map, a);
 }
 }  // namespace
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
-// items [n_items, 6]: see ITEM_WORDS; an item has at most 256 / min(heads / kv_heads, 256) tokens.  pieces, sums null: one piece a row.
+// items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most 256 / min(heads / kv_heads, 256) tokens.  pieces, sums null: one piece a row.
 HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_tokens, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table,
-                                        int table_width, const int* items, int n_items, const int* last, const int* piece_start, float* pieces, float* sums, int heads,
+                                        int table_width, const int* items, const int* first_item, int blocks, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads,
                                         int kv_heads, int page_size, int pages, float scale, int* status, cudaStream_t stream) {
-    if (n_items <= 0) return 0;
-    if (!q || !out || !cache || !block_table || !items || !last || !piece_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
+    if (blocks <= 0) return 0;
+    if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || n_tokens <= 0 || q_stride % 8 || out_stride % 4) return HB_BAD_ARGUMENT;
     if (!(scale > 0.f)) return HB_BAD_ARGUMENT;  // the row maximum is taken before the scores are scaled
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)pieces & 31) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
-    const Args a{(const signed char*)exponents, (bf16*)out, out_stride, block_table, table_width, items, n_items, last, piece_start, pieces, (float2*)sums,
+    if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
+    const Args a{(const signed char*)exponents, (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
-    return exponents ? launch<true>(a, q, q_stride, n_tokens, cache, stream) : launch<false>(a, q, q_stride, n_tokens, cache, stream);
+    return exponents ? launch<true>(a, blocks, q, q_stride, n_tokens, cache, stream) : launch<false>(a, blocks, q, q_stride, n_tokens, cache, stream);
 }

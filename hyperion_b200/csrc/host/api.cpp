@@ -9,6 +9,7 @@
 #include "cache_index.hpp"
 #include "safetensors.hpp"
 #include "scheduler.hpp"
+#include "shared_plan.hpp"
 
 #define HB_API extern "C" __attribute__((visibility("default")))
 
@@ -272,6 +273,33 @@ HB_API int hb_plan_attention(int n_rows, const int* counts, int tokens_per_tile,
         }
         *n_tiles = t;
         *n_items = it;
+    });
+}
+
+namespace {
+thread_local std::vector<int> planned;  // the last plan of attention behind shared positions
+}
+HB_API int hb_plan_shared(int n_requests, const int64_t* counts, const int64_t* lengths, int n_groups, const int64_t* groups, int64_t heads, int64_t kv_heads, int64_t sms,
+                          int64_t* sizes) {
+    return guarded([&] {
+        require(n_requests >= 0 && n_groups >= 0 && sizes, "plan_shared: counts must not be negative");
+        std::vector<hb::SharedGroup> shared;
+        for (int g = 0; g < n_groups; ++g) shared.push_back({groups[3 * g], groups[3 * g + 1], groups[3 * g + 2]});
+        const hb::SharedPlan plan = hb::plan_shared(std::vector<int64_t>(counts, counts + n_requests), std::vector<int64_t>(lengths, lengths + n_requests), shared, heads, kv_heads, sms);
+        planned.clear();
+        int64_t* places = sizes + 8;
+        for (const std::vector<int>* part : {&plan.strips.items, &plan.strips.first, &plan.tiles.items, &plan.tiles.first, &plan.last, &plan.starts, &plan.own}) {
+            *places++ = (int64_t)planned.size();
+            planned.insert(planned.end(), part->begin(), part->end());
+        }
+        const int64_t figures[8] = {(int64_t)planned.size(), plan.strips.blocks(), plan.strip_rows, plan.tiles.blocks(), (int64_t)plan.last.size(), plan.starts.back(), plan.joined, plan.longest};
+        std::copy(figures, figures + 8, sizes);
+    });
+}
+HB_API int hb_plan_shared_take(int* words, int64_t capacity) {
+    return guarded([&] {
+        require(capacity >= (int64_t)planned.size(), "plan_shared: the plan does not fit the buffer");
+        std::copy(planned.begin(), planned.end(), words);
     });
 }
 

@@ -74,6 +74,13 @@ int hb_step_decode_widths(const HbCache* cache, int n_rows, const int64_t* keys,
 int hb_plan_attention(int n_rows, const int* counts, int tokens_per_tile, int token_shape_max, int* tiles, int* n_tiles, int* items,
                       int* n_items);
 
+/* Attention behind shared positions: counts and lengths of the step's requests, groups as triples (first request, requests, positions). Plans the step and
+ * keeps the plan for this thread; sizes receives: words, strip blocks, rows of a strip, tile blocks, tokens, pieces, whether pieces have to be joined, the longest length, and
+ * the places in words of: strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces. */
+int hb_plan_shared(int n_requests, const int64_t* counts, const int64_t* lengths, int n_groups, const int64_t* groups, int64_t heads, int64_t kv_heads, int64_t sms, int64_t* sizes);
+/* Copies this thread's last plan. */
+int hb_plan_shared_take(int* words, int64_t capacity);
+
 /* ---- scheduler ---- */
 typedef struct HbScheduler HbScheduler;
 /* group_windows: one entry per paged group of the cache (0 = it keeps every key), group_keeps likewise (the first positions a windowed

@@ -6,35 +6,44 @@ import pytest
 
 from hyperion_b200.ops import KernelError, plan_shared
 
+OWN = 1 << 30
 
-def items_of(plan):
-    flat = plan.data.numpy()
-    n = (plan.strips + plan.tiles) * 6
-    return flat[:n].reshape(-1, 6), flat[n: n + plan.tokens], flat[n + plan.tokens: n + 2 * plan.tokens + 1]
+
+def parts_of(plan):
+    """(items of strips with their blocks, the same of tiles, last positions, first pieces, first own pieces)"""
+    flat, at = plan.data.numpy(), plan.places + [plan.data.numel()]
+    part = [flat[at[i]: at[i + 1]] for i in range(7)]
+    walks = []
+    for items, first in ((part[0], part[1]), (part[2], part[3])):
+        items = items.reshape(-1, 6)
+        assert first[0] == 0 and first[-1] == len(items) and (np.diff(first) > 0).all()
+        walks.append((items, np.repeat(np.arange(len(first) - 1), np.diff(first))))
+    return walks[0], walks[1], part[4], part[5], part[6]
 
 
 def covered(counts, lengths, heads, kv, groups, sms):
     plan = plan_shared(counts, lengths, heads, kv, 64, shared=groups, device="cpu", sms=sms)
-    items, last, starts = items_of(plan)
+    strips, tiles, last, starts, own = parts_of(plan)
     shared = np.zeros(len(counts), dtype=int)
     for first, n, positions in groups:
         shared[first: first + n] = positions
     owner = np.repeat(np.arange(len(counts)), counts)
     seen, pieces = [set() for _ in owner], [[] for _ in owner]
-    for i, (tok, n, row, low, high, number) in enumerate(items):
-        rows = plan.strip_rows if i < plan.strips else 256
-        assert n >= 1 and high > low and n * min(rows, heads // kv) <= rows
-        for t in range(tok, tok + n):
-            assert row == owner[t] or (high <= shared[owner[t]] == shared[row])  # another request's table for shared positions only
-            assert not seen[t] & set(range(low, high))
-            seen[t] |= set(range(low, high))
-            pieces[t].append(number)
+    for rows, (items, _) in ((plan.strip_rows, strips), (256, tiles)):
+        for tok, n, row, low, high, number in items:
+            assert n >= 1 and high > low and n * min(rows, heads // kv) <= rows
+            for t in range(tok, tok + n):
+                assert (low >= shared[row] and row == owner[t]) if number & OWN else (high <= shared[owner[t]] == shared[row])  # another request's table for shared positions only
+                assert not seen[t] & set(range(low, high))
+                seen[t] |= set(range(low, high))
+                pieces[t].append((own if number & OWN else starts)[t] + (number & (OWN - 1)))
     first = np.cumsum(np.concatenate([[0], counts]))
     for t, r in enumerate(owner):
-        assert last[t] == lengths[r] - counts[r] + (t - first[r])
-        assert seen[t] == (set(range(lengths[r])) if lengths[r] else set())
-        assert sorted(pieces[t]) == list(range(starts[t + 1] - starts[t]))
-    assert plan.pieces == (starts[-1] if len(owner) else 0) and plan.joined == any(len(p) != 1 for p in pieces)
+        assert last[t] == max(-1, lengths[r] - counts[r] + (t - first[r]))
+        assert seen[t] == set(range(lengths[r]))
+        assert sorted(pieces[t]) == list(range(starts[t], starts[t + 1]))
+    assert plan.pieces == starts[-1] and plan.joined == any(len(p) != 1 for p in pieces)
+    assert (plan.strip_blocks, plan.tile_blocks) == tuple(len(np.unique(b)) for _, b in (strips, tiles))
     return plan
 
 
@@ -58,21 +67,30 @@ def test_every_pair_once(heads, kv, sms):
         covered(counts.tolist(), lengths.tolist(), heads, kv, groups, sms)
 
 
-def test_a_prompt_s_portion_and_a_step_of_nothing():
+def test_portions_of_prompts_and_steps_of_nothing():
     covered([70], [500], 14, 2, [], 148)
+    covered([300, 1, 20], [900, 2000, 700], 16, 4, [(0, 3, 555)], 148)
     covered([0, 0], [5, 0], 14, 2, [(0, 2, 3)], 148)
     covered([], [], 14, 2, [], 148)
 
 
-def test_the_device_is_filled_but_not_cut_to_pieces():
-    plan = covered([1], [20000], 28, 4, [], 148)
-    assert 148 <= plan.strips * 4 <= 3 * 148
-    assert covered([1], [190], 28, 4, [], 148).strips == 1
+@pytest.mark.parametrize("counts,lengths,groups", [([1], [20000], ()), ([1] * 64, list(range(1000, 2000, 16))[:64][: 63] + [2000], ()), ([1] * 30, [5000] * 30, ((0, 30, 4000),))])
+def test_blocks_have_equal_shares(counts, lengths, groups):
+    plan = plan_shared(counts, lengths, 28, 4, 128, shared=groups, device="cpu", sms=148)
+    for items, block in parts_of(plan)[:2]:
+        if len(items):
+            keys = np.bincount(block, items[:, 4] - items[:, 3])
+            assert keys.max() <= 1.5 * keys.mean() + 256 and len(keys) * 4 <= 3 * 148
+
+
+def test_short_ranges_stay_whole():
+    plan = plan_shared([1, 1], [500, 190], 28, 4, 128, device="cpu", sms=148)
+    assert plan.strip_blocks == 2 and not plan.joined
 
 
 def test_refusals():
     good = dict(counts=[1, 1], lengths=[9, 9], heads=4, kv_heads=2, head_dim=64, device="cpu", sms=148)
     for bad in (dict(counts=[1]), dict(counts=[1, -1]), dict(lengths=[9, -2]), dict(heads=5), dict(kv_heads=0), dict(lengths=[2**31, 9]), dict(shared=[(0, 3, 4)]), dict(shared=[(0, 2, 4), (1, 1, 4)]),
-                dict(shared=[(1, 1, 4), (0, 1, 4)]), dict(shared=[(0, 2, 9)]), dict(shared=[(0, 1, -1)])):
+                dict(shared=[(1, 1, 4), (0, 1, 4)]), dict(shared=[(0, 2, 9)]), dict(shared=[(0, 1, -1)]), dict(shared=[(0, 1)])):
         with pytest.raises(KernelError):
             plan_shared(**{**good, **bad})
