@@ -7,11 +7,12 @@
 // running sum over the vocabulary is needed, and the answer does not hang on the order of one.  With temperature 0 a draft stands when it is
 // its row's largest logit (the lowest index of equal ones), and that token follows.
 //
-// Both kernels are bound by memory.  The first reads every row once, in pieces of CHUNK entries a block, and leaves each piece's maximum and
-// sum (or its argmax); a request's end is known only when all its rows' sums are.  The second takes, per request, the one row at which the
-// request ends, the drafter's and the noise: each of its blocks first works out the request's end from the pieces (a few kilobytes out of L2),
-// then looks through its chunk, and the block that comes last writes the request's answer.  A NaN counts as -infinity, +infinity as the
-// largest number; a row without any finite logit has p = 0 everywhere, and its token is the lowest index.
+// Both kernels are bound by memory.  The first reads every row once, a block a piece of it, and leaves each piece's maximum and sum (or its argmax); a request's end is
+// known only when all its rows' sums are.  The second takes, per request, the one row at which the request ends, the drafter's and the noise: each of its blocks first works
+// out the request's end from the pieces (a few kilobytes out of L2, with the noise on its way meanwhile), then looks through its part, and the block that comes last
+// writes the request's answer.  Pieces are as many as fill the device a few times over: a block's start (which request is this, what is its temperature; where does it
+// end) costs as much as some 20,000 entries.  A NaN counts as -infinity, +infinity as the largest number; a row without any finite logit has p = 0 everywhere, and its
+// token is the lowest index.
 #include <float.h>
 
 #include "common.cuh"
@@ -20,7 +21,8 @@ namespace {
 typedef __nv_bfloat16 bf16;
 typedef unsigned long long Key;  // (value's bits, ~index): the largest value, of equal ones the lowest index
 constexpr int THREADS = 256, STEPS = 4;
-constexpr int CHUNK = THREADS * STEPS * 4;
+constexpr int CHUNK = THREADS * STEPS * 4;  // entries a block holds at a time
+constexpr int KEPT = 64;                    // rows of a request whose sums a block keeps
 
 __device__ __forceinline__ float cleaned(float v) { return v != v ? -INFINITY : fminf(v, FLT_MAX); }
 __device__ __forceinline__ float rate_of(float temperature) { return fminf(1.4426950408889634f / temperature, FLT_MAX); }
@@ -75,8 +77,8 @@ struct Args {
     const float* uniform;
     const float* noise; long long noise_stride;
     const float* temperature;
-    int chunks;
-    float2* pieces;        // [rows, chunks]: (maximum, sum), or with temperature 0 (maximum, its index's bits)
+    int pieces_per_row, row_span, request_span;  // a block of the first kernel, and of the second, has so many entries of its row (a multiple of CHUNK)
+    float2* pieces;        // [rows, pieces_per_row]: (maximum, sum), or with temperature 0 (maximum, its index's bits)
     Key* best;             // [requests, 2]: of what is left beside the drafter's, and of the target's own
     int* arrived;          // [requests]
     int* accepted;         // [requests]
@@ -84,176 +86,233 @@ struct Args {
     int* status;
 };
 
-// The request that owns `row`: the last one whose rows start at or before it (requests without rows are passed over).
-__device__ __forceinline__ int request_of(const Args& a, int row) {
-    int low = 0, high = a.requests - 1;
-    while (low < high) {
-        const int middle = (low + high + 1) >> 1;
-        if (a.row_start[middle] <= row) low = middle; else high = middle - 1;
-    }
-    return low;
+template <typename T, bool WIDE>
+__device__ __forceinline__ void batch(const T* row, int first, int vocab, float fill, float (&v)[STEPS][4]) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) entries<T, WIDE>(row, first + s * THREADS * 4, vocab, fill, v[s]);
 }
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
     __shared__ Key keys[THREADS / 32];
-    __shared__ __align__(16) float scratch[32];
+    __shared__ float2 parts[THREADS / 32];
+    __shared__ int owner;
     let_next_kernel_start();
     wait_for_previous_kernels();
-    const int row = blockIdx.y, chunk = blockIdx.x;
-    if (row == 0 && chunk == 0)
+    const int row = blockIdx.y, piece = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (row == 0 && piece == 0)
         for (int r = threadIdx.x; r < a.requests; r += THREADS) a.best[2 * r] = a.best[2 * r + 1] = 0, a.arrived[r] = 0;
     const T* logits = (const T*)a.logits + (size_t)row * a.stride;
-    const int first = chunk * CHUNK + threadIdx.x * 4;
-    float v[STEPS][4];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) entries<T, WIDE>(logits, first + s * THREADS * 4, a.vocab, -INFINITY, v[s]);
-    const float temperature = a.temperature[request_of(a, row)];
-    float2* piece = a.pieces + (size_t)row * a.chunks + chunk;
+    const int end = min(a.vocab, (piece + 1) * a.row_span);
+    int first = piece * a.row_span + threadIdx.x * 4;
+    float v[STEPS][4], next[STEPS][4];
+    batch<T, WIDE>(logits, first, end, -INFINITY, v);
+    // The request that owns the row; a row that is no one's is treated as greedy, and never looked at.
+    if (threadIdx.x == 0) owner = -1;
+    __syncthreads();
+    for (int r = threadIdx.x; r < a.requests; r += THREADS)
+        if (a.row_start[r] <= row && row < a.row_start[r + 1]) owner = r;
+    __syncthreads();
+    const float temperature = owner < 0 ? 0.f : a.temperature[owner];
+    float2* out = a.pieces + (size_t)row * a.pieces_per_row + piece;
     if (!(temperature > 0.f)) {
         Key k = 0;
+        while (true) {
+            const bool more = first - threadIdx.x * 4 + CHUNK < end;
+            if (more) batch<T, WIDE>(logits, first + CHUNK, end, -INFINITY, next);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
+            for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int at = first + s * THREADS * 4 + e;
-                if (at >= a.vocab) continue;
-                const Key mine = key_of(cleaned(v[s][e]), at);
-                k = mine > k ? mine : k;
-            }
+                for (int e = 0; e < 4; ++e) {
+                    const int at = first + s * THREADS * 4 + e;
+                    if (at >= end) continue;
+                    const Key mine = key_of(cleaned(v[s][e]), at);
+                    k = mine > k ? mine : k;
+                }
+            if (!more) break;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[s][e] = next[s][e];
+            first += CHUNK;
+        }
         k = block_max_key(k, keys);
         if (threadIdx.x == 0) {
             const unsigned o = (unsigned)(k >> 32);
-            *piece = make_float2(__uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o), __int_as_float(index_of(k)));
+            *out = make_float2(__uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o), __int_as_float(index_of(k)));
         }
         return;
     }
     const float rate = rate_of(temperature);
-    float m = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[s][e] = cleaned(v[s][e]);
-            m = fmaxf(m, v[s][e]);
-        }
-    m = block_max(m, scratch);
-    float sum = 0.f;
-    if (m > -INFINITY) {
+    float m = -INFINITY, sum = 0.f;
+    while (true) {
+        const bool more = first - threadIdx.x * 4 + CHUNK < end;
+        if (more) batch<T, WIDE>(logits, first + CHUNK, end, -INFINITY, next);
+        float top = m;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += weight_of(v[s][e], m, rate);
+            for (int e = 0; e < 4; ++e) {
+                v[s][e] = cleaned(v[s][e]);
+                top = fmaxf(top, v[s][e]);
+            }
+        if (top > -INFINITY) {
+            sum *= m == -INFINITY ? 0.f : weight_of(m, top, rate);
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += weight_of(v[s][e], top, rate);
+            m = top;
+        }
+        if (!more) break;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[s][e] = next[s][e];
+        first += CHUNK;
     }
-    sum = block_sum(sum, scratch);
-    if (threadIdx.x == 0) *piece = make_float2(m, sum);
+    float top = warp_max(m);
+    sum = warp_sum(m == -INFINITY ? 0.f : sum * weight_of(m, top, rate));
+    if (lane == 0) parts[warp] = make_float2(top, sum);
+    __syncthreads();
+    if (warp == 0) {
+        const float2 part = lane < THREADS / 32 ? parts[lane] : make_float2(-INFINITY, 0.f);
+        top = warp_max(part.x);
+        sum = warp_sum(part.x == -INFINITY ? 0.f : part.y * weight_of(part.x, top, rate));
+        if (lane == 0) *out = make_float2(top, sum);
+    }
 }
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) verify_requests_kernel(const Args a) {
     __shared__ Key keys[THREADS / 32];
+    __shared__ float2 sums[KEPT];         // a row's maximum and sum; with temperature 0 the index of its largest logit in the latter's place
     __shared__ int refused_at;            // the first draft that does not stand, counted in the request's rows
-    __shared__ float end_max, end_total;  // of the row at which the request ends; with temperature 0 its largest logit's index
     __shared__ int last_block;
     let_next_kernel_start();
-    const int r = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     wait_for_previous_kernels();
+    const int end_at = min(a.vocab, ((int)blockIdx.x + 1) * a.request_span);
+    int first = blockIdx.x * a.request_span + threadIdx.x * 4;
+    const float* noise = a.noise + (size_t)r * a.noise_stride;
+    float n[STEPS][4];
+    batch<float, WIDE>(noise, first, end_at, 1.f, n);
     const int row0 = min(max(a.row_start[r], 0), a.rows), row1 = min(max(a.row_start[r + 1], row0), a.rows), drafted = row1 - row0 - 1;
+    const float temperature = a.temperature[r];
     if (drafted < 0) {  // a request without rows
-        if (chunk == 0) {
+        if (blockIdx.x == 0) {
             if (threadIdx.x == 0) a.accepted[r] = 0;
             for (int j = threadIdx.x; j < a.most; j += THREADS) a.tokens[(size_t)r * a.most + j] = -1;
         }
         return;
     }
-    const float temperature = a.temperature[r];
     const bool greedy = !(temperature > 0.f);
     const float rate = greedy ? 0.f : rate_of(temperature);
     if (threadIdx.x == 0) refused_at = drafted;
     __syncthreads();
     // A warp takes a row: its maximum and sum from its pieces, in the order of the lanes.
-    auto row_of_pieces = [&](int row, float& m, float& total) {
-        const float2* pieces = a.pieces + (size_t)row * a.chunks;
-        m = -INFINITY, total = 0.f;
+    auto row_of_pieces = [&](int row) {
+        const float2* pieces = a.pieces + (size_t)row * a.pieces_per_row;
         if (greedy) {
             Key k = 0;
-            for (int c = lane; c < a.chunks; c += 32) {
-                const Key mine = key_of(pieces[c].x, __float_as_int(pieces[c].y));
+            for (int c = lane; c < a.pieces_per_row; c += 32) {
+                const float2 piece = pieces[c];
+                const Key mine = key_of(piece.x, __float_as_int(piece.y));
                 k = mine > k ? mine : k;
             }
-            total = __int_as_float(index_of(warp_max_key(k)));
-            return;
+            return make_float2(0.f, __int_as_float(index_of(warp_max_key(k))));
         }
-        for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, pieces[c].x);
+        float m = -INFINITY, total = 0.f;
+        for (int c = lane; c < a.pieces_per_row; c += 32) m = fmaxf(m, pieces[c].x);
         m = warp_max(m);
         if (m > -INFINITY)
-            for (int c = lane; c < a.chunks; c += 32) total = fmaf(weight_of(pieces[c].x, m, rate), pieces[c].y, total);
-        total = warp_sum(total);
+            for (int c = lane; c < a.pieces_per_row; c += 32) total = fmaf(weight_of(pieces[c].x, m, rate), pieces[c].y, total);
+        return make_float2(m, warp_sum(total));
     };
-    for (int j = warp; j < drafted; j += THREADS / 32) {
-        const int row = row0 + j, draft = a.drafts[row];
-        float m, total;
-        row_of_pieces(row, m, total);
+    for (int j = warp; j <= drafted; j += THREADS / 32) {
+        const int row = row0 + j, draft = j < drafted ? a.drafts[row] : 0;
+        const bool known = draft >= 0 && draft < a.vocab;
+        float logit = 0.f, q = 1.f, u = 0.f;
+        if (lane == 0 && j < drafted && known && !greedy) {
+            logit = to_float(((const T*)a.logits)[(size_t)row * a.stride + draft]);
+            if (a.probabilities) q = a.probabilities[(size_t)row * a.q_stride + draft];
+            u = a.uniform[row];
+        }
+        const float2 sum = row_of_pieces(row);
         if (lane == 0) {
-            bool stands = false;
-            if (draft < 0 || draft >= a.vocab) {
-                atomicOr(a.status, HB_STATUS_BAD_TOKEN);
-            } else if (greedy) {
-                stands = draft == __float_as_int(total);
-            } else {
-                const float p = total > 0.f ? weight_of(cleaned(to_float(((const T*)a.logits)[(size_t)row * a.stride + draft])), m, rate) / total : 0.f;
-                const float q = a.probabilities ? a.probabilities[(size_t)row * a.q_stride + draft] : 1.f;
-                stands = a.uniform[row] * q < p;
+            if (j < KEPT) sums[j] = sum;
+            if (j < drafted) {
+                bool stands;
+                if (!known) {
+                    atomicOr(a.status, HB_STATUS_BAD_TOKEN);
+                    stands = false;
+                } else if (greedy) {
+                    stands = draft == __float_as_int(sum.y);
+                } else {
+                    const float p = sum.y > 0.f ? weight_of(cleaned(logit), sum.x, rate) / sum.y : 0.f;
+                    stands = u * q < p;
+                }
+                if (!stands) atomicMin(&refused_at, j);
             }
-            if (!stands) atomicMin(&refused_at, j);
         }
     }
     __syncthreads();
     const int accepted = refused_at, end = row0 + accepted;
-    if (warp == 0) {
-        float m, total;
-        row_of_pieces(end, m, total);
-        if (lane == 0) end_max = m, end_total = total;
+    if (accepted >= KEPT) {
+        if (warp == 0) {
+            const float2 sum = row_of_pieces(end);
+            if (lane == 0) sums[0] = sum;
+        }
+        __syncthreads();
     }
-    __syncthreads();
+    const float2 sum = sums[accepted < KEPT ? accepted : 0];
     auto write_answer = [&](int token) {  // the whole block
         if (threadIdx.x == 0) a.accepted[r] = accepted;
         for (int j = threadIdx.x; j < a.most; j += THREADS) a.tokens[(size_t)r * a.most + j] = j < accepted ? a.drafts[row0 + j] : (j == accepted ? token : -1);
     };
     if (greedy) {
-        if (chunk == 0) write_answer(__float_as_int(end_total));
+        if (blockIdx.x == 0) write_answer(__float_as_int(sum.y));
         return;
     }
     const bool refused = accepted < drafted;
     const int banned = refused && !a.probabilities ? a.drafts[end] : -1;  // a draft that stood for itself takes all of its place
     const bool beside = refused && a.probabilities;
     const T* logits = (const T*)a.logits + (size_t)end * a.stride;
-    const float* q = a.probabilities + (size_t)end * a.q_stride;
-    const float* noise = a.noise + (size_t)r * a.noise_stride;
-    const float m = end_max, share = end_total > 0.f ? 1.f / end_total : 0.f;
-    const int first = chunk * CHUNK + threadIdx.x * 4;
-    float v[STEPS][4], n[STEPS][4], d[STEPS][4];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        const int at = first + s * THREADS * 4;
-        entries<T, WIDE>(logits, at, a.vocab, -INFINITY, v[s]);
-        entries<float, WIDE>(noise, at, a.vocab, 1.f, n[s]);
-        if (beside) entries<float, WIDE>(q, at, a.vocab, 0.f, d[s]);
-        else d[s][0] = d[s][1] = d[s][2] = d[s][3] = 0.f;
-    }
+    const float* probabilities = a.probabilities + (size_t)end * a.q_stride;
+    const float m = sum.x, share = sum.y > 0.f ? 1.f / sum.y : 0.f;
     Key rest = 0, left = 0;
+    float v[STEPS][4], d[STEPS][4];
+    while (true) {
+        batch<T, WIDE>(logits, first, end_at, -INFINITY, v);
+        if (beside) {
+            batch<float, WIDE>(probabilities, first, end_at, 0.f, d);
+        } else {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = first + s * THREADS * 4 + e;
-            if (at >= a.vocab) continue;
-            const float p = share > 0.f ? weight_of(cleaned(v[s][e]), m, rate) * share : 0.f, clock = 1.f / fmaxf(n[s][e], FLT_MIN);
-            const Key own = key_of(p * clock, at);
-            left = own > left ? own : left;
-            const Key more = key_of(at == banned ? 0.f : fmaxf(p - d[s][e], 0.f) * clock, at);
-            rest = more > rest ? more : rest;
+            for (int s = 0; s < STEPS; ++s) d[s][0] = d[s][1] = d[s][2] = d[s][3] = 0.f;
         }
+        // the largest of this thread's, compared as floats (ties keep the lower index, which comes first); only the winner becomes a key
+        float best_rest = -1.f, best_left = -1.f;
+        int at_rest = 0, at_left = 0;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = first + s * THREADS * 4 + e;
+                if (at >= end_at) continue;
+                const float p = share > 0.f ? weight_of(cleaned(v[s][e]), m, rate) * share : 0.f, clock = 1.f / fmaxf(n[s][e], FLT_MIN);
+                const float own = p * clock, more = at == banned ? 0.f : fmaxf(p - d[s][e], 0.f) * clock;
+                if (own > best_left) best_left = own, at_left = at;
+                if (more > best_rest) best_rest = more, at_rest = at;
+            }
+        if (best_left >= 0.f) {
+            const Key a_left = key_of(best_left, at_left), a_rest = key_of(best_rest, at_rest);
+            left = a_left > left ? a_left : left;
+            rest = a_rest > rest ? a_rest : rest;
+        }
+        if (first - threadIdx.x * 4 + CHUNK >= end_at) break;
+        first += CHUNK;
+        batch<float, WIDE>(noise, first, end_at, 1.f, n);
+    }
     rest = block_max_key(rest, keys);
     left = block_max_key(left, keys);
     if (threadIdx.x == 0) {
@@ -277,22 +336,29 @@ HB_EXPORT int hb_verify_drafts(const void* logits, int is_bf16, long long stride
                                const float* probabilities, long long q_stride, const float* uniform, const float* noise, long long noise_stride,
                                const float* temperature, void* workspace, int* accepted, int* tokens, int most, int* status, cudaStream_t stream) {
     if (requests <= 0) return 0;
-    if (rows < 0 || vocab <= 0 || most <= 0 || !row_start || !temperature || !workspace || !accepted || !tokens || !status || ((uintptr_t)workspace & 7)) return HB_BAD_ARGUMENT;
-    if (rows > 0 && (!logits || !drafts || !uniform || !noise)) return HB_BAD_ARGUMENT;
-    const int chunks = (int)(((long long)vocab + CHUNK - 1) / CHUNK);
+    if (rows < 0 || vocab <= 0 || most <= 0 || !row_start || !noise || !temperature || !workspace || !accepted || !tokens || !status || ((uintptr_t)workspace & 7)) return HB_BAD_ARGUMENT;
+    if (rows > 0 && (!logits || !drafts || !uniform)) return HB_BAD_ARGUMENT;
     if (rows > 65535 || requests > 65535 || vocab > 0x7fffffff - 2 * CHUNK) return HB_UNSUPPORTED_SIZE;
+    // As many blocks a row as fill the device eight times over between all rows, four times between all requests (whose blocks hold more), one for each CHUNK at most.
+    const int chunks = (vocab + CHUNK - 1) / CHUNK;
+    const auto span = [&](int lines, int times) {
+        const int wanted = (148 * times + lines - 1) / (lines > 0 ? lines : 1), blocks = wanted < 1 ? 1 : (wanted < chunks ? wanted : chunks);
+        return (chunks + blocks - 1) / blocks * CHUNK;
+    };
+    const int row_span = span(rows, 8), request_span = span(requests, 4);
+    const int row_blocks = (vocab + row_span - 1) / row_span, request_blocks = (vocab + request_span - 1) / request_span;
     float2* pieces = (float2*)workspace;
     Key* best = (Key*)(pieces + (size_t)rows * chunks);
-    const Args a{logits, stride, row_start, requests, rows, vocab, drafts, probabilities, q_stride, uniform, noise, noise_stride, temperature, chunks, pieces, best,
-                 (int*)(best + 2 * (size_t)requests), accepted, tokens, most, status};
+    const Args a{logits, stride, row_start, requests, rows, vocab, drafts, probabilities, q_stride, uniform, noise, noise_stride, temperature, row_blocks, row_span, request_span,
+                 pieces, best, (int*)(best + 2 * (size_t)requests), accepted, tokens, most, status};
     const int element = is_bf16 ? 2 : 4;
     const bool wide = !(((uintptr_t)logits | (uintptr_t)(stride * element)) & (4 * element - 1)) && !(((uintptr_t)noise | (uintptr_t)(noise_stride * 4)) & 15) &&
                       !(((uintptr_t)probabilities | (uintptr_t)(probabilities ? q_stride * 4 : 0)) & 15);
 #define HB_VERIFY(T, W)                                                                                                                     \
     do {                                                                                                                                    \
         if (rows > 0)                                                                                                                       \
-            if (int code = launch_after_previous(verify_rows_kernel<T, W>, dim3(chunks, rows), dim3(THREADS), 0, stream, a)) return code;   \
-        return launch_after_previous(verify_requests_kernel<T, W>, dim3(chunks, requests), dim3(THREADS), 0, stream, a);                    \
+            if (int code = launch_after_previous(verify_rows_kernel<T, W>, dim3(row_blocks, rows), dim3(THREADS), 0, stream, a)) return code;   \
+        return launch_after_previous(verify_requests_kernel<T, W>, dim3(request_blocks, requests), dim3(THREADS), 0, stream, a);                    \
     } while (0)
     if (is_bf16) {
         if (wide) HB_VERIFY(bf16, true);

@@ -10,7 +10,7 @@ from typing import NamedTuple
 import torch
 
 from .basic import status_word
-from .native import KernelError, check, is_bf16, library, ptr, require_cuda, stream_ptr
+from .native import KernelError, check, entry, is_bf16, require_cuda, stream_address
 
 
 class Cache8(NamedTuple):
@@ -34,35 +34,38 @@ def new_cache8(pages: int, kv_heads: int, page_size: int, head_dim: int, device=
 def check_cache8(cache: Cache8, what: str) -> tuple[int, int, int, int]:
     """(pages, kv_heads, page_size, head_dim) of a cache that is laid out as the kernels read it."""
     codes, exponents = cache
-    require_cuda(codes, exponents)
     shape = codes.shape
-    if (codes.dtype != torch.float8_e4m3fn or exponents.dtype != torch.int8 or len(shape) != 5 or shape[1] != 2 or exponents.shape != shape[:4]
+    if (codes.dtype is not torch.float8_e4m3fn or exponents.dtype is not torch.int8 or len(shape) != 5 or shape[1] != 2 or exponents.shape != shape[:4]
             or not codes.is_contiguous() or not exponents.is_contiguous()):
         raise KernelError(f"{what}: an 8-bit cache is dense codes [pages, 2, kv_heads, page, d] in float8_e4m3fn and exponents [pages, 2, kv_heads, page] in int8")
+    if not (codes.is_cuda and exponents.is_cuda):
+        require_cuda(codes, exponents)
     return shape[0], shape[2], shape[3], shape[4]
 
 
-def _check_places(block_table, token_row, positions, what: str) -> int:
-    require_cuda(block_table, token_row, positions)
-    tokens = positions.numel()
-    if (block_table.dtype != torch.int32 or token_row.dtype != torch.int32 or positions.dtype != torch.int32 or block_table.dim() != 2 or token_row.numel() != tokens
-            or not block_table.is_contiguous() or not token_row.is_contiguous() or not positions.is_contiguous()):
+def _check_places(block_table, token_row, positions, what: str) -> tuple[int, int]:
+    tokens, width = positions.numel(), block_table.shape[-1]
+    if (block_table.dtype is not torch.int32 or token_row.dtype is not torch.int32 or positions.dtype is not torch.int32 or block_table.dim() != 2 or token_row.numel() != tokens
+            or not (block_table.is_contiguous() and token_row.is_contiguous() and positions.is_contiguous())):
         raise KernelError(f"{what}: a dense int32 block table [rows, blocks], and a row and a position (dense int32) for each token")
-    return tokens
+    if not (block_table.is_cuda and token_row.is_cuda and positions.is_cuda):
+        require_cuda(block_table, token_row, positions)
+    return tokens, width
 
 
 def cache8_store(src: torch.Tensor, k_offset: int, v_offset: int, cache: Cache8, block_table: torch.Tensor, token_row: torch.Tensor, positions: torch.Tensor) -> None:
     """Quantise each token's keys and values (columns of ``src`` [tokens, width], bfloat16 or float32) and write them to their pages, as
     :func:`.basic.kv_store` writes them as they are.  A token without a page is left out and reported (``raise_on_status``)."""
     pages, kv_heads, page_size, head_dim = check_cache8(cache, "cache8_store")
-    tokens = _check_places(block_table, token_row, positions, "cache8_store")
-    require_cuda(src)
-    width = kv_heads * head_dim
-    if src.dim() != 2 or src.shape[0] != tokens or src.stride(1) != 1 or min(k_offset, v_offset) < 0 or max(k_offset, v_offset) + width > src.shape[1]:
+    tokens, table_width = _check_places(block_table, token_row, positions, "cache8_store")
+    width, shape = kv_heads * head_dim, src.shape
+    if len(shape) != 2 or shape[0] != tokens or src.stride(1) != 1 or min(k_offset, v_offset) < 0 or max(k_offset, v_offset) + width > shape[1]:
         raise KernelError(f"cache8_store: a source [tokens, width] with unit inner stride that holds {width} columns of keys and of values at their offsets")
-    check(library("cache8").hb_cache8_store(ptr(src), is_bf16(src), src.stride(0), k_offset, v_offset, ptr(cache.codes), ptr(cache.exponents), ptr(block_table),
-                                            block_table.shape[1], ptr(token_row), ptr(positions), tokens, kv_heads, head_dim, page_size, pages,
-                                            ptr(status_word(src.device)), stream_ptr()), "cache8_store")
+    if not src.is_cuda:
+        require_cuda(src)
+    check(entry("cache8", "hb_cache8_store", "piiiipppippiiiiipp")(
+        src.data_ptr(), is_bf16(src), src.stride(0), k_offset, v_offset, cache[0].data_ptr(), cache[1].data_ptr(), block_table.data_ptr(), table_width, token_row.data_ptr(),
+        positions.data_ptr(), tokens, kv_heads, head_dim, page_size, pages, status_word(src.device).data_ptr(), stream_address()), "cache8_store")
 
 
 def cache8_load(cache: Cache8, block_table: torch.Tensor, token_row: torch.Tensor, positions: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -70,11 +73,12 @@ def cache8_load(cache: Cache8, block_table: torch.Tensor, token_row: torch.Tenso
     """The keys and values of ``positions`` (of the table rows ``token_row``) as [tokens, 2, kv_heads, d] in ``dtype`` (bfloat16 holds them exactly).
     A token without a page reads as zeros and is reported (``raise_on_status``)."""
     pages, kv_heads, page_size, head_dim = check_cache8(cache, "cache8_load")
-    tokens = _check_places(block_table, token_row, positions, "cache8_load")
+    tokens, table_width = _check_places(block_table, token_row, positions, "cache8_load")
     if out is None:
-        out = torch.empty((tokens, 2, kv_heads, head_dim), dtype=dtype, device=cache.codes.device)
+        out = torch.empty((tokens, 2, kv_heads, head_dim), dtype=dtype, device=cache[0].device)
     elif out.shape != (tokens, 2, kv_heads, head_dim) or out.dtype != dtype or not out.is_contiguous() or not out.is_cuda:
         raise KernelError(f"cache8_load: the output is a dense {dtype} tensor [tokens, 2, kv_heads, d]")
-    check(library("cache8").hb_cache8_load(ptr(cache.codes), ptr(cache.exponents), ptr(block_table), block_table.shape[1], ptr(token_row), ptr(positions), ptr(out),
-                                           is_bf16(out), tokens, kv_heads, head_dim, page_size, pages, ptr(status_word(out.device)), stream_ptr()), "cache8_load")
+    check(entry("cache8", "hb_cache8_load", "pppipppiiiiiipp")(
+        cache[0].data_ptr(), cache[1].data_ptr(), block_table.data_ptr(), table_width, token_row.data_ptr(), positions.data_ptr(), out.data_ptr(), is_bf16(out), tokens, kv_heads,
+        head_dim, page_size, pages, status_word(out.device).data_ptr(), stream_address()), "cache8_load")
     return out

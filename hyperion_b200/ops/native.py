@@ -27,11 +27,6 @@ def ptr(tensor: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(tensor.data_ptr())
 
 
-def address(value: int) -> ctypes.c_void_p:
-    """A device address that is no tensor's own start."""
-    return ctypes.c_void_p(value)
-
-
 _bound_stream: list = [None]  # the stream a step has bound for its launches, or None
 
 
@@ -102,6 +97,27 @@ def library(module: str, **defines: Any) -> ctypes.CDLL:
     if found is None:
         found = _libraries[key] = build.load(module, defines)
     return found
+
+
+_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+_entries: dict = {}
+
+
+def entry(module: str, name: str, arguments: str, head_dim: int = 0):
+    """An exported launcher with its arguments' kinds (p: address, i: int, l: long long, f: float), looked up once: plain Python numbers then go to it as they are,
+    which costs a call of twenty arguments a few microseconds less than a ctypes object for each."""
+    found = _entries.get((name, head_dim))
+    if found is None:
+        found = getattr(library(module, HB_HEAD_DIM=head_dim) if head_dim else library(module), name)
+        found.argtypes = [_KINDS[kind] for kind in arguments]
+        _entries[name, head_dim] = found
+    return found
+
+
+def stream_address() -> int:
+    """:func:`stream_ptr` as a number, without the objects on the way there."""
+    bound = _bound_stream[0]
+    return (bound.value or 0) if bound is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 i32 = int  # a Python int is passed as a C int by ctypes itself; the name marks which arguments are 32-bit

@@ -14,10 +14,9 @@ import numpy as np
 import torch
 
 from .. import host as host_runtime
-from . import native
 from .basic import status_word
 from .cache8 import Cache8, check_cache8
-from .native import KernelError, check, f32, library, ptr, require_cuda, sm_count, stream_ptr
+from .native import KernelError, check, entry, require_cuda, sm_count, stream_address
 
 
 def supported(head_dim: int, page_size: int) -> bool:
@@ -51,7 +50,7 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     plan.strip_blocks, plan.strip_rows, plan.tile_blocks, plan.tokens, plan.pieces, plan.joined, plan.longest = sizes[1:8].tolist()
     plan.data = words.to(device)
     plan.places = sizes[8:].tolist()  # strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces
-    plan.at = [native.address(plan.data.data_ptr() + 4 * place) for place in plan.places]
+    plan.at = [plan.data.data_ptr() + 4 * place for place in plan.places]
     return plan
 
 
@@ -63,46 +62,48 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     their values have to be finite."""
     if isinstance(cache, Cache8):
         pages, kv_heads, page_size, head_dim = check_cache8(cache, "attention_shared")
-        entries, exponents = cache
+        entries, exponents = cache[0].data_ptr(), cache[1].data_ptr()
     else:
-        require_cuda(cache)
-        entries, exponents = cache, None
-        if cache.dtype != torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
+        if cache.dtype is not torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
             raise KernelError("attention_shared: a dense bfloat16 cache [pages, 2, kv_heads, page, d], or a Cache8")
+        require_cuda(cache)
         pages, _, kv_heads, page_size, head_dim = cache.shape
-    require_cuda(q, block_table, out)
+        entries, exponents = cache.data_ptr(), 0
     if not supported(head_dim, page_size):
         raise KernelError(f"attention_shared: heads of 64 or 128 entries and pages of 8, 16, 32 or 64 positions, not {head_dim} and {page_size}")
     if heads != plan.heads or kv_heads != plan.kv_heads or head_dim != plan.head_dim:
         raise KernelError(f"attention_shared: planned for {plan.heads} heads over {plan.kv_heads} of {plan.head_dim} entries, called with {heads} over {kv_heads} of {head_dim}")
-    width = heads * head_dim
-    if q.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[0] != plan.tokens or q.shape[1] < width or q.stride(1) != 1:
-        raise KernelError(f"attention_shared: bfloat16 queries [{plan.tokens}, {width}] with unit inner stride")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < plan.requests or not block_table.is_contiguous():
+    tokens, width, shape = plan.tokens, heads * head_dim, q.shape
+    if q.dtype is not torch.bfloat16 or len(shape) != 2 or shape[0] != tokens or shape[1] < width or q.stride(1) != 1:
+        raise KernelError(f"attention_shared: bfloat16 queries [{tokens}, {width}] with unit inner stride")
+    shape = block_table.shape
+    if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] < plan.requests or not block_table.is_contiguous():
         raise KernelError(f"attention_shared: a dense int32 block table of at least {plan.requests} rows")
-    if block_table.shape[1] * page_size < plan.longest:
-        raise KernelError(f"attention_shared: a block table of {block_table.shape[1]} pages of {page_size} does not hold {plan.longest} positions")
+    if shape[1] * page_size < plan.longest:
+        raise KernelError(f"attention_shared: a block table of {shape[1]} pages of {page_size} does not hold {plan.longest} positions")
+    if not (q.is_cuda and block_table.is_cuda):
+        require_cuda(q, block_table)
     if out is None:
-        out = torch.empty((plan.tokens, width), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[0] != plan.tokens or out.shape[1] < width or out.stride(1) != 1:
-        raise KernelError(f"attention_shared: the output is a bfloat16 [{plan.tokens}, >= {width}] view")
-    if plan.tokens == 0:
+        out = torch.empty((tokens, width), dtype=torch.bfloat16, device=q.device)
+    elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != tokens or out.shape[1] < width or out.stride(1) != 1 or not out.is_cuda:
+        raise KernelError(f"attention_shared: the output is a bfloat16 [{tokens}, >= {width}] view")
+    if tokens == 0:
         return out
-    stream, status = stream_ptr(), ptr(status_word(q.device))
     strip_items, strip_first, tile_items, tile_first, last, starts, own = plan.at
-    pieces = sums = native.address(0)
+    pieces = sums = 0
     if plan.joined:
         workspace = torch.empty(max(1, plan.pieces * heads * (head_dim + 2)), dtype=torch.float32, device=q.device)
-        pieces = native.address(workspace.data_ptr())
-        sums = native.address(workspace.data_ptr() + 4 * plan.pieces * heads * head_dim)
-    where = (ptr(entries), ptr(exponents), ptr(block_table), block_table.shape[1])
-    what = (last, starts, own, pieces, sums, heads, kv_heads, page_size, pages, f32(scale), status, stream)
+        pieces = workspace.data_ptr()
+        sums = pieces + 4 * plan.pieces * heads * head_dim
+    out_at, out_stride, stream = out.data_ptr(), out.stride(0), stream_address()
+    where = (entries, exponents, block_table.data_ptr(), shape[1])
+    what = (last, starts, own, pieces, sums, heads, kv_heads, page_size, pages, scale, status_word(q.device).data_ptr(), stream)
     if plan.tile_blocks:
-        check(library("attention_shared_tiles", HB_HEAD_DIM=head_dim).hb_attention_shared_tiles(
-            ptr(q), q.stride(0), plan.tokens, ptr(out), out.stride(0), *where, tile_items, tile_first, plan.tile_blocks, *what), "attention_shared")
+        check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipppppiiiifpp", head_dim)(
+            q.data_ptr(), q.stride(0), tokens, out_at, out_stride, *where, tile_items, tile_first, plan.tile_blocks, *what), "attention_shared")
     if plan.strip_blocks:
-        check(library("attention_shared", HB_HEAD_DIM=head_dim).hb_attention_strips(
-            ptr(q), q.stride(0), ptr(out), out.stride(0), *where, strip_items, strip_first, plan.strip_blocks, plan.strip_rows, *what), "attention_shared")
+        check(entry("attention_shared", "hb_attention_strips", "pipipppippiipppppiiiifpp", head_dim)(
+            q.data_ptr(), q.stride(0), out_at, out_stride, *where, strip_items, strip_first, plan.strip_blocks, plan.strip_rows, *what), "attention_shared")
     if plan.joined:
-        check(library("attention_shared", HB_HEAD_DIM=head_dim).hb_attention_pieces(pieces, sums, starts, ptr(out), out.stride(0), plan.tokens, heads, stream), "attention_shared")
+        check(entry("attention_shared", "hb_attention_pieces", "ppppiiip", head_dim)(pieces, sums, starts, out_at, out_stride, tokens, heads, stream), "attention_shared")
     return out

@@ -8,21 +8,16 @@ and when all stand one more token is drawn from p_n, so that the tokens are dist
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
 
 from ..ops.basic import status_word
-from ..ops.native import KernelError, check, is_bf16, library, ptr, require_cuda, stream_ptr
+from ..ops.native import KernelError, check, entry, is_bf16, require_cuda, stream_address
 
 
 CHUNK = 4096  # entries of the vocabulary a block looks through (csrc/verify.cu)
-
-
-def _stride(matrix: Optional[torch.Tensor]) -> ctypes.c_longlong:
-    return ctypes.c_longlong(matrix.stride(0) if matrix is not None else 0)
 
 
 def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.Tensor, uniform: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor, *,
@@ -35,29 +30,33 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     last one is not read); ``probabilities`` [rows, vocab] float32: the drafter's at that row, or None where it gave none (its token then counts
     with probability 1); ``uniform`` [rows] float32 in [0, 1); ``noise`` [requests, vocab] float32, exponentially distributed, above 0;
     ``temperature`` [requests] float32, 0 for greedy.  A draft outside the vocabulary does not stand and is reported (``raise_on_status``)."""
-    require_cuda(logits, row_start, drafts, uniform, noise, temperature, probabilities)
-    if logits.dim() != 2 or row_start.dim() != 1 or row_start.shape[0] < 1:
+    shape, starts = logits.shape, row_start.shape
+    if len(shape) != 2 or len(starts) != 1 or starts[0] < 1:
         raise KernelError("verify_drafts: logits [rows, vocab] and row_start [requests + 1]")
-    rows, vocab = logits.shape
-    requests = row_start.shape[0] - 1
-    if logits.stride(1) != 1 or noise.shape != (requests, vocab) or noise.dtype != torch.float32 or noise.stride(1) != 1:
+    rows, vocab = shape
+    requests = starts[0] - 1
+    if logits.stride(1) != 1 or noise.shape != (requests, vocab) or noise.dtype is not torch.float32 or noise.stride(1) != 1:
         raise KernelError("verify_drafts: logits [rows, vocab] and float32 noise [requests, vocab], both with unit inner stride")
-    if probabilities is not None and (probabilities.shape != (rows, vocab) or probabilities.dtype != torch.float32 or probabilities.stride(1) != 1):
+    if probabilities is not None and (probabilities.shape != shape or probabilities.dtype is not torch.float32 or probabilities.stride(1) != 1):
         raise KernelError("verify_drafts: the drafter's probabilities are float32 [rows, vocab] with unit inner stride")
     for name, t, dtype, count in (("row_start", row_start, torch.int32, requests + 1), ("drafts", drafts, torch.int32, rows), ("uniform", uniform, torch.float32, rows),
                                   ("temperature", temperature, torch.float32, requests)):
-        if t.dtype != dtype or t.shape != (count,) or not t.is_contiguous():
+        if t.dtype is not dtype or t.shape != (count,) or not t.is_contiguous():
             raise KernelError(f"verify_drafts: {name} is a dense {dtype} vector of {count}")
     if most < 1:
         raise KernelError("verify_drafts: most counts a request's drafts and the token that follows them")
-    lib = library("verify")
-    answer = torch.empty((requests, 1 + most), dtype=torch.int32, device=logits.device).view(-1)
-    accepted, tokens = answer[:requests], answer[requests:].view(requests, most)
-    workspace = torch.empty(rows * -(-vocab // CHUNK) + 3 * requests, dtype=torch.int64, device=logits.device)
-    check(lib.hb_verify_drafts(ptr(logits), is_bf16(logits), _stride(logits), ptr(row_start), requests, rows, vocab, ptr(drafts), ptr(probabilities),
-                               _stride(probabilities), ptr(uniform), ptr(noise), _stride(noise), ptr(temperature), ptr(workspace), ptr(accepted), ptr(tokens), most,
-                               ptr(status_word(logits.device)), stream_ptr()), "verify_drafts")
-    return accepted, tokens
+    require_cuda(logits, row_start, drafts, uniform, noise, temperature, probabilities)
+    device = logits.device
+    # the answer (accepted, then tokens) and the kernels' workspace (pieces and keys of 8 bytes, counters) are one allocation
+    words = rows * -(-vocab // CHUNK) + 3 * requests
+    memory = torch.empty(2 * words + requests * (1 + most), dtype=torch.int32, device=device)
+    answer = memory.data_ptr() + 8 * words
+    check(entry("verify", "hb_verify_drafts", "pilpiiipplpplppppipp")(
+        logits.data_ptr(), is_bf16(logits), logits.stride(0), row_start.data_ptr(), requests, rows, vocab, drafts.data_ptr(),
+        probabilities.data_ptr() if probabilities is not None else 0, probabilities.stride(0) if probabilities is not None else 0, uniform.data_ptr(), noise.data_ptr(),
+        noise.stride(0), temperature.data_ptr(), memory.data_ptr(), answer, answer + 4 * requests, most, status_word(device).data_ptr(), stream_address()), "verify_drafts")
+    accepted, tokens = memory[2 * words:].split((requests, requests * most))
+    return accepted, tokens.view(requests, most)
 
 
 def reference_verify(logits: np.ndarray, drafts: Sequence[int], uniform: Sequence[float], noise: np.ndarray, temperature: float,
