@@ -22,15 +22,27 @@ typedef __nv_bfloat16 bf16;
 typedef unsigned long long Key;  // (value's bits, ~index): the largest value, of equal ones the lowest index
 constexpr int THREADS = 256, STEPS = 4;
 constexpr int CHUNK = THREADS * STEPS * 4;  // entries a block holds at a time
+constexpr int ROWS_PER_SM = 5, REQUESTS_PER_SM = 3;  // blocks, by registers
 constexpr int KEPT = 64;                    // rows of a request whose sums a block keeps
 
 __device__ __forceinline__ float cleaned(float v) { return v != v ? -INFINITY : fminf(v, FLT_MAX); }
 __device__ __forceinline__ float rate_of(float temperature) { return fminf(1.4426950408889634f / temperature, FLT_MAX); }
-// exp((v - m) / temperature): the difference first, which is exact where it matters
-__device__ __forceinline__ float weight_of(float v, float m, float rate) {
+__device__ __forceinline__ float fast_exp2(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((v - m) * rate));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// exp((v - m) / temperature)
+__device__ __forceinline__ float weight_of(float v, float m, float rate) { return fast_exp2((v - m) * rate); }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over a NaN, as fmaxf does
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 // Order-preserving for all floats but NaN.
 __device__ __forceinline__ unsigned ordered(float v) {
@@ -58,14 +70,42 @@ __device__ __forceinline__ Key block_max_key(Key k, Key* scratch) {  // the resu
     return k;
 }
 
-// Four entries of a row from `at` on, `fill` beyond its end.
+// Four entries of a row as they stand in memory: nothing waits for them before they are used.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+    float4 raw;
+    __device__ __forceinline__ float operator[](int e) const { return e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w; }
+    __device__ __forceinline__ void set(int e, float v) { (e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w) = v; }
+};
+template <>
+struct Four<bf16> {
+    uint2 raw;
+    __device__ __forceinline__ float operator[](int e) const {
+        const unsigned w = e < 2 ? raw.x : raw.y;
+        return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    }
+    __device__ __forceinline__ void set(int e, bf16 v) {
+        unsigned& w = e < 2 ? raw.x : raw.y;
+        w = e & 1 ? (w & 0xffffu) | (unsigned)__bfloat16_as_ushort(v) << 16 : (w & 0xffff0000u) | __bfloat16_as_ushort(v);
+    }
+};
+// A thread's part of CHUNK entries of a row, its first at `first`; what lies at `end` and beyond is not read, and is not to be looked at.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void entries(const T* row, int at, int vocab, float fill, float (&v)[4]) {
-    if (WIDE && at + 4 <= vocab) {
-        load4(row + at, v);
+__device__ __forceinline__ void batch(const T* row, int first, int end, Four<T> (&v)[STEPS]) {
+    if (WIDE && first - (int)threadIdx.x * 4 + CHUNK <= end) {  // for the whole block
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) v[s].raw = *reinterpret_cast<const decltype(v[s].raw)*>(row + first + s * THREADS * 4);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = at + e < vocab ? to_float(row[at + e]) : fill;
+        for (int s = 0; s < STEPS; ++s) {
+            const int at = first + s * THREADS * 4;
+            v[s] = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at + e < end) v[s].set(e, row[at + e]);
+        }
     }
 }
 
@@ -79,7 +119,7 @@ struct Args {
     const float* temperature;
     int pieces_per_row, row_span, request_span;  // a block of the first kernel, and of the second, has so many entries of its row (a multiple of CHUNK)
     float2* pieces;        // [rows, pieces_per_row]: (maximum, sum), or with temperature 0 (maximum, its index's bits)
-    Key* best;             // [requests, 2]: of what is left beside the drafter's, and of the target's own
+    Key* best;             // [requests]
     int* arrived;          // [requests]
     int* accepted;         // [requests]
     int* tokens; int most; // [requests, most]
@@ -87,13 +127,7 @@ struct Args {
 };
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ void batch(const T* row, int first, int vocab, float fill, float (&v)[STEPS][4]) {
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) entries<T, WIDE>(row, first + s * THREADS * 4, vocab, fill, v[s]);
-}
-
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, ROWS_PER_SM) verify_rows_kernel(const Args a) {
     __shared__ Key keys[THREADS / 32];
     __shared__ float2 parts[THREADS / 32];
     __shared__ int owner;
@@ -101,12 +135,12 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
     wait_for_previous_kernels();
     const int row = blockIdx.y, piece = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (row == 0 && piece == 0)
-        for (int r = threadIdx.x; r < a.requests; r += THREADS) a.best[2 * r] = a.best[2 * r + 1] = 0, a.arrived[r] = 0;
+        for (int r = threadIdx.x; r < a.requests; r += THREADS) a.best[r] = 0, a.arrived[r] = 0;
     const T* logits = (const T*)a.logits + (size_t)row * a.stride;
     const int end = min(a.vocab, (piece + 1) * a.row_span);
     int first = piece * a.row_span + threadIdx.x * 4;
-    float v[STEPS][4], next[STEPS][4];
-    batch<T, WIDE>(logits, first, end, -INFINITY, v);
+    Four<T> v[STEPS], next[STEPS];
+    batch<T, WIDE>(logits, first, end, v);
     // The request that owns the row; a row that is no one's is treated as greedy, and never looked at.
     if (threadIdx.x == 0) owner = -1;
     __syncthreads();
@@ -119,7 +153,7 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
         Key k = 0;
         while (true) {
             const bool more = first - threadIdx.x * 4 + CHUNK < end;
-            if (more) batch<T, WIDE>(logits, first + CHUNK, end, -INFINITY, next);
+            if (more) batch<T, WIDE>(logits, first + CHUNK, end, next);
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
@@ -131,9 +165,7 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
                 }
             if (!more) break;
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[s][e] = next[s][e];
+            for (int s = 0; s < STEPS; ++s) v[s] = next[s];
             first += CHUNK;
         }
         k = block_max_key(k, keys);
@@ -147,28 +179,45 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
     float m = -INFINITY, sum = 0.f;
     while (true) {
         const bool more = first - threadIdx.x * 4 + CHUNK < end;
-        if (more) batch<T, WIDE>(logits, first + CHUNK, end, -INFINITY, next);
-        float top = m;
+        if (more) batch<T, WIDE>(logits, first + CHUNK, end, next);
+        float z[STEPS][4], top = m;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[s][e] = cleaned(v[s][e]);
-                top = fmaxf(top, v[s][e]);
-            }
-        if (top > -INFINITY) {
-            sum *= m == -INFINITY ? 0.f : weight_of(m, top, rate);
+            for (int e = 0; e < 4; ++e) z[s][e] = v[s][e];
+        if (first - (int)threadIdx.x * 4 + CHUNK > end) {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += weight_of(v[s][e], top, rate);
+                for (int e = 0; e < 4; ++e)
+                    if (first + s * THREADS * 4 + e >= end) z[s][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) top = max3(max3(top, z[s][0], z[s][1]), z[s][2], z[s][3]);
+        top = fminf(top, FLT_MAX);
+        if (top > -INFINITY) {
+            // One multiplication and addition an entry: what m * rate is rounded by is the same for all of them.  A sum that a NaN or an infinity has got into is made again
+            // with those put right.
+            const float offset = -top * rate;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[e] += fast_exp2(fmaf(z[s][e], rate, offset));
+            float more_sum = (part[0] + part[1]) + (part[2] + part[3]);
+            if (!(more_sum < INFINITY)) {
+                more_sum = 0.f;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) more_sum += weight_of(cleaned(z[s][e]), top, rate);
+            }
+            sum = fmaf(sum, m == -INFINITY ? 0.f : weight_of(m, top, rate), more_sum);
             m = top;
         }
         if (!more) break;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[s][e] = next[s][e];
+        for (int s = 0; s < STEPS; ++s) v[s] = next[s];
         first += CHUNK;
     }
     float top = warp_max(m);
@@ -184,7 +233,7 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const Args a) {
 }
 
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(THREADS) verify_requests_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, REQUESTS_PER_SM) verify_requests_kernel(const Args a) {
     __shared__ Key keys[THREADS / 32];
     __shared__ float2 sums[KEPT];         // a row's maximum and sum; with temperature 0 the index of its largest logit in the latter's place
     __shared__ int refused_at;            // the first draft that does not stand, counted in the request's rows
@@ -195,8 +244,8 @@ __global__ void __launch_bounds__(THREADS) verify_requests_kernel(const Args a) 
     const int end_at = min(a.vocab, ((int)blockIdx.x + 1) * a.request_span);
     int first = blockIdx.x * a.request_span + threadIdx.x * 4;
     const float* noise = a.noise + (size_t)r * a.noise_stride;
-    float n[STEPS][4];
-    batch<float, WIDE>(noise, first, end_at, 1.f, n);
+    Four<float> n[STEPS];
+    batch<float, WIDE>(noise, first, end_at, n);
     const int row0 = min(max(a.row_start[r], 0), a.rows), row1 = min(max(a.row_start[r + 1], row0), a.rows), drafted = row1 - row0 - 1;
     const float temperature = a.temperature[r];
     if (drafted < 0) {  // a request without rows
@@ -280,58 +329,89 @@ __global__ void __launch_bounds__(THREADS) verify_requests_kernel(const Args a) 
     const T* logits = (const T*)a.logits + (size_t)end * a.stride;
     const float* probabilities = a.probabilities + (size_t)end * a.q_stride;
     const float m = sum.x, share = sum.y > 0.f ? 1.f / sum.y : 0.f;
-    Key rest = 0, left = 0;
-    float v[STEPS][4], d[STEPS][4];
-    while (true) {
-        batch<T, WIDE>(logits, first, end_at, -INFINITY, v);
-        if (beside) {
-            batch<float, WIDE>(probabilities, first, end_at, 0.f, d);
-        } else {
+    // Looks through entries from `first` on to `end_at`, `step` apart: the best of the target's probabilities (`own`), or of what is left of them beside the drafter's.
+    auto look = [&](int first, int end_at, int step, bool own) {
+        Key best_key = 0;
+        float best = -1.f;
+        const float offset = -m * rate;
+        const bool clean = share > 0.f && m < FLT_MAX;
+        Four<T> v[STEPS];
+        Four<float> d[STEPS];
+        while (true) {
+            batch<T, WIDE>(logits, first, end_at, v);
+            if (beside && !own) {
+                batch<float, WIDE>(probabilities, first, end_at, d);
+            } else {
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) d[s][0] = d[s][1] = d[s][2] = d[s][3] = 0.f;
-        }
-        // the largest of this thread's, compared as floats (ties keep the lower index, which comes first); only the winner becomes a key
-        float best_rest = -1.f, best_left = -1.f;
-        int at_rest = 0, at_left = 0;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int at = first + s * THREADS * 4 + e;
-                if (at >= end_at) continue;
-                const float p = share > 0.f ? weight_of(cleaned(v[s][e]), m, rate) * share : 0.f, clock = 1.f / fmaxf(n[s][e], FLT_MIN);
-                const float own = p * clock, more = at == banned ? 0.f : fmaxf(p - d[s][e], 0.f) * clock;
-                if (own > best_left) best_left = own, at_left = at;
-                if (more > best_rest) best_rest = more, at_rest = at;
+                for (int s = 0; s < STEPS; ++s) d[s].raw = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-        if (best_left >= 0.f) {
-            const Key a_left = key_of(best_left, at_left), a_rest = key_of(best_rest, at_rest);
-            left = a_left > left ? a_left : left;
-            rest = a_rest > rest ? a_rest : rest;
+            float z[STEPS][4], top = -1.f;
+            if (clean) {
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[s][e] = fast_exp2(fmaf(v[s][e], rate, offset)) * share;
+            } else {  // the row's largest logit is infinite, or there is none
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[s][e] = share > 0.f ? weight_of(cleaned(v[s][e]), m, rate) * share : 0.f;
+            }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[s][e] = fmaxf(z[s][e] - d[s][e], 0.f) * fast_reciprocal(fmaxf(n[s][e], FLT_MIN));  // a NaN, too, comes to 0
+                const int at = first + s * THREADS * 4;
+                if (!own && banned >= at && banned < at + 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (banned == at + e) z[s][e] = 0.f;
+                }
+                if (at + 4 > end_at) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at + e >= end_at) z[s][e] = -1.f;
+                }
+                top = max3(max3(top, z[s][0], z[s][1]), z[s][2], z[s][3]);
+            }
+            if (top > best) {  // seldom, once a few batches have been looked at: where does it stand?
+                best = top;
+                int at = 0;
+#pragma unroll
+                for (int s = STEPS - 1; s >= 0; --s)
+#pragma unroll
+                    for (int e = 3; e >= 0; --e)
+                        if (z[s][e] == top) at = first + s * THREADS * 4 + e;
+                best_key = key_of(best, at);
+            }
+            first += step;
+            if (first - (int)threadIdx.x * 4 >= end_at) break;
+            batch<float, WIDE>(noise, first, end_at, n);
         }
-        if (first - threadIdx.x * 4 + CHUNK >= end_at) break;
-        first += CHUNK;
-        batch<float, WIDE>(noise, first, end_at, 1.f, n);
-    }
-    rest = block_max_key(rest, keys);
-    left = block_max_key(left, keys);
+        return block_max_key(best_key, keys);
+    };
+    const Key found = look(first, end_at, CHUNK, !refused);
     if (threadIdx.x == 0) {
-        atomicMax(&a.best[2 * r], rest);
-        atomicMax(&a.best[2 * r + 1], left);
+        atomicMax(&a.best[r], found);
         __threadfence();
         last_block = atomicAdd(&a.arrived[r], 1) == (int)gridDim.x - 1;
     }
     __syncthreads();
     if (!last_block) return;
     __threadfence();
-    const volatile Key* best = a.best + 2 * r;
-    // where the drafter's probabilities leave nothing (rounding alone can do that), the target's own stand
-    const Key winner = refused && (unsigned)(best[0] >> 32) > ordered(0.f) ? best[0] : best[1];
+    Key winner = *const_cast<const volatile Key*>(a.best + r);
+    if (refused && (unsigned)(winner >> 32) <= ordered(0.f)) {  // nothing is left beside the drafter's (rounding alone can do that): the target's own probabilities stand
+        batch<float, WIDE>(noise, (int)threadIdx.x * 4, a.vocab, n);
+        winner = look((int)threadIdx.x * 4, a.vocab, CHUNK, true);
+        if (threadIdx.x == 0) keys[0] = winner;
+        __syncthreads();
+        winner = keys[0];
+    }
     write_answer(index_of(winner));
 }
 }  // namespace
 
-// workspace: rows * ceil(vocab / CHUNK) + 3 * requests words of 8 bytes.
+// workspace: rows * ceil(vocab / CHUNK) + 2 * requests words of 8 bytes.
 HB_EXPORT int hb_verify_drafts(const void* logits, int is_bf16, long long stride, const int* row_start, int requests, int rows, int vocab, const int* drafts,
                                const float* probabilities, long long q_stride, const float* uniform, const float* noise, long long noise_stride,
                                const float* temperature, void* workspace, int* accepted, int* tokens, int most, int* status, cudaStream_t stream) {
@@ -339,18 +419,19 @@ HB_EXPORT int hb_verify_drafts(const void* logits, int is_bf16, long long stride
     if (rows < 0 || vocab <= 0 || most <= 0 || !row_start || !noise || !temperature || !workspace || !accepted || !tokens || !status || ((uintptr_t)workspace & 7)) return HB_BAD_ARGUMENT;
     if (rows > 0 && (!logits || !drafts || !uniform)) return HB_BAD_ARGUMENT;
     if (rows > 65535 || requests > 65535 || vocab > 0x7fffffff - 2 * CHUNK) return HB_UNSUPPORTED_SIZE;
-    // As many blocks a row as fill the device eight times over between all rows, four times between all requests (whose blocks hold more), one for each CHUNK at most.
+    // As many blocks a row, and then a request, as the device holds at once between them, one for each CHUNK at most: a second turn of a few blocks would cost as much as
+    // the first.
     const int chunks = (vocab + CHUNK - 1) / CHUNK;
-    const auto span = [&](int lines, int times) {
-        const int wanted = (148 * times + lines - 1) / (lines > 0 ? lines : 1), blocks = wanted < 1 ? 1 : (wanted < chunks ? wanted : chunks);
+    const auto span = [&](int lines, int slots) {
+        const int wanted = slots / (lines > 0 ? lines : 1), blocks = wanted < 1 ? 1 : (wanted < chunks ? wanted : chunks);
         return (chunks + blocks - 1) / blocks * CHUNK;
     };
-    const int row_span = span(rows, 8), request_span = span(requests, 4);
+    const int row_span = span(rows, 148 * ROWS_PER_SM), request_span = span(requests, 148 * REQUESTS_PER_SM);
     const int row_blocks = (vocab + row_span - 1) / row_span, request_blocks = (vocab + request_span - 1) / request_span;
     float2* pieces = (float2*)workspace;
     Key* best = (Key*)(pieces + (size_t)rows * chunks);
     const Args a{logits, stride, row_start, requests, rows, vocab, drafts, probabilities, q_stride, uniform, noise, noise_stride, temperature, row_blocks, row_span, request_span,
-                 pieces, best, (int*)(best + 2 * (size_t)requests), accepted, tokens, most, status};
+                 pieces, best, (int*)(best + requests), accepted, tokens, most, status};
     const int element = is_bf16 ? 2 : 4;
     const bool wide = !(((uintptr_t)logits | (uintptr_t)(stride * element)) & (4 * element - 1)) && !(((uintptr_t)noise | (uintptr_t)(noise_stride * 4)) & 15) &&
                       !(((uintptr_t)probabilities | (uintptr_t)(probabilities ? q_stride * 4 : 0)) & 15);

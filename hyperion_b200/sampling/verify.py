@@ -39,24 +39,21 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
         raise KernelError("verify_drafts: logits [rows, vocab] and float32 noise [requests, vocab], both with unit inner stride")
     if probabilities is not None and (probabilities.shape != shape or probabilities.dtype is not torch.float32 or probabilities.stride(1) != 1):
         raise KernelError("verify_drafts: the drafter's probabilities are float32 [rows, vocab] with unit inner stride")
-    for name, t, dtype, count in (("row_start", row_start, torch.int32, requests + 1), ("drafts", drafts, torch.int32, rows), ("uniform", uniform, torch.float32, rows),
-                                  ("temperature", temperature, torch.float32, requests)):
-        if t.dtype is not dtype or t.shape != (count,) or not t.is_contiguous():
-            raise KernelError(f"verify_drafts: {name} is a dense {dtype} vector of {count}")
+    if (row_start.dtype is not torch.int32 or drafts.dtype is not torch.int32 or uniform.dtype is not torch.float32 or temperature.dtype is not torch.float32
+            or drafts.shape != (rows,) or uniform.shape != (rows,) or temperature.shape != (requests,)
+            or not (row_start.is_contiguous() and drafts.is_contiguous() and uniform.is_contiguous() and temperature.is_contiguous())):
+        raise KernelError(f"verify_drafts: dense vectors: row_start int32 [{requests + 1}], drafts int32 [{rows}], uniform float32 [{rows}], temperature float32 [{requests}]")
     if most < 1:
         raise KernelError("verify_drafts: most counts a request's drafts and the token that follows them")
     require_cuda(logits, row_start, drafts, uniform, noise, temperature, probabilities)
     device = logits.device
-    # the answer (accepted, then tokens) and the kernels' workspace (pieces and keys of 8 bytes, counters) are one allocation
-    words = rows * -(-vocab // CHUNK) + 3 * requests
-    memory = torch.empty(2 * words + requests * (1 + most), dtype=torch.int32, device=device)
-    answer = memory.data_ptr() + 8 * words
+    accepted, tokens = torch.empty(requests, dtype=torch.int32, device=device), torch.empty((requests, most), dtype=torch.int32, device=device)
+    workspace = torch.empty(rows * -(-vocab // CHUNK) + 2 * requests, dtype=torch.int64, device=device)
     check(entry("verify", "hb_verify_drafts", "pilpiiipplpplppppipp")(
         logits.data_ptr(), is_bf16(logits), logits.stride(0), row_start.data_ptr(), requests, rows, vocab, drafts.data_ptr(),
         probabilities.data_ptr() if probabilities is not None else 0, probabilities.stride(0) if probabilities is not None else 0, uniform.data_ptr(), noise.data_ptr(),
-        noise.stride(0), temperature.data_ptr(), memory.data_ptr(), answer, answer + 4 * requests, most, status_word(device).data_ptr(), stream_address()), "verify_drafts")
-    accepted, tokens = memory[2 * words:].split((requests, requests * most))
-    return accepted, tokens.view(requests, most)
+        noise.stride(0), temperature.data_ptr(), workspace.data_ptr(), accepted.data_ptr(), tokens.data_ptr(), most, status_word(device).data_ptr(), stream_address()), "verify_drafts")
+    return accepted, tokens
 
 
 def reference_verify(logits: np.ndarray, drafts: Sequence[int], uniform: Sequence[float], noise: np.ndarray, temperature: float,
@@ -73,7 +70,7 @@ def reference_verify(logits: np.ndarray, drafts: Sequence[int], uniform: Sequenc
     p = np.where(np.isfinite(top), np.exp((z - np.where(np.isfinite(top), top, 0.0)) / temperature), 0.0)
     p = p / np.maximum(p.sum(1, keepdims=True), np.finfo(np.float64).tiny)
     for i, x in enumerate(drafts):
-        q = probabilities[i].astype(np.float64) if probabilities is not None else np.eye(z.shape[1])[x]
+        q = probabilities[i].astype(np.float64) if probabilities is not None else (np.arange(z.shape[1]) == x).astype(np.float64)
         if not uniform[i] * q[x] < p[i, x]:
             rest = np.maximum(p[i] - q, 0.0)
             return i, [int(y) for y in drafts[:i]] + [int(((rest if rest.max() > 0 else p[i]) / noise).argmax())]
