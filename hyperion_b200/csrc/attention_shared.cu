@@ -47,7 +47,7 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int MOST_ROWS = 16;   // (token, head) rows of a strip: 8 or 16
 constexpr int WARPS = 4;        // that compute; one more fetches
 constexpr int THREADS = 32 * (WARPS + 1);
-constexpr int ITEM_WORDS = 6;   // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of a request's own positions)
+constexpr int ITEM_WORDS = 7;   // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of a request's own positions), -
 constexpr int OWN_PIECE = 1 << 30;
 constexpr unsigned WAIT_LIMIT = 1u << 24;
 constexpr float HEADROOM = 8.f;  // m stands so far below the maximum: P up to 2^8 keeps float16's small weights further from its smallest number

@@ -7,8 +7,8 @@
 //   warp 0       fetches: one cp.async.bulk.tensor per page (and 128-byte panel) of K and of V, the queries as one 3-D box per 64-column panel;
 //   warp 1       issues S_x = Q_x K^T (M 128, N 128) and O_x += P_x V (P from tensor memory, V MN-major), each half's next S right behind its last product;
 //   warps 4-11   softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by much;
-//   warps 12-19  8-bit records only: four warps turn each K tile into bfloat16 (which holds code * 2^e exactly) in the swizzled layout that the products
-//                read, four each V tile; the records' bytes come once from memory.
+//   warps 12-19  8-bit records that one run of tokens walks: four warps turn each K tile into bfloat16 (which holds code * 2^e exactly) in the swizzled layout that the products
+//                read, four each V tile; the records' bytes come once from memory.  (Records that several runs walk are made into operands beforehand, for all of them.)
 // Over bfloat16 values, weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as
 // much as its own rounding does.  8-bit values go as float16, which holds code * 2^(e - e0) exactly for exponents from e0 - 12 to e0 + 7 (e0: the largest of
 // the item's first tile; the result is scaled back at the end), and so do the weights, whose rounding then does not show and whose second part is not
@@ -43,8 +43,10 @@ constexpr int RAW_BYTES = BN * D;             // a tile of codes
 constexpr int STAGES = 2;                     // of K tiles and of V tiles as the products read them; one tile of codes of each is under way
 constexpr int TMEM_COLS = 512;                // S_H [0,128) S_L [128,256) O_H [256,256+D) O_L [384,384+D); P_x over S_x
 constexpr int O_COL = 256;
-constexpr int ITEM_WORDS = 6;                 // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of its own positions)
+constexpr int ITEM_WORDS = 7;                 // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of its own positions), first operand tile
 constexpr int OWN_PIECE = 1 << 30;
+enum Source : int { BFLOAT16 = 0, CODES = 1, OPERANDS = 2 };  // what the tiles come from: a bfloat16 cache, an 8-bit one, or operands made of one beforehand
+constexpr int LOWEST = -12, HIGHEST = 7;       // of e - e0, for values as float16
 constexpr unsigned WAIT_LIMIT = 1u << 24;
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -78,6 +80,9 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -233,6 +238,7 @@ __device__ __forceinline__ float value_of_half(unsigned short h) {
 
 struct Args {
     const signed char* exponents;  // of an 8-bit cache
+    const unsigned char* operands; const int* kinds;  // [tiles, kv_heads, 2, TILE_BYTES]; [tiles, kv_heads]: 2 * (e0 + 64) + whether the values are float16
     bf16* out; int out_stride;
     const int* block_table; int table_width;
     const int* items;
@@ -248,17 +254,16 @@ struct Args {
     int* status;
 };
 
-template <bool E8>
+template <Source FROM>
 struct Shape {
+    static constexpr bool E8 = FROM == CODES;
     static constexpr int WARPS = E8 ? 20 : 12, THREADS = 32 * WARPS;
     // Registers a thread, by groups of four warps, of the 96 that 640 threads are launched with (128 * 56 + 256 * 152 + 256 * 56 = 60,416 of 61,440)
-    [[maybe_unused]] static constexpr int FEW = 56;
-    [[maybe_unused]] static constexpr int MANY = 152;
-    [[maybe_unused]] static constexpr int CONVERTING = 56;
+    enum : int { FEW = 56, MANY = 152, CONVERTING = 56 };
     static constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
     // How far (in powers of two) a maximum may be outgrown before the row is rescaled.  A stale maximum changes no result (numerator and denominator use the same
     // one) as long as nothing overflows: weights are float16 up to 2^15, or bfloat16 and their sums float.
-    static constexpr float OUTGROWN = E8 ? 13.f : 32.f;
+    static constexpr float OUTGROWN = FROM != BFLOAT16 ? 13.f : 32.f;
     static constexpr int RAW = E8 ? 2 * RAW_BYTES + 2 * BN : 0;  // codes of K and of V, and their exponents
     static constexpr size_t USED = 1024 + (size_t)Q_BYTES + (size_t)2 * STAGES * TILE_BYTES + RAW + 256;
     // more than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory
@@ -266,17 +271,42 @@ struct Shape {
     static_assert(USED <= 227 * 1024, "an SM's shared memory");
 };
 
+// Sixteen codes times 2^e as operands: float16 (-12 <= e <= 7) or bfloat16.
+template <bool HALVES>
+__device__ __forceinline__ void widen(const uint4& codes, int e, unsigned (&wide)[8]) {
+    const unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
+    if constexpr (HALVES) {
+        const unsigned half = (unsigned)(15 + min(max(e, LOWEST), HIGHEST)) << 10, factor = half | half << 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            asm("{.reg .b16 lo, hi;\n\t.reg .b32 a, b;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 a, lo;\n\tcvt.rn.f16x2.e4m3x2 b, hi;\n\t"
+                "mul.rn.f16x2 %0, a, %3;\n\tmul.rn.f16x2 %1, b, %3;\n\t}" : "=r"(wide[2 * k]), "=r"(wide[2 * k + 1]) : "r"(words[k]), "r"(factor));
+    } else {
+        const float f = __uint_as_float((unsigned)(127 + e) << 23);
+        const Pair factor{f, f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            unsigned h0, h1;
+            asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
+            const Pair v0 = mul2(Pair{value_of_half((unsigned short)h0), value_of_half((unsigned short)(h0 >> 16))}, factor);
+            const Pair v1 = mul2(Pair{value_of_half((unsigned short)h1), value_of_half((unsigned short)(h1 >> 16))}, factor);
+            wide[2 * k] = pack_bf16x2(v0.x, v0.y), wide[2 * k + 1] = pack_bf16x2(v1.x, v1.y);
+        }
+    }
+}
+
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
 struct Item {
-    int tok0, ntok, key_lo, key_hi, piece, start, n_tiles, halves;
+    int tok0, ntok, key_lo, key_hi, piece, operand, start, n_tiles, halves;
     const int* table;
 };
 
-template <bool E8>
-__global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
-    typedef Shape<E8> S;
+template <Source FROM>
+__global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
+    typedef Shape<FROM> S;
+    constexpr bool E8 = S::E8;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* k_ring = base;
@@ -347,7 +377,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
     auto read_item = [&](int index) {
         Item it;
         const int* words = a.items + (size_t)index * ITEM_WORDS;
-        it.tok0 = words[0], it.ntok = words[1], it.key_lo = words[3], it.key_hi = words[4], it.piece = words[5];
+        it.tok0 = words[0], it.ntok = words[1], it.key_lo = words[3], it.key_hi = words[4], it.piece = words[5], it.operand = words[6];
         it.table = a.block_table + (size_t)words[2] * a.table_width;
         it.start = it.key_lo / BN * BN;
         it.n_tiles = it.key_hi > it.key_lo ? (it.key_hi - it.start + BN - 1) / BN : 0;
@@ -357,7 +387,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
     auto fail = [&] { *failed = 1; };
 
     if (warp < 4) {
-      if constexpr (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::FEW));
+      if constexpr (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"((int)S::FEW));
       if (warp == 0) {
         // ------------------------------------------------------------------ producer (the whole warp)
         if (lane == 0) {
@@ -379,6 +409,19 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
             for (int t = 0; t < it.n_tiles && alive; ++t, ++g) {
                 const int tile_base = it.start + t * BN;
+                if constexpr (FROM == OPERANDS) {  // two plain copies: they stand there as the products read them
+                    if (lane == 0) {
+                        const unsigned char* from = a.operands + ((size_t)(it.operand + t) * a.kv_heads + kvh) * (2 * TILE_BYTES);
+                        for (int which = 0; which < 2 && alive; ++which) {
+                            const int s = g & 1, turn = g >> 1;
+                            if (!mbar_wait(which ? &v_empty[s] : &k_empty[s], (turn & 1) ^ 1, failed)) { alive = false; break; }
+                            mbar_expect_tx(which ? &v_full[s] : &k_full[s], TILE_BYTES);
+                            bulk_load((which ? v_ring : k_ring) + (size_t)s * TILE_BYTES, from + which * TILE_BYTES, TILE_BYTES, which ? &v_full[s] : &k_full[s]);
+                        }
+                    }
+                    alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
+                    continue;
+                }
                 int my_page = -1;
                 const int k0 = tile_base + lane * a.page_size;
                 if (lane < pages_per_tile && k0 < it.key_hi && k0 + a.page_size > it.key_lo) {
@@ -479,6 +522,8 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                     if constexpr (E8) {
                         if (!mbar_wait(&kind_full[g & 1], (g >> 1) & 1, failed)) { ok = false; break; }
                         halves = kinds[g & 1] & 1;
+                    } else if constexpr (FROM == OPERANDS) {
+                        halves = a.kinds[(size_t)(it.operand + j) * a.kv_heads + kvh] & 1;
                     }
                     for (int x = 0; x < it.halves && ok; ++x) {
                         for (int part = 0; part < 2 && ok; ++part) {
@@ -512,7 +557,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
       }
     } else if (warp < 12) {
         // ------------------------------------------------------------------ softmax: thread = row = tensor-memory lane of its half
-        if constexpr (E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::MANY));
+        if constexpr (E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"((int)S::MANY));
         const int x = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane, v = x * BM + r;
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
         const unsigned s_addr = lane_addr + x * BN, o_addr = lane_addr + O_COL + x * BM;
@@ -531,6 +576,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             int kind = 2 * 64;
             for (int j = 0; j < it.n_tiles; ++j) {
                 const int h = hx + j;
+                if constexpr (FROM == OPERANDS) kind = a.kinds[(size_t)(it.operand + j) * a.kv_heads + kvh];  // there by the time S is
                 if (!mbar_wait(&s_full[x], h & 1, failed)) { ok = false; break; }
                 tc_fence_after();
                 const int tile_base = it.start + j * BN, last_visible = hi - tile_base, first_visible = it.key_lo - tile_base;
@@ -624,9 +670,11 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                         if (c) arrived(s1);
                     }
                 };
-                if constexpr (E8) {
-                    if (!mbar_wait(&kind_full[(g0 + j) & 1], ((g0 + j) >> 1) & 1, failed)) { ok = false; break; }
-                    kind = kinds[(g0 + j) & 1];
+                if constexpr (FROM != BFLOAT16) {
+                    if constexpr (E8) {
+                        if (!mbar_wait(&kind_full[(g0 + j) & 1], ((g0 + j) >> 1) & 1, failed)) { ok = false; break; }
+                        kind = kinds[(g0 + j) & 1];
+                    }
                     if (kind & 1) {
                         walk(weigh_halves);
                     } else {
@@ -648,7 +696,7 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
             tc_fence_after();
             if (ok) {
                 const size_t slot = row_valid && a.pieces ? (size_t)((it.piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (it.piece & (OWN_PIECE - 1))) * a.heads + first_head + hh : 0;
-                const float back = E8 ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
+                const float back = FROM != BFLOAT16 ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
                 const float inv = a.pieces ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
 #pragma unroll
                 for (int c = 0; c < D; c += 16) {
@@ -682,10 +730,9 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
         if (!ok) fail();
     } else if constexpr (E8) {
         // ------------------------------------------------------------------ codes into operands: warps 12 to 15 the K tiles, 16 to 19 the V tiles
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CONVERTING));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"((int)S::CONVERTING));
         const int which = (warp - 12) >> 2, w = warp & 3;
         constexpr int CHUNKS = D / 16;  // 16 codes each, of a row
-        constexpr int LOWEST = -12, HIGHEST = 7;  // of e - e0, for float16
         bool ok = true;
         int g = 0;
         for (int index = first_item; index < end_item && ok; ++index) {
@@ -726,26 +773,8 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
                         const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
                         const int e = min(max((int)e8[row], -40), 40) - e0;
                         const bool keep = which == 0 || (tile_base + row >= it.key_lo && tile_base + row < it.key_hi);
-                        const unsigned* words = reinterpret_cast<const unsigned*>(&codes);
                         unsigned wide[8];
-                        if constexpr (as_halves.value) {
-                            const unsigned half = (unsigned)(15 + min(max(e, LOWEST), HIGHEST)) << 10, factor = half | half << 16;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                asm("{.reg .b16 lo, hi;\n\t.reg .b32 a, b;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 a, lo;\n\tcvt.rn.f16x2.e4m3x2 b, hi;\n\t"
-                                    "mul.rn.f16x2 %0, a, %3;\n\tmul.rn.f16x2 %1, b, %3;\n\t}" : "=r"(wide[2 * k]), "=r"(wide[2 * k + 1]) : "r"(words[k]), "r"(factor));
-                        } else {
-                            const float f = __uint_as_float((unsigned)(127 + e) << 23);
-                            const Pair factor{f, f};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                unsigned h0, h1;
-                                asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
-                                const Pair v0 = mul2(Pair{value_of_half((unsigned short)h0), value_of_half((unsigned short)(h0 >> 16))}, factor);
-                                const Pair v1 = mul2(Pair{value_of_half((unsigned short)h1), value_of_half((unsigned short)(h1 >> 16))}, factor);
-                                wide[2 * k] = pack_bf16x2(v0.x, v0.y), wide[2 * k + 1] = pack_bf16x2(v1.x, v1.y);
-                            }
-                        }
+                        widen<as_halves.value>(codes, e, wide);
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const int oc = 2 * chunk + half;
@@ -775,6 +804,70 @@ __global__ void __launch_bounds__(Shape<E8>::THREADS, 1) attention_shared_kernel
     }
 }
 
+// Operands of 8-bit records that several runs of tokens walk: a block makes one tile of K or of V of one key/value head, in the layout of the attention's shared memory, so
+// that every one of those runs fetches it by two plain copies and converts nothing.  Bound by memory (three bytes an entry).  It pays from three runs on: 256 requests behind
+// 16,384 positions (eight runs) 162 us -> 154, 64 requests behind 4,096 (two runs) 35.6 without it and 39.4 with it.
+constexpr int OPERAND_THREADS = 256;
+__global__ void __launch_bounds__(OPERAND_THREADS) shared_operands_kernel(const unsigned char* __restrict__ codes, const signed char* __restrict__ exponents, const int* __restrict__ block_table,
+                                                                          int table_width, const int4* __restrict__ tiles, unsigned char* __restrict__ operands, int* __restrict__ kinds,
+                                                                          int page_size, int pages, int* status) {
+    __shared__ int bounds[BN / 32][3];
+    let_next_kernel_start();
+    const int4 tile = tiles[blockIdx.x];  // table row, first position, first key and last key + 1 of the range; written with the plan, long before
+    wait_for_previous_kernels();
+    const int kvh = blockIdx.y, kv_heads = gridDim.y, which = blockIdx.z, tid = threadIdx.x, base = tile.y, lo = tile.z, hi = tile.w, shift = 31 - __clz(page_size);
+    const int* table = block_table + (size_t)tile.x * table_width;
+    auto record = [&](int pos) -> long long {  // -1: not in the range, or without a page
+        const int block = pos >> shift, page = pos >= lo && pos < hi && block < table_width ? table[block] : -1;
+        return page >= 0 && page < pages ? (((long long)page * 2 + which) * kv_heads + kvh) * page_size + (pos & (page_size - 1)) : -1;
+    };
+    constexpr int CHUNKS = D / 16, UNITS = BN * CHUNKS / OPERAND_THREADS, STEP = OPERAND_THREADS / CHUNKS;  // a thread's chunks of 16 codes, of rows STEP apart
+    const int chunk = tid % CHUNKS, row0 = tid / CHUNKS, first = lo / BN * BN;
+    long long from[UNITS];
+    uint4 raw[UNITS];
+    int e[UNITS], e0 = 0, low = 127, high = -128;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) from[u] = record(base + row0 + u * STEP);
+    const long long there = which && tid < BN ? record(first + tid) : -1, here = tid < BN ? record(base + tid) : -1;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const long long at = max(from[u], 0ll);
+        raw[u] = *reinterpret_cast<const uint4*>(codes + at * D + chunk * 16);
+        e[u] = min(max((int)exponents[at], -40), 40);
+    }
+    if (tid < BN && kvh == 0 && here < 0 && base + tid >= lo && base + tid < hi) atomicOr(status, HB_STATUS_BAD_PAGE);
+    bool halves = false;
+    if (which) {  // e0: the largest exponent of the range's first tile; low and high: those of this one
+        if (tid < BN) {
+            e0 = there >= 0 ? min(max((int)exponents[there], -40), 40) : -40;
+            if (here >= 0) low = high = min(max((int)exponents[here], -40), 40);
+            e0 = __reduce_max_sync(0xffffffffu, e0), low = __reduce_min_sync(0xffffffffu, low), high = __reduce_max_sync(0xffffffffu, high);
+            if ((tid & 31) == 0) bounds[tid >> 5][0] = e0, bounds[tid >> 5][1] = low, bounds[tid >> 5][2] = high;
+        }
+        __syncthreads();
+        e0 = bounds[0][0], low = bounds[0][1], high = bounds[0][2];
+#pragma unroll
+        for (int w = 1; w < BN / 32; ++w) e0 = max(e0, bounds[w][0]), low = min(low, bounds[w][1]), high = max(high, bounds[w][2]);
+        halves = low - e0 >= LOWEST && high - e0 <= HIGHEST;
+        if (tid == 0) kinds[(size_t)blockIdx.x * kv_heads + kvh] = 2 * (e0 + 64) + (halves ? 1 : 0);
+    }
+    unsigned char* out = operands + (((size_t)blockIdx.x * kv_heads + kvh) * 2 + which) * TILE_BYTES;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const int row = row0 + u * STEP;
+        unsigned wide[8];
+        if (halves) widen<true>(raw[u], e[u] - e0, wide);
+        else widen<false>(raw[u], e[u] - e0, wide);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int oc = 2 * chunk + half;
+            uint4 w = make_uint4(wide[4 * half], wide[4 * half + 1], wide[4 * half + 2], wide[4 * half + 3]);
+            if (from[u] < 0) w = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out + (oc >> 3) * (KV_PANEL * 2) + row * 128 + (((oc & 7) ^ (row & 7)) << 4)) = w;
+        }
+    }
+}
+
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
@@ -790,18 +883,18 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-template <bool E8>
+template <Source FROM>
 int launch(const Args& a, int blocks, const void* q, int q_stride, int n_tokens, const void* cache, cudaStream_t stream) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return HB_BAD_ARGUMENT;
     // the cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and up to 128 bytes
     CUtensorMap map, q_map;
     const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)a.pages * 2 * a.kv_heads * a.page_size};
-    const cuuint64_t strides[1] = {(cuuint64_t)D * (E8 ? 1 : 2)};
-    const cuuint32_t box[2] = {(cuuint32_t)(E8 ? D : 64), (cuuint32_t)a.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * (FROM == BFLOAT16 ? 2 : 1)};
+    const cuuint32_t box[2] = {(cuuint32_t)(FROM == BFLOAT16 ? 64 : D), (cuuint32_t)a.page_size};
     const cuuint32_t elem[3] = {1, 1, 1};
-    if (encode(&map, E8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               E8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    if (encode(&map, FROM == BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               FROM != BFLOAT16 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return HB_BAD_ARGUMENT;
     // the queries as (column, head, token): an item's box is 64 columns of gc heads of its tokens
     const cuuint64_t q_dims[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)n_tokens};
@@ -810,16 +903,31 @@ int launch(const Args& a, int blocks, const void* q, int q_stride, int n_tokens,
     if (encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), q_dims, q_strides, q_box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return HB_BAD_ARGUMENT;
-    static const cudaError_t configured = cudaFuncSetAttribute(attention_shared_kernel<E8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8>::SMEM);
+    static const cudaError_t configured = cudaFuncSetAttribute(attention_shared_kernel<FROM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<FROM>::SMEM);
     if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(attention_shared_kernel<E8>, dim3(blocks, a.kv_heads * a.chunks), dim3(Shape<E8>::THREADS), Shape<E8>::SMEM, stream, map, q_map, a);
+    return launch_after_previous(attention_shared_kernel<FROM>, dim3(blocks, a.kv_heads * a.chunks), dim3(Shape<FROM>::THREADS), Shape<FROM>::SMEM, stream, map, q_map, a);
+}
+const int* kinds_of(const void* operands, long long tiles, long long kv_heads) {  // they stand behind the tiles
+    return operands ? (const int*)((const unsigned char*)operands + (size_t)tiles * kv_heads * (2 * TILE_BYTES)) : nullptr;
 }
 }  // namespace
+
+// tiles [n_tiles, 4]: table row, first position, first key and last key + 1 of the tile's range.  operands: n_tiles * kv_heads * (4 * 128 * D + 4) bytes.
+HB_EXPORT int hb_shared_operands(const void* codes, const void* exponents, const int* block_table, int table_width, const int* tiles, int n_tiles, void* operands, int kv_heads,
+                                 int page_size, int pages, int* status, cudaStream_t stream) {
+    if (n_tiles <= 0) return 0;
+    if (!codes || !exponents || !block_table || !tiles || !operands || !status || table_width <= 0 || kv_heads <= 0 || pages <= 0) return HB_BAD_ARGUMENT;
+    if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1)) || kv_heads > 65535) return HB_UNSUPPORTED_SIZE;
+    if (((uintptr_t)codes | (uintptr_t)operands) & 15) return HB_BAD_ARGUMENT;
+    if ((uintptr_t)tiles & 15) return HB_BAD_ARGUMENT;
+    return launch_after_previous(shared_operands_kernel, dim3(n_tiles, kv_heads, 2), dim3(OPERAND_THREADS), 0, stream, (const unsigned char*)codes, (const signed char*)exponents, block_table,
+                                 table_width, (const int4*)tiles, (unsigned char*)operands, const_cast<int*>(kinds_of(operands, n_tiles, kv_heads)), page_size, pages, status);
+}
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
 // items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most 256 / min(heads / kv_heads, 256) tokens.  pieces, sums null: one piece a row.
 HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_tokens, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table,
-                                        int table_width, const int* items, const int* first_item, int blocks, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads,
+                                        int table_width, const int* items, const int* first_item, int blocks, const void* operands, int operand_tiles, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads,
                                         int kv_heads, int page_size, int pages, float scale, int* status, cudaStream_t stream) {
     if (blocks <= 0) return 0;
     if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
@@ -830,7 +938,9 @@ HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_token
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
-    const Args a{(const signed char*)exponents, (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
+    if (operands && (!exponents || operand_tiles <= 0 || ((uintptr_t)operands & 15))) return HB_BAD_ARGUMENT;
+    const Args a{(const signed char*)exponents, (const unsigned char*)operands, kinds_of(operands, operand_tiles, kv_heads), (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
-    return exponents ? launch<true>(a, blocks, q, q_stride, n_tokens, cache, stream) : launch<false>(a, blocks, q, q_stride, n_tokens, cache, stream);
+    if (operands) return launch<OPERANDS>(a, blocks, q, q_stride, n_tokens, cache, stream);
+    return exponents ? launch<CODES>(a, blocks, q, q_stride, n_tokens, cache, stream) : launch<BFLOAT16>(a, blocks, q, q_stride, n_tokens, cache, stream);
 }

@@ -287,13 +287,14 @@ HB_API int hb_plan_shared(int n_requests, const int64_t* counts, const int64_t* 
         for (int g = 0; g < n_groups; ++g) shared.push_back({groups[3 * g], groups[3 * g + 1], groups[3 * g + 2]});
         const hb::SharedPlan plan = hb::plan_shared(std::vector<int64_t>(counts, counts + n_requests), std::vector<int64_t>(lengths, lengths + n_requests), shared, heads, kv_heads, sms);
         planned.clear();
-        int64_t* places = sizes + 8;
-        for (const std::vector<int>* part : {&plan.strips.items, &plan.strips.first, &plan.tiles.items, &plan.tiles.first, &plan.last, &plan.starts, &plan.own}) {
+        int64_t* places = sizes + 9;
+        for (const std::vector<int>* part : {&plan.strips.items, &plan.strips.first, &plan.tiles.items, &plan.tiles.first, &plan.last, &plan.starts, &plan.own, &plan.operands}) {
+            planned.resize((planned.size() + 3) / 4 * 4);  // each part on a boundary of 16 bytes
             *places++ = (int64_t)planned.size();
             planned.insert(planned.end(), part->begin(), part->end());
         }
-        const int64_t figures[8] = {(int64_t)planned.size(), plan.strips.blocks(), plan.strip_rows, plan.tiles.blocks(), (int64_t)plan.last.size(), plan.starts.back(), plan.joined, plan.longest};
-        std::copy(figures, figures + 8, sizes);
+        const int64_t figures[9] = {(int64_t)planned.size(), plan.strips.blocks(), plan.strip_rows, plan.tiles.blocks(), (int64_t)plan.last.size(), plan.starts.back(), plan.joined, plan.longest, (int64_t)plan.operands.size() / 4};
+        std::copy(figures, figures + 9, sizes);
     });
 }
 HB_API int hb_plan_shared_take(int* words, int64_t capacity) {

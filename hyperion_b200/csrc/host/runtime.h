@@ -75,8 +75,8 @@ int hb_plan_attention(int n_rows, const int* counts, int tokens_per_tile, int to
                       int* n_items);
 
 /* Attention behind shared positions: counts and lengths of the step's requests, groups as triples (first request, requests, positions). Plans the step and
- * keeps the plan for this thread; sizes receives: words, strip blocks, rows of a strip, tile blocks, tokens, pieces, whether pieces have to be joined, the longest length, and
- * the places in words of: strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces. */
+ * keeps the plan for this thread; sizes receives: words, strip blocks, rows of a strip, tile blocks, tokens, pieces, whether pieces have to be joined, the longest length,
+ * operand tiles, and the places in words of: strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces, operand tiles. */
 int hb_plan_shared(int n_requests, const int64_t* counts, const int64_t* lengths, int n_groups, const int64_t* groups, int64_t heads, int64_t kv_heads, int64_t sms, int64_t* sizes);
 /* Copies this thread's last plan. */
 int hb_plan_shared_take(int* words, int64_t capacity);

@@ -16,6 +16,7 @@ constexpr int64_t KEYS = 128;            // keys of a tile, in which shares are 
 struct Run {
     int64_t token, count, row, low, high;
     bool own;
+    int64_t operand = 0;  // of the range's first tile
 };
 
 int64_t tiles_of(const Run& run) { return (run.high + KEYS - 1) / KEYS - run.low / KEYS; }
@@ -58,7 +59,7 @@ Walk cut(const std::vector<Run>& runs, int64_t blocks, double overhead, int64_t 
                 if (take - room >= least) take = std::max(room, least);  // what would be left over must be worth an item
             }
             const int64_t low = std::max(run.low, (base + done) * KEYS), high = std::min(run.high, (base + done + take) * KEYS);
-            for (int64_t word : {run.token, run.count, run.row, low, high, (int64_t)piece + (run.own ? OWN_PIECE : 0)}) walk.items.push_back((int)word);
+            for (int64_t word : {run.token, run.count, run.row, low, high, (int64_t)piece + (run.own ? OWN_PIECE : 0), run.operand + done}) walk.items.push_back((int)word);
             used += overhead + (double)take;
             done += take;
             left -= take;
@@ -109,13 +110,28 @@ SharedPlan plan_shared(const std::vector<int64_t>& counts, const std::vector<int
     const auto is_wide = [&](const Run& range) { return range.count * group > MOST_STRIP_ROWS; };
     for (const Run& range : ranges)
         if (!is_wide(range) && range.count * group > 8) plan.strip_rows = 16;
+    int64_t walked = 0, distinct = 0;
+    for (Run& range : ranges) {
+        if (!is_wide(range)) continue;
+        const int64_t per = std::max<int64_t>(1, TILE_ROWS / group), tiles = tiles_of(range);
+        range.operand = distinct;
+        distinct += tiles;
+        walked += tiles * ((range.count + per - 1) / per);
+    }
+    if (walked >= 3 * distinct && distinct > 0) {  // measured where the operands are made (attention_shared_tiles.cu)
+        require(distinct <= most / 4, "plan_shared: the tiles of a step fit 32 bits");
+        for (const Run& range : ranges)
+            if (is_wide(range))
+                for (int64_t at = range.low / KEYS * KEYS; at < range.high; at += KEYS)
+                    for (int64_t word : {range.row, at, range.low, range.high}) plan.operands.push_back((int)word);
+    }
     const auto runs_of = [&](bool wide, int64_t rows) {
         const int64_t per = std::max<int64_t>(1, rows / group);
         std::vector<Run> runs;
         for (const Run& range : ranges)
             if (is_wide(range) == wide)
                 for (int64_t at = 0; at < range.count; at += per)
-                    runs.push_back({range.token + at, std::min(per, range.count - at), range.row, range.low, range.high, range.own});
+                    runs.push_back({range.token + at, std::min(per, range.count - at), range.row, range.low, range.high, range.own, range.operand});
         return runs;
     };
     const auto blocks_for = [&](int64_t rows, int64_t slots) { return std::max<int64_t>(1, slots / (kv_heads * ((group + rows - 1) / rows))); };

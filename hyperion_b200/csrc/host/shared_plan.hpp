@@ -9,9 +9,10 @@ struct SharedGroup {
     int64_t first, members, positions;  // requests first .. first + members - 1 hold the same pages for their first `positions` positions
 };
 
-// An item: first token, tokens, table row, first key, last key + 1, piece.  `piece` is the item's number among the shares of its range; a token's pieces are those of
-// its group's positions, from starts[token] on, and those of its own request's, from own[token] on: an item of the latter kind has OWN_PIECE added.
-constexpr int ITEM_WORDS = 6;
+// An item: first token, tokens, table row, first key, last key + 1, piece, operand tile.  `piece` is the item's number among the shares of its range; a token's pieces are those of
+// its group's positions, from starts[token] on, and those of its own request's, from own[token] on: an item of the latter kind has OWN_PIECE added.  `operand tile`: where the item's
+// first tile stands among the plan's operands.
+constexpr int ITEM_WORDS = 7;
 constexpr int OWN_PIECE = 1 << 30;
 
 struct Walk {  // of one kernel: block b takes items first[b] .. first[b + 1] - 1
@@ -22,6 +23,9 @@ struct Walk {  // of one kernel: block b takes items first[b] .. first[b + 1] - 
 struct SharedPlan {
     Walk strips, tiles;
     int strip_rows = 8;
+    // The tiles of the wide ranges, each as (table row, first position, first key, last key + 1 of its range), where 8-bit records are worth being made into operands once for all
+    // the runs of tokens that walk them; empty where every range has one run, which does that on its way.
+    std::vector<int> operands;
     std::vector<int> last, starts, own;  // the last position a token sees, its first piece, its first piece of its own request's positions
     bool joined = false;                 // some token has another number of pieces than one
     int64_t longest = 0;

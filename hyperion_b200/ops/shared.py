@@ -19,6 +19,9 @@ from .cache8 import Cache8, check_cache8
 from .native import KernelError, check, entry, require_cuda, sm_count, stream_address
 
 
+TILE_KEYS = 128  # keys of an operand tile
+
+
 def supported(head_dim: int, page_size: int) -> bool:
     return head_dim in (64, 128) and page_size in (8, 16, 32, 64)
 
@@ -27,7 +30,7 @@ class SharedPlan:
     """What the launches of a step need (csrc/host/shared_plan.hpp): which block of which kernel walks which keys for which tokens, the last position each token sees and its
     pieces, in one int32 tensor."""
 
-    __slots__ = ("requests", "tokens", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strip_blocks", "strip_rows", "tile_blocks", "data", "places", "at")
+    __slots__ = ("requests", "tokens", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strip_blocks", "strip_rows", "tile_blocks", "operand_tiles", "data", "places", "at")
 
 
 def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_heads: int, head_dim: int, *, shared: Sequence[tuple[int, int, int]] = (),
@@ -39,7 +42,7 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     n, length, groups = (host_runtime.ints(values, np.int64) for values in (counts, lengths, shared))
     if n.ndim != 1 or n.shape != length.shape or (len(groups) and groups.shape[1:] != (3,)):
         raise KernelError("plan_shared: a count of queries and a length for each request, and groups as (first request, requests, positions)")
-    lib, sizes = host_runtime.library(), np.empty(15, dtype=np.int64)
+    lib, sizes = host_runtime.library(), np.empty(17, dtype=np.int64)
     errors = {host_runtime.BAD_ARGUMENT: KernelError}
     host_runtime.check(lib.hb_plan_shared(len(n), host_runtime.address(n), host_runtime.address(length), len(groups), host_runtime.address(groups), heads, kv_heads,
                                           sms or sm_count(device), host_runtime.address(sizes)), errors)
@@ -47,9 +50,9 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     host_runtime.check(lib.hb_plan_shared_take(words.data_ptr(), words.numel()), errors)
     plan = SharedPlan()
     plan.requests, plan.heads, plan.kv_heads, plan.head_dim = len(n), heads, kv_heads, head_dim
-    plan.strip_blocks, plan.strip_rows, plan.tile_blocks, plan.tokens, plan.pieces, plan.joined, plan.longest = sizes[1:8].tolist()
+    plan.strip_blocks, plan.strip_rows, plan.tile_blocks, plan.tokens, plan.pieces, plan.joined, plan.longest, plan.operand_tiles = sizes[1:9].tolist()
     plan.data = words.to(device)
-    plan.places = sizes[8:].tolist()  # strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces
+    plan.places = sizes[9:].tolist()  # strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces, operand tiles
     plan.at = [plan.data.data_ptr() + 4 * place for place in plan.places]
     return plan
 
@@ -89,7 +92,7 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
         raise KernelError(f"attention_shared: the output is a bfloat16 [{tokens}, >= {width}] view")
     if tokens == 0:
         return out
-    strip_items, strip_first, tile_items, tile_first, last, starts, own = plan.at
+    strip_items, strip_first, tile_items, tile_first, last, starts, own, operand_list = plan.at
     pieces = sums = 0
     if plan.joined:
         workspace = torch.empty(max(1, plan.pieces * heads * (head_dim + 2)), dtype=torch.float32, device=q.device)
@@ -99,8 +102,14 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     where = (entries, exponents, block_table.data_ptr(), shape[1])
     what = (last, starts, own, pieces, sums, heads, kv_heads, page_size, pages, scale, status_word(q.device).data_ptr(), stream)
     if plan.tile_blocks:
-        check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipppppiiiifpp", head_dim)(
-            q.data_ptr(), q.stride(0), tokens, out_at, out_stride, *where, tile_items, tile_first, plan.tile_blocks, *what), "attention_shared")
+        operands = 0
+        if plan.operand_tiles and exponents:  # several runs of tokens walk the same records: they are made into operands once
+            made = torch.empty(plan.operand_tiles * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16), dtype=torch.uint8, device=q.device)
+            operands = made.data_ptr()
+            check(entry("attention_shared_tiles", "hb_shared_operands", "pppipipiiipp", head_dim)(
+                *where, operand_list, plan.operand_tiles, operands, kv_heads, page_size, pages, status_word(q.device).data_ptr(), stream), "attention_shared")
+        check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipipppppiiiifpp", head_dim)(
+            q.data_ptr(), q.stride(0), tokens, out_at, out_stride, *where, tile_items, tile_first, plan.tile_blocks, operands, plan.operand_tiles, *what), "attention_shared")
     if plan.strip_blocks:
         check(entry("attention_shared", "hb_attention_strips", "pipipppippiipppppiiiifpp", head_dim)(
             q.data_ptr(), q.stride(0), out_at, out_stride, *where, strip_items, strip_first, plan.strip_blocks, plan.strip_rows, *what), "attention_shared")

@@ -12,26 +12,32 @@ OWN = 1 << 30
 def parts_of(plan):
     """(items of strips with their blocks, the same of tiles, last positions, first pieces, first own pieces)"""
     flat, at = plan.data.numpy(), plan.places + [plan.data.numel()]
-    part = [flat[at[i]: at[i + 1]] for i in range(7)]
+    sizes = [at[1], plan.strip_blocks + 1, at[3] - at[2], plan.tile_blocks + 1, plan.tokens, plan.tokens + 1, plan.tokens, 4 * plan.operand_tiles]
+    part = [flat[at[i]: at[i] + n] for i, n in enumerate(sizes)]
+    part[0], part[2] = (items[: 7 * first[-1]] for items, first in ((part[0], part[1]), (part[2], part[3])))
+    assert all(place % 4 == 0 for place in plan.places)
     walks = []
     for items, first in ((part[0], part[1]), (part[2], part[3])):
-        items = items.reshape(-1, 6)
+        items = items.reshape(-1, 7)
         assert first[0] == 0 and first[-1] == len(items) and (np.diff(first) > 0).all()
         walks.append((items, np.repeat(np.arange(len(first) - 1), np.diff(first))))
-    return walks[0], walks[1], part[4], part[5], part[6]
+    return walks[0], walks[1], part[4], part[5], part[6], part[7].reshape(-1, 4)
 
 
 def covered(counts, lengths, heads, kv, groups, sms):
     plan = plan_shared(counts, lengths, heads, kv, 64, shared=groups, device="cpu", sms=sms)
-    strips, tiles, last, starts, own = parts_of(plan)
+    strips, tiles, last, starts, own, operands = parts_of(plan)
     shared = np.zeros(len(counts), dtype=int)
     for first, n, positions in groups:
         shared[first: first + n] = positions
     owner = np.repeat(np.arange(len(counts)), counts)
     seen, pieces = [set() for _ in owner], [[] for _ in owner]
     for rows, (items, _) in ((plan.strip_rows, strips), (256, tiles)):
-        for tok, n, row, low, high, number in items:
+        for tok, n, row, low, high, number, operand in items:
             assert n >= 1 and high > low and n * min(rows, heads // kv) <= rows
+            if rows == 256 and len(operands):  # the item's tiles stand one behind the other among the operands
+                for i, at in enumerate(range(low // 128 * 128, high, 128)):
+                    assert operands[operand + i][0] == row and operands[operand + i][1] == at and operands[operand + i][2] <= low and high <= operands[operand + i][3]
             for t in range(tok, tok + n):
                 assert (low >= shared[row] and row == owner[t]) if number & OWN else (high <= shared[owner[t]] == shared[row])  # another request's table for shared positions only
                 assert not seen[t] & set(range(low, high))
@@ -42,6 +48,7 @@ def covered(counts, lengths, heads, kv, groups, sms):
         assert last[t] == max(-1, lengths[r] - counts[r] + (t - first[r]))
         assert seen[t] == set(range(lengths[r]))
         assert sorted(pieces[t]) == list(range(starts[t], starts[t + 1]))
+    assert plan.operand_tiles == len(operands)
     assert plan.pieces == starts[-1] and plan.joined == any(len(p) != 1 for p in pieces)
     assert (plan.strip_blocks, plan.tile_blocks) == tuple(len(np.unique(b)) for _, b in (strips, tiles))
     return plan
@@ -81,6 +88,12 @@ def test_blocks_have_equal_shares(counts, lengths, groups):
         if len(items):
             keys = np.bincount(block, items[:, 4] - items[:, 3])
             assert keys.max() <= 1.5 * keys.mean() + 256 and len(keys) * 4 <= 3 * 148
+
+
+def test_operands_are_made_where_several_runs_walk_them():
+    assert plan_shared([72], [500], 14, 2, 64, device="cpu", sms=148).operand_tiles == 0  # two runs of 252 rows
+    assert plan_shared([73], [500], 14, 2, 64, device="cpu", sms=148).operand_tiles == 4
+    assert plan_shared([1] * 80, [700] * 80, 14, 2, 64, shared=[(0, 80, 600)], device="cpu", sms=148).operand_tiles == 5
 
 
 def test_short_ranges_stay_whole():
