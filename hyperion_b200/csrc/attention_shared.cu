@@ -143,8 +143,12 @@ struct Shape {
     static constexpr int STAGES = (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
     static constexpr int CHUNKS = D * BYTES / 16;             // 16-byte chunks of a row
     static constexpr int STEPS = 4 / BYTES;                   // products of 16 entries that a chunk a lane feeds
-    static constexpr int JOIN = 2 * ROWS * (D / 2 + 2) * 4;   // where the warps' results meet: of two warps, half of the entries at a time
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * (2 * TILE + EXPS) + (E8 ? WARPS * 3 * KEYS * 4 : 0) + JOIN + 2 * STAGES * 8 + 16;
+    // Where the warps' results meet: COLS entries of every row at a time, a row's LINE floats apart (lanes that store side by side then take different banks), over the
+    // keys' factors, which nobody wants any more by then.
+    static constexpr int COLS = 64 / NQ, LINE = COLS + 4;
+    static constexpr int JOIN = WARPS * ROWS * LINE * 4, FACTORS = E8 ? WARPS * 3 * KEYS * 4 : 0;
+    static_assert(FACTORS <= JOIN, "the factors lie where the results meet");
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * (2 * TILE + EXPS) + JOIN + 2 * WARPS * ROWS * 4 + 2 * STAGES * 8 + 16;
     static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "an SM's shared memory");
     // 16-byte chunk cc of row `key` as TMA's swizzle has placed it: the panel's row of 128 bytes (of 64, in pairs) with its chunks permuted.
     static __device__ __forceinline__ int at(int key, int cc) {
@@ -166,6 +170,7 @@ struct Args {
     float* pieces;           // [pieces, heads, D], or null: rows have one piece each and are stored at once
     float2* sums;            // [pieces, heads]: (m, l)
     int heads, kv_heads, page_size, pages;
+    int beside_tiles;        // the tile kernel of the same step was launched right before
     int gc, chunks;          // heads of a strip, strips of a key/value head's group
     float scale_log2;
     int* status;
@@ -180,8 +185,10 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
     // the tiles of all stages, the exponents of all stages, and each warp's keys' factors
     unsigned char* exps = ring + (size_t)S::STAGES * 2 * S::TILE;
     float* factors = reinterpret_cast<float*>(exps + (size_t)S::STAGES * S::EXPS);
-    float* join = factors + (E8 ? WARPS * 3 * S::KEYS : 0);
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(join + S::JOIN / 4);
+    float* join = factors;  // [WARPS][ROWS][LINE]
+    float* tops = join + S::JOIN / 4;  // [WARPS][ROWS]: maxima
+    float* parts = tops + WARPS * ROWS;  // [WARPS][ROWS]: sums
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(parts + WARPS * ROWS);
     unsigned long long* empty = full + S::STAGES;
     volatile int* failed = reinterpret_cast<volatile int*>(empty + S::STAGES);
     volatile int* lost = failed + 1;  // a computing warp has given up
@@ -194,7 +201,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
     }
     __syncthreads();
     let_next_kernel_start();
-    wait_for_previous_kernels();
+    // Behind the tile kernel of the same step, whose blocks let this one start only when all kernels before it had finished, there is nothing to wait for here: its pieces
+    // are others, and the two share the device.  (Whoever comes next waits for this kernel, and this one for that at its end.)
+    if (!a.beside_tiles) wait_for_previous_kernels();
     const int kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
     const int group = a.heads / a.kv_heads, first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
     const int first_item = a.first_item[blockIdx.x], end_item = a.first_item[blockIdx.x + 1];
@@ -261,10 +270,40 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
     const int t = lane & 3, g = lane >> 2;
     [[maybe_unused]] float* mine = factors + warp * 3 * KEYS;  // of this warp's keys: 2^e of the key, e of the value, 2^-e of the value
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); };
-    for (int index = first_item; index < end_item; ++index) {
+    constexpr int LANES_PER_ROW = S::COLS / 16;
+    const int store_row = lane / LANES_PER_ROW, store_col = warp * (S::COLS / 4) + lane % LANES_PER_ROW * 4;  // what this lane stores of every COLS entries
+    struct Words { int tok0, ntok, key_lo, key_hi, piece; };
+    auto words_of = [&](int index) {
         const int* item = a.items + (size_t)index * ITEM_WORDS;
-        const int tok0 = item[0], ntok = item[1], key_lo = item[3], key_hi = item[4], piece = item[5];
+        return Words{item[0], item[1], item[3], item[4], item[5]};
+    };
+    // An item's queries are on their way while the item before it is put together (of eight rows; sixteen have no registers for it).
+    uint4 raw[NQ][D / 32];  // of rows q * 8 + g: this lane's quarter, chunks t, t + 4, ...
+    int sees[NQ];
+    auto fetch_queries = [&](const Words& w) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const int v = q * 8 + g, tok = v / a.gc, hh = v - tok * a.gc;
+            const bool valid = tok < w.ntok && hh < heads_here;
+            const bf16* src = a.q + (size_t)(w.tok0 + (valid ? tok : 0)) * a.q_stride + (size_t)(first_head + (valid ? hh : 0)) * D;
+            constexpr int PER_CHUNK = 16 / S::BYTES, PIECES = PER_CHUNK / 8;  // entries of a chunk; 16-byte pieces of them in bfloat16
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) raw[q][i] = valid ? *reinterpret_cast<const uint4*>(src + (t + 4 * (i / PIECES)) * PER_CHUNK + (i % PIECES) * 8) : make_uint4(0, 0, 0, 0);
+            sees[q] = valid ? a.last[w.tok0 + tok] : 0x7fffffff;
+        }
+    };
+    Words next = words_of(first_item);
+    if (NQ == 1) fetch_queries(next);
+    for (int index = first_item; index < end_item; ++index) {
+        const int tok0 = next.tok0, ntok = next.ntok, key_lo = next.key_lo, key_hi = next.key_hi, piece = next.piece;
         const int start = key_lo / BN * BN, n_tiles = (key_hi - start + BN - 1) / BN;
+        if (NQ != 1) fetch_queries(next);
+        if (index + 1 < end_item) next = words_of(index + 1);
+        // where this lane stores
+        const int store_tok = store_row / a.gc, store_head = store_row - store_tok * a.gc;
+        const bool stores = store_tok < ntok && store_head < heads_here;
+        int piece_at = 0;
+        if (stores && a.pieces) piece_at = (piece & OWN_PIECE ? a.own_start : a.piece_start)[tok0 + store_tok] + (piece & (OWN_PIECE - 1));
         // Q's fragments: a lane's 16-byte chunk t + 4 j of a key feeds products STEPS j to STEPS j + STEPS - 1, four of its entries each, so a query's entries stand
         // in the fragments likewise.
         unsigned qf[NQ][D / 16][2];
@@ -273,16 +312,15 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
         int sees_all_to = key_hi - 1;
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            const int v = q * 8 + g, tok = v / a.gc, hh = v - tok * a.gc;
-            const bool valid = tok < ntok && hh < heads_here;
-            const int mine_sees = valid ? min(key_hi - 1, a.last[tok0 + tok]) : key_hi - 1;
-            const bf16* src = a.q + (size_t)(tok0 + (valid ? tok : 0)) * a.q_stride + (size_t)(first_head + (valid ? hh : 0)) * D;
-            constexpr int PER_CHUNK = 16 / S::BYTES, PIECES = PER_CHUNK / 8;  // entries of a chunk; 16-byte pieces of them in bfloat16
-            uint4 raw[D / 32];  // this lane's quarter of the row: chunks t, t + 4, ...
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i)
-                raw[i] = valid ? *reinterpret_cast<const uint4*>(src + (t + 4 * (i / PIECES)) * PER_CHUNK + (i % PIECES) * 8) : make_uint4(0, 0, 0, 0);
-            const unsigned* words = reinterpret_cast<const unsigned*>(raw);
+            const int mine_sees = min(key_hi - 1, sees[q]);
+            const unsigned words[D / 8] = {
+#define HB_WORDS(i) raw[q][i].x, raw[q][i].y, raw[q][i].z, raw[q][i].w
+                HB_WORDS(0), HB_WORDS(1),
+#if HB_HEAD_DIM == 128
+                HB_WORDS(2), HB_WORDS(3),
+#endif
+#undef HB_WORDS
+            };
             float factor = 1.f, scale = a.scale_log2;
             if constexpr (E8) {
                 // As float16 with the row's largest entry between 2^13 and 2^14: an entry of eight bits keeps them all down to 2^-27 of the largest.
@@ -502,9 +540,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[s]);
         }
-        // The warps' results meet: every warp brings its sums to the largest maximum, then 2 and 3 hand theirs to 0 and 1, and 1 to 0, lane by lane, half of the
-        // entries at a time.  Warp 0 stores.
-        float* tops = join + 2 * ROWS * (D / 2);  // [WARPS][ROWS]
+        if (NQ == 1 && index + 1 < end_item) fetch_queries(next);
+        // The warps' results meet: every warp brings its sums to the largest maximum and lays COLS entries of its rows down, then takes a quarter of them, adds up the four
+        // warps' in their order, and stores.
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -512,90 +550,67 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                 l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 4);
                 l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 8);
                 l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 16);
-                if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e];
+                if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e], parts[warp * ROWS + q * 8 + 2 * t + e] = l[q][e];
             }
         meet();
         if (*lost) return;  // all four warps see the same: they set it before they come here only
+        float f[NQ][2];
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = q * 8 + 2 * t + e;
-                float top = tops[row];
-#pragma unroll
-                for (int w = 1; w < WARPS; ++w) top = fmaxf(top, tops[w * ROWS + row]);
-                const float f = m[q][e] == -INFINITY ? 0.f : fast_exp2(m[q][e] - top);
-                m[q][e] = top;
-                l[q][e] *= f;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) o[q][i][e] *= f, o[q][i][2 + e] *= f;
+                const float top = fmaxf(fmaxf(tops[row], tops[ROWS + row]), fmaxf(tops[2 * ROWS + row], tops[3 * ROWS + row]));
+                f[q][e] = m[q][e] == -INFINITY ? 0.f : fast_exp2(m[q][e] - top);
             }
-        meet();
+        float top = -INFINITY, total = 0.f;  // of the row that this lane stores
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, tops[w * ROWS + store_row]);
 #pragma unroll
-            for (int step = 2; step > 0; step >>= 1) {
-                float4* mine_o = reinterpret_cast<float4*>(join) + (warp & (step - 1)) * (NQ * (D / 32) * 32) + lane;
-                float2* mine_l = reinterpret_cast<float2*>(tops) + (warp & (step - 1)) * NQ * 4 + t;
-                if (warp >= step && warp < 2 * step) {
+        for (int w = 0; w < WARPS; ++w) {
+            const float mw = tops[w * ROWS + store_row];
+            total = fmaf(mw == -INFINITY ? 0.f : fast_exp2(mw - top), parts[w * ROWS + store_row], total);
+        }
+        const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);  // a row that sees nothing is zeros; a NaN stays one
+        const size_t slot = (size_t)piece_at * a.heads + first_head + store_head;
+        if (stores && a.pieces && store_col == 0) a.sums[slot] = make_float2(top, total);
 #pragma unroll
-                    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-                        for (int i = 0; i < D / 32; ++i) mine_o[(q * (D / 32) + i) * 32] = make_float4(o[q][half * (D / 32) + i][0], o[q][half * (D / 32) + i][1], o[q][half * (D / 32) + i][2], o[q][half * (D / 32) + i][3]);
-                        if (half == 0 && g == 0) mine_l[q * 4] = make_float2(l[q][0], l[q][1]);
-                    }
-                }
-                meet();
-                if (warp < step) {
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
-                            const float4 more = mine_o[(q * (D / 32) + i) * 32];
-                            float (&into)[4] = o[q][half * (D / 32) + i];
-                            into[0] += more.x, into[1] += more.y, into[2] += more.z, into[3] += more.w;
-                        }
-                        if (half == 0) {
-                            const float2 more = mine_l[q * 4];
-                            l[q][0] += more.x, l[q][1] += more.y;
-                        }
-                    }
-                }
-                meet();
-            }
-        if (warp == 0) {
+        for (int col = 0; col < D; col += S::COLS) {
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int v = q * 8 + 2 * t + e, tok = v / a.gc, hh = v - tok * a.gc;
-                    if (tok >= ntok || hh >= heads_here) continue;
-                    const int token = tok0 + tok, head = first_head + hh;
-                    if (a.pieces) {
-                        const size_t slot = (size_t)((piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (piece & (OWN_PIECE - 1))) * a.heads + head;
-                        float* dst = a.pieces + slot * D;
-                        if (g == 0) a.sums[slot] = make_float2(m[q][e], l[q][e]);
+                    float* dst = join + (warp * ROWS + q * 8 + 2 * t + e) * S::LINE;
 #pragma unroll
-                        for (int i = 0; i < D / 16; ++i) {
-                            if constexpr (E8) *reinterpret_cast<float2*>(dst + 16 * i + 2 * g) = make_float2(o[q][i][e], o[q][i][2 + e]);
-                            else dst[16 * i + g] = o[q][i][e], dst[16 * i + 8 + g] = o[q][i][2 + e];
-                        }
-                    } else {
-                        const float inv = l[q][e] > 0.f ? 1.f / l[q][e] : (l[q][e] == 0.f ? 0.f : l[q][e]);  // a row that sees nothing is zeros; a NaN stays one
-                        bf16* dst = a.out + (size_t)token * a.out_stride + (size_t)head * D;
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i) {
-                            if constexpr (E8) {
-                                *reinterpret_cast<__nv_bfloat162*>(dst + 16 * i + 2 * g) = __floats2bfloat162_rn(o[q][i][e] * inv, o[q][i][2 + e] * inv);
-                            } else {
-                                dst[16 * i + g] = __float2bfloat16_rn(o[q][i][e] * inv);
-                                dst[16 * i + 8 + g] = __float2bfloat16_rn(o[q][i][2 + e] * inv);
-                            }
-                        }
+                    for (int i = 0; i < S::COLS / 16; ++i) {
+                        const float x = o[q][col / 16 + i][e] * f[q][e], y = o[q][col / 16 + i][2 + e] * f[q][e];
+                        if constexpr (E8) *reinterpret_cast<float2*>(dst + 16 * i + 2 * g) = make_float2(x, y);
+                        else dst[16 * i + g] = x, dst[16 * i + 8 + g] = y;
                     }
                 }
+            meet();
+            if (stores) {
+                float sum[4];
+                load4(join + store_row * S::LINE + store_col, sum);
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) {
+                    float more[4];
+                    load4(join + (w * ROWS + store_row) * S::LINE + store_col, more);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] += more[i];
+                }
+                if (a.pieces) {
+                    store4(a.pieces + slot * D + col + store_col, sum);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] *= inv;
+                    store4(a.out + (size_t)(tok0 + store_tok) * a.out_stride + (size_t)(first_head + store_head) * D + col + store_col, sum);
+                }
+            }
+            meet();
         }
     }
+    if (a.beside_tiles) wait_for_previous_kernels();
 }
 
 template <int N>
@@ -608,32 +623,41 @@ __device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
     }
 }
 
-// A warp puts a (token, head)'s pieces together.
+// Puts the pieces of a (token, head) together: TEAM warps take every TEAM-th AHEAD of them, which are on their way together, and meet in shared memory.  One warp where a
+// token has few; a long context cut over the whole device leaves a hundred, which one warp would walk a latency at a time (one token at 32,768 positions: 111 pieces of 28
+// heads).
 constexpr int MERGE_WARPS = 4;
+template <int TEAM>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) attention_pieces_kernel(const float* __restrict__ pieces, const float2* __restrict__ sums, const int* __restrict__ piece_start,
                                                                             bf16* __restrict__ out, int out_stride, int heads) {
-    constexpr int PER = D / 32, AHEAD = 8;
+    constexpr int PER = D / 32, AHEAD = 8, HEADS = MERGE_WARPS / TEAM;
+    __shared__ float2 tops[MERGE_WARPS];
+    __shared__ __align__(16) float values[MERGE_WARPS][D];
     let_next_kernel_start();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM;
+    const int token = blockIdx.x, head = blockIdx.y * HEADS + warp / TEAM;
+    const int first = piece_start[token], n = head < heads ? piece_start[token + 1] - first : 0;  // written with the plan, long before
     wait_for_previous_kernels();
-    const int token = blockIdx.x, head = blockIdx.y * MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (head >= heads) return;
-    const int first = piece_start[token], n = piece_start[token + 1] - first;
     float top = -INFINITY, total = 0.f, value[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) value[i] = 0.f;
-    for (int p = lane; p < n; p += 32) top = fmaxf(top, sums[(size_t)(first + p) * heads + head].x);
-    top = warp_max(top);
-    for (int p0 = 0; p0 < n; p0 += AHEAD) {  // AHEAD pieces are on their way together
+    for (int p0 = member * AHEAD; p0 < n; p0 += AHEAD * TEAM) {
         float part[AHEAD][PER];
         float2 ml[AHEAD];
+        float above = top;
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            if (p0 + k >= n) break;
-            const size_t slot = (size_t)(first + p0 + k) * heads + head;
+            const size_t slot = (size_t)(first + min(p0 + k, n - 1)) * heads + head;
             ml[k] = sums[slot];
-            const float* src = pieces + slot * D + lane * PER;
-            load_floats(src, part[k]);
+            load_floats(pieces + slot * D + lane * PER, part[k]);
         }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) above = p0 + k < n ? fmaxf(above, ml[k].x) : above;
+        const float down = top == -INFINITY ? 0.f : fast_exp2(top - above);
+        total *= down;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) value[i] *= down;
+        top = above;
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             if (p0 + k >= n) break;
@@ -643,6 +667,28 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) attention_pieces_kernel(cons
             for (int i = 0; i < PER; ++i) value[i] = fmaf(f, part[k][i], value[i]);
         }
     }
+    if constexpr (TEAM > 1) {
+        if (lane == 0) tops[warp] = make_float2(top, total);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) values[warp][lane * PER + i] = value[i];
+        __syncthreads();
+        if (member != 0) return;
+        float above = top;
+#pragma unroll
+        for (int w = 1; w < TEAM; ++w) above = fmaxf(above, tops[warp + w].x);
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) value[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < TEAM; ++w) {
+            const float2 theirs = tops[warp + w];
+            const float f = theirs.x == -INFINITY ? 0.f : fast_exp2(theirs.x - above);
+            total = fmaf(f, theirs.y, total);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) value[i] = fmaf(f, values[warp + w][lane * PER + i], value[i]);
+        }
+    }
+    if (head >= heads) return;
     const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
     bf16* dst = out + (size_t)token * out_stride + (size_t)head * D + lane * PER;
 #pragma unroll
@@ -689,9 +735,10 @@ int launch_strips(const Args& a, const void* cache, int blocks, cudaStream_t str
 }  // namespace
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
+// beside_tiles: hb_attention_shared_tiles for the same step was the launch right before on this stream.
 // items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row.
 HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
-                                  const int* items, const int* first_item, int blocks, int rows, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
+                                  const int* items, const int* first_item, int blocks, int rows, int beside_tiles, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
                                   int page_size, int pages, float scale, int* status, cudaStream_t stream) {
     if (blocks <= 0) return 0;
     if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
@@ -703,16 +750,18 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     const int group = heads / kv_heads, gc = group < rows ? group : rows, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
-                 heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
+                 heads, kv_heads, page_size, pages, beside_tiles, gc, chunks, scale * 1.4426950408889634f, status};
     if (rows == 8) return exponents ? launch_strips<true, 1>(a, cache, blocks, stream) : launch_strips<false, 1>(a, cache, blocks, stream);
     return exponents ? launch_strips<true, 2>(a, cache, blocks, stream) : launch_strips<false, 2>(a, cache, blocks, stream);
 }
 
-// Puts the pieces [piece_start[tokens], heads, D] of every token together.  A token without a piece is zeros.
-HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const int* piece_start, void* out, int out_stride, int tokens, int heads, cudaStream_t stream) {
+// Puts the n_pieces = piece_start[tokens] pieces [n_pieces, heads, D] of the tokens together.  A token without a piece is zeros.
+HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const int* piece_start, void* out, int out_stride, int tokens, int n_pieces, int heads, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (!pieces || !sums || !piece_start || !out || heads <= 0 || out_stride % 2 || ((uintptr_t)pieces & 15) || ((uintptr_t)out & 3)) return HB_BAD_ARGUMENT;
-    const int rows = (heads + MERGE_WARPS - 1) / MERGE_WARPS;
+    const bool many = n_pieces / tokens > 12;
+    const int per_block = many ? 1 : MERGE_WARPS, rows = (heads + per_block - 1) / per_block;
     if (rows > 65535) return HB_UNSUPPORTED_SIZE;
-    return launch_after_previous(attention_pieces_kernel, dim3(tokens, rows), dim3(32 * MERGE_WARPS), 0, stream, pieces, (const float2*)sums, piece_start, (bf16*)out, out_stride, heads);
+    return launch_after_previous(many ? attention_pieces_kernel<MERGE_WARPS> : attention_pieces_kernel<1>, dim3(tokens, rows), dim3(32 * MERGE_WARPS), 0, stream, pieces, (const float2*)sums,
+                                 piece_start, (bf16*)out, out_stride, heads);
 }

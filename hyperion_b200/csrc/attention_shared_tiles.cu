@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
     }
     // rows of Q that no copy writes (beyond tokens x heads of an item) are computed like the others and never stored
     for (int e = tid; e < S::Q_BYTES / 16; e += S::THREADS) reinterpret_cast<uint4*>(qs)[e] = make_uint4(0, 0, 0, 0);
-    let_next_kernel_start();
     wait_for_previous_kernels();
+    let_next_kernel_start();  // only now: the strip kernel of the same step takes its start as the sign that all that came before has finished
     // All of the SM's tensor memory, and only now: a block of a kernel further back in the stream that has yet to start on this SM can no longer want any.
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");

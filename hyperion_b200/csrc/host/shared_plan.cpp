@@ -134,10 +134,21 @@ SharedPlan plan_shared(const std::vector<int64_t>& counts, const std::vector<int
                     runs.push_back({range.token + at, std::min(per, range.count - at), range.row, range.low, range.high, range.own, range.operand});
         return runs;
     };
-    const auto blocks_for = [&](int64_t rows, int64_t slots) { return std::max<int64_t>(1, slots / (kv_heads * ((group + rows - 1) / rows))); };
-    // Three blocks of strips of eight rows share an SM, two of sixteen; one of tiles has it to itself.
-    plan.strips = cut(runs_of(false, plan.strip_rows), blocks_for(plan.strip_rows, sms * (plan.strip_rows == 8 ? 3 : 2)), 0.75, 2, 4);
-    plan.tiles = cut(runs_of(true, TILE_ROWS), blocks_for(TILE_ROWS, sms), 1.5, 2, 2);
+    const std::vector<Run> strips = runs_of(false, plan.strip_rows), tiles = runs_of(true, TILE_ROWS);
+    const int64_t strips_across = kv_heads * ((group + plan.strip_rows - 1) / plan.strip_rows), tiles_across = kv_heads * ((group + TILE_ROWS - 1) / TILE_ROWS);
+    // Where a step has both kinds they run side by side, each on a part of the device that its work asks for.  A tile of 256 rows takes an SM some 2.3 us and an item of them 4
+    // besides, a tile of a strip 0.65 (three blocks share the SM) and a strip 1.3.
+    int64_t tile_sms = tiles.empty() ? 0 : sms;
+    if (!tiles.empty() && !strips.empty()) {
+        double tile_work = 0, strip_work = 0;
+        for (const Run& run : tiles) tile_work += (2.3 * (double)tiles_of(run) + 4) * (double)tiles_across;
+        for (const Run& run : strips) strip_work += (0.65 * (double)tiles_of(run) + 1.3) * (double)strips_across;
+        tile_sms = std::max<int64_t>(1, std::min<int64_t>(sms - 1, (int64_t)((double)sms * tile_work / (tile_work + strip_work) + 0.5)));
+        tile_sms = std::min(sms, std::max<int64_t>(1, (tile_sms + tiles_across / 2) / tiles_across) * tiles_across);
+    }
+    const int64_t strip_sms = tile_sms < sms ? sms - tile_sms : sms;  // what is left, or all of it one after the other
+    plan.strips = cut(strips, std::max<int64_t>(1, strip_sms * (plan.strip_rows == 8 ? 3 : 2) / strips_across), 0.75, 2, 4);
+    plan.tiles = cut(tiles, std::max<int64_t>(1, tile_sms / tiles_across), 1.5, 2, 2);
 
     std::vector<int> of_group(tokens, 0), of_own(tokens, 0);
     for (const Walk* walk : {&plan.strips, &plan.tiles})
