@@ -75,7 +75,7 @@ def cache8_load(cache: Cache8, block_table: torch.Tensor, token_row: torch.Tenso
     pages, kv_heads, page_size, head_dim = check_cache8(cache, "cache8_load")
     tokens, table_width = _check_places(block_table, token_row, positions, "cache8_load")
     if out is None:
-        out = torch.empty((tokens, 2, kv_heads, head_dim), dtype=dtype, device=cache[0].device)
+        out = torch.empty(tokens, 2, kv_heads, head_dim, dtype=dtype, device=cache[0].device)
     elif out.shape != (tokens, 2, kv_heads, head_dim) or out.dtype != dtype or not out.is_contiguous() or not out.is_cuda:
         raise KernelError(f"cache8_load: the output is a dense {dtype} tensor [tokens, 2, kv_heads, d]")
     check(entry("cache8", "hb_cache8_load", "pppipppiiiiiipp")(

@@ -16,7 +16,7 @@ import torch
 from .. import host as host_runtime
 from .basic import status_word
 from .cache8 import Cache8, check_cache8
-from .native import KernelError, check, entry, require_cuda, sm_count, stream_address
+from .native import KernelError, check, entry, require_cuda, scratch, sm_count, stream_address
 
 
 TILE_KEYS = 128  # keys of an operand tile
@@ -87,25 +87,26 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     if not (q.is_cuda and block_table.is_cuda):
         require_cuda(q, block_table)
     if out is None:
-        out = torch.empty((tokens, width), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty(tokens, width, dtype=torch.bfloat16, device=q.device)
     elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != tokens or out.shape[1] < width or out.stride(1) != 1 or not out.is_cuda:
         raise KernelError(f"attention_shared: the output is a bfloat16 [{tokens}, >= {width}] view")
     if tokens == 0:
         return out
     strip_items, strip_first, tile_items, tile_first, last, starts, own, operand_list = plan.at
-    pieces = sums = 0
-    if plan.joined:
-        workspace = torch.empty(max(1, plan.pieces * heads * (head_dim + 2)), dtype=torch.float32, device=q.device)
-        pieces = workspace.data_ptr()
-        sums = pieces + 4 * plan.pieces * heads * head_dim
     out_at, out_stride, stream = out.data_ptr(), out.stride(0), stream_address()
+    pieces = sums = operands = 0
+    if plan.joined or plan.operand_tiles:
+        for_pieces = (plan.pieces * heads * (head_dim + 2) * 4 + 511) // 512 * 512 if plan.joined else 0
+        makes = plan.operand_tiles if exponents else 0  # several runs of tokens walk the same records: they are made into operands once
+        memory, owner = scratch(q.device, stream, for_pieces + makes * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16))
+        if plan.joined:
+            pieces, sums = memory, memory + 4 * plan.pieces * heads * head_dim
+        if makes:
+            operands = memory + for_pieces
     where = (entries, exponents, block_table.data_ptr(), shape[1])
     what = (last, starts, own, pieces, sums, heads, kv_heads, page_size, pages, scale, status_word(q.device).data_ptr(), stream)
     if plan.tile_blocks:
-        operands = 0
-        if plan.operand_tiles and exponents:  # several runs of tokens walk the same records: they are made into operands once
-            made = torch.empty(plan.operand_tiles * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16), dtype=torch.uint8, device=q.device)
-            operands = made.data_ptr()
+        if operands:
             check(entry("attention_shared_tiles", "hb_shared_operands", "pppipipiiipp", head_dim)(
                 *where, operand_list, plan.operand_tiles, operands, kv_heads, page_size, pages, status_word(q.device).data_ptr(), stream), "attention_shared")
         check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipipppppiiiifpp", head_dim)(
