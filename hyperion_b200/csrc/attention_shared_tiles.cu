@@ -4,21 +4,25 @@
 // An item is up to 256 (token, head) rows of one key/value head and a range of keys: all of a group's tokens over a share of the positions that they
 // hold in common, or a portion of a prompt over its own.  One block per SM holds all of the SM's tensor memory and takes its share of the items; two
 // halves of 128 rows (H and L) walk the same tiles of 128 keys, so that the tensor core runs one half's products under the other half's softmax:
-//   warp 0       fetches: one cp.async.bulk.tensor per page (and 128-byte panel) of K and of V, the queries as one 3-D box per 64-column panel;
+//   warp 0       fetches: over bfloat16 caches one cp.async.bulk.tensor per page and 64-column panel of K and of V, over operands one plain copy of each, and the queries as
+//                one 3-D box per panel;
 //   warp 1       issues S_x = Q_x K^T (M 128, N 128) and O_x += P_x V (P from tensor memory, V MN-major), each half's next S right behind its last product;
-//   warps 4-11   softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by much;
-//   warps 12-19  8-bit records that one run of tokens walks: four warps turn each K tile into bfloat16 (which holds code * 2^e exactly) in the swizzled layout that the products
-//                read, four each V tile; the records' bytes come once from memory.  (Records that several runs walk are made into operands beforehand, for all of them.)
+//   warps 4-11   softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by much.
+// 8-bit records are made into operands before (shared_operands_kernel).
+//
 // Over bfloat16 values, weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as
 // much as its own rounding does.  8-bit values go as float16, which holds code * 2^(e - e0) exactly for exponents from e0 - 12 to e0 + 7 (e0: the largest of
-// the item's first tile; the result is scaled back at the end), and so do the weights, whose rounding then does not show and whose second part is not
-// needed.  A tile with exponents beyond that range goes the way of bfloat16 values.
-// A row of S is 128 float columns of tensor memory and the two parts of its P are 2 x 64, so P takes exactly the place of the S it was made from, 32 keys at a
-// time; the softmax reads S twice (for the maximum, then for the weights), 32 columns under way while it works on 32, which lets 20 warps share the register
-// file.  P is handed over in two halves of the tile's keys, so that the product of the first runs under the making of the second.
+// the range's first tile; the result is scaled back at the end), and so do the weights, whose rounding then does not show and whose second part is not
+// needed.  A tile with exponents beyond that range goes the way of bfloat16 values.  A row of S is 128 float columns of tensor memory and the two parts of its P are
+// 2 x 64, so P takes exactly the place of the S it was made from, 32 keys at a time; the softmax reads S twice (for the maximum, then for the weights), 32 columns under way
+// while it works on 32.  P is handed over in two halves of the tile's keys, so that the product of the first runs under the making of the second.
+// What bounds it is the chain of a half: from the arrival of S 2,500 clocks until the last weights are handed over (of which 1,024 are the special function unit's for 128 columns,
+// which the other half's want as well), then 1,050 for the rest of O += P V, the next S and its arrival.  3,600 clocks a tile, of which the tensor core is busy for 2,048;
+// 4,000 over bfloat16, 3,072.  Tried and dropped: weights by the maximum so far with one reading of S (3,150 clocks as long as no maximum is outgrown, 5,000 when one of 256 rows'
+// is, and one often is); a part of the exponentials by a polynomial (no faster); two threads a row (4,700); an issuer for each half (the halves fall into step: 4,700).
 //
-// Slots beyond an item's range may hold anything: their scores are replaced, and their values are zeros before a product reads them (the warps that convert write
-// them so; over bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded; a wait that runs out sets
+// Slots beyond an item's range may hold anything: their scores are replaced, and their values are zeros before a product reads them (operands are made so; over
+// bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded; a wait that runs out sets
 // HB_STATUS_WAIT_EXPIRED, all roles leave their loops, tensor memory is freed and the block returns.
 #include <cuda.h>
 
@@ -39,13 +43,12 @@ constexpr int PANELS = D / 64;
 constexpr int KV_PANEL = BN * 64;             // elements of a 128-key x 64-column panel (16 KB)
 constexpr int Q_PANEL = ROWS * 64;            // elements of a 256-row x 64-column panel of Q (32 KB)
 constexpr int TILE_BYTES = PANELS * KV_PANEL * 2;
-constexpr int RAW_BYTES = BN * D;             // a tile of codes
-constexpr int STAGES = 2;                     // of K tiles and of V tiles as the products read them; one tile of codes of each is under way
+constexpr int STAGES = 2;                     // of K tiles and of V tiles
 constexpr int TMEM_COLS = 512;                // S_H [0,128) S_L [128,256) O_H [256,256+D) O_L [384,384+D); P_x over S_x
 constexpr int O_COL = 256;
 constexpr int ITEM_WORDS = 7;                 // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of its own positions), first operand tile
 constexpr int OWN_PIECE = 1 << 30;
-enum Source : int { BFLOAT16 = 0, CODES = 1, OPERANDS = 2 };  // what the tiles come from: a bfloat16 cache, an 8-bit one, or operands made of one beforehand
+enum Source : int { BFLOAT16 = 0, OPERANDS = 1 };  // what the tiles come from: a bfloat16 cache, or operands made of an 8-bit one
 constexpr int LOWEST = -12, HIGHEST = 7;       // of e - e0, for values as float16
 constexpr unsigned WAIT_LIMIT = 1u << 24;
 
@@ -160,16 +163,6 @@ __device__ __forceinline__ void umma_commit_at(unsigned bar_addr) {
 __device__ __forceinline__ unsigned idesc_for(int n, bool b_mn, bool f16) {
     return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(BM >> 4) << 24);
 }
-__device__ __forceinline__ void tmem_ld16(unsigned taddr, float (&v)[16]) {
-    unsigned r[16];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
 // 32 consecutive columns of this thread's lane, on their way; arrived() says that they are there, and nothing that reads them can stand before it.
 __device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -185,7 +178,7 @@ __device__ __forceinline__ void tmem_st32(unsigned taddr, const unsigned (&r)[32
                  :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
                  : "memory");
 }
-// 2^x by the hardware approximation (inputs are <= 8 here; -inf gives 0).
+// 2^x by the hardware approximation (inputs are <= OUTGROWN; -inf gives 0).
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -219,9 +212,14 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+__device__ __forceinline__ bool elected() {  // one lane of the warp, all of which are here
+    unsigned one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ void tmem_st16_words(unsigned taddr, const unsigned (&v)[16]) {
@@ -237,7 +235,6 @@ __device__ __forceinline__ float value_of_half(unsigned short h) {
 }
 
 struct Args {
-    const signed char* exponents;  // of an 8-bit cache
     const unsigned char* operands; const int* kinds;  // [tiles, kv_heads, 2, TILE_BYTES]; [tiles, kv_heads]: 2 * (e0 + 64) + whether the values are float16
     bf16* out; int out_stride;
     const int* block_table; int table_width;
@@ -254,22 +251,19 @@ struct Args {
     int* status;
 };
 
+// How far (in powers of two) a maximum may be outgrown before the row is rescaled.  A stale maximum changes no result (numerator and denominator use the same
+// one) as long as nothing overflows: weights are float16, whose largest is
+// just below 2^16, or bfloat16; their sums are float.  A row that outgrows its own makes its half of the tile wait while O is scaled.
 template <Source FROM>
-struct Shape {
-    static constexpr bool E8 = FROM == CODES;
-    static constexpr int WARPS = E8 ? 20 : 12, THREADS = 32 * WARPS;
-    // Registers a thread, by groups of four warps, of the 96 that 640 threads are launched with (128 * 56 + 256 * 152 + 256 * 56 = 60,416 of 61,440)
-    enum : int { FEW = 56, MANY = 152, CONVERTING = 56 };
-    static constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
-    // How far (in powers of two) a maximum may be outgrown before the row is rescaled.  A stale maximum changes no result (numerator and denominator use the same
-    // one) as long as nothing overflows: weights are float16 up to 2^15, or bfloat16 and their sums float.
-    static constexpr float OUTGROWN = FROM != BFLOAT16 ? 13.f : 32.f;
-    static constexpr int RAW = E8 ? 2 * RAW_BYTES + 2 * BN : 0;  // codes of K and of V, and their exponents
-    static constexpr size_t USED = 1024 + (size_t)Q_BYTES + (size_t)2 * STAGES * TILE_BYTES + RAW + 256;
-    // more than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory
-    static constexpr size_t SMEM = USED > 120 * 1024 ? USED : 120 * 1024;
-    static_assert(USED <= 227 * 1024, "an SM's shared memory");
-};
+constexpr float OUTGROWN = FROM == OPERANDS ? 15.5f : 32.f;
+
+constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
+constexpr int THREADS = 32 * 12;
+constexpr int DESK = 32 * 32;                 // floats a softmax warp has in shared memory for 32 columns of its rows on their way out
+constexpr size_t SMEM_USED = 1024 + (size_t)Q_BYTES + (size_t)2 * STAGES * TILE_BYTES + 8 * DESK * 4 + 256;
+static_assert(SMEM_USED <= 227 * 1024, "an SM's shared memory");
+// more than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory
+constexpr size_t SMEM_BYTES = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;
 
 // Sixteen codes times 2^e as operands: float16 (-12 <= e <= 7) or bfloat16.
 template <bool HALVES>
@@ -295,65 +289,55 @@ __device__ __forceinline__ void widen(const uint4& codes, int e, unsigned (&wide
     }
 }
 
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
-
 struct Item {
     int tok0, ntok, key_lo, key_hi, piece, operand, start, n_tiles, halves;
     const int* table;
 };
 
 template <Source FROM>
-__global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
-    typedef Shape<FROM> S;
-    constexpr bool E8 = S::E8;
+__global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* k_ring = base;
     unsigned char* v_ring = k_ring + (size_t)STAGES * TILE_BYTES;
     unsigned char* qs = v_ring + (size_t)STAGES * TILE_BYTES;
-    unsigned char* raw_tiles = qs + S::Q_BYTES;              // [K, V] codes
-    unsigned char* exps = raw_tiles + (E8 ? 2 * RAW_BYTES : 0);  // [K, V][BN]
-    unsigned long long* k_full = reinterpret_cast<unsigned long long*>(exps + (E8 ? 2 * BN : 0));
+    float* desks = reinterpret_cast<float*>(qs + Q_BYTES);  // [8][DESK]
+    unsigned long long* k_full = reinterpret_cast<unsigned long long*>(desks + 8 * DESK);
     unsigned long long* k_empty = k_full + 2;
     unsigned long long* v_full = k_empty + 2;
     unsigned long long* v_empty = v_full + 2;
-    unsigned long long* raw_full = v_empty + 2;    // [K, V]
-    unsigned long long* raw_empty = raw_full + 2;  // [K, V]
-    unsigned long long* s_full = raw_empty + 2;    // [2]: per half
-    unsigned long long* p_full = s_full + 2;       // [2][2]: the P of the tile's upper keys, then of its lower ones
-    unsigned long long* o_done = p_full + 4;       // [2]: the item's last product
-    unsigned long long* kind_full = o_done + 2;    // [2]: 8-bit: what the V tile will be is known
-    unsigned long long* q_full = kind_full + 2;
+    unsigned long long* s_full = v_empty + 2;    // [2]: per half
+    unsigned long long* p_full = s_full + 2;     // [2][2]: the P of the tile's upper keys, of its lower ones
+    unsigned long long* o_done = p_full + 4;     // [2]: the item's last product
+    unsigned long long* q_full = o_done + 2;
     unsigned long long* q_empty = q_full + 1;
-    unsigned long long* edge_full = q_empty + 1;   // bfloat16: a V tile whose slots beyond the range are cleared before it is announced
+    unsigned long long* edge_full = q_empty + 1;  // bfloat16: a V tile whose slots beyond the range are cleared before it is announced
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(edge_full + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* kinds = failed + 1;  // [2]: 2 * (e0 + 64) + whether the tile's values are float16
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&k_full[s], E8 ? 4 : 1);  // four converting warps, or the copies' bytes
+            mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
-            mbar_init(&v_full[s], E8 ? 4 : 1);
-            mbar_init(&raw_full[s], 33);        // the codes' bytes and 32 lanes' exponents
-            mbar_init(&raw_empty[s], 4);
+            mbar_init(&v_full[s], 1);
             mbar_init(&v_empty[s], 1);
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[2 * s], 4);
             mbar_init(&p_full[2 * s + 1], 4);
             mbar_init(&o_done[s], 1);
-            mbar_init(&kind_full[s], 1);
         }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(edge_full, 1);
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
     }
     // rows of Q that no copy writes (beyond tokens x heads of an item) are computed like the others and never stored
-    for (int e = tid; e < S::Q_BYTES / 16; e += S::THREADS) reinterpret_cast<uint4*>(qs)[e] = make_uint4(0, 0, 0, 0);
+    for (int e = tid; e < Q_BYTES / 16; e += THREADS) reinterpret_cast<uint4*>(qs)[e] = make_uint4(0, 0, 0, 0);
+    const int first_item = a.first_item[blockIdx.x], end_item = a.first_item[blockIdx.x + 1];  // written with the plan, long before, like the items
     wait_for_previous_kernels();
     let_next_kernel_start();  // only now: the strip kernel of the same step takes its start as the sign that all that came before has finished
     // All of the SM's tensor memory, and only now: a block of a kernel further back in the stream that has yet to start on this SM can no longer want any.
@@ -369,7 +353,6 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
     const int shift = 31 - __clz(a.page_size);
     const int group = a.heads / a.kv_heads, kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
     const int first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
-    const int first_item = a.first_item[blockIdx.x], end_item = a.first_item[blockIdx.x + 1];
 
     // The roles run through the block's items each at its own pace, held together by the barriers of the data alone.  A wait by parity tells "this phase is over"
     // only to a thread that is at most one phase behind: every barrier's waiter is the one whose own arrival, on the barrier's counterpart, lets the next
@@ -384,16 +367,11 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
         it.halves = it.ntok * a.gc > BM ? 2 : 1;
         return it;
     };
+    auto kind_of = [&](const Item& it, int tile) { return a.kinds[(size_t)(it.operand + tile) * a.kv_heads + kvh]; };
     auto fail = [&] { *failed = 1; };
 
-    if (warp < 4) {
-      if constexpr (E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"((int)S::FEW));
-      if (warp == 0) {
+    if (warp == 0) {
         // ------------------------------------------------------------------ producer (the whole warp)
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
-        }
         const int pages_per_tile = BN >> shift, tokens_per_item = ROWS / a.gc;
         bool alive = true;
         int g = 0, edges = 0, round = 0;  // g: tiles so far
@@ -434,66 +412,60 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
                 const bool edge = tile_base < it.key_lo || tile_base + BN > it.key_hi;
                 for (int which = 0; which < 2 && alive; ++which) {  // the K tile, then the V tile
                     const int s = g & 1, turn = g >> 1;
-                    unsigned long long* empty = E8 ? &raw_empty[which] : (which ? &v_empty[s] : &k_empty[s]);
-                    unsigned long long* full = E8 ? &raw_full[which] : (which ? (edge ? edge_full : &v_full[s]) : &k_full[s]);
+                    unsigned long long* empty = which ? &v_empty[s] : &k_empty[s];
+                    unsigned long long* full = which ? (edge ? edge_full : &v_full[s]) : &k_full[s];
                     int ok = 1;
-                    if (lane == 0) ok = mbar_wait(empty, ((E8 ? g : turn) & 1) ^ 1, failed) ? 1 : 0;
+                    if (lane == 0) ok = mbar_wait(empty, (turn & 1) ^ 1, failed) ? 1 : 0;
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) { alive = false; break; }
                     if (lane == 0) {
-                        const unsigned page_bytes = (unsigned)a.page_size * D * (E8 ? 1u : 2u);
+                        const unsigned page_bytes = (unsigned)a.page_size * D * 2u;
                         if (valid) mbar_expect_tx(full, valid * page_bytes); else mbar_arrive(full);
                     }
                     __syncwarp();
-                    if constexpr (E8) {
-                        const int key = lane * 4, from = __shfl_sync(0xffffffffu, my_page, key >> shift);
-                        if (from >= 0) {
-                            const signed char* src = a.exponents + (((size_t)from * 2 + which) * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1));
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(exps + which * BN + key)), "l"(src) : "memory");
+                    unsigned char* stage = which ? v_ring + (size_t)s * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
+                    const int ops = pages_per_tile * PANELS;
+                    for (int op0 = 0; op0 < ops; op0 += 32) {
+                        const int op = op0 + lane, p = min(op, ops - 1) / PANELS, h = op % PANELS;
+                        const int from = __shfl_sync(0xffffffffu, my_page, p);
+                        if (op < ops && from >= 0)
+                            tma_load_2d(stage + h * KV_PANEL * 2 + p * a.page_size * 128, &kv_map, full, h * 64, ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
+                    }
+                    if (which && edge) {
+                        ok = mbar_wait(edge_full, edges & 1, failed) ? 1 : 0;
+                        ++edges;
+                        if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+                        for (int e = lane; e < BN * 8 * PANELS; e += 32) {
+                            const int row = (e >> 3) & (BN - 1), pos = tile_base + row;
+                            if (pos < it.key_lo || pos >= it.key_hi) reinterpret_cast<uint4*>(stage)[e] = make_uint4(0, 0, 0, 0);
                         }
-                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
-                        if (my_page >= 0)
-                            tma_load_2d(raw_tiles + which * RAW_BYTES + lane * a.page_size * D, &kv_map, full, 0, ((my_page * 2 + which) * a.kv_heads + kvh) * a.page_size);
-                    } else {
-                        unsigned char* stage = which ? v_ring + (size_t)s * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
-                        const int ops = pages_per_tile * PANELS;
-                        for (int op0 = 0; op0 < ops; op0 += 32) {
-                            const int op = op0 + lane, p = min(op, ops - 1) / PANELS, h = op % PANELS;
-                            const int from = __shfl_sync(0xffffffffu, my_page, p);
-                            if (op < ops && from >= 0)
-                                tma_load_2d(stage + h * KV_PANEL * 2 + p * a.page_size * 128, &kv_map, full, h * 64, ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
-                        }
-                        if (which && edge) {
-                            ok = mbar_wait(edge_full, edges & 1, failed) ? 1 : 0;
-                            ++edges;
-                            if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
-                            for (int e = lane; e < BN * 8 * PANELS; e += 32) {
-                                const int row = (e >> 3) & (BN - 1), pos = tile_base + row;
-                                if (pos < it.key_lo || pos >= it.key_hi) reinterpret_cast<uint4*>(stage)[e] = make_uint4(0, 0, 0, 0);
-                            }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&v_full[s]);
-                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&v_full[s]);
                     }
                 }
             }
         }
         if (!alive) fail();
-      } else if (warp == 1) {
-        // ------------------------------------------------------------------ tensor-core issuer (one lane)
-        if (lane == 0) {
-            const unsigned idesc_s = idesc_for(BN, false, false), idesc_o = idesc_for(D, true, false), idesc_half = idesc_for(D, true, true);
-            const unsigned q_low0 = low_k_major(qs), k_low0 = low_k_major(k_ring), v_low0 = low_mn_major(v_ring, KV_PANEL * 2);
-            auto issue_s = [&](int x, int g) {  // S_x = Q_x K(g)^T
-                const unsigned k_low = k_low0 + (unsigned)(g & 1) * (TILE_BYTES >> 4), q_low = q_low0 + (unsigned)x * (BM * 128 >> 4);
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ tensor-core issuer: the warp stays together, so that descriptors are its common values
+        // (uniform registers); one elected lane issues.  Under `if (lane == 0)` every product took 65 clocks to
+        // issue, as long as it runs, and the waits came on top (a tile 4,000 clocks instead of 3,600).
+        const unsigned idesc_s = idesc_for(BN, false, false), idesc_o = idesc_for(D, true, false), idesc_half = idesc_for(D, true, true);
+        const unsigned q_low0 = low_k_major(qs), k_low0 = low_k_major(k_ring), v_low0 = low_mn_major(v_ring, KV_PANEL * 2);
+        auto wait_for = [&](unsigned long long* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, failed)) != 0; };
+        auto issue_s = [&](int x, int g) {  // S_x = Q_x K(g)^T
+            const unsigned k_low = k_low0 + (unsigned)(g & 1) * (TILE_BYTES >> 4), q_low = q_low0 + (unsigned)x * (BM * 128 >> 4);
+            if (elected()) {
                 umma_s_panel(tmem + x * BN, q_low, k_low, idesc_s, 0u);
 #pragma unroll
                 for (int h = 1; h < PANELS; ++h) umma_s_panel(tmem + x * BN, q_low + h * (Q_PANEL * 2 >> 4), k_low + h * (KV_PANEL * 2 >> 4), idesc_s, 1u);
                 umma_commit_at(smem_u32(&s_full[x]));
-            };
-            auto issue_pv = [&](int x, int g, int part, bool halves, unsigned accumulate) {  // O_x (+)= P_x V(g) over the upper (part 0) or the lower 64 keys
-                const unsigned at = part ? 0u : 64u, v_low = v_low0 + (unsigned)(g % STAGES) * (TILE_BYTES >> 4) + at * 8, o = tmem + O_COL + x * BM, p = tmem + x * BN + at;
+            }
+        };
+        auto issue_pv = [&](int x, int g, int part, bool halves, unsigned accumulate) {  // O_x (+)= P_x V(g) over the upper (part 0) or the lower 64 keys
+            const unsigned at = part ? 0u : 64u, v_low = v_low0 + (unsigned)(g & 1) * (TILE_BYTES >> 4) + at * 8, o = tmem + O_COL + x * BM, p = tmem + x * BN + at;
+            if (elected()) {
                 if (halves) {
                     umma_pv_32_whole(o, p, v_low, idesc_half, accumulate);
                     umma_pv_32_whole(o, p + 32, v_low + 256, idesc_half, 1u);
@@ -501,90 +473,98 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
                     umma_pv_32(o, p, v_low, idesc_o, accumulate);
                     umma_pv_32(o, p + 32, v_low + 256, idesc_o, 1u);
                 }
-            };
-            bool ok = true;
-            int g0 = 0, h0[2] = {0, 0}, round = 0;
-            for (int index = first_item; index < end_item && ok; ++index, ++round) {
-                const Item it = read_item(index);
-                if (!mbar_wait(q_full, round & 1, failed)) { ok = false; break; }
-                if (it.n_tiles == 0) { umma_commit_at(smem_u32(q_empty)); continue; }
-                if (!mbar_wait(&k_full[g0 & 1], (g0 >> 1) & 1, failed)) { ok = false; break; }
-                tc_fence_after();
-                // S_x of the first tile lands in the columns that the last product of the item before read its P from: products of one thread run in the
-                // order of their issue
-                for (int x = 0; x < it.halves; ++x) issue_s(x, g0);
-                umma_commit_at(smem_u32(&k_empty[g0 & 1]));
-                if (it.n_tiles == 1) umma_commit_at(smem_u32(q_empty));
-                for (int j = 0; j < it.n_tiles && ok; ++j) {
-                    const int g = g0 + j;
-                    const bool more = j + 1 < it.n_tiles;
-                    bool halves = false;
-                    if constexpr (E8) {
-                        if (!mbar_wait(&kind_full[g & 1], (g >> 1) & 1, failed)) { ok = false; break; }
-                        halves = kinds[g & 1] & 1;
-                    } else if constexpr (FROM == OPERANDS) {
-                        halves = a.kinds[(size_t)(it.operand + j) * a.kv_heads + kvh] & 1;
-                    }
-                    for (int x = 0; x < it.halves && ok; ++x) {
-                        for (int part = 0; part < 2 && ok; ++part) {
-                            if (!mbar_wait(&p_full[2 * x + part], (h0[x] + j) & 1, failed)) { ok = false; break; }
-                            if (x == 0 && part == 0 && !mbar_wait(&v_full[g % STAGES], (g / STAGES) & 1, failed)) { ok = false; break; }
-                            tc_fence_after();
-                            issue_pv(x, g, part, halves, j > 0 || part > 0 ? 1u : 0u);
-                        }
-                        if (!ok) break;
-                        if (!more) umma_commit_at(smem_u32(&o_done[x]));
-                        if (x == it.halves - 1) umma_commit_at(smem_u32(&v_empty[g % STAGES]));
-                        if (more) {
-                            if (x == 0) {
-                                if (!mbar_wait(&k_full[(g + 1) & 1], ((g + 1) >> 1) & 1, failed)) { ok = false; break; }
-                                tc_fence_after();
-                            }
-                            issue_s(x, g + 1);
-                            if (x == it.halves - 1) {
-                                umma_commit_at(smem_u32(&k_empty[(g + 1) & 1]));
-                                if (j + 2 == it.n_tiles) umma_commit_at(smem_u32(q_empty));
-                            }
-                        }
-                    }
-                }
-                g0 += it.n_tiles;
-                h0[0] += it.n_tiles;
-                if (it.halves == 2) h0[1] += it.n_tiles;
             }
-            if (!ok) fail();
+        };
+        auto commit = [&](unsigned long long* bar) {
+            if (elected()) umma_commit_at(smem_u32(bar));
+        };
+        bool ok = true;
+        int g = 0, mine[2] = {0, 0}, round = 0;  // tiles so far, and those that a half had a part in
+        for (int index = first_item; index < end_item && ok; ++index, ++round) {
+            const Item it = read_item(index);
+            if (!wait_for(q_full, round)) { ok = false; break; }
+            if (it.n_tiles == 0) { commit(q_empty); continue; }
+            if (!wait_for(&k_full[g & 1], g >> 1)) { ok = false; break; }
+            tc_fence_after();
+            // S_x of the first tile lands in the columns that the last product of the item before read its P from: products of one thread run in the
+            // order of their issue
+            for (int x = 0; x < it.halves; ++x) issue_s(x, g);
+            commit(&k_empty[g & 1]);
+            if (it.n_tiles == 1) commit(q_empty);
+            for (int j = 0; j < it.n_tiles && ok; ++j, ++g) {
+                const bool more = j + 1 < it.n_tiles;
+                bool halves = false;
+                if constexpr (FROM == OPERANDS) halves = kind_of(it, j) & 1;
+                if (!wait_for(&v_full[g & 1], g >> 1) || (more && !wait_for(&k_full[(g + 1) & 1], (g + 1) >> 1))) { ok = false; break; }  // while the softmax is busy
+                for (int x = 0; x < it.halves && ok; ++x) {
+                    for (int part = 0; part < 2 && ok; ++part) {
+                        if (!wait_for(&p_full[2 * x + part], mine[x])) { ok = false; break; }
+                        tc_fence_after();
+                        issue_pv(x, g, part, halves, j > 0 || part > 0 ? 1u : 0u);
+                    }
+                    if (!ok) break;
+                    if (more) issue_s(x, g + 1);
+                    else commit(&o_done[x]);
+                    ++mine[x];
+                }
+                if (!ok) break;
+                commit(&v_empty[g & 1]);
+                if (more) commit(&k_empty[(g + 1) & 1]);
+                if (j + 2 == it.n_tiles) commit(q_empty);
+            }
         }
-      }
-    } else if (warp < 12) {
+        if (!ok) fail();
+    } else if (warp >= 4) {
         // ------------------------------------------------------------------ softmax: thread = row = tensor-memory lane of its half
-        if constexpr (E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"((int)S::MANY));
         const int x = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane, v = x * BM + r;
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
         const unsigned s_addr = lane_addr + x * BN, o_addr = lane_addr + O_COL + x * BM;
+        float* desk = desks + (warp - 4) * DESK;
         const float scale = a.scale_log2;
         const Pair scale2{scale, scale}, minus_one{-1.f, -1.f};
-        int hx = 0, g0 = 0, mine = 0;  // tiles this half has seen; the block's tiles; items this half has had a part in
+        int hx = 0, mine = 0;  // tiles this half has seen, items it has had a part in
         bool ok = true;
         for (int index = first_item; index < end_item && ok; ++index) {
             const Item it = read_item(index);
-            if (x >= it.halves) { g0 += it.n_tiles; continue; }
+            if (x >= it.halves) continue;
             const int tok = v / a.gc, hh = v - tok * a.gc;
             const bool row_valid = tok < it.ntok && hh < heads_here;
             // a row that is no one's is computed like the item's last token and never stored: it takes the same way through the code as its neighbours
             const int token = it.tok0 + min(tok, it.ntok - 1), hi = min(it.key_hi - 1, a.last[token]);
+            int piece_at = 0;
+            if (row_valid && a.pieces) piece_at = (it.piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (it.piece & (OWN_PIECE - 1));
             float m = -INFINITY, l = 0.f;
             int kind = 2 * 64;
             for (int j = 0; j < it.n_tiles; ++j) {
                 const int h = hx + j;
-                if constexpr (FROM == OPERANDS) kind = a.kinds[(size_t)(it.operand + j) * a.kv_heads + kvh];  // there by the time S is
+                if constexpr (FROM == OPERANDS) kind = kind_of(it, j);  // there by the time S is
                 if (!mbar_wait(&s_full[x], h & 1, failed)) { ok = false; break; }
                 tc_fence_after();
                 const int tile_base = it.start + j * BN, last_visible = hi - tile_base, first_visible = it.key_lo - tile_base;
-                const bool masked = !__all_sync(0xffffffffu, last_visible >= BN - 1 && first_visible <= 0);  // one way for the whole warp
                 unsigned s0[32], s1[32];  // of this row's S, 32 columns at hand and 32 on their way
+                auto hand_over = [&](int which) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * x + which]);
+                };
+                float part[2] = {-INFINITY, -INFINITY};
+                auto look = [&](unsigned (&s)[32]) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) part[i & 1] = max3(part[i & 1], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+                };
+                auto weigh_16 = [&](const unsigned (&s)[32], unsigned (&w)[16], Pair minus_m2, Pair (&sum)[2]) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const Pair z = fma2(Pair{__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, scale2, minus_m2), p{fast_exp2(z.x), fast_exp2(z.y)};
+                        sum[i & 1] = add2(sum[i & 1], p);
+                        w[i] = pack_f16x2(p.x, p.y);
+                    }
+                };
+                const bool whole = __all_sync(0xffffffffu, last_visible >= BN - 1 && first_visible <= 0);
                 // The loops below are kept short on purpose: the roles of a block run different code on the same schedulers, and straight-line code is bound by
-                // the fetching of instructions (8-bit, 256 requests behind 16,384 positions: 163 us with every loop unrolled and masks in each of them).
-                if (masked) {  // what the row does not see is replaced where it stands
+                // the fetching of instructions (256 requests behind 16,384 positions took 19 % longer with every loop unrolled and masks in each of them).
+                if (!whole) {  // what a row does not see is replaced where it stands; one way for the whole warp
 #pragma unroll 1
                     for (int c = 0; c < BN; c += 32) {
                         tmem_ld32(s_addr + c, s0), arrived(s0);
@@ -594,11 +574,6 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                float part[2] = {-INFINITY, -INFINITY};
-                auto look = [&](unsigned (&s)[32]) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) part[i & 1] = max3(part[i & 1], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                };
                 tmem_ld32(s_addr, s0), arrived(s0);
 #pragma unroll 1
                 for (int c = 0; c < BN; c += 64) {
@@ -607,16 +582,19 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
                     look(s1);
                     if (c == 0) arrived(s0);
                 }
-                const float m_new = fmaxf(m, fmaxf(part[0], part[1]) * scale);  // the scale is positive: the largest score stays the largest
+                const float seen = max3(part[0], part[1], -INFINITY) * scale, m_new = fmaxf(m, seen);  // the scale is positive: the largest score stays the largest
+                const bool outgrown = __any_sync(0xffffffffu, m > -INFINITY && m_new - m > OUTGROWN<FROM>);  // one row's is taken as the occasion for all of the warp's
                 float alpha = 1.f;
-                if (m == -INFINITY) {
+                if (!(seen < INFINITY)) {
+                    m = __uint_as_float(0x7fffffffu);  // a NaN or an infinity among the scores: the row's softmax is no number, and stays none
+                } else if (m == -INFINITY) {
                     m = m_new;  // nothing seen so far: the row of O holds zeros (or is overwritten by the first product)
-                } else if (m_new - m > S::OUTGROWN) {
+                } else if (outgrown) {
                     alpha = exp2f(m - m_new);
                     m = m_new;
                 }
                 // The products of the tiles before were issued before this S was, and this S has arrived: O stands still.
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                if (j > 0 && outgrown) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         tmem_ld32(o_addr + c, s0), arrived(s0);
@@ -628,39 +606,24 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
                 const float minus_m = m == -INFINITY ? 0.f : -m;
                 const Pair minus_m2{minus_m, minus_m};
                 Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-                auto weights = [&](const unsigned (&s)[32], int i) {
-                    const Pair z = fma2(Pair{__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, scale2, minus_m2), p{fast_exp2(z.x), fast_exp2(z.y)};
-                    sum[i & 1] = add2(sum[i & 1], p);
-                    return p;
-                };
                 auto weigh_halves = [&](const unsigned (&s)[32], int c) {  // P of 32 columns as float16, over the first half of the columns that they came from
                     unsigned w[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const Pair p = weights(s, i);
-                        w[i] = pack_f16x2(p.x, p.y);
-                    }
+                    weigh_16(s, w, minus_m2, sum);
                     tmem_st16_words(s_addr + c, w);
                 };
                 auto weigh = [&](const unsigned (&s)[32], int c) {  // as bfloat16 in two parts, over all of them
                     unsigned w[32];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const Pair p = weights(s, i);
+                        const Pair z = fma2(Pair{__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, scale2, minus_m2), p{fast_exp2(z.x), fast_exp2(z.y)};
+                        sum[i & 1] = add2(sum[i & 1], p);
                         w[i] = __byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x7632);
                         const Pair rest = fma2(Pair{__uint_as_float(__float_as_uint(p.x) & 0xffff0000u), __uint_as_float(__float_as_uint(p.y) & 0xffff0000u)}, minus_one, p);
                         w[16 + i] = pack_bf16x2(rest.x, rest.y);
                     }
                     tmem_st32(s_addr + c, w);
                 };
-                auto hand_over = [&](int which) {
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * x + which]);
-                };
-                // columns 96 to 127 are still at hand
-                auto walk = [&](auto&& weigh_32) {
+                auto walk = [&](auto&& weigh_32) {  // columns 96 to 127 are still at hand
 #pragma unroll 1
                     for (int c = 64; c >= 0; c -= 64) {
                         tmem_ld32(s_addr + c, s0), weigh_32(s1, c + 32), arrived(s0);
@@ -670,11 +633,7 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
                         if (c) arrived(s1);
                     }
                 };
-                if constexpr (FROM != BFLOAT16) {
-                    if constexpr (E8) {
-                        if (!mbar_wait(&kind_full[(g0 + j) & 1], ((g0 + j) >> 1) & 1, failed)) { ok = false; break; }
-                        kind = kinds[(g0 + j) & 1];
-                    }
+                if constexpr (FROM == OPERANDS) {
                     if (kind & 1) {
                         walk(weigh_halves);
                     } else {
@@ -695,103 +654,44 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             if (ok) {
-                const size_t slot = row_valid && a.pieces ? (size_t)((it.piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (it.piece & (OWN_PIECE - 1))) * a.heads + first_head + hh : 0;
-                const float back = FROM != BFLOAT16 ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
-                const float inv = a.pieces ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
-#pragma unroll
-                for (int c = 0; c < D; c += 16) {
-                    float o[16];
+                if (m == -INFINITY) l = 0.f;  // a row that sees nothing: what exp2_pair gave for it is none of its weights
+                const float back = FROM == OPERANDS ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
+                const float inv = a.pieces ? back : back * (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
+                // Rows leave through shared memory, 32 columns of 32 rows at a time: eight lanes then store 128 bytes of a row side by side, where a thread storing its own row
+                // would touch 32 lines with every instruction (6,600 clocks an item).
+                const long long row_at = !row_valid ? -1 : a.pieces ? ((long long)piece_at * a.heads + first_head + hh) * D : (long long)token * a.out_stride + (long long)(first_head + hh) * D;
+                if (row_valid && a.pieces) a.sums[(size_t)piece_at * a.heads + first_head + hh] = make_float2(m, l);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    unsigned o[32];
                     if (it.n_tiles > 0) {
-                        tmem_ld16(o_addr + c, o);
+                        tmem_ld32(o_addr + c, o), arrived(o);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = 0.f;
+                        for (int i = 0; i < 32; ++i) o[i] = 0u;
                     }
+                    float4* line = reinterpret_cast<float4*>(desk) + lane * 8;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] *= back;
-                    if (row_valid && a.pieces) {
+                    for (int i = 0; i < 8; ++i)  // 16-byte pieces, turned about by the row so that neither way meets a bank twice
+                        line[i ^ (lane & 7)] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+                    __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 16; i += 8)
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(a.pieces + slot * D + c + i), "r"(__float_as_uint(o[i])), "r"(__float_as_uint(o[i + 1])),
-                                         "r"(__float_as_uint(o[i + 2])), "r"(__float_as_uint(o[i + 3])), "r"(__float_as_uint(o[i + 4])), "r"(__float_as_uint(o[i + 5])),
-                                         "r"(__float_as_uint(o[i + 6])), "r"(__float_as_uint(o[i + 7])) : "memory");
-                    } else if (row_valid) {
-                        uint2* dst = reinterpret_cast<uint2*>(a.out + (size_t)token * a.out_stride + (size_t)(first_head + hh) * D + c);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) dst[i] = make_uint2(pack_bf16x2(o[4 * i] * inv, o[4 * i + 1] * inv), pack_bf16x2(o[4 * i + 2] * inv, o[4 * i + 3] * inv));
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = i * 4 + (lane >> 3), at = lane & 7;
+                        const long long to = __shfl_sync(0xffffffffu, row_at, row);
+                        const float4 out = reinterpret_cast<const float4*>(desk)[row * 8 + (at ^ (row & 7))];
+                        if (to >= 0) {
+                            const float w[4] = {out.x, out.y, out.z, out.w};
+                            if (a.pieces) store4(a.pieces + to + c + 4 * at, w);
+                            else store4(a.out + to + c + 4 * at, w);
+                        }
                     }
+                    __syncwarp();
                 }
-                if (row_valid && a.pieces) a.sums[slot] = make_float2(m, l);
                 // the row is out of tensor memory before this thread hands over the next item's first P, and only then is O written anew
                 tc_fence_before();
             }
-            hx += it.n_tiles, g0 += it.n_tiles;
-        }
-        if (!ok) fail();
-    } else if constexpr (E8) {
-        // ------------------------------------------------------------------ codes into operands: warps 12 to 15 the K tiles, 16 to 19 the V tiles
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"((int)S::CONVERTING));
-        const int which = (warp - 12) >> 2, w = warp & 3;
-        constexpr int CHUNKS = D / 16;  // 16 codes each, of a row
-        bool ok = true;
-        int g = 0;
-        for (int index = first_item; index < end_item && ok; ++index) {
-            const Item it = read_item(index);
-            int e0 = 0;
-            for (int t = 0; t < it.n_tiles; ++t, ++g) {
-                const int s = g & 1, turn = g >> 1, tile_base = it.start + t * BN;
-                ok = mbar_wait(&raw_full[which], g & 1, failed);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const unsigned char* raw = raw_tiles + which * RAW_BYTES;
-                const signed char* e8 = reinterpret_cast<const signed char*>(exps + which * BN);
-                unsigned char* tile = (which ? v_ring : k_ring) + (size_t)s * TILE_BYTES;
-                bool halves = false;
-                if (which) {  // what the tile will be, for those who make its weights and its products
-                    int low = 127, high = -128;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int pos = tile_base + lane * 4 + k, e = min(max((int)e8[lane * 4 + k], -40), 40);
-                        if (pos >= it.key_lo && pos < it.key_hi) low = min(low, e), high = max(high, e);
-                    }
-                    low = __reduce_min_sync(0xffffffffu, low), high = __reduce_max_sync(0xffffffffu, high);
-                    if (t == 0) e0 = high;
-                    halves = low - e0 >= LOWEST && high - e0 <= HIGHEST;
-                }
-                ok = mbar_wait(which ? &v_empty[s] : &k_empty[s], (turn & 1) ^ 1, failed);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (which && w == 0 && lane == 0) {  // only now: the products of the tile that had this slot, and its word in `kinds`, are done
-                    kinds[s] = 2 * (e0 + 64) + (halves ? 1 : 0);
-                    mbar_arrive(&kind_full[s]);
-                }
-                // eight lanes take a 16-byte chunk of eight rows: the swizzles of both layouts put those in different banks
-                auto convert = [&](auto as_halves) {
-#pragma unroll 2
-                    for (int i = 0; i < BN / 8 * CHUNKS / 16; ++i) {
-                        const int octet = (i * 4 + w) * 4 + (lane >> 3), chunk = octet % CHUNKS, row = octet / CHUNKS * 8 + (lane & 7);
-                        const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * D + ((D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4));
-                        const int e = min(max((int)e8[row], -40), 40) - e0;
-                        const bool keep = which == 0 || (tile_base + row >= it.key_lo && tile_base + row < it.key_hi);
-                        unsigned wide[8];
-                        widen<as_halves.value>(codes, e, wide);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int oc = 2 * chunk + half;
-                            uint4 out = make_uint4(wide[4 * half], wide[4 * half + 1], wide[4 * half + 2], wide[4 * half + 3]);
-                            if (!keep) out = make_uint4(0, 0, 0, 0);
-                            *reinterpret_cast<uint4*>(tile + (oc >> 3) * (KV_PANEL * 2) + row * 128 + (((oc & 7) ^ (row & 7)) << 4)) = out;
-                        }
-                    }
-                };
-                if (halves) convert(Yes{}); else convert(No{});
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(which ? &v_full[s] : &k_full[s]);
-                    mbar_arrive(&raw_empty[which]);
-                }
-            }
+            hx += it.n_tiles;
         }
         if (!ok) fail();
     }
@@ -804,9 +704,10 @@ __global__ void __launch_bounds__(Shape<FROM>::THREADS, 1) attention_shared_kern
     }
 }
 
-// Operands of 8-bit records that several runs of tokens walk: a block makes one tile of K or of V of one key/value head, in the layout of the attention's shared memory, so
-// that every one of those runs fetches it by two plain copies and converts nothing.  Bound by memory (three bytes an entry).  It pays from three runs on: 256 requests behind
-// 16,384 positions (eight runs) 162 us -> 154, 64 requests behind 4,096 (two runs) 35.6 without it and 39.4 with it.
+// Operands of 8-bit records: a block makes one tile of K or of V of one key/value head, in the layout of the attention's shared memory, so that every run of tokens that
+// walks it fetches it by a plain copy and converts nothing.  Bound by memory (three bytes an entry).  (Conversion inside the attention, by eight more warps between the
+// copies and the products, was built first: it held a block back from 4,200 to 5,600 clocks a tile, for every run anew; 256 requests behind 16,384 positions, eight runs, 162 us
+// against 154, 64 requests behind 4,096, two runs, 35.6 against 39.4, with the softmax of then.)
 constexpr int OPERAND_THREADS = 256;
 __global__ void __launch_bounds__(OPERAND_THREADS) shared_operands_kernel(const unsigned char* __restrict__ codes, const signed char* __restrict__ exponents, const int* __restrict__ block_table,
                                                                           int table_width, const int4* __restrict__ tiles, unsigned char* __restrict__ operands, int* __restrict__ kinds,
@@ -887,15 +788,8 @@ template <Source FROM>
 int launch(const Args& a, int blocks, const void* q, int q_stride, int n_tokens, const void* cache, cudaStream_t stream) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return HB_BAD_ARGUMENT;
-    // the cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and up to 128 bytes
     CUtensorMap map, q_map;
-    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)a.pages * 2 * a.kv_heads * a.page_size};
-    const cuuint64_t strides[1] = {(cuuint64_t)D * (FROM == BFLOAT16 ? 2 : 1)};
-    const cuuint32_t box[2] = {(cuuint32_t)(FROM == BFLOAT16 ? 64 : D), (cuuint32_t)a.page_size};
     const cuuint32_t elem[3] = {1, 1, 1};
-    if (encode(&map, FROM == BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               FROM != BFLOAT16 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return HB_BAD_ARGUMENT;
     // the queries as (column, head, token): an item's box is 64 columns of gc heads of its tokens
     const cuuint64_t q_dims[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)n_tokens};
     const cuuint64_t q_strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)q_stride * 2};
@@ -903,9 +797,19 @@ int launch(const Args& a, int blocks, const void* q, int q_stride, int n_tokens,
     if (encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), q_dims, q_strides, q_box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return HB_BAD_ARGUMENT;
-    static const cudaError_t configured = cudaFuncSetAttribute(attention_shared_kernel<FROM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<FROM>::SMEM);
+    if constexpr (FROM == BFLOAT16) {  // the cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and 64 columns
+        const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)a.pages * 2 * a.kv_heads * a.page_size};
+        const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+        const cuuint32_t box[2] = {64, (cuuint32_t)a.page_size};
+        if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return HB_BAD_ARGUMENT;
+    } else {
+        map = q_map;  // operands are fetched without one
+    }
+    static const cudaError_t configured = cudaFuncSetAttribute(attention_shared_kernel<FROM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(attention_shared_kernel<FROM>, dim3(blocks, a.kv_heads * a.chunks), dim3(Shape<FROM>::THREADS), Shape<FROM>::SMEM, stream, map, q_map, a);
+    return launch_after_previous(attention_shared_kernel<FROM>, dim3(blocks, a.kv_heads * a.chunks), dim3(THREADS), SMEM_BYTES, stream, map, q_map, a);
 }
 const int* kinds_of(const void* operands, long long tiles, long long kv_heads) {  // they stand behind the tiles
     return operands ? (const int*)((const unsigned char*)operands + (size_t)tiles * kv_heads * (2 * TILE_BYTES)) : nullptr;
@@ -924,7 +828,7 @@ HB_EXPORT int hb_shared_operands(const void* codes, const void* exponents, const
                                  table_width, (const int4*)tiles, (unsigned char*)operands, const_cast<int*>(kinds_of(operands, n_tiles, kv_heads)), page_size, pages, status);
 }
 
-// cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
+// cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents and operands null), or e4m3 codes with exponents and the operands that hb_shared_operands has made of them.
 // items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most 256 / min(heads / kv_heads, 256) tokens.  pieces, sums null: one piece a row.
 HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_tokens, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table,
                                         int table_width, const int* items, const int* first_item, int blocks, const void* operands, int operand_tiles, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads,
@@ -938,9 +842,9 @@ HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_token
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
-    if (operands && (!exponents || operand_tiles <= 0 || ((uintptr_t)operands & 15))) return HB_BAD_ARGUMENT;
-    const Args a{(const signed char*)exponents, (const unsigned char*)operands, kinds_of(operands, operand_tiles, kv_heads), (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
+    if (!operands != !exponents || (operands && (operand_tiles <= 0 || ((uintptr_t)operands & 15)))) return HB_BAD_ARGUMENT;
+    const Args a{(const unsigned char*)operands, kinds_of(operands, operand_tiles, kv_heads), (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
     if (operands) return launch<OPERANDS>(a, blocks, q, q_stride, n_tokens, cache, stream);
-    return exponents ? launch<CODES>(a, blocks, q, q_stride, n_tokens, cache, stream) : launch<BFLOAT16>(a, blocks, q, q_stride, n_tokens, cache, stream);
+    return launch<BFLOAT16>(a, blocks, q, q_stride, n_tokens, cache, stream);
 }

@@ -110,20 +110,14 @@ SharedPlan plan_shared(const std::vector<int64_t>& counts, const std::vector<int
     const auto is_wide = [&](const Run& range) { return range.count * group > MOST_STRIP_ROWS; };
     for (const Run& range : ranges)
         if (!is_wide(range) && range.count * group > 8) plan.strip_rows = 16;
-    int64_t walked = 0, distinct = 0;
+    int64_t distinct = 0;
     for (Run& range : ranges) {
         if (!is_wide(range)) continue;
-        const int64_t per = std::max<int64_t>(1, TILE_ROWS / group), tiles = tiles_of(range);
         range.operand = distinct;
-        distinct += tiles;
-        walked += tiles * ((range.count + per - 1) / per);
-    }
-    if (walked >= 3 * distinct && distinct > 0) {  // measured where the operands are made (attention_shared_tiles.cu)
+        distinct += tiles_of(range);
         require(distinct <= most / 4, "plan_shared: the tiles of a step fit 32 bits");
-        for (const Run& range : ranges)
-            if (is_wide(range))
-                for (int64_t at = range.low / KEYS * KEYS; at < range.high; at += KEYS)
-                    for (int64_t word : {range.row, at, range.low, range.high}) plan.operands.push_back((int)word);
+        for (int64_t at = range.low / KEYS * KEYS; at < range.high; at += KEYS)
+            for (int64_t word : {range.row, at, range.low, range.high}) plan.operands.push_back((int)word);
     }
     const auto runs_of = [&](bool wide, int64_t rows) {
         const int64_t per = std::max<int64_t>(1, rows / group);

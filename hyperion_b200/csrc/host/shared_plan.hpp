@@ -23,8 +23,7 @@ struct Walk {  // of one kernel: block b takes items first[b] .. first[b + 1] - 
 struct SharedPlan {
     Walk strips, tiles;
     int strip_rows = 8;
-    // The tiles of the wide ranges, each as (table row, first position, first key, last key + 1 of its range), where 8-bit records are worth being made into operands once for all
-    // the runs of tokens that walk them; empty where every range has one run, which does that on its way.
+    // The tiles of the wide ranges, each as (table row, first position, first key, last key + 1 of its range): what 8-bit records are made into operands for.
     std::vector<int> operands;
     std::vector<int> last, starts, own;  // the last position a token sees, its first piece, its first piece of its own request's positions
     bool joined = false;                 // some token has another number of pieces than one

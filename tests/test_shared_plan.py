@@ -35,7 +35,7 @@ def covered(counts, lengths, heads, kv, groups, sms):
     for rows, (items, _) in ((plan.strip_rows, strips), (256, tiles)):
         for tok, n, row, low, high, number, operand in items:
             assert n >= 1 and high > low and n * min(rows, heads // kv) <= rows
-            if rows == 256 and len(operands):  # the item's tiles stand one behind the other among the operands
+            if rows == 256:  # the item's tiles stand one behind the other among the operands
                 for i, at in enumerate(range(low // 128 * 128, high, 128)):
                     assert operands[operand + i][0] == row and operands[operand + i][1] == at and operands[operand + i][2] <= low and high <= operands[operand + i][3]
             for t in range(tok, tok + n):
@@ -90,9 +90,9 @@ def test_blocks_have_equal_shares(counts, lengths, groups):
             assert keys.max() <= 1.5 * keys.mean() + 256 and len(keys) * 4 <= 3 * 148
 
 
-def test_operands_are_made_where_several_runs_walk_them():
-    assert plan_shared([72], [500], 14, 2, 64, device="cpu", sms=148).operand_tiles == 0  # two runs of 252 rows
-    assert plan_shared([73], [500], 14, 2, 64, device="cpu", sms=148).operand_tiles == 4
+def test_wide_ranges_have_operand_tiles():
+    assert plan_shared([4], [500], 14, 2, 64, device="cpu", sms=148).operand_tiles == 0  # strips take records as they are
+    assert plan_shared([72], [500], 14, 2, 64, device="cpu", sms=148).operand_tiles == 4
     assert plan_shared([1] * 80, [700] * 80, 14, 2, 64, shared=[(0, 80, 600)], device="cpu", sms=148).operand_tiles == 5
 
 
