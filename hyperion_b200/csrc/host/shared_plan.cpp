@@ -130,12 +130,12 @@ SharedPlan plan_shared(const std::vector<int64_t>& counts, const std::vector<int
     };
     const std::vector<Run> strips = runs_of(false, plan.strip_rows), tiles = runs_of(true, TILE_ROWS);
     const int64_t strips_across = kv_heads * ((group + plan.strip_rows - 1) / plan.strip_rows), tiles_across = kv_heads * ((group + TILE_ROWS - 1) / TILE_ROWS);
-    // Where a step has both kinds they run side by side, each on a part of the device that its work asks for.  A tile of 256 rows takes an SM some 2.3 us and an item of them 4
+    // Where a step has both kinds they run side by side, each on a part of the device that its work asks for.  A tile of 256 rows takes an SM some 2.1 us and an item of them 4
     // besides, a tile of a strip 0.65 (three blocks share the SM) and a strip 1.3.
     int64_t tile_sms = tiles.empty() ? 0 : sms;
     if (!tiles.empty() && !strips.empty()) {
         double tile_work = 0, strip_work = 0;
-        for (const Run& run : tiles) tile_work += (2.3 * (double)tiles_of(run) + 4) * (double)tiles_across;
+        for (const Run& run : tiles) tile_work += (2.1 * (double)tiles_of(run) + 4) * (double)tiles_across;
         for (const Run& run : strips) strip_work += (0.65 * (double)tiles_of(run) + 1.3) * (double)strips_across;
         tile_sms = std::max<int64_t>(1, std::min<int64_t>(sms - 1, (int64_t)((double)sms * tile_work / (tile_work + strip_work) + 0.5)));
         tile_sms = std::min(sms, std::max<int64_t>(1, (tile_sms + tiles_across / 2) / tiles_across) * tiles_across);
