@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                 const float back = FROM == OPERANDS ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
                 const float inv = a.pieces ? back : back * (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
                 // Rows leave through shared memory, 32 columns of 32 rows at a time: eight lanes then store 128 bytes of a row side by side, where a thread storing its own row
-                // would touch 32 lines with every instruction (6,600 clocks an item).
+                // would touch 32 lines with every instruction.  Some 6,000 clocks an item either way, 32 bytes a clock: what an SM stores.
                 const long long row_at = !row_valid ? -1 : a.pieces ? ((long long)piece_at * a.heads + first_head + hh) * D : (long long)token * a.out_stride + (long long)(first_head + hh) * D;
                 if (row_valid && a.pieces) a.sums[(size_t)piece_at * a.heads + first_head + hh] = make_float2(m, l);
 #pragma unroll 1
@@ -705,9 +705,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
 }
 
 // Operands of 8-bit records: a block makes one tile of K or of V of one key/value head, in the layout of the attention's shared memory, so that every run of tokens that
-// walks it fetches it by a plain copy and converts nothing.  Bound by memory (three bytes an entry).  (Conversion inside the attention, by eight more warps between the
-// copies and the products, was built first: it held a block back from 4,200 to 5,600 clocks a tile, for every run anew; 256 requests behind 16,384 positions, eight runs, 162 us
-// against 154, 64 requests behind 4,096, two runs, 35.6 against 39.4, with the softmax of then.)
+// walks it fetches it by a plain copy and converts nothing.  Bound by what the device writes to L2: 16,384 positions of 4 heads of 128 in 12 us (67 MB, 5.6 TB/s).  (Conversion inside the attention, by eight more warps between the
+// copies and the products, was built first: it held a block back from 4,200 to 5,600 clocks a tile, for every run anew: 256
+// requests behind 16,384 positions, eight runs, 162 us against 154, 64 requests behind 4,096, two runs, 35.6 against 39.4, with the slower softmax of then.)
 constexpr int OPERAND_THREADS = 256;
 __global__ void __launch_bounds__(OPERAND_THREADS) shared_operands_kernel(const unsigned char* __restrict__ codes, const signed char* __restrict__ exponents, const int* __restrict__ block_table,
                                                                           int table_width, const int4* __restrict__ tiles, unsigned char* __restrict__ operands, int* __restrict__ kinds,

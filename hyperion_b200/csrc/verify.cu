@@ -10,10 +10,10 @@
 // Both kernels are bound by memory.  The first reads every row once, a block a piece of it, and leaves each piece's maximum and sum (or its argmax); a request's end is
 // known only when all its rows' sums are.  The second takes, per request, the one row at which the request ends, the drafter's and the noise: each of its blocks first works
 // out the request's end from the pieces (a few kilobytes out of L2, with the noise on its way meanwhile), then looks through its part, and the block that comes last
-// writes the request's answer.  Pieces are as many as fill the device a few times over: a block's start (which request is this, what is its temperature; where does it
-// end) costs as much as some 20,000 entries.  Both keep the batches to come on their way while they look at the one at
-// hand, some 64 KB an SM.  64 requests of six bfloat16 rows of 152,064 logits, with the drafter's: 40 us for 165 MB, 4.1 TB/s, of which the two starts and the turn from one
-// kernel to the other are some 10 us (one batch of 8 KB ahead in the first and none in the second: 47 us).  A NaN counts as -infinity, +infinity as the largest number; a row without any finite logit has p = 0 everywhere, and its
+// writes the request's answer.  Pieces are as many as the device holds blocks at once: a block's start (which request is this, what is its temperature; where does it
+// end) costs as much as some 20,000 entries.  Both keep the batches to come on their way while they look at the one at hand, some 64 KB an SM.  64 requests of up to six
+// bfloat16 rows of 152,064 logits, with the drafter's probabilities: 40 us for 165 MB, 4.1 TB/s (one batch of 8 KB ahead in the first kernel and none in the second: 47 us).  One
+// request of five float rows: 9.3 us, two kernels' starts and a few trips to memory.  A NaN counts as -infinity, +infinity as the largest number; a row without any finite logit has p = 0 everywhere, and its
 // token is the lowest index.
 #include <float.h>
 

@@ -59,7 +59,8 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
 
 def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tensor, plan: SharedPlan, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """The planned step's queries ``q`` [tokens, >= heads * d] (bfloat16, a view of wider rows is fine) over their requests' pages: ``cache`` is a dense
-    bfloat16 tensor [pages, 2, kv_heads, page, d] or a :class:`.cache8.Cache8`, ``block_table`` [requests, blocks] int32.  Returns [tokens, heads * d].
+    bfloat16 tensor [pages, 2, kv_heads, page, d] or a :class:`.cache8.Cache8`, ``block_table`` [requests, blocks] int32, ``scale`` above 0.  Rows of ``q``
+    stand on 16-byte boundaries, rows of ``out`` on 8-byte ones.  Returns [tokens, heads * d].
 
     Slots beyond a request's length may hold anything.  What a request's own later tokens hold is masked by weights of 0 for its earlier ones, so
     their values have to be finite."""
