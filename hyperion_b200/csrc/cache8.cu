@@ -10,9 +10,9 @@
 // them, and a value fits bfloat16 without another rounding.  The bounds of e keep products of two scales inside float's range.
 //
 // codes [pages, 2, kv_heads, page, d] bytes, exponents [pages, 2, kv_heads, page] signed bytes.  Both kernels are bound by memory: the threads of a record stand side by
-// side with WIDTH entries each, and a thread serves PER tokens whose places are all looked up, and whose entries are all fetched, before the first is used.  8 heads of 128, to and
-// from bfloat16: 8,191 tokens written in 12.1 us (50 MB, 4.2 TB/s: one turn of the device, a start and two dependent trips to memory), 131,072 read in 76 us (404 MB, 5.3 TB/s,
-// 0.82 of a plain copy's rate).
+// side with WIDTH entries each, and a thread serves PER tokens whose places are all looked up, and whose entries are all fetched, before the first is used.  To and
+// from bfloat16, heads of 128: 8,191 tokens of 8 heads are written in 12.1 us (50 MB, 4.2 TB/s: one turn of the device, a start and two dependent trips to memory),
+// 131,072 of 4 heads read in 76 us (404 MB, 5.3 TB/s, 0.82 of a plain copy's rate).
 #include "common.cuh"
 
 namespace {
