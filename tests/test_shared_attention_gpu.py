@@ -155,6 +155,28 @@ def test_a_nan_in_a_seen_place_stays_one():
     assert torch.isnan(got[0].view(2, 64)[:, 5]).all() and torch.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("counts,lengths,groups", [([3], [200], ()), ([300], [1301], ()), ([1] * 70, [700] * 70, ((0, 70, 513),))])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_rows_that_see_a_key_without_a_number(bits, bad, counts, lengths, groups):
+    """A NaN or a positive infinity among a row's scores makes the row NaN; a negative infinity is a weight of 0; rows that do not see the key stay as they are."""
+    if bits == 8 and bad == "inf":
+        return  # e4m3 has no infinity
+    q, cache, table = step(counts, lengths, 8, 2, 128, 16, bits, groups, seed=8)
+    at = lengths[0] - counts[0] + counts[0] // 2 if not groups else 300
+    place = int(table[0, at // 16]), 0, 1, at % 16, 7  # an entry of a key of the second key/value head
+    if bits == 8:
+        cache.codes.view(torch.uint8)[place] = 0x7F
+    else:
+        cache[place] = float(bad)
+    got = attention_shared(q, 8, cache, table, plan_shared(counts, lengths, 8, 2, 128, shared=groups), 0.1)
+    ops.raise_on_status(got.device)
+    want, size = plain(q, 8, cache, table, counts, lengths, 0.1)
+    assert torch.isnan(want).any() and not torch.isnan(want).all()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    agree(torch.nan_to_num(got), torch.nan_to_num(want), torch.nan_to_num(size))
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 @pytest.mark.parametrize("size", [1e-3, 30.0])
 def test_large_and_small_scores(bits, size):
