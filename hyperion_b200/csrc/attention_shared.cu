@@ -737,12 +737,24 @@ int launch_strips(const Args& a, const void* cache, int blocks, cudaStream_t str
 }
 }  // namespace
 
+// Puts the n_pieces = piece_start[tokens] pieces [n_pieces, heads, D] of the tokens together.  A token without a piece is zeros.
+HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const int* piece_start, void* out, int out_stride, int tokens, int n_pieces, int heads, cudaStream_t stream) {
+    if (tokens <= 0) return 0;
+    if (!pieces || !sums || !piece_start || !out || heads <= 0 || out_stride % 2 || ((uintptr_t)pieces & 15) || ((uintptr_t)out & 3)) return HB_BAD_ARGUMENT;
+    const bool many = n_pieces / tokens > 12;
+    const int per_block = many ? 1 : MERGE_WARPS, rows = (heads + per_block - 1) / per_block;
+    if (rows > 65535) return HB_UNSUPPORTED_SIZE;
+    return launch_after_previous(many ? attention_pieces_kernel<MERGE_WARPS> : attention_pieces_kernel<1>, dim3(tokens, rows), dim3(32 * MERGE_WARPS), 0, stream, pieces, (const float2*)sums,
+                                 piece_start, (bf16*)out, out_stride, heads);
+}
+
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
 // beside_tiles: hb_attention_shared_tiles for the same step was the launch right before on this stream.
-// items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row.
+// items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row;
+// else tokens and n_pieces as hb_attention_pieces takes them, which follows.
 HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
                                   const int* items, const int* first_item, int blocks, int rows, int beside_tiles, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
-                                  int page_size, int pages, float scale, int* status, cudaStream_t stream) {
+                                  int page_size, int pages, float scale, int* status, cudaStream_t stream, int tokens, int n_pieces) {
     if (blocks <= 0) return 0;
     if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || q_stride % 8 || out_stride % 4) return HB_BAD_ARGUMENT;
@@ -754,17 +766,7 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, beside_tiles, gc, chunks, scale * 1.4426950408889634f, status};
-    if (rows == 8) return exponents ? launch_strips<true, 1>(a, cache, blocks, stream) : launch_strips<false, 1>(a, cache, blocks, stream);
-    return exponents ? launch_strips<true, 2>(a, cache, blocks, stream) : launch_strips<false, 2>(a, cache, blocks, stream);
-}
-
-// Puts the n_pieces = piece_start[tokens] pieces [n_pieces, heads, D] of the tokens together.  A token without a piece is zeros.
-HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const int* piece_start, void* out, int out_stride, int tokens, int n_pieces, int heads, cudaStream_t stream) {
-    if (tokens <= 0) return 0;
-    if (!pieces || !sums || !piece_start || !out || heads <= 0 || out_stride % 2 || ((uintptr_t)pieces & 15) || ((uintptr_t)out & 3)) return HB_BAD_ARGUMENT;
-    const bool many = n_pieces / tokens > 12;
-    const int per_block = many ? 1 : MERGE_WARPS, rows = (heads + per_block - 1) / per_block;
-    if (rows > 65535) return HB_UNSUPPORTED_SIZE;
-    return launch_after_previous(many ? attention_pieces_kernel<MERGE_WARPS> : attention_pieces_kernel<1>, dim3(tokens, rows), dim3(32 * MERGE_WARPS), 0, stream, pieces, (const float2*)sums,
-                                 piece_start, (bf16*)out, out_stride, heads);
+    const auto launch = rows == 8 ? (exponents ? launch_strips<true, 1> : launch_strips<false, 1>) : (exponents ? launch_strips<true, 2> : launch_strips<false, 2>);
+    if (int code = launch(a, cache, blocks, stream)) return code;
+    return pieces ? hb_attention_pieces(pieces, sums, piece_start, out, out_stride, tokens, n_pieces, heads, stream) : 0;
 }
