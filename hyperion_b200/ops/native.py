@@ -8,6 +8,7 @@ device, a failed build or a refused size raises.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Any
 
 import torch
@@ -120,22 +121,28 @@ def stream_address() -> int:
     return (bound.value or 0) if bound is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-_scratch: dict = {}
+class _Scratch(threading.local):
+    def __init__(self):
+        self.kept: dict = {}
+
+
+_scratch = _Scratch()
 KEPT_SCRATCH = 16 << 20  # bytes; above it a tensor of its own costs nothing beside the work that wants it
 
 
 def scratch(device: torch.device, stream: int, size: int):
-    """(address, owner) of ``size`` bytes on a boundary of 512 for one call's launches on ``stream``: launches of one stream follow one another, so each stream keeps one piece of
-    memory for all of them.  The caller holds the owner until its launches are under way.  A graph that is being captured gets memory of its own (its replays may run beside
-    other work of that stream), and so do large wishes."""
+    """(address, owner) of ``size`` bytes on a boundary of 512 for one call's launches on ``stream``: launches of one stream follow one another, so a thread keeps one piece of
+    memory per stream for all of them (another thread's may come between two launches of one call).  The caller holds the owner until its launches are under way.  A graph
+    that is being captured gets memory of its own (its replays may run beside other work of that stream), and so do large wishes."""
     if size > KEPT_SCRATCH or torch._C._cuda_isCurrentStreamCapturing():
         owner = torch.empty(max(1, size), dtype=torch.uint8, device=device)
         return owner.data_ptr(), owner
-    found = _scratch.get((device.index, stream))
+    kept = _scratch.kept
+    found = kept.get((device.index, stream))
     if found is None or found[2] < size:
         room = max(1 << 16, 1 << (size - 1).bit_length()) if size else 1 << 16
         owner = torch.empty(room, dtype=torch.uint8, device=device)
-        found = _scratch[device.index, stream] = (owner.data_ptr(), owner, room)
+        found = kept[device.index, stream] = (owner.data_ptr(), owner, room)
     return found[0], found[1]
 
 

@@ -4,6 +4,8 @@ Tolerance: weights are rounded once (bfloat16, 2^-9, over bfloat16 caches; float
 to some 50 in the exponent, sums of up to 10^4 weights) is below 2^-12.  An entry is off by at most (2^-8 + 2^-11) * sum_j p_j |v_j|."""
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -219,6 +221,20 @@ def test_strides_and_streams(bits):
         got = attention_shared(wide[:, 512:], 8, cache, table, plan, 0.125, out=out)
     stream.synchronize()
     assert torch.equal(got[:, :512], want) and (out[:, 512:] == 3).all()
+
+
+def test_threads_on_one_stream():
+    """Calls of several kernels from threads that launch on the same stream do not write over one another's pieces."""
+    def work(seed):
+        counts, lengths = [1] * 8, [2000 + 37 * seed + r for r in range(8)]
+        q, cache, table = step(counts, lengths, 14, 2, 64, 16, 8, seed=seed)
+        plan = plan_shared(counts, lengths, 14, 2, 64)
+        assert plan.joined
+        want = attention_shared(q, 14, cache, table, plan, 0.1)
+        return all(torch.equal(want, attention_shared(q, 14, cache, table, plan, 0.1)) for _ in range(300))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
 
 
 def test_pages_behind_32_bit_offsets():
