@@ -6,7 +6,10 @@
 // be cut further so that the device is filled.  An item leaves for each of its (token, head) rows a piece
 //     m,  l = sum_j 2^(y_j - m),  o = sum_j 2^(y_j - m) v_j          y_j = score_j * scale * log2(e)
 // and the pieces of a row are put together afterwards, in the order of the ranges: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
-// A step whose rows have one piece each is stored at once.
+// A step whose rows have one piece each is stored at once.  Where every row has one range and the device has room for two to eight blocks a range, those are a cluster: each walks its
+// share, and at the end they read one another's results out of shared memory (mapa, ld.shared::cluster), so that no piece goes through memory and no kernel follows.  (Both ways, over
+// 8-bit records, 28 heads over 4: one request at 512 positions 6.3 us against 7.6, eight at 2,048 10.4 against 10.8, 32 at 2,048 21 against 26, 32 at 9,000 59 against 86; a call
+// that the host bounds 12 against 15.5.)
 //
 // This file has the strip kernel, for items of few rows: it is bound by the bytes of the keys and values.  One lane of a producer warp per
 // page fetches K and V by TMA (one box a page and 128-byte panel, no multicast) into a ring of stages; each of four warps takes a quarter of a
@@ -28,9 +31,10 @@
 // Over a bfloat16 cache the weights are taken in two parts, rounded to bfloat16 and what that left over: rounded once they would cost the result as much as
 // its own rounding does (1.4 times the error in all), and float16, whose rounding does not show, does not hold every bfloat16 value.
 //
-// Measured: 64 requests at 2,048 positions each, 28 heads over 4 of 128, 32 us over 8-bit records (3.2 TB/s) and 44 us over bfloat16 (4.6 TB/s), the joining included.  Over
+// Measured: 64 requests at 2,048 positions each, 28 heads over 4 of 128, 31 us over 8-bit records (3.3 TB/s) and 43 us over bfloat16 (4.7 TB/s), the joining by a kernel included; 32 at
+// 9,000, in clusters, 59 us (5.0 TB/s) and 94 us (6.3 TB/s).  Over
 // bfloat16 the bytes and the starts and ends of the blocks bound it, over 8-bit records the instructions around the products (conversion, exponents, softmax of rows that stand
-// across lanes).  One token of 14 heads at 512 positions: 7 us, a start and three dependent trips to memory.
+// across lanes).  One token of 14 heads at 512 positions: 5.5 us, a start and three dependent trips to memory.
 //
 // Slots beyond a range's end may hold anything: their scores are replaced and their values are read as zeros.  Every mbarrier wait is
 // bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the block leaves.
@@ -174,12 +178,35 @@ struct Args {
     float2* sums;            // [pieces, heads]: (m, l)
     int heads, kv_heads, page_size, pages;
     int beside_tiles;        // the tile kernel of the same step was launched right before
+    int together;            // 0, or the blocks of a cluster, which has one run: an item each, joined among them
     int gc, chunks;          // heads of a strip, strips of a key/value head's group
     float scale_log2;
     int* status;
 };
 
-template <bool E8, int NQ>
+constexpr int MOST_TOGETHER = 8;
+// The blocks of a cluster: those of their threads that have not left.
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// What another block of the cluster has at this place of its shared memory.
+__device__ __forceinline__ unsigned their(const void* p, int rank) {
+    unsigned at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float2 theirs2(const float2* p, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(their(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 theirs4(const float* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(their(p, rank)) : "memory");
+    return v;
+}
+// TOGETHER: an instance of its own, so that the others keep the registers that the joining takes (drafts behind prefixes beside tiles 23.6 us, against 22.5).
+template <bool E8, int NQ, bool TOGETHER>
 __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_strip_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
     typedef Shape<E8, NQ> S;
     constexpr int BN = S::BN, KEYS = S::KEYS, NK = KEYS / 16, ROWS = S::ROWS;
@@ -267,9 +294,13 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                 }
             }
         }
+        if constexpr (TOGETHER) cluster_meet(), cluster_meet();
         return;
     }
     // ---------------------------------------------------------------------- consumers
+    [[maybe_unused]] float* rows_here = reinterpret_cast<float*>(ring);  // [ROWS][D]: what a block of a cluster brings; the ring has been read to its end by then
+    [[maybe_unused]] float2* sums_here = reinterpret_cast<float2*>(rows_here + ROWS * D);  // [ROWS]
+    static_assert(ROWS * (D * 4 + 8) <= S::STAGES * 2 * S::TILE, "a cluster's results lie where the ring was");
     const int t = lane & 3, g = lane >> 2;
     [[maybe_unused]] float* mine = factors + warp * 3 * KEYS;  // of this warp's keys: 2^e of the key, e of the value, 2^-e of the value
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); };
@@ -556,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                 if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e], parts[warp * ROWS + q * 8 + 2 * t + e] = l[q][e];
             }
         meet();
-        if (*lost) return;  // all four warps see the same: they set it before they come here only
+        if (*lost && !TOGETHER) return;  // all four warps see the same: they set it before they come here only.  (A cluster's blocks leave together, whatever it is that they join.)
         float f[NQ][2];
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
@@ -576,7 +607,8 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
         }
         const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);  // a row that sees nothing is zeros; a NaN stays one
         const size_t slot = (size_t)piece_at * a.heads + first_head + store_head;
-        if (stores && a.pieces && store_col == 0) a.sums[slot] = make_float2(top, total);
+        if (!TOGETHER && stores && a.pieces && store_col == 0) a.sums[slot] = make_float2(top, total);
+        if (TOGETHER && stores && store_col == 0) sums_here[store_row] = make_float2(top, total);
 #pragma unroll
         for (int col = 0; col < D; col += S::COLS) {
 #pragma unroll
@@ -602,7 +634,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[i] += more[i];
                 }
-                if (a.pieces) {
+                if (TOGETHER) {
+                    store4(rows_here + store_row * D + col + store_col, sum);
+                } else if (a.pieces) {
                     store4(a.pieces + slot * D + col + store_col, sum);
                 } else {
 #pragma unroll
@@ -611,6 +645,41 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                 }
             }
             meet();
+        }
+        if constexpr (TOGETHER) {
+            // Every block of the cluster takes a part of the rows' entries, brings the blocks' sums to the largest maximum, in the order of the blocks, and stores.
+            cluster_meet();
+            unsigned rank;
+            asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+            for (int at = (int)rank * 32 * WARPS + tid; at < ROWS * (D / 4); at += a.together * 32 * WARPS) {
+                const int row = at / (D / 4), col = at % (D / 4) * 4, tok = row / a.gc, head = row - tok * a.gc;
+                if (tok >= ntok || head >= heads_here) continue;
+                float above = -INFINITY, all = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < MOST_TOGETHER; ++r) above = fmaxf(above, theirs2(sums_here + row, min(r, a.together - 1)).x);
+#pragma unroll 1
+                for (int r0 = 0; r0 < a.together; r0 += 4) {  // four on their way together
+                    float2 ml[4];
+                    float4 part[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int from = min(r0 + r, a.together - 1);
+                        ml[r] = theirs2(sums_here + row, from), part[r] = theirs4(rows_here + row * D + col, from);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (r0 + r >= a.together) break;
+                        const float f = ml[r].x == -INFINITY ? 0.f : fast_exp2(ml[r].x - above);
+                        all = fmaf(f, ml[r].y, all);
+                        sum[0] = fmaf(f, part[r].x, sum[0]), sum[1] = fmaf(f, part[r].y, sum[1]), sum[2] = fmaf(f, part[r].z, sum[2]), sum[3] = fmaf(f, part[r].w, sum[3]);
+                    }
+                }
+                const float share = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] *= share;
+                store4(a.out + (size_t)(tok0 + tok) * a.out_stride + (size_t)(first_head + head) * D + col, sum);
+            }
+            cluster_meet();  // nobody leaves while another still reads here
         }
     }
     if (a.beside_tiles) wait_for_previous_kernels();
@@ -727,13 +796,34 @@ int cache_map(CUtensorMap* map, const void* cache, int pages, int kv_heads, int 
     return r == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
 }
 
+// launch_after_previous with clusters of `together` blocks along x.
+template <typename... Params, typename... Values>
+int launch_clusters(void (*kernel)(Params...), int together, dim3 grid, dim3 block, size_t shared_bytes, cudaStream_t stream, Values&&... values) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid, config.blockDim = block, config.dynamicSmemBytes = shared_bytes, config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = overlap_launches() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {(unsigned)together, 1, 1};
+    config.attrs = attributes, config.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(values)...);
+}
+
+template <bool E8, int NQ, bool TOGETHER>
+int launch_strips_as(const Args& a, const CUtensorMap& map, int blocks, cudaStream_t stream) {
+    const auto kernel = attention_strip_kernel<E8, NQ, TOGETHER>;
+    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8, NQ>::SMEM);
+    if (configured != cudaSuccess) return (int)configured;
+    const dim3 grid(blocks, a.kv_heads * a.chunks);
+    if constexpr (TOGETHER) return launch_clusters(kernel, a.together, grid, dim3(THREADS), Shape<E8, NQ>::SMEM, stream, map, a);
+    return launch_after_previous(kernel, grid, dim3(THREADS), Shape<E8, NQ>::SMEM, stream, map, a);
+}
 template <bool E8, int NQ>
 int launch_strips(const Args& a, const void* cache, int blocks, cudaStream_t stream) {
     CUtensorMap map;
     if (int code = cache_map<E8, NQ>(&map, cache, a.pages, a.kv_heads, a.page_size)) return code;
-    static const cudaError_t configured = cudaFuncSetAttribute(attention_strip_kernel<E8, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<E8, NQ>::SMEM);
-    if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(attention_strip_kernel<E8, NQ>, dim3(blocks, a.kv_heads * a.chunks), dim3(THREADS), Shape<E8, NQ>::SMEM, stream, map, a);
+    return a.together ? launch_strips_as<E8, NQ, true>(a, map, blocks, stream) : launch_strips_as<E8, NQ, false>(a, map, blocks, stream);
 }
 }  // namespace
 
@@ -749,11 +839,12 @@ HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const 
 }
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
-// beside_tiles: hb_attention_shared_tiles for the same step was the launch right before on this stream.
+// beside_tiles: hb_attention_shared_tiles for the same step was the launch right before on this stream.  together: 0, or 2 to 8: so many blocks in a row have one item each, of the same
+// tokens, and join them; no pieces then.
 // items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row;
 // else tokens and n_pieces as hb_attention_pieces takes them, which follows.
 HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
-                                  const int* items, const int* first_item, int blocks, int rows, int beside_tiles, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
+                                  const int* items, const int* first_item, int blocks, int rows, int beside_tiles, int together, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
                                   int page_size, int pages, float scale, int* status, cudaStream_t stream, int tokens, int n_pieces) {
     if (blocks <= 0) return 0;
     if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
@@ -762,10 +853,11 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)pieces) & 15) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     if (rows != 8 && rows != MOST_ROWS) return HB_UNSUPPORTED_SIZE;
+    if (together && (together < 2 || together > MOST_TOGETHER || blocks % together || pieces || beside_tiles)) return HB_BAD_ARGUMENT;
     const int group = heads / kv_heads, gc = group < rows ? group : rows, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
-                 heads, kv_heads, page_size, pages, beside_tiles, gc, chunks, scale * 1.4426950408889634f, status};
+                 heads, kv_heads, page_size, pages, beside_tiles, together, gc, chunks, scale * 1.4426950408889634f, status};
     const auto launch = rows == 8 ? (exponents ? launch_strips<true, 1> : launch_strips<false, 1>) : (exponents ? launch_strips<true, 2> : launch_strips<false, 2>);
     if (int code = launch(a, cache, blocks, stream)) return code;
     return pieces ? hb_attention_pieces(pieces, sums, piece_start, out, out_stride, tokens, n_pieces, heads, stream) : 0;

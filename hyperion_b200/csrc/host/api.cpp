@@ -293,6 +293,7 @@ HB_API int hb_plan_shared(int n_requests, const int64_t* counts, const int64_t* 
             *places++ = (int64_t)planned.size();
             planned.insert(planned.end(), part->begin(), part->end());
         }
+        sizes[17] = plan.together;
         const int64_t figures[9] = {(int64_t)planned.size(), plan.strips.blocks(), plan.strip_rows, plan.tiles.blocks(), (int64_t)plan.last.size(), plan.starts.back(), plan.joined, plan.longest, (int64_t)plan.operands.size() / 4};
         std::copy(figures, figures + 9, sizes);
     });

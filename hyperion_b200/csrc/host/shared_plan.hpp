@@ -23,6 +23,8 @@ struct Walk {  // of one kernel: block b takes items first[b] .. first[b + 1] - 
 struct SharedPlan {
     Walk strips, tiles;
     int strip_rows = 8;
+    // 0, or how many blocks in a row walk one run between them, an item each (an empty one is keys 0 to 0), and put its pieces together themselves: a cluster.
+    int together = 0;
     // The tiles of the wide ranges, each as (table row, first position, first key, last key + 1 of its range): what 8-bit records are made into operands for.
     std::vector<int> operands;
     std::vector<int> last, starts, own;  // the last position a token sees, its first piece, its first piece of its own request's positions

@@ -30,7 +30,7 @@ class SharedPlan:
     """What the launches of a step need (csrc/host/shared_plan.hpp): which block of which kernel walks which keys for which tokens, the last position each token sees and its
     pieces, in one int32 tensor."""
 
-    __slots__ = ("requests", "tokens", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strip_blocks", "strip_rows", "tile_blocks", "operand_tiles", "data", "places", "at")
+    __slots__ = ("requests", "tokens", "heads", "kv_heads", "head_dim", "longest", "pieces", "joined", "strip_blocks", "strip_rows", "tile_blocks", "operand_tiles", "together", "data", "places", "at")
 
 
 def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_heads: int, head_dim: int, *, shared: Sequence[tuple[int, int, int]] = (),
@@ -42,7 +42,7 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     n, length, groups = (host_runtime.ints(values, np.int64) for values in (counts, lengths, shared))
     if n.ndim != 1 or n.shape != length.shape or (len(groups) and groups.shape[1:] != (3,)):
         raise KernelError("plan_shared: a count of queries and a length for each request, and groups as (first request, requests, positions)")
-    lib, sizes = host_runtime.library(), np.empty(17, dtype=np.int64)
+    lib, sizes = host_runtime.library(), np.empty(18, dtype=np.int64)
     errors = {host_runtime.BAD_ARGUMENT: KernelError}
     host_runtime.check(lib.hb_plan_shared(len(n), host_runtime.address(n), host_runtime.address(length), len(groups), host_runtime.address(groups), heads, kv_heads,
                                           sms or sm_count(device), host_runtime.address(sizes)), errors)
@@ -52,7 +52,8 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     plan.requests, plan.heads, plan.kv_heads, plan.head_dim = len(n), heads, kv_heads, head_dim
     plan.strip_blocks, plan.strip_rows, plan.tile_blocks, plan.tokens, plan.pieces, plan.joined, plan.longest, plan.operand_tiles = sizes[1:9].tolist()
     plan.data = words.to(device)
-    plan.places = sizes[9:].tolist()  # strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces, operand tiles
+    plan.together = int(sizes[17])
+    plan.places = sizes[9:17].tolist()  # strip items, strip blocks' first items, tile items, tile blocks' first items, last positions, first pieces, first own pieces, operand tiles
     plan.at = [plan.data.data_ptr() + 4 * place for place in plan.places]
     return plan
 
@@ -96,11 +97,12 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     strip_items, strip_first, tile_items, tile_first, last, starts, own, operand_list = plan.at
     out_at, out_stride, stream = out.data_ptr(), out.stride(0), stream_address()
     pieces = sums = operands = 0
-    if plan.joined or plan.operand_tiles:
-        for_pieces = (plan.pieces * heads * (head_dim + 2) * 4 + 511) // 512 * 512 if plan.joined else 0
+    joined = plan.joined and not plan.together
+    if joined or plan.operand_tiles:
+        for_pieces = (plan.pieces * heads * (head_dim + 2) * 4 + 511) // 512 * 512 if joined else 0
         makes = plan.operand_tiles if exponents else 0  # what runs of many rows walk is made into operands first
         memory, owner = scratch(q.device, stream, for_pieces + makes * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16))
-        if plan.joined:
+        if joined:
             pieces, sums = memory, memory + 4 * plan.pieces * heads * head_dim
         if makes:
             operands = memory + for_pieces
@@ -113,8 +115,8 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
         check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipipppppiiiifpp", head_dim)(
             q.data_ptr(), q.stride(0), tokens, out_at, out_stride, *where, tile_items, tile_first, plan.tile_blocks, operands, plan.operand_tiles, *what), "attention_shared")
     if plan.strip_blocks:
-        check(entry("attention_shared", "hb_attention_strips", "pipipppippiiipppppiiiifppii", head_dim)(
-            q.data_ptr(), q.stride(0), out_at, out_stride, *where, strip_items, strip_first, plan.strip_blocks, plan.strip_rows, int(plan.tile_blocks > 0), *what, tokens, plan.pieces), "attention_shared")
-    elif plan.joined:
+        check(entry("attention_shared", "hb_attention_strips", "pipipppippiiiipppppiiiifppii", head_dim)(
+            q.data_ptr(), q.stride(0), out_at, out_stride, *where, strip_items, strip_first, plan.strip_blocks, plan.strip_rows, int(plan.tile_blocks > 0), plan.together, *what, tokens, plan.pieces), "attention_shared")
+    elif joined:
         check(entry("attention_shared", "hb_attention_pieces", "ppppiiiip", head_dim)(pieces, sums, starts, out_at, out_stride, tokens, plan.pieces, heads, stream), "attention_shared")
     return out

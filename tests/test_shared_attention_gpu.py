@@ -223,6 +223,15 @@ def test_strides_and_streams(bits):
     assert torch.equal(got[:, :512], want) and (out[:, 512:] == 3).all()
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (28, 4, 128), (40, 2, 128)])
+@pytest.mark.parametrize("counts,lengths", [([1] * 5, [1500, 0, 1, 130, 800]), ([1] * 5, [1500, 3, 1, 130, 800]), ([2, 1, 2], [700, 1100, 2]), ([1], [640]), ([1] * 30, list(range(500, 1100, 20)))])
+def test_runs_of_a_cluster(heads, kv, dim, counts, lengths, bits):
+    """Runs whose shares are joined by the blocks themselves: of few blocks and of eight, some without a key.  (A row that sees nothing is left to the kernel behind.)"""
+    assert (plan_shared(counts, lengths, heads, kv, dim).together > 0) == (0 not in lengths)
+    check(counts, lengths, heads, kv, dim, 16, bits, seed=11)
+
+
 def test_threads_on_one_stream():
     """Calls of several kernels from threads that launch on the same stream do not write over one another's pieces."""
     def work(seed):

@@ -34,7 +34,7 @@ def covered(counts, lengths, heads, kv, groups, sms):
     seen, pieces = [set() for _ in owner], [[] for _ in owner]
     for rows, (items, _) in ((plan.strip_rows, strips), (256, tiles)):
         for tok, n, row, low, high, number, operand in items:
-            assert n >= 1 and high > low and n * min(rows, heads // kv) <= rows
+            assert n >= 1 and (high > low or (plan.together and low == high == 0)) and n * min(rows, heads // kv) <= rows
             if rows == 256:  # the item's tiles stand one behind the other among the operands
                 for i, at in enumerate(range(low // 128 * 128, high, 128)):
                     assert operands[operand + i][0] == row and operands[operand + i][1] == at and operands[operand + i][2] <= low and high <= operands[operand + i][3]
@@ -50,6 +50,9 @@ def covered(counts, lengths, heads, kv, groups, sms):
         assert sorted(pieces[t]) == list(range(starts[t], starts[t + 1]))
     assert plan.operand_tiles == len(operands)
     assert plan.pieces == starts[-1] and plan.joined == any(len(p) != 1 for p in pieces)
+    if plan.together:  # blocks in a row have the same tokens, an item each
+        same = strips[0][:, :3].reshape(-1, plan.together, 3)
+        assert 2 <= plan.together <= 8 and len(tiles[0]) == 0 and (same == same[:, :1]).all() and not shared.any()
     assert (plan.strip_blocks, plan.tile_blocks) == tuple(len(np.unique(b)) for _, b in (strips, tiles))
     return plan
 
@@ -97,8 +100,23 @@ def test_wide_ranges_have_operand_tiles():
 
 
 def test_short_ranges_stay_whole():
-    plan = plan_shared([1, 1], [500, 190], 28, 4, 128, device="cpu", sms=148)
-    assert plan.strip_blocks == 2 and not plan.joined
+    plan = plan_shared([1, 1], [250, 190], 28, 4, 128, device="cpu", sms=148)
+    assert plan.strip_blocks == 2 and not plan.joined and not plan.together
+    plan = plan_shared([1, 1], [500, 190], 28, 4, 128, device="cpu", sms=148)  # a cluster for each
+    assert plan.together == 4 and plan.strip_blocks == 8
+    plan = plan_shared([1, 1, 0], [500, 190, 90], 28, 4, 128, shared=[(0, 2, 16)], device="cpu", sms=148)  # rows of two runs
+    assert not plan.together and plan.joined
+
+
+def test_clusters_walk_every_key():
+    random = np.random.default_rng(5)
+    for heads, kv in ((14, 2), (28, 4), (8, 8)):
+        for _ in range(20):
+            requests = int(random.integers(1, 12))
+            counts = random.integers(1, 4, requests)
+            lengths = counts + random.integers(0, 1500, requests)
+            lengths[0] += 400
+            assert covered(counts.tolist(), lengths.tolist(), heads, kv, [], 148).together
 
 
 def test_refusals():
