@@ -43,6 +43,14 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 }
 // exp((v - m) / temperature)
 __device__ __forceinline__ float weight_of(float v, float m, float rate) { return fast_exp2((v - m) * rate); }
+// The same for the many entries of a batch, in one multiplication and addition each: 2^(v * rate + offset) * rest with offset = -m * rate.  The offset's rounding is an absolute error of the
+// exponent, which grows with |m| / temperature; what it has been rounded by is itself a float, which one fused multiplication and addition gives, and 2^ that is the rest.
+// `exact`: the rest is between 2^-0.5 and 2^0.5; where it is not (or not finite), entries take weight_of.
+struct Offset {
+    float offset, rest;
+    bool exact;
+    __device__ __forceinline__ Offset(float m, float rate) : offset(-m * rate), rest(fast_exp2(-fmaf(m, rate, offset))), exact(fabsf(offset) < 0x1p24f) {}
+};
 __device__ __forceinline__ float max3(float a, float b, float c) {  // passes over a NaN, as fmaxf does
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -207,16 +215,15 @@ __global__ void __launch_bounds__(THREADS, ROWS_PER_SM) verify_rows_kernel(const
         for (int s = 0; s < STEPS; ++s) top = max3(max3(top, z[s][0], z[s][1]), z[s][2], z[s][3]);
         top = fminf(top, FLT_MAX);
         if (top > -INFINITY) {
-            // One multiplication and addition an entry: what m * rate is rounded by is the same for all of them.  A sum that a NaN or an infinity has got into is made again
-            // with those put right.
-            const float offset = -top * rate;
+            // A sum that a NaN or an infinity has got into is made again with those put right.
+            const Offset from(top, rate);
             float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) part[e] += fast_exp2(fmaf(z[s][e], rate, offset));
-            float more_sum = (part[0] + part[1]) + (part[2] + part[3]);
-            if (!(more_sum < INFINITY)) {
+                for (int e = 0; e < 4; ++e) part[e] += fast_exp2(fmaf(z[s][e], rate, from.offset));
+            float more_sum = ((part[0] + part[1]) + (part[2] + part[3])) * from.rest;
+            if (!(from.exact && more_sum < INFINITY)) {
                 more_sum = 0.f;
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s)
@@ -341,8 +348,9 @@ __global__ void __launch_bounds__(THREADS, REQUESTS_PER_SM) verify_requests_kern
     auto look = [&](int first, int end_at, int step, bool own) {
         Key best_key = 0;
         float best = -1.f;
-        const float offset = -m * rate;
-        const bool clean = share > 0.f && m < FLT_MAX;
+        const Offset from(m, rate);
+        const float scaled_share = share * from.rest;
+        const bool clean = share > 0.f && m < FLT_MAX && from.exact;
         const auto fetch = [&](Batch& b, int at) {  // all but the noise
             batch<T, WIDE>(logits, at, end_at, b.v);
             if (beside && !own) {
@@ -360,8 +368,8 @@ __global__ void __launch_bounds__(THREADS, REQUESTS_PER_SM) verify_requests_kern
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) z[s][e] = fast_exp2(fmaf(v[s][e], rate, offset)) * share;
-            } else {  // the row's largest logit is infinite, or there is none
+                    for (int e = 0; e < 4; ++e) z[s][e] = fast_exp2(fmaf(v[s][e], rate, from.offset)) * scaled_share;
+            } else {  // the row's largest logit is infinite, or too far from zero for the temperature, or there is none
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s)
 #pragma unroll
