@@ -56,9 +56,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// Order-preserving for all floats but NaN.
+// Order-preserving for all floats but NaN; both zeros are the same.
 __device__ __forceinline__ unsigned ordered(float v) {
-    const unsigned b = __float_as_uint(v);
+    const unsigned b = __float_as_uint(v + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ Key key_of(float v, int index) { return ((Key)ordered(v) << 32) | (unsigned)~index; }
