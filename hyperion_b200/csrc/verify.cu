@@ -30,7 +30,8 @@ constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;  // batches of a row on their way 
 constexpr int KEPT = 64;                    // rows of a request whose sums a block keeps
 
 __device__ __forceinline__ float cleaned(float v) { return v != v ? -INFINITY : fminf(v, FLT_MAX); }
-__device__ __forceinline__ float rate_of(float temperature) { return fminf(1.4426950408889634f / temperature, FLT_MAX); }
+// Above 0, too, so that a logit of -infinity has weight 0 at an infinite temperature.
+__device__ __forceinline__ float rate_of(float temperature) { return fminf(fmaxf(1.4426950408889634f / temperature, FLT_MIN), FLT_MAX); }
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
