@@ -16,7 +16,7 @@ import torch
 from .. import host as host_runtime
 from .basic import status_word
 from .cache8 import Cache8, check_cache8
-from .native import KernelError, check, entry, require_cuda, scratch, sm_count, stream_address
+from .native import KernelError, check, entry, scratch, sm_count, stream_address
 
 
 TILE_KEYS = 128  # keys of an operand tile
@@ -38,7 +38,7 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     """Plan a step of ``counts[r]`` queries of request r, whose block table (row r) holds ``lengths[r]`` positions: token i of n sees the first
     ``lengths[r] - n + i + 1`` of them (one with nothing to see comes out as zeros).  ``shared``: (first request, requests, positions) of each group
     of consecutive requests that hold the same pages for their first positions, which all of their queries see; in order, none of them overlapping.
-    ``device`` is where the plan is kept; ``sms`` its multiprocessors, asked from it when absent."""
+    ``device`` is where the plan is kept, which has to be the device of the step's tensors; ``sms`` its multiprocessors, asked from it when absent."""
     n, length, groups = (host_runtime.ints(values, np.int64) for values in (counts, lengths, shared))
     if n.ndim != 1 or n.shape != length.shape or (len(groups) and groups.shape[1:] != (3,)):
         raise KernelError("plan_shared: a count of queries and a length for each request, and groups as (first request, requests, positions)")
@@ -67,13 +67,12 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     their values have to be finite."""
     if isinstance(cache, Cache8):
         pages, kv_heads, page_size, head_dim = check_cache8(cache, "attention_shared")
-        entries, exponents = cache[0].data_ptr(), cache[1].data_ptr()
+        parts, entries, exponents = cache, cache[0].data_ptr(), cache[1].data_ptr()
     else:
         if cache.dtype is not torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
             raise KernelError("attention_shared: a dense bfloat16 cache [pages, 2, kv_heads, page, d], or a Cache8")
-        require_cuda(cache)
         pages, _, kv_heads, page_size, head_dim = cache.shape
-        entries, exponents = cache.data_ptr(), 0
+        parts, entries, exponents = (cache,), cache.data_ptr(), 0
     if not supported(head_dim, page_size):
         raise KernelError(f"attention_shared: heads of 64 or 128 entries and pages of 8, 16, 32 or 64 positions, not {head_dim} and {page_size}")
     if heads != plan.heads or kv_heads != plan.kv_heads or head_dim != plan.head_dim:
@@ -86,11 +85,12 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
         raise KernelError(f"attention_shared: a dense int32 block table of at least {plan.requests} rows")
     if shape[1] * page_size < plan.longest:
         raise KernelError(f"attention_shared: a block table of {shape[1]} pages of {page_size} does not hold {plan.longest} positions")
-    if not (q.is_cuda and block_table.is_cuda):
-        require_cuda(q, block_table)
+    device = q.device
+    if not (q.is_cuda and plan.data.device == block_table.device == parts[0].device == parts[-1].device == device) or (out is not None and out.device != device):
+        raise KernelError(f"attention_shared: queries, cache, block table, plan and output on one CUDA device; the plan is on {plan.data.device}, the queries are on {device}")
     if out is None:
-        out = torch.empty(tokens, width, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != tokens or out.shape[1] < width or out.stride(1) != 1 or not out.is_cuda:
+        out = torch.empty(tokens, width, dtype=torch.bfloat16, device=device)
+    elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != tokens or out.shape[1] < width or out.stride(1) != 1:
         raise KernelError(f"attention_shared: the output is a bfloat16 [{tokens}, >= {width}] view")
     if tokens == 0:
         return out
@@ -101,17 +101,17 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     if joined or plan.operand_tiles:
         for_pieces = (plan.pieces * heads * (head_dim + 2) * 4 + 511) // 512 * 512 if joined else 0
         makes = plan.operand_tiles if exponents else 0  # what runs of many rows walk is made into operands first
-        memory, owner = scratch(q.device, stream, for_pieces + makes * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16))
+        memory, owner = scratch(device, stream, for_pieces + makes * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16))
         if joined:
             pieces, sums = memory, memory + 4 * plan.pieces * heads * head_dim
         if makes:
             operands = memory + for_pieces
     where = (entries, exponents, block_table.data_ptr(), shape[1])
-    what = (last, starts, own, pieces, sums, heads, kv_heads, page_size, pages, scale, status_word(q.device).data_ptr(), stream)
+    what = (last, starts, own, pieces, sums, heads, kv_heads, page_size, pages, scale, status_word(device).data_ptr(), stream)
     if plan.tile_blocks:
         if operands:
             check(entry("attention_shared_tiles", "hb_shared_operands", "pppipipiiipp", head_dim)(
-                *where, operand_list, plan.operand_tiles, operands, kv_heads, page_size, pages, status_word(q.device).data_ptr(), stream), "attention_shared")
+                *where, operand_list, plan.operand_tiles, operands, kv_heads, page_size, pages, status_word(device).data_ptr(), stream), "attention_shared")
         check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipipppppiiiifpp", head_dim)(
             q.data_ptr(), q.stride(0), tokens, out_at, out_stride, *where, tile_items, tile_first, plan.tile_blocks, operands, plan.operand_tiles, *what), "attention_shared")
     if plan.strip_blocks:
