@@ -849,6 +849,7 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     if (blocks <= 0) return 0;
     if (!q || !out || !cache || !block_table || !items || !first_item || !last || !piece_start || !own_start || !status || (!pieces != !sums)) return HB_BAD_ARGUMENT;
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || q_stride % 8 || out_stride % 4) return HB_BAD_ARGUMENT;
+    if (!(scale > 0.f)) return HB_BAD_ARGUMENT;  // as in the tile kernel: a step is refused or not whatever kernels it takes
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)pieces) & 15) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map

@@ -85,6 +85,8 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
         raise KernelError(f"attention_shared: a dense int32 block table of at least {plan.requests} rows")
     if shape[1] * page_size < plan.longest:
         raise KernelError(f"attention_shared: a block table of {shape[1]} pages of {page_size} does not hold {plan.longest} positions")
+    if not scale > 0:
+        raise KernelError(f"attention_shared: a scale above 0, not {scale}")
     device = q.device
     if not (q.is_cuda and plan.data.device == block_table.device == parts[0].device == parts[-1].device == device) or (out is not None and out.device != device):
         raise KernelError(f"attention_shared: queries, cache, block table, plan and output on one CUDA device; the plan is on {plan.data.device}, the queries are on {device}")
