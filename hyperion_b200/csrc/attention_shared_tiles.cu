@@ -10,16 +10,16 @@
 //   warps 4-11   softmax, a row per thread: running maximum and sum in float, O rescaled only when the maximum has grown by much.
 // 8-bit records are made into operands before (shared_operands_kernel).
 //
-// Over bfloat16 values, weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as
-// much as its own rounding does.  8-bit values go as float16, which holds code * 2^(e - e0) exactly for exponents from e0 - 12 to e0 + 7 (e0: the largest of
-// the range's first tile; the result is scaled back at the end), and so do the weights, whose rounding then does not show and whose second part is not
-// needed.  A tile with exponents beyond that range goes the way of bfloat16 values.  A row of S is 128 float columns of tensor memory and the two parts of its P are
-// 2 x 64, so P takes exactly the place of the S it was made from, 32 keys at a time; the softmax reads S twice (for the maximum, then for the weights), 32 columns under way
-// while it works on 32.  P is handed over in two halves of the tile's keys, so that the product of the first runs under the making of the second.
-// What bounds it is the chain of a half: from the arrival of S 2,500 clocks until the last weights are handed over (of which 1,024 are the special function unit's for 128 columns,
-// which the other half's want as well), then 1,050 for the rest of O += P V, the next S and its arrival.  3,600 clocks a tile, of which the tensor core is busy for 2,048;
-// 4,000 over bfloat16, 3,072.  Tried and dropped: weights by the maximum so far with one reading of S (3,150 clocks as long as no maximum is outgrown, 5,000 when one of 256 rows'
-// is, and one often is); a part of the exponentials by a polynomial (no faster); two threads a row (4,700); an issuer for each half (the halves fall into step: 4,700).
+// Weights go to the second product in two parts, cut off to bfloat16 and what that left over: rounded once they would cost the result as
+// much as its own rounding does.  8-bit values are bfloat16 numbers as they are (code * 2^e).  (As float16, which holds codes exactly and weights in one part, a tile took a tenth less: 256 requests behind
+// 16,384 positions 128 us against 146, a portion of 1,000 tokens of 5,000 66 against 71.  But weights below 2^-25 of the largest were lost and those below 2^-14 cut short, and behind a
+// key that takes nearly all of a row's weight and brings nothing to an entry, the entry is made of thousands of those.)  A row of S is 128 float columns of tensor memory and the two
+// parts of its P are 2 x 64, so P takes exactly the place of the S it was made from, 32 keys at a time; the softmax reads S twice (for the maximum, then for the weights), 32
+// columns under way while it works on 32.  P is handed over in two halves of the tile's keys, so that the product of the first runs under the making of the second.
+// What bounds it is the chain of a half: from the arrival of S until the last weights are handed over (of which 1,024 clocks are the special function unit's for 128 columns,
+// which the other half's want as well), then the rest of O += P V, the next S and its arrival.  4,000 clocks a tile, of which the tensor core is busy for 3,072.
+// Tried and dropped, with weights as float16 and 3,600 clocks a tile: weights by the maximum so far with one reading of S (3,150 clocks as long as no maximum is outgrown, 5,000 when one of
+// 256 rows' is, and one often is); a part of the exponentials by a polynomial (no faster); two threads a row (4,700); an issuer for each half (the halves fall into step: 4,700).
 //
 // Slots beyond an item's range may hold anything: their scores are replaced, and their values are zeros before a product reads them (operands are made so; over
 // bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded; a wait that runs out sets
@@ -49,7 +49,6 @@ constexpr int O_COL = 256;
 constexpr int ITEM_WORDS = 7;                 // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of its own positions), first operand tile
 constexpr int OWN_PIECE = 1 << 30;
 enum Source : int { BFLOAT16 = 0, OPERANDS = 1 };  // what the tiles come from: a bfloat16 cache, or operands made of an 8-bit one
-constexpr int LOWEST = -12, HIGHEST = 7;       // of e - e0, for values as float16
 constexpr unsigned WAIT_LIMIT = 1u << 24;
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -142,26 +141,12 @@ __device__ __forceinline__ void umma_pv_32(unsigned tmem_o, unsigned tmem_p, uns
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %3, q;\n\t}"
         ::"r"(tmem_o), "r"(tmem_p), "r"(v_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
 }
-// The same with P in one part.
-__device__ __forceinline__ void umma_pv_32_whole(unsigned tmem_o, unsigned tmem_p, unsigned v_low, unsigned idesc, unsigned first) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t.reg .b32 bl, pa;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.eq.b32 q, 0, 0;\n\t"
-        "mov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t"
-        "add.u32 bl, %2, 128;\n\t"
-        "add.u32 pa, %1, 8;\n\t"
-        "mov.b64 db, {bl, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [pa], db, %3, q;\n\t}"
-        ::"r"(tmem_o), "r"(tmem_p), "r"(v_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
-}
 __device__ __forceinline__ void umma_commit_at(unsigned bar_addr) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr) : "memory");
 }
-// float accumulator, both operands bfloat16 or both float16, A K-major, M 128, N n; B MN-major when b_mn.
-__device__ __forceinline__ unsigned idesc_for(int n, bool b_mn, bool f16) {
-    return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(BM >> 4) << 24);
+// float accumulator, both operands bfloat16, A K-major, M 128, N n; B MN-major when b_mn.
+__device__ __forceinline__ unsigned idesc_for(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(BM >> 4) << 24);
 }
 // 32 consecutive columns of this thread's lane, on their way; arrived() says that they are there, and nothing that reads them can stand before it.
 __device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
@@ -187,11 +172,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
 __device__ __forceinline__ unsigned pack_bf16x2(float lo, float hi) {
     unsigned w;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
-    return w;
-}
-__device__ __forceinline__ unsigned pack_f16x2(float lo, float hi) {
-    unsigned w;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
     return w;
 }
 // Two floats at a time.
@@ -222,12 +202,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ void tmem_st16_words(unsigned taddr, const unsigned (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
 __device__ __forceinline__ float value_of_half(unsigned short h) {
     float f;
     asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(h));
@@ -235,7 +209,7 @@ __device__ __forceinline__ float value_of_half(unsigned short h) {
 }
 
 struct Args {
-    const unsigned char* operands; const int* kinds;  // [tiles, kv_heads, 2, TILE_BYTES]; [tiles, kv_heads]: 2 * (e0 + 64) + whether the values are float16
+    const unsigned char* operands;  // [tiles, kv_heads, 2, TILE_BYTES]
     bf16* out; int out_stride;
     const int* block_table; int table_width;
     const int* items;
@@ -252,10 +226,8 @@ struct Args {
 };
 
 // How far (in powers of two) a maximum may be outgrown before the row is rescaled.  A stale maximum changes no result (numerator and denominator use the same
-// one) as long as nothing overflows: weights are float16, whose largest is
-// just below 2^16, or bfloat16; their sums are float.  A row that outgrows its own makes its half of the tile wait while O is scaled.
-template <Source FROM>
-constexpr float OUTGROWN = FROM == OPERANDS ? 15.5f : 32.f;
+// one) as long as nothing overflows: weights are bfloat16, their sums float, and values end below 2^49.  A row that outgrows its own makes its half of the tile wait while O is scaled.
+constexpr float OUTGROWN = 32.f;
 
 constexpr int Q_BYTES = PANELS * Q_PANEL * 2;
 constexpr int THREADS = 32 * 12;
@@ -265,27 +237,18 @@ static_assert(SMEM_USED <= 227 * 1024, "an SM's shared memory");
 // more than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory
 constexpr size_t SMEM_BYTES = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;
 
-// Sixteen codes times 2^e as operands: float16 (-12 <= e <= 7) or bfloat16.
-template <bool HALVES>
+// Sixteen codes times 2^e as bfloat16, which holds them exactly.
 __device__ __forceinline__ void widen(const uint4& codes, int e, unsigned (&wide)[8]) {
     const unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
-    if constexpr (HALVES) {
-        const unsigned half = (unsigned)(15 + min(max(e, LOWEST), HIGHEST)) << 10, factor = half | half << 16;
+    const float f = __uint_as_float((unsigned)(127 + e) << 23);
+    const Pair factor{f, f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            asm("{.reg .b16 lo, hi;\n\t.reg .b32 a, b;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 a, lo;\n\tcvt.rn.f16x2.e4m3x2 b, hi;\n\t"
-                "mul.rn.f16x2 %0, a, %3;\n\tmul.rn.f16x2 %1, b, %3;\n\t}" : "=r"(wide[2 * k]), "=r"(wide[2 * k + 1]) : "r"(words[k]), "r"(factor));
-    } else {
-        const float f = __uint_as_float((unsigned)(127 + e) << 23);
-        const Pair factor{f, f};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            unsigned h0, h1;
-            asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
-            const Pair v0 = mul2(Pair{value_of_half((unsigned short)h0), value_of_half((unsigned short)(h0 >> 16))}, factor);
-            const Pair v1 = mul2(Pair{value_of_half((unsigned short)h1), value_of_half((unsigned short)(h1 >> 16))}, factor);
-            wide[2 * k] = pack_bf16x2(v0.x, v0.y), wide[2 * k + 1] = pack_bf16x2(v1.x, v1.y);
-        }
+    for (int k = 0; k < 4; ++k) {
+        unsigned h0, h1;
+        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(h0), "=r"(h1) : "r"(words[k]));
+        const Pair v0 = mul2(Pair{value_of_half((unsigned short)h0), value_of_half((unsigned short)(h0 >> 16))}, factor);
+        const Pair v1 = mul2(Pair{value_of_half((unsigned short)h1), value_of_half((unsigned short)(h1 >> 16))}, factor);
+        wide[2 * k] = pack_bf16x2(v0.x, v0.y), wide[2 * k + 1] = pack_bf16x2(v1.x, v1.y);
     }
 }
 
@@ -367,7 +330,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
         it.halves = it.ntok * a.gc > BM ? 2 : 1;
         return it;
     };
-    auto kind_of = [&](const Item& it, int tile) { return a.kinds[(size_t)(it.operand + tile) * a.kv_heads + kvh]; };
     auto fail = [&] { *failed = 1; };
 
     if (warp == 0) {
@@ -450,8 +412,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
     } else if (warp == 1) {
         // ------------------------------------------------------------------ tensor-core issuer: the warp stays together, so that descriptors are its common values
         // (uniform registers); one elected lane issues.  Under `if (lane == 0)` every product took 65 clocks to
-        // issue, as long as it runs, and the waits came on top (a tile 4,000 clocks instead of 3,600).
-        const unsigned idesc_s = idesc_for(BN, false, false), idesc_o = idesc_for(D, true, false), idesc_half = idesc_for(D, true, true);
+        // issue, as long as it runs, and the waits came on top (a tile a tenth slower).
+        const unsigned idesc_s = idesc_for(BN, false), idesc_o = idesc_for(D, true);
         const unsigned q_low0 = low_k_major(qs), k_low0 = low_k_major(k_ring), v_low0 = low_mn_major(v_ring, KV_PANEL * 2);
         auto wait_for = [&](unsigned long long* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, failed)) != 0; };
         auto issue_s = [&](int x, int g) {  // S_x = Q_x K(g)^T
@@ -463,16 +425,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                 umma_commit_at(smem_u32(&s_full[x]));
             }
         };
-        auto issue_pv = [&](int x, int g, int part, bool halves, unsigned accumulate) {  // O_x (+)= P_x V(g) over the upper (part 0) or the lower 64 keys
+        auto issue_pv = [&](int x, int g, int part, unsigned accumulate) {  // O_x (+)= P_x V(g) over the upper (part 0) or the lower 64 keys
             const unsigned at = part ? 0u : 64u, v_low = v_low0 + (unsigned)(g & 1) * (TILE_BYTES >> 4) + at * 8, o = tmem + O_COL + x * BM, p = tmem + x * BN + at;
             if (elected()) {
-                if (halves) {
-                    umma_pv_32_whole(o, p, v_low, idesc_half, accumulate);
-                    umma_pv_32_whole(o, p + 32, v_low + 256, idesc_half, 1u);
-                } else {
-                    umma_pv_32(o, p, v_low, idesc_o, accumulate);
-                    umma_pv_32(o, p + 32, v_low + 256, idesc_o, 1u);
-                }
+                umma_pv_32(o, p, v_low, idesc_o, accumulate);
+                umma_pv_32(o, p + 32, v_low + 256, idesc_o, 1u);
             }
         };
         auto commit = [&](unsigned long long* bar) {
@@ -493,14 +450,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
             if (it.n_tiles == 1) commit(q_empty);
             for (int j = 0; j < it.n_tiles && ok; ++j, ++g) {
                 const bool more = j + 1 < it.n_tiles;
-                bool halves = false;
-                if constexpr (FROM == OPERANDS) halves = kind_of(it, j) & 1;
                 if (!wait_for(&v_full[g & 1], g >> 1) || (more && !wait_for(&k_full[(g + 1) & 1], (g + 1) >> 1))) { ok = false; break; }  // while the softmax is busy
                 for (int x = 0; x < it.halves && ok; ++x) {
                     for (int part = 0; part < 2 && ok; ++part) {
                         if (!wait_for(&p_full[2 * x + part], mine[x])) { ok = false; break; }
                         tc_fence_after();
-                        issue_pv(x, g, part, halves, j > 0 || part > 0 ? 1u : 0u);
+                        issue_pv(x, g, part, j > 0 || part > 0 ? 1u : 0u);
                     }
                     if (!ok) break;
                     if (more) issue_s(x, g + 1);
@@ -534,10 +489,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
             int piece_at = 0;
             if (row_valid && a.pieces) piece_at = (it.piece & OWN_PIECE ? a.own_start : a.piece_start)[token] + (it.piece & (OWN_PIECE - 1));
             float m = -INFINITY, l = 0.f;
-            int kind = 2 * 64;
             for (int j = 0; j < it.n_tiles; ++j) {
                 const int h = hx + j;
-                if constexpr (FROM == OPERANDS) kind = kind_of(it, j);  // there by the time S is
                 if (!mbar_wait(&s_full[x], h & 1, failed)) { ok = false; break; }
                 tc_fence_after();
                 const int tile_base = it.start + j * BN, last_visible = hi - tile_base, first_visible = it.key_lo - tile_base;
@@ -552,14 +505,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                 auto look = [&](unsigned (&s)[32]) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) part[i & 1] = max3(part[i & 1], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                };
-                auto weigh_16 = [&](const unsigned (&s)[32], unsigned (&w)[16], Pair minus_m2, Pair (&sum)[2]) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const Pair z = fma2(Pair{__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, scale2, minus_m2), p{fast_exp2(z.x), fast_exp2(z.y)};
-                        sum[i & 1] = add2(sum[i & 1], p);
-                        w[i] = pack_f16x2(p.x, p.y);
-                    }
                 };
                 const bool whole = __all_sync(0xffffffffu, last_visible >= BN - 1 && first_visible <= 0);
                 // The loops below are kept short on purpose: the roles of a block run different code on the same schedulers, and straight-line code is bound by
@@ -583,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                     if (c == 0) arrived(s0);
                 }
                 const float seen = max3(part[0], part[1], -INFINITY) * scale, m_new = fmaxf(m, seen);  // the scale is positive: the largest score stays the largest
-                const bool outgrown = __any_sync(0xffffffffu, m > -INFINITY && m_new - m > OUTGROWN<FROM>);  // one row's is taken as the occasion for all of the warp's
+                const bool outgrown = __any_sync(0xffffffffu, m > -INFINITY && m_new - m > OUTGROWN);  // one row's is taken as the occasion for all of the warp's
                 float alpha = 1.f;
                 if (!(seen < INFINITY)) {
                     m = __uint_as_float(0x7fffffffu);  // a NaN or an infinity among the scores: the row's softmax is no number, and stays none
@@ -606,12 +551,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                 const float minus_m = m == -INFINITY ? 0.f : -m;
                 const Pair minus_m2{minus_m, minus_m};
                 Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-                auto weigh_halves = [&](const unsigned (&s)[32], int c) {  // P of 32 columns as float16, over the first half of the columns that they came from
-                    unsigned w[16];
-                    weigh_16(s, w, minus_m2, sum);
-                    tmem_st16_words(s_addr + c, w);
-                };
-                auto weigh = [&](const unsigned (&s)[32], int c) {  // as bfloat16 in two parts, over all of them
+                auto weigh = [&](const unsigned (&s)[32], int c) {  // P of 32 columns as bfloat16 in two parts, over the columns that they came from
                     unsigned w[32];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -623,30 +563,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                     }
                     tmem_st32(s_addr + c, w);
                 };
-                auto walk = [&](auto&& weigh_32) {  // columns 96 to 127 are still at hand
 #pragma unroll 1
-                    for (int c = 64; c >= 0; c -= 64) {
-                        tmem_ld32(s_addr + c, s0), weigh_32(s1, c + 32), arrived(s0);
-                        if (c) tmem_ld32(s_addr + c - 32, s1);
-                        weigh_32(s0, c);
-                        hand_over(c ? 0 : 1);
-                        if (c) arrived(s1);
-                    }
-                };
-                if constexpr (FROM == OPERANDS) {
-                    if (kind & 1) {
-                        walk(weigh_halves);
-                    } else {
-#pragma unroll 1
-                        for (int c = 96; c >= 0; c -= 32) {
-                            tmem_ld32(s_addr + c, s0), arrived(s0);
-                            weigh(s0, c);
-                            if (c == 64) hand_over(0);
-                        }
-                        hand_over(1);
-                    }
-                } else {
-                    walk(weigh);
+                for (int c = 64; c >= 0; c -= 64) {  // columns 96 to 127 are still at hand
+                    tmem_ld32(s_addr + c, s0), weigh(s1, c + 32), arrived(s0);
+                    if (c) tmem_ld32(s_addr + c - 32, s1);
+                    weigh(s0, c);
+                    hand_over(c ? 0 : 1);
+                    if (c) arrived(s1);
                 }
                 l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             }
@@ -655,8 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
             tc_fence_after();
             if (ok) {
                 if (m == -INFINITY) l = 0.f;  // a row that sees nothing: what exp2_pair gave for it is none of its weights
-                const float back = FROM == OPERANDS ? __uint_as_float((unsigned)(127 + (kind >> 1) - 64) << 23) : 1.f;  // of values that were scaled by 2^-e0
-                const float inv = a.pieces ? back : back * (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
+                const float inv = a.pieces ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a row that sees nothing is zeros; a NaN stays one
                 // Rows leave through shared memory, 32 columns of 32 rows at a time: eight lanes then store 128 bytes of a row side by side, where a thread storing its own row
                 // would touch 32 lines with every instruction.  Some 6,000 clocks an item either way, 32 bytes a clock: what an SM stores.
                 const long long row_at = !row_valid ? -1 : a.pieces ? ((long long)piece_at * a.heads + first_head + hh) * D : (long long)token * a.out_stride + (long long)(first_head + hh) * D;
@@ -710,9 +632,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
 // requests behind 16,384 positions, eight runs, 162 us against 154, 64 requests behind 4,096, two runs, 35.6 against 39.4, with the slower softmax of then.)
 constexpr int OPERAND_THREADS = 256;
 __global__ void __launch_bounds__(OPERAND_THREADS) shared_operands_kernel(const unsigned char* __restrict__ codes, const signed char* __restrict__ exponents, const int* __restrict__ block_table,
-                                                                          int table_width, const int4* __restrict__ tiles, unsigned char* __restrict__ operands, int* __restrict__ kinds,
+                                                                          int table_width, const int4* __restrict__ tiles, unsigned char* __restrict__ operands,
                                                                           int page_size, int pages, int* status) {
-    __shared__ int bounds[BN / 32][3];
     let_next_kernel_start();
     const int4 tile = tiles[blockIdx.x];  // table row, first position, first key and last key + 1 of the range; written with the plan, long before
     wait_for_previous_kernels();
@@ -723,42 +644,29 @@ __global__ void __launch_bounds__(OPERAND_THREADS) shared_operands_kernel(const 
         return page >= 0 && page < pages ? (((long long)page * 2 + which) * kv_heads + kvh) * page_size + (pos & (page_size - 1)) : -1;
     };
     constexpr int CHUNKS = D / 16, UNITS = BN * CHUNKS / OPERAND_THREADS, STEP = OPERAND_THREADS / CHUNKS;  // a thread's chunks of 16 codes, of rows STEP apart
-    const int chunk = tid % CHUNKS, row0 = tid / CHUNKS, first = lo / BN * BN;
+    const int chunk = tid % CHUNKS, row0 = tid / CHUNKS;
     long long from[UNITS];
     uint4 raw[UNITS];
-    int e[UNITS], e0 = 0, low = 127, high = -128;
+    int e[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) from[u] = record(base + row0 + u * STEP);
-    const long long there = which && tid < BN ? record(first + tid) : -1, here = tid < BN ? record(base + tid) : -1;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const long long at = max(from[u], 0ll);
         raw[u] = *reinterpret_cast<const uint4*>(codes + at * D + chunk * 16);
         e[u] = min(max((int)exponents[at], -40), 40);
     }
-    if (tid < BN && kvh == 0 && here < 0 && base + tid >= lo && base + tid < hi) atomicOr(status, HB_STATUS_BAD_PAGE);
-    bool halves = false;
-    if (which) {  // e0: the largest exponent of the range's first tile; low and high: those of this one
-        if (tid < BN) {
-            e0 = there >= 0 ? min(max((int)exponents[there], -40), 40) : -40;
-            if (here >= 0) low = high = min(max((int)exponents[here], -40), 40);
-            e0 = __reduce_max_sync(0xffffffffu, e0), low = __reduce_min_sync(0xffffffffu, low), high = __reduce_max_sync(0xffffffffu, high);
-            if ((tid & 31) == 0) bounds[tid >> 5][0] = e0, bounds[tid >> 5][1] = low, bounds[tid >> 5][2] = high;
-        }
-        __syncthreads();
-        e0 = bounds[0][0], low = bounds[0][1], high = bounds[0][2];
 #pragma unroll
-        for (int w = 1; w < BN / 32; ++w) e0 = max(e0, bounds[w][0]), low = min(low, bounds[w][1]), high = max(high, bounds[w][2]);
-        halves = low - e0 >= LOWEST && high - e0 <= HIGHEST;
-        if (tid == 0) kinds[(size_t)blockIdx.x * kv_heads + kvh] = 2 * (e0 + 64) + (halves ? 1 : 0);
+    for (int u = 0; u < UNITS; ++u) {
+        const int pos = base + row0 + u * STEP;
+        if (chunk == 0 && kvh == 0 && which == 0 && from[u] < 0 && pos >= lo && pos < hi) atomicOr(status, HB_STATUS_BAD_PAGE);
     }
     unsigned char* out = operands + (((size_t)blockIdx.x * kv_heads + kvh) * 2 + which) * TILE_BYTES;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const int row = row0 + u * STEP;
         unsigned wide[8];
-        if (halves) widen<true>(raw[u], e[u] - e0, wide);
-        else widen<false>(raw[u], e[u] - e0, wide);
+        widen(raw[u], e[u], wide);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int oc = 2 * chunk + half;
@@ -811,12 +719,9 @@ int launch(const Args& a, int blocks, const void* q, int q_stride, int n_tokens,
     if (configured != cudaSuccess) return (int)configured;
     return launch_after_previous(attention_shared_kernel<FROM>, dim3(blocks, a.kv_heads * a.chunks), dim3(THREADS), SMEM_BYTES, stream, map, q_map, a);
 }
-const int* kinds_of(const void* operands, long long tiles, long long kv_heads) {  // they stand behind the tiles
-    return operands ? (const int*)((const unsigned char*)operands + (size_t)tiles * kv_heads * (2 * TILE_BYTES)) : nullptr;
-}
 }  // namespace
 
-// tiles [n_tiles, 4]: table row, first position, first key and last key + 1 of the tile's range.  operands: n_tiles * kv_heads * (4 * 128 * D + 4) bytes.
+// tiles [n_tiles, 4]: table row, first position, first key and last key + 1 of the tile's range.  operands: n_tiles * kv_heads * 4 * 128 * D bytes.
 HB_EXPORT int hb_shared_operands(const void* codes, const void* exponents, const int* block_table, int table_width, const int* tiles, int n_tiles, void* operands, int kv_heads,
                                  int page_size, int pages, int* status, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
@@ -825,7 +730,7 @@ HB_EXPORT int hb_shared_operands(const void* codes, const void* exponents, const
     if (((uintptr_t)codes | (uintptr_t)operands) & 15) return HB_BAD_ARGUMENT;
     if ((uintptr_t)tiles & 15) return HB_BAD_ARGUMENT;
     return launch_after_previous(shared_operands_kernel, dim3(n_tiles, kv_heads, 2), dim3(OPERAND_THREADS), 0, stream, (const unsigned char*)codes, (const signed char*)exponents, block_table,
-                                 table_width, (const int4*)tiles, (unsigned char*)operands, const_cast<int*>(kinds_of(operands, n_tiles, kv_heads)), page_size, pages, status);
+                                 table_width, (const int4*)tiles, (unsigned char*)operands, page_size, pages, status);
 }
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents and operands null), or e4m3 codes with exponents and the operands that hb_shared_operands has made of them.
@@ -843,7 +748,7 @@ HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_token
     const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     if (!operands != !exponents || (operands && (operand_tiles <= 0 || ((uintptr_t)operands & 15)))) return HB_BAD_ARGUMENT;
-    const Args a{(const unsigned char*)operands, kinds_of(operands, operand_tiles, kv_heads), (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
+    const Args a{(const unsigned char*)operands, (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
     if (operands) return launch<OPERANDS>(a, blocks, q, q_stride, n_tokens, cache, stream);
     return launch<BFLOAT16>(a, blocks, q, q_stride, n_tokens, cache, stream);

@@ -103,7 +103,7 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     if joined or plan.operand_tiles:
         for_pieces = (plan.pieces * heads * (head_dim + 2) * 4 + 511) // 512 * 512 if joined else 0
         makes = plan.operand_tiles if exponents else 0  # what runs of many rows walk is made into operands first
-        memory, owner = scratch(device, stream, for_pieces + makes * kv_heads * (2 * TILE_KEYS * 2 * head_dim + 16))
+        memory, owner = scratch(device, stream, for_pieces + makes * kv_heads * 2 * TILE_KEYS * 2 * head_dim)
         if joined:
             pieces, sums = memory, memory + 4 * plan.pieces * heads * head_dim
         if makes:
