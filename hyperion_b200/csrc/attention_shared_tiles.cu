@@ -302,7 +302,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
     for (int e = tid; e < Q_BYTES / 16; e += THREADS) reinterpret_cast<uint4*>(qs)[e] = make_uint4(0, 0, 0, 0);
     const int first_item = a.first_item[blockIdx.x], end_item = a.first_item[blockIdx.x + 1];  // written with the plan, long before, like the items
     wait_for_previous_kernels();
-    let_next_kernel_start();  // only now: the strip kernel of the same step takes its start as the sign that all that came before has finished
     // All of the SM's tensor memory, and only now: a block of a kernel further back in the stream that has yet to start on this SM can no longer want any.
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
@@ -311,6 +310,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
+    // Only now: the strip kernel of the same step takes its start as the sign that all that came before has finished, and a kernel behind that takes tensor memory before it waits for
+    // this one must find it taken, not take what this block still has to ask for.
+    let_next_kernel_start();
     tc_fence_after();
     const unsigned tmem = *tmem_slot;
     const int shift = 31 - __clz(a.page_size);

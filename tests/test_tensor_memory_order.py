@@ -1,0 +1,14 @@
+"""A kernel that takes tensor memory after it has waited for the kernels before it lets the next one start only when it has what it wants: a block of the next kernel that came first
+would hold columns while it waits for this kernel, which would wait for them.  (Read from the source: on a device the two orders differ in nothing but in when they fail.)"""
+from __future__ import annotations
+
+from pathlib import Path
+
+SOURCES = Path(__file__).resolve().parent.parent / "hyperion_b200" / "csrc"
+
+
+def test_tiles_behind_shared_positions():
+    text = (SOURCES / "attention_shared_tiles.cu").read_text()
+    kernel = text[text.index("attention_shared_kernel("): text.index("// Operands of 8-bit records")]
+    waited, taken, met, started = (kernel.index(what) for what in ("wait_for_previous_kernels();", "tcgen05.alloc", "__syncthreads();\n    // Only now", "let_next_kernel_start();"))
+    assert waited < taken < met < started and kernel.count("let_next_kernel_start();") == 1
