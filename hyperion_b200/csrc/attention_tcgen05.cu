@@ -754,11 +754,12 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// More than half of an SM's shared memory, so that one block is all an SM takes: the block holds all of its tensor memory.
+// So much of an SM's shared memory that one block is all an SM takes: the block holds all of its tensor memory.  Nor may a block of a kernel behind stand beside it that takes tensor
+// memory before it waits for this one, which asks for its own only when it has waited: the matrix products' smallest block has 97 KB (gemm_tcgen05.cu), an SM 228 and a KB a block.
 constexpr size_t SMEM_USED = 1024 + (size_t)STAGES * KEY_TILE_BYTES + (size_t)V_STAGES * TILE_BYTES + (size_t)KEY_PANELS * Q_PANEL * sizeof(bf16) + (4 * STAGES + 12) * 8 + 96 +
                              (DK == D ? 4 * BM * sizeof(float) : 0);  // the last for two maps per head only
 static_assert(SMEM_USED <= 227 * 1024, "an SM's shared memory");
-constexpr size_t SMEM_BYTES = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;
+constexpr size_t SMEM_BYTES = SMEM_USED > 132 * 1024 ? SMEM_USED : 132 * 1024;
 }  // namespace
 
 // Rows of a tile (tokens x heads of a group) this kernel wants: the host planner cuts rows into tiles of
