@@ -37,7 +37,7 @@
 // across lanes).  One token of 14 heads at 512 positions: 5.5 us, a start and three dependent trips to memory.
 //
 // Slots beyond a range's end may hold anything: their scores are replaced and their values are read as zeros.  Every mbarrier wait is
-// bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the block leaves.
+// bounded (HB_WAIT_LIMIT looks); one that runs out sets HB_STATUS_WAIT_EXPIRED and the block leaves, once the copies that it has on their way have arrived.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -45,6 +45,9 @@
 
 #ifndef HB_HEAD_DIM
 #define HB_HEAD_DIM 128
+#endif
+#ifndef HB_WAIT_LIMIT
+#define HB_WAIT_LIMIT (1u << 24)
 #endif
 
 namespace {
@@ -56,7 +59,7 @@ constexpr int WARPS = 4;        // that compute; one more fetches
 constexpr int THREADS = 32 * (WARPS + 1);
 constexpr int ITEM_WORDS = 7;   // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of a request's own positions), -
 constexpr int OWN_PIECE = 1 << 30;
-constexpr unsigned WAIT_LIMIT = 1u << 24;
+constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
 constexpr float HEADROOM = 8.f;  // m stands so far below the maximum: P up to 2^8 keeps float16's small weights further from its smallest number
 
 constexpr int FAR_APART = 12;    // exponents of values that differ by more: a weight P that counts may lie below what float16 holds well
@@ -71,19 +74,26 @@ __device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned
 __device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ bool mbar_over(unsigned long long* bar, unsigned parity) {
+    unsigned done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
 __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
-    const unsigned addr = smem_u32(bar);
     for (unsigned spin = 0; spin < WAIT_LIMIT; ++spin) {
-        unsigned done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(addr), "r"(parity) : "memory");
-        if (done) return true;
+        if (mbar_over(bar, parity)) return true;
         if ((spin & 1023) == 1023 && *failed) return false;
     }
     return false;
+}
+// Before a block leaves: what it has set going is done, whatever has become of its other waits.
+__device__ __forceinline__ void mbar_last_wait(unsigned long long* bar, unsigned parity) {
+    for (unsigned spin = 0; spin < LAST_WAIT_LIMIT; ++spin)
+        if (mbar_over(bar, parity)) return;
 }
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -246,7 +256,8 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
         const int ops = pages_per_tile * OPS_PER_PAGE;
         const unsigned page_bytes = 2u * a.page_size * D * S::BYTES;
         if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
-        for (int index = first_item; index < end_item; ++index) {
+        int ok = 1;
+        for (int index = first_item; index < end_item && ok; ++index) {
             const int* item = a.items + (size_t)index * ITEM_WORDS;
             const int key_lo = item[3], key_hi = item[4], start = key_lo / BN * BN, n_tiles = (key_hi - start + BN - 1) / BN;
             const int* table = a.block_table + (size_t)item[2] * a.table_width;
@@ -257,12 +268,11 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                     const int block = ((start + it * BN) >> shift) + lane;
                     looked = block < a.table_width ? __ldg(table + block) : -1;
                 }
-                int ok = 1;
                 if (lane == 0) ok = mbar_wait(&empty[s], (round & 1) ^ 1, failed) ? 1 : 0;
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) {
                     if (lane == 0) { *failed = 1; atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_STRIPS); }
-                    return;
+                    break;
                 }
                 const int base = start + it * BN, k0 = base + lane * a.page_size;
                 int page = __shfl_sync(0xffffffffu, looked, (it % tiles_per_look) * pages_per_tile + lane);
@@ -294,6 +304,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                 }
             }
         }
+        if (lane == 0)
+            for (int k = max(0, stage - S::STAGES); k < stage; ++k) mbar_last_wait(&full[k % S::STAGES], (k / S::STAGES) & 1);
+        __syncwarp();
         if constexpr (TOGETHER) cluster_meet(), cluster_meet();
         return;
     }

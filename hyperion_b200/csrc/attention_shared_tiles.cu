@@ -22,14 +22,17 @@
 // 256 rows' is, and one often is); a part of the exponentials by a polynomial (no faster); two threads a row (4,700); an issuer for each half (the halves fall into step: 4,700).
 //
 // Slots beyond an item's range may hold anything: their scores are replaced, and their values are zeros before a product reads them (operands are made so; over
-// bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded; a wait that runs out sets
-// HB_STATUS_WAIT_EXPIRED, all roles leave their loops, tensor memory is freed and the block returns.
+// bfloat16 the fetching warp clears them in the item's first and last tile).  Every mbarrier wait is bounded (HB_WAIT_LIMIT looks); a wait that runs out sets
+// HB_STATUS_WAIT_EXPIRED, all roles leave their loops, what the block has on its way (copies, products) is waited for, tensor memory is freed and the block returns.
 #include <cuda.h>
 
 #include "common.cuh"
 
 #ifndef HB_HEAD_DIM
 #define HB_HEAD_DIM 128
+#endif
+#ifndef HB_WAIT_LIMIT
+#define HB_WAIT_LIMIT (1u << 24)
 #endif
 
 namespace {
@@ -49,7 +52,7 @@ constexpr int O_COL = 256;
 constexpr int ITEM_WORDS = 7;                 // first token, tokens, table row, first key, last key + 1, number of the piece (with OWN_PIECE: among those of its own positions), first operand tile
 constexpr int OWN_PIECE = 1 << 30;
 enum Source : int { BFLOAT16 = 0, OPERANDS = 1 };  // what the tiles come from: a bfloat16 cache, or operands made of an 8-bit one
-constexpr unsigned WAIT_LIMIT = 1u << 24;
+constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
@@ -61,19 +64,26 @@ __device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned
 __device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ bool mbar_over(unsigned long long* bar, unsigned parity) {
+    unsigned done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
 __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
-    const unsigned addr = smem_u32(bar);
     for (unsigned spin = 0; spin < WAIT_LIMIT; ++spin) {
-        unsigned done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(addr), "r"(parity) : "memory");
-        if (done) return true;
+        if (mbar_over(bar, parity)) return true;
         if ((spin & 1023) == 1023 && *failed) return false;
     }
     return false;
+}
+// Before a block leaves: what it has set going is done, whatever has become of its other waits.
+__device__ __forceinline__ void mbar_last_wait(unsigned long long* bar, unsigned parity) {
+    for (unsigned spin = 0; spin < LAST_WAIT_LIMIT; ++spin)
+        if (mbar_over(bar, parity)) return;
 }
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -275,7 +285,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
     unsigned long long* q_full = o_done + 2;
     unsigned long long* q_empty = q_full + 1;
     unsigned long long* edge_full = q_empty + 1;  // bfloat16: a V tile whose slots beyond the range are cleared before it is announced
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(edge_full + 1);
+    unsigned long long* all_done = edge_full + 1;  // every product that was issued
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(all_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -293,6 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(edge_full, 1);
+        mbar_init(all_done, 1);
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
@@ -339,12 +351,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
         const int pages_per_tile = BN >> shift, tokens_per_item = ROWS / a.gc;
         bool alive = true;
         int g = 0, edges = 0, round = 0;  // g: tiles so far
+        int k_sent = 0, v_sent = 0, q_sent = 0, edges_sent = 0;  // phases of the barriers that lane 0 has set going
         for (int index = first_item; index < end_item && alive; ++index, ++round) {
             const Item it = read_item(index);
             if (lane == 0) {  // the queries: tokens beyond the item's own come along, or are filled with zeros
                 if (!mbar_wait(q_empty, (round & 1) ^ 1, failed)) alive = false;
                 if (alive) {
                     mbar_expect_tx(q_full, (unsigned)(PANELS * 128 * a.gc * tokens_per_item));
+                    ++q_sent;
                     for (int h = 0; h < PANELS; ++h) tma_load_3d(qs + h * Q_PANEL * 2, &q_map, q_full, h * 64, first_head, it.tok0);
                 }
             }
@@ -358,6 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                             const int s = g & 1, turn = g >> 1;
                             if (!mbar_wait(which ? &v_empty[s] : &k_empty[s], (turn & 1) ^ 1, failed)) { alive = false; break; }
                             mbar_expect_tx(which ? &v_full[s] : &k_full[s], TILE_BYTES);
+                            ++(which ? v_sent : k_sent);
                             bulk_load((which ? v_ring : k_ring) + (size_t)s * TILE_BYTES, from + which * TILE_BYTES, TILE_BYTES, which ? &v_full[s] : &k_full[s]);
                         }
                     }
@@ -385,6 +400,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                     if (lane == 0) {
                         const unsigned page_bytes = (unsigned)a.page_size * D * 2u;
                         if (valid) mbar_expect_tx(full, valid * page_bytes); else mbar_arrive(full);
+                        ++(which ? (edge ? edges_sent : v_sent) : k_sent);
                     }
                     __syncwarp();
                     unsigned char* stage = which ? v_ring + (size_t)s * TILE_BYTES : k_ring + (size_t)s * TILE_BYTES;
@@ -405,12 +421,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&v_full[s]);
+                        if (lane == 0) mbar_arrive(&v_full[s]), ++v_sent;
                     }
                 }
             }
         }
         if (!alive) fail();
+        if (lane == 0) {  // all that was sent arrives before the block leaves
+            for (int t = max(0, k_sent - 2); t < k_sent; ++t) mbar_last_wait(&k_full[t & 1], (t >> 1) & 1);
+            for (int t = max(0, v_sent - 2); t < v_sent; ++t) mbar_last_wait(&v_full[t & 1], (t >> 1) & 1);
+            if (q_sent) mbar_last_wait(q_full, (q_sent - 1) & 1);
+            if (edges_sent) mbar_last_wait(edge_full, (edges_sent - 1) & 1);
+        }
+        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ tensor-core issuer: the warp stays together, so that descriptors are its common values
         // (uniform registers); one elected lane issues.  Under `if (lane == 0)` every product took 65 clocks to
@@ -471,6 +494,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_shared_kernel(const __gr
             }
         }
         if (!ok) fail();
+        commit(all_done);  // the products and the arrivals that tell of them, before tensor memory is freed
+        mbar_last_wait(all_done, 0);
+        __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------------------ softmax: thread = row = tensor-memory lane of its half
         const int x = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane, v = x * BM + r;
