@@ -841,14 +841,15 @@ int launch_strips(const Args& a, const void* cache, int blocks, cudaStream_t str
 }  // namespace
 
 // Puts the n_pieces = piece_start[tokens] pieces [n_pieces, heads, D] of the tokens together.  A token without a piece is zeros.
-HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const int* piece_start, void* out, int out_stride, int tokens, int n_pieces, int heads, cudaStream_t stream) {
+HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const int* piece_start, void* out, long long out_stride, int tokens, int n_pieces, int heads, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (!pieces || !sums || !piece_start || !out || heads <= 0 || out_stride % 2 || ((uintptr_t)pieces & 15) || ((uintptr_t)out & 3)) return HB_BAD_ARGUMENT;
+    if (out_stride > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const bool many = n_pieces / tokens > 12;
     const int per_block = many ? 1 : MERGE_WARPS, rows = (heads + per_block - 1) / per_block;
     if (rows > 65535) return HB_UNSUPPORTED_SIZE;
     return launch_after_previous(many ? attention_pieces_kernel<MERGE_WARPS> : attention_pieces_kernel<1>, dim3(tokens, rows), dim3(32 * MERGE_WARPS), 0, stream, pieces, (const float2*)sums,
-                                 piece_start, (bf16*)out, out_stride, heads);
+                                 piece_start, (bf16*)out, (int)out_stride, heads);
 }
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents null) or e4m3 codes with exponents [pages, 2, kv_heads, page_size].
@@ -856,7 +857,7 @@ HB_EXPORT int hb_attention_pieces(const float* pieces, const float* sums, const 
 // tokens, and join them; no pieces then.
 // items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most rows / min(heads / kv_heads, rows) tokens, rows being 8 or 16.  pieces, sums null: one piece a row;
 // else tokens and n_pieces as hb_attention_pieces takes them, which follows.
-HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
+HB_EXPORT int hb_attention_strips(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, const void* exponents, const int* block_table, int table_width,
                                   const int* items, const int* first_item, int blocks, int rows, int beside_tiles, int together, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads, int kv_heads,
                                   int page_size, int pages, float scale, int* status, cudaStream_t stream, int tokens, int n_pieces) {
     if (blocks <= 0) return 0;
@@ -866,11 +867,12 @@ HB_EXPORT int hb_attention_strips(const void* q, int q_stride, void* out, int ou
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)pieces) & 15) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
+    if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     if (rows != 8 && rows != MOST_ROWS) return HB_UNSUPPORTED_SIZE;
     if (together && (together < 2 || together > MOST_TOGETHER || blocks % together || pieces || beside_tiles)) return HB_BAD_ARGUMENT;
     const int group = heads / kv_heads, gc = group < rows ? group : rows, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
-    const Args a{(const bf16*)q, q_stride, (bf16*)out, out_stride, (const signed char*)exponents, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
+    const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, (const signed char*)exponents, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, beside_tiles, together, gc, chunks, scale * 1.4426950408889634f, status};
     const auto launch = rows == 8 ? (exponents ? launch_strips<true, 1> : launch_strips<false, 1>) : (exponents ? launch_strips<true, 2> : launch_strips<false, 2>);
     if (int code = launch(a, cache, blocks, stream)) return code;

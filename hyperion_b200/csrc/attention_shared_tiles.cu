@@ -763,7 +763,7 @@ HB_EXPORT int hb_shared_operands(const void* codes, const void* exponents, const
 
 // cache: [pages, 2, kv_heads, page_size, D] in bfloat16 (exponents and operands null), or e4m3 codes with exponents and the operands that hb_shared_operands has made of them.
 // items: see ITEM_WORDS; first_item [blocks + 1]; an item has at most 256 / min(heads / kv_heads, 256) tokens.  pieces, sums null: one piece a row.
-HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_tokens, void* out, int out_stride, const void* cache, const void* exponents, const int* block_table,
+HB_EXPORT int hb_attention_shared_tiles(const void* q, long long q_stride, int n_tokens, void* out, long long out_stride, const void* cache, const void* exponents, const int* block_table,
                                         int table_width, const int* items, const int* first_item, int blocks, const void* operands, int operand_tiles, const int* last, const int* piece_start, const int* own_start, float* pieces, float* sums, int heads,
                                         int kv_heads, int page_size, int pages, float scale, int* status, cudaStream_t stream) {
     if (blocks <= 0) return 0;
@@ -773,11 +773,12 @@ HB_EXPORT int hb_attention_shared_tiles(const void* q, int q_stride, int n_token
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)pieces & 31) || ((uintptr_t)exponents & 3) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
+    if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const int group = heads / kv_heads, gc = group < ROWS ? group : ROWS, chunks = (group + gc - 1) / gc;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     if (!operands != !exponents || (operands && (operand_tiles <= 0 || ((uintptr_t)operands & 15)))) return HB_BAD_ARGUMENT;
-    const Args a{(const unsigned char*)operands, (bf16*)out, out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
+    const Args a{(const unsigned char*)operands, (bf16*)out, (int)out_stride, block_table, table_width, items, first_item, last, piece_start, own_start, pieces, (float2*)sums,
                  heads, kv_heads, page_size, pages, gc, chunks, scale * 1.4426950408889634f, status};
-    if (operands) return launch<OPERANDS>(a, blocks, q, q_stride, n_tokens, cache, stream);
-    return launch<BFLOAT16>(a, blocks, q, q_stride, n_tokens, cache, stream);
+    if (operands) return launch<OPERANDS>(a, blocks, q, (int)q_stride, n_tokens, cache, stream);
+    return launch<BFLOAT16>(a, blocks, q, (int)q_stride, n_tokens, cache, stream);
 }

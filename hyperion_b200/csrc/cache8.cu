@@ -244,13 +244,14 @@ constexpr int PER = 4;
 bool takes_several(const Places& p) { return p.head_dim % 16 == 0 && (long long)p.tokens * 2 * p.kv_heads * p.head_dim >= (long long)PER * 16 * 148 * 1024; }
 }  // namespace
 
-HB_EXPORT int hb_cache8_store(const void* src, int is_bf16, int stride, int k_offset, int v_offset, void* codes, void* exponents, const int* block_table,
+HB_EXPORT int hb_cache8_store(const void* src, int is_bf16, long long stride, long long k_offset, long long v_offset, void* codes, void* exponents, const int* block_table,
                               int table_width, const int* token_row, const int* positions, int tokens, int kv_heads, int head_dim, int page_size, int pages,
                               int* status, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (!src || !codes || !exponents || k_offset < 0 || v_offset < 0 || ((uintptr_t)codes & 15)) return HB_BAD_ARGUMENT;
     Places p;
     if (int code = places(p, block_table, table_width, token_row, positions, tokens, kv_heads, head_dim, page_size, pages, status)) return code;
+    if (stride > 0x7fffffffLL || k_offset > 0x7fffffffLL || v_offset > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const unsigned element = is_bf16 ? 2 : 4;
     const auto on = [&](unsigned bytes) {  // every record starts on such a boundary
         return !(((uintptr_t)src | (uintptr_t)stride * element | (uintptr_t)k_offset * element | (uintptr_t)v_offset * element | (uintptr_t)head_dim * element) & (bytes - 1));
@@ -258,8 +259,8 @@ HB_EXPORT int hb_cache8_store(const void* src, int is_bf16, int stride, int k_of
 #define HB_STORE(T, WIDTH, N, ALIGNED)                                                                                                                     \
     do {                                                                                                                                                   \
         const unsigned blocks = set_width(p, WIDTH, N);                                                                                                    \
-        return launch_after_previous(cache8_store_kernel<T, WIDTH, N, ALIGNED>, dim3(blocks), dim3(THREADS), 0, stream, (const T*)src, stride, k_offset,   \
-                                     v_offset, p, (unsigned char*)codes, (signed char*)exponents);                                                         \
+        return launch_after_previous(cache8_store_kernel<T, WIDTH, N, ALIGNED>, dim3(blocks), dim3(THREADS), 0, stream, (const T*)src, (int)stride, (int)k_offset, \
+                                     (int)v_offset, p, (unsigned char*)codes, (signed char*)exponents);                                                         \
     } while (0)
     if (is_bf16) {
         if (on(32) && takes_several(p)) HB_STORE(bf16, 16, PER, true);

@@ -63,7 +63,7 @@ def cache8_store(src: torch.Tensor, k_offset: int, v_offset: int, cache: Cache8,
         raise KernelError(f"cache8_store: a source [tokens, width] with unit inner stride that holds {width} columns of keys and of values at their offsets")
     if not src.is_cuda:
         require_cuda(src)
-    check(entry("cache8", "hb_cache8_store", "piiiipppippiiiiipp")(
+    check(entry("cache8", "hb_cache8_store", "pilllpppippiiiiipp")(
         src.data_ptr(), is_bf16(src), src.stride(0), k_offset, v_offset, cache[0].data_ptr(), cache[1].data_ptr(), block_table.data_ptr(), table_width, token_row.data_ptr(),
         positions.data_ptr(), tokens, kv_heads, head_dim, page_size, pages, status_word(src.device).data_ptr(), stream_address()), "cache8_store")
 

@@ -114,11 +114,11 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
         if operands:
             check(entry("attention_shared_tiles", "hb_shared_operands", "pppipipiiipp", head_dim)(
                 *where, operand_list, plan.operand_tiles, operands, kv_heads, page_size, pages, status_word(device).data_ptr(), stream), "attention_shared")
-        check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "piipipppippipipppppiiiifpp", head_dim)(
+        check(entry("attention_shared_tiles", "hb_attention_shared_tiles", "pliplpppippipipppppiiiifpp", head_dim)(
             q.data_ptr(), q.stride(0), tokens, out_at, out_stride, *where, tile_items, tile_first, plan.tile_blocks, operands, plan.operand_tiles, *what), "attention_shared")
     if plan.strip_blocks:
-        check(entry("attention_shared", "hb_attention_strips", "pipipppippiiiipppppiiiifppii", head_dim)(
+        check(entry("attention_shared", "hb_attention_strips", "plplpppippiiiipppppiiiifppii", head_dim)(
             q.data_ptr(), q.stride(0), out_at, out_stride, *where, strip_items, strip_first, plan.strip_blocks, plan.strip_rows, int(plan.tile_blocks > 0), plan.together, *what, tokens, plan.pieces), "attention_shared")
     elif joined:
-        check(entry("attention_shared", "hb_attention_pieces", "ppppiiiip", head_dim)(pieces, sums, starts, out_at, out_stride, tokens, plan.pieces, heads, stream), "attention_shared")
+        check(entry("attention_shared", "hb_attention_pieces", "ppppliiip", head_dim)(pieces, sums, starts, out_at, out_stride, tokens, plan.pieces, heads, stream), "attention_shared")
     return out
