@@ -239,14 +239,14 @@ unsigned set_width(Places& p, int width, int per) {
     return (unsigned)((groups * ((2LL * p.kv_heads) << p.lanes_log) + THREADS - 1) / THREADS);
 }
 constexpr int PER = 4;
-// Four tokens and sixteen entries a thread once their threads alone fill the device (148 SMs of 1,024 such threads); below that one token and eight entries, for the
+// Four tokens and sixteen entries a thread once their threads alone fill the device (multiprocessors of 1,024 such threads); below that one token and eight entries, for the
 // shorter way of a thread: 700 tokens of 4 heads of 128 read back in 2.6 us.
-bool takes_several(const Places& p) { return p.head_dim % 16 == 0 && (long long)p.tokens * 2 * p.kv_heads * p.head_dim >= (long long)PER * 16 * 148 * 1024; }
+bool takes_several(const Places& p, int sms) { return p.head_dim % 16 == 0 && (long long)p.tokens * 2 * p.kv_heads * p.head_dim >= (long long)PER * 16 * 1024 * sms; }
 }  // namespace
 
 HB_EXPORT int hb_cache8_store(const void* src, int is_bf16, long long stride, long long k_offset, long long v_offset, void* codes, void* exponents, const int* block_table,
                               int table_width, const int* token_row, const int* positions, int tokens, int kv_heads, int head_dim, int page_size, int pages,
-                              int* status, cudaStream_t stream) {
+                              int sms, int* status, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (!src || !codes || !exponents || k_offset < 0 || v_offset < 0 || ((uintptr_t)codes & 15)) return HB_BAD_ARGUMENT;
     Places p;
@@ -263,7 +263,7 @@ HB_EXPORT int hb_cache8_store(const void* src, int is_bf16, long long stride, lo
                                      (int)v_offset, p, (unsigned char*)codes, (signed char*)exponents);                                                         \
     } while (0)
     if (is_bf16) {
-        if (on(32) && takes_several(p)) HB_STORE(bf16, 16, PER, true);
+        if (on(32) && takes_several(p, sms)) HB_STORE(bf16, 16, PER, true);
         if (on(16)) HB_STORE(bf16, 8, 1, true);
         HB_STORE(bf16, 8, 1, false);
     }
@@ -273,12 +273,12 @@ HB_EXPORT int hb_cache8_store(const void* src, int is_bf16, long long stride, lo
 }
 
 HB_EXPORT int hb_cache8_load(const void* codes, const void* exponents, const int* block_table, int table_width, const int* token_row, const int* positions,
-                             void* out, int is_bf16, int tokens, int kv_heads, int head_dim, int page_size, int pages, int* status, cudaStream_t stream) {
+                             void* out, int is_bf16, int tokens, int kv_heads, int head_dim, int page_size, int pages, int sms, int* status, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (!codes || !exponents || !out || ((uintptr_t)codes & 15) || ((uintptr_t)out & 31)) return HB_BAD_ARGUMENT;
     Places p;
     if (int code = places(p, block_table, table_width, token_row, positions, tokens, kv_heads, head_dim, page_size, pages, status)) return code;
-    const bool several = takes_several(p);
+    const bool several = takes_several(p, sms);
 #define HB_LOAD(T, WIDTH, N)                                                                                                                               \
     do {                                                                                                                                                   \
         const unsigned blocks = set_width(p, WIDTH, N);                                                                                                    \

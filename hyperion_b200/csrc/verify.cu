@@ -437,12 +437,12 @@ __global__ void __launch_bounds__(THREADS, REQUESTS_PER_SM) verify_requests_kern
 }
 }  // namespace
 
-// workspace: rows * ceil(vocab / CHUNK) + 2 * requests words of 8 bytes.
+// workspace: rows * ceil(vocab / CHUNK) + 2 * requests words of 8 bytes.  sms: the device's multiprocessors.
 HB_EXPORT int hb_verify_drafts(const void* logits, int is_bf16, long long stride, const int* row_start, int requests, int rows, int vocab, const int* drafts,
                                const float* probabilities, long long q_stride, const float* uniform, const float* noise, long long noise_stride,
-                               const float* temperature, void* workspace, int* accepted, int* tokens, int most, int* status, cudaStream_t stream) {
+                               const float* temperature, void* workspace, int* accepted, int* tokens, int most, int sms, int* status, cudaStream_t stream) {
     if (requests <= 0) return 0;
-    if (rows < 0 || vocab <= 0 || most <= 0 || !row_start || !noise || !temperature || !workspace || !accepted || !tokens || !status || ((uintptr_t)workspace & 7)) return HB_BAD_ARGUMENT;
+    if (rows < 0 || vocab <= 0 || most <= 0 || sms <= 0 || !row_start || !noise || !temperature || !workspace || !accepted || !tokens || !status || ((uintptr_t)workspace & 7)) return HB_BAD_ARGUMENT;
     if (rows > 0 && (!logits || !drafts || !uniform)) return HB_BAD_ARGUMENT;
     if (rows > 65535 || requests > 65535 || vocab > 0x7fffffff - 2 * CHUNK) return HB_UNSUPPORTED_SIZE;
     // As many blocks a row, and then a request, as the device holds at once between them, one for each CHUNK at most: a second turn of a few blocks would cost as much as
@@ -452,7 +452,7 @@ HB_EXPORT int hb_verify_drafts(const void* logits, int is_bf16, long long stride
         const int wanted = slots / (lines > 0 ? lines : 1), blocks = wanted < 1 ? 1 : (wanted < chunks ? wanted : chunks);
         return (chunks + blocks - 1) / blocks * CHUNK;
     };
-    const int row_span = span(rows, 148 * ROWS_PER_SM), request_span = span(requests, 148 * REQUESTS_PER_SM);
+    const int row_span = span(rows, sms * ROWS_PER_SM), request_span = span(requests, sms * REQUESTS_PER_SM);
     const int row_blocks = (vocab + row_span - 1) / row_span, request_blocks = (vocab + request_span - 1) / request_span;
     float2* pieces = (float2*)workspace;
     Key* best = (Key*)(pieces + (size_t)rows * chunks);

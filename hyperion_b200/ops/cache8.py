@@ -10,7 +10,7 @@ from typing import NamedTuple
 import torch
 
 from .basic import status_word
-from .native import KernelError, check, entry, is_bf16, require_cuda, stream_address
+from .native import KernelError, check, entry, is_bf16, require_cuda, sm_count, stream_address
 
 
 class Cache8(NamedTuple):
@@ -63,9 +63,9 @@ def cache8_store(src: torch.Tensor, k_offset: int, v_offset: int, cache: Cache8,
         raise KernelError(f"cache8_store: a source [tokens, width] with unit inner stride that holds {width} columns of keys and of values at their offsets")
     if not src.is_cuda:
         require_cuda(src)
-    check(entry("cache8", "hb_cache8_store", "pilllpppippiiiiipp")(
+    check(entry("cache8", "hb_cache8_store", "pilllpppippiiiiiipp")(
         src.data_ptr(), is_bf16(src), src.stride(0), k_offset, v_offset, cache[0].data_ptr(), cache[1].data_ptr(), block_table.data_ptr(), table_width, token_row.data_ptr(),
-        positions.data_ptr(), tokens, kv_heads, head_dim, page_size, pages, status_word(src.device).data_ptr(), stream_address()), "cache8_store")
+        positions.data_ptr(), tokens, kv_heads, head_dim, page_size, pages, sm_count(src.device), status_word(src.device).data_ptr(), stream_address()), "cache8_store")
 
 
 def cache8_load(cache: Cache8, block_table: torch.Tensor, token_row: torch.Tensor, positions: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -78,7 +78,7 @@ def cache8_load(cache: Cache8, block_table: torch.Tensor, token_row: torch.Tenso
         out = torch.empty(tokens, 2, kv_heads, head_dim, dtype=dtype, device=cache[0].device)
     elif out.shape != (tokens, 2, kv_heads, head_dim) or out.dtype != dtype or not out.is_contiguous() or not out.is_cuda:
         raise KernelError(f"cache8_load: the output is a dense {dtype} tensor [tokens, 2, kv_heads, d]")
-    check(entry("cache8", "hb_cache8_load", "pppipppiiiiiipp")(
+    check(entry("cache8", "hb_cache8_load", "pppipppiiiiiiipp")(
         cache[0].data_ptr(), cache[1].data_ptr(), block_table.data_ptr(), table_width, token_row.data_ptr(), positions.data_ptr(), out.data_ptr(), is_bf16(out), tokens, kv_heads,
-        head_dim, page_size, pages, status_word(out.device).data_ptr(), stream_address()), "cache8_load")
+        head_dim, page_size, pages, sm_count(out.device), status_word(out.device).data_ptr(), stream_address()), "cache8_load")
     return out

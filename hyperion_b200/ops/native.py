@@ -62,7 +62,9 @@ _sm_counts: dict = {}
 
 def sm_count(device=None) -> int:
     """Multiprocessors of the device (the current one by default), asked once per device: grids and split counts follow it."""
-    index = torch.cuda.current_device() if device is None or torch.device(device).index is None else torch.device(device).index
+    index = None if device is None else (device if isinstance(device, torch.device) else torch.device(device)).index
+    if index is None:
+        index = torch.cuda.current_device()
     found = _sm_counts.get(index)
     if found is None:
         found = _sm_counts[index] = int(torch.cuda.get_device_properties(index).multi_processor_count)

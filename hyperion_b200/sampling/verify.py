@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from ..ops.basic import status_word
-from ..ops.native import KernelError, check, entry, is_bf16, require_cuda, scratch, stream_address
+from ..ops.native import KernelError, check, entry, is_bf16, require_cuda, scratch, sm_count, stream_address
 
 
 CHUNK = 4096  # entries of the vocabulary a block looks through (csrc/verify.cu)
@@ -50,10 +50,10 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     accepted, tokens = torch.empty(requests, dtype=torch.int32, device=device), torch.empty(requests, most, dtype=torch.int32, device=device)
     stream = stream_address()
     memory, owner = scratch(device, stream, 8 * (rows * -(-vocab // CHUNK) + 2 * requests))
-    check(entry("verify", "hb_verify_drafts", "pilpiiipplpplppppipp")(
+    check(entry("verify", "hb_verify_drafts", "pilpiiipplpplppppiipp")(
         logits.data_ptr(), is_bf16(logits), logits.stride(0), row_start.data_ptr(), requests, rows, vocab, drafts.data_ptr(),
         probabilities.data_ptr() if probabilities is not None else 0, probabilities.stride(0) if probabilities is not None else 0, uniform.data_ptr(), noise.data_ptr(),
-        noise.stride(0), temperature.data_ptr(), memory, accepted.data_ptr(), tokens.data_ptr(), most, status_word(device).data_ptr(), stream), "verify_drafts")
+        noise.stride(0), temperature.data_ptr(), memory, accepted.data_ptr(), tokens.data_ptr(), most, sm_count(device), status_word(device).data_ptr(), stream), "verify_drafts")
     return accepted, tokens
 
 
