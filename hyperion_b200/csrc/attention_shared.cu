@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<E8, NQ>::BLOCKS)) attention_st
                 if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e], parts[warp * ROWS + q * 8 + 2 * t + e] = l[q][e];
             }
         meet();
-        if (*lost && !TOGETHER) return;  // all four warps see the same: they set it before they come here only.  (A cluster's blocks leave together, whatever it is that they join.)
+        if (*lost && !TOGETHER) break;  // all four warps see the same: they set it before they come here only.  (A cluster's blocks leave together, whatever it is that they join.)
         float f[NQ][2];
 #pragma unroll
         for (int q = 0; q < NQ; ++q)

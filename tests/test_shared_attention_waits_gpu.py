@@ -44,3 +44,23 @@ def test_waits_that_run_out(bits, limit, monkeypatch):
     for call, want in calls:
         agree(attention_shared(*call), *want)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_strips_that_leave_early_still_end_behind_the_tiles(bits, monkeypatch):
+    """Strips start beside the tiles of their step, and whoever comes next waits for the strips alone: also where their waits run out, they end when the tiles have."""
+    counts, lengths, groups = [1] * 60, [8100] * 60, ((0, 60, 8000),)
+    q, cache, table = step(counts, lengths, 8, 2, 64, 16, bits, groups)
+    plan = plan_shared(counts, lengths, 8, 2, 64, shared=groups)
+    assert plan.tile_blocks and plan.strip_blocks
+    call = (q, 8, cache, table, plan, 0.125)
+    want = attention_shared(*call)
+    short = native.library("attention_shared", HB_HEAD_DIM=64, HB_WAIT_LIMIT=0).hb_attention_strips
+    short.argtypes = native._entries["hb_attention_strips", 64].argtypes
+    for _ in range(20):
+        with monkeypatch.context() as patch:
+            patch.setitem(native._entries, ("hb_attention_strips", 64), short)
+            attention_shared(*call)
+        assert torch.equal(attention_shared(*call), want)  # over the same scratch memory
+    with pytest.raises(ops.KernelError, match="bounded wait"):
+        ops.raise_on_status(q.device)
