@@ -21,7 +21,7 @@
 // e4m3 as it is, too, but on this architecture each such product costs the conversions and four additions besides: 46 us against 42 where both were built.)  The
 // exponents are kept out of the entries: a key's multiplies its score, and a value's goes into the softmax's exponent,
 //     z_j = y_j + e_j,  P_j = 2^(z_j - m),  o = sum P_j code_j,  l = sum P_j 2^-e_j,
-// with m the maximum of z.  Which entry of a head a lane's fragment holds does not matter to Q K^T as long as it is the same one in Q and K, so a
+// with m 2^8 below the maximum of z.  A P below 2^-14 is rounded to 2^-25, 2^-33 of the largest: with the value's exponent in it that is a share of what the heaviest record brings.  Which entry of a head a lane's fragment holds does not matter to Q K^T as long as it is the same one in Q and K, so a
 // lane takes 16 bytes of a key at once, and Q's fragments are loaded to match; the columns of P V come out in another order than they are stored in, and are
 // stored where they belong.
 //

@@ -16,8 +16,8 @@
 // key that takes nearly all of a row's weight and brings nothing to an entry, the entry is made of thousands of those.)  A row of S is 128 float columns of tensor memory and the two
 // parts of its P are 2 x 64, so P takes exactly the place of the S it was made from, 32 keys at a time; the softmax reads S twice (for the maximum, then for the weights), 32
 // columns under way while it works on 32.  P is handed over in two halves of the tile's keys, so that the product of the first runs under the making of the second.
-// What bounds it is the chain of a half: from the arrival of S until the last weights are handed over (of which 1,024 clocks are the special function unit's for 128 columns,
-// which the other half's want as well), then the rest of O += P V, the next S and its arrival.  4,000 clocks a tile, of which the tensor core is busy for 3,072.
+// What bounds it is the chain of a half: from the arrival of S 2,750 clocks until the last weights are handed over (of which 1,024 are the special function unit's for 128 columns,
+// which the other half's want as well), then 1,390 for the rest of O += P V, the next S and its arrival.  4,100 clocks a tile, of which the tensor core is busy for 3,072.
 // Tried and dropped, with weights as float16 and 3,600 clocks a tile: weights by the maximum so far with one reading of S (3,150 clocks as long as no maximum is outgrown, 5,000 when one of
 // 256 rows' is, and one often is); a part of the exponentials by a polynomial (no faster); two threads a row (4,700); an issuer for each half (the halves fall into step: 4,700).
 //

@@ -7,13 +7,14 @@
 // running sum over the vocabulary is needed, and the answer does not hang on the order of one.  With temperature 0 a draft stands when it is
 // its row's largest logit (the lowest index of equal ones), and that token follows.
 //
-// Both kernels are bound by memory.  The first reads every row once, a block a piece of it, and leaves each piece's maximum and sum (or its argmax); a request's end is
+// The first kernel reads every row once, a block a piece of it, and leaves each piece's maximum and sum (or its argmax); a request's end is
 // known only when all its rows' sums are.  The second takes, per request, the one row at which the request ends, the drafter's and the noise: each of its blocks first works
 // out the request's end from the pieces (a few kilobytes out of L2, with the noise on its way meanwhile), then looks through its part, and the block that comes last
 // writes the request's answer.  Pieces are as many as the device holds blocks at once: a block's start (which request is this, what is its temperature; where does it
 // end) costs as much as some 20,000 entries.  Both keep the batches to come on their way while they look at the one at hand, some 64 KB an SM.  64 requests of up to six
-// bfloat16 rows of 152,064 logits, with the drafter's probabilities: 40 us for 165 MB, 4.1 TB/s (one batch of 8 KB ahead in the first kernel and none in the second: 47 us).  One
-// request of five float rows: 9.3 us, two kernels' starts and a few trips to memory.  A NaN counts as -infinity, +infinity as the largest number; a row without any finite logit has p = 0 everywhere, and its
+// bfloat16 rows of 152,064 logits, with the drafter's probabilities: 41 us for 165 MB, 4.0 TB/s (one batch of 8 KB ahead in the first kernel and none in the second: 47 us).  Alone the two run at 3.2 and 3.1 TB/s
+// with issue slots at 45 and 28 %: neither memory nor instructions bound them, but the trips of the batches on their way, and the starts.  One
+// request of five float rows: 9.4 us, two kernels' starts and a few trips to memory.  Exponentials and reciprocals are the hardware's (2^-22 of a weight), sums float.  A NaN counts as -infinity, +infinity as the largest number; a row without any finite logit has p = 0 everywhere, and its
 // token is the lowest index.
 #include <float.h>
 

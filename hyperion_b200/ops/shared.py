@@ -38,7 +38,9 @@ def plan_shared(counts: Sequence[int], lengths: Sequence[int], heads: int, kv_he
     """Plan a step of ``counts[r]`` queries of request r, whose block table (row r) holds ``lengths[r]`` positions: token i of n sees the first
     ``lengths[r] - n + i + 1`` of them (one with nothing to see comes out as zeros).  ``shared``: (first request, requests, positions) of each group
     of consecutive requests that hold the same pages for their first positions, which all of their queries see; in order, none of them overlapping.
-    ``device`` is where the plan is kept, which has to be the device of the step's tensors; ``sms`` its multiprocessors, asked from it when absent."""
+    ``device`` is where the plan is kept, which has to be the device of the step's tensors; ``sms`` its multiprocessors, asked from it when absent.
+
+    The plan is copied there from ordinary memory, so this returns when the current stream has come to the copy: a step is planned before its work is queued."""""
     n, length, groups = (host_runtime.ints(values, np.int64) for values in (counts, lengths, shared))
     if n.ndim != 1 or n.shape != length.shape or (len(groups) and groups.shape[1:] != (3,)):
         raise KernelError("plan_shared: a count of queries and a length for each request, and groups as (first request, requests, positions)")
@@ -64,7 +66,10 @@ def attention_shared(q: torch.Tensor, heads: int, cache, block_table: torch.Tens
     stand on 16-byte boundaries, rows of ``out`` on 8-byte ones.  Returns [tokens, heads * d].
 
     Slots beyond a request's length may hold anything.  What a request's own later tokens hold is masked by weights of 0 for its earlier ones, so
-    their values have to be finite."""
+    their values have to be finite.
+
+    A call's scratch memory is 4 * heads * (d + 2) bytes per piece, and over a Cache8 512 * d bytes per 128 positions and key/value head that runs of more than 64 (token, head) rows
+    walk (twice those records): up to 16 MB are kept per thread and stream, more is allocated for the call."""""
     if isinstance(cache, Cache8):
         pages, kv_heads, page_size, head_dim = check_cache8(cache, "attention_shared")
         parts, entries, exponents = cache, cache[0].data_ptr(), cache[1].data_ptr()

@@ -29,7 +29,7 @@ def verify_drafts(logits: torch.Tensor, row_start: torch.Tensor, drafts: torch.T
     than it has drafts; ``most`` is at least the largest such number of rows.  ``drafts`` [rows] int32: the token drafted at each row (a request's
     last one is not read); ``probabilities`` [rows, vocab] float32: the drafter's at that row, or None where it gave none (its token then counts
     with probability 1); ``uniform`` [rows] float32 in [0, 1); ``noise`` [requests, vocab] float32, exponentially distributed, above 0;
-    ``temperature`` [requests] float32, 0 for greedy.  A draft outside the vocabulary does not stand and is reported (``raise_on_status``)."""
+    ``temperature`` [requests] float32, 0 for greedy.  At most 65,535 rows and requests.  A draft outside the vocabulary does not stand and is reported (``raise_on_status``)."""
     shape, starts = logits.shape, row_start.shape
     if len(shape) != 2 or len(starts) != 1 or starts[0] < 1:
         raise KernelError("verify_drafts: logits [rows, vocab] and row_start [requests + 1]")
