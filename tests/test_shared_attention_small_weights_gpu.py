@@ -1,8 +1,9 @@
 """A key that takes nearly all of a row's weight and brings little or nothing to an entry, before thousands of keys whose weights are small beside its own: the entry is theirs.
 
-Tolerance: the result's rounding (2^-9 of it), and the weights'.  Over 8-bit records, runs of many rows carry weights in two parts of bfloat16 (2^-16 of each); runs of few rows carry them
-in float16, 2^8 above one for the largest: 2^-12 of a weight, and 2^-25 where it lies below 2^-14.  With the largest weight 2^29 times the others that is up to 2^-4 of one
-weight, and of the sum of 3,000 of random size 2^-4 / sqrt(3 * 3,000) < 2^-10.  2^-8 of sum_j p_j |v_j| holds both, and what float32 adds."""
+Tolerance: the result's rounding (up to 2^-8 of it, and results are well below sum_j p_j |v_j| here: 3,000 terms of either sign), and the weights'.  Over 8-bit records, runs of many rows carry
+weights in two parts of bfloat16 (2^-15 of each); runs of few rows carry them in float16, 2^8 above one for the largest: 2^-11 of a weight, and 2^-25 where it lies below 2^-14.  With
+the largest weight 2^29 times the others that is up to 2^-4 of one weight, and of the sum of 3,000 of random size 2^-4 / sqrt(3 * 3,000) < 2^-10.  2^-8 of sum_j p_j |v_j| holds both, and
+what float32 adds."""
 from __future__ import annotations
 
 import pytest
