@@ -1,0 +1,599 @@
+// Attention of one new token per request over its pages, whose weights are kept: what the token gives each slot, summed over the query heads of a key/value head, is added to
+// the slot's weight, by which a cache of a fixed budget is cut back later (evict.cu).  bfloat16 pages, head sizes 64 and 128 (HB_HEAD_DIM), pages of 8 to 64 slots.
+//
+//     y_hj = q_h . k_j scale log2(e),   m_h = max_j y_hj,   l_h = sum_j 2^(y_hj - m_h),   out_h = sum_j 2^(y_hj - m_h) v_j / l_h
+//     weights[j] += sum_h 2^(y_hj - m_h) / l_h                  the token's own slot, the last: = instead of +=, and its position is written beside
+//
+// A weight is known only when its head's whole row has been seen, so the scores themselves are kept until then: 4 bytes a head and slot beside the 4 d bytes of a key and a value.  (Reading the
+// keys a second time would cost 2 d bytes a slot against 8 a head and slot for writing the scores and reading them back.)
+//
+// The first kernel walks keys and values.  The lengths stay on the device: the requests' slots stand in a line, in tiles of 64, and each of the blocks works out where its equal share of the line begins
+// and ends.  A share's part of one request is a piece (m, l and o of its heads); block b's piece of request r has the number b + r, which grows along the line and so is no other one's.  The second
+// kernel puts the pieces of a request together, in the order of the line, and adds the weights.
+//
+// In a block one lane of a producer warp per page fetches keys and values by TMA into a ring of stages, and each of four warps takes 16 of a stage's 64 slots for all rows.  The products are
+// S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): slots and entries stand where the instruction has 16 rows, the few heads of a key/value head where it has 8 columns.  The weights are taken into the second
+// product in two parts, rounded to bfloat16 and what that left over: rounded once they would cost the result as much as its own rounding does.
+//
+// Slots beyond a request's length may hold anything: their scores are replaced and their values read as zeros.  Every wait is bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the
+// block leaves, once the copies that it has on their way have arrived.
+#include <cuda.h>
+
+#include "common.cuh"
+
+#ifndef HB_HEAD_DIM
+#define HB_HEAD_DIM 128
+#endif
+#ifndef HB_WAIT_LIMIT
+#define HB_WAIT_LIMIT (1u << 24)
+#endif
+
+namespace {
+typedef __nv_bfloat16 bf16;
+constexpr int D = HB_HEAD_DIM;
+static_assert(D == 64 || D == 128, "head sizes 64 and 128");
+constexpr int WARPS = 4;  // that compute; one more fetches
+constexpr int THREADS = 32 * (WARPS + 1);
+constexpr int BN = 64;    // slots of a tile
+constexpr int TILE = BN * D * 2, PANELS = D / 64;
+constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
+static_assert(BN / WARPS == 16, "a warp takes the 16 rows of a product");
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count)); }
+__device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ bool mbar_over(unsigned long long* bar, unsigned parity) {
+    unsigned done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
+    for (unsigned spin = 0; spin < WAIT_LIMIT; ++spin) {
+        if (mbar_over(bar, parity)) return true;
+        if ((spin & 1023) == 1023 && *failed) return false;
+    }
+    return false;
+}
+// Before a block leaves: what it has set going is done, whatever has become of its other waits.
+__device__ __forceinline__ void mbar_last_wait(unsigned long long* bar, unsigned parity) {
+    for (unsigned spin = 0; spin < LAST_WAIT_LIMIT; ++spin)
+        if (mbar_over(bar, parity)) return;
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ unsigned turned(unsigned w) {  // an 8 x 8 matrix of 16-bit entries, two of a row a lane, transposed
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(unsigned (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack(float lo, float hi) {
+    unsigned w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16-byte chunk cc of slot `key` of a tile as TMA's swizzle has placed it.
+__device__ __forceinline__ int tile_at(int key, int cc) { return (cc >> 3) * (BN * 128) + key * 128 + (((cc & 7) ^ (key & 7)) << 4); }
+
+template <int NQ>  // eights of rows
+struct Shape {
+    static constexpr int ROWS = 8 * NQ;
+    static constexpr int BLOCKS = NQ == 1 ? 3 : 2;  // an SM, by registers
+    static constexpr int STAGES = (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
+    // Where the warps' results meet: COLS entries of every row at a time, a row's LINE floats apart (lanes that store side by side then take different banks).
+    static constexpr int COLS = 64 / NQ, LINE = COLS + 4;
+    static constexpr int JOIN = WARPS * ROWS * LINE * 4;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * TILE + JOIN + 2 * WARPS * ROWS * 4 + 2 * STAGES * 8 + 32;
+    static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "an SM's shared memory");
+};
+
+struct Args {
+    const bf16* q; int q_stride;
+    bf16* out; int out_stride;
+    const int* block_table; int table_width;
+    const int* lengths; int requests;
+    int longest, slots;      // the longest that a request may be; the same in whole tiles: a row of scores
+    float* scores;           // [requests, heads, slots]
+    float* pieces;           // [blocks + requests, heads, D]
+    float2* sums;            // [blocks + requests, heads]: (m, l)
+    float* weights;          // [requests, kv_heads, capacity]
+    int* positions;          // [requests, kv_heads, capacity]
+    const int* newest;       // [requests]
+    int capacity;
+    int heads, kv_heads, page_size, pages;
+    int gc, chunks;          // heads of a strip, strips of a key/value head's group
+    int blocks;              // of the first kernel, side by side
+    float scale_log2;
+    int* status;
+};
+
+// The line of all requests' tiles, as one warp sees it.
+__device__ __forceinline__ int length_of(const Args& a, int request) { return min(max(a.lengths[request], 0), a.longest); }
+__device__ __forceinline__ int tiles_of(const Args& a, int request) { return (length_of(a, request) + BN - 1) / BN; }
+__device__ __forceinline__ long long line_length(const Args& a, int lane) {
+    long long total = 0;
+    for (int r = lane; r < a.requests; r += 32) total += tiles_of(a, r);
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
+    return total;
+}
+// The last request that begins at or before tile `at` of the line and has tiles, and where it begins.  `at` is below the line's length.
+__device__ __forceinline__ int request_at(const Args& a, long long at, long long& begins, int lane) {
+    long long before = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += 32) {
+        const int n = r0 + lane < a.requests ? tiles_of(a, r0 + lane) : 0;
+        long long end = n;  // inclusive sum
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const long long other = __shfl_up_sync(0xffffffffu, end, offset);
+            if (lane >= offset) end += other;
+        }
+        end += before;
+        const unsigned beyond = __ballot_sync(0xffffffffu, end > at);
+        if (beyond) {
+            const int who = __ffs(beyond) - 1;
+            begins = __shfl_sync(0xffffffffu, end - n, who);
+            return r0 + who;
+        }
+        before = __shfl_sync(0xffffffffu, end, 31);
+    }
+    begins = before;
+    return a.requests;
+}
+// Block b of n takes the tiles from b total / n on; the block that has tile `at`.  n <= total: every block has one.
+__device__ __forceinline__ long long share_from(long long b, long long n, long long total) { return b * total / n; }
+__device__ __forceinline__ int block_at(long long at, long long n, long long total) { return (int)(((at + 1) * n - 1) / total); }
+
+template <int NQ>
+__global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
+    typedef Shape<NQ> S;
+    constexpr int ROWS = S::ROWS;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    float* join = reinterpret_cast<float*>(ring + (size_t)S::STAGES * 2 * TILE);  // [WARPS][ROWS][LINE]
+    float* tops = join + S::JOIN / 4;                                               // [WARPS][ROWS]: maxima
+    float* parts = tops + WARPS * ROWS;                                             // [WARPS][ROWS]: sums
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(parts + WARPS * ROWS);
+    unsigned long long* empty = full + S::STAGES;
+    volatile int* failed = reinterpret_cast<volatile int*>(empty + S::STAGES);
+    volatile int* lost = failed + 1;  // a computing warp has given up
+    int* share = const_cast<int*>(failed) + 2;  // first request, its first tile here, tiles in all
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], WARPS); }
+        *failed = 0, *lost = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == WARPS && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
+    let_next_kernel_start();
+    wait_for_previous_kernels();
+    if (warp == WARPS) {
+        const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
+        int request = 0, tile = 0, tiles = 0;
+        if ((long long)blockIdx.x < n) {
+            const long long from = share_from(blockIdx.x, n, total), to = share_from(blockIdx.x + 1, n, total);
+            long long begins;
+            request = request_at(a, from, begins, lane);
+            tile = (int)(from - begins), tiles = (int)(to - from);
+        }
+        if (lane == 0) share[0] = request, share[1] = tile, share[2] = tiles;
+    }
+    __syncthreads();
+    const int kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
+    const int group = a.heads / a.kv_heads, first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
+    int request = share[0], tile = share[1], left = share[2], stage = 0;  // the ring runs on across the block's requests
+
+    if (warp == WARPS) {
+        // ------------------------------------------------------------------ producer (the whole warp)
+        const int shift = 31 - __clz(a.page_size), pages_per_tile = BN >> shift, tiles_per_look = 32 / pages_per_tile;
+        constexpr int OPS_PER_PAGE = 2 * PANELS;
+        const int ops = pages_per_tile * OPS_PER_PAGE;
+        const unsigned page_bytes = 2u * a.page_size * D * 2;
+        int ok = 1;
+        for (; left > 0 && ok; ++request, tile = 0) {
+            const int length = length_of(a, request), here = min(left, (length + BN - 1) / BN - tile);
+            const int* table = a.block_table + (size_t)request * a.table_width;
+            int looked = -1;
+            for (int it = 0; it < here; ++it, ++stage) {
+                const int s = stage % S::STAGES, round = stage / S::STAGES, base = (tile + it) * BN;
+                if (it % tiles_per_look == 0) {  // a page number per lane, for the next tiles
+                    const int block = (base >> shift) + lane;
+                    looked = block < a.table_width ? __ldg(table + block) : -1;
+                }
+                if (lane == 0) ok = mbar_wait(&empty[s], (round & 1) ^ 1, failed) ? 1 : 0;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) {
+                    if (lane == 0) { *failed = 1; atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_TALLIED); }
+                    break;
+                }
+                int page = __shfl_sync(0xffffffffu, looked, (it % tiles_per_look) * pages_per_tile + (lane & (pages_per_tile - 1)));
+                const bool wanted = lane < pages_per_tile && base + lane * a.page_size < length;
+                if (wanted && (page < 0 || page >= a.pages)) atomicOr(a.status, HB_STATUS_BAD_PAGE);
+                if (!wanted || page >= a.pages) page = -1;
+                const unsigned valid = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) {
+                    if (valid) mbar_expect_tx(&full[s], valid * page_bytes); else mbar_arrive(&full[s]);
+                }
+                __syncwarp();
+                unsigned char* tiles = ring + (size_t)s * 2 * TILE;
+                for (int op0 = 0; op0 < ops; op0 += 32) {
+                    const int op = op0 + lane;
+                    const int p = min(op, ops - 1) / OPS_PER_PAGE, rest = op % OPS_PER_PAGE, which = rest / PANELS, panel = rest - which * PANELS;
+                    const int from = __shfl_sync(0xffffffffu, page, p);
+                    if (op < ops && from >= 0)
+                        tma_load_2d(tiles + which * TILE + panel * (BN * 128) + p * a.page_size * 128, &kv_map, &full[s], panel * 64, ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
+                }
+            }
+            left -= here;
+        }
+        if (lane == 0)
+            for (int k = max(0, stage - S::STAGES); k < stage; ++k) mbar_last_wait(&full[k % S::STAGES], (k / S::STAGES) & 1);
+        return;
+    }
+    // ---------------------------------------------------------------------- consumers
+    const int t = lane & 3, g = lane >> 2;
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); };
+    constexpr int LANES_PER_ROW = S::COLS / 16;
+    const int store_row = lane / LANES_PER_ROW, store_col = warp * (S::COLS / 4) + lane % LANES_PER_ROW * 4;  // what this lane stores of every COLS entries
+    const bool stores = store_row < heads_here;
+    for (; left > 0; ++request, tile = 0) {
+        const int length = length_of(a, request), here = min(left, (length + BN - 1) / BN - tile), start = tile * BN;
+        left -= here;
+        // Q's fragments: a lane's 16-byte chunk t + 4 j of a key feeds products 2 j and 2 j + 1, four of its entries each, so a query's entries stand in the fragments likewise.
+        unsigned qf[NQ][D / 16][2];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const int head = q * 8 + g;
+            const bf16* src = a.q + (size_t)request * a.q_stride + (size_t)(first_head + (head < heads_here ? head : 0)) * D;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const uint4 raw = head < heads_here ? *reinterpret_cast<const uint4*>(src + (t + 4 * j) * 8) : make_uint4(0, 0, 0, 0);
+                qf[q][2 * j][0] = raw.x, qf[q][2 * j][1] = raw.y, qf[q][2 * j + 1][0] = raw.z, qf[q][2 * j + 1][1] = raw.w;
+            }
+        }
+        float* scores[NQ][2];  // of columns 2 t and 2 t + 1
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int head = q * 8 + 2 * t + e;
+                scores[q][e] = head < heads_here ? a.scores + ((size_t)request * a.heads + first_head + head) * a.slots : nullptr;
+            }
+        float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            m[q][0] = m[q][1] = -INFINITY, l[q][0] = l[q][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[q][i][0] = o[q][i][1] = o[q][i][2] = o[q][i][3] = 0.f;
+        }
+        for (int it = 0; it < here; ++it, ++stage) {
+            const int s = stage % S::STAGES, round = stage / S::STAGES;
+            if (!mbar_wait(&full[s], round & 1, failed)) {
+                *failed = 1, *lost = 1;
+                atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_ATTENTION_TALLIED);
+                break;
+            }
+            const unsigned char* ks = ring + (size_t)s * 2 * TILE;
+            const unsigned char* vs = ks + TILE;
+            const int key0 = warp * 16, pos0 = start + it * BN + key0;  // this warp's slots
+            if (pos0 < length) {
+                const bool whole = pos0 + 16 <= length;
+                float sc[NQ][4];  // of slots g and g + 8 and columns 2 t and 2 t + 1: [(slot, column)]
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) sc[q][0] = sc[q][1] = sc[q][2] = sc[q][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    const uint4 k0 = *reinterpret_cast<const uint4*>(ks + tile_at(key0 + g, t + 4 * j)), k1 = *reinterpret_cast<const uint4*>(ks + tile_at(key0 + 8 + g, t + 4 * j));
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        mma(sc[q], k0.x, k1.x, k0.y, k1.y, qf[q][2 * j][0], qf[q][2 * j][1]);
+                        mma(sc[q], k0.z, k1.z, k0.w, k1.w, qf[q][2 * j + 1][0], qf[q][2 * j + 1][1]);
+                    }
+                }
+                bool rescale = false;
+                float alpha[NQ][2];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sc[q][e] *= a.scale_log2;
+                        const int pos = pos0 + (e >> 1) * 8 + g;
+                        if (!whole && pos >= length) sc[q][e] = -INFINITY;
+                        else if (scores[q][e & 1]) scores[q][e & 1][pos] = sc[q][e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(sc[q][e], sc[q][2 + e]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float m_new = fmaxf(m[q][e], mx);
+                        alpha[q][e] = m_new == -INFINITY ? 1.f : fast_exp2(m[q][e] - m_new);
+                        m[q][e] = m_new;
+                        rescale |= alpha[q][e] != 1.f;
+                        const float base = m_new == -INFINITY ? 0.f : m_new;
+                        l[q][e] *= alpha[q][e];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            sc[q][2 * h + e] = fast_exp2(sc[q][2 * h + e] - base);
+                            l[q][e] += sc[q][2 * h + e];  // of this lane's slots; the lanes are added up at the end
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) o[q][i][0] *= alpha[q][0], o[q][i][1] *= alpha[q][1], o[q][i][2] *= alpha[q][0], o[q][i][3] *= alpha[q][1];
+                }
+                // Values beyond the length read as zeros, whatever their slots hold.  A fragment register holds slots 2 t and 2 t + 1 in its halves.
+                unsigned keep[2] = {0xffffffffu, 0xffffffffu};
+                if (!whole) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int pos = pos0 + h * 8 + t * 2;
+                        keep[h] = (pos < length ? 0xffffu : 0u) | (pos + 1 < length ? 0xffff0000u : 0u);
+                    }
+                }
+                unsigned pf[NQ][2], pr[NQ][2];  // the weights, and what they lose by rounding, as weights of their own
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float p0 = sc[q][2 * h], p1 = sc[q][2 * h + 1];
+                        const unsigned w = pack(p0, p1);
+                        pf[q][h] = turned(w);
+                        pr[q][h] = turned(pack(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
+                    }
+#pragma unroll
+                for (int c = 0; c < D / 8; c += 2) {
+                    unsigned b[4];
+                    ldmatrix_x4_trans(b, vs + tile_at(key0 + (lane & 15), c + (lane >> 4)));
+                    if (!whole) b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        mma(o[q][c / 2], b[0], b[2], b[1], b[3], pf[q][0], pf[q][1]);
+                        mma(o[q][c / 2], b[0], b[2], b[1], b[3], pr[q][0], pr[q][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+        // The warps' results meet: every warp brings its sums to the largest maximum and lays COLS entries of its rows down, then takes a quarter of them, adds up the four
+        // warps' in their order, and stores.
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 4);
+                l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 8);
+                l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], 16);
+                if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e], parts[warp * ROWS + q * 8 + 2 * t + e] = l[q][e];
+            }
+        meet();
+        if (*lost) break;  // all four warps see the same: they set it before they come here only
+        float f[NQ][2];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = q * 8 + 2 * t + e;
+                const float top = fmaxf(fmaxf(tops[row], tops[ROWS + row]), fmaxf(tops[2 * ROWS + row], tops[3 * ROWS + row]));
+                f[q][e] = m[q][e] == -INFINITY ? 0.f : fast_exp2(m[q][e] - top);
+            }
+        float top = -INFINITY, all = 0.f;  // of the row that this lane stores
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, tops[w * ROWS + store_row]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float mw = tops[w * ROWS + store_row];
+            all = fmaf(mw == -INFINITY ? 0.f : fast_exp2(mw - top), parts[w * ROWS + store_row], all);
+        }
+        const size_t slot = ((size_t)blockIdx.x + request) * a.heads + first_head + store_row;
+        if (stores && store_col == 0) a.sums[slot] = make_float2(top, all);
+#pragma unroll
+        for (int col = 0; col < D; col += S::COLS) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float* dst = join + (warp * ROWS + q * 8 + 2 * t + e) * S::LINE;
+#pragma unroll
+                    for (int i = 0; i < S::COLS / 16; ++i) dst[16 * i + g] = o[q][col / 16 + i][e] * f[q][e], dst[16 * i + 8 + g] = o[q][col / 16 + i][2 + e] * f[q][e];
+                }
+            meet();
+            if (stores) {
+                float sum[4];
+                load4(join + store_row * S::LINE + store_col, sum);
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) {
+                    float more[4];
+                    load4(join + (w * ROWS + store_row) * S::LINE + store_col, more);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] += more[i];
+                }
+                store4(a.pieces + slot * D + col + store_col, sum);
+            }
+            meet();
+        }
+    }
+}
+
+// The second kernel: block x of a (key/value head, request) adds the weights of SPAN slots, the last x puts the request's result together.  Every block first brings the pieces' sums together.
+constexpr int ADD_THREADS = 256, SPAN = 4 * ADD_THREADS, MOST_GROUP = 64;  // heads whose sums a block holds at a time
+__global__ void __launch_bounds__(ADD_THREADS) tally_kernel(const Args a) {
+    __shared__ float2 heads_sum[MOST_GROUP];  // (m, 1 / l) of the heads
+    __shared__ int range[2];                  // the request's first block of the first kernel, and its pieces
+    let_next_kernel_start();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, request = blockIdx.z, group = a.heads / a.kv_heads;
+    const bool puts_together = blockIdx.x == gridDim.x - 1;
+    wait_for_previous_kernels();
+    const int length = length_of(a, request), first = blockIdx.x * SPAN;
+    if (tid == 0 && puts_together && kvh == 0 && a.lengths[request] > a.longest) atomicOr(a.status, HB_STATUS_BAD_POSITION);
+    if (!puts_together && first >= length) return;
+    if (length && warp == 0) {
+        const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
+        long long begins = 0;
+        for (int r = lane; r < request; r += 32) begins += tiles_of(a, r);
+#pragma unroll
+        for (int offset = 16; offset > 0; offset >>= 1) begins += __shfl_xor_sync(0xffffffffu, begins, offset);
+        const int b0 = block_at(begins, n, total), b1 = block_at(begins + (length + BN - 1) / BN - 1, n, total);
+        if (lane == 0) range[0] = b0, range[1] = b1 - b0 + 1;
+    }
+    __syncthreads();
+    const int count = length ? range[1] : 0;
+    const size_t piece0 = ((size_t)(length ? range[0] : 0) + request) * a.heads + (size_t)kvh * group;  // of the group's first head
+    const size_t tally = ((size_t)request * a.kv_heads + kvh) * a.capacity;
+    float added[SPAN / ADD_THREADS] = {};
+    for (int g0 = 0; g0 < group; g0 += MOST_GROUP) {
+        const int here = min(MOST_GROUP, group - g0);
+        for (int h = warp; h < here; h += ADD_THREADS / 32) {
+            float top = -INFINITY, all = 0.f;
+            for (int p = lane; p < count; p += 32) {
+                const float2 ml = a.sums[piece0 + (size_t)p * a.heads + g0 + h];
+                const float above = fmaxf(top, ml.x);
+                all = above == -INFINITY ? all + ml.y : fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - above), ml.y, all * (top == -INFINITY ? 0.f : fast_exp2(top - above)));
+                top = above;
+            }
+            const float above = warp_max(top);
+            all = warp_sum(top == -INFINITY ? all : all * fast_exp2(top - above));
+            if (lane == 0) heads_sum[h] = make_float2(above == -INFINITY ? 0.f : above, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
+        }
+        __syncthreads();
+        if (!puts_together) {
+            for (int h = 0; h < here; ++h) {
+                const float* row = a.scores + ((size_t)request * a.heads + (size_t)kvh * group + g0 + h) * a.slots + first;
+                const float2 ml = heads_sum[h];
+#pragma unroll
+                for (int i = 0; i < SPAN / ADD_THREADS; ++i) {
+                    const int at = i * ADD_THREADS + tid;
+                    if (first + at < length) added[i] = fmaf(fast_exp2(row[at] - ml.x), ml.y, added[i]);
+                }
+            }
+        } else {
+            for (int at = tid; at < here * (D / 4); at += ADD_THREADS) {
+                const int h = at / (D / 4), col = at % (D / 4) * 4;
+                const float2 ml = heads_sum[h];
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int p = 0; p < count; ++p) {
+                    const size_t slot = piece0 + (size_t)p * a.heads + g0 + h;
+                    const float m = a.sums[slot].x, f = m == -INFINITY ? 0.f : fast_exp2(m - ml.x);
+                    float part[4];
+                    load4(a.pieces + slot * D + col, part);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, part[e], sum[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] *= ml.y;
+                store4(a.out + (size_t)request * a.out_stride + ((size_t)kvh * group + g0 + h) * D + col, sum);
+            }
+        }
+        __syncthreads();
+    }
+    if (puts_together) return;
+#pragma unroll
+    for (int i = 0; i < SPAN / ADD_THREADS; ++i) {
+        const int slot = first + i * ADD_THREADS + tid;
+        if (slot >= length) continue;
+        if (slot == length - 1) {
+            a.weights[tally + slot] = added[i];
+            a.positions[tally + slot] = a.newest[request];
+        } else {
+            a.weights[tally + slot] += added[i];
+        }
+    }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* found = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &found, cudaEnableDefault, &result) == cudaSuccess && result == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiled>(found) : nullptr;
+    }();
+    return fn;
+}
+// The cache as a matrix [pages * 2 * kv_heads * page_size, D], fetched in boxes of a page's rows and 64 entries.
+int cache_map(CUtensorMap* map, const void* cache, const Args& a) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return HB_BAD_ARGUMENT;
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)a.pages * 2 * a.kv_heads * a.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)a.page_size};
+    const cuuint32_t elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
+}
+template <int NQ>
+int launch_strips(const Args& a, const CUtensorMap& map, cudaStream_t stream) {
+    const auto kernel = attention_tallied_kernel<NQ>;
+    const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<NQ>::SMEM);
+    if (configured != cudaSuccess) return (int)configured;
+    return launch_after_previous(kernel, dim3(a.blocks, a.kv_heads * a.chunks), dim3(THREADS), Shape<NQ>::SMEM, stream, map, a);
+}
+}  // namespace
+
+// Blocks of the first kernel that stand side by side for a key/value head's strip: what the device holds, but no more than there can be tiles.
+static int blocks_for(int requests, int longest, int heads, int kv_heads, int sms) {
+    const int group = heads / kv_heads, gc = group <= 8 ? group : group < 16 ? group : 16, chunks = (group + gc - 1) / gc;
+    const long long room = (long long)sms * (gc <= 8 ? Shape<1>::BLOCKS : Shape<2>::BLOCKS) / ((long long)kv_heads * chunks), tiles = (long long)requests * ((longest + BN - 1) / BN);
+    return (int)(room < 1 ? 1 : room < tiles ? room : tiles);
+}
+// Bytes of scratch that hb_attention_tallied takes.
+HB_EXPORT long long hb_attention_tallied_scratch(int requests, int longest, int heads, int kv_heads, int sms) {
+    if (requests <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || sms <= 0) return 0;
+    const long long slots = (longest + BN - 1) / BN * BN, pieces = (long long)blocks_for(requests, longest, heads, kv_heads, sms) + requests;
+    return 4 * heads * (requests * slots + pieces * (D + 2));
+}
+// q [requests, heads * D] with rows q_stride apart; cache [pages, 2, kv_heads, page_size, D]; weights, positions [requests, kv_heads, capacity]; lengths, newest [requests], lengths at most
+// `longest`, which table and capacity hold.  scratch: hb_attention_tallied_scratch bytes on a 16-byte boundary.
+HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, const int* block_table, int table_width, const int* lengths, int requests,
+                                   int longest, float* weights, int* positions, const int* newest, int capacity, int heads, int kv_heads, int page_size, int pages, float scale, int sms, void* scratch,
+                                   int* status, cudaStream_t stream) {
+    if (requests <= 0) return 0;
+    if (!q || !out || !cache || !block_table || !lengths || !weights || !positions || !newest || !scratch || !status) return HB_BAD_ARGUMENT;
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || out_stride % 4 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
+    if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
+    if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
+    if ((long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
+    if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
+    if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL || longest > 0x7fffffff - SPAN || requests > 65535) return HB_UNSUPPORTED_SIZE;
+    const int group = heads / kv_heads, gc = group < 16 ? group : 16, chunks = (group + gc - 1) / gc, slots = (longest + BN - 1) / BN * BN;
+    if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
+    const int blocks = blocks_for(requests, longest, heads, kv_heads, sms);
+    const size_t n_pieces = (size_t)blocks + requests;
+    float* pieces = (float*)scratch;
+    float2* sums = (float2*)(pieces + n_pieces * heads * D);
+    float* scores = (float*)(sums + n_pieces * heads);
+    const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, block_table, table_width, lengths, requests, longest, slots, scores, pieces, sums, weights, positions, newest, capacity,
+                 heads, kv_heads, page_size, pages, gc, chunks, blocks, scale * 1.4426950408889634f, status};
+    CUtensorMap map;
+    if (int code = cache_map(&map, cache, a)) return code;
+    if (int code = gc <= 8 ? launch_strips<1>(a, map, stream) : launch_strips<2>(a, map, stream)) return code;
+    return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + 1, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
+}

@@ -106,13 +106,14 @@ _KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": 
 _entries: dict = {}
 
 
-def entry(module: str, name: str, arguments: str, head_dim: int = 0):
-    """An exported launcher with its arguments' kinds (p: address, i: int, l: long long, f: float), looked up once: plain Python numbers then go to it as they are,
+def entry(module: str, name: str, arguments: str, head_dim: int = 0, result: str = "i"):
+    """An exported launcher with its arguments' and its result's kinds (p: address, i: int, l: long long, f: float), looked up once: plain Python numbers then go to it as they are,
     which costs a call of twenty arguments a few microseconds less than a ctypes object for each."""
     found = _entries.get((name, head_dim))
     if found is None:
         found = getattr(library(module, HB_HEAD_DIM=head_dim) if head_dim else library(module), name)
         found.argtypes = [_KINDS[kind] for kind in arguments]
+        found.restype = _KINDS[result]
         _entries[name, head_dim] = found
     return found
 

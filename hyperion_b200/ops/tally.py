@@ -1,0 +1,197 @@
+"""Caches of a fixed budget: attention that keeps its weights (csrc/attention_tallied.cu), the weights of a prompt's queries (csrc/tally_queries.cu), and the eviction of what weighs least
+(csrc/evict.cu).
+
+Beside its pages a request has a tally: for each key/value head and slot the weight that its queries have given the slot so far, summed over queries and query heads, and the position of the token
+that stands there.  Each key/value head keeps slots of its own; all of a request's heads hold the same number of them, its length.  A prompt's slots hold positions 0, 1, ... as a new tally has them;
+keys are stored rotated, so attention does not ask which slot a key stands in, and a slot that eviction fills goes on with its position."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .basic import status_word
+from .native import KernelError, check, entry, scratch, sm_count, stream_address
+
+
+class Tally(NamedTuple):
+    """``weights`` float32 and ``positions`` int32, both [requests, kv_heads, capacity], or [layers, requests, kv_heads, capacity]."""
+    weights: torch.Tensor
+    positions: torch.Tensor
+
+
+def supported(head_dim: int, page_size: int) -> bool:
+    return head_dim in (64, 128) and page_size in (8, 16, 32, 64)
+
+
+def new_tally(requests: int, kv_heads: int, capacity: int, layers: Optional[int] = None, device="cuda") -> Tally:
+    """A tally in which every slot weighs nothing and holds the position of its number, as a prompt's slots do."""
+    shape = (requests, kv_heads, capacity) if layers is None else (layers, requests, kv_heads, capacity)
+    positions = torch.arange(capacity, dtype=torch.int32, device=device).expand(shape).contiguous()
+    return Tally(torch.zeros(shape, device=device), positions)
+
+
+def _check_tally(tally: Tally, shape: tuple, what: str) -> int:
+    """The capacity of a tally [*shape, capacity]."""
+    weights, positions = tally
+    if (weights.dtype is not torch.float32 or positions.dtype is not torch.int32 or weights.dim() != len(shape) + 1 or weights.shape[:-1] != shape or positions.shape != weights.shape
+            or not weights.is_contiguous() or not positions.is_contiguous()):
+        raise KernelError(f"{what}: a tally is dense float32 weights and int32 positions {[*shape, 'capacity']}")
+    return weights.shape[-1]
+
+
+def _check_vectors(what: str, **vectors) -> None:
+    for name, (vector, size) in vectors.items():
+        if vector.dtype is not torch.int32 or vector.dim() != 1 or vector.shape[0] != size or not vector.is_contiguous():
+            raise KernelError(f"{what}: {name} is a dense int32 vector of {size}")
+
+
+def _check_device(what: str, *tensors) -> torch.device:
+    device = tensors[0].device
+    for tensor in tensors:
+        if tensor is not None and (tensor.device != device or not tensor.is_cuda):
+            raise KernelError(f"{what}: all tensors on one CUDA device, not on {device} and {tensor.device}")
+    if device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the tensors are on {device}, which is not the current device")
+    return device
+
+
+def _check_pages(what: str, cache, heads: int, q, block_table, requests: int, longest: int, scale: float) -> tuple[int, int, int, int]:
+    """(pages, kv_heads, page_size, head_dim) of a bfloat16 cache that ``q`` is to look at."""
+    if cache.dtype is not torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
+        raise KernelError(f"{what}: a dense bfloat16 cache [pages, 2, kv_heads, page, d]")
+    pages, _, kv_heads, page_size, head_dim = cache.shape
+    if not supported(head_dim, page_size):
+        raise KernelError(f"{what}: heads of 64 or 128 entries and pages of 8, 16, 32 or 64 slots, not {head_dim} and {page_size}")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise KernelError(f"{what}: {heads} heads over {kv_heads}")
+    if q.dtype is not torch.bfloat16 or q.dim() != 2 or q.shape[1] < heads * head_dim or q.stride(1) != 1:
+        raise KernelError(f"{what}: bfloat16 queries [tokens, {heads * head_dim}] with unit inner stride")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] < requests or not block_table.is_contiguous():
+        raise KernelError(f"{what}: a dense int32 block table of at least {requests} rows")
+    if longest < 0 or block_table.shape[1] * page_size < longest:
+        raise KernelError(f"{what}: a block table of {block_table.shape[1]} pages of {page_size} does not hold {longest} slots")
+    if not scale > 0:
+        raise KernelError(f"{what}: a scale above 0, not {scale}")
+    return pages, kv_heads, page_size, head_dim
+
+
+def _longest(what: str, longest: Optional[int], block_table, page_size: int, capacity: int) -> int:
+    holds = min(block_table.shape[-1] * page_size, capacity)
+    if longest is None:
+        return holds
+    if not 0 <= longest <= holds:
+        raise KernelError(f"{what}: block table and tally hold {holds} slots, not {longest}")
+    return longest
+
+
+def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, newest: torch.Tensor, tally: Tally, scale: float, *,
+                      longest: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per request: ``q`` [requests, >= heads * d] (bfloat16, a view of wider rows is fine, rows on 16-byte boundaries) over the ``lengths[r]`` (int32) slots of request
+    r's pages, the last of which is the new token's own.  ``cache``: dense bfloat16 [pages, 2, kv_heads, page, d]; ``block_table`` [requests, blocks] int32; ``scale`` above 0.  Returns [requests, heads * d].
+
+    What the token gives each slot, summed over the query heads of a key/value head, is added to ``tally`` [requests, kv_heads, capacity]; its own slot enters the tally with what it gives itself and
+    with the position ``newest[r]`` (int32).  A request of length 0 comes out as zeros and leaves its tally as it is.  A NaN or an infinity among the scores of a head makes that head's result and its key/value
+    head's weights NaN.
+
+    ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that long and is reported (``raise_on_status``).  Work is cut by the lengths as they are on the device, so
+    a captured call goes on with other lengths.  Slots beyond a length may hold anything.
+
+    A call's scratch memory is 4 * heads bytes per request and slot up to ``longest``, and 4 * heads * (d + 2) per request and block: up to 16 MB are kept per thread and stream, more is allocated for the call."""
+    what, requests = "attention_tallied", q.shape[0]
+    longest = _longest(what, longest, block_table, cache.shape[3] if cache.dim() == 5 else 0, tally.weights.shape[-1])
+    pages, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, block_table, requests, longest, scale)
+    capacity, width = _check_tally(tally, (requests, kv_heads), what), heads * head_dim
+    _check_vectors(what, lengths=(lengths, requests), newest=(newest, requests))
+    device = _check_device(what, q, cache, block_table, lengths, newest, tally.weights, tally.positions, out)
+    if out is None:
+        out = torch.empty(requests, width, dtype=torch.bfloat16, device=device)
+    elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != requests or out.shape[1] < width or out.stride(1) != 1:
+        raise KernelError(f"{what}: the output is a bfloat16 [{requests}, >= {width}] view")
+    if requests == 0:
+        return out
+    if longest == 0:
+        out[:, :width].zero_()
+        return out
+    stream, sms = stream_address(), sm_count(device)
+    size = entry("attention_tallied", "hb_attention_tallied_scratch", "iiiii", head_dim, result="l")(requests, longest, heads, kv_heads, sms)
+    memory, owner = scratch(device, stream, size)
+    check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim)(
+        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, tally.weights.data_ptr(),
+        tally.positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
+    return out
+
+
+def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, tally: Tally, scale: float, *, most: int,
+                  longest: Optional[int] = None) -> None:
+    """Add to ``tally`` [requests, kv_heads, capacity] what queries give the slots that they see, as :func:`attention_tallied` does for a decoded token, without a result: ``q`` [tokens, >= heads * d] (bfloat16, rows
+    on 16-byte boundaries), of which request r has the rows ``starts[r]`` to ``starts[r + 1] - 1`` (int32 [requests + 1]), a whole prompt or the last tokens of one.  They stand in the last of its
+    ``lengths[r]`` (int32) slots: query i of n sees the first ``lengths[r] - n + i + 1``, and one with nothing to see gives nothing.  Positions are not touched.
+
+    ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  What is beyond them is left out and reported (``raise_on_status``).  A NaN or an
+    infinity among the scores that a query sees makes the weights of those slots NaN.
+
+    A call's scratch memory is at least 8 * heads bytes per query, and where few queries look at many slots as much again for each cut of those."""
+    what, requests, tokens = "tally_queries", lengths.shape[0], q.shape[0]
+    longest = _longest(what, longest, block_table, cache.shape[3] if cache.dim() == 5 else 0, tally.weights.shape[-1])
+    pages, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, block_table, requests, longest, scale)
+    capacity = _check_tally(tally, (requests, kv_heads), what)
+    _check_vectors(what, lengths=(lengths, requests), starts=(starts, requests + 1))
+    if most < 0:
+        raise KernelError(f"{what}: most counts a request's queries")
+    device = _check_device(what, q, cache, block_table, starts, lengths, tally.weights, tally.positions)
+    most = min(most, tokens)
+    if requests == 0 or most == 0 or longest == 0:
+        return
+    stream, sms = stream_address(), sm_count(device)
+    size = entry("tally_queries", "hb_tally_queries_scratch", "iiiiiii", head_dim, result="l")(tokens, requests, most, longest, heads, kv_heads, sms)
+    memory, owner = scratch(device, stream, size)
+    check(entry("tally_queries", "hb_tally_queries", "plippippiiipiiiiifippp", head_dim)(
+        q.data_ptr(), q.stride(0), tokens, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], starts.data_ptr(), lengths.data_ptr(), requests, most, longest, tally.weights.data_ptr(), capacity,
+        heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
+
+
+def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, newest: torch.Tensor, tally: Tally, keep: int, *, first: int = 0, recent: int = 0, longest: Optional[int] = None,
+          out: Optional[Tally] = None) -> torch.Tensor:
+    """Cut requests of more than ``keep`` slots back to ``keep``, the same for every key/value head of every layer, and return the new lengths [requests] int32.  ``cache``: dense
+    [layers, pages, 2, kv_heads, page, d] with a ``tally`` [layers, requests, kv_heads, capacity], or both without the layers; any type, records of whole 16 bytes.  ``lengths`` and ``newest`` (the position of each
+    request's newest token): int32 [requests].
+
+    Slots whose positions are below ``first`` or among the last ``recent`` rank as an infinite weight, the others by their weights (a NaN as -infinity); of equal ranks the lowest slots stay.  What stays in slots
+    from ``keep`` on moves into those below that are left free, in order: keys and values, weights and positions.  Records from the new length on stay as they were, in the tally slots from there on weigh nothing
+    and have position -1.  The new tally goes to ``out`` where it is given, else in place.
+
+    Pages are written in place, so a request's pages may not be another one's as well (up to its length).  ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that
+    long and is reported (``raise_on_status``).  A move from or to a page that is not there is left out and reported.
+
+    A call's scratch memory is 8 bytes for each of the min(keep, longest - keep) moves that a head of a layer and request can have."""
+    what, requests = "evict", lengths.shape[0]
+    layered = cache.dim() == 6
+    if cache.dim() not in (5, 6) or cache.shape[-4] != 2 or not cache.is_contiguous():
+        raise KernelError(f"{what}: a dense cache [layers, pages, 2, kv_heads, page, d], or without the layers")
+    layers, (pages, _, kv_heads, page_size, head_dim) = cache.shape[0] if layered else 1, cache.shape[-5:]
+    record = head_dim * cache.element_size()
+    if page_size & (page_size - 1) or page_size == 0 or record == 0 or record % 16 or record > 65536:
+        raise KernelError(f"{what}: pages of a power of two and records of whole 16 bytes, not {page_size} and {record}")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] < requests or not block_table.is_contiguous():
+        raise KernelError(f"{what}: a dense int32 block table of at least {requests} rows")
+    shape = (layers, requests, kv_heads) if layered else (requests, kv_heads)
+    capacity = _check_tally(tally, shape, what)
+    to = tally if out is None else out
+    if _check_tally(to, shape, what) != capacity or (to.weights.data_ptr() == tally.weights.data_ptr()) != (to.positions.data_ptr() == tally.positions.data_ptr()):
+        raise KernelError(f"{what}: the new tally is as large as the old one, and all of it in its place or none")
+    _check_vectors(what, lengths=(lengths, requests), newest=(newest, requests))
+    if keep < 1 or first < 0 or recent < 0:
+        raise KernelError(f"{what}: keep at least 1, first and recent at least 0, not {keep}, {first} and {recent}")
+    longest = _longest(what, longest, block_table, page_size, capacity)
+    device = _check_device(what, cache, block_table, lengths, newest, *tally, *to)
+    left = torch.empty(requests, dtype=torch.int32, device=device)
+    if requests == 0 or layers == 0 or kv_heads == 0 or longest == 0:
+        return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
+    keep, first, recent = (min(value, 2**31 - 1) for value in (keep, first, recent))
+    stream = stream_address()
+    memory, owner = scratch(device, stream, entry("evict", "hb_evict_scratch", "iiiii", result="l")(layers, requests, kv_heads, longest, keep))
+    check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppp")(
+        cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, tally.weights.data_ptr(),
+        tally.positions.data_ptr(), to.weights.data_ptr(), to.positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), stream), what)
+    return left
