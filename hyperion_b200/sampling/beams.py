@@ -1,0 +1,68 @@
+"""Selection of a beam search's continuations over beams and vocabulary (csrc/beam_select.cu), and a slow host reference of the same rule for tests.
+
+A continuation of beam b by token v scores ``score_b + z_bv - log sum_u e^(z_bu)``, the sum of the log probabilities of its tokens; of equal scores the lowest (beam, token) comes first.
+:func:`..ops.beams.beam_reorder` lets the chosen beams go on from what their parents hold."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from ..ops.native import KernelError, check, entry, is_bf16, require_cuda, scratch, sm_count, stream_address
+
+MOST_BEAMS = 32
+MOST_TAKE = 64
+
+
+class BeamChoice(NamedTuple):
+    """Best first, [groups, take] each: the beam that a continuation comes from and its token (int32), and its score (float32)."""
+    parents: torch.Tensor
+    tokens: torch.Tensor
+    scores: torch.Tensor
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamChoice:
+    """The ``take`` best continuations of each group's beams (as many as it has beams, or twice that where some may end).  ``logits`` [groups * beams, vocab] float32 or bfloat16 with unit inner stride, a
+    row per beam; ``scores`` [groups, beams] float32, what the beams have scored so far.  At most 32 beams, ``take`` at most 64, at most 65,535 rows.
+
+    A logit of -infinity or NaN is no continuation (+infinity counts as the largest number), nor is anything of a beam whose score is -infinity or NaN: a group begins with one beam at 0 and the others at
+    -infinity.  Where there are fewer than ``take``, the places left have parent -1, token -1 and score -infinity."""
+    if scores.dtype is not torch.float32 or scores.dim() != 2 or not scores.is_contiguous() or not 1 <= scores.shape[1] <= MOST_BEAMS:
+        raise KernelError(f"beam_select: scores are dense float32 [groups, beams], 1 to {MOST_BEAMS} beams")
+    groups, beams = scores.shape
+    if logits.dim() != 2 or logits.shape[0] != groups * beams or logits.shape[1] < 1 or logits.stride(1) != 1 or (groups * beams > 1 and logits.stride(0) < logits.shape[1]):
+        raise KernelError(f"beam_select: logits [{groups * beams}, vocab] with unit inner stride, rows that do not overlap")
+    if not 1 <= take <= MOST_TAKE:
+        raise KernelError(f"beam_select: 1 to {MOST_TAKE} continuations, not {take}")
+    kind, device, vocab = is_bf16(logits), logits.device, logits.shape[1]
+    require_cuda(logits, scores)
+    if scores.device != device or device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"beam_select: logits and scores on the current CUDA device, not on {device} and {scores.device}")
+    parents, tokens = (torch.empty(groups, take, dtype=torch.int32, device=device) for _ in range(2))
+    found = torch.empty(groups, take, dtype=torch.float32, device=device)
+    if groups == 0:
+        return BeamChoice(parents, tokens, found)
+    stream, sms = stream_address(), sm_count(device)
+    memory, owner = scratch(device, stream, entry("beam_select", "hb_beam_select_scratch", "iiiii", result="l")(groups, beams, vocab, take, sms))
+    check(entry("beam_select", "hb_beam_select", "pilpiiiipppipp")(logits.data_ptr(), kind, max(logits.stride(0), vocab), scores.data_ptr(), groups, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(),
+                                                             found.data_ptr(), sms, memory, stream), "beam_select")
+    return BeamChoice(parents, tokens, found)
+
+
+def reference_beam_select(logits: np.ndarray, scores: np.ndarray, take: int) -> list[tuple[int, int, float]]:
+    """One group by the same rule in float64: (beam, token, score) of the best continuations, as many as there are."""
+    z = np.asarray(logits, dtype=np.float64).copy()
+    z[np.isnan(z)] = -np.inf
+    z = np.minimum(z, np.finfo(np.float32).max)
+    s = np.asarray(scores, dtype=np.float64).copy()
+    s[np.isnan(s)] = -np.inf
+    s = np.minimum(s, np.finfo(np.float32).max)
+    top = z.max(1, keepdims=True)
+    alive = np.isfinite(top) & np.isfinite(s)[:, None]
+    with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
+        total = np.exp(z - np.where(np.isfinite(top), top, 0.0)).sum(1, keepdims=True)
+        score = np.where(alive, z + (s[:, None] - (np.where(np.isfinite(top), top, 0.0) + np.log(np.maximum(total, np.finfo(np.float64).tiny)))), -np.inf)
+    flat = score.reshape(-1)
+    order = np.lexsort((np.arange(flat.size), -flat))[:take]
+    return [(int(i) // z.shape[1], int(i) % z.shape[1], float(flat[i])) for i in order if flat[i] > -np.inf]
