@@ -31,6 +31,7 @@ enum : int {
     HB_STATUS_IN_ATTENTION_STRIPS = 0x4000,
     HB_STATUS_IN_ATTENTION_SHARED = 0x8000,
     HB_STATUS_IN_ATTENTION_TALLIED = 0x10000,
+    HB_STATUS_IN_TALLY_QUERIES = 0x20000,
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }

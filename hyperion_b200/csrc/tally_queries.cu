@@ -5,44 +5,142 @@
 // v counts a request's (token, head) rows of a key/value head, token by token; token i of n sees the first length - n + i + 1 slots.  There is no result beside the weights, so values are not read.
 //
 // A weight is known only when its row's sum is, and a sum over rows has another owner than a row's, so the scores are made twice: the first walk goes along the slots and leaves m and 1 / l of every row,
-// the second goes along the rows and adds up every slot's weights.  (Keeping them would move 8 bytes a score, against 2 d operations for making them again.)  Both walks have one shape: a tile of 64 rows
-// (of Q; then of K) stays in registers as the products' operand of 16 rows a warp, tiles of the others pass through shared memory, two at a time.  Sums over what passes end up in one lane's hands, and
-// nothing is added by atomics, so results do not depend on which block came first.
+// the second goes along the rows and adds up every slot's weights.  (Keeping them would move 8 bytes a score, against 2 d operations for making them again.)
 //
-// Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.
+// Both walks have one shape: a tile of 128 rows stays in shared memory (of Q; then of K), tiles of the other pass through a ring, and each pair is one product of 128 x 128 on the tensor cores (tcgen05) into
+// one of two buffers of tensor memory.  The rows that stay are the product's lanes and what passes its columns, so one thread owns a row's maximum and sum, or a slot's sum, and nothing is exchanged.
+// A tile of Q has whole tokens: 128 / group of them with all heads of a key/value head, by one TMA box a panel.
 //
-// Slots beyond a request's length may hold anything: they are read as zeros and their scores are not looked at.
+// Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.  Nothing is added by atomics, so results
+// do not depend on which block came first.
+//
+// Slots beyond a request's length may hold anything: their scores are not looked at.  Every wait is bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the block leaves, once the copies and products that it
+// has on their way are done.
+#include <cuda.h>
+
 #include "common.cuh"
 
 #ifndef HB_HEAD_DIM
 #define HB_HEAD_DIM 128
+#endif
+#ifndef HB_WAIT_LIMIT
+#define HB_WAIT_LIMIT (1u << 24)
 #endif
 
 namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int D = HB_HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
-constexpr int ROWS = 64, WARPS = 4, THREADS = 32 * WARPS, TILE = ROWS * D * 2, CHUNKS = D / 8;
+constexpr int BM = 128;                        // rows that stay, and rows that pass
+constexpr int PANEL = BM * 128, PANELS = D / 64, TILE = PANELS * PANEL;  // bytes
+constexpr int STAGES = D == 128 ? 2 : 4;       // of the ring: two blocks share an SM's memory
+constexpr int EPILOGUE = 4, PRODUCER = 4, ISSUER = 5, THREADS = 32 * 6;
+constexpr int TMEM_COLS = 2 * BM;              // two blocks have all of an SM's
+constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
+constexpr size_t SMEM_BYTES = 1024 + (size_t)TILE * (1 + STAGES) + 2 * 2 * BM * 4 + 128;
+static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "an SM's shared memory");
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void ldmatrix_x4(unsigned (&r)[4], unsigned at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+__device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
 }
-__device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_over(unsigned long long* bar, unsigned parity) {
+    unsigned done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity, volatile int* failed) {
+    for (unsigned spin = 0; spin < WAIT_LIMIT; ++spin) {
+        if (mbar_over(bar, parity)) return true;
+        if ((spin & 1023) == 1023 && *failed) return false;
+    }
+    return false;
+}
+// Before a block leaves: what it has set going is done, whatever has become of its other waits.
+__device__ __forceinline__ void mbar_last_wait(unsigned long long* bar, unsigned parity) {
+    for (unsigned spin = 0; spin < LAST_WAIT_LIMIT; ++spin)
+        if (mbar_over(bar, parity)) return;
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+constexpr unsigned DESC_HIGH = (unsigned)(1024 >> 4) | (1u << 14) | (2u << 29);  // 8-row groups 1,024 bytes apart, sm_100 descriptor, 128-byte swizzle
+constexpr unsigned IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(BM >> 3) << 17) | ((unsigned)(BM >> 4) << 24);  // float from bfloat16, both K-major, 128 x 128
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ unsigned low_k_major(const void* tile) { return ((smem_u32(tile) & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ void umma_commit_at(unsigned bar_addr) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr) : "memory");
+}
+__device__ __forceinline__ bool elected() {  // one lane of the warp, all of which are here
+    unsigned one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+// The product of a 64-entry panel of both tiles (4 of 16 entries); `first` = 0 starts a new one.
+__device__ __forceinline__ void umma_s_panel(unsigned tmem_d, unsigned a_low, unsigned b_low, unsigned idesc, unsigned first) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 al, bl;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
+        "add.u32 al, %1, 2;\n\t"
+        "add.u32 bl, %2, 2;\n\t"
+        "mov.b64 da, {al, %5};\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t"
+        "add.u32 al, %1, 4;\n\t"
+        "add.u32 bl, %2, 4;\n\t"
+        "mov.b64 da, {al, %5};\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t"
+        "add.u32 al, %1, 6;\n\t"
+        "add.u32 bl, %2, 6;\n\t"
+        "mov.b64 da, {al, %5};\n\t"
+        "mov.b64 db, {bl, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t}"
+        ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(first), "r"(DESC_HIGH) : "memory");
+}
+// 32 consecutive columns of this thread's lane, on their way; arrived() says that they are there, and nothing that reads them can stand before it.
+__device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void arrived(unsigned (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 16-byte chunk c of row r of a tile: rows of 128 bytes in panels, their chunks permuted so that eight rows of one column meet eight banks.
-__device__ __forceinline__ unsigned tile_at(int r, int c) { return (unsigned)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over a NaN, as fmaxf does
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 struct Args {
-    const bf16* q; int q_stride;
-    const bf16* cache;
     const int* block_table; int table_width;
     const int* starts;    // [requests + 1]
     const int* lengths;   // [requests]
@@ -52,7 +150,8 @@ struct Args {
     float2* rows;         // [tokens * heads]: (m, 1 / l)
     float2* cuts;         // [n_cuts, tokens * heads]: (m, l), where the slots are cut
     int n_cuts;
-    int heads, kv_heads, page_shift, pages;
+    int heads, kv_heads, group, page_shift, pages;
+    int per_tile;         // tokens of a tile of Q
     float scale_log2;
     int* status;
 };
@@ -65,128 +164,253 @@ __device__ __forceinline__ Request request_of(const Args& a, int r, bool reports
     first = min(max(first, 0), a.tokens), tokens = min(min(max(tokens, 0), a.most), a.tokens - first), length = min(max(length, 0), a.longest);
     return {first, tokens, length};
 }
+__device__ __forceinline__ float2 as_factor(float m, float l) { return make_float2(m == -INFINITY ? 0.f : m, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)); }
 
-// Rows row0 .. row0 + 63 of a request's queries, or slots slot0 .. of its keys, on their way into a tile; zeros beyond their end.
-__device__ __forceinline__ void copy_chunk(unsigned dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void fetch_queries(const Args& a, const Request& q, int kvh, int group, int row0, unsigned tile) {
-    for (int i = threadIdx.x; i < ROWS * CHUNKS; i += THREADS) {
-        const int r = i / CHUNKS, c = i % CHUNKS, v = row0 + r, token = v / group;
-        const bool valid = token < q.tokens;
-        copy_chunk(tile + tile_at(r, c), valid ? a.q + (size_t)(q.first + token) * a.q_stride + (size_t)(kvh * group + v - token * group) * D + c * 8 : a.q, valid);
+// One walk.  KEYS_STAY: block (tile of slots, key/value head, request), tiles of Q pass; else block (cut, tile of Q and key/value head, request), tiles of K pass.
+template <bool KEYS_STAY>
+__global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* stays = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* ring = stays + TILE;
+    float* tops = reinterpret_cast<float*>(ring + STAGES * TILE);  // KEYS_STAY: [2][BM], m of the passing rows
+    float* shares = tops + 2 * BM;                                  // [2][BM], their 1 / l
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(shares + 2 * BM);
+    unsigned long long* empty = full + STAGES;
+    unsigned long long* s_full = empty + STAGES;  // [2]
+    unsigned long long* s_empty = s_full + 2;     // [2]
+    unsigned long long* stays_full = s_empty + 2;
+    unsigned long long* all_done = stays_full + 1;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(all_done + 1);
+    volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, request = blockIdx.z;
+    wait_for_previous_kernels();
+    const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.y % a.kv_heads, group = a.group;
+    const Request r = request_of(a, request, !KEYS_STAY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
+    const int before = r.length - r.tokens;  // token i sees before + i + 1 slots
+    const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile, base = KEYS_STAY ? blockIdx.x * BM : (int)(gridDim.y / a.kv_heads - 1 - blockIdx.y / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
+    int from, to;  // tiles that pass
+    if (KEYS_STAY) {
+        if (base >= r.length || r.tokens == 0) return;
+        from = max(0, base - before) / a.per_tile, to = q_tiles;  // token base - before is the first that sees slot base
+        if (from >= to) return;
+    } else {
+        if (base >= r.tokens) return;
+        const int reach = min(r.length, max(0, before + min(base + a.per_tile, r.tokens))), n = (reach + BM - 1) / BM;  // slots that any of the tokens sees
+        from = (int)((long long)n * blockIdx.x / a.n_cuts), to = (int)((long long)n * (blockIdx.x + 1) / a.n_cuts);
     }
-}
-__device__ __forceinline__ void fetch_keys(const Args& a, int request, int length, int kvh, int slot0, unsigned tile) {
-    for (int i = threadIdx.x; i < ROWS * CHUNKS; i += THREADS) {
-        const int r = i / CHUNKS, c = i % CHUNKS, slot = slot0 + r;
-        int page = -1;
-        if (slot < length) {
-            page = __ldg(a.block_table + (size_t)request * a.table_width + (slot >> a.page_shift));
-            if (page < 0 || page >= a.pages) {
-                atomicOr(a.status, HB_STATUS_BAD_PAGE);
-                page = -1;
+    const int n_tiles = to - from;
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], EPILOGUE); }
+        mbar_init(stays_full, 1), mbar_init(all_done, 1);
+        *failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+    }
+    // rows of Q's tiles that no copy writes (beyond whole tokens)
+    const int q_rows = a.per_tile * group;
+    for (int e = tid; e < (BM - q_rows) * 8 * PANELS * (KEYS_STAY ? STAGES : 1); e += THREADS) {
+        const int chunk = e & 7, row = q_rows + (e >> 3) % (BM - q_rows), panel = (e >> 3) / (BM - q_rows);
+        reinterpret_cast<uint4*>((KEYS_STAY ? ring : stays) + panel * PANEL + row * 128)[chunk] = make_uint4(0, 0, 0, 0);
+    }
+    // Tensor memory is taken only now that the kernels before have finished, and the next kernel is let in only once it is: a block further back or further on that holds some while it waits could wait for this one.
+    if (warp == ISSUER) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    let_next_kernel_start();
+    tc_fence_after();
+    const unsigned tmem = *tmem_slot;
+
+    if (warp == PRODUCER) {
+        // ------------------------------------------------------------------ the whole warp
+        const int page_size = 1 << a.page_shift, pages_per_tile = BM >> a.page_shift;
+        const int* table = a.block_table + (size_t)request * a.table_width;
+        auto page_at = [&](int slot0) {  // this lane's page of the tile of K from slot0 on; -1: none
+            const int k0 = slot0 + lane * page_size;
+            if (lane >= pages_per_tile || k0 >= r.length) return -1;
+            const int id = __ldg(table + (k0 >> a.page_shift));
+            if (id >= 0 && id < a.pages) return id;
+            atomicOr(a.status, HB_STATUS_BAD_PAGE);
+            return -1;
+        };
+        auto fetch_keys = [&](unsigned char* tile, int page, unsigned long long* bar) {
+            const unsigned valid = __popc(__ballot_sync(0xffffffffu, page >= 0));
+            if (lane == 0) {
+                if (valid) mbar_expect_tx(bar, valid * page_size * D * 2u); else mbar_arrive(bar);
+            }
+            __syncwarp();
+            const int ops = pages_per_tile * PANELS;  // at most 32
+            const int p = min(lane, ops - 1) / PANELS, h = lane % PANELS, id = __shfl_sync(0xffffffffu, page, p);
+            if (lane < ops && id >= 0) tma_load_2d(tile + h * PANEL + p * page_size * 128, &kv_map, bar, h * 64, (id * 2 * a.kv_heads + kvh) << a.page_shift);
+        };
+        auto fetch_queries = [&](unsigned char* tile, int token, unsigned long long* bar) {  // tokens beyond the request's own come along, or are filled with zeros
+            if (lane == 0) {
+                mbar_expect_tx(bar, (unsigned)(PANELS * 128 * q_rows));
+                for (int h = 0; h < PANELS; ++h) tma_load_3d(tile + h * PANEL, &q_map, bar, h * 64, kvh * group, r.first + token);
+            }
+        };
+        int sent = 0;
+        if (n_tiles > 0) {
+            if (KEYS_STAY) fetch_keys(stays, page_at(base), stays_full); else fetch_queries(stays, base, stays_full);
+            int page = KEYS_STAY ? 0 : page_at(from * BM);
+            for (int i = 0; i < n_tiles; ++i, ++sent) {
+                const int s = i % STAGES;
+                if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / STAGES) & 1) ^ 1, failed))) { *failed = 1; break; }
+                if (KEYS_STAY) {
+                    fetch_queries(ring + s * TILE, (from + i) * a.per_tile, &full[s]);
+                } else {
+                    fetch_keys(ring + s * TILE, page, &full[s]);
+                    page = i + 1 < n_tiles ? page_at((from + i + 1) * BM) : -1;
+                }
+            }
+            if (lane == 0) {
+                mbar_last_wait(stays_full, 0);
+                for (int k = max(0, sent - STAGES); k < sent; ++k) mbar_last_wait(&full[k % STAGES], (k / STAGES) & 1);
+            }
+            __syncwarp();
+        }
+    } else if (warp == ISSUER) {
+        // ------------------------------------------------------------------ the warp stays together, so that descriptors are its common values; one elected lane issues
+        const unsigned a_low = low_k_major(stays), b_low0 = low_k_major(ring);
+        auto wait_for = [&](unsigned long long* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, failed)) != 0; };
+        bool ok = n_tiles == 0 || wait_for(stays_full, 0);
+        for (int i = 0; i < n_tiles && ok; ++i) {
+            const int s = i % STAGES, b = i & 1;
+            ok = wait_for(&full[s], i / STAGES) && wait_for(&s_empty[b], (i >> 1) ^ 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elected()) {
+                const unsigned b_low = b_low0 + (unsigned)s * (TILE >> 4);
+#pragma unroll
+                for (int h = 0; h < PANELS; ++h) umma_s_panel(tmem + b * BM, a_low + h * (PANEL >> 4), b_low + h * (PANEL >> 4), IDESC, h ? 1u : 0u);
+                umma_commit_at(smem_u32(&empty[s]));
+                umma_commit_at(smem_u32(&s_full[b]));
+            }
+            __syncwarp();
+        }
+        if (!ok) *failed = 1;
+        if (elected()) umma_commit_at(smem_u32(all_done));
+        __syncwarp();
+        mbar_last_wait(all_done, 0);
+    } else {
+        // ------------------------------------------------------------------ four warps: a thread has a lane of the product
+        const int mine = warp * 32 + lane;
+        const unsigned lanes = tmem + ((unsigned)(warp * 32) << 16);
+        const float c = a.scale_log2;
+        bool ok = true;
+        [[maybe_unused]] float m = -INFINITY, l = 0.f;         // of this thread's row
+        [[maybe_unused]] float sum = 0.f, rest = 0.f;          // of this thread's slot, and what its additions lost
+        [[maybe_unused]] const int token = base + mine / group;
+        [[maybe_unused]] const int sees = token < r.tokens && mine < q_rows ? min(r.length, before + token + 1) : 0;
+        [[maybe_unused]] const int all_see = min(r.length, before + base + 1);  // slots that every row of the tile sees
+        auto factor_of = [&](int tile) {  // of row `mine` of a tile of Q
+            const int t = tile * a.per_tile + mine / group;
+            return tile < to && mine < q_rows && t < r.tokens ? a.rows[(size_t)(r.first + t) * a.heads + kvh * group + mine % group] : make_float2(0.f, 0.f);
+        };
+        float2 factor;
+        if (KEYS_STAY) factor = factor_of(from);
+        for (int i = 0; i < n_tiles; ++i) {
+            const int b = i & 1;
+            if constexpr (KEYS_STAY) {
+                tops[b * BM + mine] = factor.x, shares[b * BM + mine] = factor.y;
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * EPILOGUE) : "memory");  // whoever still reads the other buffer has this one's turn before it is written again
+                factor = factor_of(from + i + 1);
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[b], (i >> 1) & 1, failed))) {
+                *failed = 1, ok = false;
+                if (KEYS_STAY) continue;  // to meet the others at the barrier above
+                break;
+            }
+            tc_fence_after();
+            unsigned raw[4][32];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tmem_ld32(lanes + b * BM + 32 * k, raw[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) arrived(raw[k]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[b]);
+            auto s_at = [&](int j) -> float { return __uint_as_float(raw[j >> 5][j & 31]); };
+            if constexpr (KEYS_STAY) {
+                const int token0 = (from + i) * a.per_tile;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const float* top = tops + b * BM;
+                const float* share = shares + b * BM;
+                const int from_row = (base + mine - before - token0) * group, rows = (r.tokens - token0) * group;  // rows that see this slot, and rows of the request
+                const bool all = (base + BM - 1 - before - token0) <= 0 && r.tokens - token0 >= a.per_tile;
+                if (all) {
+#pragma unroll
+                    for (int j = 0; j < BM; j += 4) {
+                        float mm[4], ss[4];
+                        load4(top + j, mm), load4(share + j, ss);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) part[e] = fmaf(fast_exp2(fmaf(s_at(j + e), c, -mm[e])), ss[e], part[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < BM; j += 4) {
+                        float mm[4], ss[4];
+                        load4(top + j, mm), load4(share + j, ss);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float p = fast_exp2(fmaf(s_at(j + e), c, -mm[e])) * ss[e];
+                            if (j + e >= from_row && j + e < rows && j + e < q_rows) part[e] += p;
+                        }
+                    }
+                }
+                // added up with what is lost: a slot that thousands of rows see would be off by more than all else
+                const float y = (part[0] + part[1]) + (part[2] + part[3]) - rest, t = sum + y;
+                rest = (t - sum) - y, sum = t;
+            } else {
+                const int slot0 = (from + i) * BM;
+                if (slot0 + BM > all_see) {
+#pragma unroll
+                    for (int j = 0; j < BM; ++j)
+                        if (slot0 + j >= sees) raw[j >> 5][j & 31] = 0xff800000u;
+                }
+                float top[4] = {m, m, m, m};
+#pragma unroll
+                for (int j = 0; j < BM; j += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // c is above 0: the largest score is the largest product
+                        top[e] = max3(top[e], s_at(j + e) * c, s_at(j + e + 4) * c);
+                    }
+                const float above = fmaxf(max3(top[0], top[1], top[2]), top[3]), low = above == -INFINITY ? 0.f : above;
+                l *= m == -INFINITY ? 1.f : fast_exp2(m - low);  // nothing but zeros and NaN has been added up below -infinity
+                m = above;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < BM; j += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) part[e] += fast_exp2(fmaf(s_at(j + e), c, -low));
+                l += (part[0] + part[1]) + (part[2] + part[3]);
             }
         }
-        const size_t row = (((size_t)(page < 0 ? 0 : page) * 2 * a.kv_heads + kvh) << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
-        copy_chunk(tile + tile_at(r, c), page < 0 ? a.cache : a.cache + row * D + c * 8, page >= 0);
-    }
-}
-__device__ __forceinline__ void committed() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// This warp's 16 rows of the tile that stays.
-__device__ __forceinline__ void load_staying(unsigned (&x)[D / 16][4], unsigned tile) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) ldmatrix_x4(x[k], tile + tile_at(warp * 16 + (lane & 15), 2 * k + (lane >> 4)));
-}
-// The scores of this warp's 16 rows and the 64 of the passing tile: [8 of them][(row g or g + 8, row 2 t or 2 t + 1 of the 8)].
-__device__ __forceinline__ void products(float (&s)[8][4], const unsigned (&x)[D / 16][4], unsigned tile) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int n = 0; n < 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            unsigned b[4];
-            ldmatrix_x4(b, tile + tile_at(n * 8 + (lane & 7), 4 * k + (lane >> 3)));
-            mma(s[n], x[2 * k], b[0], b[1]);
-            mma(s[n], x[2 * k + 1], b[2], b[3]);
+        if constexpr (KEYS_STAY) {
+            if (base + mine < r.length && ok) a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + base + mine] += sum;
+        } else if (mine < q_rows && token < r.tokens && ok) {
+            const size_t at = (size_t)(r.first + token) * a.heads + kvh * group + mine % group;
+            if (a.n_cuts == 1) a.rows[at] = as_factor(m, l);
+            else a.cuts[(size_t)blockIdx.x * a.tokens * a.heads + at] = make_float2(m, l);
         }
-}
-
-// The first walk: block (cut, row tile and key/value head, request).
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    const unsigned tiles = smem_u32(smem);
-    let_next_kernel_start();
-    wait_for_previous_kernels();
-    const int kvh = blockIdx.y % a.kv_heads, row0 = blockIdx.y / a.kv_heads * ROWS, group = a.heads / a.kv_heads;
-    const Request r = request_of(a, blockIdx.z, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
-    const int n_rows = r.tokens * group;
-    if (row0 >= n_rows) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, before = r.length - r.tokens;  // row v sees before + v / group + 1 slots
-    const int reach = min(r.length, max(0, before + min(row0 + ROWS - 1, n_rows - 1) / group + 1));  // slots that any of the rows sees
-    const int n_tiles = (reach + ROWS - 1) / ROWS, from = (int)((long long)n_tiles * blockIdx.x / a.n_cuts), to = (int)((long long)n_tiles * (blockIdx.x + 1) / a.n_cuts);
-    unsigned x[D / 16][4];
-    fetch_queries(a, r, kvh, group, row0, tiles);
-    committed();
-    arrived<0>();
+    }
+    tc_fence_before();
     __syncthreads();
-    load_staying(x, tiles);
-    __syncthreads();
-    int sees[2];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) sees[h] = min(r.length, before + (row0 + warp * 16 + h * 8 + g) / group + 1);
-    if (from < to) fetch_keys(a, blockIdx.z, r.length, kvh, from * ROWS, tiles);
-    committed();
-    for (int i = from; i < to; ++i) {
-        const unsigned tile = tiles + ((i - from) & 1) * TILE;
-        if (i + 1 < to) fetch_keys(a, blockIdx.z, r.length, kvh, (i + 1) * ROWS, tiles + ((i - from + 1) & 1) * TILE);
-        committed();
-        arrived<1>();
-        __syncthreads();
-        float s[8][4];
-        products(s, x, tile);
-        __syncthreads();  // the tile is free
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float top = m[h];
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& y = s[n][2 * h + e];
-                    y = i * ROWS + n * 8 + 2 * t + e < sees[h] ? y * a.scale_log2 : -INFINITY;
-                    top = fmaxf(top, y);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float base = top == -INFINITY ? 0.f : top;
-            l[h] *= m[h] == -INFINITY ? 1.f : fast_exp2(m[h] - base);  // nothing but zeros and NaN has been added up below -infinity
-            m[h] = top;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) l[h] += fast_exp2(s[n][2 * h] - base) + fast_exp2(s[n][2 * h + 1] - base);
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        const int v = row0 + warp * 16 + h * 8 + g;
-        if (t == 0 && v < n_rows) {
-            const size_t at = (size_t)(r.first + v / group) * a.heads + kvh * group + v % group;
-            if (a.n_cuts == 1) a.rows[at] = make_float2(m[h] == -INFINITY ? 0.f : m[h], l[h] > 0.f ? 1.f / l[h] : (l[h] == 0.f ? 0.f : l[h]));
-            else a.cuts[(size_t)blockIdx.x * a.tokens * a.heads + at] = make_float2(m[h], l[h]);
-        }
+    if (tid == 0 && *failed) atomicOr(a.status, HB_STATUS_WAIT_EXPIRED | HB_STATUS_IN_TALLY_QUERIES);
+    if (warp == ISSUER) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
 }
 
-__global__ void __launch_bounds__(256) cuts_kernel(const Args a) {
+__global__ void __launch_bounds__(256) tally_cuts_kernel(const Args a) {
     let_next_kernel_start();
     wait_for_previous_kernels();
     const int n = a.tokens * a.heads, at = blockIdx.x * 256 + threadIdx.x;
@@ -197,83 +421,44 @@ __global__ void __launch_bounds__(256) cuts_kernel(const Args a) {
         const float2 ml = a.cuts[(size_t)c * n + at];
         all = fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top), ml.y, all);
     }
-    a.rows[at] = make_float2(top == -INFINITY ? 0.f : top, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
+    a.rows[at] = as_factor(top, all);
 }
 
-// The second walk: block (tile of slots, key/value head, request).
-__global__ void __launch_bounds__(THREADS) slots_kernel(const Args a) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    float2* sums = reinterpret_cast<float2*>(smem + 2 * TILE);  // [2][ROWS]
-    const unsigned tiles = smem_u32(smem);
-    let_next_kernel_start();
-    wait_for_previous_kernels();
-    const int kvh = blockIdx.y, slot0 = blockIdx.x * ROWS, group = a.heads / a.kv_heads;
-    const Request r = request_of(a, blockIdx.z, false);
-    const int n_rows = r.tokens * group;
-    if (slot0 >= r.length || n_rows == 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, before = r.length - r.tokens;
-    const int from = max(0, slot0 - before) * group / ROWS, to = (n_rows + ROWS - 1) / ROWS;  // token slot0 - before is the first that sees slot slot0
-    auto fetch = [&](int i) {
-        const int buffer = (i - from) & 1;
-        fetch_queries(a, r, kvh, group, i * ROWS, tiles + buffer * TILE);
-        if (threadIdx.x < ROWS) {
-            const int v = min(i * ROWS + (int)threadIdx.x, n_rows - 1);
-            const float2* src = a.rows + (size_t)(r.first + v / group) * a.heads + kvh * group + v % group;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(sums + buffer * ROWS + threadIdx.x)), "l"(src) : "memory");
-        }
-        committed();
-    };
-    unsigned x[D / 16][4];
-    fetch_keys(a, blockIdx.z, r.length, kvh, slot0, tiles);
-    committed();
-    arrived<0>();
-    __syncthreads();
-    load_staying(x, tiles);
-    __syncthreads();
-    float sum[2] = {0.f, 0.f};
-    fetch(from);
-    for (int i = from; i < to; ++i) {
-        const int buffer = (i - from) & 1;
-        if (i + 1 < to) fetch(i + 1);
-        else committed();
-        arrived<1>();
-        __syncthreads();
-        float s[8][4];
-        products(s, x, tiles + buffer * TILE);
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int v = i * ROWS + n * 8 + 2 * t + e, token = v / group;
-                const float2 ml = sums[buffer * ROWS + n * 8 + 2 * t + e];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bool sees = token < r.tokens && slot0 + warp * 16 + h * 8 + g <= before + token;
-                    const float p = fast_exp2(s[n][2 * h + e] * a.scale_log2 - ml.x) * ml.y;
-                    if (sees) sum[h] += p;
-                }
-            }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        const int slot = slot0 + warp * 16 + h * 8 + g;
-        if (t == 0 && slot < r.length) a.weights[((size_t)blockIdx.z * a.kv_heads + kvh) * a.capacity + slot] += sum[h];
-    }
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* found = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &found, cudaEnableDefault, &result) == cudaSuccess && result == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiled>(found) : nullptr;
+    }();
+    return fn;
+}
+int encoded(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return HB_BAD_ARGUMENT;
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
+}
+template <bool KEYS_STAY>
+int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const Args& a, dim3 grid, cudaStream_t stream) {
+    const cudaError_t configured = cudaFuncSetAttribute(tally_walk_kernel<KEYS_STAY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+    if (configured != cudaSuccess) return (int)configured;
+    return launch_after_previous(tally_walk_kernel<KEYS_STAY>, grid, dim3(THREADS), SMEM_BYTES, stream, kv_map, q_map, a);
 }
 }  // namespace
 
-// Into how many cuts the first walk's slots go: as many as fill the device four times over, of four tiles at least.
+// Into how many cuts the first walk's slots go: as many as give the device two blocks an SM, of a tile at least.
 static int cuts_for(int requests, int most, int longest, int heads, int kv_heads, int sms) {
-    const long long rows = (long long)most * (heads / kv_heads), blocks = (rows + ROWS - 1) / ROWS * kv_heads * requests;
-    const long long wanted = 4LL * sms / (blocks ? blocks : 1), most_cuts = (longest + 4 * ROWS - 1) / (4 * ROWS);
+    const int per_tile = BM / (heads / kv_heads);
+    const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = (longest + BM - 1) / BM;
     return (int)(wanted < 1 ? 1 : wanted < most_cuts ? wanted : most_cuts);
 }
 // Bytes of scratch that hb_tally_queries takes.
 HB_EXPORT long long hb_tally_queries_scratch(int tokens, int requests, int most, int longest, int heads, int kv_heads, int sms) {
-    if (tokens <= 0 || requests <= 0 || most <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || sms <= 0) return 0;
+    if (tokens <= 0 || requests <= 0 || most <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > BM || sms <= 0) return 0;
     const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
     return 8LL * tokens * heads * (cuts > 1 ? cuts + 1 : 1);
 }
@@ -284,18 +469,27 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     if (requests <= 0 || tokens <= 0) return 0;
     if (!q || !cache || !block_table || !starts || !lengths || !weights || !scratch || !status) return HB_BAD_ARGUMENT;
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || most <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
-    if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
+    if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1)) || heads / kv_heads > BM) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)scratch & 7) || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
-    const int group = heads / kv_heads;
-    if (q_stride > 0x7fffffffLL || (long long)tokens * heads > 0x7fffffffLL - 256 || longest > 0x7fffffff - ROWS || requests > 65535 || kv_heads > 65535) return HB_UNSUPPORTED_SIZE;
-    const long long row_blocks = ((long long)most * group + ROWS - 1) / ROWS * kv_heads;
+    const int group = heads / kv_heads, per_tile = BM / group;
+    if (q_stride > 0x7fffffffLL || (long long)tokens * heads > 0x7fffffffLL - 256 || longest > 0x7fffffff - BM || requests > 65535 || kv_heads > 65535) return HB_UNSUPPORTED_SIZE;
+    if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
+    const long long row_blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads;
     if (row_blocks > 65535) return HB_UNSUPPORTED_SIZE;
-    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), page_shift = __builtin_ctz(page_size);
+    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
+    CUtensorMap kv_map, q_map;
+    const cuuint64_t kv_dims[2] = {(cuuint64_t)D, (cuuint64_t)pages * 2 * kv_heads * page_size}, kv_strides[1] = {(cuuint64_t)D * 2};
+    const cuuint32_t kv_box[2] = {64, (cuuint32_t)page_size};
+    if (int code = encoded(&kv_map, cache, 2, kv_dims, kv_strides, kv_box)) return code;
+    // a single row has no stride of its own
+    const cuuint64_t q_dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens}, q_strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)(tokens > 1 ? q_stride : (long long)heads * D) * 2};
+    const cuuint32_t q_box[3] = {64, (cuuint32_t)group, (cuuint32_t)per_tile};
+    if (int code = encoded(&q_map, q, 3, q_dims, q_strides, q_box)) return code;
     float2* rows = (float2*)scratch;
-    const Args a{(const bf16*)q, (int)q_stride, (const bf16*)cache, block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, rows + (size_t)tokens * heads, cuts,
-                 heads, kv_heads, page_shift, pages, scale * 1.4426950408889634f, status};
-    if (int code = launch_after_previous(rows_kernel, dim3(cuts, (unsigned)row_blocks, requests), dim3(THREADS), 2 * TILE, stream, a)) return code;
+    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, rows + (size_t)tokens * heads, cuts, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
+                 scale * 1.4426950408889634f, status};
+    if (int code = launch_walk<false>(kv_map, q_map, a, dim3(cuts, (unsigned)row_blocks, requests), stream)) return code;
     if (cuts > 1)
-        if (int code = launch_after_previous(cuts_kernel, dim3((tokens * heads + 255) / 256), dim3(256), 0, stream, a)) return code;
-    return launch_after_previous(slots_kernel, dim3((longest + ROWS - 1) / ROWS, kv_heads, requests), dim3(THREADS), 2 * TILE + 2 * ROWS * 8, stream, a);
+        if (int code = launch_after_previous(tally_cuts_kernel, dim3((tokens * heads + 255) / 256), dim3(256), 0, stream, a)) return code;
+    return launch_walk<true>(kv_map, q_map, a, dim3((longest + BM - 1) / BM, kv_heads, requests), stream);
 }

@@ -13,7 +13,7 @@ STATUS_BITS = {1: "a block-table entry that had to be valid was missing", 2: "a 
                0x100: "(in the tile-shaped GEMM)", 0x200: "(in the swapped GEMM)", 0x400: "(in the TMA attention, tile shape)",
                0x800: "(in the TMA attention, token shape)", 0x1000: "(in the tcgen05 attention)", 0x2000: "(in the walk through chunks)",
                0x4000: "(in the attention behind shared positions, strips)", 0x8000: "(in the attention behind shared positions, tiles)",
-               0x10000: "(in the attention whose weights are kept)"}
+               0x10000: "(in the attention whose weights are kept)", 0x20000: "(in the weights of many queries)"}
 
 
 def status_word(device: torch.device) -> torch.Tensor:

@@ -139,6 +139,8 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     _check_vectors(what, lengths=(lengths, requests), starts=(starts, requests + 1))
     if most < 0:
         raise KernelError(f"{what}: most counts a request's queries")
+    if heads // kv_heads > 128:
+        raise KernelError(f"{what}: at most 128 heads a key/value head, not {heads // kv_heads}")
     device = _check_device(what, q, cache, block_table, starts, lengths, tally.weights, tally.positions)
     most = min(most, tokens)
     if requests == 0 or most == 0 or longest == 0:
