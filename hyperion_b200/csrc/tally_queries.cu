@@ -9,6 +9,8 @@
 //
 // Both walks have one shape: a tile of 128 rows stays in shared memory (of Q; then of K), tiles of the other pass through a ring, and each pair is one product of 128 x 128 on the tensor cores (tcgen05) into
 // one of two buffers of tensor memory.  The rows that stay are the product's lanes and what passes its columns, so one thread owns a row's maximum and sum, or a slot's sum, and nothing is exchanged.
+// In the second walk a row's maximum and sum are part of the product: 16 more columns stand beside both tiles, 1 1 1 0 ... beside a slot and -(m + log2 l) / (scale log2 e) in three parts of bfloat16 beside a row,
+// so that a thread takes 2^(c s) of what the product gives and adds it up.  (Read out of shared memory by all threads of a warp they cost as much of its bandwidth as the products' operands: 104 us where this takes XX.)
 // A tile of Q has whole tokens: 128 / group of them with all heads of a key/value head, by one TMA box a panel.
 //
 // Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.  Nothing is added by atomics, so results
@@ -34,10 +36,12 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int BM = 128;                        // rows that stay, and rows that pass
 constexpr int PANEL = BM * 128, PANELS = D / 64, TILE = PANELS * PANEL;  // bytes
 constexpr int STAGES = D == 128 ? 2 : 4;       // of the ring: two blocks share an SM's memory
-constexpr int EPILOGUE = 4, PRODUCER = 4, ISSUER = 5, THREADS = 32 * 6;
+constexpr int SPAN = 16;                       // tiles of Q that pass one block
+constexpr int HALF = 4, PRODUCER = 2 * HALF, ISSUER = PRODUCER + 1, THREADS = 32 * (ISSUER + 1);  // warps that look at scores: four for each of the two buffers
 constexpr int TMEM_COLS = 2 * BM;              // two blocks have all of an SM's
 constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
-constexpr size_t SMEM_BYTES = 1024 + (size_t)TILE * (1 + STAGES) + 2 * 2 * BM * 4 + 128;
+constexpr int BESIDE = 2 * BM * 16;            // bytes of a tile's 16 more columns: two groups of 8, rows of 16 bytes one behind the other (no swizzle)
+constexpr size_t SMEM_BYTES = 1024 + (size_t)(TILE + BESIDE) * (1 + STAGES) + 2 * BM * 4 + 128;
 static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "an SM's shared memory");
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -87,6 +91,18 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ unsigned low_k_major(const void* tile) { return ((smem_u32(tile) & 0x3FFFFu) >> 4) | (1u << 16); }
 __device__ __forceinline__ void umma_commit_at(unsigned bar_addr) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr) : "memory");
+}
+// The product of the 16 columns beside the tiles, added to what is there: two 8-column groups BM * 16 bytes apart, 8-row groups 128 bytes apart, no swizzle.
+constexpr unsigned BESIDE_HIGH = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ unsigned beside_low(const void* tile) { return ((smem_u32(tile) & 0x3FFFFu) >> 4) | ((unsigned)(BM * 16 >> 4) << 16); }
+__device__ __forceinline__ void umma_beside(unsigned tmem_d, unsigned a_low, unsigned b_low, unsigned idesc) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t.reg .b64 da, db;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 da, {%1, %4};\n\t"
+        "mov.b64 db, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, q;\n\t}"
+        ::"r"(tmem_d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(BESIDE_HIGH) : "memory");
 }
 __device__ __forceinline__ bool elected() {  // one lane of the warp, all of which are here
     unsigned one;
@@ -140,6 +156,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
     return d;
 }
 
+// Two floats at a time.
+struct Pair { float x, y; };
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("{.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 struct Args {
     const int* block_table; int table_width;
     const int* starts;    // [requests + 1]
@@ -147,9 +177,11 @@ struct Args {
     int tokens, most, longest;
     float* weights;       // [requests, kv_heads, capacity]
     int capacity;
-    float2* rows;         // [tokens * heads]: (m, 1 / l)
+    uint4* rows;          // [tokens * heads]: -(m + log2 l) / c in three parts of bfloat16, and zeros
     float2* cuts;         // [n_cuts, tokens * heads]: (m, l), where the slots are cut
     int n_cuts;
+    float* parts;         // [spans, requests, kv_heads, padded]: a span's part of the slots' sums, where there is more than one
+    int spans, padded;    // spans of tiles of Q; slots in whole tiles
     int heads, kv_heads, group, page_shift, pages;
     int per_tile;         // tokens of a tile of Q
     float scale_log2;
@@ -164,17 +196,30 @@ __device__ __forceinline__ Request request_of(const Args& a, int r, bool reports
     first = min(max(first, 0), a.tokens), tokens = min(min(max(tokens, 0), a.most), a.tokens - first), length = min(max(length, 0), a.longest);
     return {first, tokens, length};
 }
-__device__ __forceinline__ float2 as_factor(float m, float l) { return make_float2(m == -INFINITY ? 0.f : m, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)); }
+// What stands beside a row: -(m + log2 l) / c in three parts, which together hold a float's 24 bits.  A row without a score that counts has -infinity, and gives nothing.
+__device__ __forceinline__ unsigned half_word(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ uint4 beside_row(float m, float l, float c) {
+    const float x = l == 0.f ? -INFINITY : -(m + log2f(l)) / c;
+    const unsigned hi = half_word(x);
+    unsigned mid = 0, lo = 0;
+    if (fabsf(x) < INFINITY) {
+        const float rest = x - __uint_as_float(hi << 16);
+        mid = half_word(rest), lo = half_word(rest - __uint_as_float(mid << 16));
+    }
+    return make_uint4(hi | mid << 16, lo, 0, 0);
+}
+__device__ __forceinline__ int first_tile(const Args& a, int slot, int before) { return max(0, slot - before) / a.per_tile; }  // token slot - before is the first that sees the slot
 
-// One walk.  KEYS_STAY: block (tile of slots, key/value head, request), tiles of Q pass; else block (cut, tile of Q and key/value head, request), tiles of K pass.
+// One walk.  KEYS_STAY: block (span of tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (cut, tile of Q and key/value head, request), tiles of K pass.
 template <bool KEYS_STAY>
-__global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap rows_map, const Args a) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* stays = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* ring = stays + TILE;
-    float* tops = reinterpret_cast<float*>(ring + STAGES * TILE);  // KEYS_STAY: [2][BM], m of the passing rows
-    float* shares = tops + 2 * BM;                                  // [2][BM], their 1 / l
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(shares + 2 * BM);
+    unsigned char* beside_stays = ring + STAGES * TILE;              // KEYS_STAY
+    unsigned char* beside = beside_stays + BESIDE;                   // KEYS_STAY: [STAGES]
+    float* theirs = reinterpret_cast<float*>(beside + STAGES * BESIDE);  // [2][BM]: what one half of the warps tells the other
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(theirs + 2 * BM);
     unsigned long long* empty = full + STAGES;
     unsigned long long* s_full = empty + STAGES;  // [2]
     unsigned long long* s_empty = s_full + 2;     // [2]
@@ -188,11 +233,13 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.y % a.kv_heads, group = a.group;
     const Request r = request_of(a, request, !KEYS_STAY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
     const int before = r.length - r.tokens;  // token i sees before + i + 1 slots
-    const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile, base = KEYS_STAY ? blockIdx.x * BM : (int)(gridDim.y / a.kv_heads - 1 - blockIdx.y / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
+    const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile;
+    const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.y / a.kv_heads - 1 - blockIdx.y / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
     int from, to;  // tiles that pass
     if (KEYS_STAY) {
         if (base >= r.length || r.tokens == 0) return;
-        from = max(0, base - before) / a.per_tile, to = q_tiles;  // token base - before is the first that sees slot base
+        const int span = blockIdx.x % a.spans;
+        from = max(span * SPAN, first_tile(a, base, before)), to = min(q_tiles, (span + 1) * SPAN);
         if (from >= to) return;
     } else {
         if (base >= r.tokens) return;
@@ -202,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     const int n_tiles = to - from;
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], EPILOGUE); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], HALF); }
         mbar_init(stays_full, 1), mbar_init(all_done, 1);
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -214,6 +261,15 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     for (int e = tid; e < (BM - q_rows) * 8 * PANELS * (KEYS_STAY ? STAGES : 1); e += THREADS) {
         const int chunk = e & 7, row = q_rows + (e >> 3) % (BM - q_rows), panel = (e >> 3) / (BM - q_rows);
         reinterpret_cast<uint4*>((KEYS_STAY ? ring : stays) + panel * PANEL + row * 128)[chunk] = make_uint4(0, 0, 0, 0);
+    }
+    if (KEYS_STAY) {
+        for (int e = tid; e < 2 * BM * (1 + STAGES); e += THREADS) {
+            const int row = e % BM, second = e / BM & 1, tile = e / (2 * BM);  // of the tiles, the first stays
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (!second && tile == 0) x = make_uint4(0x3f803f80u, 0x3f80u, 0, 0);  // 1 1 1 0 ...
+            if (!second && tile && row >= q_rows) x.x = 0xff7fu;                    // the lowest number: a row that is none gives nothing
+            if (second || !tile || row >= q_rows) reinterpret_cast<uint4*>(beside_stays)[e] = x;
+        }
     }
     // Tensor memory is taken only now that the kernels before have finished, and the next kernel is let in only once it is: a block further back or further on that holds some while it waits could wait for this one.
     if (warp == ISSUER) {
@@ -251,8 +307,9 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         };
         auto fetch_queries = [&](unsigned char* tile, int token, unsigned long long* bar) {  // tokens beyond the request's own come along, or are filled with zeros
             if (lane == 0) {
-                mbar_expect_tx(bar, (unsigned)(PANELS * 128 * q_rows));
+                mbar_expect_tx(bar, (unsigned)((PANELS * 128 + (KEYS_STAY ? 16 : 0)) * q_rows));
                 for (int h = 0; h < PANELS; ++h) tma_load_3d(tile + h * PANEL, &q_map, bar, h * 64, kvh * group, r.first + token);
+                if (KEYS_STAY) tma_load_3d(beside + (tile - ring) / TILE * BESIDE, &rows_map, bar, 0, kvh * group, r.first + token);
             }
         };
         int sent = 0;
@@ -289,6 +346,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
                 const unsigned b_low = b_low0 + (unsigned)s * (TILE >> 4);
 #pragma unroll
                 for (int h = 0; h < PANELS; ++h) umma_s_panel(tmem + b * BM, a_low + h * (PANEL >> 4), b_low + h * (PANEL >> 4), IDESC, h ? 1u : 0u);
+                if (KEYS_STAY) umma_beside(tmem + b * BM, beside_low(beside_stays), beside_low(beside) + (unsigned)s * (BESIDE >> 4), IDESC);
                 umma_commit_at(smem_u32(&empty[s]));
                 umma_commit_at(smem_u32(&s_full[b]));
             }
@@ -299,106 +357,101 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         __syncwarp();
         mbar_last_wait(all_done, 0);
     } else {
-        // ------------------------------------------------------------------ four warps: a thread has a lane of the product
-        const int mine = warp * 32 + lane;
-        const unsigned lanes = tmem + ((unsigned)(warp * 32) << 16);
+        // ------------------------------------------------------------------ four warps a buffer: a thread has a lane of the product, 32 columns of it at a time
+        const int half = warp / HALF, mine = (warp & 3) * 32 + lane;
+        const unsigned lanes = tmem + half * BM + ((unsigned)((warp & 3) * 32) << 16);
         const float c = a.scale_log2;
         bool ok = true;
         [[maybe_unused]] float m = -INFINITY, l = 0.f;         // of this thread's row
         [[maybe_unused]] float sum = 0.f, rest = 0.f;          // of this thread's slot, and what its additions lost
-        [[maybe_unused]] const int token = base + mine / group;
+        const int my_token = mine / group, my_head = kvh * group + mine - my_token * group;
+        [[maybe_unused]] const int token = base + my_token;
         [[maybe_unused]] const int sees = token < r.tokens && mine < q_rows ? min(r.length, before + token + 1) : 0;
         [[maybe_unused]] const int all_see = min(r.length, before + base + 1);  // slots that every row of the tile sees
-        auto factor_of = [&](int tile) {  // of row `mine` of a tile of Q
-            const int t = tile * a.per_tile + mine / group;
-            return tile < to && mine < q_rows && t < r.tokens ? a.rows[(size_t)(r.first + t) * a.heads + kvh * group + mine % group] : make_float2(0.f, 0.f);
-        };
-        float2 factor;
-        if (KEYS_STAY) factor = factor_of(from);
-        for (int i = 0; i < n_tiles; ++i) {
-            const int b = i & 1;
-            if constexpr (KEYS_STAY) {
-                tops[b * BM + mine] = factor.x, shares[b * BM + mine] = factor.y;
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * EPILOGUE) : "memory");  // whoever still reads the other buffer has this one's turn before it is written again
-                factor = factor_of(from + i + 1);
-            }
-            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[b], (i >> 1) & 1, failed))) {
+        for (int i = half; i < n_tiles; i += 2) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[half], (i >> 1) & 1, failed))) {
                 *failed = 1, ok = false;
-                if (KEYS_STAY) continue;  // to meet the others at the barrier above
                 break;
             }
             tc_fence_after();
-            unsigned raw[4][32];
+            unsigned raw[2][32];
+            tmem_ld32(lanes, raw[0]);
+            arrived(raw[0]);
+            const int slot0 = (from + i) * BM, token0 = (from + i) * a.per_tile;
+            // KEYS_STAY: the first row that sees this slot, and the rows that are the request's; whether all rows see all slots
+            [[maybe_unused]] const int from_row = (base + mine - before - token0) * group, rows = min((r.tokens - token0) * group, q_rows);
+            const bool all = KEYS_STAY ? base + BM - 1 - before <= token0 && r.tokens - token0 >= a.per_tile : slot0 + BM <= all_see;
+            Pair part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tmem_ld32(lanes + b * BM + 32 * k, raw[k]);
+            for (int k = 0; k < 4; ++k) {
+                unsigned (&v)[32] = raw[k & 1];
+                if (k < 3) tmem_ld32(lanes + 32 * (k + 1), raw[(k + 1) & 1]);
+                auto pair_at = [&](int j) { return Pair{__uint_as_float(v[j]), __uint_as_float(v[j + 1])}; };
+                if constexpr (KEYS_STAY) {
+                    if (!all) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) arrived(raw[k]);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[b]);
-            auto s_at = [&](int j) -> float { return __uint_as_float(raw[j >> 5][j & 31]); };
-            if constexpr (KEYS_STAY) {
-                const int token0 = (from + i) * a.per_tile;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-                const float* top = tops + b * BM;
-                const float* share = shares + b * BM;
-                const int from_row = (base + mine - before - token0) * group, rows = (r.tokens - token0) * group;  // rows that see this slot, and rows of the request
-                const bool all = (base + BM - 1 - before - token0) <= 0 && r.tokens - token0 >= a.per_tile;
-                if (all) {
-#pragma unroll
-                    for (int j = 0; j < BM; j += 4) {
-                        float mm[4], ss[4];
-                        load4(top + j, mm), load4(share + j, ss);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) part[e] = fmaf(fast_exp2(fmaf(s_at(j + e), c, -mm[e])), ss[e], part[e]);
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;  // a row that does not see this slot gives it nothing, whatever the row is
                     }
-                } else {
 #pragma unroll
-                    for (int j = 0; j < BM; j += 4) {
-                        float mm[4], ss[4];
-                        load4(top + j, mm), load4(share + j, ss);
+                    for (int j = 0; j < 32; j += 4)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float p = fast_exp2(fmaf(s_at(j + e), c, -mm[e])) * ss[e];
-                            if (j + e >= from_row && j + e < rows && j + e < q_rows) part[e] += p;
+                        for (int e = 0; e < 2; ++e) {
+                            const Pair y = fma2(pair_at(j + 2 * e), Pair{c, c}, Pair{0.f, 0.f});
+                            part[e] = add2(part[e], Pair{fast_exp2(y.x), fast_exp2(y.y)});
                         }
+                } else {
+                    if (!all) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (slot0 + 32 * k + j >= sees) v[j] = 0xff800000u;
                     }
+                    float top = -INFINITY, other = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        top = max3(top, pair_at(j).x, pair_at(j).y), other = max3(other, pair_at(j + 2).x, pair_at(j + 2).y);
+                    }
+                    const float above = fmaxf(m, fmaxf(top, other) * c), low = above == -INFINITY ? 0.f : above;  // c is above 0
+                    l *= m == -INFINITY ? 1.f : fast_exp2(m - low);  // nothing but zeros and NaN has been added up below -infinity
+                    m = above;
+                    part[0] = part[1] = Pair{0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const Pair y = fma2(pair_at(j + 2 * e), Pair{c, c}, Pair{-low, -low});
+                            part[e] = add2(part[e], Pair{fast_exp2(y.x), fast_exp2(y.y)});
+                        }
+                    l += (part[0].x + part[0].y) + (part[1].x + part[1].y);
                 }
+                if (k < 3) arrived(raw[(k + 1) & 1]);
+                if (k == 2) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_empty[half]);
+                }
+            }
+            if constexpr (KEYS_STAY) {
                 // added up with what is lost: a slot that thousands of rows see would be off by more than all else
-                const float y = (part[0] + part[1]) + (part[2] + part[3]) - rest, t = sum + y;
+                const float y = (part[0].x + part[0].y) + (part[1].x + part[1].y) - rest, t = sum + y;
                 rest = (t - sum) - y, sum = t;
-            } else {
-                const int slot0 = (from + i) * BM;
-                if (slot0 + BM > all_see) {
-#pragma unroll
-                    for (int j = 0; j < BM; ++j)
-                        if (slot0 + j >= sees) raw[j >> 5][j & 31] = 0xff800000u;
-                }
-                float top[4] = {m, m, m, m};
-#pragma unroll
-                for (int j = 0; j < BM; j += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        // c is above 0: the largest score is the largest product
-                        top[e] = max3(top[e], s_at(j + e) * c, s_at(j + e + 4) * c);
-                    }
-                const float above = fmaxf(max3(top[0], top[1], top[2]), top[3]), low = above == -INFINITY ? 0.f : above;
-                l *= m == -INFINITY ? 1.f : fast_exp2(m - low);  // nothing but zeros and NaN has been added up below -infinity
-                m = above;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < BM; j += 4)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) part[e] += fast_exp2(fmaf(s_at(j + e), c, -low));
-                l += (part[0] + part[1]) + (part[2] + part[3]);
             }
         }
-        if constexpr (KEYS_STAY) {
-            if (base + mine < r.length && ok) a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + base + mine] += sum;
-        } else if (mine < q_rows && token < r.tokens && ok) {
-            const size_t at = (size_t)(r.first + token) * a.heads + kvh * group + mine % group;
-            if (a.n_cuts == 1) a.rows[at] = as_factor(m, l);
-            else a.cuts[(size_t)blockIdx.x * a.tokens * a.heads + at] = make_float2(m, l);
+        // the second half's sums come to the first
+        if (half == 1) theirs[mine] = KEYS_STAY ? sum : m, theirs[BM + mine] = KEYS_STAY ? rest : l;
+        asm volatile("bar.sync 3, %0;" ::"n"(64 * HALF) : "memory");
+        if (half == 0 && ok) {
+            if constexpr (KEYS_STAY) {
+                sum += theirs[mine] - (rest + theirs[BM + mine]);
+                if (a.spans > 1) a.parts[(((size_t)(blockIdx.x % a.spans) * gridDim.z + request) * a.kv_heads + kvh) * a.padded + base + mine] = sum;
+                else if (base + mine < r.length) a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + base + mine] += sum;
+            } else if (mine < q_rows && token < r.tokens) {
+                const float other = theirs[mine], above = fmaxf(m, other);
+                l = (m == -INFINITY ? l : l * fast_exp2(m - above)) + (other == -INFINITY ? theirs[BM + mine] : theirs[BM + mine] * fast_exp2(other - above));
+                const size_t at = (size_t)(r.first + token) * a.heads + my_head;
+                if (a.n_cuts == 1) a.rows[at] = beside_row(above, l, c);
+                else a.cuts[(size_t)blockIdx.x * a.tokens * a.heads + at] = make_float2(above, l);
+            }
         }
     }
     tc_fence_before();
@@ -421,7 +474,20 @@ __global__ void __launch_bounds__(256) tally_cuts_kernel(const Args a) {
         const float2 ml = a.cuts[(size_t)c * n + at];
         all = fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top), ml.y, all);
     }
-    a.rows[at] = as_factor(top, all);
+    a.rows[at] = beside_row(top, all, a.scale_log2);
+}
+
+// The spans' parts of the slots' sums, in their order.
+__global__ void __launch_bounds__(256) tally_parts_kernel(const Args a) {
+    let_next_kernel_start();
+    wait_for_previous_kernels();
+    const int slot = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, request = blockIdx.z;
+    const Request r = request_of(a, request, false);
+    if (slot >= r.length) return;
+    const int first = first_tile(a, slot / BM * BM, r.length - r.tokens) / SPAN, end = ((r.tokens + a.per_tile - 1) / a.per_tile + SPAN - 1) / SPAN;  // spans that the tile of slots has a block for
+    float sum = 0.f;
+    for (int span = first; span < end; ++span) sum += a.parts[(((size_t)span * gridDim.z + request) * a.kv_heads + kvh) * a.padded + slot];
+    a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + slot] += sum;
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -435,18 +501,18 @@ EncodeTiled encode_tiled() {
     }();
     return fn;
 }
-int encoded(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+int encoded(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return HB_BAD_ARGUMENT;
     const cuuint32_t elem[3] = {1, 1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
 }
 template <bool KEYS_STAY>
-int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const Args& a, dim3 grid, cudaStream_t stream) {
+int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUtensorMap& rows_map, const Args& a, dim3 grid, cudaStream_t stream) {
     const cudaError_t configured = cudaFuncSetAttribute(tally_walk_kernel<KEYS_STAY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(tally_walk_kernel<KEYS_STAY>, grid, dim3(THREADS), SMEM_BYTES, stream, kv_map, q_map, a);
+    return launch_after_previous(tally_walk_kernel<KEYS_STAY>, grid, dim3(THREADS), SMEM_BYTES, stream, kv_map, q_map, rows_map, a);
 }
 }  // namespace
 
@@ -456,28 +522,31 @@ static int cuts_for(int requests, int most, int longest, int heads, int kv_heads
     const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = (longest + BM - 1) / BM;
     return (int)(wanted < 1 ? 1 : wanted < most_cuts ? wanted : most_cuts);
 }
+static int spans_for(int most, int group) { return ((most + BM / group - 1) / (BM / group) + SPAN - 1) / SPAN; }
 // Bytes of scratch that hb_tally_queries takes.
 HB_EXPORT long long hb_tally_queries_scratch(int tokens, int requests, int most, int longest, int heads, int kv_heads, int sms) {
     if (tokens <= 0 || requests <= 0 || most <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > BM || sms <= 0) return 0;
     const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
-    return 8LL * tokens * heads * (cuts > 1 ? cuts + 1 : 1);
+    const long long spans = spans_for(most, heads / kv_heads), padded = (longest + BM - 1) / BM * (long long)BM;
+    return 16LL * tokens * heads + (cuts > 1 ? 8LL * tokens * heads * cuts : 0) + (spans > 1 ? 4 * spans * requests * kv_heads * padded : 0);
 }
 // q [tokens, heads * D] with rows q_stride apart, request r's from starts[r] to starts[r + 1] - 1, at most `most`, the last of which stands in its last slot; cache [pages, 2, kv_heads, page_size, D];
-// lengths [requests], at most `longest`, which table and capacity hold; weights [requests, kv_heads, capacity].  scratch: hb_tally_queries_scratch bytes on an 8-byte boundary.
+// lengths [requests], at most `longest`, which table and capacity hold; weights [requests, kv_heads, capacity].  scratch: hb_tally_queries_scratch bytes on a 16-byte boundary.
 HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, const void* cache, const int* block_table, int table_width, const int* starts, const int* lengths, int requests, int most,
                                int longest, float* weights, int capacity, int heads, int kv_heads, int page_size, int pages, float scale, int sms, void* scratch, int* status, cudaStream_t stream) {
     if (requests <= 0 || tokens <= 0) return 0;
     if (!q || !cache || !block_table || !starts || !lengths || !weights || !scratch || !status) return HB_BAD_ARGUMENT;
-    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || most <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || most <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || !(scale >= 0x1p-100f)) return HB_BAD_ARGUMENT;
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1)) || heads / kv_heads > BM) return HB_UNSUPPORTED_SIZE;
-    if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)scratch & 7) || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
+    if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)scratch & 15) || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     const int group = heads / kv_heads, per_tile = BM / group;
     if (q_stride > 0x7fffffffLL || (long long)tokens * heads > 0x7fffffffLL - 256 || longest > 0x7fffffff - BM || requests > 65535 || kv_heads > 65535) return HB_UNSUPPORTED_SIZE;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     const long long row_blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads;
     if (row_blocks > 65535) return HB_UNSUPPORTED_SIZE;
-    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
-    CUtensorMap kv_map, q_map;
+    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), spans = spans_for(most, group), padded = (longest + BM - 1) / BM * BM;
+    if ((long long)padded / BM * spans > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
+    CUtensorMap kv_map, q_map, rows_map;
     const cuuint64_t kv_dims[2] = {(cuuint64_t)D, (cuuint64_t)pages * 2 * kv_heads * page_size}, kv_strides[1] = {(cuuint64_t)D * 2};
     const cuuint32_t kv_box[2] = {64, (cuuint32_t)page_size};
     if (int code = encoded(&kv_map, cache, 2, kv_dims, kv_strides, kv_box)) return code;
@@ -485,11 +554,16 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     const cuuint64_t q_dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens}, q_strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)(tokens > 1 ? q_stride : (long long)heads * D) * 2};
     const cuuint32_t q_box[3] = {64, (cuuint32_t)group, (cuuint32_t)per_tile};
     if (int code = encoded(&q_map, q, 3, q_dims, q_strides, q_box)) return code;
-    float2* rows = (float2*)scratch;
-    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, rows + (size_t)tokens * heads, cuts, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
+    uint4* rows = (uint4*)scratch;
+    const cuuint64_t rows_dims[3] = {8, (cuuint64_t)heads, (cuuint64_t)tokens}, rows_strides[2] = {16, (cuuint64_t)heads * 16};
+    const cuuint32_t rows_box[3] = {8, (cuuint32_t)group, (cuuint32_t)per_tile};
+    if (int code = encoded(&rows_map, rows, 3, rows_dims, rows_strides, rows_box, CU_TENSOR_MAP_SWIZZLE_NONE)) return code;
+    float2* cut_sums = (float2*)(rows + (size_t)tokens * heads);
+    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, (float*)(cut_sums + (cuts > 1 ? (size_t)tokens * heads * cuts : 0)), spans, padded, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
                  scale * 1.4426950408889634f, status};
-    if (int code = launch_walk<false>(kv_map, q_map, a, dim3(cuts, (unsigned)row_blocks, requests), stream)) return code;
+    if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3(cuts, (unsigned)row_blocks, requests), stream)) return code;
     if (cuts > 1)
         if (int code = launch_after_previous(tally_cuts_kernel, dim3((tokens * heads + 255) / 256), dim3(256), 0, stream, a)) return code;
-    return launch_walk<true>(kv_map, q_map, a, dim3((longest + BM - 1) / BM, kv_heads, requests), stream);
+    if (int code = launch_walk<true>(kv_map, q_map, rows_map, a, dim3(padded / BM * spans, kv_heads, requests), stream)) return code;
+    return spans > 1 ? launch_after_previous(tally_parts_kernel, dim3((longest + 255) / 256, kv_heads, requests), dim3(256), 0, stream, a) : 0;
 }

@@ -1,8 +1,9 @@
 """Attention that keeps its weights, and the weights of a prompt's queries, against the formulas in 64 bits.
 
 Tolerances.  A score is a sum of d products that are exact in float, added up in d / 16 steps of the tensor cores, each off by at most 2^-22 of what it adds up (they cut, where rounding would be half of
-it), then multiplied by scale * log2(e), two roundings: with S = max_j sum_i |q_i k_ji| scale log2(e), y is off by less than delta = (d / 16 * 2^-22 + 2^-22) S.  A softmax weight p is 2^(y - m) / l: the power is
-off by ln2 delta and 2^-22 (the hardware's), l by as much on average, so p by less than e_p = 2 (ln2 delta + 2^-21) of itself.  Sums over up to n terms in float add n 2^-24 at the most (a lane adds up few; n = 64 here).
+it), then multiplied by scale * log2(e), two roundings: with S = max_j sum_i |q_i k_ji| scale log2(e), y is off by less than (d / 16 + 1) 2^-22 S.  Where queries are many, m + log2 l, which is at most S + 17 here, goes
+through one more step of the tensor cores: 2^-22 (2 S + 17), and 2^-22 (S + 3) for the logarithm, the division and its three parts.  So delta = 2^-22 ((d / 16 + 4) S + 20).  A softmax weight p is 2^(y - m) / l: the power
+is off by ln2 delta and 2^-22 (the hardware's), l by as much on average, so p by less than e_p = 2 (ln2 delta + 2^-21) of itself.  Sums over up to n terms in float add n 2^-24 at the most (a lane adds up few; n = 64 here).
 A result is sum p v, its weights in two parts of bfloat16 (2^-16 of a weight), rounded to bfloat16 (2^-8 of it) at the end."""
 from __future__ import annotations
 
@@ -57,7 +58,7 @@ def attended(q, heads, cache, table, counts, lengths, scale):
             y = torch.einsum("kgd,knd->kgn", x, k[:, :sees]) * scale
             p = torch.softmax(y, -1)
             size = torch.einsum("kgd,knd->kgn", x.abs(), k[:, :sees].abs()).amax(-1, keepdim=True) * scale * LOG2E
-            e = 2 * (0.6931471805599453 * (dim / 16 * 2.0 ** -22 + 2.0 ** -22) * size + 2.0 ** -21) + 64 * 2.0 ** -24
+            e = 2 * (0.6931471805599453 * 2.0 ** -22 * ((dim / 16 + 4) * size + 20) + 2.0 ** -21) + 64 * 2.0 ** -24
             weights[:, :sees] += p.sum(1)
             off[:, :sees] += (p * e).sum(1)
             found.append((r, (p @ v[:, :sees]).reshape(-1), ((p * (e + 2.0 ** -16)) @ v[:, :sees].abs()).reshape(-1), e.max().item()))
@@ -190,6 +191,36 @@ def test_queries(heads, kv, dim, page, counts, lengths):
             rows = counts[r] * heads // kv  # sums over the rows, a quarter of them by one lane one behind the other
             close(tally.weights[r, :, :n], want, off + want * (rows / 4 + 4) * 2.0 ** -24 + 2.0 ** -23)
             assert torch.equal(tally.weights[r, :, n:], before[r, :, n:])
+
+
+def test_a_query_with_a_nan_spoils_the_slots_that_it_sees_and_no_others():
+    cache, table, random = pages_of([300], 2, 64, 16, seed=12)
+    q, tally = queries(random, 250, 6 * 64), new_tally(1, 2, 304)
+    q[170, 64] = float("nan")   # a head of key/value head 0: sees slots 0 .. 220
+    q[100, 5 * 64] = float("inf")  # of key/value head 1: slots 0 .. 150
+    tally_queries(q, 6, cache, table, torch.tensor([0, 250], dtype=torch.int32, device="cuda"), torch.tensor([300], dtype=torch.int32, device="cuda"), tally, 0.125, most=250)
+    ops.raise_on_status(q.device)
+    assert [tally.weights[0, h].isnan().nonzero().flatten().tolist() for h in range(2)] == [list(range(221)), list(range(151))]
+
+
+def test_prompts_of_many_spans():
+    """Tiles of queries are cut into spans of 16, whose parts are put together."""
+    counts, lengths, heads, kv, dim = [2500, 700], [2600, 3000], 8, 1, 64
+    cache, table, random = pages_of(lengths, kv, dim, 64, seed=13)
+    q, tally = queries(random, sum(counts), heads * dim, size=1.0), new_tally(2, kv, 3008)
+    starts = torch.tensor([0, 2500, 3200], dtype=torch.int32, device="cuda")
+    tally_queries(q, heads, cache, table, starts, torch.tensor(lengths, dtype=torch.int32, device="cuda"), tally, 0.125, most=2500)
+    ops.raise_on_status(q.device)
+    first = 0
+    for r, (count, length) in enumerate(zip(counts, lengths)):
+        k, _ = records(cache, table, r, length)
+        y = torch.einsum("ihd,nd->ihn", q[first: first + count].double().view(count, heads, dim), k[0]) * 0.125
+        y.masked_fill_((torch.arange(length, device="cuda") > torch.arange(length - count, length, device="cuda")[:, None])[:, None], float("-inf"))
+        p = torch.softmax(y, -1)
+        size = torch.einsum("ihd,nd->ihn", q[first: first + count].double().view(count, heads, dim).abs(), k[0].abs()).amax(-1, keepdim=True) * 0.125 * LOG2E
+        e = 2 * (0.6931471805599453 * 2.0 ** -22 * ((dim / 16 + 4) * size + 20) + 2.0 ** -21) + 64 * 2.0 ** -24
+        first += count
+        close(tally.weights[r, 0, :length], p.sum((0, 1)), (p * e).sum((0, 1)) + p.sum((0, 1)) * 8 * 2.0 ** -24)
 
 
 def test_more_queries_than_slots_see_nothing():
