@@ -169,6 +169,33 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^y of a pair without the special function unit, which takes 8 clocks for a warp's 32 where the other units take half a one for each of these operations: y = n + f with n the nearest whole number (adding and
+// taking away 1.5 * 2^23 rounds, and leaves n in the low bits), 2^f by the polynomial of degree 5 with the smallest relative error over [-1/2, 1/2] (7.5e-8; 2.1e-7 with its roundings), 2^n from its bits.  Below
+// 2^-126 it is 0; a NaN stays one.  y at most 126.
+__device__ __forceinline__ Pair polynomial_exp2(Pair y) {
+    const Pair t{max_nan(y.x, -127.f), max_nan(y.y, -127.f)}, r = add2(t, Pair{12582912.f, 12582912.f}), n = add2(r, Pair{-12582912.f, -12582912.f}), f = fma2(n, Pair{-1.f, -1.f}, t);
+    Pair p = fma2(f, Pair{1.3276472e-3f, 1.3276472e-3f}, Pair{9.675541e-3f, 9.675541e-3f});
+    p = fma2(p, f, Pair{5.550713e-2f, 5.550713e-2f});
+    p = fma2(p, f, Pair{0.2402212f, 0.2402212f});
+    p = fma2(p, f, Pair{0.69314694f, 0.69314694f});
+    p = fma2(p, f, Pair{1.0000001f, 1.0000001f});
+    return mul2(p, Pair{__uint_as_float((__float_as_uint(r.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(r.y) << 23) + 0x3f800000u)});
+}
+// Of 16 pairs so many take the polynomial, spread evenly.
+#ifndef HB_POLY
+#define HB_POLY 5
+#endif
+__device__ __forceinline__ Pair exp2_of(Pair y, int pair) { return (pair + 1) * HB_POLY / 16 != pair * HB_POLY / 16 ? polynomial_exp2(y) : Pair{fast_exp2(y.x), fast_exp2(y.y)}; }
 
 struct Args {
     const int* block_table; int table_width;
@@ -229,24 +256,6 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, request = blockIdx.z;
-    wait_for_previous_kernels();
-    const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.y % a.kv_heads, group = a.group;
-    const Request r = request_of(a, request, !KEYS_STAY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
-    const int before = r.length - r.tokens;  // token i sees before + i + 1 slots
-    const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile;
-    const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.y / a.kv_heads - 1 - blockIdx.y / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
-    int from, to;  // tiles that pass
-    if (KEYS_STAY) {
-        if (base >= r.length || r.tokens == 0) return;
-        const int span = blockIdx.x % a.spans;
-        from = max(span * SPAN, first_tile(a, base, before)), to = min(q_tiles, (span + 1) * SPAN);
-        if (from >= to) return;
-    } else {
-        if (base >= r.tokens) return;
-        const int reach = min(r.length, max(0, before + min(base + a.per_tile, r.tokens))), n = (reach + BM - 1) / BM;  // slots that any of the tokens sees
-        from = (int)((long long)n * blockIdx.x / a.n_cuts), to = (int)((long long)n * (blockIdx.x + 1) / a.n_cuts);
-    }
-    const int n_tiles = to - from;
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], HALF); }
@@ -255,7 +264,33 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+        if (KEYS_STAY) asm volatile("prefetch.tensormap [%0];" ::"l"(&rows_map) : "memory");
     }
+    // The second walk waits only before it asks for what stands beside the rows: its blocks are let in once all of the first walk's have their tensor memory, so what came before that one has finished.
+    if (!KEYS_STAY) wait_for_previous_kernels();
+    const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.y % a.kv_heads, group = a.group;
+    const Request r = request_of(a, request, !KEYS_STAY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
+    const int before = r.length - r.tokens;  // token i sees before + i + 1 slots
+    const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile;
+    const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.y / a.kv_heads - 1 - blockIdx.y / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
+    int from, to;  // tiles that pass
+    if (KEYS_STAY) {
+        if (base >= r.length || r.tokens == 0) {
+            wait_for_previous_kernels();  // whoever comes next takes this kernel's end as the end of all
+            return;
+        }
+        const int span = blockIdx.x % a.spans;
+        from = max(span * SPAN, first_tile(a, base, before)), to = min(q_tiles, (span + 1) * SPAN);
+        if (from >= to) {
+            wait_for_previous_kernels();
+            return;
+        }
+    } else {
+        if (base >= r.tokens) return;
+        const int reach = min(r.length, max(0, before + min(base + a.per_tile, r.tokens))), n = (reach + BM - 1) / BM;  // slots that any of the tokens sees
+        from = (int)((long long)n * blockIdx.x / a.n_cuts), to = (int)((long long)n * (blockIdx.x + 1) / a.n_cuts);
+    }
+    const int n_tiles = to - from;
     // rows of Q's tiles that no copy writes (beyond whole tokens)
     const int q_rows = a.per_tile * group;
     for (int e = tid; e < (BM - q_rows) * 8 * PANELS * (KEYS_STAY ? STAGES : 1); e += THREADS) {
@@ -271,7 +306,8 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             if (second || !tile || row >= q_rows) reinterpret_cast<uint4*>(beside_stays)[e] = x;
         }
     }
-    // Tensor memory is taken only now that the kernels before have finished, and the next kernel is let in only once it is: a block further back or further on that holds some while it waits could wait for this one.
+    // Tensor memory is taken only now that no kernel before wants any more of it (those before the first walk have finished, and the first walk's blocks have theirs), and the next kernel is let in only once it is:
+    // a block further back or further on that holds some while it waits could wait for this one.
     if (warp == ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -283,6 +319,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     tc_fence_after();
     const unsigned tmem = *tmem_slot;
 
+    if (KEYS_STAY && warp != PRODUCER) wait_for_previous_kernels();  // not at the barriers, where looking takes turns from the first walk's last blocks (three prompts 196 us)
     if (warp == PRODUCER) {
         // ------------------------------------------------------------------ the whole warp
         const int page_size = 1 << a.page_shift, pages_per_tile = BM >> a.page_shift;
@@ -305,8 +342,10 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             const int p = min(lane, ops - 1) / PANELS, h = lane % PANELS, id = __shfl_sync(0xffffffffu, page, p);
             if (lane < ops && id >= 0) tma_load_2d(tile + h * PANEL + p * page_size * 128, &kv_map, bar, h * 64, (id * 2 * a.kv_heads + kvh) << a.page_shift);
         };
+        [[maybe_unused]] bool waited = false;
         auto fetch_queries = [&](unsigned char* tile, int token, unsigned long long* bar) {  // tokens beyond the request's own come along, or are filled with zeros
             if (lane == 0) {
+                if (KEYS_STAY && !waited) wait_for_previous_kernels(), waited = true;
                 mbar_expect_tx(bar, (unsigned)((PANELS * 128 + (KEYS_STAY ? 16 : 0)) * q_rows));
                 for (int h = 0; h < PANELS; ++h) tma_load_3d(tile + h * PANEL, &q_map, bar, h * 64, kvh * group, r.first + token);
                 if (KEYS_STAY) tma_load_3d(beside + (tile - ring) / TILE * BESIDE, &rows_map, bar, 0, kvh * group, r.first + token);
@@ -398,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const Pair y = fma2(pair_at(j + 2 * e), Pair{c, c}, Pair{0.f, 0.f});
-                            part[e] = add2(part[e], Pair{fast_exp2(y.x), fast_exp2(y.y)});
+                            part[e] = add2(part[e], exp2_of(y, j / 2 + e));
                         }
                 } else {
                     if (!all) {
@@ -420,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const Pair y = fma2(pair_at(j + 2 * e), Pair{c, c}, Pair{-low, -low});
-                            part[e] = add2(part[e], Pair{fast_exp2(y.x), fast_exp2(y.y)});
+                            part[e] = add2(part[e], exp2_of(y, j / 2 + e));
                         }
                     l += (part[0].x + part[0].y) + (part[1].x + part[1].y);
                 }
@@ -485,9 +524,17 @@ __global__ void __launch_bounds__(256) tally_parts_kernel(const Args a) {
     const Request r = request_of(a, request, false);
     if (slot >= r.length) return;
     const int first = first_tile(a, slot / BM * BM, r.length - r.tokens) / SPAN, end = ((r.tokens + a.per_tile - 1) / a.per_tile + SPAN - 1) / SPAN;  // spans that the tile of slots has a block for
+    float* weight = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + slot;
+    const float before = *weight;
     float sum = 0.f;
-    for (int span = first; span < end; ++span) sum += a.parts[(((size_t)span * gridDim.z + request) * a.kv_heads + kvh) * a.padded + slot];
-    a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + slot] += sum;
+    for (int span = first; span < end; span += 4) {  // four on their way together
+        float part[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[k] = span + k < end ? a.parts[(((size_t)(span + k) * gridDim.z + request) * a.kv_heads + kvh) * a.padded + slot] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += part[k];
+    }
+    *weight = before + sum;
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
