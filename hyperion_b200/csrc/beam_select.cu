@@ -2,10 +2,10 @@
 //
 //     score(b, v) = score_b + z_bv - log sum_u e^(z_bu)            the `take` largest of them, of equal ones the lowest (b, v)
 //
-// Within a row the order is that of the logits, so a row's best are found without its sum, in the one walk that makes the sum.  The first kernel reads every row once, a block a piece of it: each thread adds
-// up exponentials below its own running maximum, and entries above the `take`-th best so far go into a list in shared memory, which is cut back to `take` when it grows.  In the first batch, where
-// nothing is known yet, the `take`-th largest of the threads' own maxima is a bound that at least `take` entries reach.  After it few entries do: of the n-th batch about take / n.
-// The second kernel has a block per group: it brings the pieces' sums together, and finds the best of the rows' best.
+// The first kernel reads every row once and leaves the sum, and the maximum of every run of 256 logits.  The second has a block per group: with the rows' sums it knows every run's best score.  The runs whose best
+// are the `take` best of all runs hold the `take` best continuations (of a run that is not among them, `take` others hold something better), so only those are read again: a few KB of them.  Both
+// searches take a bound first, the `take`-th largest of what the threads have each found to be their best, and then look at what reaches it: little more than `take` in all but contrived rows, for which there is a way that goes by one
+// continuation after the other.
 //
 // Scores are compared as float64: a score is score_b - lse_b, a number of the row, plus the logit, and float32 would make ties of scores that are not equal.  Sums of a thread's 16 entries are float, everything above
 // them float64; exponentials are the hardware's (2^-22 of a term).  Which thread adds up what goes by the entry's index alone, not by the row's alignment, so rows that hold the same have the same sums.
@@ -18,10 +18,10 @@
 
 namespace {
 typedef __nv_bfloat16 bf16;
-typedef unsigned long long Key;  // (value's bits, ~index): the largest value, of equal ones the lowest index; 0: none
-constexpr int THREADS = 256, PER = 16, CHUNK = THREADS * PER;
-constexpr int MOST_TAKE = 64;
-constexpr int ROOM = CHUNK + 4 * MOST_TAKE + 256;  // of the list: a whole batch may join it
+typedef unsigned long long Key;  // a float64's bits in its order; 0: none
+constexpr int THREADS = 256, WARPS = THREADS / 32, RUN = 256, PER = RUN / 32, AT_ONCE = 2;  // a warp looks at AT_ONCE runs at a time, PER entries a lane of each
+constexpr int MOST_TAKE = 64, MOST_BEAMS = 32;
+constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float cleaned(float v) { return v != v ? -INFINITY : fminf(v, FLT_MAX); }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -29,263 +29,338 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Order-preserving for all floats but NaN; both zeros are the same.
+__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over a NaN, as fmaxf does
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float warp_largest(float v) {
+    float d;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+    return d;
+}
+// Order-preserving for all numbers; both zeros are the same.
 __device__ __forceinline__ unsigned ordered(float v) {
     const unsigned b = __float_as_uint(v + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ Key ordered(double v) {
     const Key b = (Key)__double_as_longlong(v + 0.0);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 __device__ __forceinline__ double value_of(Key o) { return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o)); }
 
-// The sum over the block, in every thread.  `words` holds a word a warp.
-__device__ __forceinline__ int block_count(int n, int* words) {
-    n = __reduce_add_sync(0xffffffffu, n);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = n;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) all += words[w];
-    return all;
-}
-
 struct Args {
     const void* logits; long long stride;
     const float* scores;
-    int groups, beams, vocab, take, pieces, span;  // a block has `span` entries of its row, a multiple of CHUNK
-    Key* best;        // [rows, pieces, take]
+    int groups, beams, vocab, take, runs, pieces, piece_runs;  // runs of a row; blocks of a row, and runs of each
+    float* tops;      // [rows, runs]
     double2* sums;    // [rows, pieces]: (maximum, sum of e^(z - maximum))
     int* parents; int* tokens; float* out_scores;  // [groups, take]
 };
 
-// The list cut back to its `take` largest keys, all of which are different; what stays has no order.
-__device__ int cut_back(Key* list, int n, int take, int* words, int* fill) {
-    if (n <= take) return n;
-    Key last = 0;  // the largest number that `take` keys reach, from its highest digit down
-    for (int bit = 63; bit >= 0; --bit) {
-        const Key higher = last | 1ull << bit;
-        int reach = 0;
-        for (int i = threadIdx.x; i < n; i += THREADS) reach += list[i] >= higher;
-        if (block_count(reach, words) >= take) last = higher;
-    }
-    // the places below `take` that do not reach it take those behind that do
-    __syncthreads();
-    if (threadIdx.x == 0) *fill = 0;
-    __syncthreads();
-    Key kept[ROOM / THREADS + 1];
-    int mine = 0;
-#pragma unroll
-    for (int k = 0; k < ROOM / THREADS + 1; ++k) {
-        const int i = k * THREADS + threadIdx.x;
-        kept[k] = i < n && list[i] >= last ? list[i] : 0;
-        mine += kept[k] != 0;
-    }
-    __syncthreads();
-    int at = mine ? atomicAdd(fill, mine) : 0;
-#pragma unroll
-    for (int k = 0; k < ROOM / THREADS + 1; ++k)
-        if (kept[k]) list[at++] = kept[k];
-    __syncthreads();
-    return take;
+// A lane's eight entries of the run that begins at `first`: bfloat16 [8 lane, 8 lane + 8), float [4 lane, 4 lane + 4) and 128 further on.  Where rows do not begin on 16 bytes the words that hold a lane's entries are
+// fetched from the boundary before and shifted; at a row's ends, entry by entry.
+struct Words { uint4 lo, hi; };
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int words) {  // four of the eight words, from `words` on
+    uint4 r = a;
+    unsigned s0 = b.x, s1 = b.y, s2 = b.z;
+    if (words & 2) r = make_uint4(r.z, r.w, s0, s1), s0 = s2;
+    if (words & 1) r = make_uint4(r.y, r.z, r.w, s0);
+    return r;
 }
-
 template <typename T>
-__device__ __forceinline__ void batch(const T* row, int first, int end, bool wide, float (&v)[PER]) {
-    constexpr int AT_ONCE = 16 / sizeof(T);
-    // a thread has PER / AT_ONCE runs of AT_ONCE entries, THREADS * AT_ONCE apart
-#pragma unroll
-    for (int s = 0; s < PER / AT_ONCE; ++s) {
-        const int at = first + (s * THREADS + threadIdx.x) * AT_ONCE;
-        if (wide && at + AT_ONCE <= end) {
-            if constexpr (sizeof(T) == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(row + at);
-                v[4 * s] = x.x, v[4 * s + 1] = x.y, v[4 * s + 2] = x.z, v[4 * s + 3] = x.w;
+__device__ __forceinline__ Words fetch(const T* row, int first, int end, int off, int lane) {  // off: entries that a row begins behind a 16-byte boundary
+    Words w;
+    if (sizeof(T) == 2) {
+        const int at = first + 8 * lane;
+        if (off == 0 && first + RUN <= end) {
+            w.lo = *reinterpret_cast<const uint4*>(row + at);
+        } else if (first >= 8 && first + RUN + 8 <= end) {
+            const uint4* p = reinterpret_cast<const uint4*>(row + at - off);
+            const uint4 a = p[0], b = p[1];
+            const uint4 c = shifted(a, b, off >> 1);
+            if (off & 1) {
+                const unsigned next = (off >> 1) == 0 ? b.x : (off >> 1) == 1 ? b.y : (off >> 1) == 2 ? b.z : b.w;
+                w.lo = make_uint4(__funnelshift_r(c.x, c.y, 16), __funnelshift_r(c.y, c.z, 16), __funnelshift_r(c.z, c.w, 16), __funnelshift_r(c.w, next, 16));
             } else {
-                const uint4 x = *reinterpret_cast<const uint4*>(row + at);
-                const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[8 * s + 2 * i] = __uint_as_float(w[i] << 16), v[8 * s + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                w.lo = c;
             }
         } else {
+            unsigned short h[8];
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) v[AT_ONCE * s + i] = at + i < end ? to_float(row[at + i]) : -INFINITY;
+            for (int i = 0; i < 8; ++i) h[i] = at + i < end ? __bfloat16_as_ushort(reinterpret_cast<const bf16*>(row)[at + i]) : 0xff80;
+            w.lo = make_uint4(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16, h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16);
+        }
+    } else {
+        const int at = first + 4 * lane;
+        if (off == 0 && first + RUN <= end) {
+            w.lo = *reinterpret_cast<const uint4*>(row + at), w.hi = *reinterpret_cast<const uint4*>(row + at + 128);
+        } else if (first >= 4 && first + RUN + 4 <= end) {
+            const uint4* p = reinterpret_cast<const uint4*>(row + at - off);
+            const uint4 a = p[0], b = p[1], c = p[32], d = p[33];
+            w.lo = shifted(a, b, off), w.hi = shifted(c, d, off);
+        } else {
+            unsigned x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = at + (i & 3) + (i >> 2) * 128;
+                x[i] = k < end ? reinterpret_cast<const unsigned*>(row)[k] : 0xff800000u;
+            }
+            w.lo = make_uint4(x[0], x[1], x[2], x[3]), w.hi = make_uint4(x[4], x[5], x[6], x[7]);
         }
     }
+    return w;
 }
 template <typename T>
-__device__ __forceinline__ int index_of(int first, int k) {
-    constexpr int AT_ONCE = 16 / sizeof(T);
-    return first + (k / AT_ONCE * THREADS + threadIdx.x) * AT_ONCE + k % AT_ONCE;
+__device__ __forceinline__ void unpack(const Words& w, float (&v)[PER]) {
+    const unsigned a[4] = {w.lo.x, w.lo.y, w.lo.z, w.lo.w}, b[4] = {w.hi.x, w.hi.y, w.hi.z, w.hi.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 2) v[2 * i] = __uint_as_float(a[i] << 16), v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+        else v[i] = __uint_as_float(a[i]), v[4 + i] = __uint_as_float(b[i]);
+    }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
-    __shared__ Key list[ROOM];
-    __shared__ int words[THREADS / 32], fill, count;
-    __shared__ double2 parts[THREADS / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y, piece = blockIdx.x;
+    __shared__ double2 parts[WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y;
     let_next_kernel_start();
     wait_for_previous_kernels();
     const T* logits = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.stride;
-    const bool wide = ((uintptr_t)logits & 15) == 0;
-    const int from = piece * a.span, end = min(a.vocab, from + a.span);
+    const int off = (int)(((uintptr_t)logits & 15) / sizeof(T)), end_run = min(a.runs, (int)(blockIdx.x + 1) * a.piece_runs);
+    float* tops = a.tops + (size_t)row * a.runs;
     float m = -INFINITY;  // this thread's
     double sum = 0.0;
-    Key bound = 0;        // a key below it is not among the best
-    if (tid == 0) count = 0;
-    int n = 0;            // of the list, as all threads know it
-    for (int first = from; first < end; first += CHUNK) {
-        float v[PER];
-        batch(logits, first, end, wide, v);
-        float top = -INFINITY;
+    for (int run = blockIdx.x * a.piece_runs + warp; run < end_run; run += WARPS * AT_ONCE) {
+        Words w[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) v[k] = cleaned(v[k]), top = fmaxf(top, v[k]);
-        if (first == from) {
-            // the `take`-th largest of the threads' maxima
-            const unsigned mine = top == -INFINITY ? 0u : ordered(top);
-            unsigned reached = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const unsigned higher = reached | 1u << bit;
-                if (__syncthreads_count(mine >= higher) >= a.take) reached = higher;
-            }
-            bound = (Key)reached << 32;
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (run + u * WARPS < end_run) w[u] = fetch<T>(logits, (run + u * WARPS) * RUN, a.vocab, off, lane);
+            else w[u].lo = w[u].hi = sizeof(T) == 2 ? make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u) : make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
         }
-        if (top != -INFINITY && ((Key)ordered(top) << 32 | 0xffffffffu) >= bound) {
+        float v[AT_ONCE][PER], top[AT_ONCE], above = m;
+        auto tops_of = [&] {
+            above = m;
 #pragma unroll
-            for (int k = 0; k < PER; ++k) {
-                const Key key = (Key)ordered(v[k]) << 32 | (unsigned)~index_of<T>(first, k);
-                if (v[k] != -INFINITY && key >= bound) list[atomicAdd(&count, 1)] = key;
+            for (int u = 0; u < AT_ONCE; ++u) {
+                top[u] = max3(max3(v[u][0], v[u][1], v[u][2]), max3(v[u][3], v[u][4], v[u][5]), fmaxf(v[u][6], v[u][7]));
+                above = fmaxf(above, top[u]);
             }
+        };
+        auto added = [&] {
+            float part[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                part[u] = 0.f;
+#pragma unroll
+                for (int k = 0; k < PER; ++k) part[u] += fast_exp2((v[u][k] - above) * LOG2E);
+            }
+            float all = 0.f;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) all += part[u];
+            return all;
+        };
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) unpack<T>(w[u], v[u]);
+        tops_of();
+        float part = added();
+        if (!(part < INFINITY)) {  // a NaN, an infinity, or nothing but -infinity
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                for (int k = 0; k < PER; ++k) v[u][k] = cleaned(v[u][k]);
+            tops_of();
+            part = above == -INFINITY ? 0.f : added();
         }
-        if (top != -INFINITY) {
-            const float above = fmaxf(m, top);
-            if (above > m) sum *= m == -INFINITY ? 0.0 : (double)fast_exp2((m - above) * 1.4426950408889634f);
+        if (above > m) {
+            sum *= m == -INFINITY ? 0.0 : (double)fast_exp2((m - above) * LOG2E);
             m = above;
-            float part = 0.f;
-#pragma unroll
-            for (int k = 0; k < PER; ++k) part += fast_exp2((v[k] - above) * 1.4426950408889634f);
-            sum += part;
         }
-        __syncthreads();
-        n = count;
-        __syncthreads();
-        if (n > ROOM - CHUNK || (n > a.take && first + CHUNK >= end) || (first == from && n >= a.take) || n > 2 * a.take + 32) {
-            n = cut_back(list, n, a.take, words, &fill);
-            if (n == a.take) {  // the smallest of them is the new bound
-                Key smallest = ~0ull;
-                for (int i = lane; i < n; i += 32) smallest = list[i] < smallest ? list[i] : smallest;
+        sum += part;
 #pragma unroll
-                for (int offset = 16; offset > 0; offset >>= 1) {
-                    const Key other = __shfl_xor_sync(0xffffffffu, smallest, offset);
-                    smallest = other < smallest ? other : smallest;
-                }
-                bound = smallest;
-            }
-            if (tid == 0) count = n;
-            __syncthreads();
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const float largest = warp_largest(top[u]);
+            if (lane == 0 && run + u * WARPS < end_run) tops[run + u * WARPS] = largest;
         }
     }
-    Key* best = a.best + ((size_t)row * a.pieces + piece) * a.take;
-    for (int i = tid; i < a.take; i += THREADS) best[i] = i < n ? list[i] : 0;
     // the threads' sums, below the block's maximum, in the order of the threads
     const float above = warp_max(m);
-    double part = m == -INFINITY ? 0.0 : sum * (double)fast_exp2((m - above) * 1.4426950408889634f);
+    double part = m == -INFINITY ? 0.0 : sum * (double)fast_exp2((m - above) * LOG2E);
 #pragma unroll
     for (int offset = 16; offset > 0; offset >>= 1) part += __shfl_xor_sync(0xffffffffu, part, offset);
     if (lane == 0) parts[warp] = make_double2(above, part);
     __syncthreads();
     if (tid == 0) {
         double top = -INFINITY, all = 0.0;
-        for (int w = 0; w < THREADS / 32; ++w) top = fmax(top, parts[w].x);
-        for (int w = 0; w < THREADS / 32; ++w) all += parts[w].x == -INFINITY ? 0.0 : parts[w].y * exp(parts[w].x - top);
-        a.sums[(size_t)row * a.pieces + piece] = make_double2(top, all);
+        for (int w = 0; w < WARPS; ++w) top = fmax(top, parts[w].x);
+        for (int w = 0; w < WARPS; ++w) all += parts[w].x == -INFINITY ? 0.0 : parts[w].y * (double)fast_exp2((float)(parts[w].x - top) * LOG2E);
+        a.sums[(size_t)row * a.pieces + blockIdx.x] = make_double2(top, all);
     }
 }
 
-// The second kernel: block = group.  Shared memory: the candidates' values, and the numbers of those that reach the last of the best.
-constexpr int GROUP_THREADS = 512, MOST_BEAMS = 32, MOST_CANDIDATES = 12288;
+// The second kernel: block = group.
+constexpr int GROUP_THREADS = 1024, MOST_RUNS = 256, MOST_CANDIDATES = GROUP_THREADS;
+struct Best {
+    Key value;
+    long long place;  // (beam, run or token): of equal values the lowest
+};
+__device__ __forceinline__ bool before(const Best& a, const Best& b) { return a.value > b.value || (a.value == b.value && a.place < b.place); }
+// The best of the block, in every thread.
+__device__ Best best_of_block(Best mine, Best* words) {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) {
+        const Best other{__shfl_xor_sync(0xffffffffu, mine.value, offset), __shfl_xor_sync(0xffffffffu, mine.place, offset)};
+        if (before(other, mine)) mine = other;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    Best best = words[0];
+    for (int w = 1; w < GROUP_THREADS / 32; ++w)
+        if (before(words[w], best)) best = words[w];
+    return best;
+}
+
+template <typename T>
 __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a) {
-    extern __shared__ Key values[];
-    int* reaching = reinterpret_cast<int*>(values + a.beams * a.pieces * a.take);
     __shared__ double offset[MOST_BEAMS];
-    __shared__ int words[GROUP_THREADS / 32], count;
-    const int tid = threadIdx.x, group = blockIdx.x, per_row = a.pieces * a.take, n = a.beams * per_row;
+    __shared__ Best words[GROUP_THREADS / 32];
+    __shared__ Best candidates[MOST_CANDIDATES];
+    __shared__ int chosen[MOST_RUNS], n_chosen, n_candidates;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = blockIdx.x, n = a.beams * a.runs;
     let_next_kernel_start();
     wait_for_previous_kernels();
-    const Key* best = a.best + (size_t)group * n;
-    if (tid < a.beams) {
-        const double2* sums = a.sums + ((size_t)group * a.beams + tid) * a.pieces;
+    const float* tops = a.tops + (size_t)group * n;
+    if (warp < a.beams) {  // a warp a beam
+        const double2* sums = a.sums + ((size_t)group * a.beams + warp) * a.pieces;
         double top = -INFINITY, all = 0.0;
-        for (int p = 0; p < a.pieces; ++p) top = fmax(top, sums[p].x);
-        for (int p = 0; p < a.pieces; ++p) all += sums[p].x == -INFINITY ? 0.0 : sums[p].y * exp(sums[p].x - top);
-        const float score = cleaned(a.scores[group * a.beams + tid]);
-        offset[tid] = score == -INFINITY || top == -INFINITY ? -INFINITY : (double)score - (top + log(all));
-    }
-    if (tid == 0) count = 0;
-    __syncthreads();
-    int there = 0;
-    for (int i = tid; i < n; i += GROUP_THREADS) {
-        const Key key = best[i];
-        const double off = offset[i / per_row];
-        const Key value = key && off != -INFINITY ? ordered((double)value_of((unsigned)(key >> 32)) + off) : 0;
-        values[i] = value;
-        there += value != 0;
-    }
-    there = block_count(there, words);
-    const int take = min(a.take, there);
-    Key last = 0;  // the largest number that `take` values reach
-    if (there > take) {
-        for (int bit = 63; bit >= 0; --bit) {
-            const Key higher = last | 1ull << bit;
-            int reach = 0;
-            for (int i = tid; i < n; i += GROUP_THREADS) reach += values[i] >= higher;
-            if (block_count(reach, words) >= take) last = higher;
+        for (int p = lane; p < a.pieces; p += 32) {
+            const double2 part = sums[p];
+            const double higher = fmax(top, part.x);
+            if (higher != -INFINITY) all = (top == -INFINITY ? 0.0 : all * (double)fast_exp2((float)(top - higher) * LOG2E)) + (part.x == -INFINITY ? 0.0 : part.y * (double)fast_exp2((float)(part.x - higher) * LOG2E));
+            top = higher;
+        }
+        const float above = warp_max((float)top);  // a logit, which float holds
+        all = top == -INFINITY ? 0.0 : all * (double)fast_exp2(((float)top - above) * LOG2E);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (lane == 0) {
+            const float score = cleaned(a.scores[group * a.beams + warp]);
+            offset[warp] = score == -INFINITY || above == -INFINITY ? -INFINITY : (double)score - ((double)above + log(all));
         }
     }
+    if (tid == 0) n_chosen = n_candidates = 0;
     __syncthreads();
-    // those that reach it, and their places: the number of those before them
+    auto score_of = [&](float logit, double off) -> Key { return logit == -INFINITY || off == -INFINITY ? 0 : ordered((double)logit + off); };
+    auto short_of = [&](Key value) -> unsigned { return value ? ordered((float)value_of(value)) : 0u; };  // never falls as the value grows
+    // the runs: a bound that the best of at least `take` of them reach, if there are so many
+    unsigned mine = 0;
+#pragma unroll 4
+    for (int i = tid; i < n; i += GROUP_THREADS) mine = max(mine, short_of(score_of(tops[i], offset[i / a.runs])));
+    unsigned bound = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned higher = bound | 1u << bit;
+        if (__syncthreads_count(mine >= higher) >= a.take) bound = higher;
+    }
+    bound = max(bound, 1u);
+#pragma unroll 4
     for (int i = tid; i < n; i += GROUP_THREADS)
-        if (values[i] != 0 && values[i] >= last) reaching[atomicAdd(&count, 1)] = i;
-    __syncthreads();
-    auto place_of = [&](int i) { return ((long long)(i / per_row) << 32) | (unsigned)~(unsigned)best[i]; };  // (beam, token)
-    for (int k = tid; k < count; k += GROUP_THREADS) {
-        const int i = reaching[k];
-        const Key value = values[i];
-        const long long place = place_of(i);
-        int before = 0;
-        for (int c = 0; c < count; ++c) {
-            const int j = reaching[c];
-            const Key other = values[j];
-            before += other > value || (other == value && j != i && place_of(j) < place);
+        if (short_of(score_of(tops[i], offset[i / a.runs])) >= bound) {
+            const int at = atomicAdd(&n_chosen, 1);
+            if (at < MOST_RUNS) chosen[at] = i;
         }
-        if (before < take) {
-            const size_t at = (size_t)group * a.take + before;
-            a.parents[at] = i / per_row, a.tokens[at] = (int)(unsigned)place, a.out_scores[at] = (float)value_of(value);
+    __syncthreads();
+    int n_runs = n_chosen;
+    if (n_runs > MOST_RUNS) {  // many equal ones: the `take` best, one after the other
+        Best last{~0ull, -1};
+        for (n_runs = 0; n_runs < a.take; ++n_runs) {
+            Best best{0, 0x7fffffffffffffffll};
+            for (int i = tid; i < n; i += GROUP_THREADS) {
+                const Best here{score_of(tops[i], offset[i / a.runs]), i};
+                if (here.value && before(last, here) && before(here, best)) best = here;
+            }
+            last = best_of_block(best, words);
+            if (!last.value) break;
+            if (tid == 0) chosen[n_runs] = (int)last.place;
+            __syncthreads();
         }
     }
-    for (int i = take + tid; i < a.take; i += GROUP_THREADS) {
+    // their entries that reach it
+    auto entry = [&](int i, int k) -> Best {  // entry k of chosen run i
+        const int run = chosen[i], beam = run / a.runs, token = (run - beam * a.runs) * RUN + k;
+        if (token >= a.vocab) return {0, 0};
+        const float logit = cleaned(to_float(reinterpret_cast<const T*>(a.logits)[(size_t)(group * a.beams + beam) * a.stride + token]));
+        return {score_of(logit, offset[beam]), (long long)beam << 32 | token};
+    };
+    for (int i = warp; i < n_runs; i += GROUP_THREADS / 32) {
+        Best e[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) e[k] = entry(i, k * 32 + lane);
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (e[k].value && short_of(e[k].value) >= bound) {
+                const int at = atomicAdd(&n_candidates, 1);
+                if (at < MOST_CANDIDATES) candidates[at] = e[k];
+            }
+    }
+    __syncthreads();
+    const int found = n_candidates;
+    int written = min(a.take, found);
+    auto write = [&](int place, const Best& best) {
+        const size_t at = (size_t)group * a.take + place;
+        a.parents[at] = (int)(best.place >> 32), a.tokens[at] = (int)best.place, a.out_scores[at] = (float)value_of(best.value);
+    };
+    if (found <= MOST_CANDIDATES) {
+        if (tid < found) {
+            const Best me = candidates[tid];
+            int ahead = 0;
+            for (int i = 0; i < found; ++i) ahead += before(candidates[i], me);
+            if (ahead < a.take) write(ahead, me);
+        }
+    } else {  // one after the other
+        Best last{~0ull, -1};
+        for (written = 0; written < a.take; ++written) {
+            Best best{0, 0x7fffffffffffffffll};
+            for (int i = warp; i < n_runs; i += GROUP_THREADS / 32)
+                for (int k = lane; k < RUN; k += 32) {
+                    const Best here = entry(i, k);
+                    if (here.value && before(last, here) && before(here, best)) best = here;
+                }
+            last = best_of_block(best, words);
+            if (!last.value) break;
+            if (tid == 0) write(written, last);
+        }
+    }
+    for (int i = written + tid; i < a.take; i += GROUP_THREADS) {
         const size_t at = (size_t)group * a.take + i;
         a.parents[at] = -1, a.tokens[at] = -1, a.out_scores[at] = -INFINITY;
     }
 }
+template <typename T>
+int launch(const Args& a, cudaStream_t stream) {
+    if (int code = launch_after_previous(beam_rows_kernel<T>, dim3(a.pieces, a.groups * a.beams), dim3(THREADS), 0, stream, a)) return code;
+    return launch_after_previous(beam_group_kernel<T>, dim3(a.groups), dim3(GROUP_THREADS), 0, stream, a);
+}
 }  // namespace
 
-// Into how many pieces rows are cut: what fills the device, four blocks a multiprocessor, and no more candidates of a group than the second kernel holds.
-static int pieces_for(int groups, int beams, int vocab, int take, int sms) {
-    const long long chunks = (vocab + CHUNK - 1) / CHUNK, room = 4LL * sms / ((long long)groups * beams), most = MOST_CANDIDATES / ((long long)beams * take);
+// Into how many pieces rows are cut, and runs of a piece: what fills the device, six blocks a multiprocessor, of two looks of its warps at least.
+static int pieces_for(int rows, int vocab, int sms, int* piece_runs) {
+    const long long runs = (vocab + RUN - 1) / RUN, room = 6LL * sms / rows, most = (runs + 2 * WARPS * AT_ONCE - 1) / (2 * WARPS * AT_ONCE);
     long long n = room < 1 ? 1 : room;
-    n = n < chunks ? n : chunks;
     n = n < most ? n : most;
-    const long long span = (chunks + n - 1) / n;
-    return (int)((chunks + span - 1) / span);
+    const long long each = ((runs + n - 1) / n + WARPS * AT_ONCE - 1) / (WARPS * AT_ONCE) * (WARPS * AT_ONCE);
+    *piece_runs = (int)each;
+    return (int)((runs + each - 1) / each);
 }
 // Bytes of scratch that hb_beam_select takes.
 HB_EXPORT long long hb_beam_select_scratch(int groups, int beams, int vocab, int take, int sms) {
-    if (groups <= 0 || beams <= 0 || beams > MOST_BEAMS || vocab <= 0 || take <= 0 || take > MOST_TAKE || sms <= 0) return 0;
-    return (long long)groups * beams * pieces_for(groups, beams, vocab, take, sms) * (16 + 8 * take);
+    if (groups <= 0 || beams <= 0 || beams > MOST_BEAMS || vocab <= 0 || vocab > 0x7fffffff - RUN || take <= 0 || take > MOST_TAKE || sms <= 0) return 0;
+    const long long rows = (long long)groups * beams;
+    if (rows > 65535) return 0;
+    int piece_runs;
+    return rows * pieces_for((int)rows, vocab, sms, &piece_runs) * 16 + rows * ((vocab + RUN - 1) / RUN) * 4;
 }
 // logits [groups * beams, vocab] (bfloat16 or float) with rows `stride` apart; scores [groups, beams]; parents, tokens, out_scores [groups, take].  scratch: hb_beam_select_scratch bytes on a
 // 16-byte boundary.
@@ -293,14 +368,11 @@ HB_EXPORT int hb_beam_select(const void* logits, int is_bf16, long long stride, 
                              void* scratch, cudaStream_t stream) {
     if (groups <= 0) return 0;
     if (!logits || !scores || !parents || !tokens || !out_scores || !scratch || beams <= 0 || vocab <= 0 || take <= 0 || sms <= 0 || stride < vocab || ((uintptr_t)scratch & 15)) return HB_BAD_ARGUMENT;
-    if (beams > MOST_BEAMS || take > MOST_TAKE || (long long)groups * beams > 65535 || vocab > 0x7fffffff - 2 * CHUNK) return HB_UNSUPPORTED_SIZE;
-    const int pieces = pieces_for(groups, beams, vocab, take, sms), chunks = (vocab + CHUNK - 1) / CHUNK;
-    const size_t rows = (size_t)groups * beams;
-    double2* sums = (double2*)scratch;
-    const Args a{logits, stride, scores, groups, beams, vocab, take, pieces, (chunks + pieces - 1) / pieces * CHUNK, (Key*)(sums + rows * pieces), sums, parents, tokens, out_scores};
-    if (int code = launch_after_previous(is_bf16 ? beam_rows_kernel<bf16> : beam_rows_kernel<float>, dim3(pieces, (unsigned)rows), dim3(THREADS), 0, stream, a)) return code;
-    const size_t shared = (size_t)beams * pieces * take * 12;
-    const cudaError_t configured = cudaFuncSetAttribute(beam_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_CANDIDATES * 12);
-    if (configured != cudaSuccess) return (int)configured;
-    return launch_after_previous(beam_group_kernel, dim3(groups), dim3(GROUP_THREADS), shared, stream, a);
+    if (((uintptr_t)logits & (is_bf16 ? 1 : 3))) return HB_BAD_ARGUMENT;
+    const long long rows = (long long)groups * beams, runs = ((long long)vocab + RUN - 1) / RUN;
+    if (beams > MOST_BEAMS || take > MOST_TAKE || rows > 65535 || vocab > 0x7fffffff - RUN || beams * runs > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
+    Args a{logits, stride, scores, groups, beams, vocab, take, (int)runs};
+    a.pieces = pieces_for((int)rows, vocab, sms, &a.piece_runs);
+    a.sums = (double2*)scratch, a.tops = (float*)(a.sums + rows * a.pieces), a.parents = parents, a.tokens = tokens, a.out_scores = out_scores;
+    return is_bf16 ? launch<bf16>(a, stream) : launch<float>(a, stream);
 }

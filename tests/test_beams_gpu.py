@@ -12,16 +12,29 @@ from hyperion_b200.sampling import beam_select, reference_beam_select
 pytestmark = pytest.mark.gpu
 
 
+UNDECIDED = 2.0 ** -20
+
+
 def check_selection(logits, scores, take):
+    """Every place holds the continuation that the rule puts there.  A row's sum is made of terms that are off by 2^-22 each at most (the exponential of the hardware) and float sums of 16 of them (2^-22 on top, at the
+    very most), so its logarithm is off by less than 2^-21, and scores of two rows that lie closer than 2^-20 come in either order; within a row the order is that of the logits, to the bit."""
     choice = beam_select(logits, scores, take)
     groups, beams = scores.shape
     z = logits.float().cpu().numpy().reshape(groups, beams, -1)
     for g in range(groups):
-        want = reference_beam_select(z[g], scores[g].cpu().numpy(), take)
+        more = reference_beam_select(z[g], scores[g].cpu().numpy(), take + 64)
+        want, score_of = more[:take], {(b, v): score for b, v, score in more}
         got = list(zip(choice.parents[g].tolist(), choice.tokens[g].tolist()))
-        assert got == [(b, v) for b, v, _ in want] + [(-1, -1)] * (take - len(want))
-        for place, (_, _, score) in enumerate(want):
-            # the score is rounded once to float32; the row's sum is made of terms that are off by some 2^-21 at most, which is as much of its logarithm
+        assert got[len(want):] == [(-1, -1)] * (take - len(want)) and len(set(got[: len(want)])) == len(want)
+        for (b, v), (wanted_b, wanted_v, score) in zip(got, want):
+            assert (b, v) == (wanted_b, wanted_v) or (b != wanted_b and abs(score_of[b, v] - score) < UNDECIDED) or abs(score_of[b, v] - score) < UNDECIDED and any(
+                x != b and abs(s - score) < UNDECIDED for (x, _), s in score_of.items()), (got, want)
+        for beam in range(beams):  # within a beam: the best of its own, in their order
+            mine = [v for b, v in got if b == beam]
+            assert mine == [v for b, v, _ in more if b == beam][: len(mine)]
+        for place, (b, v) in enumerate(got[: len(want)]):
+            # the score is rounded once to float32
+            score = score_of[b, v]
             assert abs(choice.scores[g, place].item() - score) <= abs(score) * 2.0 ** -24 + 2.0 ** -21
         assert all(s == float("-inf") for s in choice.scores[g, len(want):].tolist())
     return choice
@@ -55,6 +68,8 @@ def test_equal_scores_go_to_the_lowest_beam_and_token():
     scores = torch.zeros(2, 3, device="cuda")
     choice = check_selection(logits, scores, 20)
     assert choice.parents.tolist() == [[0] * 20] * 2 and choice.tokens.tolist() == [list(range(20))] * 2
+    choice = check_selection(torch.full((4, 70000), -3.5, device="cuda"), torch.tensor([[-2.0, -1.0, -1.0, -3.0]], device="cuda"), 64)
+    assert choice.parents.tolist() == [[1] * 64] and choice.tokens.tolist() == [list(range(64))]
     logits, _ = some_logits(1, 1, 9001)  # beams that hold the same, at addresses that are aligned differently
     same = torch.empty(4, 9001, device="cuda").copy_(logits)
     choice = check_selection(same, torch.zeros(1, 4, device="cuda"), 8)
