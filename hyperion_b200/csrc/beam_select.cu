@@ -4,22 +4,24 @@
 //
 // The first kernel reads every row once and leaves the sum, and the maximum of every run of 256 logits.  The second has a block per group: with the rows' sums it knows every run's best score.  The runs whose best
 // are the `take` best of all runs hold the `take` best continuations (of a run that is not among them, `take` others hold something better), so only those are read again: a few KB of them.  Both
-// searches take a bound first, the `take`-th largest of what the threads have each found to be their best, and then look at what reaches it: little more than `take` in all but contrived rows, for which there is a way that goes by one
+// searches take a bound first, the `take`-th largest of what eighths of the warps have found to be their best, and then look at what reaches it: little more than `take` in all but contrived rows, for which there is a way that goes by one
 // continuation after the other.
 //
-// Scores are compared as float64: a score is score_b - lse_b, a number of the row, plus the logit, and float32 would make ties of scores that are not equal.  Sums of a thread's 16 entries are float, everything above
+// Scores are compared as float64: a score is score_b - lse_b, a number of the row, plus the logit, and float32 would make ties of scores that are not equal.  Sums of a thread's 32 entries are float, everything above
 // them float64; exponentials are the hardware's (2^-22 of a term).  Which thread adds up what goes by the entry's index alone, not by the row's alignment, so rows that hold the same have the same sums.
 //
 // A NaN counts as -infinity, +infinity as the largest number.  A logit of -infinity, and everything of a beam whose score is -infinity or NaN, is no candidate.  A place without a candidate has parent -1,
 // token -1 and score -infinity.
 #include <float.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace {
 typedef __nv_bfloat16 bf16;
 typedef unsigned long long Key;  // a float64's bits in its order; 0: none
-constexpr int THREADS = 256, WARPS = THREADS / 32, RUN = 256, PER = RUN / 32, AT_ONCE = 2;  // a warp looks at AT_ONCE runs at a time, PER entries a lane of each
+constexpr int THREADS = 256, WARPS = THREADS / 32, RUN = 256, PER = RUN / 32, AT_ONCE = 4;  // a warp looks at AT_ONCE runs at a time, PER entries a lane of each
 constexpr int MOST_TAKE = 64, MOST_BEAMS = 32;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -50,6 +52,20 @@ __device__ __forceinline__ Key ordered(double v) {
 }
 __device__ __forceinline__ double value_of(Key o) { return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o)); }
 
+// Two floats at a time.
+struct Pair { float x, y; };
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("{.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 struct Args {
     const void* logits; long long stride;
     const float* scores;
@@ -69,12 +85,12 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int wor
     if (words & 1) r = make_uint4(r.y, r.z, r.w, s0);
     return r;
 }
-template <typename T>
-__device__ __forceinline__ Words fetch(const T* row, int first, int end, int off, int lane) {  // off: entries that a row begins behind a 16-byte boundary
+template <typename T, bool PLAIN>
+__device__ __forceinline__ Words fetch(const T* row, int first, int end, int off, int lane) {  // off: entries that a row begins behind a 16-byte boundary; PLAIN: none, and the run is whole
     Words w;
     if (sizeof(T) == 2) {
         const int at = first + 8 * lane;
-        if (off == 0 && first + RUN <= end) {
+        if (PLAIN || (off == 0 && first + RUN <= end)) {
             w.lo = *reinterpret_cast<const uint4*>(row + at);
         } else if (first >= 8 && first + RUN + 8 <= end) {
             const uint4* p = reinterpret_cast<const uint4*>(row + at - off);
@@ -94,7 +110,7 @@ __device__ __forceinline__ Words fetch(const T* row, int first, int end, int off
         }
     } else {
         const int at = first + 4 * lane;
-        if (off == 0 && first + RUN <= end) {
+        if (PLAIN || (off == 0 && first + RUN <= end)) {
             w.lo = *reinterpret_cast<const uint4*>(row + at), w.hi = *reinterpret_cast<const uint4*>(row + at + 128);
         } else if (first >= 4 && first + RUN + 4 <= end) {
             const uint4* p = reinterpret_cast<const uint4*>(row + at - off);
@@ -133,11 +149,12 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     float* tops = a.tops + (size_t)row * a.runs;
     float m = -INFINITY;  // this thread's
     double sum = 0.0;
-    for (int run = blockIdx.x * a.piece_runs + warp; run < end_run; run += WARPS * AT_ONCE) {
+    auto look = [&](int run, auto plain) {
+        constexpr bool PLAIN = decltype(plain)::value;
         Words w[AT_ONCE];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
-            if (run + u * WARPS < end_run) w[u] = fetch<T>(logits, (run + u * WARPS) * RUN, a.vocab, off, lane);
+            if (PLAIN || run + u * WARPS < end_run) w[u] = fetch<T, PLAIN>(logits, (run + u * WARPS) * RUN, a.vocab, off, lane);
             else w[u].lo = w[u].hi = sizeof(T) == 2 ? make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u) : make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
         }
         float v[AT_ONCE][PER], top[AT_ONCE], above = m;
@@ -149,30 +166,34 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
                 above = fmaxf(above, top[u]);
             }
         };
-        auto added = [&] {
-            float part[AT_ONCE];
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) {
-                part[u] = 0.f;
-#pragma unroll
-                for (int k = 0; k < PER; ++k) part[u] += fast_exp2((v[u][k] - above) * LOG2E);
-            }
-            float all = 0.f;
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) all += part[u];
-            return all;
-        };
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) unpack<T>(w[u], v[u]);
         tops_of();
-        float part = added();
-        if (!(part < INFINITY)) {  // a NaN, an infinity, or nothing but -infinity
+        // 2^(v log2 e + offset) * rest: the offset's rounding is an error of the exponent that all entries share, and what it has been rounded by is a float, too
+        const float offset = -above * LOG2E, rest = fast_exp2(-fmaf(above, LOG2E, offset));
+        Pair parts[4] = {};
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int k = 0; k < PER; k += 2) {
+                const Pair y = fma2(Pair{v[u][k], v[u][k + 1]}, Pair{LOG2E, LOG2E}, Pair{offset, offset});
+                parts[k / 2] = add2(parts[k / 2], Pair{fast_exp2(y.x), fast_exp2(y.y)});
+            }
+        const Pair half = add2(add2(parts[0], parts[1]), add2(parts[2], parts[3]));
+        float part = (half.x + half.y) * rest;
+        if (!(part < INFINITY) || !(fabsf(offset) < 0x1p24f)) {  // a NaN, an infinity, nothing but -infinity, or a maximum whose offset is too large to be precise
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
                 for (int k = 0; k < PER; ++k) v[u][k] = cleaned(v[u][k]);
             tops_of();
-            part = above == -INFINITY ? 0.f : added();
+            part = 0.f;
+            if (above != -INFINITY) {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                    for (int k = 0; k < PER; ++k) part += fast_exp2((v[u][k] - above) * LOG2E);
+            }
         }
         if (above > m) {
             sum *= m == -INFINITY ? 0.0 : (double)fast_exp2((m - above) * LOG2E);
@@ -182,9 +203,14 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
             const float largest = warp_largest(top[u]);
-            if (lane == 0 && run + u * WARPS < end_run) tops[run + u * WARPS] = largest;
+            if (lane == 0 && (PLAIN || run + u * WARPS < end_run)) tops[run + u * WARPS] = largest;
         }
-    }
+    };
+    // the runs that a look has whole, in a loop that asks no more questions
+    const int whole = min(end_run, off ? 0 : a.vocab / RUN);
+    int run = blockIdx.x * a.piece_runs + warp;
+    for (; run + (AT_ONCE - 1) * WARPS < whole; run += WARPS * AT_ONCE) look(run, std::true_type{});
+    for (; run < end_run; run += WARPS * AT_ONCE) look(run, std::false_type{});
     // the threads' sums, below the block's maximum, in the order of the threads
     const float above = warp_max(m);
     double part = m == -INFINITY ? 0.0 : sum * (double)fast_exp2((m - above) * LOG2E);
@@ -201,7 +227,8 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
 }
 
 // The second kernel: block = group.
-constexpr int GROUP_THREADS = 1024, MOST_RUNS = 256, MOST_CANDIDATES = GROUP_THREADS;
+constexpr int GROUP_THREADS = 1024, MOST_RUNS = 256, MOST_CANDIDATES = GROUP_THREADS, BESTS = GROUP_THREADS / 8;
+static_assert(BESTS >= MOST_TAKE, "as many as are wanted");
 struct Best {
     Key value;
     long long place;  // (beam, run or token): of equal values the lowest
@@ -228,6 +255,8 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     __shared__ double offset[MOST_BEAMS];
     __shared__ Best words[GROUP_THREADS / 32];
     __shared__ Best candidates[MOST_CANDIDATES];
+    __shared__ __align__(16) unsigned bests[BESTS];
+    __shared__ unsigned shared_bound;
     __shared__ int chosen[MOST_RUNS], n_chosen, n_candidates;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = blockIdx.x, n = a.beams * a.runs;
     let_next_kernel_start();
@@ -255,21 +284,36 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     __syncthreads();
     auto score_of = [&](float logit, double off) -> Key { return logit == -INFINITY || off == -INFINITY ? 0 : ordered((double)logit + off); };
     auto short_of = [&](Key value) -> unsigned { return value ? ordered((float)value_of(value)) : 0u; };  // never falls as the value grows
-    // the runs: a bound that the best of at least `take` of them reach, if there are so many
+    // the runs: a bound that the best of at least `take` of them reach, if there are so many: the `take`-th largest of what eight lanes together have as theirs
+    const int team = GROUP_THREADS / 32 / a.beams, beam_here = warp / team;  // warps of a beam
+    const int first_run = (warp - beam_here * team) * 32 + lane;
+    const double off_here = beam_here < a.beams ? offset[beam_here] : -INFINITY;
+    const float* row_tops = tops + (size_t)(beam_here < a.beams ? beam_here : 0) * a.runs;
+    const int runs_here = beam_here < a.beams ? a.runs : 0;
     unsigned mine = 0;
 #pragma unroll 4
-    for (int i = tid; i < n; i += GROUP_THREADS) mine = max(mine, short_of(score_of(tops[i], offset[i / a.runs])));
-    unsigned bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned higher = bound | 1u << bit;
-        if (__syncthreads_count(mine >= higher) >= a.take) bound = higher;
+    for (int i = first_run; i < runs_here; i += team * 32) mine = max(mine, short_of(score_of(row_tops[i], off_here)));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if ((lane & 7) == 0) bests[tid / 8] = mine;
+    __syncthreads();
+    if (tid < BESTS) {
+        const unsigned me = bests[tid];
+        int ahead = 0;  // equal ones by their number
+#pragma unroll 8
+        for (int i = 0; i < BESTS; i += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(bests + i);
+            ahead += (x.x > me || (x.x == me && i < tid)) + (x.y > me || (x.y == me && i + 1 < tid)) + (x.z > me || (x.z == me && i + 2 < tid)) + (x.w > me || (x.w == me && i + 3 < tid));
+        }
+        if (ahead == a.take - 1) shared_bound = max(me, 1u);
     }
-    bound = max(bound, 1u);
+    __syncthreads();
+    const unsigned bound = shared_bound;
 #pragma unroll 4
-    for (int i = tid; i < n; i += GROUP_THREADS)
-        if (short_of(score_of(tops[i], offset[i / a.runs])) >= bound) {
+    for (int i = first_run; i < runs_here; i += team * 32)
+        if (short_of(score_of(row_tops[i], off_here)) >= bound) {
             const int at = atomicAdd(&n_chosen, 1);
-            if (at < MOST_RUNS) chosen[at] = i;
+            if (at < MOST_RUNS) chosen[at] = beam_here * a.runs + i;
         }
     __syncthreads();
     int n_runs = n_chosen;
