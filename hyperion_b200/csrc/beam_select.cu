@@ -42,10 +42,6 @@ __device__ __forceinline__ float warp_largest(float v) {
     return d;
 }
 // Order-preserving for all numbers; both zeros are the same.
-__device__ __forceinline__ unsigned ordered(float v) {
-    const unsigned b = __float_as_uint(v + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
 __device__ __forceinline__ Key ordered(double v) {
     const Key b = (Key)__double_as_longlong(v + 0.0);
     return b >> 63 ? ~b : b | 1ull << 63;
@@ -227,7 +223,7 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
 }
 
 // The second kernel: block = group.
-constexpr int GROUP_THREADS = 1024, MOST_RUNS = 256, MOST_CANDIDATES = GROUP_THREADS, BESTS = GROUP_THREADS / 8;
+constexpr int GROUP_THREADS = 1024, MOST_RUNS = 256, MOST_CANDIDATES = GROUP_THREADS, BESTS = GROUP_THREADS / 8, EARLY = 6;
 static_assert(BESTS >= MOST_TAKE, "as many as are wanted");
 struct Best {
     Key value;
@@ -255,15 +251,22 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     __shared__ double offset[MOST_BEAMS];
     __shared__ Best words[GROUP_THREADS / 32];
     __shared__ Best candidates[MOST_CANDIDATES];
-    __shared__ __align__(16) unsigned bests[BESTS];
-    __shared__ unsigned shared_bound;
+    __shared__ __align__(16) float bests[BESTS];
+    __shared__ float shared_bound;
     __shared__ int chosen[MOST_RUNS], n_chosen, n_candidates;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = blockIdx.x, n = a.beams * a.runs;
     let_next_kernel_start();
     wait_for_previous_kernels();
     const float* tops = a.tops + (size_t)group * n;
+    // a beam's runs are a team of warps'; a thread's first ones are on their way while the sums are put together
+    const int team = GROUP_THREADS / 32 / a.beams, beam_here = warp / team, runs_here = beam_here < a.beams ? a.runs : 0, first_run = (warp - beam_here * team) * 32 + lane;
+    const float* row_tops = tops + (size_t)(beam_here < a.beams ? beam_here : 0) * a.runs;
+    float early[EARLY];
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) early[k] = first_run + k * team * 32 < runs_here ? row_tops[first_run + k * team * 32] : -INFINITY;
     if (warp < a.beams) {  // a warp a beam
         const double2* sums = a.sums + ((size_t)group * a.beams + warp) * a.pieces;
+        const float score = cleaned(a.scores[group * a.beams + warp]);
         double top = -INFINITY, all = 0.0;
         for (int p = lane; p < a.pieces; p += 32) {
             const double2 part = sums[p];
@@ -271,50 +274,55 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
             if (higher != -INFINITY) all = (top == -INFINITY ? 0.0 : all * (double)fast_exp2((float)(top - higher) * LOG2E)) + (part.x == -INFINITY ? 0.0 : part.y * (double)fast_exp2((float)(part.x - higher) * LOG2E));
             top = higher;
         }
-        const float above = warp_max((float)top);  // a logit, which float holds
+        const float above = warp_largest((float)top);  // a logit, which float holds
         all = top == -INFINITY ? 0.0 : all * (double)fast_exp2(((float)top - above) * LOG2E);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-        if (lane == 0) {
-            const float score = cleaned(a.scores[group * a.beams + warp]);
-            offset[warp] = score == -INFINITY || above == -INFINITY ? -INFINITY : (double)score - ((double)above + log(all));
-        }
+        if (lane == 0) offset[warp] = score == -INFINITY || above == -INFINITY ? -INFINITY : (double)score - ((double)above + log(all));
     }
     if (tid == 0) n_chosen = n_candidates = 0;
     __syncthreads();
     auto score_of = [&](float logit, double off) -> Key { return logit == -INFINITY || off == -INFINITY ? 0 : ordered((double)logit + off); };
-    auto short_of = [&](Key value) -> unsigned { return value ? ordered((float)value_of(value)) : 0u; };  // never falls as the value grows
-    // the runs: a bound that the best of at least `take` of them reach, if there are so many: the `take`-th largest of what eight lanes together have as theirs
-    const int team = GROUP_THREADS / 32 / a.beams, beam_here = warp / team;  // warps of a beam
-    const int first_run = (warp - beam_here * team) * 32 + lane;
-    const double off_here = beam_here < a.beams ? offset[beam_here] : -INFINITY;
-    const float* row_tops = tops + (size_t)(beam_here < a.beams ? beam_here : 0) * a.runs;
-    const int runs_here = beam_here < a.beams ? a.runs : 0;
-    unsigned mine = 0;
-#pragma unroll 4
-    for (int i = first_run; i < runs_here; i += team * 32) mine = max(mine, short_of(score_of(row_tops[i], off_here)));
+    // The runs: a bound that the best of at least `take` of them reach, if there are so many: the `take`-th largest of what eight lanes together have as theirs.  In float: what is added up there is off by 2^-24 of the
+    // offset and of itself, so the bound is lowered by 2^-21 of both, and whatever scores as much as the `take`-th best in earnest reaches it.
+    const float off_here = beam_here < a.beams ? (float)offset[beam_here] : -INFINITY;
+    float mine = -INFINITY;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    for (int k = 0; k < EARLY; ++k) mine = fmaxf(mine, early[k] + off_here);
+    for (int i = first_run + EARLY * team * 32; i < runs_here; i += team * 32) mine = fmaxf(mine, row_tops[i] + off_here);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
     if ((lane & 7) == 0) bests[tid / 8] = mine;
     __syncthreads();
-    if (tid < BESTS) {
-        const unsigned me = bests[tid];
-        int ahead = 0;  // equal ones by their number
-#pragma unroll 8
-        for (int i = 0; i < BESTS; i += 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(bests + i);
-            ahead += (x.x > me || (x.x == me && i < tid)) + (x.y > me || (x.y == me && i + 1 < tid)) + (x.z > me || (x.z == me && i + 2 < tid)) + (x.w > me || (x.w == me && i + 3 < tid));
+    {  // eight threads count for one of them what comes before it, equal ones by their numbers
+        const int of = tid / 8;
+        const float me = bests[of];
+        int ahead = 0;
+#pragma unroll
+        for (int k = 0; k < BESTS / 8; ++k) {
+            const int other = k * 8 + (lane & 7);
+            ahead += bests[other] > me || (bests[other] == me && other < of);
         }
-        if (ahead == a.take - 1) shared_bound = max(me, 1u);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+        if (ahead == a.take - 1 && (lane & 7) == 0) {
+            float largest = 0.f;
+            for (int b = 0; b < a.beams; ++b)
+                if (offset[b] != -INFINITY) largest = fmaxf(largest, fabsf((float)offset[b]));
+            const float lowered = me - 0x1p-21f * (largest + fabsf(me));
+            shared_bound = lowered > -INFINITY ? lowered : -INFINITY;  // no number, either: everything reaches it
+        }
     }
     __syncthreads();
-    const unsigned bound = shared_bound;
-#pragma unroll 4
-    for (int i = first_run; i < runs_here; i += team * 32)
-        if (short_of(score_of(row_tops[i], off_here)) >= bound) {
-            const int at = atomicAdd(&n_chosen, 1);
-            if (at < MOST_RUNS) chosen[at] = beam_here * a.runs + i;
-        }
+    const float bound = shared_bound;
+    auto choose = [&](int i, float top) {
+        if (top == -INFINITY || !(top + off_here >= bound) || beam_here >= a.beams) return;
+        const int at = atomicAdd(&n_chosen, 1);
+        if (at < MOST_RUNS) chosen[at] = beam_here * a.runs + i;
+    };
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) choose(first_run + k * team * 32, early[k]);
+    for (int i = first_run + EARLY * team * 32; i < runs_here; i += team * 32) choose(i, row_tops[i]);
     __syncthreads();
     int n_runs = n_chosen;
     if (n_runs > MOST_RUNS) {  // many equal ones: the `take` best, one after the other
@@ -332,22 +340,24 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
         }
     }
     // their entries that reach it
-    auto entry = [&](int i, int k) -> Best {  // entry k of chosen run i
+    struct Entry { float logit; int beam, token; };
+    auto entry = [&](int i, int k) -> Entry {  // entry k of chosen run i
         const int run = chosen[i], beam = run / a.runs, token = (run - beam * a.runs) * RUN + k;
-        if (token >= a.vocab) return {0, 0};
-        const float logit = cleaned(to_float(reinterpret_cast<const T*>(a.logits)[(size_t)(group * a.beams + beam) * a.stride + token]));
-        return {score_of(logit, offset[beam]), (long long)beam << 32 | token};
+        return {token < a.vocab ? cleaned(to_float(reinterpret_cast<const T*>(a.logits)[(size_t)(group * a.beams + beam) * a.stride + token])) : -INFINITY, beam, token};
     };
+    auto exactly = [&](const Entry& e) -> Best { return {score_of(e.logit, offset[e.beam]), (long long)e.beam << 32 | e.token}; };
     for (int i = warp; i < n_runs; i += GROUP_THREADS / 32) {
-        Best e[PER];
+        Entry e[PER];
 #pragma unroll
         for (int k = 0; k < PER; ++k) e[k] = entry(i, k * 32 + lane);
+        const float off = (float)offset[e[0].beam];
+        unsigned reach = 0;
 #pragma unroll
-        for (int k = 0; k < PER; ++k)
-            if (e[k].value && short_of(e[k].value) >= bound) {
-                const int at = atomicAdd(&n_candidates, 1);
-                if (at < MOST_CANDIDATES) candidates[at] = e[k];
-            }
+        for (int k = 0; k < PER; ++k) reach |= (e[k].logit != -INFINITY && e[k].logit + off >= bound ? 1u : 0u) << k;
+        for (; reach; reach &= reach - 1) {
+            const int k = __ffs(reach) - 1, at = atomicAdd(&n_candidates, 1);
+            if (at < MOST_CANDIDATES) candidates[at] = exactly(entry(i, k * 32 + lane));
+        }
     }
     __syncthreads();
     const int found = n_candidates;
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
             Best best{0, 0x7fffffffffffffffll};
             for (int i = warp; i < n_runs; i += GROUP_THREADS / 32)
                 for (int k = lane; k < RUN; k += 32) {
-                    const Best here = entry(i, k);
+                    const Best here = exactly(entry(i, k));
                     if (here.value && before(last, here) && before(here, best)) best = here;
                 }
             last = best_of_block(best, words);
