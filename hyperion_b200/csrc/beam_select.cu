@@ -135,7 +135,7 @@ __device__ __forceinline__ void unpack(const Words& w, float (&v)[PER]) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 4) beam_rows_kernel(const Args a) {
     __shared__ double2 parts[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y;
     let_next_kernel_start();
@@ -399,9 +399,9 @@ int launch(const Args& a, cudaStream_t stream) {
 }
 }  // namespace
 
-// Into how many pieces rows are cut, and runs of a piece: what fills the device, six blocks a multiprocessor, of two looks of its warps at least.
+// Into how many pieces rows are cut, and runs of a piece: eight blocks a multiprocessor, which holds four of them, of two looks of its warps at least.  (32 groups of 8 beams: 28.2 us; four 29.6, six 30.7, twelve 28.5.)
 static int pieces_for(int rows, int vocab, int sms, int* piece_runs) {
-    const long long runs = (vocab + RUN - 1) / RUN, room = 6LL * sms / rows, most = (runs + 2 * WARPS * AT_ONCE - 1) / (2 * WARPS * AT_ONCE);
+    const long long runs = (vocab + RUN - 1) / RUN, room = 8LL * sms / rows, most = (runs + 2 * WARPS * AT_ONCE - 1) / (2 * WARPS * AT_ONCE);
     long long n = room < 1 ? 1 : room;
     n = n < most ? n : most;
     const long long each = ((runs + n - 1) / n + WARPS * AT_ONCE - 1) / (WARPS * AT_ONCE) * (WARPS * AT_ONCE);

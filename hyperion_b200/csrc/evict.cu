@@ -11,7 +11,15 @@
 #include "common.cuh"
 
 namespace {
-constexpr int THREADS = 1024, WARPS = THREADS / 32;
+constexpr int THREADS = 1024, WARPS = THREADS / 32, MOST_BLOCKS = 8;
+constexpr int FIRST_BITS = 12, MORE_BITS = 10, BINS = 1 << FIRST_BITS;  // 12 + 10 + 10 bits of a rank
+constexpr int MOST_HELD = 48 * 1024;  // ranks that a block holds
+#ifndef HB_PART
+#define HB_PART 1024
+#endif
+#ifndef HB_MOVED
+#define HB_MOVED (1 << 20)
+#endif
 
 struct Args {
     const int* lengths; const int* newest; int requests;
@@ -21,12 +29,15 @@ struct Args {
     int layers, kv_heads;
     int* left;           // [requests]: min(length, keep)
     int* moves;          // [layers * requests * kv_heads]
-    int2* lists;         // [layers * requests * kv_heads, most]: (from, to)
+    int* from;           // [layers * requests * kv_heads, most]
+    int* to;             // likewise
     int most;            // moves of a head: min(keep, longest - keep)
     uint4* cache;        // [layers, pages, 2, kv_heads, page, record]
     int record;          // 16-byte pieces of a record
     const int* block_table; int table_width;
     int page_shift, pages;
+    int blocks;          // of a cluster
+    int moves_here;      // the records are moved by the first kernel, too
     int* status;
 };
 
@@ -41,31 +52,81 @@ __device__ __forceinline__ unsigned rank_of(float weight, int position, int firs
 }
 __device__ __forceinline__ int length_of(const Args& a, int request) { return min(max(a.lengths[request], 0), a.longest); }
 
-// How many of the threads before this one say yes, and how many do in all.  Every thread calls it; `counts` holds WARPS + 1 words.
-__device__ __forceinline__ int before_me(bool yes, int& all, int* counts) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned said = __ballot_sync(0xffffffffu, yes);
-    __syncthreads();
-    if (lane == 0) counts[warp] = __popc(said);
-    __syncthreads();
-    const int mine = counts[lane];
-    int end = mine;
+__device__ __forceinline__ unsigned their(const void* p, int rank) {  // what another block of the cluster has at this place of its shared memory
+    unsigned at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ int4 theirs4(const int* p, int rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(their(p, rank)) : "memory");
+    return v;
+}
+// All threads of the cluster; what they have written before, everywhere, is there for them behind it.
+__device__ __forceinline__ void cluster_meet(int blocks) {
+    if (blocks == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ int warp_before(int v, int lane) {  // sum over the lanes before this one
+    int end = v;
 #pragma unroll
     for (int offset = 1; offset < 32; offset <<= 1) {
         const int other = __shfl_up_sync(0xffffffffu, end, offset);
         if (lane >= offset) end += other;
     }
-    all = __shfl_sync(0xffffffffu, end, 31);
-    return __shfl_sync(0xffffffffu, end - mine, warp) + __popc(said & ((1u << lane) - 1));
+    return end - v;
 }
 
+// The records of move `move` of a head, 16 bytes a call: piece 0 .. 2 * record - 1 of its key and value.
+__device__ __forceinline__ bool record_at(const Args& a, const int* table, int layer, int kvh, int slot, int piece, size_t& at) {
+    const int page = table[slot >> a.page_shift], which = piece >= a.record;
+    if (page < 0 || page >= a.pages) {
+        atomicOr(a.status, HB_STATUS_BAD_PAGE);
+        return false;
+    }
+    at = ((((((size_t)layer * a.pages + page) * 2 + which) * a.kv_heads + kvh) << a.page_shift) + (slot & ((1 << a.page_shift) - 1))) * a.record + piece - which * a.record;
+    return true;
+}
+// Pieces first, first + step, ... of the moves: AHEAD of them are on their way together.
+constexpr int AHEAD = 4;
+__device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, long long first, long long step) {
+    const int pieces = 2 * a.record;
+    const long long n = (long long)n_moves * pieces;
+    for (long long at = first; at < n; at += AHEAD * step) {
+        uint4 held[AHEAD];
+        size_t target[AHEAD];
+        bool fine[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const long long here = at + k * step;
+            fine[k] = false;
+            if (here < n) {
+                const int move = (int)(here / pieces), piece = (int)(here - (long long)move * pieces);
+                size_t source;
+                fine[k] = record_at(a, table, layer, kvh, from[move], piece, source) & record_at(a, table, layer, kvh, to[move], piece, target[k]);
+                if (fine[k]) held[k] = a.cache[source];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (fine[k]) a.cache[target[k]] = held[k];
+    }
+}
+
+// HOLDS: the block's ranks are in shared memory; else they are made anew from the weights by every walk.
+template <bool HOLDS>
 __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
-    __shared__ int histogram[256], counts[WARPS + 1], found[2];
-    const int tid = threadIdx.x, kvh = blockIdx.x, request = blockIdx.y, layer = blockIdx.z;
+    extern __shared__ unsigned ranks[];
+    __shared__ __align__(16) int histogram[BINS];
+    __shared__ int warp_sums[WARPS], found[2];
+    __shared__ int4 counts[WARPS];      // of each warp's slots: above the rank below `keep`, above it from `keep` on, of the rank likewise
+    __shared__ __align__(16) int totals[4];  // of the block's
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int block = blockIdx.x % a.blocks, kvh = blockIdx.x / a.blocks, request = blockIdx.y, layer = blockIdx.z;
     let_next_kernel_start();
     wait_for_previous_kernels();
     const int length = length_of(a, request), head = (layer * a.requests + request) * a.kv_heads + kvh;
-    if (tid == 0 && kvh == 0 && layer == 0) {
+    if (tid == 0 && block == 0 && kvh == 0 && layer == 0) {
         a.left[request] = min(length, a.keep);
         if (a.lengths[request] > a.longest || a.lengths[request] < 0) atomicOr(a.status, HB_STATUS_BAD_POSITION);
     }
@@ -74,92 +135,142 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
     float* to_weights = a.to_weights + (size_t)head * a.capacity;
     int* to_positions = a.to_positions + (size_t)head * a.capacity;
     const bool in_place = a.to_weights == a.weights;
-    const long long after = (long long)a.newest[request] - a.recent;
+    // the block's slots, a run of them for each warp
+    const int per_warp = (length + a.blocks * WARPS * 32 - 1) / (a.blocks * WARPS * 32) * 32, slot0 = block * WARPS * per_warp, warp0 = slot0 + warp * per_warp, warp_end = min(length, warp0 + per_warp);
     int n_moves = 0;
     if (length > a.keep) {
+        const long long after = (long long)a.newest[request] - a.recent;
+        auto rank_at = [&](int slot) { return HOLDS ? ranks[slot - slot0] : rank_of(weights[slot], positions[slot], a.first, after); };
+        for (int i = tid; i < BINS; i += THREADS) histogram[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
+            const unsigned r = rank_of(weights[slot], positions[slot], a.first, after);
+            if (HOLDS) ranks[slot - slot0] = r;
+            atomicAdd(&histogram[r >> (32 - FIRST_BITS)], 1);
+        }
         // the rank of the last that stays, and how many of that rank do
         unsigned rank = 0;
         int wanted = a.keep;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += THREADS) histogram[i] = 0;
-            __syncthreads();
-            const unsigned above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-            for (int slot = tid; slot < length; slot += THREADS) {
-                const unsigned r = rank_of(weights[slot], positions[slot], a.first, after);
-                if ((r & above) == rank) atomicAdd(&histogram[(r >> shift) & 255], 1);
+#pragma unroll 1
+        for (int shift = 32 - FIRST_BITS;; shift -= MORE_BITS) {
+            cluster_meet(a.blocks);
+            // a thread has four bins, from the highest down
+            const int bins = shift == 32 - FIRST_BITS ? BINS : 1 << MORE_BITS, bin0 = bins - 4 - 4 * tid;
+            int4 mine = make_int4(0, 0, 0, 0);
+            if (bin0 >= 0) {
+                if (a.blocks == 1) {
+                    mine = *reinterpret_cast<const int4*>(histogram + bin0);
+                } else {
+                    for (int b = 0; b < a.blocks; ++b) {
+                        const int4 x = theirs4(histogram + bin0, b);
+                        mine.x += x.x, mine.y += x.y, mine.z += x.z, mine.w += x.w;
+                    }
+                }
             }
+            const int sum = mine.x + mine.y + mine.z + mine.w;
+            int before = warp_before(sum, lane);
+            if (lane == 31) warp_sums[warp] = before + sum;
             __syncthreads();
-            if (tid == 0) {
-                int digit = 255, left = wanted;
-                while (digit > 0 && histogram[digit] < left) left -= histogram[digit--];
-                found[0] = digit, found[1] = left;
+            before += __shfl_sync(0xffffffffu, warp_before(warp_sums[lane], lane), warp);
+            if (before < wanted && before + sum >= wanted) {
+                const int n[4] = {mine.w, mine.z, mine.y, mine.x};
+                int k = 0;
+                for (; before + n[k] < wanted; ++k) before += n[k];
+                found[0] = bin0 + 3 - k, found[1] = wanted - before;
             }
-            __syncthreads();
+            cluster_meet(a.blocks);  // nobody counts anew while another still reads
             rank |= (unsigned)found[0] << shift, wanted = found[1];
-        }
-        int2* list = a.lists + (size_t)head * a.most;
-        int equals = 0, holes = 0;
-        for (int base = 0; base < length; base += THREADS) {
-            const int slot = base + tid;
-            const unsigned r = slot < length ? rank_of(weights[slot], positions[slot], a.first, after) : 0u;
-            int all;
-            const int mine = before_me(slot < length && r == rank, all, counts);
-            const bool stays = slot < length && (r > rank || (r == rank && equals + mine < wanted));
-            equals += all;
-            const bool moves = stays && slot >= a.keep, hole = slot < a.keep && !stays;
-            int at = before_me(moves, all, counts);
-            if (moves) list[n_moves + at].x = slot;
-            n_moves += all;
-            at = before_me(hole, all, counts);
-            if (hole) list[holes + at].y = slot;
-            holes += all;
-        }
-        __syncthreads();
-        for (int i = tid; i < n_moves; i += THREADS) {
-            const int2 move = list[i];
-            to_weights[move.y] = weights[move.x], to_positions[move.y] = positions[move.x];
-        }
-        if (!in_place) {
-            // those that stay where they are: all of the first slots that are no target
-            int equals = 0;
-            for (int base = 0; base < a.keep; base += THREADS) {
-                const int slot = base + tid;
-                const unsigned r = slot < a.keep ? rank_of(weights[slot], positions[slot], a.first, after) : 0u;
-                int all;
-                const int mine = before_me(slot < a.keep && r == rank, all, counts);
-                if (slot < a.keep && (r > rank || (r == rank && equals + mine < wanted))) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
-                equals += all;
+            if (shift == 0) break;
+            for (int i = tid; i < 1 << MORE_BITS; i += THREADS) histogram[i] = 0;
+            __syncthreads();
+            const int next = shift - MORE_BITS;
+            for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
+                const unsigned r = rank_at(slot);
+                if ((r ^ rank) >> shift == 0) atomicAdd(&histogram[r >> next & ((1 << MORE_BITS) - 1)], 1);
             }
         }
+        // what each warp has
+        int above_low = 0, above_high = 0, equal_low = 0, equal_high = 0;
+        for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
+            const unsigned r = rank_at(slot);
+            const bool low = slot < a.keep;
+            above_low += r > rank && low, above_high += r > rank && !low, equal_low += r == rank && low, equal_high += r == rank && !low;
+        }
+        above_low = __reduce_add_sync(0xffffffffu, above_low), above_high = __reduce_add_sync(0xffffffffu, above_high);
+        equal_low = __reduce_add_sync(0xffffffffu, equal_low), equal_high = __reduce_add_sync(0xffffffffu, equal_high);
+        if (lane == 0) counts[warp] = make_int4(above_low, above_high, equal_low, equal_high);
+        __syncthreads();
+        // What is before this warp, in the block and in the blocks before, and what there is in all.
+        const int4 c = counts[lane];
+        int4 mine{warp_before(c.x, lane), warp_before(c.y, lane), warp_before(c.z, lane), warp_before(c.w, lane)};
+        if (warp == 0 && lane == 31) totals[0] = mine.x + c.x, totals[1] = mine.y + c.y, totals[2] = mine.z + c.z, totals[3] = mine.w + c.w;
+        mine = make_int4(__shfl_sync(0xffffffffu, mine.x, warp), __shfl_sync(0xffffffffu, mine.y, warp), __shfl_sync(0xffffffffu, mine.z, warp), __shfl_sync(0xffffffffu, mine.w, warp));
+        cluster_meet(a.blocks);
+        int4 all = make_int4(0, 0, 0, 0);
+        for (int b = 0; b < a.blocks; ++b) {
+            const int4 t = a.blocks == 1 ? *reinterpret_cast<const int4*>(totals) : theirs4(totals, b);
+            if (b < block) mine.x += t.x, mine.y += t.y, mine.z += t.z, mine.w += t.w;
+            all.x += t.x, all.y += t.y, all.z += t.z, all.w += t.w;
+        }
+        // Of the slots of the rank the first `wanted` stay, and those below `keep` are the first of all.
+        const int stay_low = min(all.z, wanted);
+        auto stay_high = [&](int equals) { return max(0, min(all.z + equals, wanted) - stay_low); };  // of the first so many from `keep` on
+        int holes = min(warp0, a.keep) - mine.x - min(mine.z, wanted), movers = mine.y + stay_high(mine.w);
+        n_moves = all.y + stay_high(all.w);
+        int* from = a.from + (size_t)head * a.most;
+        int* to = a.to + (size_t)head * a.most;
+        for (int slot = warp0 + lane; slot - lane < warp_end; slot += 32) {
+            const bool here = slot < warp_end, low = slot < a.keep;
+            const unsigned r = here ? rank_at(slot) : 0u, lower_lanes = (1u << lane) - 1;
+            const unsigned equal_low = __ballot_sync(0xffffffffu, here && r == rank && low), equal_high = __ballot_sync(0xffffffffu, here && r == rank && !low);
+            const int place = low ? mine.z + __popc(equal_low & lower_lanes) : all.z + mine.w + __popc(equal_high & lower_lanes);
+            mine.z += __popc(equal_low), mine.w += __popc(equal_high);
+            const bool stays = here && (r > rank || (r == rank && place < wanted));
+            const unsigned moving = __ballot_sync(0xffffffffu, stays && !low), empty = __ballot_sync(0xffffffffu, here && low && !stays);
+            if (stays && !low) from[movers + __popc(moving & lower_lanes)] = slot;
+            if (here && low && !stays) to[holes + __popc(empty & lower_lanes)] = slot;
+            movers += __popc(moving), holes += __popc(empty);
+            if (stays && low && !in_place) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
+        }
+        cluster_meet(a.blocks);
+        for (int i = block * THREADS + tid; i < n_moves; i += a.blocks * THREADS) {
+            const int source = from[i], target = to[i];
+            to_weights[target] = weights[source], to_positions[target] = positions[source];
+        }
+        if (in_place) cluster_meet(a.blocks);  // what moves has been read
     } else if (!in_place) {
-        for (int slot = tid; slot < length; slot += THREADS) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
+        for (int slot = block * THREADS + tid; slot < length; slot += a.blocks * THREADS) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
     }
-    __syncthreads();
-    for (int slot = min(length, a.keep) + tid; slot < a.capacity; slot += THREADS) to_weights[slot] = 0.f, to_positions[slot] = -1;
-    if (tid == 0) a.moves[head] = n_moves;
+    for (int slot = min(length, a.keep) + block * THREADS + tid; slot < a.capacity; slot += a.blocks * THREADS) to_weights[slot] = 0.f, to_positions[slot] = -1;
+    if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, block * THREADS + tid, (long long)a.blocks * THREADS);
+    else if (tid == 0 && block == 0) a.moves[head] = n_moves;
 }
 
-// A key's and a value's record a group of lanes; block x takes the moves from x * PER_BLOCK on.
+// The records, where the first kernel leaves them: block (part, key/value head and request, layer).
 constexpr int MOVE_THREADS = 256, PER_BLOCK = 64;
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const Args a) {
     let_next_kernel_start();
     wait_for_previous_kernels();
     const int kvh = blockIdx.y % a.kv_heads, request = blockIdx.y / a.kv_heads, layer = blockIdx.z, head = (layer * a.requests + request) * a.kv_heads + kvh;
     const int first = blockIdx.x * PER_BLOCK, n = min(a.moves[head] - first, PER_BLOCK);
-    const int2* list = a.lists + (size_t)head * a.most + first;
-    const int* table = a.block_table + (size_t)request * a.table_width;
-    const int mask = (1 << a.page_shift) - 1;
-    for (int at = threadIdx.x; at < n * 2 * a.record; at += MOVE_THREADS) {
-        const int move = at / (2 * a.record), piece = at - move * 2 * a.record, which = piece >= a.record;
-        const int2 slots = list[move];
-        const int from = table[slots.x >> a.page_shift], to = table[slots.y >> a.page_shift];
-        if (from < 0 || from >= a.pages || to < 0 || to >= a.pages) {
-            atomicOr(a.status, HB_STATUS_BAD_PAGE);
-            continue;
-        }
-        auto place = [&](int page, int slot) { return ((((size_t)layer * a.pages + page) * 2 + which) * a.kv_heads + kvh << a.page_shift) + (slot & mask); };
-        a.cache[place(to, slots.y) * a.record + piece - which * a.record] = a.cache[place(from, slots.x) * a.record + piece - which * a.record];
-    }
+    if (n > 0) move_records(a, a.from + (size_t)head * a.most + first, a.to + (size_t)head * a.most + first, n, a.block_table + (size_t)request * a.table_width, layer, kvh, threadIdx.x, MOVE_THREADS);
+}
+
+template <bool HOLDS>
+int launch_choose(const Args& a, size_t shared_bytes, cudaStream_t stream) {
+    const auto kernel = evict_choose_kernel<HOLDS>;
+    const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_HELD * 4);
+    if (configured != cudaSuccess) return (int)configured;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(a.blocks * a.kv_heads, a.requests, a.layers), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = shared_bytes, config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = overlap_launches() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {(unsigned)a.blocks, 1, 1};
+    config.attrs = attributes, config.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&config, kernel, a);
 }
 }  // namespace
 
@@ -172,19 +283,25 @@ HB_EXPORT long long hb_evict_scratch(int layers, int requests, int kv_heads, int
 // table and capacity hold.  scratch: hb_evict_scratch bytes on a 16-byte boundary.
 HB_EXPORT int hb_evict(void* cache, int layers, int pages, int kv_heads, int page_size, int record_bytes, const int* block_table, int table_width, const int* lengths, const int* newest, int requests,
                        int longest, const float* weights, const int* positions, float* to_weights, int* to_positions, int capacity, int keep, int first, int recent, int* left, void* scratch, int* status,
-                       cudaStream_t stream) {
+                       int sms, cudaStream_t stream) {
     if (requests <= 0 || layers <= 0) return 0;
     if (!cache || !block_table || !lengths || !newest || !weights || !positions || !to_weights || !to_positions || !left || !scratch || !status) return HB_BAD_ARGUMENT;
-    if (pages <= 0 || kv_heads <= 0 || page_size <= 0 || (page_size & (page_size - 1)) || record_bytes <= 0 || record_bytes % 16 || table_width <= 0 || longest <= 0 || capacity < longest || keep < 1 || recent < 0)
+    if (pages <= 0 || kv_heads <= 0 || page_size <= 0 || (page_size & (page_size - 1)) || record_bytes <= 0 || record_bytes % 16 || table_width <= 0 || longest <= 0 || capacity < longest || keep < 1 || recent < 0 || sms <= 0)
         return HB_BAD_ARGUMENT;
     if (((uintptr_t)cache | (uintptr_t)scratch) & 15 || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     const long long heads = (long long)layers * requests * kv_heads;
     if (requests > 65535 || layers > 65535 || (long long)requests * kv_heads > 65535 || heads > 0x7fffffffLL || longest > 0x7fffffff - THREADS || record_bytes > 65536) return HB_UNSUPPORTED_SIZE;
+    if (longest > 0x7fffffff - MOST_BLOCKS * THREADS || (long long)kv_heads * MOST_BLOCKS > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const int most = longest - keep < keep ? (longest > keep ? longest - keep : 0) : keep;
+    int blocks = 1;
+    while (blocks < MOST_BLOCKS && heads * blocks * 2 <= sms && longest >= blocks * 2 * HB_PART) blocks *= 2;
+    const size_t held = (size_t)((longest + blocks * THREADS - 1) / (blocks * THREADS)) * THREADS;
     int* moves = (int*)scratch;
-    const Args a{lengths, newest, requests, weights, positions, to_weights, to_positions, capacity, longest, keep, first, recent, layers, kv_heads, left, moves,
-                 (int2*)((char*)scratch + (heads * 4 + 15) / 16 * 16), most, (uint4*)cache, record_bytes / 16, block_table, table_width, __builtin_ctz(page_size), pages, status};
-    if (int code = launch_after_previous(evict_choose_kernel, dim3(kv_heads, requests, layers), dim3(THREADS), 0, stream, a)) return code;
-    if (!most) return 0;
+    int* lists = (int*)((char*)scratch + (heads * 4 + 15) / 16 * 16);
+    const bool moves_here = (long long)most * 2 * record_bytes <= (long long)blocks * HB_MOVED;
+    const Args a{lengths, newest, requests, weights, positions, to_weights, to_positions, capacity, longest, keep, first, recent, layers, kv_heads, left, moves, lists, lists + heads * most, most,
+                 (uint4*)cache, record_bytes / 16, block_table, table_width, __builtin_ctz(page_size), pages, blocks, moves_here ? 1 : 0, status};
+    if (int code = held <= MOST_HELD ? launch_choose<true>(a, held * 4, stream) : launch_choose<false>(a, 0, stream)) return code;
+    if (!most || moves_here) return 0;
     return launch_after_previous(evict_move_kernel, dim3((most + PER_BLOCK - 1) / PER_BLOCK, kv_heads * requests, layers), dim3(MOVE_THREADS), 0, stream, a);
 }

@@ -8,6 +8,7 @@ import torch
 
 from .basic import status_word
 from .native import KernelError, check, entry, stream_address
+from .tally import _check_device
 
 MOST_TENSORS = 24
 MOST_BEAMS = 32
@@ -51,11 +52,7 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
             raise KernelError(f"{what}: states are dense [layers, {rows if state_rows is None else 'rows'}, ...]")
         layers, places = state.shape[:2]
         words += [state.data_ptr(), layers, places, 1, 1, state.numel() // max(1, layers * places) * state.element_size(), 1]
-    for tensor in (parents, lengths, block_table, state_rows, *caches, *states):
-        if tensor is not None and (not tensor.is_cuda or tensor.device != parents.device):
-            raise KernelError(f"{what}: all tensors on one CUDA device, not on {parents.device} and {tensor.device}")
-    if parents.device.index != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: the tensors are on {parents.device}, which is not the current device")
+    _check_device(what, parents, lengths, *(tensor for tensor in (block_table, state_rows) if tensor is not None), *caches, *states)
     if rows == 0 or not words:
         return
     check(entry("beam_reorder", "hb_beam_reorder", "ppiipiipippp")(

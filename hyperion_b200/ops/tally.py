@@ -6,6 +6,7 @@ that stands there.  Each key/value head keeps slots of its own; all of a request
 keys are stored rotated, so attention does not ask which slot a key stands in, and a slot that eviction fills goes on with its position."""
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -34,26 +35,29 @@ def new_tally(requests: int, kv_heads: int, capacity: int, layers: Optional[int]
 def _check_tally(tally: Tally, shape: tuple, what: str) -> int:
     """The capacity of a tally [*shape, capacity]."""
     weights, positions = tally
-    if (weights.dtype is not torch.float32 or positions.dtype is not torch.int32 or weights.dim() != len(shape) + 1 or weights.shape[:-1] != shape or positions.shape != weights.shape
-            or not weights.is_contiguous() or not positions.is_contiguous()):
+    found = weights.shape
+    if (weights.dtype is not torch.float32 or positions.dtype is not torch.int32 or found[:-1] != shape or positions.shape != found or not (weights.is_contiguous() and positions.is_contiguous())):
         raise KernelError(f"{what}: a tally is dense float32 weights and int32 positions {[*shape, 'capacity']}")
-    return weights.shape[-1]
+    return found[-1]
 
 
-def _check_vectors(what: str, **vectors) -> None:
-    for name, (vector, size) in vectors.items():
-        if vector.dtype is not torch.int32 or vector.dim() != 1 or vector.shape[0] != size or not vector.is_contiguous():
-            raise KernelError(f"{what}: {name} is a dense int32 vector of {size}")
+def _check_vector(what: str, name: str, vector: torch.Tensor, size: int) -> None:
+    if vector.dtype is not torch.int32 or vector.shape != (size,) or not vector.is_contiguous():
+        raise KernelError(f"{what}: {name} is a dense int32 vector of {size}")
 
 
-def _check_device(what: str, *tensors) -> torch.device:
-    device = tensors[0].device
+def _check_device(what: str, *tensors) -> int:
+    """The number of the current device, on which all of them are."""
+    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
     for tensor in tensors:
-        if tensor is not None and (tensor.device != device or not tensor.is_cuda):
-            raise KernelError(f"{what}: all tensors on one CUDA device, not on {device} and {tensor.device}")
-    if device.index != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: the tensors are on {device}, which is not the current device")
-    return device
+        if tensor.get_device() != current:
+            raise KernelError(f"{what}: all tensors on the current CUDA device, not on {tensor.device}")
+    return current
+
+
+@lru_cache(maxsize=4096)
+def _scratch_size(module: str, name: str, head_dim: int, *sizes: int) -> int:
+    return entry(module, name, "i" * len(sizes), head_dim, result="l")(*sizes)
 
 
 def _check_pages(what: str, cache, heads: int, q, block_table, requests: int, longest: int, scale: float) -> tuple[int, int, int, int]:
@@ -102,8 +106,10 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     longest = _longest(what, longest, block_table, cache.shape[3] if cache.dim() == 5 else 0, tally.weights.shape[-1])
     pages, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, block_table, requests, longest, scale)
     capacity, width = _check_tally(tally, (requests, kv_heads), what), heads * head_dim
-    _check_vectors(what, lengths=(lengths, requests), newest=(newest, requests))
-    device = _check_device(what, q, cache, block_table, lengths, newest, tally.weights, tally.positions, out)
+    _check_vector(what, "lengths", lengths, requests)
+    _check_vector(what, "newest", newest, requests)
+    _check_device(what, q, cache, block_table, lengths, newest, *tally, q if out is None else out)
+    device = q.device
     if out is None:
         out = torch.empty(requests, width, dtype=torch.bfloat16, device=device)
     elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != requests or out.shape[1] < width or out.stride(1) != 1:
@@ -114,8 +120,7 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
         out[:, :width].zero_()
         return out
     stream, sms = stream_address(), sm_count(device)
-    size = entry("attention_tallied", "hb_attention_tallied_scratch", "iiiii", head_dim, result="l")(requests, longest, heads, kv_heads, sms)
-    memory, owner = scratch(device, stream, size)
+    memory, owner = scratch(device, stream, _scratch_size("attention_tallied", "hb_attention_tallied_scratch", head_dim, requests, longest, heads, kv_heads, sms))
     check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim)(
         q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, tally.weights.data_ptr(),
         tally.positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
@@ -136,18 +141,19 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     longest = _longest(what, longest, block_table, cache.shape[3] if cache.dim() == 5 else 0, tally.weights.shape[-1])
     pages, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, block_table, requests, longest, scale)
     capacity = _check_tally(tally, (requests, kv_heads), what)
-    _check_vectors(what, lengths=(lengths, requests), starts=(starts, requests + 1))
+    _check_vector(what, "lengths", lengths, requests)
+    _check_vector(what, "starts", starts, requests + 1)
     if most < 0:
         raise KernelError(f"{what}: most counts a request's queries")
     if heads // kv_heads > 128:
         raise KernelError(f"{what}: at most 128 heads a key/value head, not {heads // kv_heads}")
-    device = _check_device(what, q, cache, block_table, starts, lengths, tally.weights, tally.positions)
+    _check_device(what, q, cache, block_table, starts, lengths, *tally)
+    device = q.device
     most = min(most, tokens)
     if requests == 0 or most == 0 or longest == 0:
         return
     stream, sms = stream_address(), sm_count(device)
-    size = entry("tally_queries", "hb_tally_queries_scratch", "iiiiiii", head_dim, result="l")(tokens, requests, most, longest, heads, kv_heads, sms)
-    memory, owner = scratch(device, stream, size)
+    memory, owner = scratch(device, stream, _scratch_size("tally_queries", "hb_tally_queries_scratch", head_dim, tokens, requests, most, longest, heads, kv_heads, sms))
     check(entry("tally_queries", "hb_tally_queries", "plippippiiipiiiiifippp", head_dim)(
         q.data_ptr(), q.stride(0), tokens, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], starts.data_ptr(), lengths.data_ptr(), requests, most, longest, tally.weights.data_ptr(), capacity,
         heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
@@ -182,18 +188,20 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     to = tally if out is None else out
     if _check_tally(to, shape, what) != capacity or (to.weights.data_ptr() == tally.weights.data_ptr()) != (to.positions.data_ptr() == tally.positions.data_ptr()):
         raise KernelError(f"{what}: the new tally is as large as the old one, and all of it in its place or none")
-    _check_vectors(what, lengths=(lengths, requests), newest=(newest, requests))
+    _check_vector(what, "lengths", lengths, requests)
+    _check_vector(what, "newest", newest, requests)
     if keep < 1 or first < 0 or recent < 0:
         raise KernelError(f"{what}: keep at least 1, first and recent at least 0, not {keep}, {first} and {recent}")
     longest = _longest(what, longest, block_table, page_size, capacity)
-    device = _check_device(what, cache, block_table, lengths, newest, *tally, *to)
+    _check_device(what, cache, block_table, lengths, newest, *tally, *to)
+    device = cache.device
     left = torch.empty(requests, dtype=torch.int32, device=device)
     if requests == 0 or layers == 0 or kv_heads == 0 or longest == 0:
         return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
     keep, first, recent = (min(value, 2**31 - 1) for value in (keep, first, recent))
     stream = stream_address()
-    memory, owner = scratch(device, stream, entry("evict", "hb_evict_scratch", "iiiii", result="l")(layers, requests, kv_heads, longest, keep))
-    check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppp")(
+    memory, owner = scratch(device, stream, _scratch_size("evict", "hb_evict_scratch", 0, layers, requests, kv_heads, longest, keep))
+    check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppip")(
         cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, tally.weights.data_ptr(),
-        tally.positions.data_ptr(), to.weights.data_ptr(), to.positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), stream), what)
+        tally.positions.data_ptr(), to.weights.data_ptr(), to.positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), sm_count(device), stream), what)
     return left

@@ -9,7 +9,8 @@ from typing import NamedTuple
 import numpy as np
 import torch
 
-from ..ops.native import KernelError, check, entry, is_bf16, require_cuda, scratch, sm_count, stream_address
+from ..ops.native import KernelError, check, entry, is_bf16, scratch, sm_count, stream_address
+from ..ops.tally import _check_device, _scratch_size
 
 MOST_BEAMS = 32
 MOST_TAKE = 64
@@ -36,15 +37,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamCh
     if not 1 <= take <= MOST_TAKE:
         raise KernelError(f"beam_select: 1 to {MOST_TAKE} continuations, not {take}")
     kind, device, vocab = is_bf16(logits), logits.device, logits.shape[1]
-    require_cuda(logits, scores)
-    if scores.device != device or device.index != torch._C._cuda_getDevice():
-        raise KernelError(f"beam_select: logits and scores on the current CUDA device, not on {device} and {scores.device}")
-    parents, tokens = (torch.empty(groups, take, dtype=torch.int32, device=device) for _ in range(2))
-    found = torch.empty(groups, take, dtype=torch.float32, device=device)
+    _check_device("beam_select", logits, scores)
+    answer = torch.empty(3, groups, take, dtype=torch.int32, device=device)
+    parents, tokens, found = answer[0], answer[1], answer[2].view(torch.float32)
     if groups == 0:
         return BeamChoice(parents, tokens, found)
     stream, sms = stream_address(), sm_count(device)
-    memory, owner = scratch(device, stream, entry("beam_select", "hb_beam_select_scratch", "iiiii", result="l")(groups, beams, vocab, take, sms))
+    memory, owner = scratch(device, stream, _scratch_size("beam_select", "hb_beam_select_scratch", 0, groups, beams, vocab, take, sms))
     check(entry("beam_select", "hb_beam_select", "pilpiiiipppipp")(logits.data_ptr(), kind, max(logits.stride(0), vocab), scores.data_ptr(), groups, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(),
                                                              found.data_ptr(), sms, memory, stream), "beam_select")
     return BeamChoice(parents, tokens, found)

@@ -114,6 +114,21 @@ def test_long_requests(length, keep, layers, kv):
     run([length], layers=layers, kv=kv, dim=16, page=64, keep=keep, first=4, recent=min(keep, 64))
 
 
+def test_more_slots_than_a_cluster_holds():
+    run([450001, 5000], kv=1, dim=8, page=64, keep=1000, first=4, recent=64, separate=True)
+
+
+@pytest.mark.parametrize("separate", [False, True])
+def test_records_that_a_second_kernel_moves(separate):
+    run([9000, 200], kv=2, dim=256, page=64, dtype=torch.float32, keep=4000, separate=separate)
+
+
+@pytest.mark.parametrize("kv,layers", [(1, 1), (8, 4), (8, 20)])  # clusters of many blocks, of some, of one
+def test_equal_weights_across_the_blocks_of_a_cluster(kv, layers):
+    for spread in (0.001, 2):
+        run([12000], kv=kv, layers=layers, dim=8, page=64, keep=5000, first=3, recent=100, spread=spread)
+
+
 def test_a_bound_on_the_lengths():
     run([300, 120], keep=40, longest=300)
     run([30, 12], keep=40, longest=30)
