@@ -62,10 +62,23 @@ __device__ __forceinline__ int4 theirs4(const int* p, int rank) {
     asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(their(p, rank)) : "memory");
     return v;
 }
-// All threads of the cluster; what they have written before, everywhere, is there for them behind it.
+// All threads of the cluster; what they have written before, everywhere, is there for them behind it.  One thread's fence stands for its block, which has met before it (as many fences as there are warps take a
+// thousand clocks).
 __device__ __forceinline__ void cluster_meet(int blocks) {
-    if (blocks == 1) __syncthreads();
-    else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    __syncthreads();
+    if (blocks == 1) return;
+    if (threadIdx.x == 0) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// What the blocks have at this place, all on their way together.
+__device__ __forceinline__ void all_of_theirs(const int* p, int blocks, int4 (&x)[MOST_BLOCKS]) {
+    if (blocks == 1) {
+        x[0] = *reinterpret_cast<const int4*>(p);
+        return;
+    }
+#pragma unroll
+    for (int b = 0; b < MOST_BLOCKS; ++b)
+        if (b < blocks) x[b] = theirs4(p, b);
 }
 __device__ __forceinline__ int warp_before(int v, int lane) {  // sum over the lanes before this one
     int end = v;
@@ -77,39 +90,44 @@ __device__ __forceinline__ int warp_before(int v, int lane) {  // sum over the l
     return end - v;
 }
 
-// The records of move `move` of a head, 16 bytes a call: piece 0 .. 2 * record - 1 of its key and value.
-__device__ __forceinline__ bool record_at(const Args& a, const int* table, int layer, int kvh, int slot, int piece, size_t& at) {
-    const int page = table[slot >> a.page_shift], which = piece >= a.record;
-    if (page < 0 || page >= a.pages) {
-        atomicOr(a.status, HB_STATUS_BAD_PAGE);
-        return false;
-    }
-    at = ((((((size_t)layer * a.pages + page) * 2 + which) * a.kv_heads + kvh) << a.page_shift) + (slot & ((1 << a.page_shift) - 1))) * a.record + piece - which * a.record;
-    return true;
-}
-// Pieces first, first + step, ... of the moves: AHEAD of them are on their way together.
+// The records of moves first, first + step, ...: a team of lanes a move, 16 bytes of its key and value a lane and turn.  AHEAD moves of a team are on their way together.
 constexpr int AHEAD = 4;
-__device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, long long first, long long step) {
-    const int pieces = 2 * a.record;
-    const long long n = (long long)n_moves * pieces;
-    for (long long at = first; at < n; at += AHEAD * step) {
-        uint4 held[AHEAD];
-        size_t target[AHEAD];
+__device__ __forceinline__ int team_of(const Args& a) {  // lanes: a power of two
+    int lanes = 1;
+    while (lanes < 32 && lanes < 2 * a.record) lanes *= 2;
+    return lanes;
+}
+__device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, int first, int step, int lane, int team) {
+    const int mask = (1 << a.page_shift) - 1;
+    uint4* layer_cache = a.cache + (((size_t)layer * a.pages * 2 * a.kv_heads) << a.page_shift) * a.record;
+    const size_t values = ((size_t)a.kv_heads << a.page_shift) * a.record;  // from a key to its value
+    for (int move0 = first; move0 < n_moves; move0 += AHEAD * step) {
+        size_t source[AHEAD], target[AHEAD];
         bool fine[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            const long long here = at + k * step;
-            fine[k] = false;
-            if (here < n) {
-                const int move = (int)(here / pieces), piece = (int)(here - (long long)move * pieces);
-                size_t source;
-                fine[k] = record_at(a, table, layer, kvh, from[move], piece, source) & record_at(a, table, layer, kvh, to[move], piece, target[k]);
-                if (fine[k]) held[k] = a.cache[source];
+            const int move = move0 + k * step;
+            fine[k] = move < n_moves;
+            if (fine[k]) {
+                const int s = from[move], t = to[move], page = table[s >> a.page_shift], to_page = table[t >> a.page_shift];
+                if (page < 0 || page >= a.pages || to_page < 0 || to_page >= a.pages) {
+                    atomicOr(a.status, HB_STATUS_BAD_PAGE);
+                    fine[k] = false;
+                }
+                source[k] = ((((size_t)page * 2 * a.kv_heads + kvh) << a.page_shift) + (s & mask)) * a.record;
+                target[k] = ((((size_t)to_page * 2 * a.kv_heads + kvh) << a.page_shift) + (t & mask)) * a.record;
             }
         }
+        for (int piece = lane; piece < 2 * a.record; piece += team) {
+            const size_t at = piece < a.record ? piece : values + piece - a.record;
+            uint4 held[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-            if (fine[k]) a.cache[target[k]] = held[k];
+            for (int k = 0; k < AHEAD; ++k)
+                if (fine[k]) held[k] = layer_cache[source[k] + at];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (fine[k]) layer_cache[target[k] + at] = held[k];
+        }
     }
 }
 
@@ -117,7 +135,7 @@ __device__ __forceinline__ void move_records(const Args& a, const int* from, con
 template <bool HOLDS>
 __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
     extern __shared__ unsigned ranks[];
-    __shared__ __align__(16) int histogram[BINS];
+    __shared__ __align__(16) int histograms[BINS + 2 * (1 << MORE_BITS)];  // of each digit
     __shared__ int warp_sums[WARPS], found[2];
     __shared__ int4 counts[WARPS];      // of each warp's slots: above the rank below `keep`, above it from `keep` on, of the rank likewise
     __shared__ __align__(16) int totals[4];  // of the block's
@@ -141,17 +159,20 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
     if (length > a.keep) {
         const long long after = (long long)a.newest[request] - a.recent;
         auto rank_at = [&](int slot) { return HOLDS ? ranks[slot - slot0] : rank_of(weights[slot], positions[slot], a.first, after); };
-        for (int i = tid; i < BINS; i += THREADS) histogram[i] = 0;
+        for (int i = tid; i < BINS + 2 * (1 << MORE_BITS); i += THREADS) histograms[i] = 0;
         __syncthreads();
 #pragma unroll 4
         for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
-            const unsigned r = rank_of(weights[slot], positions[slot], a.first, after);
+            const float weight = weights[slot];
+            const int position = positions[slot];
+            const unsigned r = rank_of(weight, position, a.first, after);
             if (HOLDS) ranks[slot - slot0] = r;
-            atomicAdd(&histogram[r >> (32 - FIRST_BITS)], 1);
+            atomicAdd(&histograms[r >> (32 - FIRST_BITS)], 1);
+            if (!in_place && slot < a.keep) to_weights[slot] = weight, to_positions[slot] = position;  // what moves into a free one comes later
         }
         // the rank of the last that stays, and how many of that rank do
         unsigned rank = 0;
-        int wanted = a.keep;
+        int wanted = a.keep, *histogram = histograms;
 #pragma unroll 1
         for (int shift = 32 - FIRST_BITS;; shift -= MORE_BITS) {
             cluster_meet(a.blocks);
@@ -159,14 +180,11 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
             const int bins = shift == 32 - FIRST_BITS ? BINS : 1 << MORE_BITS, bin0 = bins - 4 - 4 * tid;
             int4 mine = make_int4(0, 0, 0, 0);
             if (bin0 >= 0) {
-                if (a.blocks == 1) {
-                    mine = *reinterpret_cast<const int4*>(histogram + bin0);
-                } else {
-                    for (int b = 0; b < a.blocks; ++b) {
-                        const int4 x = theirs4(histogram + bin0, b);
-                        mine.x += x.x, mine.y += x.y, mine.z += x.z, mine.w += x.w;
-                    }
-                }
+                int4 x[MOST_BLOCKS];
+                all_of_theirs(histogram + bin0, a.blocks, x);
+#pragma unroll
+                for (int b = 0; b < MOST_BLOCKS; ++b)
+                    if (b < a.blocks) mine.x += x[b].x, mine.y += x[b].y, mine.z += x[b].z, mine.w += x[b].w;
             }
             const int sum = mine.x + mine.y + mine.z + mine.w;
             int before = warp_before(sum, lane);
@@ -179,12 +197,12 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
                 for (; before + n[k] < wanted; ++k) before += n[k];
                 found[0] = bin0 + 3 - k, found[1] = wanted - before;
             }
-            cluster_meet(a.blocks);  // nobody counts anew while another still reads
+            __syncthreads();
             rank |= (unsigned)found[0] << shift, wanted = found[1];
             if (shift == 0) break;
-            for (int i = tid; i < 1 << MORE_BITS; i += THREADS) histogram[i] = 0;
-            __syncthreads();
+            histogram += bins;
             const int next = shift - MORE_BITS;
+#pragma unroll 4
             for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
                 const unsigned r = rank_at(slot);
                 if ((r ^ rank) >> shift == 0) atomicAdd(&histogram[r >> next & ((1 << MORE_BITS) - 1)], 1);
@@ -208,8 +226,12 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
         mine = make_int4(__shfl_sync(0xffffffffu, mine.x, warp), __shfl_sync(0xffffffffu, mine.y, warp), __shfl_sync(0xffffffffu, mine.z, warp), __shfl_sync(0xffffffffu, mine.w, warp));
         cluster_meet(a.blocks);
         int4 all = make_int4(0, 0, 0, 0);
-        for (int b = 0; b < a.blocks; ++b) {
-            const int4 t = a.blocks == 1 ? *reinterpret_cast<const int4*>(totals) : theirs4(totals, b);
+        int4 x[MOST_BLOCKS];
+        all_of_theirs(totals, a.blocks, x);
+#pragma unroll
+        for (int b = 0; b < MOST_BLOCKS; ++b) {
+            if (b >= a.blocks) break;
+            const int4 t = x[b];
             if (b < block) mine.x += t.x, mine.y += t.y, mine.z += t.z, mine.w += t.w;
             all.x += t.x, all.y += t.y, all.z += t.z, all.w += t.w;
         }
@@ -231,7 +253,6 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
             if (stays && !low) from[movers + __popc(moving & lower_lanes)] = slot;
             if (here && low && !stays) to[holes + __popc(empty & lower_lanes)] = slot;
             movers += __popc(moving), holes += __popc(empty);
-            if (stays && low && !in_place) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
         }
         cluster_meet(a.blocks);
         for (int i = block * THREADS + tid; i < n_moves; i += a.blocks * THREADS) {
@@ -243,7 +264,8 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
         for (int slot = block * THREADS + tid; slot < length; slot += a.blocks * THREADS) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
     }
     for (int slot = min(length, a.keep) + block * THREADS + tid; slot < a.capacity; slot += a.blocks * THREADS) to_weights[slot] = 0.f, to_positions[slot] = -1;
-    if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, block * THREADS + tid, (long long)a.blocks * THREADS);
+    const int team = team_of(a), at = block * THREADS + tid;
+    if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, at / team, a.blocks * THREADS / team, at % team, team);
     else if (tid == 0 && block == 0) a.moves[head] = n_moves;
 }
 
@@ -254,7 +276,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const Args a) 
     wait_for_previous_kernels();
     const int kvh = blockIdx.y % a.kv_heads, request = blockIdx.y / a.kv_heads, layer = blockIdx.z, head = (layer * a.requests + request) * a.kv_heads + kvh;
     const int first = blockIdx.x * PER_BLOCK, n = min(a.moves[head] - first, PER_BLOCK);
-    if (n > 0) move_records(a, a.from + (size_t)head * a.most + first, a.to + (size_t)head * a.most + first, n, a.block_table + (size_t)request * a.table_width, layer, kvh, threadIdx.x, MOVE_THREADS);
+    const int team = team_of(a);
+    if (n > 0) move_records(a, a.from + (size_t)head * a.most + first, a.to + (size_t)head * a.most + first, n, a.block_table + (size_t)request * a.table_width, layer, kvh, threadIdx.x / team, MOVE_THREADS / team, threadIdx.x % team, team);
 }
 
 template <bool HOLDS>
