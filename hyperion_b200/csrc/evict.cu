@@ -90,43 +90,49 @@ __device__ __forceinline__ int warp_before(int v, int lane) {  // sum over the l
     return end - v;
 }
 
-// The records of moves first, first + step, ...: a team of lanes a move, 16 bytes of its key and value a lane and turn.  AHEAD moves of a team are on their way together.
-constexpr int AHEAD = 4;
-__device__ __forceinline__ int team_of(const Args& a) {  // lanes: a power of two
-    int lanes = 1;
-    while (lanes < 32 && lanes < 2 * a.record) lanes *= 2;
-    return lanes;
-}
-__device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, int first, int step, int lane, int team) {
-    const int mask = (1 << a.page_shift) - 1;
+// The records of a head's moves: warp `first` of `step` takes every step-th CHUNK of them.  A lane finds out where one of them goes from and to; then a team of lanes a move carries 16 bytes of its key and value a lane and
+// turn, AHEAD moves of a team on their way together.
+#ifndef HB_AHEAD
+#define HB_AHEAD 4
+#endif
+constexpr int CHUNK = 16, AHEAD = HB_AHEAD;
+__device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, int first, int step) {
+    const int lane = threadIdx.x & 31, mask = (1 << a.page_shift) - 1;
+    int team = 1;  // lanes: a power of two
+    while (team < 32 && team < 2 * a.record) team *= 2;
+    const int teams = 32 / team, mine = lane / team;
     uint4* layer_cache = a.cache + (((size_t)layer * a.pages * 2 * a.kv_heads) << a.page_shift) * a.record;
     const size_t values = ((size_t)a.kv_heads << a.page_shift) * a.record;  // from a key to its value
-    for (int move0 = first; move0 < n_moves; move0 += AHEAD * step) {
-        size_t source[AHEAD], target[AHEAD];
-        bool fine[AHEAD];
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int move = move0 + k * step;
-            fine[k] = move < n_moves;
-            if (fine[k]) {
-                const int s = from[move], t = to[move], page = table[s >> a.page_shift], to_page = table[t >> a.page_shift];
-                if (page < 0 || page >= a.pages || to_page < 0 || to_page >= a.pages) {
-                    atomicOr(a.status, HB_STATUS_BAD_PAGE);
-                    fine[k] = false;
-                }
-                source[k] = ((((size_t)page * 2 * a.kv_heads + kvh) << a.page_shift) + (s & mask)) * a.record;
-                target[k] = ((((size_t)to_page * 2 * a.kv_heads + kvh) << a.page_shift) + (t & mask)) * a.record;
+    for (int base = first * CHUNK; base < n_moves; base += step * CHUNK) {
+        const int n = min(CHUNK, n_moves - base);
+        long long source = -1, target = -1;  // of this lane's move
+        if (lane < n) {
+            const int s = from[base + lane], t = to[base + lane], page = table[s >> a.page_shift], to_page = table[t >> a.page_shift];
+            if (page < 0 || page >= a.pages || to_page < 0 || to_page >= a.pages) {
+                atomicOr(a.status, HB_STATUS_BAD_PAGE);
+            } else {
+                source = ((((long long)page * 2 * a.kv_heads + kvh) << a.page_shift) + (s & mask)) * a.record;
+                target = ((((long long)to_page * 2 * a.kv_heads + kvh) << a.page_shift) + (t & mask)) * a.record;
             }
         }
-        for (int piece = lane; piece < 2 * a.record; piece += team) {
-            const size_t at = piece < a.record ? piece : values + piece - a.record;
-            uint4 held[AHEAD];
+        for (int k0 = 0; k0 < n; k0 += AHEAD * teams) {
+            long long s[AHEAD], t[AHEAD];
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k)
-                if (fine[k]) held[k] = layer_cache[source[k] + at];
+            for (int k = 0; k < AHEAD; ++k) {
+                const int move = k0 + k * teams + mine;
+                s[k] = __shfl_sync(0xffffffffu, source, move & 31), t[k] = __shfl_sync(0xffffffffu, target, move & 31);
+                if (move >= n) s[k] = -1;
+            }
+            for (int piece = lane & (team - 1); piece < 2 * a.record; piece += team) {
+                const size_t at = piece < a.record ? piece : values + piece - a.record;
+                uint4 held[AHEAD];
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k)
-                if (fine[k]) layer_cache[target[k] + at] = held[k];
+                for (int k = 0; k < AHEAD; ++k)
+                    if (s[k] >= 0) held[k] = layer_cache[s[k] + at];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+                    if (s[k] >= 0) layer_cache[t[k] + at] = held[k];
+            }
         }
     }
 }
@@ -264,20 +270,18 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
         for (int slot = block * THREADS + tid; slot < length; slot += a.blocks * THREADS) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
     }
     for (int slot = min(length, a.keep) + block * THREADS + tid; slot < a.capacity; slot += a.blocks * THREADS) to_weights[slot] = 0.f, to_positions[slot] = -1;
-    const int team = team_of(a), at = block * THREADS + tid;
-    if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, at / team, a.blocks * THREADS / team, at % team, team);
+    if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, block * WARPS + warp, a.blocks * WARPS);
     else if (tid == 0 && block == 0) a.moves[head] = n_moves;
 }
 
 // The records, where the first kernel leaves them: block (part, key/value head and request, layer).
-constexpr int MOVE_THREADS = 256, PER_BLOCK = 64;
+constexpr int MOVE_THREADS = 256, PER_BLOCK = CHUNK * MOVE_THREADS / 32;
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const Args a) {
     let_next_kernel_start();
     wait_for_previous_kernels();
     const int kvh = blockIdx.y % a.kv_heads, request = blockIdx.y / a.kv_heads, layer = blockIdx.z, head = (layer * a.requests + request) * a.kv_heads + kvh;
-    const int first = blockIdx.x * PER_BLOCK, n = min(a.moves[head] - first, PER_BLOCK);
-    const int team = team_of(a);
-    if (n > 0) move_records(a, a.from + (size_t)head * a.most + first, a.to + (size_t)head * a.most + first, n, a.block_table + (size_t)request * a.table_width, layer, kvh, threadIdx.x / team, MOVE_THREADS / team, threadIdx.x % team, team);
+    move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, a.moves[head], a.block_table + (size_t)request * a.table_width, layer, kvh,
+                 blockIdx.x * (MOVE_THREADS / 32) + (threadIdx.x >> 5), gridDim.x * (MOVE_THREADS / 32));
 }
 
 template <bool HOLDS>
