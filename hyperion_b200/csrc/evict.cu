@@ -12,8 +12,9 @@
 
 namespace {
 constexpr int THREADS = 1024, WARPS = THREADS / 32, MOST_BLOCKS = 8;
-constexpr int FIRST_BITS = 12, MORE_BITS = 10, BINS = 1 << FIRST_BITS;  // 12 + 10 + 10 bits of a rank
-constexpr int MOST_HELD = 48 * 1024;  // ranks that a block holds
+constexpr int DIGIT = 11, BINS = 2 * (1 << DIGIT) + (1 << (32 - 2 * DIGIT));  // 11, 11 and 10 bits of a rank
+constexpr int LOOK = 128;  // slots of a warp's look, four a lane
+constexpr int MOST_HELD = 40 * 1024;  // ranks that a block holds
 #ifndef HB_PART
 #define HB_PART 1024
 #endif
@@ -69,6 +70,10 @@ __device__ __forceinline__ void cluster_meet(int blocks) {
     if (blocks == 1) return;
     if (threadIdx.x == 0) asm volatile("fence.acq_rel.cluster;" ::: "memory");
     asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Adds to what each block of the cluster has at this place.
+__device__ __forceinline__ void add_to_all(int* p, int n, int blocks) {
+    for (int b = 0; b < blocks; ++b) asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(their(p, b)), "r"(n) : "memory");
 }
 // What the blocks have at this place, all on their way together.
 __device__ __forceinline__ void all_of_theirs(const int* p, int blocks, int4 (&x)[MOST_BLOCKS]) {
@@ -140,14 +145,17 @@ __device__ __forceinline__ void move_records(const Args& a, const int* from, con
 // HOLDS: the block's ranks are in shared memory; else they are made anew from the weights by every walk.
 template <bool HOLDS>
 __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
-    extern __shared__ unsigned ranks[];
-    __shared__ __align__(16) int histograms[BINS + 2 * (1 << MORE_BITS)];  // of each digit
+    extern __shared__ __align__(16) unsigned ranks[];
+    __shared__ __align__(16) int counted[BINS];  // of each digit, in the block
+    __shared__ __align__(16) int summed[BINS];   // and in the cluster
     __shared__ int warp_sums[WARPS], found[2];
     __shared__ int4 counts[WARPS];      // of each warp's slots: above the rank below `keep`, above it from `keep` on, of the rank likewise
     __shared__ __align__(16) int totals[4];  // of the block's
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int block = blockIdx.x % a.blocks, kvh = blockIdx.x / a.blocks, request = blockIdx.y, layer = blockIdx.z;
+    for (int i = tid; i < BINS / 4; i += THREADS) reinterpret_cast<int4*>(counted)[i] = reinterpret_cast<int4*>(summed)[i] = make_int4(0, 0, 0, 0);
     let_next_kernel_start();
+    cluster_meet(a.blocks);  // the sums are zeros everywhere
     wait_for_previous_kernels();
     const int length = length_of(a, request), head = (layer * a.requests + request) * a.kv_heads + kvh;
     if (tid == 0 && block == 0 && kvh == 0 && layer == 0) {
@@ -158,68 +166,125 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
     const int* positions = a.positions + (size_t)head * a.capacity;
     float* to_weights = a.to_weights + (size_t)head * a.capacity;
     int* to_positions = a.to_positions + (size_t)head * a.capacity;
-    const bool in_place = a.to_weights == a.weights;
-    // the block's slots, a run of them for each warp
-    const int per_warp = (length + a.blocks * WARPS * 32 - 1) / (a.blocks * WARPS * 32) * 32, slot0 = block * WARPS * per_warp, warp0 = slot0 + warp * per_warp, warp_end = min(length, warp0 + per_warp);
+    const bool in_place = a.to_weights == a.weights, aligned = (((uintptr_t)weights | (uintptr_t)positions | (uintptr_t)to_weights | (uintptr_t)to_positions) & 15) == 0;
+    // the block's slots, a run of looks for each warp
+    const int per_warp = (length + a.blocks * WARPS * LOOK - 1) / (a.blocks * WARPS * LOOK) * LOOK, slot0 = block * WARPS * per_warp, warp0 = slot0 + warp * per_warp, warp_end = min(length, warp0 + per_warp);
     int n_moves = 0;
     if (length > a.keep) {
         const long long after = (long long)a.newest[request] - a.recent;
-        auto rank_at = [&](int slot) { return HOLDS ? ranks[slot - slot0] : rank_of(weights[slot], positions[slot], a.first, after); };
-        for (int i = tid; i < BINS + 2 * (1 << MORE_BITS); i += THREADS) histograms[i] = 0;
-        __syncthreads();
-#pragma unroll 4
-        for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
-            const float weight = weights[slot];
-            const int position = positions[slot];
-            const unsigned r = rank_of(weight, position, a.first, after);
-            if (HOLDS) ranks[slot - slot0] = r;
-            atomicAdd(&histograms[r >> (32 - FIRST_BITS)], 1);
-            if (!in_place && slot < a.keep) to_weights[slot] = weight, to_positions[slot] = position;  // what moves into a free one comes later
+        // a lane's four slots; 0, which is below every rank, beyond the length
+        auto fetch = [&](int slot, float (&w)[4], int (&p)[4]) {
+            if (aligned && slot + 4 <= length) {
+                load4(weights + slot, w);
+                const int4 x = *reinterpret_cast<const int4*>(positions + slot);
+                p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = slot + e < length ? weights[slot + e] : 0.f, p[e] = slot + e < length ? positions[slot + e] : 0;
+            }
+        };
+        auto ranked = [&](int slot, const float (&w)[4], const int (&p)[4], unsigned (&r)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = slot + e < length ? rank_of(w[e], p[e], a.first, after) : 0u;
+        };
+        auto ranks_at = [&](int slot, unsigned (&r)[4]) {
+            if (HOLDS) {
+                const uint4 x = *reinterpret_cast<const uint4*>(ranks + slot - slot0);
+                r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
+            } else {
+                float w[4];
+                int p[4];
+                fetch(slot, w, p), ranked(slot, w, p, r);
+            }
+        };
+        constexpr int TOGETHER = 4;  // looks that are on their way together
+        for (int base = warp0; base < warp_end; base += TOGETHER * LOOK) {
+            float w[TOGETHER][4];
+            int p[TOGETHER][4];
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k)
+                if (base + k * LOOK < warp_end) fetch(base + k * LOOK + 4 * lane, w[k], p[k]);
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k) {
+                const int slot = base + k * LOOK + 4 * lane;
+                if (base + k * LOOK >= warp_end) break;
+                unsigned r[4];
+                ranked(slot, w[k], p[k], r);
+                if (HOLDS) *reinterpret_cast<uint4*>(ranks + slot - slot0) = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (r[e]) atomicAdd(&counted[r[e] >> (32 - DIGIT)], 1);
+                if (in_place || slot >= a.keep) continue;
+                // what moves into a free one comes later
+                if (aligned && slot + 4 <= a.keep) {
+                    store4(to_weights + slot, w[k]);
+                    *reinterpret_cast<int4*>(to_positions + slot) = make_int4(p[k][0], p[k][1], p[k][2], p[k][3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (slot + e < a.keep) to_weights[slot + e] = w[k][e], to_positions[slot + e] = p[k][e];
+                }
+            }
         }
         // the rank of the last that stays, and how many of that rank do
         unsigned rank = 0;
-        int wanted = a.keep, *histogram = histograms;
+        int wanted = a.keep, digit0 = 0;
 #pragma unroll 1
-        for (int shift = 32 - FIRST_BITS;; shift -= MORE_BITS) {
-            cluster_meet(a.blocks);
-            // a thread has four bins, from the highest down
-            const int bins = shift == 32 - FIRST_BITS ? BINS : 1 << MORE_BITS, bin0 = bins - 4 - 4 * tid;
-            int4 mine = make_int4(0, 0, 0, 0);
-            if (bin0 >= 0) {
-                int4 x[MOST_BLOCKS];
-                all_of_theirs(histogram + bin0, a.blocks, x);
-#pragma unroll
-                for (int b = 0; b < MOST_BLOCKS; ++b)
-                    if (b < a.blocks) mine.x += x[b].x, mine.y += x[b].y, mine.z += x[b].z, mine.w += x[b].w;
-            }
-            const int sum = mine.x + mine.y + mine.z + mine.w;
-            int before = warp_before(sum, lane);
-            if (lane == 31) warp_sums[warp] = before + sum;
+        for (int shift = 32 - DIGIT, bits = DIGIT;;) {
             __syncthreads();
-            before += __shfl_sync(0xffffffffu, warp_before(warp_sums[lane], lane), warp);
-            if (before < wanted && before + sum >= wanted) {
-                const int n[4] = {mine.w, mine.z, mine.y, mine.x};
-                int k = 0;
-                for (; before + n[k] < wanted; ++k) before += n[k];
-                found[0] = bin0 + 3 - k, found[1] = wanted - before;
+            // a thread has four bins, from the highest down
+            const int bins = 1 << bits, bin0 = bins - 4 - 4 * tid;
+            const int* here = counted + digit0;
+            if (a.blocks > 1) {
+                if (bin0 >= 0) {
+                    const int4 x = *reinterpret_cast<const int4*>(here + bin0);
+                    if (x.x) add_to_all(summed + digit0 + bin0, x.x, a.blocks);
+                    if (x.y) add_to_all(summed + digit0 + bin0 + 1, x.y, a.blocks);
+                    if (x.z) add_to_all(summed + digit0 + bin0 + 2, x.z, a.blocks);
+                    if (x.w) add_to_all(summed + digit0 + bin0 + 3, x.w, a.blocks);
+                }
+                cluster_meet(a.blocks);
+                here = summed + digit0;
+            }
+            const int4 mine = bin0 >= 0 ? *reinterpret_cast<const int4*>(here + bin0) : make_int4(0, 0, 0, 0);
+            const int sum = mine.x + mine.y + mine.z + mine.w, warp_sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) warp_sums[warp] = warp_sum;
+            __syncthreads();
+            const int those = warp_sums[lane], before_those = warp_before(those, lane);
+            const int target = __ffs(__ballot_sync(0xffffffffu, before_those + those >= wanted)) - 1;  // the warp in whose bins it is
+            if (warp == target) {
+                int before = __shfl_sync(0xffffffffu, before_those, target) + warp_before(sum, lane);
+                if (before < wanted && before + sum >= wanted) {
+                    const int w = before + mine.w, z = w + mine.z, y = z + mine.y;
+                    found[0] = bin0 + (wanted <= w ? 3 : wanted <= z ? 2 : wanted <= y ? 1 : 0);
+                    found[1] = wanted - (wanted <= w ? before : wanted <= z ? w : wanted <= y ? z : y);
+                }
             }
             __syncthreads();
             rank |= (unsigned)found[0] << shift, wanted = found[1];
             if (shift == 0) break;
-            histogram += bins;
-            const int next = shift - MORE_BITS;
-#pragma unroll 4
-            for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
-                const unsigned r = rank_at(slot);
-                if ((r ^ rank) >> shift == 0) atomicAdd(&histogram[r >> next & ((1 << MORE_BITS) - 1)], 1);
+            digit0 += bins;
+            bits = min(shift, DIGIT);
+            const int next = shift - bits;
+            for (int slot = warp0 + 4 * lane; slot < warp_end; slot += LOOK) {
+                unsigned r[4];
+                ranks_at(slot, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (r[e] && (r[e] ^ rank) >> shift == 0) atomicAdd(&counted[digit0 + (r[e] >> next & ((1 << bits) - 1))], 1);
             }
+            shift = next;
         }
         // what each warp has
         int above_low = 0, above_high = 0, equal_low = 0, equal_high = 0;
-        for (int slot = warp0 + lane; slot < warp_end; slot += 32) {
-            const unsigned r = rank_at(slot);
-            const bool low = slot < a.keep;
-            above_low += r > rank && low, above_high += r > rank && !low, equal_low += r == rank && low, equal_high += r == rank && !low;
+        for (int slot = warp0 + 4 * lane; slot < warp_end; slot += LOOK) {
+            unsigned r[4];
+            ranks_at(slot, r);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool low = slot + e < a.keep;
+                above_low += r[e] > rank && low, above_high += r[e] > rank && !low, equal_low += r[e] == rank && low, equal_high += r[e] == rank && !low;
+            }
         }
         above_low = __reduce_add_sync(0xffffffffu, above_low), above_high = __reduce_add_sync(0xffffffffu, above_high);
         equal_low = __reduce_add_sync(0xffffffffu, equal_low), equal_high = __reduce_add_sync(0xffffffffu, equal_high);
@@ -248,17 +313,39 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
         n_moves = all.y + stay_high(all.w);
         int* from = a.from + (size_t)head * a.most;
         int* to = a.to + (size_t)head * a.most;
-        for (int slot = warp0 + lane; slot - lane < warp_end; slot += 32) {
-            const bool here = slot < warp_end, low = slot < a.keep;
-            const unsigned r = here ? rank_at(slot) : 0u, lower_lanes = (1u << lane) - 1;
-            const unsigned equal_low = __ballot_sync(0xffffffffu, here && r == rank && low), equal_high = __ballot_sync(0xffffffffu, here && r == rank && !low);
-            const int place = low ? mine.z + __popc(equal_low & lower_lanes) : all.z + mine.w + __popc(equal_high & lower_lanes);
-            mine.z += __popc(equal_low), mine.w += __popc(equal_high);
-            const bool stays = here && (r > rank || (r == rank && place < wanted));
-            const unsigned moving = __ballot_sync(0xffffffffu, stays && !low), empty = __ballot_sync(0xffffffffu, here && low && !stays);
-            if (stays && !low) from[movers + __popc(moving & lower_lanes)] = slot;
-            if (here && low && !stays) to[holes + __popc(empty & lower_lanes)] = slot;
-            movers += __popc(moving), holes += __popc(empty);
+        for (int base = warp0; base < warp_end; base += LOOK) {
+            const int slot = base + 4 * lane;
+            unsigned r[4];
+            ranks_at(slot, r);
+            bool equal = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) equal |= r[e] == rank;
+            int low_place = 0, high_place = 0;  // of this lane's first slot of the rank
+            if (__any_sync(0xffffffffu, equal)) {
+                int low_here = 0, high_here = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) low_here += r[e] == rank && slot + e < a.keep, high_here += r[e] == rank && slot + e >= a.keep;
+                const int both = low_here | high_here << 16, before = warp_before(both, lane);
+                low_place = mine.z + (before & 0xffff), high_place = all.z + mine.w + (before >> 16);
+                const int sums = __reduce_add_sync(0xffffffffu, both);
+                mine.z += sums & 0xffff, mine.w += sums >> 16;
+            }
+            unsigned moving = 0, empty = 0;  // of the four
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool low = slot + e < a.keep;
+                bool stays = r[e] > rank;
+                if (r[e] == rank) stays = (low ? low_place++ : high_place++) < wanted;
+                moving |= (stays && !low ? 1u : 0u) << e, empty |= (low && !stays ? 1u : 0u) << e;
+            }
+            const int both = __popc(moving) | __popc(empty) << 16, before = warp_before(both, lane), sums = __reduce_add_sync(0xffffffffu, both);
+            int at_from = movers + (before & 0xffff), at_to = holes + (before >> 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (moving >> e & 1) from[at_from++] = slot + e;
+                if (empty >> e & 1) to[at_to++] = slot + e;
+            }
+            movers += sums & 0xffff, holes += sums >> 16;
         }
         cluster_meet(a.blocks);
         for (int i = block * THREADS + tid; i < n_moves; i += a.blocks * THREADS) {
@@ -269,7 +356,17 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
     } else if (!in_place) {
         for (int slot = block * THREADS + tid; slot < length; slot += a.blocks * THREADS) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
     }
-    for (int slot = min(length, a.keep) + block * THREADS + tid; slot < a.capacity; slot += a.blocks * THREADS) to_weights[slot] = 0.f, to_positions[slot] = -1;
+    const int left = min(length, a.keep);
+    for (int slot = (left & ~3) + 4 * (block * THREADS + tid); slot < a.capacity; slot += 4 * a.blocks * THREADS) {
+        if (aligned && slot >= left && slot + 4 <= a.capacity) {
+            *reinterpret_cast<float4*>(to_weights + slot) = make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<int4*>(to_positions + slot) = make_int4(-1, -1, -1, -1);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (slot + e >= left && slot + e < a.capacity) to_weights[slot + e] = 0.f, to_positions[slot + e] = -1;
+        }
+    }
     if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, block * WARPS + warp, a.blocks * WARPS);
     else if (tid == 0 && block == 0) a.moves[head] = n_moves;
 }
@@ -317,12 +414,12 @@ HB_EXPORT int hb_evict(void* cache, int layers, int pages, int kv_heads, int pag
         return HB_BAD_ARGUMENT;
     if (((uintptr_t)cache | (uintptr_t)scratch) & 15 || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     const long long heads = (long long)layers * requests * kv_heads;
-    if (requests > 65535 || layers > 65535 || (long long)requests * kv_heads > 65535 || heads > 0x7fffffffLL || longest > 0x7fffffff - THREADS || record_bytes > 65536) return HB_UNSUPPORTED_SIZE;
-    if (longest > 0x7fffffff - MOST_BLOCKS * THREADS || (long long)kv_heads * MOST_BLOCKS > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
+    if (requests > 65535 || layers > 65535 || (long long)requests * kv_heads > 65535 || heads > 0x7fffffffLL || record_bytes > 65536) return HB_UNSUPPORTED_SIZE;
+    if (longest > 0x7fffffff - MOST_BLOCKS * WARPS * LOOK || capacity > 0x7fffffff - 4 * MOST_BLOCKS * THREADS || (long long)kv_heads * MOST_BLOCKS > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const int most = longest - keep < keep ? (longest > keep ? longest - keep : 0) : keep;
     int blocks = 1;
     while (blocks < MOST_BLOCKS && heads * blocks * 2 <= sms && longest >= blocks * 2 * HB_PART) blocks *= 2;
-    const size_t held = (size_t)((longest + blocks * THREADS - 1) / (blocks * THREADS)) * THREADS;
+    const size_t held = (size_t)((longest + blocks * WARPS * LOOK - 1) / (blocks * WARPS * LOOK)) * WARPS * LOOK;
     int* moves = (int*)scratch;
     int* lists = (int*)((char*)scratch + (heads * 4 + 15) / 16 * 16);
     const bool moves_here = (long long)most * 2 * record_bytes <= (long long)blocks * HB_MOVED;
