@@ -66,9 +66,9 @@ __device__ __forceinline__ void mbar_last_wait(unsigned long long* bar, unsigned
     for (unsigned spin = 0; spin < LAST_WAIT_LIMIT; ++spin)
         if (mbar_over(bar, parity)) return;
 }
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y, unsigned long long policy) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy) : "memory");
 }
 __device__ __forceinline__ unsigned turned(unsigned w) {  // an 8 x 8 matrix of 16-bit entries, two of a row a lane, transposed
     unsigned r;
@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == WARPS && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
-    let_next_kernel_start();
     wait_for_previous_kernels();
+    let_next_kernel_start();  // behind the wait: the second kernel reads what came before this one without waiting for this one
     if (warp == WARPS) {
         const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
         int request = 0, tile = 0, tiles = 0;
@@ -211,6 +211,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
         constexpr int OPS_PER_PAGE = 2 * PANELS;
         const int ops = pages_per_tile * OPS_PER_PAGE;
         const unsigned page_bytes = 2u * a.page_size * D * 2;
+        unsigned long long once;  // keys and values pass through L2, where the scores are to stay until the second kernel reads them
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
         int ok = 1;
         for (; left > 0 && ok; ++request, tile = 0) {
             const int length = length_of(a, request), here = min(left, (length + BN - 1) / BN - tile);
@@ -243,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
                     const int p = min(op, ops - 1) / OPS_PER_PAGE, rest = op % OPS_PER_PAGE, which = rest / PANELS, panel = rest - which * PANELS;
                     const int from = __shfl_sync(0xffffffffu, page, p);
                     if (op < ops && from >= 0)
-                        tma_load_2d(tiles + which * TILE + panel * (BN * 128) + p * a.page_size * 128, &kv_map, &full[s], panel * 64, ((from * 2 + which) * a.kv_heads + kvh) * a.page_size);
+                        tma_load_2d(tiles + which * TILE + panel * (BN * 128) + p * a.page_size * 128, &kv_map, &full[s], panel * 64, ((from * 2 + which) * a.kv_heads + kvh) * a.page_size, once);
                 }
             }
             left -= here;
@@ -442,18 +444,17 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
     }
 }
 
-// The second kernel: block x of a (key/value head, request) adds the weights of SPAN slots, the last x puts the request's result together.  Every block first brings the pieces' sums together.
-constexpr int ADD_THREADS = 256, SPAN = 4 * ADD_THREADS, MOST_GROUP = 64;  // heads whose sums a block holds at a time
-__global__ void __launch_bounds__(ADD_THREADS) tally_kernel(const Args a) {
-    __shared__ float2 heads_sum[MOST_GROUP];  // (m, 1 / l) of the heads
-    __shared__ int range[2];                  // the request's first block of the first kernel, and its pieces
-    let_next_kernel_start();
+// The second kernel: block x of a (key/value head, request) adds the weights of SPAN slots, four of them a thread, the last x puts the request's result together.  What the first kernel has not written is
+// read while that one still runs; behind it the scores are on their way while each block brings the pieces' sums together.
+constexpr int ADD_THREADS = 256, SPAN = 4 * ADD_THREADS, HEADS = 8;  // heads at a time
+__global__ void __launch_bounds__(ADD_THREADS, 3) tally_kernel(const Args a) {
+    __shared__ float2 heads_sum[HEADS];  // (m, 1 / l) of the heads
+    __shared__ int range[2];             // the request's first block of the first kernel, and its pieces
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, request = blockIdx.z, group = a.heads / a.kv_heads;
     const bool puts_together = blockIdx.x == gridDim.x - 1;
-    wait_for_previous_kernels();
-    const int length = length_of(a, request), first = blockIdx.x * SPAN;
-    if (tid == 0 && puts_together && kvh == 0 && a.lengths[request] > a.longest) atomicOr(a.status, HB_STATUS_BAD_POSITION);
-    if (!puts_together && first >= length) return;
+    const int length = length_of(a, request), slot0 = blockIdx.x * SPAN + 4 * tid;
+    let_next_kernel_start();
+    if (!puts_together && (int)blockIdx.x * SPAN >= length) return;
     if (length && warp == 0) {
         const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
         long long begins = 0;
@@ -463,48 +464,79 @@ __global__ void __launch_bounds__(ADD_THREADS) tally_kernel(const Args a) {
         const int b0 = block_at(begins, n, total), b1 = block_at(begins + (length + BN - 1) / BN - 1, n, total);
         if (lane == 0) range[0] = b0, range[1] = b1 - b0 + 1;
     }
+    float* weights = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + slot0;
+    const bool whole = slot0 + 4 <= length && ((uintptr_t)weights & 15) == 0;
+    float added[4] = {0.f, 0.f, 0.f, 0.f}, given[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!puts_together) {
+        if (whole) {
+            load4(weights, added);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (slot0 + e < length) added[e] = weights[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (slot0 + e == length - 1) added[e] = 0.f;  // the token's own slot enters the tally
+    }
+    if (tid == 0 && puts_together && kvh == 0 && (a.lengths[request] > a.longest || a.lengths[request] < 0)) atomicOr(a.status, HB_STATUS_BAD_POSITION);
     __syncthreads();
     const int count = length ? range[1] : 0;
     const size_t piece0 = ((size_t)(length ? range[0] : 0) + request) * a.heads + (size_t)kvh * group;  // of the group's first head
-    const size_t tally = ((size_t)request * a.kv_heads + kvh) * a.capacity;
-    float added[SPAN / ADD_THREADS] = {};
-    for (int g0 = 0; g0 < group; g0 += MOST_GROUP) {
-        const int here = min(MOST_GROUP, group - g0);
-        for (int h = warp; h < here; h += ADD_THREADS / 32) {
+    const float* scores = a.scores + ((size_t)request * a.heads + (size_t)kvh * group) * a.slots + slot0;
+    const bool mine = !puts_together && slot0 < length;  // a row of scores has whole tiles
+    wait_for_previous_kernels();
+    for (int g0 = 0; g0 < group; g0 += HEADS) {
+        const int here = min(HEADS, group - g0);
+        float y[HEADS][4];
+        if (mine) {
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h)
+                if (h < here) load4(scores + (size_t)(g0 + h) * a.slots, y[h]);
+        }
+        if (warp < here) {
             float top = -INFINITY, all = 0.f;
             for (int p = lane; p < count; p += 32) {
-                const float2 ml = a.sums[piece0 + (size_t)p * a.heads + g0 + h];
+                const float2 ml = a.sums[piece0 + (size_t)p * a.heads + g0 + warp];
                 const float above = fmaxf(top, ml.x);
                 all = above == -INFINITY ? all + ml.y : fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - above), ml.y, all * (top == -INFINITY ? 0.f : fast_exp2(top - above)));
                 top = above;
             }
             const float above = warp_max(top);
             all = warp_sum(top == -INFINITY ? all : all * fast_exp2(top - above));
-            if (lane == 0) heads_sum[h] = make_float2(above == -INFINITY ? 0.f : above, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
+            if (lane == 0) heads_sum[warp] = make_float2(above == -INFINITY ? 0.f : above, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
         }
         __syncthreads();
-        if (!puts_together) {
-            for (int h = 0; h < here; ++h) {
-                const float* row = a.scores + ((size_t)request * a.heads + (size_t)kvh * group + g0 + h) * a.slots + first;
+        if (mine) {
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) {
+                if (h >= here) break;
                 const float2 ml = heads_sum[h];
 #pragma unroll
-                for (int i = 0; i < SPAN / ADD_THREADS; ++i) {
-                    const int at = i * ADD_THREADS + tid;
-                    if (first + at < length) added[i] = fmaf(fast_exp2(row[at] - ml.x), ml.y, added[i]);
-                }
+                for (int e = 0; e < 4; ++e) given[e] = fmaf(fast_exp2(y[h][e] - ml.x), ml.y, given[e]);
             }
-        } else {
+        }
+        if (puts_together) {
             for (int at = tid; at < here * (D / 4); at += ADD_THREADS) {
                 const int h = at / (D / 4), col = at % (D / 4) * 4;
                 const float2 ml = heads_sum[h];
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int p = 0; p < count; ++p) {
-                    const size_t slot = piece0 + (size_t)p * a.heads + g0 + h;
-                    const float m = a.sums[slot].x, f = m == -INFINITY ? 0.f : fast_exp2(m - ml.x);
-                    float part[4];
-                    load4(a.pieces + slot * D + col, part);
+                constexpr int TOGETHER = 4;  // pieces that are on their way together
+                for (int p0 = 0; p0 < count; p0 += TOGETHER) {
+                    float m[TOGETHER], part[TOGETHER][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, part[e], sum[e]);
+                    for (int k = 0; k < TOGETHER; ++k) {
+                        const size_t slot = piece0 + (size_t)min(p0 + k, count - 1) * a.heads + g0 + h;
+                        m[k] = a.sums[slot].x;
+                        load4(a.pieces + slot * D + col, part[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < TOGETHER; ++k) {
+                        if (p0 + k >= count) break;
+                        const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - ml.x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, part[k][e], sum[e]);
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] *= ml.y;
@@ -513,18 +545,17 @@ __global__ void __launch_bounds__(ADD_THREADS) tally_kernel(const Args a) {
         }
         __syncthreads();
     }
-    if (puts_together) return;
+    if (!mine) return;
 #pragma unroll
-    for (int i = 0; i < SPAN / ADD_THREADS; ++i) {
-        const int slot = first + i * ADD_THREADS + tid;
-        if (slot >= length) continue;
-        if (slot == length - 1) {
-            a.weights[tally + slot] = added[i];
-            a.positions[tally + slot] = a.newest[request];
-        } else {
-            a.weights[tally + slot] += added[i];
-        }
+    for (int e = 0; e < 4; ++e) added[e] += given[e];
+    if (whole) {
+        store4(weights, added);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (slot0 + e < length) weights[e] = added[e];
     }
+    if (slot0 <= length - 1 && length - 1 < slot0 + 4) a.positions[((size_t)request * a.kv_heads + kvh) * a.capacity + length - 1] = a.newest[request];
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -588,8 +619,8 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     const int blocks = blocks_for(requests, longest, heads, kv_heads, sms);
     const size_t n_pieces = (size_t)blocks + requests;
     float* pieces = (float*)scratch;
-    float2* sums = (float2*)(pieces + n_pieces * heads * D);
-    float* scores = (float*)(sums + n_pieces * heads);
+    float* scores = pieces + n_pieces * heads * D;  // before the sums, so that its rows begin on 16 bytes
+    float2* sums = (float2*)(scores + (size_t)requests * heads * slots);
     const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, block_table, table_width, lengths, requests, longest, slots, scores, pieces, sums, weights, positions, newest, capacity,
                  heads, kv_heads, page_size, pages, gc, chunks, blocks, scale * 1.4426950408889634f, status};
     CUtensorMap map;
