@@ -583,8 +583,8 @@ int cache_map(CUtensorMap* map, const void* cache, const Args& a) {
 template <int NQ>
 int launch_strips(const Args& a, const CUtensorMap& map, cudaStream_t stream) {
     const auto kernel = attention_tallied_kernel<NQ>;
-    const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<NQ>::SMEM);
-    if (configured != cudaSuccess) return (int)configured;
+    static std::atomic<unsigned long long> allowed{0};
+    if (const cudaError_t error = allow_shared((const void*)kernel, Shape<NQ>::SMEM, allowed)) return (int)error;
     return launch_after_previous(kernel, dim3(a.blocks, a.kv_heads * a.chunks), dim3(THREADS), Shape<NQ>::SMEM, stream, map, a);
 }
 }  // namespace

@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <atomic>
+
 #define HB_EXPORT extern "C" __attribute__((visibility("default")))
 
 // Refusals a launcher reports without touching the device.
@@ -159,6 +161,17 @@ template <typename... Params, typename... Args>
 static inline int launch_after_previous(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared_bytes, cudaStream_t stream,
                                         Args&&... args) {
     return launch_in_turn(true, kernel, grid, block, shared_bytes, stream, args...);
+}
+
+// Lets a kernel have more than 48 KB of shared memory a block, once per device; `done` is the kernel's own, and zero at first.
+static inline cudaError_t allow_shared(const void* kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+    int device = 0;
+    if (cudaError_t error = cudaGetDevice(&device)) return error;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (error == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return error;
 }
 
 // The first position that a query at position `pos` sees.  window > 0: the last `window` positions (pos - window + 1 at the least);

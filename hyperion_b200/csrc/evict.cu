@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const Args a) 
 template <bool HOLDS>
 int launch_choose(const Args& a, size_t shared_bytes, cudaStream_t stream) {
     const auto kernel = evict_choose_kernel<HOLDS>;
-    const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_HELD * 4);
-    if (configured != cudaSuccess) return (int)configured;
+    static std::atomic<unsigned long long> allowed{0};
+    if (const cudaError_t error = allow_shared((const void*)kernel, MOST_HELD * 4, allowed)) return (int)error;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(a.blocks * a.kv_heads, a.requests, a.layers), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = shared_bytes, config.stream = stream;
     cudaLaunchAttribute attributes[2];

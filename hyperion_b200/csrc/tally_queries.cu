@@ -557,8 +557,8 @@ int encoded(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims
 }
 template <bool KEYS_STAY>
 int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUtensorMap& rows_map, const Args& a, dim3 grid, cudaStream_t stream) {
-    const cudaError_t configured = cudaFuncSetAttribute(tally_walk_kernel<KEYS_STAY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
-    if (configured != cudaSuccess) return (int)configured;
+    static std::atomic<unsigned long long> allowed{0};
+    if (const cudaError_t error = allow_shared((const void*)tally_walk_kernel<KEYS_STAY>, SMEM_BYTES, allowed)) return (int)error;
     return launch_after_previous(tally_walk_kernel<KEYS_STAY>, grid, dim3(THREADS), SMEM_BYTES, stream, kv_map, q_map, rows_map, a);
 }
 }  // namespace

@@ -36,26 +36,33 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
         raise KernelError(f"{what}: at most {MOST_TENSORS} tensors, not {len(caches) + len(states)}")
     if caches and block_table is None or block_table is not None and not caches:
         raise KernelError(f"{what}: a block table and the caches that it points into")
-    words, rows = [], groups * beams
+    words, rows, page_size, width = [], groups * beams, 0, 0
     if block_table is not None:
-        if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != rows or block_table.shape[1] < 1 or not block_table.is_contiguous():
+        width = block_table.shape[-1] if block_table.shape else 0
+        if block_table.dtype is not torch.int32 or block_table.shape != (rows, width) or width < 1 or not block_table.is_contiguous():
             raise KernelError(f"{what}: a dense int32 block table of {rows} rows")
         pages, page_size = caches[0].shape[1:4:2] if caches[0].dim() == 5 else (0, 0)
         for cache in caches:
-            if cache.dim() != 5 or cache.shape[1:4:2] != (pages, page_size) or pages < 1 or page_size < 1 or not cache.is_contiguous():
+            shape = cache.shape
+            if len(shape) != 5 or shape[1] != pages or shape[3] != page_size or pages < 1 or page_size < 1 or not cache.is_contiguous():
                 raise KernelError(f"{what}: caches are dense [layers, pages, outer, page, inner], all of the same pages and page size")
-            words += [cache.data_ptr(), cache.shape[0], pages, cache.shape[2], page_size, cache.shape[4] * cache.element_size(), 0]
+            words += (cache.data_ptr(), shape[0], pages, shape[2], page_size, shape[4] * cache.element_size(), 0)
     if state_rows is not None and (state_rows.dtype is not torch.int32 or state_rows.shape != (rows,) or not state_rows.is_contiguous()):
         raise KernelError(f"{what}: state_rows is a dense int32 vector of {rows}")
     for state in states:
         if state.dim() < 2 or state.shape[1] != states[0].shape[1] or not state.is_contiguous() or (state.shape[1] != rows if state_rows is None else state.shape[1] < 1):
             raise KernelError(f"{what}: states are dense [layers, {rows if state_rows is None else 'rows'}, ...]")
         layers, places = state.shape[:2]
-        words += [state.data_ptr(), layers, places, 1, 1, state.numel() // max(1, layers * places) * state.element_size(), 1]
-    _check_device(what, parents, lengths, *(tensor for tensor in (block_table, state_rows) if tensor is not None), *caches, *states)
+        words += (state.data_ptr(), layers, places, 1, 1, state.numel() // max(1, layers * places) * state.element_size(), 1)
+    tensors = [parents, lengths, *caches, *states]
+    if block_table is not None:
+        tensors.append(block_table)
+    if state_rows is not None:
+        tensors.append(state_rows)
+    _check_device(what, *tensors)
     if rows == 0 or not words:
         return
     check(entry("beam_reorder", "hb_beam_reorder", "ppiipiipippp")(
-        parents.data_ptr(), lengths.data_ptr(), groups, beams, block_table.data_ptr() if block_table is not None else 0, block_table.shape[1] if block_table is not None else 0,
-        page_size if block_table is not None else 0, (ctypes.c_longlong * len(words))(*words), len(words) // 7, state_rows.data_ptr() if state_rows is not None else 0,
+        parents.data_ptr(), lengths.data_ptr(), groups, beams, block_table.data_ptr() if block_table is not None else 0, width, page_size,
+        (ctypes.c_longlong * len(words))(*words), len(words) // 7, state_rows.data_ptr() if state_rows is not None else 0,
         status_word(parents.device).data_ptr(), stream_address()), what)

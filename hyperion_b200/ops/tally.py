@@ -15,6 +15,10 @@ from .basic import status_word
 from .native import KernelError, check, entry, scratch, sm_count, stream_address
 
 
+LARGEST = 2 ** 31 - 1
+LEAST_SCALE = 2.0 ** -100
+
+
 class Tally(NamedTuple):
     """``weights`` float32 and ``positions`` int32, both [requests, kv_heads, capacity], or [layers, requests, kv_heads, capacity]."""
     weights: torch.Tensor
@@ -32,13 +36,25 @@ def new_tally(requests: int, kv_heads: int, capacity: int, layers: Optional[int]
     return Tally(torch.zeros(shape, device=device), positions)
 
 
-def _check_tally(tally: Tally, shape: tuple, what: str) -> int:
-    """The capacity of a tally [*shape, capacity]."""
+def _check_tally(tally: Tally, shape: tuple, what: str) -> None:
+    """A tally [layers or not, requests, kv_heads, capacity], as it says itself what it holds."""
     weights, positions = tally
-    found = weights.shape
-    if (weights.dtype is not torch.float32 or positions.dtype is not torch.int32 or found[:-1] != shape or positions.shape != found or not (weights.is_contiguous() and positions.is_contiguous())):
-        raise KernelError(f"{what}: a tally is dense float32 weights and int32 positions {[*shape, 'capacity']}")
-    return found[-1]
+    if (weights.shape != shape or positions.shape != shape or weights.dtype is not torch.float32 or positions.dtype is not torch.int32 or not (weights.is_contiguous() and positions.is_contiguous())):
+        raise KernelError(f"{what}: a tally is dense float32 weights and int32 positions {[*shape[:-1], 'capacity']}")
+
+
+def _check_table(what: str, block_table: torch.Tensor, requests: int, page_size: int, longest: Optional[int], capacity: int) -> int:
+    """How long a request may be."""
+    shape = block_table.shape
+    if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] < requests or not block_table.is_contiguous():
+        raise KernelError(f"{what}: a dense int32 block table of at least {requests} rows")
+    holds = shape[1] * page_size
+    holds = holds if holds < capacity else capacity
+    if longest is None:
+        return holds
+    if not 0 <= longest <= holds:
+        raise KernelError(f"{what}: block table and tally hold {holds} slots, not {longest}")
+    return longest
 
 
 def _check_vector(what: str, name: str, vector: torch.Tensor, size: int) -> None:
@@ -46,13 +62,14 @@ def _check_vector(what: str, name: str, vector: torch.Tensor, size: int) -> None
         raise KernelError(f"{what}: {name} is a dense int32 vector of {size}")
 
 
-def _check_device(what: str, *tensors) -> int:
-    """The number of the current device, on which all of them are."""
-    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+def _check_device(what: str, *tensors) -> None:
+    """All of them are on the current device."""
+    index = tensors[0].get_device()
+    if index < 0 or index != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: all tensors on the current CUDA device, not on {tensors[0].device}")
     for tensor in tensors:
-        if tensor.get_device() != current:
+        if tensor.get_device() != index:
             raise KernelError(f"{what}: all tensors on the current CUDA device, not on {tensor.device}")
-    return current
 
 
 @lru_cache(maxsize=4096)
@@ -60,33 +77,22 @@ def _scratch_size(module: str, name: str, head_dim: int, *sizes: int) -> int:
     return entry(module, name, "i" * len(sizes), head_dim, result="l")(*sizes)
 
 
-def _check_pages(what: str, cache, heads: int, q, block_table, requests: int, longest: int, scale: float) -> tuple[int, int, int, int]:
-    """(pages, kv_heads, page_size, head_dim) of a bfloat16 cache that ``q`` is to look at."""
-    if cache.dtype is not torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
+def _check_pages(what: str, cache: torch.Tensor, heads: int, q: torch.Tensor, scale: float) -> torch.Size:
+    """[pages, 2, kv_heads, page_size, head_dim] of a bfloat16 cache that ``q`` is to look at."""
+    shape = cache.shape
+    if cache.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1] != 2 or not cache.is_contiguous():
         raise KernelError(f"{what}: a dense bfloat16 cache [pages, 2, kv_heads, page, d]")
-    pages, _, kv_heads, page_size, head_dim = cache.shape
+    _, _, kv_heads, page_size, head_dim = shape
     if not supported(head_dim, page_size):
         raise KernelError(f"{what}: heads of 64 or 128 entries and pages of 8, 16, 32 or 64 slots, not {head_dim} and {page_size}")
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise KernelError(f"{what}: {heads} heads over {kv_heads}")
-    if q.dtype is not torch.bfloat16 or q.dim() != 2 or q.shape[1] < heads * head_dim or q.stride(1) != 1:
+    queries = q.shape
+    if q.dtype is not torch.bfloat16 or len(queries) != 2 or queries[1] < heads * head_dim or q.stride(1) != 1:
         raise KernelError(f"{what}: bfloat16 queries [tokens, {heads * head_dim}] with unit inner stride")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] < requests or not block_table.is_contiguous():
-        raise KernelError(f"{what}: a dense int32 block table of at least {requests} rows")
-    if longest < 0 or block_table.shape[1] * page_size < longest:
-        raise KernelError(f"{what}: a block table of {block_table.shape[1]} pages of {page_size} does not hold {longest} slots")
-    if not scale > 0:
+    if not scale >= LEAST_SCALE:
         raise KernelError(f"{what}: a scale above 0, not {scale}")
-    return pages, kv_heads, page_size, head_dim
-
-
-def _longest(what: str, longest: Optional[int], block_table, page_size: int, capacity: int) -> int:
-    holds = min(block_table.shape[-1] * page_size, capacity)
-    if longest is None:
-        return holds
-    if not 0 <= longest <= holds:
-        raise KernelError(f"{what}: block table and tally hold {holds} slots, not {longest}")
-    return longest
+    return shape
 
 
 def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, newest: torch.Tensor, tally: Tally, scale: float, *,
@@ -102,13 +108,15 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     a captured call goes on with other lengths.  Slots beyond a length may hold anything.
 
     A call's scratch memory is 4 * heads bytes per request and slot up to ``longest``, and 4 * heads * (d + 2) per request and block: up to 16 MB are kept per thread and stream, more is allocated for the call."""
-    what, requests = "attention_tallied", q.shape[0]
-    longest = _longest(what, longest, block_table, cache.shape[3] if cache.dim() == 5 else 0, tally.weights.shape[-1])
-    pages, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, block_table, requests, longest, scale)
-    capacity, width = _check_tally(tally, (requests, kv_heads), what), heads * head_dim
+    what = "attention_tallied"
+    pages, _, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, scale)
+    weights, positions = tally
+    requests, capacity, width = q.shape[0], weights.shape[-1] if weights.shape else 0, heads * head_dim
+    _check_tally(tally, (requests, kv_heads, capacity), what)
+    longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
     _check_vector(what, "newest", newest, requests)
-    _check_device(what, q, cache, block_table, lengths, newest, *tally, q if out is None else out)
+    _check_device(what, q, cache, block_table, lengths, newest, weights, positions, q if out is None else out)
     device = q.device
     if out is None:
         out = torch.empty(requests, width, dtype=torch.bfloat16, device=device)
@@ -122,8 +130,8 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     stream, sms = stream_address(), sm_count(device)
     memory, owner = scratch(device, stream, _scratch_size("attention_tallied", "hb_attention_tallied_scratch", head_dim, requests, longest, heads, kv_heads, sms))
     check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim)(
-        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, tally.weights.data_ptr(),
-        tally.positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
+        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, weights.data_ptr(),
+        positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
     return out
 
 
@@ -137,10 +145,11 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     infinity among the scores that a query sees makes the weights of those slots NaN.
 
     A call's scratch memory is at least 8 * heads bytes per query, and where few queries look at many slots as much again for each cut of those."""
-    what, requests, tokens = "tally_queries", lengths.shape[0], q.shape[0]
-    longest = _longest(what, longest, block_table, cache.shape[3] if cache.dim() == 5 else 0, tally.weights.shape[-1])
-    pages, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, block_table, requests, longest, scale)
-    capacity = _check_tally(tally, (requests, kv_heads), what)
+    what = "tally_queries"
+    pages, _, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, scale)
+    requests, tokens, capacity = lengths.numel(), q.shape[0], tally.weights.shape[-1] if tally.weights.shape else 0
+    _check_tally(tally, (requests, kv_heads, capacity), what)
+    longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
     _check_vector(what, "starts", starts, requests + 1)
     if most < 0:
@@ -173,35 +182,36 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     long and is reported (``raise_on_status``).  A move from or to a page that is not there is left out and reported.
 
     A call's scratch memory is 8 bytes for each of the min(keep, longest - keep) moves that a head of a layer and request can have."""
-    what, requests = "evict", lengths.shape[0]
-    layered = cache.dim() == 6
-    if cache.dim() not in (5, 6) or cache.shape[-4] != 2 or not cache.is_contiguous():
+    what, shape = "evict", cache.shape
+    layered = len(shape) == 6
+    if len(shape) not in (5, 6) or shape[-4] != 2 or not cache.is_contiguous():
         raise KernelError(f"{what}: a dense cache [layers, pages, 2, kv_heads, page, d], or without the layers")
-    layers, (pages, _, kv_heads, page_size, head_dim) = cache.shape[0] if layered else 1, cache.shape[-5:]
+    layers, pages, _, kv_heads, page_size, head_dim = shape if layered else (1, *shape)
     record = head_dim * cache.element_size()
     if page_size & (page_size - 1) or page_size == 0 or record == 0 or record % 16 or record > 65536:
         raise KernelError(f"{what}: pages of a power of two and records of whole 16 bytes, not {page_size} and {record}")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] < requests or not block_table.is_contiguous():
-        raise KernelError(f"{what}: a dense int32 block table of at least {requests} rows")
-    shape = (layers, requests, kv_heads) if layered else (requests, kv_heads)
-    capacity = _check_tally(tally, shape, what)
-    to = tally if out is None else out
-    if _check_tally(to, shape, what) != capacity or (to.weights.data_ptr() == tally.weights.data_ptr()) != (to.positions.data_ptr() == tally.positions.data_ptr()):
-        raise KernelError(f"{what}: the new tally is as large as the old one, and all of it in its place or none")
+    weights, positions = tally
+    to_weights, to_positions = to = tally if out is None else out
+    requests, capacity = lengths.numel(), weights.shape[-1] if weights.shape else 0
+    held = (layers, requests, kv_heads, capacity) if layered else (requests, kv_heads, capacity)
+    _check_tally(tally, held, what)
+    if to is not tally:
+        _check_tally(to, held, what)
+        if (to_weights.data_ptr() == weights.data_ptr()) != (to_positions.data_ptr() == positions.data_ptr()):
+            raise KernelError(f"{what}: the new tally takes the place of all of the old one, or of none of it")
+    longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
     _check_vector(what, "newest", newest, requests)
-    if keep < 1 or first < 0 or recent < 0:
-        raise KernelError(f"{what}: keep at least 1, first and recent at least 0, not {keep}, {first} and {recent}")
-    longest = _longest(what, longest, block_table, page_size, capacity)
-    _check_device(what, cache, block_table, lengths, newest, *tally, *to)
+    if not (1 <= keep <= LARGEST and 0 <= first <= LARGEST and 0 <= recent <= LARGEST):
+        raise KernelError(f"{what}: keep from 1, first and recent from 0 to {LARGEST}, not {keep}, {first} and {recent}")
+    _check_device(what, cache, block_table, lengths, newest, weights, positions, to_weights, to_positions)
     device = cache.device
     left = torch.empty(requests, dtype=torch.int32, device=device)
     if requests == 0 or layers == 0 or kv_heads == 0 or longest == 0:
         return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
-    keep, first, recent = (min(value, 2**31 - 1) for value in (keep, first, recent))
     stream = stream_address()
     memory, owner = scratch(device, stream, _scratch_size("evict", "hb_evict_scratch", 0, layers, requests, kv_heads, longest, keep))
     check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppip")(
-        cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, tally.weights.data_ptr(),
-        tally.positions.data_ptr(), to.weights.data_ptr(), to.positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), sm_count(device), stream), what)
+        cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, weights.data_ptr(),
+        positions.data_ptr(), to_weights.data_ptr(), to_positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), sm_count(device), stream), what)
     return left

@@ -29,14 +29,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamCh
 
     A logit of -infinity or NaN is no continuation (+infinity counts as the largest number), nor is anything of a beam whose score is -infinity or NaN: a group begins with one beam at 0 and the others at
     -infinity.  Where there are fewer than ``take``, the places left have parent -1, token -1 and score -infinity."""
-    if scores.dtype is not torch.float32 or scores.dim() != 2 or not scores.is_contiguous() or not 1 <= scores.shape[1] <= MOST_BEAMS:
+    held, shape = scores.shape, logits.shape
+    if scores.dtype is not torch.float32 or len(held) != 2 or not scores.is_contiguous() or not 1 <= held[1] <= MOST_BEAMS:
         raise KernelError(f"beam_select: scores are dense float32 [groups, beams], 1 to {MOST_BEAMS} beams")
-    groups, beams = scores.shape
-    if logits.dim() != 2 or logits.shape[0] != groups * beams or logits.shape[1] < 1 or logits.stride(1) != 1 or (groups * beams > 1 and logits.stride(0) < logits.shape[1]):
-        raise KernelError(f"beam_select: logits [{groups * beams}, vocab] with unit inner stride, rows that do not overlap")
+    groups, beams = held
+    rows = groups * beams
+    if len(shape) != 2 or shape[0] != rows or shape[1] < 1 or logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < shape[1]):
+        raise KernelError(f"beam_select: logits [{rows}, vocab] with unit inner stride, rows that do not overlap")
     if not 1 <= take <= MOST_TAKE:
         raise KernelError(f"beam_select: 1 to {MOST_TAKE} continuations, not {take}")
-    kind, device, vocab = is_bf16(logits), logits.device, logits.shape[1]
+    kind, device, vocab = is_bf16(logits), logits.device, shape[1]
     _check_device("beam_select", logits, scores)
     answer = torch.empty(3, groups, take, dtype=torch.int32, device=device)
     parents, tokens, found = answer[0], answer[1], answer[2].view(torch.float32)
@@ -44,7 +46,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamCh
         return BeamChoice(parents, tokens, found)
     stream, sms = stream_address(), sm_count(device)
     memory, owner = scratch(device, stream, _scratch_size("beam_select", "hb_beam_select_scratch", 0, groups, beams, vocab, take, sms))
-    check(entry("beam_select", "hb_beam_select", "pilpiiiipppipp")(logits.data_ptr(), kind, max(logits.stride(0), vocab), scores.data_ptr(), groups, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(),
+    check(entry("beam_select", "hb_beam_select", "pilpiiiipppipp")(logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab, scores.data_ptr(), groups, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(),
                                                              found.data_ptr(), sms, memory, stream), "beam_select")
     return BeamChoice(parents, tokens, found)
 

@@ -78,7 +78,7 @@ def test_evict(change):
 
 def test_evict_half_in_place():
     tally = Tally(torch.zeros(3, 2, 2, 48), ints(3, 2, 2, 48))
-    with pytest.raises(KernelError, match="all of it in its place or none"):
+    with pytest.raises(KernelError, match="takes the place of all of the old one"):
         evicted(tally=tally, out=Tally(tally.weights, ints(3, 2, 2, 48)))()
 
 
