@@ -36,7 +36,7 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int BM = 128;                        // rows that stay, and rows that pass
 constexpr int PANEL = BM * 128, PANELS = D / 64, TILE = PANELS * PANEL;  // bytes
 constexpr int STAGES = D == 128 ? 2 : 4;       // of the ring: two blocks share an SM's memory
-constexpr int SPAN = 16;                       // tiles of Q that pass one block
+constexpr int SPAN = 16, MOST_SPANS = 16;      // tiles of Q that pass one block at least; blocks that they pass at most, each of which leaves a part of the sums
 constexpr int HALF = 4, PRODUCER = 2 * HALF, ISSUER = PRODUCER + 1, THREADS = 32 * (ISSUER + 1);  // warps that look at scores: four for each of the two buffers
 constexpr int TMEM_COLS = 2 * BM;              // two blocks have all of an SM's
 constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
@@ -208,7 +208,7 @@ struct Args {
     float2* cuts;         // [n_cuts, tokens * heads]: (m, l), where the slots are cut
     int n_cuts;
     float* parts;         // [spans, requests, kv_heads, padded]: a span's part of the slots' sums, where there is more than one
-    int spans, padded;    // spans of tiles of Q; slots in whole tiles
+    int span, spans, padded;  // tiles of Q that pass a block, and into how many such spans they go; slots in whole tiles
     int heads, kv_heads, group, page_shift, pages;
     int per_tile;         // tokens of a tile of Q
     float scale_log2;
@@ -237,7 +237,7 @@ __device__ __forceinline__ uint4 beside_row(float m, float l, float c) {
 }
 __device__ __forceinline__ int first_tile(const Args& a, int slot, int before) { return max(0, slot - before) / a.per_tile; }  // token slot - before is the first that sees the slot
 
-// One walk.  KEYS_STAY: block (span of tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (cut, tile of Q and key/value head, request), tiles of K pass.
+// One walk.  KEYS_STAY: block (span of tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (tile of Q and key/value head, cut, request), tiles of K pass.
 template <bool KEYS_STAY>
 __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap rows_map, const Args a) {
     extern __shared__ unsigned char smem_raw[];
@@ -266,13 +266,12 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
         if (KEYS_STAY) asm volatile("prefetch.tensormap [%0];" ::"l"(&rows_map) : "memory");
     }
-    // The second walk waits only before it asks for what stands beside the rows: its blocks are let in once all of the first walk's have their tensor memory, so what came before that one has finished.
     if (!KEYS_STAY) wait_for_previous_kernels();
-    const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.y % a.kv_heads, group = a.group;
+    const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.x % a.kv_heads, group = a.group;
     const Request r = request_of(a, request, !KEYS_STAY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
     const int before = r.length - r.tokens;  // token i sees before + i + 1 slots
     const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile;
-    const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.y / a.kv_heads - 1 - blockIdx.y / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
+    const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
     int from, to;  // tiles that pass
     if (KEYS_STAY) {
         if (base >= r.length || r.tokens == 0) {
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             return;
         }
         const int span = blockIdx.x % a.spans;
-        from = max(span * SPAN, first_tile(a, base, before)), to = min(q_tiles, (span + 1) * SPAN);
+        from = max(span * a.span, first_tile(a, base, before)), to = min(q_tiles, (span + 1) * a.span);
         if (from >= to) {
             wait_for_previous_kernels();
             return;
@@ -288,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     } else {
         if (base >= r.tokens) return;
         const int reach = min(r.length, max(0, before + min(base + a.per_tile, r.tokens))), n = (reach + BM - 1) / BM;  // slots that any of the tokens sees
-        from = (int)((long long)n * blockIdx.x / a.n_cuts), to = (int)((long long)n * (blockIdx.x + 1) / a.n_cuts);
+        from = (int)((long long)n * blockIdx.y / a.n_cuts), to = (int)((long long)n * (blockIdx.y + 1) / a.n_cuts);
     }
     const int n_tiles = to - from;
     // rows of Q's tiles that no copy writes (beyond whole tokens)
@@ -306,46 +305,48 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             if (second || !tile || row >= q_rows) reinterpret_cast<uint4*>(beside_stays)[e] = x;
         }
     }
-    // Tensor memory is taken only now that no kernel before wants any more of it (those before the first walk have finished, and the first walk's blocks have theirs), and the next kernel is let in only once it is:
-    // a block further back or further on that holds some while it waits could wait for this one.
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    const int page_size = 1 << a.page_shift, pages_per_tile = BM >> a.page_shift;
+    const int* table = a.block_table + (size_t)request * a.table_width;
+    auto page_at = [&](int slot0) {  // this lane's page of the tile of K from slot0 on; -1: none
+        const int k0 = slot0 + lane * page_size;
+        if (lane >= pages_per_tile || k0 >= r.length) return -1;
+        const int id = __ldg(table + (k0 >> a.page_shift));
+        if (id >= 0 && id < a.pages) return id;
+        atomicOr(a.status, HB_STATUS_BAD_PAGE);
+        return -1;
+    };
+    auto fetch_keys = [&](unsigned char* tile, int page, unsigned long long* bar) {
+        const unsigned valid = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) {
+            if (valid) mbar_expect_tx(bar, valid * page_size * D * 2u); else mbar_arrive(bar);
+        }
+        __syncwarp();
+        const int ops = pages_per_tile * PANELS;  // at most 32
+        const int p = min(lane, ops - 1) / PANELS, h = lane % PANELS, id = __shfl_sync(0xffffffffu, page, p);
+        if (lane < ops && id >= 0) tma_load_2d(tile + h * PANEL + p * page_size * 128, &kv_map, bar, h * 64, (id * 2 * a.kv_heads + kvh) << a.page_shift);
+    };
+    // The second walk's tile is on its way while the first one ends: its blocks are let in once all of the first walk's have waited, so what came before that one has finished.
+    if (KEYS_STAY) {
+        if (warp == PRODUCER) fetch_keys(stays, page_at(base), stays_full);
+        wait_for_previous_kernels();
+    }
+    // Tensor memory is taken only now that the kernels before have finished, and the next kernel is let in only once it is: a block further back or further on that holds some while it waits could wait for this one.
     if (warp == ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     let_next_kernel_start();
     tc_fence_after();
     const unsigned tmem = *tmem_slot;
 
-    if (KEYS_STAY && warp != PRODUCER) wait_for_previous_kernels();  // not at the barriers, where looking takes turns from the first walk's last blocks (three prompts 196 us)
     if (warp == PRODUCER) {
         // ------------------------------------------------------------------ the whole warp
-        const int page_size = 1 << a.page_shift, pages_per_tile = BM >> a.page_shift;
-        const int* table = a.block_table + (size_t)request * a.table_width;
-        auto page_at = [&](int slot0) {  // this lane's page of the tile of K from slot0 on; -1: none
-            const int k0 = slot0 + lane * page_size;
-            if (lane >= pages_per_tile || k0 >= r.length) return -1;
-            const int id = __ldg(table + (k0 >> a.page_shift));
-            if (id >= 0 && id < a.pages) return id;
-            atomicOr(a.status, HB_STATUS_BAD_PAGE);
-            return -1;
-        };
-        auto fetch_keys = [&](unsigned char* tile, int page, unsigned long long* bar) {
-            const unsigned valid = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            if (lane == 0) {
-                if (valid) mbar_expect_tx(bar, valid * page_size * D * 2u); else mbar_arrive(bar);
-            }
-            __syncwarp();
-            const int ops = pages_per_tile * PANELS;  // at most 32
-            const int p = min(lane, ops - 1) / PANELS, h = lane % PANELS, id = __shfl_sync(0xffffffffu, page, p);
-            if (lane < ops && id >= 0) tma_load_2d(tile + h * PANEL + p * page_size * 128, &kv_map, bar, h * 64, (id * 2 * a.kv_heads + kvh) << a.page_shift);
-        };
-        [[maybe_unused]] bool waited = false;
         auto fetch_queries = [&](unsigned char* tile, int token, unsigned long long* bar) {  // tokens beyond the request's own come along, or are filled with zeros
             if (lane == 0) {
-                if (KEYS_STAY && !waited) wait_for_previous_kernels(), waited = true;
                 mbar_expect_tx(bar, (unsigned)((PANELS * 128 + (KEYS_STAY ? 16 : 0)) * q_rows));
                 for (int h = 0; h < PANELS; ++h) tma_load_3d(tile + h * PANEL, &q_map, bar, h * 64, kvh * group, r.first + token);
                 if (KEYS_STAY) tma_load_3d(beside + (tile - ring) / TILE * BESIDE, &rows_map, bar, 0, kvh * group, r.first + token);
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         };
         int sent = 0;
         if (n_tiles > 0) {
-            if (KEYS_STAY) fetch_keys(stays, page_at(base), stays_full); else fetch_queries(stays, base, stays_full);
+            if (!KEYS_STAY) fetch_queries(stays, base, stays_full);
             int page = KEYS_STAY ? 0 : page_at(from * BM);
             for (int i = 0; i < n_tiles; ++i, ++sent) {
                 const int s = i % STAGES;
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
                 l = (m == -INFINITY ? l : l * fast_exp2(m - above)) + (other == -INFINITY ? theirs[BM + mine] : theirs[BM + mine] * fast_exp2(other - above));
                 const size_t at = (size_t)(r.first + token) * a.heads + my_head;
                 if (a.n_cuts == 1) a.rows[at] = beside_row(above, l, c);
-                else a.cuts[(size_t)blockIdx.x * a.tokens * a.heads + at] = make_float2(above, l);
+                else a.cuts[(size_t)blockIdx.y * a.tokens * a.heads + at] = make_float2(above, l);
             }
         }
     }
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(256) tally_parts_kernel(const Args a) {
     const int slot = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, request = blockIdx.z;
     const Request r = request_of(a, request, false);
     if (slot >= r.length) return;
-    const int first = first_tile(a, slot / BM * BM, r.length - r.tokens) / SPAN, end = ((r.tokens + a.per_tile - 1) / a.per_tile + SPAN - 1) / SPAN;  // spans that the tile of slots has a block for
+    const int first = first_tile(a, slot / BM * BM, r.length - r.tokens) / a.span, end = ((r.tokens + a.per_tile - 1) / a.per_tile + a.span - 1) / a.span;  // spans that the tile of slots has a block for
     float* weight = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + slot;
     const float before = *weight;
     float sum = 0.f;
@@ -569,13 +570,19 @@ static int cuts_for(int requests, int most, int longest, int heads, int kv_heads
     const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = (longest + BM - 1) / BM;
     return (int)(wanted < 1 ? 1 : wanted < most_cuts ? wanted : most_cuts);
 }
-static int spans_for(int most, int group) { return ((most + BM / group - 1) / (BM / group) + SPAN - 1) / SPAN; }
+static int span_for(int most, int group, int* spans) {
+    const int tiles = (most + BM / group - 1) / (BM / group), span = (tiles + MOST_SPANS - 1) / MOST_SPANS > SPAN ? (tiles + MOST_SPANS - 1) / MOST_SPANS : SPAN;
+    *spans = (tiles + span - 1) / span;
+    return span;
+}
 // Bytes of scratch that hb_tally_queries takes.
 HB_EXPORT long long hb_tally_queries_scratch(int tokens, int requests, int most, int longest, int heads, int kv_heads, int sms) {
     if (tokens <= 0 || requests <= 0 || most <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > BM || sms <= 0) return 0;
     const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
-    const long long spans = spans_for(most, heads / kv_heads), padded = (longest + BM - 1) / BM * (long long)BM;
-    return 16LL * tokens * heads + (cuts > 1 ? 8LL * tokens * heads * cuts : 0) + (spans > 1 ? 4 * spans * requests * kv_heads * padded : 0);
+    int spans;
+    span_for(most, heads / kv_heads, &spans);
+    const long long padded = (longest + BM - 1) / BM * (long long)BM;
+    return 16LL * tokens * heads + (cuts > 1 ? 8LL * tokens * heads * cuts : 0) + (spans > 1 ? 4LL * spans * requests * kv_heads * padded : 0);
 }
 // q [tokens, heads * D] with rows q_stride apart, request r's from starts[r] to starts[r + 1] - 1, at most `most`, the last of which stands in its last slot; cache [pages, 2, kv_heads, page_size, D];
 // lengths [requests], at most `longest`, which table and capacity hold; weights [requests, kv_heads, capacity].  scratch: hb_tally_queries_scratch bytes on a 16-byte boundary.
@@ -590,8 +597,9 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     if (q_stride > 0x7fffffffLL || (long long)tokens * heads > 0x7fffffffLL - 256 || longest > 0x7fffffff - BM || requests > 65535 || kv_heads > 65535) return HB_UNSUPPORTED_SIZE;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     const long long row_blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads;
-    if (row_blocks > 65535) return HB_UNSUPPORTED_SIZE;
-    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), spans = spans_for(most, group), padded = (longest + BM - 1) / BM * BM;
+    if (row_blocks > 0x7fffffffLL || sms > 16384) return HB_UNSUPPORTED_SIZE;
+    int spans;
+    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), span = span_for(most, group, &spans), padded = (longest + BM - 1) / BM * BM;
     if ((long long)padded / BM * spans > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     CUtensorMap kv_map, q_map, rows_map;
     const cuuint64_t kv_dims[2] = {(cuuint64_t)D, (cuuint64_t)pages * 2 * kv_heads * page_size}, kv_strides[1] = {(cuuint64_t)D * 2};
@@ -606,9 +614,9 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     const cuuint32_t rows_box[3] = {8, (cuuint32_t)group, (cuuint32_t)per_tile};
     if (int code = encoded(&rows_map, rows, 3, rows_dims, rows_strides, rows_box, CU_TENSOR_MAP_SWIZZLE_NONE)) return code;
     float2* cut_sums = (float2*)(rows + (size_t)tokens * heads);
-    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, (float*)(cut_sums + (cuts > 1 ? (size_t)tokens * heads * cuts : 0)), spans, padded, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
+    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, (float*)(cut_sums + (cuts > 1 ? (size_t)tokens * heads * cuts : 0)), span, spans, padded, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
                  scale * 1.4426950408889634f, status};
-    if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3(cuts, (unsigned)row_blocks, requests), stream)) return code;
+    if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3((unsigned)row_blocks, cuts, requests), stream)) return code;
     if (cuts > 1)
         if (int code = launch_after_previous(tally_cuts_kernel, dim3((tokens * heads + 255) / 256), dim3(256), 0, stream, a)) return code;
     if (int code = launch_walk<true>(kv_map, q_map, rows_map, a, dim3(padded / BM * spans, kv_heads, requests), stream)) return code;

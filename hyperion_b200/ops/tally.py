@@ -130,7 +130,7 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     stream, sms = stream_address(), sm_count(device)
     memory, owner = scratch(device, stream, _scratch_size("attention_tallied", "hb_attention_tallied_scratch", head_dim, requests, longest, heads, kv_heads, sms))
     check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim)(
-        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, weights.data_ptr(),
+        q.data_ptr(), q.stride(0) if requests > 1 else width, out.data_ptr(), out.stride(0) if requests > 1 else width, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, weights.data_ptr(),
         positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
     return out
 
@@ -144,7 +144,8 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  What is beyond them is left out and reported (``raise_on_status``).  A NaN or an
     infinity among the scores that a query sees makes the weights of those slots NaN.
 
-    A call's scratch memory is at least 8 * heads bytes per query, and where few queries look at many slots as much again for each cut of those."""
+    A call's scratch memory is 16 * heads bytes per query, 8 * heads more for each of the cuts into which slots go where few queries look at many (two blocks a multiprocessor in all), and for prompts of more
+    than 2,048 (token, head) rows a key/value head 4 * kv_heads bytes per request, slot up to ``longest`` and span of those rows, 16 spans at most: up to 16 MB are kept per thread and stream, more is allocated for the call."""
     what = "tally_queries"
     pages, _, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, scale)
     requests, tokens, capacity = lengths.numel(), q.shape[0], tally.weights.shape[-1] if tally.weights.shape else 0
@@ -164,7 +165,7 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     stream, sms = stream_address(), sm_count(device)
     memory, owner = scratch(device, stream, _scratch_size("tally_queries", "hb_tally_queries_scratch", head_dim, tokens, requests, most, longest, heads, kv_heads, sms))
     check(entry("tally_queries", "hb_tally_queries", "plippippiiipiiiiifippp", head_dim)(
-        q.data_ptr(), q.stride(0), tokens, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], starts.data_ptr(), lengths.data_ptr(), requests, most, longest, tally.weights.data_ptr(), capacity,
+        q.data_ptr(), q.stride(0) if tokens > 1 else heads * head_dim, tokens, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], starts.data_ptr(), lengths.data_ptr(), requests, most, longest, tally.weights.data_ptr(), capacity,
         heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
 
 

@@ -109,7 +109,7 @@ def test_weights_of_all_kinds():
         run([777, 900], keep=keep, change=change, seed=keep, separate=keep == 300)
 
 
-@pytest.mark.parametrize("length,keep,layers,kv", [(40001, 9000, 1, 2), (9001, 9000, 2, 1), (33000, 1, 1, 1), (70000, 69000, 1, 1)])
+@pytest.mark.parametrize("length,keep,layers,kv", [(300000, 200, 1, 1), (40001, 9000, 1, 2), (9001, 9000, 2, 1), (33000, 1, 1, 1), (70000, 69000, 1, 1)])
 def test_long_requests(length, keep, layers, kv):
     run([length], layers=layers, kv=kv, dim=16, page=64, keep=keep, first=4, recent=min(keep, 64))
 
