@@ -7,9 +7,12 @@
 // A weight is known only when its head's whole row has been seen, so the scores themselves are kept until then: 4 bytes a head and slot beside the 4 d bytes of a key and a value.  (Reading the
 // keys a second time would cost 2 d bytes a slot against 8 a head and slot for writing the scores and reading them back.)
 //
-// The first kernel walks keys and values.  The lengths stay on the device: the requests' slots stand in a line, in tiles of 64, and each of the blocks works out where its equal share of the line begins
-// and ends.  A share's part of one request is a piece (m, l and o of its heads); block b's piece of request r has the number b + r, which grows along the line and so is no other one's.  The second
-// kernel puts the pieces of a request together, in the order of the line, and adds the weights.
+// Where there is much to do there are two kernels.  The first walks keys and values.  The lengths stay on the device: the requests' slots stand in a line, in tiles of 64, and each of the blocks works out where its
+// equal share of the line begins and ends.  A share's part of one request is a piece (m, l and o of its heads); block b's piece of request r has the number b + r, which grows along the line and so is no other one's.
+// The second kernel puts the pieces of a request together, in the order of the line, and adds the weights; the scores between the two stay in L2, which keys and values only pass through.
+//
+// Where there is little, a request and key/value head is a cluster's of one to eight blocks: each walks its share and keeps its scores in shared memory, then they read one another's results there (mapa,
+// ld.shared::cluster) and add the weights of their own slots.
 //
 // In a block one lane of a producer warp per page fetches keys and values by TMA into a ring of stages, and each of four warps takes 16 of a stage's 64 slots for all rows.  The products are
 // S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): slots and entries stand where the instruction has 16 rows, the few heads of a key/value head where it has 8 columns.  The weights are taken into the second
@@ -124,6 +127,7 @@ struct Args {
     int heads, kv_heads, page_size, pages;
     int gc, chunks;          // heads of a strip, strips of a key/value head's group
     int blocks;              // of the first kernel, side by side
+    int together, kept;      // or 0, or the blocks of a cluster, which has one request and key/value head; slots whose scores each of them keeps
     float scale_log2;
     int* status;
 };
@@ -165,8 +169,31 @@ __device__ __forceinline__ int request_at(const Args& a, long long at, long long
 __device__ __forceinline__ long long share_from(long long b, long long n, long long total) { return b * total / n; }
 __device__ __forceinline__ int block_at(long long at, long long n, long long total) { return (int)(((at + 1) * n - 1) / total); }
 
-template <int NQ>
-__global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
+// A kept row of scores is 4 floats longer than its slots: lanes that store side by side then take different banks.
+__host__ __device__ constexpr size_t kept_bytes(int rows, int kept) { return 32 + (size_t)rows * ((kept + 4) * 4 + 8); }
+constexpr int MOST_TOGETHER = 8, KEPT_LOADS = 8, MOST_KEPT = KEPT_LOADS * 32 * WARPS;  // slots that a block keeps, KEPT_LOADS of a thread
+// The blocks of a cluster.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ unsigned their(const void* p, int rank) {  // what another block of the cluster has at this place of its shared memory
+    unsigned at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float2 theirs2(const float2* p, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(their(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 theirs4(const float* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(their(p, rank)) : "memory");
+    return v;
+}
+
+// TOGETHER: the blocks of a cluster share one request's slots of one key/value head (all of whose query heads a strip has), keep their scores in shared memory, and end with the result and the weights.
+template <int NQ, bool TOGETHER>
+__global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape<NQ>::BLOCKS)) attention_tallied_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
     typedef Shape<NQ> S;
     constexpr int ROWS = S::ROWS;
     extern __shared__ unsigned char smem_raw[];
@@ -179,6 +206,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
     volatile int* failed = reinterpret_cast<volatile int*>(empty + S::STAGES);
     volatile int* lost = failed + 1;  // a computing warp has given up
     int* share = const_cast<int*>(failed) + 2;  // first request, its first tile here, tiles in all
+    [[maybe_unused]] float2* factors = reinterpret_cast<float2*>((reinterpret_cast<uintptr_t>(share + 4) + 15) & ~(uintptr_t)15);  // TOGETHER: [ROWS]: (m, 1 / l) of the request's rows
+    [[maybe_unused]] float* kept = reinterpret_cast<float*>(factors + ROWS);                                                   // [ROWS][a.kept + 4]
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
@@ -189,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
     if (warp == WARPS && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
     wait_for_previous_kernels();
     let_next_kernel_start();  // behind the wait: the second kernel reads what came before this one without waiting for this one
-    if (warp == WARPS) {
+    if (!TOGETHER && warp == WARPS) {
         const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
         int request = 0, tile = 0, tiles = 0;
         if ((long long)blockIdx.x < n) {
@@ -203,7 +232,16 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
     __syncthreads();
     const int kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
     const int group = a.heads / a.kv_heads, first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
-    int request = share[0], tile = share[1], left = share[2], stage = 0;  // the ring runs on across the block's requests
+    int request, tile, left, stage = 0;  // the ring runs on across the block's requests
+    [[maybe_unused]] int rank = 0;
+    if constexpr (TOGETHER) {
+        request = blockIdx.x / a.together, rank = blockIdx.x % a.together;
+        const long long n = tiles_of(a, request);
+        tile = (int)(n * rank / a.together), left = (int)(n * (rank + 1) / a.together) - tile;
+        if (tid == 0 && rank == 0 && kvh == 0 && (a.lengths[request] > a.longest || a.lengths[request] < 0)) atomicOr(a.status, HB_STATUS_BAD_POSITION);
+    } else {
+        request = share[0], tile = share[1], left = share[2];
+    }
 
     if (warp == WARPS) {
         // ------------------------------------------------------------------ producer (the whole warp)
@@ -252,6 +290,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
         }
         if (lane == 0)
             for (int k = max(0, stage - S::STAGES); k < stage; ++k) mbar_last_wait(&full[k % S::STAGES], (k / S::STAGES) & 1);
+        __syncwarp();
+        if constexpr (TOGETHER) cluster_arrive(), cluster_wait(), cluster_arrive(), cluster_wait();
         return;
     }
     // ---------------------------------------------------------------------- consumers
@@ -260,7 +300,12 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
     constexpr int LANES_PER_ROW = S::COLS / 16;
     const int store_row = lane / LANES_PER_ROW, store_col = warp * (S::COLS / 4) + lane % LANES_PER_ROW * 4;  // what this lane stores of every COLS entries
     const bool stores = store_row < heads_here;
-    for (; left > 0; ++request, tile = 0) {
+    [[maybe_unused]] float* rows_here = reinterpret_cast<float*>(ring);                    // TOGETHER: [ROWS][D], what the block brings; the ring has been read to its end by then
+    [[maybe_unused]] float2* sums_here = reinterpret_cast<float2*>(rows_here + ROWS * D);  // [ROWS]
+    static_assert(ROWS * (D * 4 + 8) <= S::STAGES * 2 * TILE, "a cluster's results lie where the ring was");
+    bool once = TOGETHER;  // a block of a cluster has its part in it without slots, too
+    for (; left > 0 || once; ++request, tile = 0) {
+        once = false;
         const int length = length_of(a, request), here = min(left, (length + BN - 1) / BN - tile), start = tile * BN;
         left -= here;
         // Q's fragments: a lane's 16-byte chunk t + 4 j of a key feeds products 2 j and 2 j + 1, four of its entries each, so a query's entries stand in the fragments likewise.
@@ -281,7 +326,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int head = q * 8 + 2 * t + e;
-                scores[q][e] = head < heads_here ? a.scores + ((size_t)request * a.heads + first_head + head) * a.slots : nullptr;
+                if constexpr (TOGETHER) scores[q][e] = kept + (size_t)head * (a.kept + 4) - start;  // all rows: those that are no one's are not added up
+                else scores[q][e] = head < heads_here ? a.scores + ((size_t)request * a.heads + first_head + head) * a.slots : nullptr;
             }
         float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];
 #pragma unroll
@@ -323,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
                         sc[q][e] *= a.scale_log2;
                         const int pos = pos0 + (e >> 1) * 8 + g;
                         if (!whole && pos >= length) sc[q][e] = -INFINITY;
-                        else if (scores[q][e & 1]) scores[q][e & 1][pos] = sc[q][e];
+                        else if (TOGETHER || scores[q][e & 1]) scores[q][e & 1][pos] = sc[q][e];
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -396,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
                 if (g == 0) tops[warp * ROWS + q * 8 + 2 * t + e] = m[q][e], parts[warp * ROWS + q * 8 + 2 * t + e] = l[q][e];
             }
         meet();
-        if (*lost) break;  // all four warps see the same: they set it before they come here only
+        if (*lost && !TOGETHER) break;  // all four warps see the same: they set it before they come here only.  (A cluster's blocks leave together, whatever it is that they join.)
         float f[NQ][2];
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
@@ -415,7 +461,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
             all = fmaf(mw == -INFINITY ? 0.f : fast_exp2(mw - top), parts[w * ROWS + store_row], all);
         }
         const size_t slot = ((size_t)blockIdx.x + request) * a.heads + first_head + store_row;
-        if (stores && store_col == 0) a.sums[slot] = make_float2(top, all);
+        if (!TOGETHER && stores && store_col == 0) a.sums[slot] = make_float2(top, all);
+        if (TOGETHER && store_col == 0) sums_here[store_row] = make_float2(top, all);
 #pragma unroll
         for (int col = 0; col < D; col += S::COLS) {
 #pragma unroll
@@ -437,9 +484,66 @@ __global__ void __launch_bounds__(THREADS, Shape<NQ>::BLOCKS) attention_tallied_
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[i] += more[i];
                 }
-                store4(a.pieces + slot * D + col + store_col, sum);
+                if (TOGETHER) store4(rows_here + store_row * D + col + store_col, sum);
+                else store4(a.pieces + slot * D + col + store_col, sum);
             }
             meet();
+        }
+        if constexpr (TOGETHER) {
+            // the old weights are on their way while the blocks meet
+            float* weights = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + start;
+            const int mine = max(0, min(here * BN, length - start));  // slots of this block
+            float old[KEPT_LOADS];
+#pragma unroll
+            for (int k = 0; k < KEPT_LOADS; ++k) {
+                const int at = k * 32 * WARPS + tid;
+                old[k] = at < mine && start + at != length - 1 ? weights[at] : 0.f;  // the token's own slot enters the tally
+            }
+            cluster_arrive(), cluster_wait();
+            float2 ml[MOST_TOGETHER];
+            auto joined = [&](int row) {  // (m, 1 / l) over the blocks
+                float above = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < MOST_TOGETHER; ++r) ml[r] = theirs2(sums_here + row, min(r, a.together - 1)), above = fmaxf(above, ml[r].x);
+#pragma unroll
+                for (int r = 0; r < MOST_TOGETHER; ++r) {
+                    ml[r].x = ml[r].x == -INFINITY ? 0.f : fast_exp2(ml[r].x - above);  // the block's share of it
+                    if (r < a.together) sum = fmaf(ml[r].x, ml[r].y, sum);
+                }
+                return make_float2(above == -INFINITY ? 0.f : above, sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum));  // a row that sees nothing is zeros; a NaN stays one
+            };
+            if (tid < ROWS) factors[tid] = joined(tid);
+            for (int at = rank * 32 * WARPS + tid; at < heads_here * (D / 4); at += a.together * 32 * WARPS) {
+                const int row = at / (D / 4), col = at % (D / 4) * 4;
+                const float2 f = joined(row);
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                float4 part[MOST_TOGETHER];
+#pragma unroll
+                for (int r = 0; r < MOST_TOGETHER; ++r) part[r] = theirs4(rows_here + row * D + col, min(r, a.together - 1));
+#pragma unroll
+                for (int r = 0; r < MOST_TOGETHER; ++r) {
+                    if (r >= a.together) break;
+                    sum[0] = fmaf(ml[r].x, part[r].x, sum[0]), sum[1] = fmaf(ml[r].x, part[r].y, sum[1]), sum[2] = fmaf(ml[r].x, part[r].z, sum[2]), sum[3] = fmaf(ml[r].x, part[r].w, sum[3]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] *= f.y;
+                store4(a.out + (size_t)request * a.out_stride + (size_t)(first_head + row) * D + col, sum);
+            }
+            cluster_arrive();  // nothing of the others is read any more
+            meet();
+#pragma unroll
+            for (int k = 0; k < KEPT_LOADS; ++k) {
+                const int at = k * 32 * WARPS + tid;
+                if (at >= mine) break;
+                float given = 0.f;
+                for (int row = 0; row < heads_here; ++row) {
+                    const float2 f = factors[row];
+                    given = fmaf(fast_exp2(kept[(size_t)row * (a.kept + 4) + at] - f.x), f.y, given);
+                }
+                weights[at] = old[k] + given;
+                if (start + at == length - 1) a.positions[((size_t)request * a.kv_heads + kvh) * a.capacity + length - 1] = a.newest[request];
+            }
+            cluster_wait();
         }
     }
 }
@@ -580,15 +684,48 @@ int cache_map(CUtensorMap* map, const void* cache, const Args& a) {
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
 }
+// launch_after_previous with clusters of `together` blocks along x.
+template <typename... Params, typename... Values>
+int launch_clusters(void (*kernel)(Params...), int together, dim3 grid, dim3 block, size_t shared_bytes, cudaStream_t stream, Values&&... values) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid, config.blockDim = block, config.dynamicSmemBytes = shared_bytes, config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = overlap_launches() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {(unsigned)together, 1, 1};
+    config.attrs = attributes, config.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(values)...);
+}
 template <int NQ>
 int launch_strips(const Args& a, const CUtensorMap& map, cudaStream_t stream) {
-    const auto kernel = attention_tallied_kernel<NQ>;
+    if (a.together) {
+        const auto kernel = attention_tallied_kernel<NQ, true>;
+        constexpr size_t most = Shape<NQ>::SMEM + kept_bytes(Shape<NQ>::ROWS, MOST_KEPT);
+        static_assert(most <= 227 * 1024, "a block's shared memory");
+        static std::atomic<unsigned long long> allowed{0};
+        if (const cudaError_t error = allow_shared((const void*)kernel, most, allowed)) return (int)error;
+        return launch_clusters(kernel, a.together, dim3(a.requests * a.together, a.kv_heads), dim3(THREADS), Shape<NQ>::SMEM + kept_bytes(Shape<NQ>::ROWS, a.kept), stream, map, a);
+    }
+    const auto kernel = attention_tallied_kernel<NQ, false>;
     static std::atomic<unsigned long long> allowed{0};
     if (const cudaError_t error = allow_shared((const void*)kernel, Shape<NQ>::SMEM, allowed)) return (int)error;
     return launch_after_previous(kernel, dim3(a.blocks, a.kv_heads * a.chunks), dim3(THREADS), Shape<NQ>::SMEM, stream, map, a);
 }
 }  // namespace
 
+// The blocks of a cluster that keeps its scores, and how many slots each keeps; or 0, where there are two kernels.  A cluster has one request and key/value head, so its work is as long as the longest request; the line's is
+// equal for all blocks but costs a second kernel.  Clusters are the faster ones up to some 14 tiles of 64 slots a multiprocessor (us, clusters / line, 28 heads over 4 of 128: one request at 512 slots 6.6 / 8.6, at 8,192
+// 25 / 38; four at 4,099 17.5 / 20.3, at 8,192 29 / 26; 16 at 512 8.6 / 10.7, at 2,048 19.1 / 19.0, at 4,099 35 / 27; 64 at 512 19 / 20, at 2,048 54 / 42; 14 heads over 2 of 64, four at 8,192 18 / 25).  As many blocks a
+// cluster as the device holds at once, two a multiprocessor, one of more than eight heads.
+static int together_for(int requests, int longest, int heads, int kv_heads, int sms, int* kept) {
+    const long long pairs = (long long)requests * kv_heads, tiles = (longest + BN - 1) / BN, room = heads / kv_heads <= 8 ? 2LL * sms : sms;
+    if (heads / kv_heads > 16 || tiles > MOST_TOGETHER * MOST_KEPT / BN || pairs * tiles > 14LL * sms) return 0;
+    int blocks = 1;
+    while (blocks < MOST_TOGETHER && ((tiles + blocks - 1) / blocks * BN > MOST_KEPT || (pairs * blocks * 2 <= room && tiles > blocks))) blocks *= 2;
+    *kept = (int)((tiles + blocks - 1) / blocks * BN);
+    return blocks;
+}
 // Blocks of the first kernel that stand side by side for a key/value head's strip: what the device holds, but no more than there can be tiles.
 static int blocks_for(int requests, int longest, int heads, int kv_heads, int sms) {
     const int group = heads / kv_heads, gc = group <= 8 ? group : group < 16 ? group : 16, chunks = (group + gc - 1) / gc;
@@ -598,6 +735,8 @@ static int blocks_for(int requests, int longest, int heads, int kv_heads, int sm
 // Bytes of scratch that hb_attention_tallied takes.
 HB_EXPORT long long hb_attention_tallied_scratch(int requests, int longest, int heads, int kv_heads, int sms) {
     if (requests <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || sms <= 0) return 0;
+    int kept;
+    if (together_for(requests, longest, heads, kv_heads, sms, &kept)) return 0;
     const long long slots = (longest + BN - 1) / BN * BN, pieces = (long long)blocks_for(requests, longest, heads, kv_heads, sms) + requests;
     return 4 * heads * (requests * slots + pieces * (D + 2));
 }
@@ -616,15 +755,17 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL || longest > 0x7fffffff - SPAN || requests > 65535) return HB_UNSUPPORTED_SIZE;
     const int group = heads / kv_heads, gc = group < 16 ? group : 16, chunks = (group + gc - 1) / gc, slots = (longest + BN - 1) / BN * BN;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
-    const int blocks = blocks_for(requests, longest, heads, kv_heads, sms);
+    int kept = 0;
+    const int together = together_for(requests, longest, heads, kv_heads, sms, &kept), blocks = together ? 0 : blocks_for(requests, longest, heads, kv_heads, sms);
     const size_t n_pieces = (size_t)blocks + requests;
     float* pieces = (float*)scratch;
     float* scores = pieces + n_pieces * heads * D;  // before the sums, so that its rows begin on 16 bytes
     float2* sums = (float2*)(scores + (size_t)requests * heads * slots);
     const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, block_table, table_width, lengths, requests, longest, slots, scores, pieces, sums, weights, positions, newest, capacity,
-                 heads, kv_heads, page_size, pages, gc, chunks, blocks, scale * 1.4426950408889634f, status};
+                 heads, kv_heads, page_size, pages, gc, chunks, blocks, together, kept, scale * 1.4426950408889634f, status};
     CUtensorMap map;
     if (int code = cache_map(&map, cache, a)) return code;
     if (int code = gc <= 8 ? launch_strips<1>(a, map, stream) : launch_strips<2>(a, map, stream)) return code;
+    if (together) return 0;
     return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + 1, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
 }

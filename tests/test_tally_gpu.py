@@ -82,8 +82,9 @@ SHAPES = [(14, 2, 64, 16), (28, 4, 128, 16), (16, 16, 64, 8), (24, 1, 128, 64), 
 
 @pytest.mark.parametrize("heads,kv,dim,page", SHAPES)
 @pytest.mark.parametrize("lengths", [[1], [63, 64, 65], [0, 17, 0, 300, 1], [1000, 3, 129], [2500]])
-def test_a_decoded_token(heads, kv, dim, page, lengths):
-    cache, table, random = pages_of(lengths, kv, dim, page, seed=len(lengths))
+@pytest.mark.parametrize("room", [0, 8400])  # a table that may hold more slots than a cluster of blocks keeps the scores of
+def test_a_decoded_token(heads, kv, dim, page, lengths, room):
+    cache, table, random = pages_of(lengths, kv, dim, page, seed=len(lengths), slack=1 + room // page)
     q = queries(random, len(lengths), heads * dim, 24)
     capacity = table.shape[1] * page
     tally = new_tally(len(lengths), kv, capacity)
@@ -109,15 +110,32 @@ def test_a_decoded_token(heads, kv, dim, page, lengths):
         assert torch.equal(tally.positions[r], where.expand(kv, -1))
 
 
-def test_many_requests_of_all_lengths_and_a_bound_on_them():
-    heads, kv, dim, page = 14, 2, 64, 16
+@pytest.mark.parametrize("bound", [None, 8300])
+@pytest.mark.parametrize("heads,kv", [(14, 2), (20, 2)])
+def test_many_requests_of_all_lengths_and_a_bound_on_them(heads, kv, bound):
+    dim, page = 64, 16
     lengths = [(37 * i) % 700 for i in range(90)]
-    cache, table, random = pages_of(lengths, kv, dim, page, seed=4, slack=0)
+    cache, table, random = pages_of(lengths, kv, dim, page, seed=4, slack=0 if bound is None else 500)
     q = queries(random, len(lengths), heads * dim)
-    tally = new_tally(len(lengths), kv, 701)
-    out = attention_tallied(q, heads, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.zeros(len(lengths), dtype=torch.int32, device="cuda"), tally, 0.1, longest=max(lengths))
+    tally = new_tally(len(lengths), kv, bound or 701)
+    out = attention_tallied(q, heads, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.zeros(len(lengths), dtype=torch.int32, device="cuda"), tally, 0.1, longest=bound or max(lengths))
     ops.raise_on_status(q.device)
     for r, want, off, e in attended(q, heads, cache, table, [1] * len(lengths), lengths, 0.1):
+        if e is not None:
+            close(out[r], want, off + want.abs() * 2.0 ** -8)
+        else:
+            close(tally.weights[r, :, : lengths[r]], want, off + want * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("lengths", [[8192, 8001, 5], [4097]])
+@pytest.mark.parametrize("heads,kv,dim", [(28, 4, 128), (32, 2, 64), (16, 1, 128)])
+def test_requests_that_fill_a_cluster(heads, kv, dim, lengths):
+    cache, table, random = pages_of(lengths, kv, dim, 64, seed=11, slack=0)
+    q, tally = queries(random, len(lengths), heads * dim), new_tally(len(lengths), kv, 8192)
+    length = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = attention_tallied(q, heads, cache, table, length, length, tally, dim ** -0.5)
+    ops.raise_on_status(q.device)
+    for r, want, off, e in attended(q, heads, cache, table, [1] * len(lengths), lengths, dim ** -0.5):
         if e is not None:
             close(out[r], want, off + want.abs() * 2.0 ** -8)
         else:

@@ -18,8 +18,8 @@ def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
-def tallied(lengths):
-    cache, table, random = pages_of(lengths, 2, 64, 16, seed=len(lengths))
+def tallied(lengths, slack=1):
+    cache, table, random = pages_of(lengths, 2, 64, 16, seed=len(lengths), slack=slack)
     q, tally = queries(random, len(lengths), 8 * 64), new_tally(len(lengths), 2, table.shape[1] * 16)
 
     def call():
@@ -43,7 +43,7 @@ def many(counts, lengths):
 
 @pytest.mark.parametrize("limit", [0, 1])
 def test_waits_that_run_out(limit, monkeypatch):
-    calls = {"hb_attention_tallied": [tallied([1500, 3, 1, 130, 800]), tallied([5000]), tallied([300] * 30)], "hb_tally_queries": [many([20], [3000]), many([700, 1, 300], [700, 50, 900]), many([1], [1])]}
+    calls = {"hb_attention_tallied": [tallied([1500, 3, 1, 130, 800]), tallied([5000]), tallied([300] * 30), tallied([1500, 3, 1, 130, 800], 600), tallied([9000])], "hb_tally_queries": [many([20], [3000]), many([700, 1, 300], [700, 50, 900]), many([1], [1])]}
     want = {name: [call() for call in some] for name, some in calls.items()}
     ops.raise_on_status(torch.device("cuda", torch.cuda.current_device()))
     with monkeypatch.context() as patch:
