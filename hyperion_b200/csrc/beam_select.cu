@@ -347,16 +347,18 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     };
     auto exactly = [&](const Entry& e) -> Best { return {score_of(e.logit, offset[e.beam]), (long long)e.beam << 32 | e.token}; };
     for (int i = warp; i < n_runs; i += GROUP_THREADS / 32) {
-        Entry e[PER];
+        const int run = chosen[i], beam = run / a.runs, token = (run - beam * a.runs) * RUN + lane;
+        const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)(group * a.beams + beam) * a.stride;
+        float v[PER];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) e[k] = entry(i, k * 32 + lane);
-        const float off = (float)offset[e[0].beam];
-        unsigned reach = 0;
+        for (int k = 0; k < PER; ++k) v[k] = token + k * 32 < a.vocab ? to_float(row[token + k * 32]) : -INFINITY;
+        const float off = (float)offset[beam];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) reach |= (e[k].logit != -INFINITY && e[k].logit + off >= bound ? 1u : 0u) << k;
-        for (; reach; reach &= reach - 1) {
-            const int k = __ffs(reach) - 1, at = atomicAdd(&n_candidates, 1);
-            if (at < MOST_CANDIDATES) candidates[at] = exactly(entry(i, k * 32 + lane));
+        for (int k = 0; k < PER; ++k) {
+            const float logit = cleaned(v[k]);
+            if (logit == -INFINITY || !(logit + off >= bound)) continue;
+            const int at = atomicAdd(&n_candidates, 1);
+            if (at < MOST_CANDIDATES) candidates[at] = exactly(Entry{logit, beam, token + k * 32});
         }
     }
     __syncthreads();

@@ -564,10 +564,12 @@ int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUten
 }
 }  // namespace
 
-// Into how many cuts the first walk's slots go: as many as give the device two blocks an SM, of a tile at least.
+// Into how many cuts the first walk's slots go: as many as give the device two blocks an SM, of two tiles at least, and none up to four tiles, where the kernel that puts cuts together would cost more than it saves.  (us,
+// 28 heads over 4 of 128, tiles a cut at least 1 / 2 / 4: 8 queries of 300 slots, three tiles, 10.9 / 11.3 / 10.6 where 4 leaves one cut; 16 of 1,000 10.8 / 11.5 / 13.5; 32 of 8,192 21.6 / 20.6 / 19.0; 14 over 2 of 64, 32 of
+// 8,192 19.4 / 14.8 / 14.6; four requests' 32 of 2,048 14.2 / 12.4 / 13.6.)
 static int cuts_for(int requests, int most, int longest, int heads, int kv_heads, int sms) {
-    const int per_tile = BM / (heads / kv_heads);
-    const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = (longest + BM - 1) / BM;
+    const int per_tile = BM / (heads / kv_heads), tiles = (longest + BM - 1) / BM;
+    const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = tiles <= 4 ? 1 : (tiles + 1) / 2;
     return (int)(wanted < 1 ? 1 : wanted < most_cuts ? wanted : most_cuts);
 }
 static int span_for(int most, int group, int* spans) {
