@@ -356,15 +356,16 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
     } else if (!in_place) {
         for (int slot = block * THREADS + tid; slot < length; slot += a.blocks * THREADS) to_weights[slot] = weights[slot], to_positions[slot] = positions[slot];
     }
-    const int left = min(length, a.keep);
-    for (int slot = (left & ~3) + 4 * (block * THREADS + tid); slot < a.capacity; slot += 4 * a.blocks * THREADS) {
-        if (aligned && slot >= left && slot + 4 <= a.capacity) {
+    // what has been given up; a tally in a place of its own is written to its end
+    const int left = min(length, a.keep), end = in_place ? length : a.capacity;
+    for (int slot = (left & ~3) + 4 * (block * THREADS + tid); slot < end; slot += 4 * a.blocks * THREADS) {
+        if (aligned && slot >= left && slot + 4 <= end) {
             *reinterpret_cast<float4*>(to_weights + slot) = make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<int4*>(to_positions + slot) = make_int4(-1, -1, -1, -1);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (slot + e >= left && slot + e < a.capacity) to_weights[slot + e] = 0.f, to_positions[slot + e] = -1;
+                if (slot + e >= left && slot + e < end) to_weights[slot + e] = 0.f, to_positions[slot + e] = -1;
         }
     }
     if (a.moves_here) move_records(a, a.from + (size_t)head * a.most, a.to + (size_t)head * a.most, n_moves, a.block_table + (size_t)request * a.table_width, layer, kvh, block * WARPS + warp, a.blocks * WARPS);

@@ -23,9 +23,9 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
     parent's that are filled are copied into it.  ``caches``: dense tensors viewed as [layers, pages, outer, page, inner], all of the same pages and page size (``storage.view(layers, pages, 2 * kv_heads, page, d)``; the codes and
     exponents of an 8-bit cache likewise).
 
-    States: ``states`` are dense [layers, rows, ...], a beam's record copied whole (recurrent states, tallies); a beam's row is its number, or ``state_rows[beam]`` (int32).
+    States: ``states`` are dense [layers, rows, ...], a beam's record copied whole (recurrent states, tallies); a beam's row is its number, or ``state_rows[beam]`` (int32), no two the same.
 
-    At most 24 tensors.  A parent that is no beam, a row or a page that is not there leaves its beam as it is, and is reported (``raise_on_status``)."""
+    At most 24 tensors, each once.  A parent that is no beam, a row or a page that is not there leaves its beam as it is, and is reported (``raise_on_status``)."""
     what = "beam_reorder"
     if parents.dtype is not torch.int32 or parents.dim() != 2 or not parents.is_contiguous() or parents.shape[1] > MOST_BEAMS:
         raise KernelError(f"{what}: parents are dense int32 [groups, beams], at most {MOST_BEAMS} beams")
@@ -60,6 +60,9 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
     if state_rows is not None:
         tensors.append(state_rows)
     _check_device(what, *tensors)
+    places = [place for place in words[::7] if place]
+    if len(set(places)) != len(places):
+        raise KernelError(f"{what}: a tensor once only")
     if rows == 0 or not words:
         return
     check(entry("beam_reorder", "hb_beam_reorder", "ppiipiipippp")(

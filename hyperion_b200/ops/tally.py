@@ -176,8 +176,8 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     request's newest token): int32 [requests].
 
     Slots whose positions are below ``first`` or among the last ``recent`` rank as an infinite weight, the others by their weights (a NaN as -infinity); of equal ranks the lowest slots stay.  What stays in slots
-    from ``keep`` on moves into those below that are left free, in order: keys and values, weights and positions.  Records from the new length on stay as they were, in the tally slots from there on weigh nothing
-    and have position -1.  The new tally goes to ``out`` where it is given, else in place.
+    from ``keep`` on moves into those below that are left free, in order: keys and values, weights and positions.  Records from the new length on stay as they were; in the tally the slots that were given up
+    weigh nothing and have position -1.  The new tally goes to ``out`` where it is given, all of it, with slots behind a request like those given up; else in place, where slots behind a request stay as they were.
 
     Pages are written in place, so a request's pages may not be another one's as well (up to its length).  ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that
     long and is reported (``raise_on_status``).  A move from or to a page that is not there is left out and reported.

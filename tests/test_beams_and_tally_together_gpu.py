@@ -155,5 +155,5 @@ def test_nothing_to_do():
     assert torch.equal(two.weights, before)
     given = cache.clone()
     assert ops.evict(cache, table, ints([0, 0]), ints([0, 0]), two, 4).tolist() == [0, 0]
-    assert torch.equal(given.view(torch.int16), cache.view(torch.int16)) and bool((two.positions == -1).all())
+    assert torch.equal(given.view(torch.int16), cache.view(torch.int16)) and torch.equal(two.weights, before) and two.positions[0, 0].tolist() == list(range(48))
     ops.raise_on_status(cache.device)

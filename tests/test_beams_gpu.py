@@ -212,3 +212,9 @@ def test_what_is_not_there_is_reported_and_stays():
         with pytest.raises(ops.KernelError, match=match):
             ops.raise_on_status(cache.device)
         assert torch.equal(pages[0, 0], cache[0, 0]) or parents[0][0] in (1, 2) and 0 <= table[parents[0][0]][0] < 4
+
+
+def test_a_tensor_comes_once():
+    state = torch.zeros(1, 4, 8, device="cuda")
+    with pytest.raises(ops.KernelError, match="once"):
+        beam_reorder(torch.zeros(1, 4, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), None, [], [state, state])

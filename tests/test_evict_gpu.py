@@ -15,9 +15,12 @@ def bits(x):
     return x.contiguous().view(torch.uint8).cpu().numpy().copy()
 
 
-def expected(cache, table, lengths, newest, weights, positions, keep, first, recent):
-    """cache [layers, pages, 2, kv, page, bytes]; the rest as it goes into evict; all numpy."""
+def expected(cache, table, lengths, newest, weights, positions, keep, first, recent, separate):
+    """cache [layers, pages, 2, kv, page, bytes]; the rest as it goes into evict; all numpy.  In place, slots behind a request stay as they were."""
     cache, out_w, out_p = cache.copy(), np.zeros_like(weights), np.full_like(positions, -1)
+    if not separate:
+        for r, n in enumerate(lengths):
+            out_w[:, r, :, n:], out_p[:, r, :, n:] = weights[:, r, :, n:], positions[:, r, :, n:]
     page = cache.shape[4]
     for layer in range(weights.shape[0]):
         for r, n in enumerate(lengths):
@@ -59,7 +62,7 @@ def run(lengths, *, layers=1, kv=2, dim=64, page=16, keep=10, first=0, recent=0,
     out = Tally(torch.full_like(tally.weights, 3.0), torch.full_like(tally.positions, 3)) if separate else None
     left = evict(cache, torch.from_numpy(table).cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.from_numpy(newest).cuda(), tally, keep, first=first, recent=recent, out=out, longest=longest)
     ops.raise_on_status(cache.device)
-    want_left, want_cache, want_w, want_p = expected(given, table, np.array(lengths), newest, weights, positions, keep, first, recent)
+    want_left, want_cache, want_w, want_p = expected(given, table, np.array(lengths), newest, weights, positions, keep, first, recent, separate)
     to = out if separate else tally
     assert left.tolist() == want_left.tolist()
     assert np.array_equal(to.positions.cpu().numpy().reshape(want_p.shape), want_p)
