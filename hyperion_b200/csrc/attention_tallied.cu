@@ -127,6 +127,7 @@ struct Args {
     int heads, kv_heads, page_size, pages;
     int gc, chunks;          // heads of a strip, strips of a key/value head's group
     int blocks;              // of the first kernel, side by side
+    int join_blocks;         // of the second, a request and key/value head, that put results together: one, or one a head
     int together, kept;      // or 0, or the blocks of a cluster, which has one request and key/value head; slots whose scores each of them keeps
     float scale_log2;
     int* status;
@@ -548,14 +549,15 @@ __global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape
     }
 }
 
-// The second kernel: block x of a (key/value head, request) adds the weights of SPAN slots, four of them a thread, the last x puts the request's result together.  What the first kernel has not written is
+// The second kernel: block x of a (key/value head, request) adds the weights of SPAN slots, four of them a thread; behind those one block puts the request's results together, a warp a head, or, where pieces are many, a block a head.  What the first kernel has not written is
 // read while that one still runs; behind it the scores are on their way while each block brings the pieces' sums together.
 constexpr int ADD_THREADS = 256, SPAN = 4 * ADD_THREADS, HEADS = 8;  // heads at a time
 __global__ void __launch_bounds__(ADD_THREADS, 3) tally_kernel(const Args a) {
     __shared__ float2 heads_sum[HEADS];  // (m, 1 / l) of the heads
     __shared__ int range[2];             // the request's first block of the first kernel, and its pieces
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, request = blockIdx.z, group = a.heads / a.kv_heads;
-    const bool puts_together = blockIdx.x == gridDim.x - 1;
+    const int head = (int)blockIdx.x - (int)(gridDim.x - a.join_blocks);  // that this block puts together (or all of them), or below 0
+    const bool puts_together = head >= 0;
     const int length = length_of(a, request), slot0 = blockIdx.x * SPAN + 4 * tid;
     let_next_kernel_start();
     if (!puts_together && (int)blockIdx.x * SPAN >= length) return;
@@ -583,13 +585,94 @@ __global__ void __launch_bounds__(ADD_THREADS, 3) tally_kernel(const Args a) {
         for (int e = 0; e < 4; ++e)
             if (slot0 + e == length - 1) added[e] = 0.f;  // the token's own slot enters the tally
     }
-    if (tid == 0 && puts_together && kvh == 0 && (a.lengths[request] > a.longest || a.lengths[request] < 0)) atomicOr(a.status, HB_STATUS_BAD_POSITION);
+    if (tid == 0 && head == 0 && kvh == 0 && (a.lengths[request] > a.longest || a.lengths[request] < 0)) atomicOr(a.status, HB_STATUS_BAD_POSITION);
     __syncthreads();
     const int count = length ? range[1] : 0;
     const size_t piece0 = ((size_t)(length ? range[0] : 0) + request) * a.heads + (size_t)kvh * group;  // of the group's first head
     const float* scores = a.scores + ((size_t)request * a.heads + (size_t)kvh * group) * a.slots + slot0;
     const bool mine = !puts_together && slot0 < length;  // a row of scores has whole tiles
     wait_for_previous_kernels();
+    auto joined = [&](const float2* sums) {  // (m, 1 / l) of a head, by one warp
+        float top = -INFINITY, all = 0.f;
+        for (int p = lane; p < count; p += 32) {
+            const float2 ml = sums[(size_t)p * a.heads];
+            const float above = fmaxf(top, ml.x);
+            all = above == -INFINITY ? all + ml.y : fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - above), ml.y, all * (top == -INFINITY ? 0.f : fast_exp2(top - above)));
+            top = above;
+        }
+        const float above = warp_max(top);
+        all = warp_sum(top == -INFINITY ? all : all * fast_exp2(top - above));
+        return make_float2(above == -INFINITY ? 0.f : above, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
+    };
+    if (puts_together && a.join_blocks == 1) {
+        constexpr int TOGETHER = 4;  // pieces that are on their way together
+        for (int h = warp; h < group; h += ADD_THREADS / 32) {
+            const size_t slot0 = piece0 + h;
+            const float2 ml = joined(a.sums + slot0);
+            if (lane >= D / 4) continue;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int p0 = 0; p0 < count; p0 += TOGETHER) {
+                float m[TOGETHER], part[TOGETHER][4];
+#pragma unroll
+                for (int k = 0; k < TOGETHER; ++k) {
+                    const size_t slot = slot0 + (size_t)min(p0 + k, count - 1) * a.heads;
+                    m[k] = a.sums[slot].x;
+                    load4(a.pieces + slot * D + 4 * lane, part[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < TOGETHER; ++k) {
+                    if (p0 + k >= count) break;
+                    const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - ml.x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, part[k][e], sum[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] *= ml.y;
+            store4(a.out + (size_t)request * a.out_stride + ((size_t)kvh * group + h) * D + 4 * lane, sum);
+        }
+        return;
+    }
+    if (puts_together) {
+        // a team of threads has the head's entries, four each, and every TEAMS-th piece; the teams' sums are added up in their order
+        constexpr int TEAM = D / 4, TEAMS = ADD_THREADS / TEAM, TOGETHER = 4;  // pieces of a team that are on their way together
+        __shared__ __align__(16) float parts[TEAMS][D];
+        const int team = tid / TEAM, col = tid % TEAM * 4;
+        const size_t slot0 = piece0 + head;
+        const float2 ml = joined(a.sums + slot0);  // every warp for itself
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = team; p0 < count; p0 += TEAMS * TOGETHER) {
+            float m[TOGETHER], part[TOGETHER][4];
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k) {
+                const size_t slot = slot0 + (size_t)min(p0 + k * TEAMS, count - 1) * a.heads;
+                m[k] = a.sums[slot].x;
+                load4(a.pieces + slot * D + col, part[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k) {
+                if (p0 + k * TEAMS >= count) break;
+                const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - ml.x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, part[k][e], sum[e]);
+            }
+        }
+        store4(&parts[team][col], sum);
+        __syncthreads();
+        if (team == 0) {
+#pragma unroll
+            for (int t = 1; t < TEAMS; ++t) {
+                float more[4];
+                load4(&parts[t][col], more);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += more[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] *= ml.y;
+            store4(a.out + (size_t)request * a.out_stride + ((size_t)kvh * group + head) * D + col, sum);
+        }
+        return;
+    }
     for (int g0 = 0; g0 < group; g0 += HEADS) {
         const int here = min(HEADS, group - g0);
         float y[HEADS][4];
@@ -599,16 +682,8 @@ __global__ void __launch_bounds__(ADD_THREADS, 3) tally_kernel(const Args a) {
                 if (h < here) load4(scores + (size_t)(g0 + h) * a.slots, y[h]);
         }
         if (warp < here) {
-            float top = -INFINITY, all = 0.f;
-            for (int p = lane; p < count; p += 32) {
-                const float2 ml = a.sums[piece0 + (size_t)p * a.heads + g0 + warp];
-                const float above = fmaxf(top, ml.x);
-                all = above == -INFINITY ? all + ml.y : fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - above), ml.y, all * (top == -INFINITY ? 0.f : fast_exp2(top - above)));
-                top = above;
-            }
-            const float above = warp_max(top);
-            all = warp_sum(top == -INFINITY ? all : all * fast_exp2(top - above));
-            if (lane == 0) heads_sum[warp] = make_float2(above == -INFINITY ? 0.f : above, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
+            const float2 ml = joined(a.sums + piece0 + g0 + warp);
+            if (lane == 0) heads_sum[warp] = ml;
         }
         __syncthreads();
         if (mine) {
@@ -618,33 +693,6 @@ __global__ void __launch_bounds__(ADD_THREADS, 3) tally_kernel(const Args a) {
                 const float2 ml = heads_sum[h];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) given[e] = fmaf(fast_exp2(y[h][e] - ml.x), ml.y, given[e]);
-            }
-        }
-        if (puts_together) {
-            for (int at = tid; at < here * (D / 4); at += ADD_THREADS) {
-                const int h = at / (D / 4), col = at % (D / 4) * 4;
-                const float2 ml = heads_sum[h];
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                constexpr int TOGETHER = 4;  // pieces that are on their way together
-                for (int p0 = 0; p0 < count; p0 += TOGETHER) {
-                    float m[TOGETHER], part[TOGETHER][4];
-#pragma unroll
-                    for (int k = 0; k < TOGETHER; ++k) {
-                        const size_t slot = piece0 + (size_t)min(p0 + k, count - 1) * a.heads + g0 + h;
-                        m[k] = a.sums[slot].x;
-                        load4(a.pieces + slot * D + col, part[k]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < TOGETHER; ++k) {
-                        if (p0 + k >= count) break;
-                        const float f = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - ml.x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, part[k][e], sum[e]);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] *= ml.y;
-                store4(a.out + (size_t)request * a.out_stride + ((size_t)kvh * group + g0 + h) * D + col, sum);
             }
         }
         __syncthreads();
@@ -752,20 +800,22 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
-    if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL || longest > 0x7fffffff - SPAN || requests > 65535) return HB_UNSUPPORTED_SIZE;
+    if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL || longest > 0x7fffffff - SPAN - heads || requests > 65535) return HB_UNSUPPORTED_SIZE;
     const int group = heads / kv_heads, gc = group < 16 ? group : 16, chunks = (group + gc - 1) / gc, slots = (longest + BN - 1) / BN * BN;
     if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
     int kept = 0;
     const int together = together_for(requests, longest, heads, kv_heads, sms, &kept), blocks = together ? 0 : blocks_for(requests, longest, heads, kv_heads, sms);
+    // (us, one block / one a head: 16 requests at 4,099, 7 pieces each, 26.5 / 27.6; 64 at 8,192 151 / 158; three at 23,080 of 14 heads over 2 of 64, 74 pieces each, 34 / 14)
+    const int join_blocks = (blocks / requests) * ((group + 7) / 8) > 16 ? group : 1;
     const size_t n_pieces = (size_t)blocks + requests;
     float* pieces = (float*)scratch;
     float* scores = pieces + n_pieces * heads * D;  // before the sums, so that its rows begin on 16 bytes
     float2* sums = (float2*)(scores + (size_t)requests * heads * slots);
     const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, block_table, table_width, lengths, requests, longest, slots, scores, pieces, sums, weights, positions, newest, capacity,
-                 heads, kv_heads, page_size, pages, gc, chunks, blocks, together, kept, scale * 1.4426950408889634f, status};
+                 heads, kv_heads, page_size, pages, gc, chunks, blocks, join_blocks, together, kept, scale * 1.4426950408889634f, status};
     CUtensorMap map;
     if (int code = cache_map(&map, cache, a)) return code;
     if (int code = gc <= 8 ? launch_strips<1>(a, map, stream) : launch_strips<2>(a, map, stream)) return code;
     if (together) return 0;
-    return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + 1, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
+    return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + join_blocks, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
 }

@@ -115,7 +115,7 @@ HB_EXPORT int hb_beam_reorder(const int* parents, const int* lengths, int groups
     a.parents = parents, a.lengths = lengths, a.block_table = block_table, a.table_width = table_width, a.slots = slots, a.beams = beams, a.page_size = block_table ? page_size : 0, a.status = status;
     a.table_blocks = block_table ? (table_width + THREADS - 1) / THREADS : 0;
     long long blocks = 0;
-    for (int i = 0; i < n_tensors; ++i) {
+    for (int i = 0; i < n_tensors && beams > 1; ++i) {  // a beam alone has no other parent: there is nothing to move
         const BeamTensor& t = tensors[i];
         if (t.layers <= 0 || t.outers <= 0 || t.bytes <= 0) continue;
         if (!t.base || t.places <= 0 || t.slots <= 0 || (!t.states && (!block_table || t.slots != page_size))) return HB_BAD_ARGUMENT;
@@ -138,7 +138,7 @@ HB_EXPORT int hb_beam_reorder(const int* parents, const int* lengths, int groups
         }
         ++a.n_jobs;
     }
-    if (blocks + a.table_blocks == 0) return 0;
+    if (blocks + a.table_blocks == 0) a.table_blocks = 1;  // parents are looked at in any case
     const auto kernel = beams <= 4 ? beam_reorder_kernel<4> : beams <= 8 ? beam_reorder_kernel<8> : beams <= 16 ? beam_reorder_kernel<16> : beam_reorder_kernel<32>;
     return launch_after_previous(kernel, dim3((unsigned)(blocks + a.table_blocks), groups), dim3(THREADS), 0, stream, a);
 }

@@ -11,16 +11,10 @@
 #include "common.cuh"
 
 namespace {
-constexpr int THREADS = 1024, WARPS = THREADS / 32, MOST_BLOCKS = 8;
+constexpr int MOST_BLOCKS = 8;
 constexpr int DIGIT = 11, BINS = 2 * (1 << DIGIT) + (1 << (32 - 2 * DIGIT));  // 11, 11 and 10 bits of a rank
 constexpr int LOOK = 128;  // slots of a warp's look, four a lane
 constexpr int MOST_HELD = 40 * 1024;  // ranks that a block holds
-#ifndef HB_PART
-#define HB_PART 1024
-#endif
-#ifndef HB_MOVED
-#define HB_MOVED (1 << 20)
-#endif
 
 struct Args {
     const int* lengths; const int* newest; int requests;
@@ -97,10 +91,7 @@ __device__ __forceinline__ int warp_before(int v, int lane) {  // sum over the l
 
 // The records of a head's moves: warp `first` of `step` takes every step-th CHUNK of them.  A lane finds out where one of them goes from and to; then a team of lanes a move carries 16 bytes of its key and value a lane and
 // turn, AHEAD moves of a team on their way together.
-#ifndef HB_AHEAD
-#define HB_AHEAD 4
-#endif
-constexpr int CHUNK = 16, AHEAD = HB_AHEAD;
+constexpr int CHUNK = 16, AHEAD = 4;
 __device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, int first, int step) {
     const int lane = threadIdx.x & 31, mask = (1 << a.page_shift) - 1;
     int team = 1;  // lanes: a power of two
@@ -143,8 +134,9 @@ __device__ __forceinline__ void move_records(const Args& a, const int* from, con
 }
 
 // HOLDS: the block's ranks are in shared memory; else they are made anew from the weights by every walk.
-template <bool HOLDS>
-__global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
+template <int THREADS, bool HOLDS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_choose_kernel(const Args a) {
+    constexpr int WARPS = THREADS / 32, MINE = (1 << DIGIT) / THREADS < 4 ? 4 : (1 << DIGIT) / THREADS;  // bins of a thread
     extern __shared__ __align__(16) unsigned ranks[];
     __shared__ __align__(16) int counted[BINS];  // of each digit, in the block
     __shared__ __align__(16) int summed[BINS];   // and in the cluster
@@ -232,32 +224,40 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
 #pragma unroll 1
         for (int shift = 32 - DIGIT, bits = DIGIT;;) {
             __syncthreads();
-            // a thread has four bins, from the highest down
-            const int bins = 1 << bits, bin0 = bins - 4 - 4 * tid;
+            // a thread has MINE bins, from the highest down
+            const int bins = 1 << bits, bin0 = bins - MINE - MINE * tid;
             const int* here = counted + digit0;
             if (a.blocks > 1) {
                 if (bin0 >= 0) {
-                    const int4 x = *reinterpret_cast<const int4*>(here + bin0);
-                    if (x.x) add_to_all(summed + digit0 + bin0, x.x, a.blocks);
-                    if (x.y) add_to_all(summed + digit0 + bin0 + 1, x.y, a.blocks);
-                    if (x.z) add_to_all(summed + digit0 + bin0 + 2, x.z, a.blocks);
-                    if (x.w) add_to_all(summed + digit0 + bin0 + 3, x.w, a.blocks);
+#pragma unroll
+                    for (int k = 0; k < MINE; ++k) {
+                        const int n = here[bin0 + k];
+                        if (n) add_to_all(summed + digit0 + bin0 + k, n, a.blocks);
+                    }
                 }
                 cluster_meet(a.blocks);
                 here = summed + digit0;
             }
-            const int4 mine = bin0 >= 0 ? *reinterpret_cast<const int4*>(here + bin0) : make_int4(0, 0, 0, 0);
-            const int sum = mine.x + mine.y + mine.z + mine.w, warp_sum = __reduce_add_sync(0xffffffffu, sum);
+            int mine[MINE], sum = 0;
+#pragma unroll
+            for (int k = 0; k < MINE; k += 4) {
+                const int4 x = bin0 >= 0 ? *reinterpret_cast<const int4*>(here + bin0 + k) : make_int4(0, 0, 0, 0);
+                mine[k] = x.x, mine[k + 1] = x.y, mine[k + 2] = x.z, mine[k + 3] = x.w;
+                sum += x.x + x.y + x.z + x.w;
+            }
+            const int warp_sum = __reduce_add_sync(0xffffffffu, sum);
             if (lane == 0) warp_sums[warp] = warp_sum;
             __syncthreads();
-            const int those = warp_sums[lane], before_those = warp_before(those, lane);
+            const int those = lane < WARPS ? warp_sums[lane] : 0, before_those = warp_before(those, lane);
             const int target = __ffs(__ballot_sync(0xffffffffu, before_those + those >= wanted)) - 1;  // the warp in whose bins it is
             if (warp == target) {
                 int before = __shfl_sync(0xffffffffu, before_those, target) + warp_before(sum, lane);
                 if (before < wanted && before + sum >= wanted) {
-                    const int w = before + mine.w, z = w + mine.z, y = z + mine.y;
-                    found[0] = bin0 + (wanted <= w ? 3 : wanted <= z ? 2 : wanted <= y ? 1 : 0);
-                    found[1] = wanted - (wanted <= w ? before : wanted <= z ? w : wanted <= y ? z : y);
+#pragma unroll
+                    for (int k = MINE - 1; k >= 0; --k) {
+                        if (before < wanted && before + mine[k] >= wanted) found[0] = bin0 + k, found[1] = wanted - before;
+                        before += mine[k];
+                    }
                 }
             }
             __syncthreads();
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(THREADS) evict_choose_kernel(const Args a) {
         if (lane == 0) counts[warp] = make_int4(above_low, above_high, equal_low, equal_high);
         __syncthreads();
         // What is before this warp, in the block and in the blocks before, and what there is in all.
-        const int4 c = counts[lane];
+        const int4 c = lane < WARPS ? counts[lane] : make_int4(0, 0, 0, 0);
         int4 mine{warp_before(c.x, lane), warp_before(c.y, lane), warp_before(c.z, lane), warp_before(c.w, lane)};
         if (warp == 0 && lane == 31) totals[0] = mine.x + c.x, totals[1] = mine.y + c.y, totals[2] = mine.z + c.z, totals[3] = mine.w + c.w;
         mine = make_int4(__shfl_sync(0xffffffffu, mine.x, warp), __shfl_sync(0xffffffffu, mine.y, warp), __shfl_sync(0xffffffffu, mine.z, warp), __shfl_sync(0xffffffffu, mine.w, warp));
@@ -382,9 +382,9 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const Args a) 
                  blockIdx.x * (MOVE_THREADS / 32) + (threadIdx.x >> 5), gridDim.x * (MOVE_THREADS / 32));
 }
 
-template <bool HOLDS>
+template <int THREADS, bool HOLDS>
 int launch_choose(const Args& a, size_t shared_bytes, cudaStream_t stream) {
-    const auto kernel = evict_choose_kernel<HOLDS>;
+    const auto kernel = evict_choose_kernel<THREADS, HOLDS>;
     static std::atomic<unsigned long long> allowed{0};
     if (const cudaError_t error = allow_shared((const void*)kernel, MOST_HELD * 4, allowed)) return (int)error;
     cudaLaunchConfig_t config = {};
@@ -416,17 +416,23 @@ HB_EXPORT int hb_evict(void* cache, int layers, int pages, int kv_heads, int pag
     if (((uintptr_t)cache | (uintptr_t)scratch) & 15 || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     const long long heads = (long long)layers * requests * kv_heads;
     if (requests > 65535 || layers > 65535 || (long long)requests * kv_heads > 65535 || heads > 0x7fffffffLL || record_bytes > 65536) return HB_UNSUPPORTED_SIZE;
-    if (longest > 0x7fffffff - MOST_BLOCKS * WARPS * LOOK || capacity > 0x7fffffff - 4 * MOST_BLOCKS * THREADS || (long long)kv_heads * MOST_BLOCKS > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
+    if (longest > 0x7fffffff - MOST_BLOCKS * 32 * LOOK || capacity > 0x7fffffff - 4 * MOST_BLOCKS * 1024 || (long long)kv_heads * MOST_BLOCKS > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const int most = longest - keep < keep ? (longest > keep ? longest - keep : 0) : keep;
+    // Clusters where heads are few and long: up to four blocks while there is an SM for each and more than 3,584 slots, eight only for a few heads, because clusters of eight SMs leave others empty.  (us, one / two / four /
+    // eight blocks: 48 heads of 4,097 slots 10.0 / 13.2; 48 of 7,470 19.7 / 18.2; 64 of 15,625 24.1 / 21.1; 16 of 18,734 19.3 / - / 16.4 / 27.5; 32 of 32,771, 28,675 of them given up, 42.8 / - / 33.3; 8 of 131,000
+    // 99 / - / 56 / 36.)  Blocks of 256 threads where heads are short, or more than there are SMs, which hold three to five of those: 224 heads of 1,025 10.2 against 15.9, 896 of 2,049 18.4 against 32.9, 256 of 4,097 15.8
+    // against 19.8, but 48 of 4,097 11.5 against 10.0.
     int blocks = 1;
-    while (blocks < MOST_BLOCKS && heads * blocks * 2 <= sms && longest >= blocks * 2 * HB_PART) blocks *= 2;
-    const size_t held = (size_t)((longest + blocks * WARPS * LOOK - 1) / (blocks * WARPS * LOOK)) * WARPS * LOOK;
+    while (blocks < MOST_BLOCKS && heads * blocks * (blocks < 4 ? 2 : 4) <= sms && longest >= blocks * 2 * 3584) blocks *= 2;
+    const int threads = longest <= 2048 || (heads > sms && longest <= 8192) ? 256 : 1024, looks = threads / 32 * LOOK;
+    const size_t held = (size_t)((longest + blocks * looks - 1) / (blocks * looks)) * looks;
     int* moves = (int*)scratch;
     int* lists = (int*)((char*)scratch + (heads * 4 + 15) / 16 * 16);
-    const bool moves_here = (long long)most * 2 * record_bytes <= (long long)blocks * HB_MOVED;
+    // A head's records are moved by its own blocks up to a megabyte each: 1 slot of 1,025 8.1 us against 9.7 with a second kernel, 4,096 of 32,771 by four blocks 46.2 against 48.5.
+    const bool moves_here = (long long)most * 2 * record_bytes <= (long long)blocks << 20;
     const Args a{lengths, newest, requests, weights, positions, to_weights, to_positions, capacity, longest, keep, first, recent, layers, kv_heads, left, moves, lists, lists + heads * most, most,
                  (uint4*)cache, record_bytes / 16, block_table, table_width, __builtin_ctz(page_size), pages, blocks, moves_here ? 1 : 0, status};
-    if (int code = held <= MOST_HELD ? launch_choose<true>(a, held * 4, stream) : launch_choose<false>(a, 0, stream)) return code;
+    if (int code = threads == 256 ? launch_choose<256, true>(a, held * 4, stream) : held <= MOST_HELD ? launch_choose<1024, true>(a, held * 4, stream) : launch_choose<1024, false>(a, 0, stream)) return code;
     if (!most || moves_here) return 0;
     return launch_after_previous(evict_move_kernel, dim3((most + PER_BLOCK - 1) / PER_BLOCK, kv_heads * requests, layers), dim3(MOVE_THREADS), 0, stream, a);
 }

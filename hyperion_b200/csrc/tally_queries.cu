@@ -36,7 +36,7 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int BM = 128;                        // rows that stay, and rows that pass
 constexpr int PANEL = BM * 128, PANELS = D / 64, TILE = PANELS * PANEL;  // bytes
 constexpr int STAGES = D == 128 ? 2 : 4;       // of the ring: two blocks share an SM's memory
-constexpr int SPAN = 16, MOST_SPANS = 16;      // tiles of Q that pass one block at least; blocks that they pass at most, each of which leaves a part of the sums
+constexpr int MOST_SPANS = 16;                 // blocks that a request's tiles of Q pass at most, each of which leaves a part of the sums
 constexpr int HALF = 4, PRODUCER = 2 * HALF, ISSUER = PRODUCER + 1, THREADS = 32 * (ISSUER + 1);  // warps that look at scores: four for each of the two buffers
 constexpr int TMEM_COLS = 2 * BM;              // two blocks have all of an SM's
 constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
@@ -572,17 +572,24 @@ static int cuts_for(int requests, int most, int longest, int heads, int kv_heads
     const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = tiles <= 4 ? 1 : (tiles + 1) / 2;
     return (int)(wanted < 1 ? 1 : wanted < most_cuts ? wanted : most_cuts);
 }
-static int span_for(int most, int group, int* spans) {
-    const int tiles = (most + BM / group - 1) / (BM / group), span = (tiles + MOST_SPANS - 1) / MOST_SPANS > SPAN ? (tiles + MOST_SPANS - 1) / MOST_SPANS : SPAN;
-    *spans = (tiles + span - 1) / span;
-    return span;
+// Tiles of Q that pass a block of the second walk, and into how many such spans they go: 16 where there are blocks enough for the device, two an SM; down to three where there are not, but one span up to four tiles.  (us, at
+// least 2 / 3 / 4 / 8 / 16 tiles: 14 heads over 2 of 64, a prompt of 500 tokens 14.1 / 15.0 / 15.5 / 19.1 / 23.1, four of 300 15.9 / 13.9 / 14.7 / 18.3 / 22.4; 28 over 4 of 128, 500 tokens 18.7 / 18.9 / 17.2 / 20.6 /
+// 25.1; 16 over 1 of 128, 200 tokens 12.6 / 13.2 / 13.9 / 17.2 / 24.6.)
+static int span_for(int requests, int most, int longest, int heads, int kv_heads, int sms, int* spans) {
+    const int per_tile = BM / (heads / kv_heads), tiles = (most + per_tile - 1) / per_tile;
+    const long long blocks = (long long)((longest + BM - 1) / BM) * kv_heads * requests, wanted = (2LL * sms + blocks - 1) / blocks;
+    long long span = (tiles + wanted - 1) / wanted;
+    span = tiles <= 4 ? 4 : span < 3 ? 3 : span > 16 ? 16 : span;
+    if ((tiles + MOST_SPANS - 1) / MOST_SPANS > span) span = (tiles + MOST_SPANS - 1) / MOST_SPANS;
+    *spans = (int)((tiles + span - 1) / span);
+    return (int)span;
 }
 // Bytes of scratch that hb_tally_queries takes.
 HB_EXPORT long long hb_tally_queries_scratch(int tokens, int requests, int most, int longest, int heads, int kv_heads, int sms) {
     if (tokens <= 0 || requests <= 0 || most <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > BM || sms <= 0) return 0;
     const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
     int spans;
-    span_for(most, heads / kv_heads, &spans);
+    span_for(requests, most, longest, heads, kv_heads, sms, &spans);
     const long long padded = (longest + BM - 1) / BM * (long long)BM;
     return 16LL * tokens * heads + (cuts > 1 ? 8LL * tokens * heads * cuts : 0) + (spans > 1 ? 4LL * spans * requests * kv_heads * padded : 0);
 }
@@ -601,7 +608,7 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     const long long row_blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads;
     if (row_blocks > 0x7fffffffLL || sms > 16384) return HB_UNSUPPORTED_SIZE;
     int spans;
-    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), span = span_for(most, group, &spans), padded = (longest + BM - 1) / BM * BM;
+    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), span = span_for(requests, most, longest, heads, kv_heads, sms, &spans), padded = (longest + BM - 1) / BM * BM;
     if ((long long)padded / BM * spans > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     CUtensorMap kv_map, q_map, rows_map;
     const cuuint64_t kv_dims[2] = {(cuuint64_t)D, (cuuint64_t)pages * 2 * kv_heads * page_size}, kv_strides[1] = {(cuuint64_t)D * 2};
