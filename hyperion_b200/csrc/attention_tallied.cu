@@ -166,6 +166,7 @@ __device__ __forceinline__ int request_at(const Args& a, long long at, long long
     begins = before;
     return a.requests;
 }
+constexpr int FEW = 4;  // requests of a lane whose tiles stay in registers
 // Block b of n takes the tiles from b total / n on; the block that has tile `at`.  n <= total: every block has one.
 __device__ __forceinline__ long long share_from(long long b, long long n, long long total) { return b * total / n; }
 __device__ __forceinline__ int block_at(long long at, long long n, long long total) { return (int)(((at + 1) * n - 1) / total); }
@@ -220,13 +221,44 @@ __global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape
     wait_for_previous_kernels();
     let_next_kernel_start();  // behind the wait: the second kernel reads what came before this one without waiting for this one
     if (!TOGETHER && warp == WARPS) {
-        const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
         int request = 0, tile = 0, tiles = 0;
-        if ((long long)blockIdx.x < n) {
-            const long long from = share_from(blockIdx.x, n, total), to = share_from(blockIdx.x + 1, n, total);
-            long long begins;
-            request = request_at(a, from, begins, lane);
-            tile = (int)(from - begins), tiles = (int)(to - from);
+        if (a.requests <= 32 * FEW && (long long)a.requests * a.slots / BN < 0x7fffffffLL) {
+            // the requests' tiles stay in registers, and everything fits 32 bits
+            int n[FEW], sum = 0;
+#pragma unroll
+            for (int k = 0; k < FEW; ++k) n[k] = 32 * k + lane < a.requests ? tiles_of(a, 32 * k + lane) : 0;
+#pragma unroll
+            for (int k = 0; k < FEW; ++k) sum += n[k];
+            const unsigned total = __reduce_add_sync(0xffffffffu, (unsigned)sum), blocks = min((unsigned)a.blocks, total), b = blockIdx.x;
+            if (b < blocks) {
+                const unsigned each = total / blocks, rest = total - each * blocks;  // floor(b total / blocks) = b each + floor(b rest / blocks); blocks are a few an SM, below 2^16
+                const int from = (int)(b * each + b * rest / blocks), to = (int)((b + 1) * each + (b + 1) * rest / blocks);
+                int before = 0;
+#pragma unroll
+                for (int k = 0; k < FEW; ++k) {
+                    int end = n[k];  // inclusive sum
+#pragma unroll
+                    for (int offset = 1; offset < 32; offset <<= 1) {
+                        const int other = __shfl_up_sync(0xffffffffu, end, offset);
+                        if (lane >= offset) end += other;
+                    }
+                    const unsigned beyond = __ballot_sync(0xffffffffu, before + end > from && before <= from);
+                    if (beyond) {
+                        const int who = __ffs(beyond) - 1;
+                        request = 32 * k + who, tile = from - before - __shfl_sync(0xffffffffu, end - n[k], who), tiles = to - from;
+                        break;
+                    }
+                    before += __shfl_sync(0xffffffffu, end, 31);
+                }
+            }
+        } else {
+            const long long total = line_length(a, lane), n = min((long long)a.blocks, total);
+            if ((long long)blockIdx.x < n) {
+                const long long from = share_from(blockIdx.x, n, total), to = share_from(blockIdx.x + 1, n, total);
+                long long begins;
+                request = request_at(a, from, begins, lane);
+                tile = (int)(from - begins), tiles = (int)(to - from);
+            }
         }
         if (lane == 0) share[0] = request, share[1] = tile, share[2] = tiles;
     }
@@ -795,7 +827,7 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
                                    int* status, cudaStream_t stream) {
     if (requests <= 0) return 0;
     if (!q || !out || !cache || !block_table || !lengths || !weights || !positions || !newest || !scratch || !status) return HB_BAD_ARGUMENT;
-    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || out_stride % 4 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || capacity < longest || sms <= 0 || sms > 16384 || q_stride % 8 || out_stride % 4 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
