@@ -10,11 +10,15 @@
 // Both walks have one shape: a tile of 128 rows stays in shared memory (of Q; then of K), tiles of the other pass through a ring, and each pair is one product of 128 x 128 on the tensor cores (tcgen05) into
 // one of two buffers of tensor memory.  The rows that stay are the product's lanes and what passes its columns, so one thread owns a row's maximum and sum, or a slot's sum, and nothing is exchanged.
 // In the second walk a row's maximum and sum are part of the product: 16 more columns stand beside both tiles, 1 1 1 0 ... beside a slot and -(m + log2 l) / (scale log2 e) in three parts of bfloat16 beside a row,
-// so that a thread takes 2^(c s) of what the product gives and adds it up.  (Read out of shared memory by all threads of a warp they cost as much of its bandwidth as the products' operands: 104 us where this takes XX.)
+// so that a thread takes 2^(c s) of what the product gives and adds it up.  (Read out of shared memory by all threads of a warp they cost more of its bandwidth than the products' operands: the second walk of three prompts 104 us, and 73 so.)
 // A tile of Q has whole tokens: 128 / group of them with all heads of a key/value head, by one TMA box a panel.
 //
 // Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.  Nothing is added by atomics, so results
 // do not depend on which block came first.
+//
+// Measured: three prompts of up to 2,047 tokens, 32 heads over 8 of 128, 127 us (both walks' products 0.58 PFLOP/s), of which the first walk takes 60, the second 60 and the parts 5.  In the loop a tile of 128 x 128 takes an SM
+// 950 to 1,150 clocks: 576 of them are its products, 730 its exponentials on the special function unit (11 of 16 pairs), some 700 its instructions; blocks of two halves with a buffer each do not quite keep them all
+// busy, and starts and ends of blocks cost another 15 %.  The last 32 of 8,192 tokens, 28 heads over 4: 18.5 us, three kernels' starts and trips to memory.  (With mma.sync and registers in place of tensor memory 890 and 49 us.)
 //
 // Slots beyond a request's length may hold anything: their scores are not looked at.  Every wait is bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the block leaves, once the copies and products that it
 // has on their way are done.
@@ -503,18 +507,23 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     }
 }
 
-__global__ void __launch_bounds__(256) tally_cuts_kernel(const Args a) {
+// Puts the cuts of a row together: `lanes` threads of a warp a row, a power of two, so that all of a row's cuts are on their way at once (32 cuts by one thread a row took 7 us).
+__global__ void __launch_bounds__(256) tally_cuts_kernel(const Args a, int lanes) {
     let_next_kernel_start();
     wait_for_previous_kernels();
-    const int n = a.tokens * a.heads, at = blockIdx.x * 256 + threadIdx.x;
-    if (at >= n) return;
+    const int n = a.tokens * a.heads, at = (blockIdx.x * 256 + threadIdx.x) / lanes, mine = threadIdx.x % lanes;
     float top = -INFINITY, all = 0.f;
-    for (int c = 0; c < a.n_cuts; ++c) top = fmaxf(top, a.cuts[(size_t)c * n + at].x);
-    for (int c = 0; c < a.n_cuts; ++c) {
+    for (int c = mine; at < n && c < a.n_cuts; c += lanes) {
         const float2 ml = a.cuts[(size_t)c * n + at];
-        all = fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top), ml.y, all);
+        const float above = fmaxf(top, ml.x);
+        all = above == -INFINITY ? all + ml.y : fmaf(ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - above), ml.y, all * (top == -INFINITY ? 0.f : fast_exp2(top - above)));
+        top = above;
     }
-    a.rows[at] = beside_row(top, all, a.scale_log2);
+    float above = top;
+    for (int offset = 1; offset < lanes; offset <<= 1) above = fmaxf(above, __shfl_xor_sync(0xffffffffu, above, offset));
+    if (top != -INFINITY) all *= fast_exp2(top - above);
+    for (int offset = 1; offset < lanes; offset <<= 1) all += __shfl_xor_sync(0xffffffffu, all, offset);
+    if (mine == 0 && at < n) a.rows[at] = beside_row(above, all, a.scale_log2);
 }
 
 // The spans' parts of the slots' sums, in their order.
@@ -626,8 +635,13 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, (float*)(cut_sums + (cuts > 1 ? (size_t)tokens * heads * cuts : 0)), span, spans, padded, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
                  scale * 1.4426950408889634f, status};
     if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3((unsigned)row_blocks, cuts, requests), stream)) return code;
-    if (cuts > 1)
-        if (int code = launch_after_previous(tally_cuts_kernel, dim3((tokens * heads + 255) / 256), dim3(256), 0, stream, a)) return code;
+    if (cuts > 1) {
+        int lanes = 2;
+        while (lanes < 32 && lanes < cuts) lanes *= 2;
+        const long long threads = (long long)tokens * heads * lanes;
+        if (threads > 0x7fffffffLL - 256) return HB_UNSUPPORTED_SIZE;
+        if (int code = launch_after_previous(tally_cuts_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, lanes)) return code;
+    }
     if (int code = launch_walk<true>(kv_map, q_map, rows_map, a, dim3(padded / BM * spans, kv_heads, requests), stream)) return code;
     return spans > 1 ? launch_after_previous(tally_parts_kernel, dim3((longest + 255) / 256, kv_heads, requests), dim3(256), 0, stream, a) : 0;
 }
