@@ -7,6 +7,9 @@
 // searches take a bound first, the `take`-th largest of what eighths of the warps have found to be their best, and then look at what reaches it: little more than `take` in all but contrived rows, for which there is a way that goes by one
 // continuation after the other.
 //
+// Measured: 32 groups of 8 beams over bfloat16 logits of 152,064 26.3 us for 78 MB: the first kernel 17 (4.6 TB/s; as long without its exponentials, and with more or fewer blocks or loads on their way), the second 9, a chain of a
+// logarithm, three meetings of the block and two trips to memory.  One group of four beams 8.6 us.
+//
 // Scores are compared as float64: a score is score_b - lse_b, a number of the row, plus the logit, and float32 would make ties of scores that are not equal.  Sums of a thread's 32 entries are float, everything above
 // them float64; exponentials are the hardware's (2^-22 of a term).  Which thread adds up what goes by the entry's index alone, not by the row's alignment, so rows that hold the same have the same sums.
 //

@@ -6,8 +6,13 @@
 //
 // A request of at most `keep` slots stays as it is.
 //
-// The first kernel has a block per head: the rank of the last slot that stays is found digit by digit (8 bits of the weight's ordered bits at a time, by counting), then one walk along the slots lists
-// what moves and what is free and writes the slots' new weights and positions.  The second moves the records.
+// A head is a cluster of one to eight blocks, each of which has a part of the slots and holds their ranks in shared memory.  The rank of the last slot that stays is found digit by digit (11, 11 and 10 bits of the
+// weight's ordered bits), by counting: after the first digit few slots are left to count, and each block adds what it has counted to all blocks' sums.  Two more walks along the ranks say how many slots move and are
+// free before each warp's, and then which; where a slot stands in its list follows from the slots before it alone, so nothing depends on which block came first.  Then the cluster moves what is to move, records
+// included, or leaves those to a second kernel.
+//
+// Measured: 24 layers of 2 heads that give up one slot of 1,025 7.9 us, a chain of some 14,000 clocks: the slots' arrival, three digits of 1,500 clocks each (counts, a sum over the bins, two meetings of the block), lists.  Four layers of 8
+// heads that keep 4,096 of 32,771 slots 42 us: half of it the choice (arrival 8,000 clocks, digits 14,000 with the cluster's meetings, lists and sums 10,000), half the moves of 117 MB of records at 5.4 TB/s.
 #include "common.cuh"
 
 namespace {
