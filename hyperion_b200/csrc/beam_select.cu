@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     __syncthreads();
     const float bound = shared_bound;
     auto choose = [&](int i, float top) {
-        if (top == -INFINITY || !(top + off_here >= bound) || beam_here >= a.beams) return;
+        if (top == -INFINITY || beam_here >= a.beams || offset[beam_here] == -INFINITY || !(top + off_here >= bound)) return;  // a dead beam's run reaches a bound of -infinity, too
         const int at = atomicAdd(&n_chosen, 1);
         if (at < MOST_RUNS) chosen[at] = beam_here * a.runs + i;
     };

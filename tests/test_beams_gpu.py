@@ -114,6 +114,17 @@ def test_a_first_step_of_one_beam():
     assert check_selection(logits, scores, 4).parents.tolist() == [[0] * 4] * 3
 
 
+@pytest.mark.parametrize("vocab,take", [(10, 30), (1, 4), (40, 64), (300, 64)])
+def test_dead_beams_have_no_continuations(vocab, take):
+    """Not even where there are places left."""
+    logits, scores = some_logits(2, 3, vocab, seed=vocab)
+    scores[0, 1:] = -float("inf")
+    scores[1, 0], scores[1, 2] = float("nan"), -float("inf")
+    choice = check_selection(logits, scores, take)
+    there = min(take, vocab)
+    assert choice.parents.tolist() == [[0] * there + [-1] * (take - there), [1] * there + [-1] * (take - there)]
+
+
 def reordered(parents, lengths, table, caches, states, rows=None):
     """Plain: everything is read before anything is written."""
     groups, beams = parents.shape
