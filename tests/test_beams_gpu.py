@@ -125,6 +125,39 @@ def test_dead_beams_have_no_continuations(vocab, take):
     assert choice.parents.tolist() == [[0] * there + [-1] * (take - there), [1] * there + [-1] * (take - there)]
 
 
+@pytest.mark.parametrize("beams,take", [(8, 16), (16, 16), (16, 32), (32, 64)])
+@pytest.mark.parametrize("step", [float("inf"), 40.0, 3.0, 0.01])
+def test_a_few_beams_hold_all_that_is_best(beams, take, step):
+    logits, _ = some_logits(2, beams, 40001, torch.bfloat16, seed=beams)
+    scores = torch.stack([-torch.arange(beams).float().mul(step).nan_to_num(0.0), -torch.arange(beams).flip(0).float().mul(step).nan_to_num(0.0)]).cuda()
+    check_selection(logits, scores, take)
+
+
+def test_scores_beyond_what_float_adds_up():
+    """Sums of a score and a logit that pass the largest number, and scores beside which a logit is lost."""
+    logits, _ = some_logits(1, 4, 3000, seed=5)
+    for score in ([0.0, -3e38, -1e9, -3.4e38], [3e38, 3.4e38, 1e9, 0.0], [-3.4e38, -3.4e38, -float("inf"), -3.4e38]):
+        choice = beam_select(logits, torch.tensor([score], device="cuda"), 8)
+        best = max(range(4), key=lambda b: score[b])
+        want = logits[best].double().sort(descending=True, stable=True).indices[:8]
+        assert choice.parents.tolist() == [[best] * 8]
+        if abs(score[best]) < 1e8:  # above, logits of different size are one score in float64, too
+            assert choice.tokens.tolist() == [want.tolist()]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [1, 255, 256, 257, 511, 513, 8191, 8193, 33000])
+def test_every_alignment_gives_the_same(vocab, dtype):
+    """To the bit, for the rows of a call: eight bfloat16 or four float fit between two boundaries of 16 bytes."""
+    logits, _ = some_logits(1, 1, vocab, dtype, seed=vocab)
+    stride = (vocab + 7) // 8 * 8 + 9
+    memory = torch.full((stride * 8,), float("inf"), dtype=dtype, device="cuda")  # what is beside a row is not looked at
+    rows = memory.view(8, stride)[:, :vocab]
+    rows.copy_(logits.expand(8, vocab))
+    choice = check_selection(rows, torch.full((8, 1), -2.5, device="cuda"), 3)
+    assert all((x == x[:1]).all() for x in choice)
+
+
 def reordered(parents, lengths, table, caches, states, rows=None):
     """Plain: everything is read before anything is written."""
     groups, beams = parents.shape
