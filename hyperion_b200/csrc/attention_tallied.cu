@@ -14,7 +14,8 @@
 // Where there is little, a request and key/value head is a cluster's of one to eight blocks: each walks its share and keeps its scores in shared memory, then they read one another's results there (mapa,
 // ld.shared::cluster) and add the weights of their own slots.
 //
-// In a block one lane of a producer warp per page fetches keys and values by TMA into a ring of stages, and each of four warps takes 16 of a stage's 64 slots for all rows.  The products are
+// In a block one lane of a producer warp per page fetches keys and values by TMA into a ring of stages, and each of four warps takes 16 of a stage's 64 slots for all rows (or for a set's rows: a block has one set of four
+// warps, or three).  The products are
 // S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): slots and entries stand where the instruction has 16 rows, the few heads of a key/value head where it has 8 columns.  The weights are taken into the second
 // product in two parts, rounded to bfloat16 and what that left over: rounded once they would cost the result as much as its own rounding does.
 //
@@ -38,8 +39,7 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int D = HB_HEAD_DIM;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
-constexpr int WARPS = 4;  // that compute; one more fetches
-constexpr int THREADS = 32 * (WARPS + 1);
+constexpr int WARPS = 4;  // that compute for the same rows
 constexpr int BN = 64;    // slots of a tile
 constexpr int TILE = BN * D * 2, PANELS = D / 64;
 constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
@@ -102,15 +102,16 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // 16-byte chunk cc of slot `key` of a tile as TMA's swizzle has placed it.
 __device__ __forceinline__ int tile_at(int key, int cc) { return (cc >> 3) * (BN * 128) + key * 128 + (((cc & 7) ^ (key & 7)) << 4); }
 
-template <int NQ>  // eights of rows
+template <int NQ, int SETS>  // eights of rows that four warps have; sets of four warps, each with rows of its own; one more warp fetches
 struct Shape {
-    static constexpr int ROWS = 8 * NQ;
-    static constexpr int BLOCKS = NQ == 1 ? 3 : 2;  // an SM, by registers
-    static constexpr int STAGES = (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
+    static constexpr int ROWS = 8 * NQ, THREADS = 32 * (WARPS * SETS + 1);
+    static_assert(SETS == 1 || (NQ == 1 && SETS == 3), "what registers hold");
+    static constexpr int BLOCKS = SETS > 1 ? 1 : NQ == 1 ? 3 : 2;  // an SM, by registers
+    static constexpr int STAGES = SETS > 1 ? (D == 128 ? 6 : 12) : (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
     // Where the warps' results meet: COLS entries of every row at a time, a row's LINE floats apart (lanes that store side by side then take different banks).
     static constexpr int COLS = 64 / NQ, LINE = COLS + 4;
-    static constexpr int JOIN = WARPS * ROWS * LINE * 4;
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * TILE + JOIN + 2 * WARPS * ROWS * 4 + 2 * STAGES * 8 + 32;
+    static constexpr int JOIN = WARPS * ROWS * LINE * 4;  // a set
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * TILE + SETS * (JOIN + 2 * WARPS * ROWS * 4) + 2 * STAGES * 8 + 32 + 4 * SETS;
     static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "an SM's shared memory");
 };
 
@@ -128,7 +129,7 @@ struct Args {
     const int* newest;       // [requests]
     int capacity;
     int heads, kv_heads, page_size, pages;
-    int gc, chunks;          // heads of a strip, strips of a key/value head's group
+    int gc, chunks;          // heads of a set, blocks' chunks of a key/value head's group
     int blocks;              // of the first kernel, side by side
     int join_blocks;         // of the second, a request and key/value head, that put results together: one, or one a head
     int together, kept;      // or 0, or the blocks of a cluster, which has one request and key/value head; slots whose scores each of them keeps
@@ -197,33 +198,37 @@ __device__ __forceinline__ float4 theirs4(const float* p, int rank) {
 }
 
 // TOGETHER: the blocks of a cluster share one request's slots of one key/value head (all of whose query heads a strip has), keep their scores in shared memory, and end with the result and the weights.
-template <int NQ, bool TOGETHER>
-__global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape<NQ>::BLOCKS)) attention_tallied_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
-    typedef Shape<NQ> S;
-    constexpr int ROWS = S::ROWS;
+template <int NQ, int SETS, bool TOGETHER>
+__global__ void __launch_bounds__(Shape<NQ, SETS>::THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape<NQ, SETS>::BLOCKS)) attention_tallied_kernel(const __grid_constant__ CUtensorMap kv_map, const Args a) {
+    typedef Shape<NQ, SETS> S;
+    constexpr int ROWS = S::ROWS, PRODUCER = WARPS * SETS;
+    static_assert(SETS == 1 || !TOGETHER, "a cluster's blocks have one set");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* join = reinterpret_cast<float*>(ring + (size_t)S::STAGES * 2 * TILE);  // [WARPS][ROWS][LINE]
-    float* tops = join + S::JOIN / 4;                                               // [WARPS][ROWS]: maxima
-    float* parts = tops + WARPS * ROWS;                                             // [WARPS][ROWS]: sums
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(parts + WARPS * ROWS);
+    const int tid = threadIdx.x, lane = tid & 31, set = threadIdx.x / (32 * WARPS), warp = (threadIdx.x >> 5) - (SETS > 1 ? set * WARPS : 0);  // of its set; the producer's is PRODUCER or, behind other sets, 0
+    const bool producer = (tid >> 5) == PRODUCER;
+    float* of_sets = reinterpret_cast<float*>(ring + (size_t)S::STAGES * 2 * TILE);
+    float* join = of_sets + (producer ? 0 : set) * (S::JOIN / 4 + 2 * WARPS * ROWS);  // [WARPS][ROWS][LINE]
+    float* tops = join + S::JOIN / 4;                                                   // [WARPS][ROWS]: maxima
+    float* parts = tops + WARPS * ROWS;                                                 // [WARPS][ROWS]: sums
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(of_sets + SETS * (S::JOIN / 4 + 2 * WARPS * ROWS));
     unsigned long long* empty = full + S::STAGES;
     volatile int* failed = reinterpret_cast<volatile int*>(empty + S::STAGES);
-    volatile int* lost = failed + 1;  // a computing warp has given up
-    int* share = const_cast<int*>(failed) + 2;  // first request, its first tile here, tiles in all
-    [[maybe_unused]] float2* factors = reinterpret_cast<float2*>((reinterpret_cast<uintptr_t>(share + 4) + 15) & ~(uintptr_t)15);  // TOGETHER: [ROWS]: (m, 1 / l) of the request's rows
+    int* share = const_cast<int*>(failed) + 1;  // first request, its first tile here, tiles in all
+    volatile int* lost = failed + 4 + (producer ? 0 : set);  // a computing warp of the set has given up
+    [[maybe_unused]] float2* factors = reinterpret_cast<float2*>((reinterpret_cast<uintptr_t>(share + 3 + SETS) + 15) & ~(uintptr_t)15);  // TOGETHER: [ROWS]: (m, 1 / l) of the request's rows
     [[maybe_unused]] float* kept = reinterpret_cast<float*>(factors + ROWS);                                                   // [ROWS][a.kept + 4]
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], WARPS); }
-        *failed = 0, *lost = 0;
+        for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], WARPS * SETS); }
+        *failed = 0;
+        for (int k = 0; k < SETS; ++k) lost[k] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == WARPS && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
+    if (producer && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
     wait_for_previous_kernels();
     let_next_kernel_start();  // behind the wait: the second kernel reads what came before this one without waiting for this one
-    if (!TOGETHER && warp == WARPS) {
+    if (!TOGETHER && producer) {
         int request = 0, tile = 0, tiles = 0;
         if (a.requests <= 32 * FEW && (long long)a.requests * a.slots / BN < 0x7fffffffLL) {
             // the requests' tiles stay in registers, and everything fits 32 bits
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape
     }
     __syncthreads();
     const int kvh = blockIdx.y / a.chunks, chunk = blockIdx.y - kvh * a.chunks;
-    const int group = a.heads / a.kv_heads, first_head = kvh * group + chunk * a.gc, heads_here = min(a.gc, group - chunk * a.gc);
+    const int group = a.heads / a.kv_heads, head0 = (SETS > 1 ? chunk * SETS + set : chunk) * a.gc, first_head = kvh * group + head0, heads_here = max(0, min(a.gc, group - head0));  // (those of the producer are no one's)
     int request, tile, left, stage = 0;  // the ring runs on across the block's requests
     [[maybe_unused]] int rank = 0;
     if constexpr (TOGETHER) {
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape
         request = share[0], tile = share[1], left = share[2];
     }
 
-    if (warp == WARPS) {
+    if (producer) {
         // ------------------------------------------------------------------ producer (the whole warp)
         const int shift = 31 - __clz(a.page_size), pages_per_tile = BN >> shift, tiles_per_look = 32 / pages_per_tile;
         constexpr int OPS_PER_PAGE = 2 * PANELS;
@@ -332,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, (TOGETHER ? (NQ == 1 ? 2 : 1) : Shape
     }
     // ---------------------------------------------------------------------- consumers
     const int t = lane & 3, g = lane >> 2;
-    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); };
+    auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(SETS > 1 ? 1 + set : 1), "n"(32 * WARPS) : "memory"); };  // the set's warps
     constexpr int LANES_PER_ROW = S::COLS / 16;
     const int store_row = lane / LANES_PER_ROW, store_col = warp * (S::COLS / 4) + lane % LANES_PER_ROW * 4;  // what this lane stores of every COLS entries
     const bool stores = store_row < heads_here;
@@ -780,20 +785,21 @@ int launch_clusters(void (*kernel)(Params...), int together, dim3 grid, dim3 blo
     config.attrs = attributes, config.numAttrs = 2;
     return (int)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(values)...);
 }
-template <int NQ>
+template <int NQ, int SETS>
 int launch_strips(const Args& a, const CUtensorMap& map, cudaStream_t stream) {
-    if (a.together) {
-        const auto kernel = attention_tallied_kernel<NQ, true>;
-        constexpr size_t most = Shape<NQ>::SMEM + kept_bytes(Shape<NQ>::ROWS, MOST_KEPT);
+    typedef Shape<NQ, SETS> S;
+    if constexpr (SETS == 1) if (a.together) {
+        const auto kernel = attention_tallied_kernel<NQ, 1, true>;
+        constexpr size_t most = S::SMEM + kept_bytes(S::ROWS, MOST_KEPT);
         static_assert(most <= 227 * 1024, "a block's shared memory");
         static std::atomic<unsigned long long> allowed{0};
         if (const cudaError_t error = allow_shared((const void*)kernel, most, allowed)) return (int)error;
-        return launch_clusters(kernel, a.together, dim3(a.requests * a.together, a.kv_heads), dim3(THREADS), Shape<NQ>::SMEM + kept_bytes(Shape<NQ>::ROWS, a.kept), stream, map, a);
+        return launch_clusters(kernel, a.together, dim3(a.requests * a.together, a.kv_heads), dim3(S::THREADS), S::SMEM + kept_bytes(S::ROWS, a.kept), stream, map, a);
     }
-    const auto kernel = attention_tallied_kernel<NQ, false>;
+    const auto kernel = attention_tallied_kernel<NQ, SETS, false>;
     static std::atomic<unsigned long long> allowed{0};
-    if (const cudaError_t error = allow_shared((const void*)kernel, Shape<NQ>::SMEM, allowed)) return (int)error;
-    return launch_after_previous(kernel, dim3(a.blocks, a.kv_heads * a.chunks), dim3(THREADS), Shape<NQ>::SMEM, stream, map, a);
+    if (const cudaError_t error = allow_shared((const void*)kernel, S::SMEM, allowed)) return (int)error;
+    return launch_after_previous(kernel, dim3(a.blocks, a.kv_heads * a.chunks), dim3(S::THREADS), S::SMEM, stream, map, a);
 }
 }  // namespace
 
@@ -809,10 +815,20 @@ static int together_for(int requests, int longest, int heads, int kv_heads, int 
     *kept = (int)((tiles + blocks - 1) / blocks * BN);
     return blocks;
 }
+// How a key/value head's group of heads is cut: into chunks, each a block's, and those into sets.
+struct Strips { int heads, sets, chunks, blocks; };  // of a set; of a chunk; of a group; that an SM holds
+static Strips strips_for(int group) {
+    if (group <= 8) return {group, 1, 1, Shape<1, 1>::BLOCKS};
+    if (group <= 16) return {group, 1, 1, Shape<2, 1>::BLOCKS};
+    // Three sets read keys and values once where two strips of 16 read them twice (us, 24 heads over 1: of 128, 11 requests at 23,692 slots 40.2 / 47.0, 64 of them 184 / 224, one at 512 9.9 / 9.3; of 64, where they are half as
+    // many bytes for as many instructions, 11 30.6 / 30.6 and 64 141 / 136).  Two sets of 16 rows for 32 heads gain nothing: 51.2 / 51.4.  Rows of 24 or 32 in a warp's registers do not fit: 56 and 70.
+    if (group <= 24 && D == 128) return {(group + 2) / 3, 3, 1, Shape<1, 3>::BLOCKS};
+    return {16, 1, (group + 15) / 16, Shape<2, 1>::BLOCKS};
+}
 // Blocks of the first kernel that stand side by side for a key/value head's strip: what the device holds, but no more than there can be tiles.
 static int blocks_for(int requests, int longest, int heads, int kv_heads, int sms) {
-    const int group = heads / kv_heads, gc = group <= 8 ? group : group < 16 ? group : 16, chunks = (group + gc - 1) / gc;
-    const long long room = (long long)sms * (gc <= 8 ? Shape<1>::BLOCKS : Shape<2>::BLOCKS) / ((long long)kv_heads * chunks), tiles = (long long)requests * ((longest + BN - 1) / BN);
+    const Strips strips = strips_for(heads / kv_heads);
+    const long long room = (long long)sms * strips.blocks / ((long long)kv_heads * strips.chunks), tiles = (long long)requests * ((longest + BN - 1) / BN);
     return (int)(room < 1 ? 1 : room < tiles ? room : tiles);
 }
 // Bytes of scratch that hb_attention_tallied takes.
@@ -836,8 +852,9 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     if ((long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     if (q_stride > 0x7fffffffLL || out_stride > 0x7fffffffLL || longest > 0x7fffffff - SPAN - heads || requests > 65535) return HB_UNSUPPORTED_SIZE;
-    const int group = heads / kv_heads, gc = group < 16 ? group : 16, chunks = (group + gc - 1) / gc, slots = (longest + BN - 1) / BN * BN;
-    if ((long long)kv_heads * chunks > 65535) return HB_UNSUPPORTED_SIZE;
+    const int group = heads / kv_heads, slots = (longest + BN - 1) / BN * BN;
+    const Strips strips = strips_for(group);
+    if ((long long)kv_heads * strips.chunks > 65535) return HB_UNSUPPORTED_SIZE;
     int kept = 0;
     const int together = together_for(requests, longest, heads, kv_heads, sms, &kept), blocks = together ? 0 : blocks_for(requests, longest, heads, kv_heads, sms);
     // (us, one block / one a head: 16 requests at 4,099, 7 pieces each, 26.5 / 27.6; 64 at 8,192 151 / 158; three at 23,080 of 14 heads over 2 of 64, 74 pieces each, 34 / 14)
@@ -847,10 +864,10 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     float* scores = pieces + n_pieces * heads * D;  // before the sums, so that its rows begin on 16 bytes
     float2* sums = (float2*)(scores + (size_t)requests * heads * slots);
     const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, block_table, table_width, lengths, requests, longest, slots, scores, pieces, sums, weights, positions, newest, capacity,
-                 heads, kv_heads, page_size, pages, gc, chunks, blocks, join_blocks, together, kept, scale * 1.4426950408889634f, status};
+                 heads, kv_heads, page_size, pages, strips.heads, strips.chunks, blocks, join_blocks, together, kept, scale * 1.4426950408889634f, status};
     CUtensorMap map;
     if (int code = cache_map(&map, cache, a)) return code;
-    if (int code = gc <= 8 ? launch_strips<1>(a, map, stream) : launch_strips<2>(a, map, stream)) return code;
+    if (int code = strips.sets == 3 ? launch_strips<1, 3>(a, map, stream) : strips.heads <= 8 ? launch_strips<1, 1>(a, map, stream) : launch_strips<2, 1>(a, map, stream)) return code;
     if (together) return 0;
     return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + join_blocks, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
 }

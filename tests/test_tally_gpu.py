@@ -127,6 +127,20 @@ def test_many_requests_of_all_lengths_and_a_bound_on_them(heads, kv, bound):
             close(tally.weights[r, :, : lengths[r]], want, off + want * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(17, 1, 128), (18, 1, 128), (40, 2, 128), (23, 1, 128), (25, 1, 128), (48, 2, 128), (18, 1, 64), (48, 2, 64)])
+def test_groups_of_more_heads_than_a_strip(heads, kv, dim):
+    lengths = [1500, 0, 129, 64, 1, 700, 2900]
+    cache, table, random = pages_of(lengths, kv, dim, 16, seed=heads)
+    q, tally = queries(random, len(lengths), heads * dim), new_tally(len(lengths), kv, table.shape[1] * 16)
+    out = attention_tallied(q, heads, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.zeros(len(lengths), dtype=torch.int32, device="cuda"), tally, dim ** -0.5)
+    ops.raise_on_status(q.device)
+    for r, want, off, e in attended(q, heads, cache, table, [1] * len(lengths), lengths, dim ** -0.5):
+        if e is not None:
+            close(out[r], want, off + want.abs() * 2.0 ** -8)
+        else:
+            close(tally.weights[r, :, : lengths[r]], want, off + want * 2.0 ** -23)
+
+
 @pytest.mark.parametrize("lengths", [[8192, 8001, 5], [4097]])
 @pytest.mark.parametrize("heads,kv,dim", [(28, 4, 128), (32, 2, 64), (16, 1, 128)])
 def test_requests_that_fill_a_cluster(heads, kv, dim, lengths):

@@ -18,13 +18,13 @@ def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
-def tallied(lengths, slack=1):
-    cache, table, random = pages_of(lengths, 2, 64, 16, seed=len(lengths), slack=slack)
-    q, tally = queries(random, len(lengths), 8 * 64), new_tally(len(lengths), 2, table.shape[1] * 16)
+def tallied(lengths, slack=1, heads=8, kv=2, dim=64):
+    cache, table, random = pages_of(lengths, kv, dim, 16, seed=len(lengths), slack=slack)
+    q, tally = queries(random, len(lengths), heads * dim), new_tally(len(lengths), kv, table.shape[1] * 16)
 
     def call():
         tally.weights.zero_()
-        out = attention_tallied(q, 8, cache, table, ints(lengths), ints(lengths), tally, 0.125)
+        out = attention_tallied(q, heads, cache, table, ints(lengths), ints(lengths), tally, 0.125)
         return out, tally.weights.clone()
     return call
 
@@ -68,3 +68,28 @@ def test_waits_that_run_out(limit, monkeypatch):
         for call, right in zip(some, want[name]):
             assert all(torch.equal(a, b) for a, b in zip(call(), right))
     ops.raise_on_status(torch.device("cuda", torch.cuda.current_device()))
+
+
+@pytest.mark.parametrize("limit", [0, 1])
+def test_waits_of_three_sets_that_run_out(limit, monkeypatch):
+    calls = [tallied([1500, 3, 1, 130, 800], heads=24, kv=1, dim=128), tallied([30000], heads=20, kv=1, dim=128)]
+    want, name = [call() for call in calls], "hb_attention_tallied"
+    ops.raise_on_status(torch.device("cuda", torch.cuda.current_device()))
+    found = native._entries[name, 128]
+    with monkeypatch.context() as patch:
+        short = getattr(native.library(name[3:], HB_HEAD_DIM=128, HB_WAIT_LIMIT=limit), name)
+        short.argtypes = found.argtypes
+        patch.setitem(native._entries, (name, 128), short)
+        for call in calls:
+            got = call()
+            if limit == 0:
+                with pytest.raises(ops.KernelError, match="bounded wait"):
+                    ops.raise_on_status(got[0].device)
+            else:
+                try:
+                    ops.raise_on_status(got[0].device)
+                except ops.KernelError:
+                    pass
+    for call, right in zip(calls, want):
+        assert all(torch.equal(a, b) for a, b in zip(call(), right))
+        ops.raise_on_status(right[0].device)
