@@ -163,16 +163,19 @@ static inline int launch_after_previous(void (*kernel)(Params...), dim3 grid, di
     return launch_in_turn(true, kernel, grid, block, shared_bytes, stream, args...);
 }
 
-// Lets a kernel have more than 48 KB of shared memory a block, once per device; `done` is the kernel's own, and zero at first.
-static inline cudaError_t allow_shared(const void* kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+// Gives a kernel an attribute once per device; `done` is the kernel's and the attribute's own, and zero at first.
+static inline cudaError_t allow_once(const void* kernel, cudaFuncAttribute attribute, int value, std::atomic<unsigned long long>& done) {
     int device = 0;
     if (cudaError_t error = cudaGetDevice(&device)) return error;
     const unsigned long long bit = device < 64 ? 1ull << device : 0;
     if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    const cudaError_t error = cudaFuncSetAttribute(kernel, attribute, value);
     if (error == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return error;
 }
+// More than 48 KB of shared memory a block; clusters of more than eight blocks.
+static inline cudaError_t allow_shared(const void* kernel, size_t bytes, std::atomic<unsigned long long>& done) { return allow_once(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes, done); }
+static inline cudaError_t allow_wide_clusters(const void* kernel, std::atomic<unsigned long long>& done) { return allow_once(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, done); }
 
 // The first position that a query at position `pos` sees.  window > 0: the last `window` positions (pos - window + 1 at the least);
 // window < 0: the query's own chunk of -window positions, chunks counted from position 0; window == 0: everything.

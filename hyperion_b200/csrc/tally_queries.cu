@@ -13,10 +13,11 @@
 // so that a thread takes 2^(c s) of what the product gives and adds it up.  (Read out of shared memory by all threads of a warp they cost more of its bandwidth than the products' operands: the second walk of three prompts 104 us, and 73 so.)
 // A tile of Q has whole tokens: 128 / group of them with all heads of a key/value head, by one TMA box a panel.
 //
-// Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.  Nothing is added by atomics, so results
-// do not depend on which block came first.
+// Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.  (By clusters of up to 16 cuts two requests' 8 queries of
+// 1,000 slots take 11.0 us in place of 11.8, but 32 of 8,192 20.0 in place of 18.4 and 8 of 60,000 82 in place of 61.)  In the second walk a cluster's blocks share the tiles of Q that see a tile of slots, and read one
+// another's sums in shared memory.  Nothing is added by atomics, so results do not depend on which block came first.
 //
-// Measured: three prompts of up to 2,047 tokens, 32 heads over 8 of 128, 127 us (both walks' products 0.58 PFLOP/s), of which the first walk takes 60, the second 60 and the parts 5.  In the loop a tile of 128 x 128 takes an SM
+// Measured: three prompts of up to 2,047 tokens, 32 heads over 8 of 128, 123 us (both walks' products 0.6 PFLOP/s), of which either walk takes some 60.  In the loop a tile of 128 x 128 takes an SM
 // 950 to 1,150 clocks: 576 of them are its products, 730 its exponentials on the special function unit (11 of 16 pairs), some 700 its instructions; blocks of two halves with a buffer each do not quite keep them all
 // busy, and starts and ends of blocks cost another 15 %.  The last 32 of 8,192 tokens, 28 heads over 4: 18.5 us, three kernels' starts and trips to memory.  (With mma.sync and registers in place of tensor memory 890 and 49 us.)
 //
@@ -40,7 +41,7 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 constexpr int BM = 128;                        // rows that stay, and rows that pass
 constexpr int PANEL = BM * 128, PANELS = D / 64, TILE = PANELS * PANEL;  // bytes
 constexpr int STAGES = D == 128 ? 2 : 4;       // of the ring: two blocks share an SM's memory
-constexpr int MOST_SPANS = 16;                 // blocks that a request's tiles of Q pass at most, each of which leaves a part of the sums
+constexpr int MOST_SPANS = 16;                 // blocks that share the tiles of Q that pass a tile of slots, a cluster
 constexpr int HALF = 4, PRODUCER = 2 * HALF, ISSUER = PRODUCER + 1, THREADS = 32 * (ISSUER + 1);  // warps that look at scores: four for each of the two buffers
 constexpr int TMEM_COLS = 2 * BM;              // two blocks have all of an SM's
 constexpr unsigned WAIT_LIMIT = HB_WAIT_LIMIT, LAST_WAIT_LIMIT = 1u << 24;
@@ -199,6 +200,17 @@ __device__ __forceinline__ Pair polynomial_exp2(Pair y) {
 constexpr int POLYNOMIAL = 5;
 __device__ __forceinline__ Pair exp2_of(Pair y, int pair) { return (pair + 1) * POLYNOMIAL / 16 != pair * POLYNOMIAL / 16 ? polynomial_exp2(y) : Pair{fast_exp2(y.x), fast_exp2(y.y)}; }
 
+// The blocks of a cluster.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ float of_block(const float* p, int rank) {  // what another block of the cluster has at this place of its shared memory
+    unsigned at;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
 struct Args {
     const int* block_table; int table_width;
     const int* starts;    // [requests + 1]
@@ -209,8 +221,7 @@ struct Args {
     uint4* rows;          // [tokens * heads]: -(m + log2 l) / c in three parts of bfloat16, and zeros
     float2* cuts;         // [n_cuts, tokens * heads]: (m, l), where the slots are cut
     int n_cuts;
-    float* parts;         // [spans, requests, kv_heads, padded]: a span's part of the slots' sums, where there is more than one
-    int span, spans, padded;  // tiles of Q that pass a block, and into how many such spans they go; slots in whole tiles
+    int spans;            // blocks of a cluster, which share the tiles of Q that pass a tile of slots
     int heads, kv_heads, group, page_shift, pages;
     int per_tile;         // tokens of a tile of Q
     float scale_log2;
@@ -239,7 +250,7 @@ __device__ __forceinline__ uint4 beside_row(float m, float l, float c) {
 }
 __device__ __forceinline__ int first_tile(const Args& a, int slot, int before) { return max(0, slot - before) / a.per_tile; }  // token slot - before is the first that sees the slot
 
-// One walk.  KEYS_STAY: block (span of tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (tile of Q and key/value head, cut, request), tiles of K pass.
+// One walk.  KEYS_STAY: block (span of the tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (tile of Q and key/value head, cut, request), tiles of K pass.
 template <bool KEYS_STAY>
 __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap rows_map, const Args a) {
     extern __shared__ unsigned char smem_raw[];
@@ -276,15 +287,15 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
     int from, to;  // tiles that pass
     if (KEYS_STAY) {
-        if (base >= r.length || r.tokens == 0) {
-            wait_for_previous_kernels();  // whoever comes next takes this kernel's end as the end of all
+        from = first_tile(a, base, before), to = q_tiles;
+        const int see = to - from;  // tiles that see any of the slots
+        if (base >= r.length || see <= 0) {  // the same for all blocks of a cluster
+            wait_for_previous_kernels();     // whoever comes next takes this kernel's end as the end of all
             return;
         }
-        const int span = blockIdx.x % a.spans;
-        from = max(span * a.span, first_tile(a, base, before)), to = min(q_tiles, (span + 1) * a.span);
-        if (from >= to) {
-            wait_for_previous_kernels();
-            return;
+        if (a.spans > 1) {
+            const int span = blockIdx.x % a.spans;
+            to = from + see * (span + 1) / a.spans, from += see * span / a.spans;  // at most 2^24 tiles: tokens * heads fit 31 bits
         }
     } else {
         if (base >= r.tokens) return;
@@ -331,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     };
     // The second walk's tile is on its way while the first one ends: its blocks are let in once all of the first walk's have waited, so what came before that one has finished.
     if (KEYS_STAY) {
-        if (warp == PRODUCER) fetch_keys(stays, page_at(base), stays_full);
+        if (warp == PRODUCER && n_tiles > 0) fetch_keys(stays, page_at(base), stays_full);
         wait_for_previous_kernels();
     }
     // Tensor memory is taken only now that the kernels before have finished, and the next kernel is let in only once it is: a block further back or further on that holds some while it waits could wait for this one.
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         if (half == 0 && ok) {
             if constexpr (KEYS_STAY) {
                 sum += theirs[mine] - (rest + theirs[BM + mine]);
-                if (a.spans > 1) a.parts[(((size_t)(blockIdx.x % a.spans) * gridDim.z + request) * a.kv_heads + kvh) * a.padded + base + mine] = sum;
+                if (a.spans > 1) theirs[mine] = sum;
                 else if (base + mine < r.length) a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + base + mine] += sum;
             } else if (mine < q_rows && token < r.tokens) {
                 const float other = theirs[mine], above = fmaxf(m, other);
@@ -502,6 +513,24 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     if (warp == ISSUER) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }    if constexpr (KEYS_STAY) {
+        // The spans' sums of a slot, in their order.  Tensor memory has been given back, so that no block has some while it waits for another.
+        if (a.spans > 1) {
+            const int rank = blockIdx.x % a.spans, slot = rank + tid * a.spans;  // whose sums this thread adds up
+            const bool adds = slot < BM && base + slot < r.length;
+            float* weight = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + base + slot;
+            const float old = adds ? *weight : 0.f;
+            cluster_arrive(), cluster_wait();
+            if (adds) {
+                float part[MOST_SPANS], sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < MOST_SPANS; ++k) part[k] = k < a.spans ? of_block(theirs + slot, k) : 0.f;
+#pragma unroll
+                for (int k = 0; k < MOST_SPANS; ++k) sum += part[k];
+                *weight = old + sum;
+            }
+            cluster_arrive(), cluster_wait();  // the sums have been read
+        }
     }
 }
 
@@ -524,27 +553,6 @@ __global__ void __launch_bounds__(256) tally_cuts_kernel(const Args a, int lanes
     if (mine == 0 && at < n) a.rows[at] = beside_row(above, all, a.scale_log2);
 }
 
-// The spans' parts of the slots' sums, in their order.
-__global__ void __launch_bounds__(256) tally_parts_kernel(const Args a) {
-    let_next_kernel_start();
-    wait_for_previous_kernels();
-    const int slot = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y, request = blockIdx.z;
-    const Request r = request_of(a, request, false);
-    if (slot >= r.length) return;
-    const int first = first_tile(a, slot / BM * BM, r.length - r.tokens) / a.span, end = ((r.tokens + a.per_tile - 1) / a.per_tile + a.span - 1) / a.span;  // spans that the tile of slots has a block for
-    float* weight = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + slot;
-    const float before = *weight;
-    float sum = 0.f;
-    for (int span = first; span < end; span += 4) {  // four on their way together
-        float part[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) part[k] = span + k < end ? a.parts[(((size_t)(span + k) * gridDim.z + request) * a.kv_heads + kvh) * a.padded + slot] : 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum += part[k];
-    }
-    *weight = before + sum;
-}
-
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
@@ -564,10 +572,21 @@ int encoded(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
 }
 template <bool KEYS_STAY>
-int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUtensorMap& rows_map, const Args& a, dim3 grid, cudaStream_t stream) {
+int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUtensorMap& rows_map, const Args& a, dim3 grid, int together, cudaStream_t stream) {  // blocks of a cluster, along x
     static std::atomic<unsigned long long> allowed{0};
     if (const cudaError_t error = allow_shared((const void*)tally_walk_kernel<KEYS_STAY>, SMEM_BYTES, allowed)) return (int)error;
-    return launch_after_previous(tally_walk_kernel<KEYS_STAY>, grid, dim3(THREADS), SMEM_BYTES, stream, kv_map, q_map, rows_map, a);
+    static std::atomic<unsigned long long> wide{0};
+    if (together > 8)
+        if (const cudaError_t error = allow_wide_clusters((const void*)tally_walk_kernel<KEYS_STAY>, wide)) return (int)error;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid, config.blockDim = dim3(THREADS), config.dynamicSmemBytes = SMEM_BYTES, config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = overlap_launches() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim = {(unsigned)together, 1, 1};
+    config.attrs = attributes, config.numAttrs = together > 1 ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&config, tally_walk_kernel<KEYS_STAY>, kv_map, q_map, rows_map, a);
 }
 }  // namespace
 
@@ -579,26 +598,27 @@ static int cuts_for(int requests, int most, int longest, int heads, int kv_heads
     const long long blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads * requests, wanted = 2LL * sms / (blocks ? blocks : 1), most_cuts = tiles <= 4 ? 1 : (tiles + 1) / 2;
     return (int)(wanted < 1 ? 1 : wanted < most_cuts ? wanted : most_cuts);
 }
-// Tiles of Q that pass a block of the second walk, and into how many such spans they go: 16 where there are blocks enough for the device, two an SM; down to three where there are not, but one span up to four tiles.  (us, at
-// least 2 / 3 / 4 / 8 / 16 tiles: 14 heads over 2 of 64, a prompt of 500 tokens 14.1 / 15.0 / 15.5 / 19.1 / 23.1, four of 300 15.9 / 13.9 / 14.7 / 18.3 / 22.4; 28 over 4 of 128, 500 tokens 18.7 / 18.9 / 17.2 / 20.6 /
-// 25.1; 16 over 1 of 128, 200 tokens 12.6 / 13.2 / 13.9 / 17.2 / 24.6.)
-static int span_for(int requests, int most, int longest, int heads, int kv_heads, int sms, int* spans) {
+// Blocks of the second walk that share the tiles of Q that pass a tile of slots.  A block takes the time of its tiles and of some three more, for its start, and longer the more blocks an SM has, from 0.7 on: of some sizes the one
+// with the smallest such product.  Even ones, because an SM holds two, and no 10 to 14, of which few fit a group of SMs.  (us, one / two / four / six / eight / 16 blocks, the one that is taken in brackets: 14 heads over 2 of
+// 64, a prompt of 300 tokens 21.9 / 16.9 / 13.4 / 12.5 / 11.7 / [11.1], of 895 43.7 / 30.1 / 23.0 / 20.4 / [18.7] / 19.7; 28 over 4 of 128, 500 tokens 32.0 / 23.0 / 18.6 / [16.6] / 17.5 / 20.8, three prompts of 700 46.2 /
+// 35.2 / [34.3] / 36.2 / 39.1 / 56.5; 32 over 8 of 128, three of 2,047 127.5 / [123.5] / 135.4 / 153.9 / 173.5 / 266.5.  Over 85 sizes it comes within 1 % of the best on average.)
+static int spans_for(int requests, int most, int longest, int heads, int kv_heads, int sms) {
     const int per_tile = BM / (heads / kv_heads), tiles = (most + per_tile - 1) / per_tile;
-    const long long blocks = (long long)((longest + BM - 1) / BM) * kv_heads * requests, wanted = (2LL * sms + blocks - 1) / blocks;
-    long long span = (tiles + wanted - 1) / wanted;
-    span = tiles <= 4 ? 4 : span < 3 ? 3 : span > 16 ? 16 : span;
-    if ((tiles + MOST_SPANS - 1) / MOST_SPANS > span) span = (tiles + MOST_SPANS - 1) / MOST_SPANS;
-    *spans = (int)((tiles + span - 1) / span);
-    return (int)span;
+    const float blocks = (float)((longest + BM - 1) / BM) * (float)kv_heads * (float)requests;
+    int best = 1;
+    float least = INFINITY;
+    for (int n : {1, 2, 4, 6, 8, MOST_SPANS}) {
+        if (n > tiles) break;
+        const float crowd = blocks * (float)n / (float)sms - 0.7f, cost = ((float)tiles / (float)n + 3.f) * (1.f + 0.8f * (crowd > 0.f ? crowd : 0.f));
+        if (cost < least) least = cost, best = n;
+    }
+    return best;
 }
 // Bytes of scratch that hb_tally_queries takes.
 HB_EXPORT long long hb_tally_queries_scratch(int tokens, int requests, int most, int longest, int heads, int kv_heads, int sms) {
     if (tokens <= 0 || requests <= 0 || most <= 0 || longest <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > BM || sms <= 0) return 0;
     const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms);
-    int spans;
-    span_for(requests, most, longest, heads, kv_heads, sms, &spans);
-    const long long padded = (longest + BM - 1) / BM * (long long)BM;
-    return 16LL * tokens * heads + (cuts > 1 ? 8LL * tokens * heads * cuts : 0) + (spans > 1 ? 4LL * spans * requests * kv_heads * padded : 0);
+    return 16LL * tokens * heads + (cuts > 1 ? 8LL * tokens * heads * cuts : 0);
 }
 // q [tokens, heads * D] with rows q_stride apart, request r's from starts[r] to starts[r + 1] - 1, at most `most`, the last of which stands in its last slot; cache [pages, 2, kv_heads, page_size, D];
 // lengths [requests], at most `longest`, which table and capacity hold; weights [requests, kv_heads, capacity].  scratch: hb_tally_queries_scratch bytes on a 16-byte boundary.
@@ -614,9 +634,8 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     if ((long long)pages * 2 * kv_heads * page_size > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;  // a row's number in the cache's tensor map
     const long long row_blocks = (long long)((most + per_tile - 1) / per_tile) * kv_heads;
     if (row_blocks > 0x7fffffffLL || sms > 16384) return HB_UNSUPPORTED_SIZE;
-    int spans;
-    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), span = span_for(requests, most, longest, heads, kv_heads, sms, &spans), padded = (longest + BM - 1) / BM * BM;
-    if ((long long)padded / BM * spans > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
+    const int cuts = cuts_for(requests, most, longest, heads, kv_heads, sms), spans = spans_for(requests, most, longest, heads, kv_heads, sms), slot_tiles = (longest + BM - 1) / BM;
+    if ((long long)slot_tiles * spans > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     CUtensorMap kv_map, q_map, rows_map;
     const cuuint64_t kv_dims[2] = {(cuuint64_t)D, (cuuint64_t)pages * 2 * kv_heads * page_size}, kv_strides[1] = {(cuuint64_t)D * 2};
     const cuuint32_t kv_box[2] = {64, (cuuint32_t)page_size};
@@ -630,9 +649,9 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     const cuuint32_t rows_box[3] = {8, (cuuint32_t)group, (cuuint32_t)per_tile};
     if (int code = encoded(&rows_map, rows, 3, rows_dims, rows_strides, rows_box, CU_TENSOR_MAP_SWIZZLE_NONE)) return code;
     float2* cut_sums = (float2*)(rows + (size_t)tokens * heads);
-    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, (float*)(cut_sums + (cuts > 1 ? (size_t)tokens * heads * cuts : 0)), span, spans, padded, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
+    const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, spans, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
                  scale * 1.4426950408889634f, status};
-    if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3((unsigned)row_blocks, cuts, requests), stream)) return code;
+    if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3((unsigned)row_blocks, cuts, requests), 1, stream)) return code;
     if (cuts > 1) {
         int lanes = 2;
         while (lanes < 32 && lanes < cuts) lanes *= 2;
@@ -640,6 +659,5 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
         if (threads > 0x7fffffffLL - 256) return HB_UNSUPPORTED_SIZE;
         if (int code = launch_after_previous(tally_cuts_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, lanes)) return code;
     }
-    if (int code = launch_walk<true>(kv_map, q_map, rows_map, a, dim3(padded / BM * spans, kv_heads, requests), stream)) return code;
-    return spans > 1 ? launch_after_previous(tally_parts_kernel, dim3((longest + 255) / 256, kv_heads, requests), dim3(256), 0, stream, a) : 0;
+    return launch_walk<true>(kv_map, q_map, rows_map, a, dim3(slot_tiles * spans, kv_heads, requests), spans, stream);
 }

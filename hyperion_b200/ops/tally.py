@@ -144,8 +144,8 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  What is beyond them is left out and reported (``raise_on_status``).  A NaN or an
     infinity among the scores that a query sees makes the weights of those slots NaN.
 
-    A call's scratch memory is 16 * heads bytes per query, 8 * heads more for each of the cuts into which slots go where few queries look at many (two blocks a multiprocessor in all), and for prompts of more
-    than 512 (token, head) rows a key/value head 4 * kv_heads bytes per request, slot up to ``longest`` and span of those rows, 16 spans at most: up to 16 MB are kept per thread and stream, more is allocated for the call."""
+    A call's scratch memory is 16 * heads bytes per query, and 8 * heads more for each of the cuts into which slots go where few queries look at many (two blocks a multiprocessor in all): up to 16 MB are kept
+    per thread and stream, more is allocated for the call."""
     what = "tally_queries"
     pages, _, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, scale)
     requests, tokens, capacity = lengths.numel(), q.shape[0], tally.weights.shape[-1] if tally.weights.shape else 0
