@@ -840,12 +840,12 @@ HB_EXPORT long long hb_attention_tallied_scratch(int requests, int longest, int 
     return 4 * heads * (requests * slots + pieces * (D + 2));
 }
 // q [requests, heads * D] with rows q_stride apart; cache [pages, 2, kv_heads, page_size, D]; weights, positions [requests, kv_heads, capacity]; lengths, newest [requests], lengths at most
-// `longest`, which table and capacity hold.  scratch: hb_attention_tallied_scratch bytes on a 16-byte boundary.
+// `longest`, which table and capacity hold.  scratch: hb_attention_tallied_scratch bytes on a 16-byte boundary, null where it takes none.
 HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, const int* block_table, int table_width, const int* lengths, int requests,
                                    int longest, float* weights, int* positions, const int* newest, int capacity, int heads, int kv_heads, int page_size, int pages, float scale, int sms, void* scratch,
                                    int* status, cudaStream_t stream) {
     if (requests <= 0) return 0;
-    if (!q || !out || !cache || !block_table || !lengths || !weights || !positions || !newest || !scratch || !status) return HB_BAD_ARGUMENT;
+    if (!q || !out || !cache || !block_table || !lengths || !weights || !positions || !newest || !status) return HB_BAD_ARGUMENT;
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || capacity < longest || sms <= 0 || sms > 16384 || q_stride % 8 || out_stride % 4 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
@@ -857,6 +857,7 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     if ((long long)kv_heads * strips.chunks > 65535) return HB_UNSUPPORTED_SIZE;
     int kept = 0;
     const int together = together_for(requests, longest, heads, kv_heads, sms, &kept), blocks = together ? 0 : blocks_for(requests, longest, heads, kv_heads, sms);
+    if (!together && !scratch) return HB_BAD_ARGUMENT;
     // (us, one block / one a head: 16 requests at 4,099, 7 pieces each, 26.5 / 27.6; 64 at 8,192 151 / 158; three at 23,080 of 14 heads over 2 of 64, 74 pieces each, 34 / 14)
     const int join_blocks = (blocks / requests) * ((group + 7) / 8) > 16 ? group : 1;
     const size_t n_pieces = (size_t)blocks + requests;

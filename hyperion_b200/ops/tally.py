@@ -111,7 +111,8 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     what = "attention_tallied"
     pages, _, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, scale)
     weights, positions = tally
-    requests, capacity, width = q.shape[0], weights.shape[-1] if weights.shape else 0, heads * head_dim
+    requests, held, width = q.shape[0], weights.shape, heads * head_dim
+    capacity = held[-1] if held else 0
     _check_tally(tally, (requests, kv_heads, capacity), what)
     longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
@@ -128,7 +129,8 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
         out[:, :width].zero_()
         return out
     stream, sms = stream_address(), sm_count(device)
-    memory, owner = scratch(device, stream, _scratch_size("attention_tallied", "hb_attention_tallied_scratch", head_dim, requests, longest, heads, kv_heads, sms))
+    size = _scratch_size("attention_tallied", "hb_attention_tallied_scratch", head_dim, requests, longest, heads, kv_heads, sms)
+    memory, owner = scratch(device, stream, size) if size else (0, None)  # clusters need none
     check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim)(
         q.data_ptr(), q.stride(0) if requests > 1 else width, out.data_ptr(), out.stride(0) if requests > 1 else width, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, weights.data_ptr(),
         positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
@@ -148,7 +150,8 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     per thread and stream, more is allocated for the call."""
     what = "tally_queries"
     pages, _, kv_heads, page_size, head_dim = _check_pages(what, cache, heads, q, scale)
-    requests, tokens, capacity = lengths.numel(), q.shape[0], tally.weights.shape[-1] if tally.weights.shape else 0
+    requests, tokens, held = lengths.numel(), q.shape[0], tally.weights.shape
+    capacity = held[-1] if held else 0
     _check_tally(tally, (requests, kv_heads, capacity), what)
     longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
@@ -193,7 +196,8 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
         raise KernelError(f"{what}: pages of a power of two and records of whole 16 bytes, not {page_size} and {record}")
     weights, positions = tally
     to_weights, to_positions = to = tally if out is None else out
-    requests, capacity = lengths.numel(), weights.shape[-1] if weights.shape else 0
+    requests, held = lengths.numel(), weights.shape
+    capacity = held[-1] if held else 0
     held = (layers, requests, kv_heads, capacity) if layered else (requests, kv_heads, capacity)
     _check_tally(tally, held, what)
     if to is not tally:
@@ -207,7 +211,7 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
         raise KernelError(f"{what}: keep from 1, first and recent from 0 to {LARGEST}, not {keep}, {first} and {recent}")
     _check_device(what, cache, block_table, lengths, newest, weights, positions, to_weights, to_positions)
     device = cache.device
-    left = torch.empty(requests, dtype=torch.int32, device=device)
+    left = torch.empty_like(lengths)
     if requests == 0 or layers == 0 or kv_heads == 0 or longest == 0:
         return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
     stream = stream_address()
