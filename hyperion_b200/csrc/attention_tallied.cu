@@ -131,7 +131,7 @@ struct Args {
     int heads, kv_heads, page_size, pages;
     int gc, chunks;          // heads of a set, blocks' chunks of a key/value head's group
     int blocks;              // of the first kernel, side by side
-    int join_blocks;         // of the second, a request and key/value head, that put results together: one, or one a head
+    int join_blocks, by_head;  // of the second, a request and key/value head, that put results together: one a head, or one for all of them, a warp each
     int together, kept;      // or 0, or the blocks of a cluster, which has one request and key/value head; slots whose scores each of them keeps
     float scale_log2;
     int* status;
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 3) tally_kernel(const Args a) {
         all = warp_sum(top == -INFINITY ? all : all * fast_exp2(top - above));
         return make_float2(above == -INFINITY ? 0.f : above, all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all));
     };
-    if (puts_together && a.join_blocks == 1) {
+    if (puts_together && !a.by_head) {
         constexpr int TOGETHER = 4;  // pieces that are on their way together
         for (int h = warp; h < group; h += ADD_THREADS / 32) {
             const size_t slot0 = piece0 + h;
@@ -803,16 +803,22 @@ int launch_strips(const Args& a, const CUtensorMap& map, cudaStream_t stream) {
 }
 }  // namespace
 
+// Whether the second kernel has a block for each head.
+static bool few_heads(int requests, int heads, int sms) { return (long long)requests * heads <= 2LL * sms; }
 // The blocks of a cluster that keeps its scores, and how many slots each keeps; or 0, where there are two kernels.  A cluster has one request and key/value head, so its work is as long as the longest request; the line's is
-// equal for all blocks but costs a second kernel.  Clusters are the faster ones up to some 14 tiles of 64 slots a multiprocessor (us, clusters / line, 28 heads over 4 of 128: one request at 512 slots 6.6 / 8.6, at 8,192
-// 25 / 38; four at 4,099 17.5 / 20.3, at 8,192 29 / 26; 16 at 512 8.6 / 10.7, at 2,048 19.1 / 19.0, at 4,099 35 / 27; 64 at 512 19 / 20, at 2,048 54 / 42; 14 heads over 2 of 64, four at 8,192 18 / 25).  As many blocks a
-// cluster as the device holds at once, two a multiprocessor, one of more than eight heads.
+// equal for all blocks but costs a second kernel.  Clusters are the faster ones for few tiles of 64 slots, in all or a block, and for more of them where the second kernel has no
+// block for each head, as long as all of them are on the device at once (us, clusters / line, 28 heads over 4 of 128: one request at 512 slots 6.5 / 6.2 and a launch less for the host, at 2,048 10.1 / 7.4, at 8,192 24.3 / 14.9; 16 at 256 7.3 / 8.5, at 512 9.1 / 10.8, at 2,048
+// 18.9 / 18.4; 64 at 256 11.7 / 15.0; 16 heads over 1: eight at 1,024 8.8 / 10.4, one at 4,099 16.4 / 9.7).  As many blocks a cluster as leave room, with some to spare: two are on an SM, one of more than eight heads, and
+// few clusters of eight fit a group of SMs (eight requests at 512: of eight blocks 10.0, of four 8.0).
 static int together_for(int requests, int longest, int heads, int kv_heads, int sms, int* kept) {
-    const long long pairs = (long long)requests * kv_heads, tiles = (longest + BN - 1) / BN, room = heads / kv_heads <= 8 ? 2LL * sms : sms;
-    if (heads / kv_heads > 16 || tiles > MOST_TOGETHER * MOST_KEPT / BN || pairs * tiles > 14LL * sms) return 0;
+    const bool narrow = heads / kv_heads <= 8;
+    const long long pairs = (long long)requests * kv_heads, tiles = (longest + BN - 1) / BN, room = narrow ? 2LL * sms : sms;
+    if (heads / kv_heads > 16 || pairs > room) return 0;
     int blocks = 1;
-    while (blocks < MOST_TOGETHER && ((tiles + blocks - 1) / blocks * BN > MOST_KEPT || (pairs * blocks * 2 <= room && tiles > blocks))) blocks *= 2;
-    *kept = (int)((tiles + blocks - 1) / blocks * BN);
+    while (blocks < MOST_TOGETHER && blocks < tiles && pairs * blocks * 2 * 100 <= room * (blocks == 4 ? 65 : 87)) blocks *= 2;
+    const long long each = (tiles + blocks - 1) / blocks;
+    if (tiles > (narrow ? 8 : 16) && each > (few_heads(requests, heads, sms) ? (narrow ? 2 : 3) : (narrow ? 4 : 8))) return 0;
+    *kept = (int)each * BN;
     return blocks;
 }
 // How a key/value head's group of heads is cut: into chunks, each a block's, and those into sets.
@@ -858,14 +864,15 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     int kept = 0;
     const int together = together_for(requests, longest, heads, kv_heads, sms, &kept), blocks = together ? 0 : blocks_for(requests, longest, heads, kv_heads, sms);
     if (!together && !scratch) return HB_BAD_ARGUMENT;
-    // (us, one block / one a head: 16 requests at 4,099, 7 pieces each, 26.5 / 27.6; 64 at 8,192 151 / 158; three at 23,080 of 14 heads over 2 of 64, 74 pieces each, 34 / 14)
-    const int join_blocks = (blocks / requests) * ((group + 7) / 8) > 16 ? group : 1;
+    // One block a head where they are few or have many pieces (us, one block for all heads / one a head: 28 heads over 4, one request at 1,024 slots 9.6 / 6.5, four 11.2 / 8.0, but 16 at 1,024 14.1 / 14.9, at 4,099
+    // 26.1 / 27.4; 14 over 2 of 64, 16 at 2,048 12.1 / 8.7, three at 23,080, 74 pieces each, 34 / 14).
+    const int by_head = few_heads(requests, heads, sms) || (blocks / requests) * ((group + 7) / 8) > 16, join_blocks = by_head ? group : 1;
     const size_t n_pieces = (size_t)blocks + requests;
     float* pieces = (float*)scratch;
     float* scores = pieces + n_pieces * heads * D;  // before the sums, so that its rows begin on 16 bytes
     float2* sums = (float2*)(scores + (size_t)requests * heads * slots);
     const Args a{(const bf16*)q, (int)q_stride, (bf16*)out, (int)out_stride, block_table, table_width, lengths, requests, longest, slots, scores, pieces, sums, weights, positions, newest, capacity,
-                 heads, kv_heads, page_size, pages, strips.heads, strips.chunks, blocks, join_blocks, together, kept, scale * 1.4426950408889634f, status};
+                 heads, kv_heads, page_size, pages, strips.heads, strips.chunks, blocks, join_blocks, by_head, together, kept, scale * 1.4426950408889634f, status};
     CUtensorMap map;
     if (int code = cache_map(&map, cache, a)) return code;
     if (int code = strips.sets == 3 ? launch_strips<1, 3>(a, map, stream) : strips.heads <= 8 ? launch_strips<1, 1>(a, map, stream) : launch_strips<2, 1>(a, map, stream)) return code;
