@@ -423,13 +423,14 @@ HB_EXPORT int hb_evict(void* cache, int layers, int pages, int kv_heads, int pag
     if (requests > 65535 || layers > 65535 || (long long)requests * kv_heads > 65535 || heads > 0x7fffffffLL || record_bytes > 65536) return HB_UNSUPPORTED_SIZE;
     if (longest > 0x7fffffff - MOST_BLOCKS * 32 * LOOK || capacity > 0x7fffffff - 4 * MOST_BLOCKS * 1024 || (long long)kv_heads * MOST_BLOCKS > 0x7fffffffLL) return HB_UNSUPPORTED_SIZE;
     const int most = longest - keep < keep ? (longest > keep ? longest - keep : 0) : keep;
-    // Clusters where heads are few and long: up to four blocks while there is an SM for each and more than 3,584 slots, eight only for a few heads, because clusters of eight SMs leave others empty.  (us, one / two / four /
-    // eight blocks: 48 heads of 4,097 slots 10.0 / 13.2; 48 of 7,470 19.7 / 18.2; 64 of 15,625 24.1 / 21.1; 16 of 18,734 19.3 / - / 16.4 / 27.5; 32 of 32,771, 28,675 of them given up, 42.8 / - / 33.3; 8 of 131,000
-    // 99 / - / 56 / 36.)  Blocks of 256 threads where heads are short, or more than there are SMs, which hold three to five of those: 224 heads of 1,025 10.2 against 15.9, 896 of 2,049 18.4 against 32.9, 256 of 4,097 15.8
-    // against 19.8, but 48 of 4,097 11.5 against 10.0.
-    int blocks = 1;
-    while (blocks < MOST_BLOCKS && heads * blocks * (blocks < 4 ? 2 : 4) <= sms && longest >= blocks * 2 * 3584) blocks *= 2;
-    const int threads = longest <= 2048 || (heads > sms && longest <= 8192) ? 256 : 1024, looks = threads / 32 * LOOK;
+    // Clusters where heads are few and long or give up much, of four blocks while there is an SM for each, else two; eight only for a few heads, because clusters of eight SMs leave others empty.  (us, one / two / four / eight
+    // blocks, 16 heads, one slot given up of 8,192 12.0 / 13.1 / 13.4 / 26.8, of 16,384 16.8 / 15.5 / 13.4 / 26.9, a quarter of 8,192 22.5 / 19.9 / 17.2 / 32.5; four heads, a quarter of 16,384 39.2 / 27.8 / 21.3 / 19.3; 64
+    // heads, a quarter of 16,384 46.7 / 39.4 / 50.5.)  Blocks of 256 threads where heads are short, or more than there are SMs, which hold three to five of those (us, 256 / 1,024 threads, one slot given up of 1,000: 16 heads
+    // 6.9 / 8.3, 256 heads 9.7 / 16.3, of 4,097: 256 heads 15.8 / 19.8, 16 heads 11.5 / 10.0; a quarter of 1,000: 128 heads 12.5 / 9.4, 512 heads 16.2 / 28.3, of 8,192: 512 heads 101 / 80).
+    const long long size = longest + 2LL * most;
+    const int blocks = size < 10240 ? 1 : size >= 24576 && heads * 16 <= sms ? 8 : heads * 4 <= sms ? 4 : heads * 2 <= sms ? 2 : 1;
+    const bool few = heads * 2 <= sms, many = heads > sms;
+    const int threads = longest <= (many ? 6144 : few ? 2048 : 512) && blocks == 1 ? 256 : 1024, looks = threads / 32 * LOOK;
     const size_t held = (size_t)((longest + blocks * looks - 1) / (blocks * looks)) * looks;
     int* moves = (int*)scratch;
     int* lists = (int*)((char*)scratch + (heads * 4 + 15) / 16 * 16);
