@@ -879,3 +879,4 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
     if (together) return 0;
     return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + join_blocks, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
 }
+HB_EXPORT int hb_attention_tallied_packed(const void* arguments) { return call_packed(&hb_attention_tallied, arguments); }

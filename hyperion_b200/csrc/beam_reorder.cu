@@ -144,3 +144,4 @@ HB_EXPORT int hb_beam_reorder(const int* parents, const int* lengths, int groups
     const auto kernel = beams <= 4 ? beam_reorder_kernel<4> : beams <= 8 ? beam_reorder_kernel<8> : beams <= 16 ? beam_reorder_kernel<16> : beam_reorder_kernel<32>;
     return launch_after_previous(kernel, dim3((unsigned)(blocks + a.table_blocks), groups), dim3(THREADS), 0, stream, a);
 }
+HB_EXPORT int hb_beam_reorder_packed(const void* arguments) { return call_packed(&hb_beam_reorder, arguments); }

@@ -559,3 +559,4 @@ HB_EXPORT int hb_beam_select(const void* logits, int is_bf16, long long stride, 
     a.sums = (double2*)scratch, a.tops = (float*)(a.sums + rows * a.pieces), a.parents = parents, a.tokens = tokens, a.out_scores = out_scores;
     return is_bf16 ? launch<bf16>(a, stream) : launch<float>(a, stream);
 }
+HB_EXPORT int hb_beam_select_packed(const void* arguments) { return call_packed(&hb_beam_select, arguments); }

@@ -7,8 +7,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
+#include <string.h>
 
 #include <atomic>
+#include <tuple>
 
 #define HB_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -120,6 +122,21 @@ __device__ __forceinline__ float activated(float v, int act) {
 }
 
 static inline int launch_status() { return (int)cudaGetLastError(); }
+
+// ---------------------------------------------------------------- launchers whose arguments come as one structure
+// The arguments of `launcher` one behind the other, each on a boundary of its own size.
+template <typename... Params>
+static inline int call_packed(int (*launcher)(Params...), const void* packed) {
+    size_t at = 0;
+    const auto next = [&](auto value) {
+        at = (at + sizeof(value) - 1) / sizeof(value) * sizeof(value);
+        memcpy(&value, static_cast<const char*>(packed) + at, sizeof(value));
+        at += sizeof(value);
+        return value;
+    };
+    const std::tuple<Params...> values{next(Params{})...};  // in their order
+    return std::apply(launcher, values);
+}
 
 // ---------------------------------------------------------------- programmatic dependent launch
 // A kernel launched through launch_after_previous() may start while the kernel before it in the

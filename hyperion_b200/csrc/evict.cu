@@ -442,3 +442,4 @@ HB_EXPORT int hb_evict(void* cache, int layers, int pages, int kv_heads, int pag
     if (!most || moves_here) return 0;
     return launch_after_previous(evict_move_kernel, dim3((most + PER_BLOCK - 1) / PER_BLOCK, kv_heads * requests, layers), dim3(MOVE_THREADS), 0, stream, a);
 }
+HB_EXPORT int hb_evict_packed(const void* arguments) { return call_packed(&hb_evict, arguments); }

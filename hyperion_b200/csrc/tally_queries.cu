@@ -661,3 +661,4 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     }
     return launch_walk<true>(kv_map, q_map, rows_map, a, dim3(slot_tiles * spans, kv_heads, requests), spans, stream);
 }
+HB_EXPORT int hb_tally_queries_packed(const void* arguments) { return call_packed(&hb_tally_queries, arguments); }

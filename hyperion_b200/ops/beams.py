@@ -65,7 +65,8 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
         raise KernelError(f"{what}: a tensor once only")
     if rows == 0 or not words:
         return
-    check(entry("beam_reorder", "hb_beam_reorder", "ppiipiipippp")(
+    described = (ctypes.c_longlong * len(words))(*words)
+    check(entry("beam_reorder", "hb_beam_reorder", "ppiipiipippp", packed=True)(
         parents.data_ptr(), lengths.data_ptr(), groups, beams, block_table.data_ptr() if block_table is not None else 0, width, page_size,
-        (ctypes.c_longlong * len(words))(*words), len(words) // 7, state_rows.data_ptr() if state_rows is not None else 0,
+        ctypes.addressof(described), len(words) // 7, state_rows.data_ptr() if state_rows is not None else 0,
         status_word(parents.device).data_ptr(), stream_address()), what)

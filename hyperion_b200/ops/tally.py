@@ -131,7 +131,7 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     stream, sms = stream_address(), sm_count(device)
     size = _scratch_size("attention_tallied", "hb_attention_tallied_scratch", head_dim, requests, longest, heads, kv_heads, sms)
     memory, owner = scratch(device, stream, size) if size else (0, None)  # clusters need none
-    check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim)(
+    check(entry("attention_tallied", "hb_attention_tallied", "plplppipiipppiiiiifippp", head_dim, packed=True)(
         q.data_ptr(), q.stride(0) if requests > 1 else width, out.data_ptr(), out.stride(0) if requests > 1 else width, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), requests, longest, weights.data_ptr(),
         positions.data_ptr(), newest.data_ptr(), capacity, heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
     return out
@@ -167,7 +167,7 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
         return
     stream, sms = stream_address(), sm_count(device)
     memory, owner = scratch(device, stream, _scratch_size("tally_queries", "hb_tally_queries_scratch", head_dim, tokens, requests, most, longest, heads, kv_heads, sms))
-    check(entry("tally_queries", "hb_tally_queries", "plippippiiipiiiiifippp", head_dim)(
+    check(entry("tally_queries", "hb_tally_queries", "plippippiiipiiiiifippp", head_dim, packed=True)(
         q.data_ptr(), q.stride(0) if tokens > 1 else heads * head_dim, tokens, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], starts.data_ptr(), lengths.data_ptr(), requests, most, longest, tally.weights.data_ptr(), capacity,
         heads, kv_heads, page_size, pages, scale, sms, memory, status_word(device).data_ptr(), stream), what)
 
@@ -216,7 +216,7 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
         return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
     stream = stream_address()
     memory, owner = scratch(device, stream, _scratch_size("evict", "hb_evict_scratch", 0, layers, requests, kv_heads, longest, keep))
-    check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppip")(
+    check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppip", packed=True)(
         cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, weights.data_ptr(),
         positions.data_ptr(), to_weights.data_ptr(), to_positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), sm_count(device), stream), what)
     return left

@@ -46,7 +46,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamCh
         return BeamChoice(parents, tokens, found)
     stream, sms = stream_address(), sm_count(device)
     memory, owner = scratch(device, stream, _scratch_size("beam_select", "hb_beam_select_scratch", 0, groups, beams, vocab, take, sms))
-    check(entry("beam_select", "hb_beam_select", "pilpiiiipppipp")(logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab, scores.data_ptr(), groups, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(),
+    check(entry("beam_select", "hb_beam_select", "pilpiiiipppipp", packed=True)(logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab, scores.data_ptr(), groups, beams, vocab, take, parents.data_ptr(), tokens.data_ptr(),
                                                              found.data_ptr(), sms, memory, stream), "beam_select")
     return BeamChoice(parents, tokens, found)
 

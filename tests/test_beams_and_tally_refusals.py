@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from hyperion_b200 import ops
-from hyperion_b200.ops import KernelError, Tally
+from hyperion_b200.ops import KernelError, Tally, native
 from hyperion_b200.sampling import beam_select, reference_beam_select
 
 
@@ -107,3 +107,23 @@ def test_the_reference_selection():
     z[0, 1] = -np.inf
     assert [(b, v) for b, v, _ in reference_beam_select(z, np.array([0.0, -np.inf]), 4)] == [(0, 0), (0, 2)]
     assert reference_beam_select(np.full((2, 3), np.nan), np.zeros(2), 2) == []
+
+
+def test_a_launchers_arguments_come_as_one_structure():
+    """In their order and sizes: the launcher refuses what is wrong with any one of them, before it looks at the device."""
+    evict = native.entry("evict", "hb_evict", "piiiiipippiippppiiiipppip", packed=True)
+    names = ("cache layers pages kv_heads page_size record block_table width lengths newest requests longest weights positions to_weights to_positions capacity keep first recent left scratch status sms "
+             "stream").split()
+    sound = dict.fromkeys(names, 1 << 40) | dict(layers=1, pages=4, kv_heads=2, page_size=16, record=128, width=4, requests=70000, longest=64, capacity=64, keep=32, first=0, recent=0, sms=148, stream=0)
+
+    def call(**changed):
+        return evict(*(sound | changed).values())
+
+    assert call(requests=0) == 0 and call(layers=0) == 0
+    assert call() == -2  # more requests than a grid has room for
+    for name in ("cache", "block_table", "lengths", "newest", "weights", "positions", "to_weights", "to_positions", "left", "scratch", "status"):
+        assert call(**{name: 0}) == -1, name
+    for name, wrong in (("pages", 0), ("kv_heads", 0), ("page_size", 24), ("record", 24), ("width", 3), ("longest", 65), ("capacity", 63), ("keep", 0), ("recent", -1), ("sms", 0), ("cache", (1 << 40) + 8), ("scratch", (1 << 40) + 8)):
+        assert call(**{name: wrong}) == -1, name
+    with pytest.raises(KernelError, match="hb_evict"):
+        call(capacity=1 << 31)
