@@ -120,7 +120,7 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     _check_device(what, q, cache, block_table, lengths, newest, weights, positions, q if out is None else out)
     device = q.device
     if out is None:
-        out = torch.empty(requests, width, dtype=torch.bfloat16, device=device)
+        out = q.new_empty(requests, width)
     elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != requests or out.shape[1] < width or out.stride(1) != 1:
         raise KernelError(f"{what}: the output is a bfloat16 [{requests}, >= {width}] view")
     if requests == 0:

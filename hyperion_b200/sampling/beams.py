@@ -41,7 +41,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamCh
     kind, device, vocab = is_bf16(logits), logits.device, shape[1]
     _check_device("beam_select", logits, scores)
     parents, tokens = torch.empty(groups, take, dtype=torch.int32, device=device), torch.empty(groups, take, dtype=torch.int32, device=device)
-    found = torch.empty(groups, take, dtype=torch.float32, device=device)  # (three tensors cost the host 1 us less than views of one)
+    found = scores.new_empty(groups, take)  # (three tensors cost the host 1 us less than views of one)
     if groups == 0:
         return BeamChoice(parents, tokens, found)
     stream, sms = stream_address(), sm_count(device)
