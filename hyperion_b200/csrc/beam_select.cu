@@ -387,14 +387,14 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
         }
         return __uint_as_float(reached >> 31 ? reached ^ 1u << 31 : ~reached);  // no number where fewer threads have one
     };
-    // First the `take`-th largest of what eight threads together have as their best.
+    // First the `take`-th largest of what teams of threads have as their best.
     {
         float best = mine;
 #pragma unroll
         for (int o = 1; o < TEAM; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
         if (tid % TEAM == 0) bests[tid / TEAM] = best;
         __syncthreads();
-        // eight threads count for one of them what comes before it, equal ones by their numbers
+        // a team counts for one of them what comes before it, equal ones by their numbers
         const int of = tid / TEAM;
         const float me = bests[of];
         int ahead = 0;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     float bound = lowered(shared_best);
     choose(bound);
     __syncthreads();
-    if (n_chosen > 2 * a.take + 32) {  // a few beams have all that is best, and so do few of the eights
+    if (n_chosen > 2 * a.take + 32) {  // a few beams have all that is best, and so do few of the teams
         bound = lowered(reached_by_take(mine));
         if (tid == 0) n_chosen = 0;
         __syncthreads();
