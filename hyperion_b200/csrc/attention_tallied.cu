@@ -105,9 +105,9 @@ __device__ __forceinline__ int tile_at(int key, int cc) { return (cc >> 3) * (BN
 template <int NQ, int SETS>  // eights of rows that four warps have; sets of four warps, each with rows of its own; one more warp fetches
 struct Shape {
     static constexpr int ROWS = 8 * NQ, THREADS = 32 * (WARPS * SETS + 1);
-    static_assert(SETS == 1 || (NQ == 1 && SETS == 3), "what registers hold");
+    static_assert(SETS == 1 || (NQ == 1 && SETS == 3 && D == 128), "what registers hold");
     static constexpr int BLOCKS = SETS > 1 ? 1 : NQ == 1 ? 3 : 2;  // an SM, by registers
-    static constexpr int STAGES = SETS > 1 ? (D == 128 ? 6 : 12) : (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
+    static constexpr int STAGES = SETS > 1 ? 6 : (D == 128 ? 2 : 4) + (NQ == 1 ? 0 : 1);  // BLOCKS blocks share an SM's memory
     // Where the warps' results meet: COLS entries of every row at a time, a row's LINE floats apart (lanes that store side by side then take different banks).
     static constexpr int COLS = 64 / NQ, LINE = COLS + 4;
     static constexpr int JOIN = WARPS * ROWS * LINE * 4;  // a set
@@ -801,6 +801,13 @@ int launch_strips(const Args& a, const CUtensorMap& map, cudaStream_t stream) {
     if (const cudaError_t error = allow_shared((const void*)kernel, S::SMEM, allowed)) return (int)error;
     return launch_after_previous(kernel, dim3(a.blocks, a.kv_heads * a.chunks), dim3(S::THREADS), S::SMEM, stream, map, a);
 }
+template <int DIM>
+int launch_first(int heads, int sets, const Args& a, const CUtensorMap& map, cudaStream_t stream) {
+    if constexpr (DIM == 128) {
+        if (sets == 3) return launch_strips<1, 3>(a, map, stream);
+    }
+    return heads <= 8 ? launch_strips<1, 1>(a, map, stream) : launch_strips<2, 1>(a, map, stream);
+}
 }  // namespace
 
 // Whether the second kernel has a block for each head.
@@ -828,7 +835,7 @@ static Strips strips_for(int group) {
     if (group <= 16) return {group, 1, 1, Shape<2, 1>::BLOCKS};
     // Three sets read keys and values once where two strips of 16 read them twice (us, 24 heads over 1: of 128, 11 requests at 23,692 slots 40.2 / 47.0, 64 of them 184 / 224, one at 512 9.9 / 9.3; of 64, where they are half as
     // many bytes for as many instructions, 11 30.6 / 30.6 and 64 141 / 136).  Two sets of 16 rows for 32 heads gain nothing: 51.2 / 51.4.  Rows of 24 or 32 in a warp's registers do not fit: 56 and 70.
-    if (group <= 24 && D == 128) return {(group + 2) / 3, 3, 1, Shape<1, 3>::BLOCKS};
+    if (group <= 24 && D == 128) return {(group + 2) / 3, 3, 1, 1};
     return {16, 1, (group + 15) / 16, Shape<2, 1>::BLOCKS};
 }
 // Blocks of the first kernel that stand side by side for a key/value head's strip: what the device holds, but no more than there can be tiles.
@@ -875,7 +882,7 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
                  heads, kv_heads, page_size, pages, strips.heads, strips.chunks, blocks, join_blocks, by_head, together, kept, scale * 1.4426950408889634f, status};
     CUtensorMap map;
     if (int code = cache_map(&map, cache, a)) return code;
-    if (int code = strips.sets == 3 ? launch_strips<1, 3>(a, map, stream) : strips.heads <= 8 ? launch_strips<1, 1>(a, map, stream) : launch_strips<2, 1>(a, map, stream)) return code;
+    if (int code = launch_first<D>(strips.heads, strips.sets, a, map, stream)) return code;
     if (together) return 0;
     return launch_after_previous(tally_kernel, dim3((longest + SPAN - 1) / SPAN + join_blocks, kv_heads, requests), dim3(ADD_THREADS), 0, stream, a);
 }
