@@ -15,7 +15,7 @@
 //
 // Where few rows would leave the device empty, the first walk's slots are cut, and its blocks leave (m, l) of every row and cut, which a small kernel puts together.  (By clusters of up to 16 cuts two requests' 8 queries of
 // 1,000 slots take 11.0 us in place of 11.8, but 32 of 8,192 20.0 in place of 18.4 and 8 of 60,000 82 in place of 61.)  In the second walk a cluster's blocks share the tiles of Q that see a tile of slots, and read one
-// another's sums in shared memory.  Nothing is added by atomics, so results do not depend on which block came first.
+// another's sums in shared memory; where a request's rows are one tile, that stays, and the tiles of slots pass.  Nothing is added by atomics, so results do not depend on which block came first.
 //
 // Measured: three prompts of up to 2,047 tokens, 32 heads over 8 of 128, 123 us (both walks' products 0.6 PFLOP/s), of which either walk takes some 60.  In the loop a tile of 128 x 128 takes an SM
 // 950 to 1,150 clocks: 576 of them are its products, 730 its exponentials on the special function unit (11 of 16 pairs), some 700 its instructions; blocks of two halves with a buffer each do not quite keep them all
@@ -250,14 +250,16 @@ __device__ __forceinline__ uint4 beside_row(float m, float l, float c) {
 }
 __device__ __forceinline__ int first_tile(const Args& a, int slot, int before) { return max(0, slot - before) / a.per_tile; }  // token slot - before is the first that sees the slot
 
-// One walk.  KEYS_STAY: block (span of the tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (tile of Q and key/value head, cut, request), tiles of K pass.
-template <bool KEYS_STAY>
+// One walk, the first or the second (SECOND).  KEYS_STAY: block (span of the tiles of Q within tile of slots, key/value head, request), tiles of Q pass; else block (tile of Q and key/value head, cut, request), tiles of K pass.
+// The second walk has the slots as the product's lanes either way: where a request's rows are one tile, that tile may stay and the slots pass.
+template <bool KEYS_STAY, bool SECOND>
 __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap rows_map, const Args a) {
     extern __shared__ unsigned char smem_raw[];
+    static_assert(SECOND || !KEYS_STAY, "rows stay in the first walk");
     unsigned char* stays = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* ring = stays + TILE;
-    unsigned char* beside_stays = ring + STAGES * TILE;              // KEYS_STAY
-    unsigned char* beside = beside_stays + BESIDE;                   // KEYS_STAY: [STAGES]
+    unsigned char* beside_stays = ring + STAGES * TILE;              // SECOND
+    unsigned char* beside = beside_stays + BESIDE;                   // SECOND: [STAGES], or one for all slots' tiles
     float* theirs = reinterpret_cast<float*>(beside + STAGES * BESIDE);  // [2][BM]: what one half of the warps tells the other
     unsigned long long* full = reinterpret_cast<unsigned long long*>(theirs + 2 * BM);
     unsigned long long* empty = full + STAGES;
@@ -268,6 +270,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(all_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+    constexpr bool SLOTS_PASS = SECOND && !KEYS_STAY;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, request = blockIdx.z;
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -277,11 +280,11 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kv_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
-        if (KEYS_STAY) asm volatile("prefetch.tensormap [%0];" ::"l"(&rows_map) : "memory");
+        if (SECOND) asm volatile("prefetch.tensormap [%0];" ::"l"(&rows_map) : "memory");
     }
     if (!KEYS_STAY) wait_for_previous_kernels();
     const int kvh = KEYS_STAY ? blockIdx.y : blockIdx.x % a.kv_heads, group = a.group;
-    const Request r = request_of(a, request, !KEYS_STAY && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
+    const Request r = request_of(a, request, !SECOND && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
     const int before = r.length - r.tokens;  // token i sees before + i + 1 slots
     const int q_tiles = (r.tokens + a.per_tile - 1) / a.per_tile;
     const int base = KEYS_STAY ? blockIdx.x / a.spans * BM : (int)(gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads) * a.per_tile;  // the first slot, or the first token, that stays
@@ -309,13 +312,14 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         const int chunk = e & 7, row = q_rows + (e >> 3) % (BM - q_rows), panel = (e >> 3) / (BM - q_rows);
         reinterpret_cast<uint4*>((KEYS_STAY ? ring : stays) + panel * PANEL + row * 128)[chunk] = make_uint4(0, 0, 0, 0);
     }
-    if (KEYS_STAY) {
-        for (int e = tid; e < 2 * BM * (1 + STAGES); e += THREADS) {
-            const int row = e % BM, second = e / BM & 1, tile = e / (2 * BM);  // of the tiles, the first stays
+    if (SECOND) {
+        for (int e = tid; e < 2 * BM * (KEYS_STAY ? 1 + STAGES : 2); e += THREADS) {
+            const int row = e % BM, second = e / BM & 1, tile = e / (2 * BM);  // the first tile is what stays
+            const bool slots = KEYS_STAY == (tile == 0);
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (!second && tile == 0) x = make_uint4(0x3f803f80u, 0x3f80u, 0, 0);  // 1 1 1 0 ...
-            if (!second && tile && row >= q_rows) x.x = 0xff7fu;                    // the lowest number: a row that is none gives nothing
-            if (second || !tile || row >= q_rows) reinterpret_cast<uint4*>(beside_stays)[e] = x;
+            if (!second && slots) x = make_uint4(0x3f803f80u, 0x3f80u, 0, 0);  // 1 1 1 0 ...
+            if (!second && !slots && row >= q_rows) x.x = 0xff7fu;                // the lowest number: a row that is none gives nothing
+            if (second || slots || row >= q_rows) reinterpret_cast<uint4*>(beside_stays)[e] = x;
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -360,9 +364,9 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
         // ------------------------------------------------------------------ the whole warp
         auto fetch_queries = [&](unsigned char* tile, int token, unsigned long long* bar) {  // tokens beyond the request's own come along, or are filled with zeros
             if (lane == 0) {
-                mbar_expect_tx(bar, (unsigned)((PANELS * 128 + (KEYS_STAY ? 16 : 0)) * q_rows));
+                mbar_expect_tx(bar, (unsigned)((PANELS * 128 + (SECOND ? 16 : 0)) * q_rows));
                 for (int h = 0; h < PANELS; ++h) tma_load_3d(tile + h * PANEL, &q_map, bar, h * 64, kvh * group, r.first + token);
-                if (KEYS_STAY) tma_load_3d(beside + (tile - ring) / TILE * BESIDE, &rows_map, bar, 0, kvh * group, r.first + token);
+                if (SECOND) tma_load_3d(KEYS_STAY ? beside + (tile - ring) / TILE * BESIDE : beside_stays, &rows_map, bar, 0, kvh * group, r.first + token);
             }
         };
         int sent = 0;
@@ -398,8 +402,9 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             if (elected()) {
                 const unsigned b_low = b_low0 + (unsigned)s * (TILE >> 4);
 #pragma unroll
-                for (int h = 0; h < PANELS; ++h) umma_s_panel(tmem + b * BM, a_low + h * (PANEL >> 4), b_low + h * (PANEL >> 4), IDESC, h ? 1u : 0u);
-                if (KEYS_STAY) umma_beside(tmem + b * BM, beside_low(beside_stays), beside_low(beside) + (unsigned)s * (BESIDE >> 4), IDESC);
+                for (int h = 0; h < PANELS; ++h) umma_s_panel(tmem + b * BM, (SLOTS_PASS ? b_low : a_low) + h * (PANEL >> 4), (SLOTS_PASS ? a_low : b_low) + h * (PANEL >> 4), IDESC, h ? 1u : 0u);
+                if (SLOTS_PASS) umma_beside(tmem + b * BM, beside_low(beside), beside_low(beside_stays), IDESC);
+                else if (KEYS_STAY) umma_beside(tmem + b * BM, beside_low(beside_stays), beside_low(beside) + (unsigned)s * (BESIDE >> 4), IDESC);
                 umma_commit_at(smem_u32(&empty[s]));
                 umma_commit_at(smem_u32(&s_full[b]));
             }
@@ -427,14 +432,44 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
                 break;
             }
             tc_fence_after();
+            const int slot0 = KEYS_STAY ? base : (from + i) * BM, token0 = KEYS_STAY ? (from + i) * a.per_tile : base;
+            // SECOND: the first row that sees this slot, and the rows that are the request's; whether all rows see all slots
+            [[maybe_unused]] const int from_row = max(0, slot0 + mine - before - token0) * group, rows = min((r.tokens - token0) * group, q_rows);
+            const bool all = SECOND ? slot0 + BM - 1 - before <= token0 && r.tokens - token0 >= a.per_tile : slot0 + BM <= all_see;
+            Pair part[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            if constexpr (SLOTS_PASS) {  // rows are few: of the product's columns those that are rows are looked at, 32 at a time
+                float* weight = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + slot0 + mine;
+                const float old = slot0 + mine < r.length ? *weight : 0.f;
+                const int chunks = (rows + 31) / 32;
+#pragma unroll 1
+                for (int k = 0; k < chunks; ++k) {
+                    unsigned v[32];
+                    tmem_ld32(lanes + 32 * k, v);
+                    arrived(v);
+                    if (k + 1 == chunks) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&s_empty[half]);
+                    }
+                    if (!all) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const Pair y = fma2(Pair{__uint_as_float(v[j + 2 * e]), __uint_as_float(v[j + 2 * e + 1])}, Pair{c, c}, Pair{0.f, 0.f});
+                            part[e] = add2(part[e], Pair{fast_exp2(y.x), fast_exp2(y.y)});
+                        }
+                }
+                if (slot0 + mine < r.length) *weight = old + ((part[0].x + part[0].y) + (part[1].x + part[1].y));
+                continue;
+            }
             unsigned raw[2][32];
             tmem_ld32(lanes, raw[0]);
             arrived(raw[0]);
-            const int slot0 = (from + i) * BM, token0 = (from + i) * a.per_tile;
-            // KEYS_STAY: the first row that sees this slot, and the rows that are the request's; whether all rows see all slots
-            [[maybe_unused]] const int from_row = (base + mine - before - token0) * group, rows = min((r.tokens - token0) * group, q_rows);
-            const bool all = KEYS_STAY ? base + BM - 1 - before <= token0 && r.tokens - token0 >= a.per_tile : slot0 + BM <= all_see;
-            Pair part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 unsigned (&v)[32] = raw[k & 1];
@@ -490,20 +525,22 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
                 rest = (t - sum) - y, sum = t;
             }
         }
-        // the second half's sums come to the first
-        if (half == 1) theirs[mine] = KEYS_STAY ? sum : m, theirs[BM + mine] = KEYS_STAY ? rest : l;
-        asm volatile("bar.sync 3, %0;" ::"n"(64 * HALF) : "memory");
-        if (half == 0 && ok) {
-            if constexpr (KEYS_STAY) {
-                sum += theirs[mine] - (rest + theirs[BM + mine]);
-                if (a.spans > 1) theirs[mine] = sum;
-                else if (base + mine < r.length) a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + base + mine] += sum;
-            } else if (mine < q_rows && token < r.tokens) {
-                const float other = theirs[mine], above = fmaxf(m, other);
-                l = (m == -INFINITY ? l : l * fast_exp2(m - above)) + (other == -INFINITY ? theirs[BM + mine] : theirs[BM + mine] * fast_exp2(other - above));
-                const size_t at = (size_t)(r.first + token) * a.heads + my_head;
-                if (a.n_cuts == 1) a.rows[at] = beside_row(above, l, c);
-                else a.cuts[(size_t)blockIdx.y * a.tokens * a.heads + at] = make_float2(above, l);
+        if constexpr (!SLOTS_PASS) {
+            // the second half's sums come to the first
+            if (half == 1) theirs[mine] = KEYS_STAY ? sum : m, theirs[BM + mine] = KEYS_STAY ? rest : l;
+            asm volatile("bar.sync 3, %0;" ::"n"(64 * HALF) : "memory");
+            if (half == 0 && ok) {
+                if constexpr (KEYS_STAY) {
+                    sum += theirs[mine] - (rest + theirs[BM + mine]);
+                    if (a.spans > 1) theirs[mine] = sum;
+                    else if (base + mine < r.length) a.weights[((size_t)request * a.kv_heads + kvh) * a.capacity + base + mine] += sum;
+                } else if (mine < q_rows && token < r.tokens) {
+                    const float other = theirs[mine], above = fmaxf(m, other);
+                    l = (m == -INFINITY ? l : l * fast_exp2(m - above)) + (other == -INFINITY ? theirs[BM + mine] : theirs[BM + mine] * fast_exp2(other - above));
+                    const size_t at = (size_t)(r.first + token) * a.heads + my_head;
+                    if (a.n_cuts == 1) a.rows[at] = beside_row(above, l, c);
+                    else a.cuts[(size_t)blockIdx.y * a.tokens * a.heads + at] = make_float2(above, l);
+                }
             }
         }
     }
@@ -571,13 +608,13 @@ int encoded(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : HB_BAD_ARGUMENT;
 }
-template <bool KEYS_STAY>
+template <bool KEYS_STAY, bool SECOND>
 int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUtensorMap& rows_map, const Args& a, dim3 grid, int together, cudaStream_t stream) {  // blocks of a cluster, along x
     static std::atomic<unsigned long long> allowed{0};
-    if (const cudaError_t error = allow_shared((const void*)tally_walk_kernel<KEYS_STAY>, SMEM_BYTES, allowed)) return (int)error;
+    if (const cudaError_t error = allow_shared((const void*)tally_walk_kernel<KEYS_STAY, SECOND>, SMEM_BYTES, allowed)) return (int)error;
     static std::atomic<unsigned long long> wide{0};
     if (together > 8)
-        if (const cudaError_t error = allow_wide_clusters((const void*)tally_walk_kernel<KEYS_STAY>, wide)) return (int)error;
+        if (const cudaError_t error = allow_wide_clusters((const void*)tally_walk_kernel<KEYS_STAY, SECOND>, wide)) return (int)error;
     cudaLaunchConfig_t config = {};
     config.gridDim = grid, config.blockDim = dim3(THREADS), config.dynamicSmemBytes = SMEM_BYTES, config.stream = stream;
     cudaLaunchAttribute attributes[2];
@@ -586,7 +623,7 @@ int launch_walk(const CUtensorMap& kv_map, const CUtensorMap& q_map, const CUten
     attributes[1].id = cudaLaunchAttributeClusterDimension;
     attributes[1].val.clusterDim = {(unsigned)together, 1, 1};
     config.attrs = attributes, config.numAttrs = together > 1 ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&config, tally_walk_kernel<KEYS_STAY>, kv_map, q_map, rows_map, a);
+    return (int)cudaLaunchKernelEx(&config, tally_walk_kernel<KEYS_STAY, SECOND>, kv_map, q_map, rows_map, a);
 }
 }  // namespace
 
@@ -651,7 +688,7 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
     float2* cut_sums = (float2*)(rows + (size_t)tokens * heads);
     const Args a{block_table, table_width, starts, lengths, tokens, most, longest, weights, capacity, rows, cut_sums, cuts, spans, heads, kv_heads, group, __builtin_ctz(page_size), pages, per_tile,
                  scale * 1.4426950408889634f, status};
-    if (int code = launch_walk<false>(kv_map, q_map, rows_map, a, dim3((unsigned)row_blocks, cuts, requests), 1, stream)) return code;
+    if (int code = launch_walk<false, false>(kv_map, q_map, rows_map, a, dim3((unsigned)row_blocks, cuts, requests), 1, stream)) return code;
     if (cuts > 1) {
         int lanes = 2;
         while (lanes < 32 && lanes < cuts) lanes *= 2;
@@ -659,6 +696,10 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
         if (threads > 0x7fffffffLL - 256) return HB_UNSUPPORTED_SIZE;
         if (int code = launch_after_previous(tally_cuts_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, lanes)) return code;
     }
-    return launch_walk<true>(kv_map, q_map, rows_map, a, dim3(slot_tiles * spans, kv_heads, requests), spans, stream);
+    // Where a request's rows are one tile, a block of the second walk goes on from tile of slots to tile of slots, if there are more of those than SMs (us, by a block each / so: three queries of 16,384 slots, 14 heads over 2 of 64,
+    // 256 tiles, 14.3 / 12.2, 28 over 4 of 128, 512 tiles, 22.9 / 17.0, 16 over 16 of 64, 2,048 tiles, 55.6 / 25.4; five of 60,000, 32 over 8, 3,752 tiles, 103 / 52; eight requests' five of 300, 28 over 4, 96 tiles, 11.6 /
+    // 13.2).  More tiles of rows one after the other gain nothing up to some 700 tiles of slots.
+    if (row_blocks == kv_heads && (long long)slot_tiles * kv_heads * requests > sms) return launch_walk<false, true>(kv_map, q_map, rows_map, a, dim3(kv_heads, cuts, requests), 1, stream);
+    return launch_walk<true, true>(kv_map, q_map, rows_map, a, dim3(slot_tiles * spans, kv_heads, requests), spans, stream);
 }
 HB_EXPORT int hb_tally_queries_packed(const void* arguments) { return call_packed(&hb_tally_queries, arguments); }

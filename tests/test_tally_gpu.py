@@ -225,6 +225,25 @@ def test_queries(heads, kv, dim, page, counts, lengths):
             assert torch.equal(tally.weights[r, :, n:], before[r, :, n:])
 
 
+@pytest.mark.parametrize("heads,kv,dim,page", [(14, 2, 64, 16), (28, 4, 128, 16), (16, 16, 64, 8), (32, 8, 128, 32), (24, 1, 128, 64)])
+def test_a_few_queries_of_long_contexts(heads, kv, dim, page):
+    """Rows of one tile, beside which tiles of slots pass; weights that slots have already are added to."""
+    counts, lengths = [3, 0, 1, 5, 2, 4], [2900, 700, 1, 1537, 1, 128 * (9 if kv > 1 else 60)]
+    counts[4] = 1
+    cache, table, random = pages_of(lengths, kv, dim, page, seed=heads)
+    q, tally = queries(random, sum(counts), heads * dim, 8), new_tally(len(lengths), kv, table.shape[1] * page)
+    tally.weights.copy_(torch.rand(tally.weights.shape, generator=random))
+    before = tally.weights.clone()
+    starts = torch.tensor([sum(counts[:i]) for i in range(len(counts) + 1)], dtype=torch.int32, device="cuda")
+    tally_queries(q, heads, cache, table, starts, torch.tensor(lengths, dtype=torch.int32, device="cuda"), tally, dim ** -0.5, most=max(counts))
+    ops.raise_on_status(q.device)
+    for r, want, off, e in attended(q, heads, cache, table, counts, lengths, dim ** -0.5):
+        if e is None:
+            want = want + before[r, :, : lengths[r]].double()
+            close(tally.weights[r, :, : lengths[r]], want, off + want * 2.0 ** -23)
+            assert torch.equal(tally.weights[r, :, lengths[r]:], before[r, :, lengths[r]:])
+
+
 def test_a_query_with_a_nan_spoils_the_slots_that_it_sees_and_no_others():
     cache, table, random = pages_of([300], 2, 64, 16, seed=12)
     q, tally = queries(random, 250, 6 * 64), new_tally(1, 2, 304)

@@ -93,3 +93,26 @@ def test_waits_of_three_sets_that_run_out(limit, monkeypatch):
     for call, right in zip(calls, want):
         assert all(torch.equal(a, b) for a, b in zip(call(), right))
         ops.raise_on_status(right[0].device)
+
+
+@pytest.mark.parametrize("limit", [0, 1])
+def test_waits_of_a_few_queries_of_long_contexts(limit, monkeypatch):
+    call, name = many([4, 3, 0], [9000, 5000, 300]), "hb_tally_queries"
+    want = call()
+    ops.raise_on_status(want[0].device)
+    found = native._entries[name, 64]
+    with monkeypatch.context() as patch:
+        short = getattr(native.library(name[3:], HB_HEAD_DIM=64, HB_WAIT_LIMIT=limit), name)
+        short.argtypes = found.argtypes
+        patch.setitem(native._entries, (name, 64), short)
+        got = call()
+        if limit == 0:
+            with pytest.raises(ops.KernelError, match="bounded wait"):
+                ops.raise_on_status(got[0].device)
+        else:
+            try:
+                ops.raise_on_status(got[0].device)
+            except ops.KernelError:
+                pass
+    assert torch.equal(call()[0], want[0])
+    ops.raise_on_status(want[0].device)
