@@ -318,7 +318,6 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             const bool slots = KEYS_STAY == (tile == 0);
             uint4 x = make_uint4(0, 0, 0, 0);
             if (!second && slots) x = make_uint4(0x3f803f80u, 0x3f80u, 0, 0);  // 1 1 1 0 ...
-            if (!second && !slots && row >= q_rows) x.x = 0xff7fu;                // the lowest number: a row that is none gives nothing
             if (second || slots || row >= q_rows) reinterpret_cast<uint4*>(beside_stays)[e] = x;
         }
     }
@@ -455,6 +454,10 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;
+                    } else if (32 * k + 32 > q_rows) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * k + j >= q_rows) v[j] = 0xff800000u;
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
@@ -480,6 +483,10 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;  // a row that does not see this slot gives it nothing, whatever the row is
+                    } else if (k >= 2 && 32 * k + 32 > q_rows) {  // nor does one that is none, whose zeros a key's infinity has made a NaN of (more than half of a tile's rows are rows)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * k + j >= q_rows) v[j] = 0xff800000u;
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)

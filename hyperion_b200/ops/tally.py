@@ -101,8 +101,8 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     r's pages, the last of which is the new token's own.  ``cache``: dense bfloat16 [pages, 2, kv_heads, page, d]; ``block_table`` [requests, blocks] int32; ``scale`` above 0.  Returns [requests, heads * d].
 
     What the token gives each slot, summed over the query heads of a key/value head, is added to ``tally`` [requests, kv_heads, capacity]; its own slot enters the tally with what it gives itself and
-    with the position ``newest[r]`` (int32).  A request of length 0 comes out as zeros and leaves its tally as it is.  A NaN or an infinity among the scores of a head makes that head's result and its key/value
-    head's weights NaN.
+    with the position ``newest[r]`` (int32).  A request of length 0 comes out as zeros and leaves its tally as it is.  A score of -infinity gives its slot nothing (where all of a head's are, its
+    result is zeros); a NaN or +infinity among the scores of a head makes that head's result and its key/value head's weights NaN.
 
     ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that long and is reported (``raise_on_status``).  Work is cut by the lengths as they are on the device, so
     a captured call goes on with other lengths.  Slots beyond a length may hold anything.
@@ -143,8 +143,8 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     on 16-byte boundaries), of which request r has the rows ``starts[r]`` to ``starts[r + 1] - 1`` (int32 [requests + 1]), a whole prompt or the last tokens of one.  They stand in the last of its
     ``lengths[r]`` (int32) slots: query i of n sees the first ``lengths[r] - n + i + 1``, and one with nothing to see gives nothing.  Positions are not touched.
 
-    ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  What is beyond them is left out and reported (``raise_on_status``).  A NaN or an
-    infinity among the scores that a query sees makes the weights of those slots NaN.
+    ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  What is beyond them is left out and reported (``raise_on_status``).  A score of
+    -infinity gives its slot nothing; a NaN or +infinity among the scores that a query sees makes the weights of those slots NaN.
 
     A call's scratch memory is 16 * heads bytes per query, and 8 * heads more for each of the cuts into which slots go where few queries look at many (two blocks a multiprocessor in all): up to 16 MB are kept
     per thread and stream, more is allocated for the call."""
