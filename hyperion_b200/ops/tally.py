@@ -143,8 +143,9 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
     on 16-byte boundaries), of which request r has the rows ``starts[r]`` to ``starts[r + 1] - 1`` (int32 [requests + 1]), a whole prompt or the last tokens of one.  They stand in the last of its
     ``lengths[r]`` (int32) slots: query i of n sees the first ``lengths[r] - n + i + 1``, and one with nothing to see gives nothing.  Positions are not touched.
 
-    ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  What is beyond them is left out and reported (``raise_on_status``).  A score of
-    -infinity gives its slot nothing; a NaN or +infinity among the scores that a query sees makes the weights of those slots NaN.
+    ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  Queries from ``most`` on, slots from ``longest`` on, and rows that ``q`` does not have are left out
+    and reported (``raise_on_status``); the queries that remain see what they would see without the bounds, up to ``longest``.  A score of -infinity gives its slot nothing; a NaN or +infinity among the scores that a
+    query sees makes the weights of those slots NaN.
 
     A call's scratch memory is 16 * heads bytes per query, and 8 * heads more for each of the cuts into which slots go where few queries look at many (two blocks a multiprocessor in all): up to 16 MB are kept
     per thread and stream, more is allocated for the call."""
