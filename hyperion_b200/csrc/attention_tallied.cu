@@ -859,7 +859,7 @@ HB_EXPORT int hb_attention_tallied(const void* q, long long q_stride, void* out,
                                    int* status, cudaStream_t stream) {
     if (requests <= 0) return 0;
     if (!q || !out || !cache || !block_table || !lengths || !weights || !positions || !newest || !status) return HB_BAD_ARGUMENT;
-    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || capacity < longest || sms <= 0 || sms > 16384 || q_stride % 8 || out_stride % 4 || !(scale > 0.f)) return HB_BAD_ARGUMENT;
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || capacity < longest || sms <= 0 || sms > 16384 || q_stride % 8 || out_stride % 4 || !(scale > 0.f && scale <= 0x1p127f)) return HB_BAD_ARGUMENT;
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1))) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) return HB_BAD_ARGUMENT;
     if ((long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;

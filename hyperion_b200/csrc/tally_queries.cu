@@ -673,7 +673,7 @@ HB_EXPORT int hb_tally_queries(const void* q, long long q_stride, int tokens, co
                                int longest, float* weights, int capacity, int heads, int kv_heads, int page_size, int pages, float scale, int sms, void* scratch, int* status, cudaStream_t stream) {
     if (requests <= 0 || tokens <= 0) return 0;
     if (!q || !cache || !block_table || !starts || !lengths || !weights || !scratch || !status) return HB_BAD_ARGUMENT;
-    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || most <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || !(scale >= 0x1p-100f)) return HB_BAD_ARGUMENT;
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || pages <= 0 || table_width <= 0 || longest <= 0 || most <= 0 || capacity < longest || sms <= 0 || q_stride % 8 || !(scale >= 0x1p-100f && scale <= 0x1p127f)) return HB_BAD_ARGUMENT;
     if (page_size < 8 || page_size > 64 || (page_size & (page_size - 1)) || heads / kv_heads > BM) return HB_UNSUPPORTED_SIZE;
     if ((((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)scratch & 15) || (long long)table_width * page_size < longest) return HB_BAD_ARGUMENT;
     const int group = heads / kv_heads, per_tile = BM / group;

@@ -16,7 +16,7 @@ from .native import KernelError, check, entry, scratch, sm_count, stream_address
 
 
 LARGEST = 2 ** 31 - 1
-LEAST_SCALE = 2.0 ** -100
+LEAST_SCALE, MOST_SCALE = 2.0 ** -100, 2.0 ** 127  # times log2(e) it is a float still
 
 
 class Tally(NamedTuple):
@@ -90,15 +90,15 @@ def _check_pages(what: str, cache: torch.Tensor, heads: int, q: torch.Tensor, sc
     queries = q.shape
     if q.dtype is not torch.bfloat16 or len(queries) != 2 or queries[1] < heads * head_dim or q.stride(1) != 1:
         raise KernelError(f"{what}: bfloat16 queries [tokens, {heads * head_dim}] with unit inner stride")
-    if not scale >= LEAST_SCALE:
-        raise KernelError(f"{what}: a scale above 0, not {scale}")
+    if not LEAST_SCALE <= scale <= MOST_SCALE:
+        raise KernelError(f"{what}: a finite scale above 0, not {scale}")
     return shape
 
 
 def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, newest: torch.Tensor, tally: Tally, scale: float, *,
                       longest: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per request: ``q`` [requests, >= heads * d] (bfloat16, a view of wider rows is fine, rows on 16-byte boundaries) over the ``lengths[r]`` (int32) slots of request
-    r's pages, the last of which is the new token's own.  ``cache``: dense bfloat16 [pages, 2, kv_heads, page, d]; ``block_table`` [requests, blocks] int32; ``scale`` above 0.  Returns [requests, heads * d].
+    r's pages, the last of which is the new token's own.  ``cache``: dense bfloat16 [pages, 2, kv_heads, page, d]; ``block_table`` [requests, blocks] int32; ``scale`` from 2^-100 to 2^127.  Returns [requests, heads * d].
 
     What the token gives each slot, summed over the query heads of a key/value head, is added to ``tally`` [requests, kv_heads, capacity]; its own slot enters the tally with what it gives itself and
     with the position ``newest[r]`` (int32).  A request of length 0 comes out as zeros and leaves its tally as it is.  A score of -infinity gives its slot nothing (where all of a head's are, its
