@@ -98,7 +98,8 @@ def _check_pages(what: str, cache: torch.Tensor, heads: int, q: torch.Tensor, sc
 def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, newest: torch.Tensor, tally: Tally, scale: float, *,
                       longest: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per request: ``q`` [requests, >= heads * d] (bfloat16, a view of wider rows is fine, rows on 16-byte boundaries) over the ``lengths[r]`` (int32) slots of request
-    r's pages, the last of which is the new token's own.  ``cache``: dense bfloat16 [pages, 2, kv_heads, page, d]; ``block_table`` [requests, blocks] int32; ``scale`` from 2^-100 to 2^127.  Returns [requests, heads * d].
+    r's pages, the last of which is the new token's own.  ``cache``: dense bfloat16 [pages, 2, kv_heads, page, d]; ``block_table`` [requests, blocks] int32; ``scale`` from 2^-100 to 2^127.  Returns [requests, heads * d], or
+    ``out``, a view [requests, >= heads * d] whose rows do not overlap, on 8-byte boundaries.
 
     What the token gives each slot, summed over the query heads of a key/value head, is added to ``tally`` [requests, kv_heads, capacity]; its own slot enters the tally with what it gives itself and
     with the position ``newest[r]`` (int32).  A request of length 0 comes out as zeros and leaves its tally as it is.  A score of -infinity gives its slot nothing (where all of a head's are, its
@@ -117,12 +118,12 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
     _check_vector(what, "newest", newest, requests)
+    if out is not None and (out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != requests or out.shape[1] < width or out.stride(1) != 1 or (requests > 1 and out.stride(0) < width)):
+        raise KernelError(f"{what}: the output is a bfloat16 [{requests}, >= {width}] view with unit inner stride, of rows that do not overlap")
     _check_device(what, q, cache, block_table, lengths, newest, weights, positions, q if out is None else out)
     device = q.device
     if out is None:
         out = q.new_empty(requests, width)
-    elif out.dtype is not torch.bfloat16 or out.dim() != 2 or out.shape[0] != requests or out.shape[1] < width or out.stride(1) != 1:
-        raise KernelError(f"{what}: the output is a bfloat16 [{requests}, >= {width}] view")
     if requests == 0:
         return out
     if longest == 0:

@@ -2,10 +2,24 @@
 from __future__ import annotations
 
 import pytest
-from test_beams_and_tally_refusals import queried, refuses, tallied
+import torch
+from test_beams_and_tally_refusals import bf16, ints, queried, refuses, tallied
+
+from hyperion_b200.ops import Tally
 
 
 @pytest.mark.parametrize("scale,fits", [(float("inf"), False), (1e39, False), (2.0 ** 128, False), (2.0 ** 127, True), (2.0 ** -100, True), (2.0 ** -101, False)])
 def test_scales_beyond_float(scale, fits):
     refuses(tallied(scale=scale), fits)
     refuses(queried(scale=scale), fits)
+
+
+@pytest.mark.parametrize("requests,out,fits", [(2, torch.zeros(1, 256, dtype=bf16).expand(2, 256), False), (2, torch.zeros(600, dtype=bf16).as_strided((2, 256), (252, 1)), False),
+                                               (2, torch.zeros(600, dtype=bf16).as_strided((2, 256), (256, 1)), True), (2, torch.zeros(2, 300, dtype=bf16), True), (1, torch.zeros(1, 256, dtype=bf16).expand(1, 256), True),
+                                               (1, torch.zeros(600, dtype=bf16).as_strided((1, 256), (4, 1)), True)])
+def test_results_whose_rows_overlap(requests, out, fits):
+    """Two requests would write the same place."""
+    change = dict(out=out)
+    if requests == 1:
+        change |= dict(q=torch.zeros(1, 256, dtype=bf16), lengths=ints(1), newest=ints(1), tally=Tally(torch.zeros(1, 2, 48), ints(1, 2, 48)))
+    refuses(tallied(**change), fits)
