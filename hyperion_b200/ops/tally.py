@@ -204,7 +204,8 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     _check_tally(tally, held, what)
     if to is not tally:
         _check_tally(to, held, what)
-        if (to_weights.data_ptr() == weights.data_ptr()) != (to_positions.data_ptr() == positions.data_ptr()):
+        apart = abs(to_weights.data_ptr() - weights.data_ptr()), abs(to_positions.data_ptr() - positions.data_ptr())
+        if apart != (0, 0) and min(apart) < 4 * weights.numel():
             raise KernelError(f"{what}: the new tally takes the place of all of the old one, or of none of it")
     longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)

@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_beams_and_tally_refusals import bf16, ints, queried, refuses, tallied
+from test_beams_and_tally_refusals import bf16, evicted, ints, queried, refuses, tallied
 
 from hyperion_b200.ops import Tally
 
@@ -23,3 +23,16 @@ def test_results_whose_rows_overlap(requests, out, fits):
     if requests == 1:
         change |= dict(q=torch.zeros(1, 256, dtype=bf16), lengths=ints(1), newest=ints(1), tally=Tally(torch.zeros(1, 2, 48), ints(1, 2, 48)))
     refuses(tallied(**change), fits)
+
+
+@pytest.mark.parametrize("shift,fits", [(0, True), (1, False), (48, False), (575, False), (576, True)])
+@pytest.mark.parametrize("which", ["weights", "positions"])
+def test_a_new_tally_that_overlaps_the_old_one(which, shift, fits):
+    """It takes the place of the old one, or stands beside it: what is partly in its place would be written before it is read."""
+    memory, numbers = torch.zeros(2 * 576), ints(2 * 576)
+    old = Tally(memory[:576].view(3, 2, 2, 48), numbers[:576].view(3, 2, 2, 48))
+    new = Tally(memory[shift: shift + 576].view(3, 2, 2, 48), numbers[shift: shift + 576].view(3, 2, 2, 48))
+    if shift:  # the other of the two is beside the old one
+        new = new._replace(**{"positions": ints(3, 2, 2, 48)} if which == "weights" else {"weights": torch.zeros(3, 2, 2, 48)})
+    refuses(evicted(tally=old, out=new), fits)
+    refuses(evicted(tally=new, out=old), fits)
