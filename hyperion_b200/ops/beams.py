@@ -25,7 +25,7 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
 
     States: ``states`` are dense [layers, rows, ...], a beam's record copied whole (recurrent states, tallies); a beam's row is its number, or ``state_rows[beam]`` (int32), no two the same.
 
-    At most 24 tensors, each once.  A parent that is no beam, a row or a page that is not there leaves its beam as it is, and is reported (``raise_on_status``)."""
+    At most 24 tensors, each once, none of which overlap.  A parent that is no beam, a row or a page that is not there leaves its beam as it is, and is reported (``raise_on_status``)."""
     what = "beam_reorder"
     if parents.dtype is not torch.int32 or parents.dim() != 2 or not parents.is_contiguous() or parents.shape[1] > MOST_BEAMS:
         raise KernelError(f"{what}: parents are dense int32 [groups, beams], at most {MOST_BEAMS} beams")
@@ -36,7 +36,7 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
         raise KernelError(f"{what}: at most {MOST_TENSORS} tensors, not {len(caches) + len(states)}")
     if caches and block_table is None or block_table is not None and not caches:
         raise KernelError(f"{what}: a block table and the caches that it points into")
-    words, rows, page_size, width = [], groups * beams, 0, 0
+    words, spans, rows, page_size, width = [], [], groups * beams, 0, 0
     if block_table is not None:
         width = block_table.shape[-1] if block_table.shape else 0
         if block_table.dtype is not torch.int32 or block_table.shape != (rows, width) or width < 1 or not block_table.is_contiguous():
@@ -46,23 +46,32 @@ def beam_reorder(parents: torch.Tensor, lengths: torch.Tensor, block_table: Opti
             shape = cache.shape
             if len(shape) != 5 or shape[1] != pages or shape[3] != page_size or pages < 1 or page_size < 1 or not cache.is_contiguous():
                 raise KernelError(f"{what}: caches are dense [layers, pages, outer, page, inner], all of the same pages and page size")
-            words += (cache.data_ptr(), shape[0], pages, shape[2], page_size, shape[4] * cache.element_size(), 0)
+            at, layers, _, outer, _, inner = cache.data_ptr(), *shape
+            slot = inner * cache.element_size()
+            words += (at, layers, pages, outer, page_size, slot, 0)
+            spans.append((at, at + layers * pages * outer * page_size * slot))
     if state_rows is not None and (state_rows.dtype is not torch.int32 or state_rows.shape != (rows,) or not state_rows.is_contiguous()):
         raise KernelError(f"{what}: state_rows is a dense int32 vector of {rows}")
     for state in states:
         if state.dim() < 2 or state.shape[1] != states[0].shape[1] or not state.is_contiguous() or (state.shape[1] != rows if state_rows is None else state.shape[1] < 1):
             raise KernelError(f"{what}: states are dense [layers, {rows if state_rows is None else 'rows'}, ...]")
         layers, places = state.shape[:2]
-        words += (state.data_ptr(), layers, places, 1, 1, state.numel() // max(1, layers * places) * state.element_size(), 1)
+        at, size = state.data_ptr(), state.numel() * state.element_size()
+        words += (at, layers, places, 1, 1, size // max(1, layers * places), 1)
+        spans.append((at, at + size))
+    if len(spans) > 1:
+        spans.sort()
+        end = 0
+        for start, its_end in spans:
+            if start < end and start < its_end:
+                raise KernelError(f"{what}: a tensor once only, and no two that overlap")
+            end = max(end, its_end)
     tensors = [parents, lengths, *caches, *states]
     if block_table is not None:
         tensors.append(block_table)
     if state_rows is not None:
         tensors.append(state_rows)
     _check_device(what, *tensors)
-    places = [place for place in words[::7] if place]
-    if len(set(places)) != len(places):
-        raise KernelError(f"{what}: a tensor once only")
     if rows == 0 or not words:
         return
     described = (ctypes.c_longlong * len(words))(*words)

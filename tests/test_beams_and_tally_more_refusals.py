@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_beams_and_tally_refusals import bf16, evicted, ints, queried, refuses, tallied
+from test_beams_and_tally_refusals import bf16, evicted, ints, queried, refuses, reordered, tallied
 
 from hyperion_b200.ops import Tally
 
@@ -36,3 +36,12 @@ def test_a_new_tally_that_overlaps_the_old_one(which, shift, fits):
         new = new._replace(**{"positions": ints(3, 2, 2, 48)} if which == "weights" else {"weights": torch.zeros(3, 2, 2, 48)})
     refuses(evicted(tally=old, out=new), fits)
     refuses(evicted(tally=new, out=old), fits)
+
+
+def test_what_beams_hold_comes_once():
+    """Parts of a tensor that is there already would move twice, one move beside the other."""
+    pages, states = torch.zeros(3, 30, 4, 16, 64), torch.zeros(4, 6, 9)
+    for caches, others, fits in (([pages[:2], pages[1:]], [states], False), ([pages[1:], pages[:2]], [], False), ([pages[:1], pages[1:]], [states], True), ([pages], [states[:2], states[2:], states[:1]], False),
+                                 ([pages], [states[:2], states[2:]], True), ([pages], [states[:0], states], True), ([pages], [pages.view(-1)[64: 64 + 6 * 9].view(1, 6, 9)], False),
+                                 ([pages], [states, states.view(torch.uint8)[3:]], False)):
+        refuses(reordered(caches=caches, states=others), fits)
