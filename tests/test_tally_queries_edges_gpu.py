@@ -55,3 +55,18 @@ def test_keys_of_negative_infinity_are_given_nothing(heads, kv, dim, few):
     assert bool((want[:, lost] == 0).all()) and bool((tally.weights[0][:, lost] == 0).all())
     assert not tally.weights.isnan().any()
     close(tally.weights[0, :, :length], want, off)
+
+
+@pytest.mark.parametrize("heads,kv,count,length", [(8, 1, 500, 500), (14, 2, 300, 300), (8, 1, 450, 640), (24, 1, 90, 512)])
+def test_clusters_of_sixteen_blocks(heads, kv, count, length):
+    """Few tiles of slots (of 128) and many of queries (of 128 // group): with less than 0.7 blocks a multiprocessor, sixteen share a tile of slots."""
+    tiles, per_tile = -(-length // 128) * kv, 128 // (heads // kv)
+    assert 16 * tiles <= 0.7 * sm_count() and count > 15 * per_tile
+    cache, table, random = pages_of([length], kv, 64, 16, seed=count)
+    q, tally = queries(random, count, heads * 64), new_tally(1, kv, table.shape[1] * 16)
+    tally_queries(q, heads, cache, table, ints([0, count]), ints([length]), tally, 0.125, most=count)
+    ops.raise_on_status(q.device)
+    keys, _ = records(cache, table, 0, length)
+    want, off = given(q.view(count, heads, 64), keys, [length - count + i + 1 for i in range(count)], 0.125)
+    close(tally.weights[0, :, :length], want, off)
+    assert bool((tally.weights[0, :, length:] == 0).all())
