@@ -19,8 +19,9 @@
 // S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): slots and entries stand where the instruction has 16 rows, the few heads of a key/value head where it has 8 columns.  The weights are taken into the second
 // product in two parts, rounded to bfloat16 and what that left over: rounded once they would cost the result as much as its own rounding does.
 //
-// Measured (28 heads over 4 of 128): 64 requests of up to 8,192 slots 150 us for the 823 MB of keys, values and weights (5.5 TB/s), 16 of up to 4,099 26.2 us for 105 MB (4.1 TB/s).  The first kernel alone streams at 6.2 TB/s and
-// takes 133 and 24 us; writing scores is a tenth of it, the second kernel's exposed part the rest.  One token of 14 heads over 2 of 64 at 512 slots: 5.8 us, a start, three dependent trips to memory and the cluster's meeting.
+// Measured (28 heads over 4 of 128): 64 requests of up to 8,192 slots 150 us for the 823 MB of keys, values and weights (5.5 TB/s), 16 of up to 4,099 26.1 us for 105 MB (4.0 TB/s).  The first kernel alone
+// takes 133 us (6.2 TB/s) and 24 (4.4); writing scores is a tenth of it, the second kernel's exposed part the rest.  For heads of 128 a few of the line's registers do not fit (32 bytes spilled for groups of up to 8 heads, 72 of up to 16,
+// 20 by three sets); what that costs has not been measured apart.  One token of 14 heads over 2 of 64 at 512 slots: 5.8 us, a start, three dependent trips to memory and the cluster's meeting.
 //
 // Slots beyond a request's length may hold anything: their scores are replaced and their values read as zeros.  Every wait is bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the
 // block leaves, once the copies that it has on their way have arrived.

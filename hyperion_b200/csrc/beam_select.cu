@@ -13,7 +13,7 @@
 //
 // Scores are compared as float64: a score is score_b - lse_b, a number of the row, plus the logit, and float32 would make ties of scores that are not equal.  Sums of a thread's 32 entries are float, everything above
 // them float64; exponentials are the hardware's (2^-22 of a term), of differences rounded to float.  A row's sum is off by (2.224 D + 4 R + 31) 2^-24 of itself at most, where D, at most ln vocab, is how far below the maximum its
-// terms lie on average and R how often a thread's maximum rises behind a term: scores of two beams may come in either order where they are closer than that (measured 2^-20.8 for one outlier over equal logits, 2^-23 else).
+// terms lie on average and R how often a thread's maximum rises behind a term: scores of two beams may come in either order where they are closer than two such errors (measured 2^-20.8 for one outlier over equal logits, 2^-23 else).
 // Which thread adds up what goes by the entry's index alone, not by the row's alignment, so rows of a call that hold the same have the same sums.
 //
 // A NaN counts as -infinity, +infinity as the largest number.  A logit of -infinity, and everything of a beam whose score is -infinity or NaN, is no candidate.  A place without a candidate has parent -1,
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(GROUP_THREADS) beam_group_kernel(const Args a)
     let_next_kernel_start();
     wait_for_previous_kernels();
     const float* tops = a.tops + (size_t)group * n;
-    // thread t has the runs t, t + 1024, ... of all beams; its first ones are on their way while the sums are put together
+    // thread t has the runs t, t + GROUP_THREADS, ... of all beams; its first ones are on their way while the sums are put together
     float early[EARLY];
 #pragma unroll
     for (int k = 0; k < EARLY; ++k) early[k] = tid + k * GROUP_THREADS < n ? tops[tid + k * GROUP_THREADS] : -INFINITY;

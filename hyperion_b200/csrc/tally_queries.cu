@@ -196,7 +196,7 @@ __device__ __forceinline__ Pair polynomial_exp2(Pair y) {
     p = fma2(p, f, Pair{1.0000001f, 1.0000001f});
     return mul2(p, Pair{__uint_as_float((__float_as_uint(r.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(r.y) << 23) + 0x3f800000u)});
 }
-// Of 16 pairs so many take the polynomial, spread evenly.  (Three prompts, none / 2 / 4 / 5: 138 / 131 / 128 / 127 us; six spill registers.)
+// Of 16 pairs so many take the polynomial, spread evenly.  (Three prompts, none / 2 / 4 / 5 / 6: 132.3 / 126.0 / 123.3 / 122.9 / 126.5 us.)
 constexpr int POLYNOMIAL = 5;
 __device__ __forceinline__ Pair exp2_of(Pair y, int pair) { return (pair + 1) * POLYNOMIAL / 16 != pair * POLYNOMIAL / 16 ? polynomial_exp2(y) : Pair{fast_exp2(y.x), fast_exp2(y.y)}; }
 
@@ -560,7 +560,8 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     if (warp == ISSUER) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
-    }    if constexpr (KEYS_STAY) {
+    }
+    if constexpr (KEYS_STAY) {
         // The spans' sums of a slot, in their order.  Tensor memory has been given back, so that no block has some while it waits for another.
         if (a.spans > 1) {
             const int rank = blockIdx.x % a.spans, slot = rank + tid * a.spans;  // whose sums this thread adds up

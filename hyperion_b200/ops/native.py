@@ -118,7 +118,7 @@ def entry(module: str, name: str, arguments: str, head_dim: int = 0, result: str
         else:
             found = getattr(loaded, name)
             found.restype = _KINDS[result]
-        found.argtypes = kinds
+        found.argtypes = kinds  # of a packed one, too: those of its launcher
         _entries[name, head_dim] = found
     return found
 

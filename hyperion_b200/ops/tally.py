@@ -105,8 +105,8 @@ def attention_tallied(q: torch.Tensor, heads: int, cache: torch.Tensor, block_ta
     with the position ``newest[r]`` (int32).  A request of length 0 comes out as zeros and leaves its tally as it is.  A score of -infinity gives its slot nothing (where all of a head's are, its
     result is zeros); a NaN or +infinity among the scores of a head makes that head's result and its key/value head's weights NaN.
 
-    ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that long and is reported (``raise_on_status``).  Work is cut by the lengths as they are on the device, so
-    a captured call goes on with other lengths.  Slots beyond a length may hold anything.
+    ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that long and is reported (``raise_on_status``), unless the bound is 0, where lengths are not looked at.  Work is cut by the
+    lengths as they are on the device, so a captured call goes on with other lengths.  Slots beyond a length may hold anything.
 
     A call's scratch memory is 4 * heads bytes per request and slot up to ``longest``, and 4 * heads * (d + 2) per request and block: up to 16 MB are kept per thread and stream, more is allocated for the call."""
     what = "attention_tallied"
@@ -142,10 +142,11 @@ def tally_queries(q: torch.Tensor, heads: int, cache: torch.Tensor, block_table:
                   longest: Optional[int] = None) -> None:
     """Add to ``tally`` [requests, kv_heads, capacity] what queries give the slots that they see, as :func:`attention_tallied` does for a decoded token, without a result: ``q`` [tokens, >= heads * d] (bfloat16, rows
     on 16-byte boundaries), of which request r has the rows ``starts[r]`` to ``starts[r + 1] - 1`` (int32 [requests + 1]), a whole prompt or the last tokens of one.  They stand in the last of its
-    ``lengths[r]`` (int32) slots: query i of n sees the first ``lengths[r] - n + i + 1``, and one with nothing to see gives nothing.  Positions are not touched.
+    ``lengths[r]`` (int32) slots: query i of n sees the first ``lengths[r] - n + i + 1``, and one with nothing to see gives nothing.  All slots are added to, those of the queries' own tokens too, which have weighed nothing
+    before in a new tally; positions are not touched.
 
     ``most``: no request has more queries; ``longest``: no request is longer (what table and tally hold, when absent).  Queries from ``most`` on, slots from ``longest`` on, and rows that ``q`` does not have are left out
-    and reported (``raise_on_status``); the queries that remain see what they would see without the bounds, up to ``longest``.  A score of -infinity gives its slot nothing; a NaN or +infinity among the scores that a
+    and reported (``raise_on_status``); the queries that remain see what they would see without the bounds, up to ``longest``.  Where a bound or the number of rows is 0, nothing is looked at.  A score of -infinity gives its slot nothing; a NaN or +infinity among the scores that a
     query sees makes the weights of those slots NaN.
 
     A call's scratch memory is 16 * heads bytes per query, and 8 * heads more for each of the cuts into which slots go where few queries look at many (two blocks a multiprocessor in all): up to 16 MB are kept
@@ -182,10 +183,10 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
 
     Slots whose positions are below ``first`` or among the last ``recent`` rank as an infinite weight, the others by their weights (a NaN as -infinity); of equal ranks the lowest slots stay.  What stays in slots
     from ``keep`` on moves into those below that are left free, in order: keys and values, weights and positions.  Records from the new length on stay as they were; in the tally the slots that were given up
-    weigh nothing and have position -1.  The new tally goes to ``out`` where it is given, all of it, with slots behind a request like those given up; else in place, where slots behind a request stay as they were.
+    weigh nothing and have position -1.  The new tally goes to ``out`` where it is given (beside the old one), all of it, with slots behind a request like those given up; else in place, where slots behind a request stay as they were.
 
     Pages are written in place, so a request's pages may not be another one's as well (up to its length).  ``longest``: no request is longer (what table and tally hold, when absent); one that is counts as that
-    long and is reported (``raise_on_status``).  A move from or to a page that is not there is left out and reported.
+    long and is reported (``raise_on_status``), unless the bound is 0.  A move from or to a page that is not there is left out and reported.
 
     A call's scratch memory is 8 bytes for each of the min(keep, longest - keep) moves that a head of a layer and request can have."""
     what, shape = "evict", cache.shape

@@ -27,7 +27,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: int) -> BeamCh
     """The ``take`` best continuations of each group's beams (as many as it has beams, or twice that where some may end).  ``logits`` [groups * beams, vocab] float32 or bfloat16 with unit inner stride, a
     row per beam; ``scores`` [groups, beams] float32, what the beams have scored so far.  At most 32 beams, ``take`` at most 64, at most 65,535 rows.
 
-    A beam's own tokens come in the order of their logits.  The sums of beams' probabilities are off by some 2^-18 of themselves at most, so continuations of two beams whose scores are closer than that may come in either order;
+    A beam's own tokens come in the order of their logits.  The sums of beams' probabilities are off by some 2^-18 of themselves at most, so continuations of two beams whose scores are closer than 2^-17 may come in either order;
     beams whose logits and scores are the same go by their numbers.
 
     A logit of -infinity or NaN is no continuation (+infinity counts as the largest number), nor is anything of a beam whose score is -infinity or NaN: a group begins with one beam at 0 and the others at
