@@ -217,6 +217,8 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     device = cache.device
     left = torch.empty_like(lengths)
     if requests == 0 or layers == 0 or kv_heads == 0 or longest == 0:
+        if to_weights.data_ptr() != weights.data_ptr():  # nobody has slots
+            to_weights.zero_(), to_positions.fill_(-1)
         return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
     stream = stream_address()
     memory, owner = scratch(device, stream, _scratch_size("evict", "hb_evict_scratch", 0, layers, requests, kv_heads, longest, keep))
