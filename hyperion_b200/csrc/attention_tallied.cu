@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(Shape<NQ, SETS>::THREADS, (TOGETHER ? (NQ == 1
                 const int s = stage % S::STAGES, round = stage / S::STAGES, base = (tile + it) * BN;
                 if (it % tiles_per_look == 0) {  // a page number per lane, for the next tiles
                     const int block = (base >> shift) + lane;
-                    looked = block < a.table_width ? __ldg(table + block) : -1;
+                    looked = block < a.table_width ? table[block] : -1;
                 }
                 if (lane == 0) ok = mbar_wait(&empty[s], (round & 1) ^ 1, failed) ? 1 : 0;
                 ok = __shfl_sync(0xffffffffu, ok, 0);

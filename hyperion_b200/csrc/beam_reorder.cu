@@ -32,12 +32,14 @@ struct Args {
     int* status;
 };
 
+// What is written in place is read past L1 (ld.global.cg): the next kernel may be on the multiprocessor by now, and a line that another one writes after it was read here would be what that kernel finds in L1, if its loads are not
+// coherent ones, as those of block tables are in places.
 template <typename T, int B>
 __device__ __forceinline__ void move(char* const* rows, const int* parent, int beams, long long byte) {
     T value[B];
 #pragma unroll
     for (int j = 0; j < B; ++j)
-        if (j < beams && parent[j] != j) value[j] = *reinterpret_cast<const T*>(rows[parent[j]] + byte);
+        if (j < beams && parent[j] != j) value[j] = __ldcg(reinterpret_cast<const T*>(rows[parent[j]] + byte));
 #pragma unroll
     for (int j = 0; j < B; ++j)
         if (j < beams && parent[j] != j) *reinterpret_cast<T*>(rows[j] + byte) = value[j];
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(THREADS) beam_reorder_kernel(const __grid_cons
             place = a.slots ? a.slots[beam] : beam;
             if (place < 0 || place >= a.slots_rows) atomicOr(a.status, HB_STATUS_BAD_POSITION), place = -1;
         } else {
-            place = full < a.table_width ? a.block_table[(size_t)beam * a.table_width + full] : -1;
+            place = full < a.table_width ? __ldcg(a.block_table + (size_t)beam * a.table_width + full) : -1;
             if (place < 0 || place >= a.pages) atomicOr(a.status, HB_STATUS_BAD_PAGE), place = -1;
         }
         rows[tid] = place < 0 ? nullptr : job.base + layer * job.layer + place * job.page + outer * job.outer;

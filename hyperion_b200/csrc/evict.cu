@@ -95,7 +95,7 @@ __device__ __forceinline__ int warp_before(int v, int lane) {  // sum over the l
 }
 
 // The records of a head's moves: warp `first` of `step` takes every step-th CHUNK of them.  A lane finds out where one of them goes from and to; then a team of lanes a move carries 16 bytes of its key and value a lane and
-// turn, AHEAD moves of a team on their way together.
+// turn, AHEAD moves of a team on their way together.  Records are read past L1, where a line that also holds a slot that is filled elsewhere must not stay for the kernel behind this one.
 constexpr int CHUNK = 16, AHEAD = 4;
 __device__ __forceinline__ void move_records(const Args& a, const int* from, const int* to, int n_moves, const int* table, int layer, int kvh, int first, int step) {
     const int lane = threadIdx.x & 31, mask = (1 << a.page_shift) - 1;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void move_records(const Args& a, const int* from, con
                 uint4 held[AHEAD];
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k)
-                    if (s[k] >= 0) held[k] = layer_cache[s[k] + at];
+                    if (s[k] >= 0) held[k] = __ldcg(layer_cache + s[k] + at);
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k)
                     if (s[k] >= 0) layer_cache[t[k] + at] = held[k];

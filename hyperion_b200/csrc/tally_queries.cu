@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
     auto page_at = [&](int slot0) {  // this lane's page of the tile of K from slot0 on; -1: none
         const int k0 = slot0 + lane * page_size;
         if (lane >= pages_per_tile || k0 >= r.length) return -1;
-        const int id = __ldg(table + (k0 >> a.page_shift));
+        const int id = table[k0 >> a.page_shift];
         if (id >= 0 && id < a.pages) return id;
         atomicOr(a.status, HB_STATUS_BAD_PAGE);
         return -1;
