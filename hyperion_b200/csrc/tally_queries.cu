@@ -438,6 +438,8 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
             // SECOND: the first row that sees this slot, and the rows that are the request's; whether all rows see all slots
             [[maybe_unused]] const int from_row = max(0, slot0 + mine - before - token0) * group, rows = min((r.tokens - token0) * group, q_rows);
             const bool all = SECOND ? slot0 + BM - 1 - before <= token0 && r.tokens - token0 >= a.per_tile : slot0 + BM <= all_see;
+            // SECOND: a row that does not see this slot gives it nothing, whatever the row is, nor does one that is none, whose zeros a key's infinity has made a NaN of: the first columns, by 32, that need not be asked
+            [[maybe_unused]] const int whole = all ? q_rows / 32 : 0;
             Pair part[2] = {{0.f, 0.f}, {0.f, 0.f}};
             if constexpr (SLOTS_PASS) {  // rows are few: of the product's columns those that are rows are looked at, 32 at a time
                 float* weight = a.weights + ((size_t)request * a.kv_heads + kvh) * a.capacity + slot0 + mine;
@@ -453,14 +455,10 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&s_empty[half]);
                     }
-                    if (!all) {
+                    if (k >= whole) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;
-                    } else if (32 * k + 32 > q_rows) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (32 * k + j >= q_rows) v[j] = 0xff800000u;
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
@@ -482,14 +480,10 @@ __global__ void __launch_bounds__(THREADS, 2) tally_walk_kernel(const __grid_con
                 if (k < 3) tmem_ld32(lanes + 32 * (k + 1), raw[(k + 1) & 1]);
                 auto pair_at = [&](int j) { return Pair{__uint_as_float(v[j]), __uint_as_float(v[j + 1])}; };
                 if constexpr (KEYS_STAY) {
-                    if (!all) {
+                    if (k >= whole) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;  // a row that does not see this slot gives it nothing, whatever the row is
-                    } else if (k >= 2 && 32 * k + 32 > q_rows) {  // nor does one that is none, whose zeros a key's infinity has made a NaN of (more than half of a tile's rows are rows)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (32 * k + j >= q_rows) v[j] = 0xff800000u;
+                            if (32 * k + j < from_row || 32 * k + j >= rows) v[j] = 0xff800000u;
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
