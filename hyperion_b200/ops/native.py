@@ -29,26 +29,30 @@ def ptr(tensor: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(tensor.data_ptr())
 
 
-_bound_stream: list = [None]  # the stream a step has bound for its launches, or None
+class _Bound(threading.local):
+    stream = None  # the one that a step of this thread has bound for its launches
+
+
+_bound = _Bound()
 
 
 def stream_ptr() -> ctypes.c_void_p:
     """The stream launches go to: the one bound by ``stream_bound`` if any, else torch's current stream."""
-    bound = _bound_stream[0]
+    bound = _bound.stream
     return bound if bound is not None else ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
 class stream_bound:
-    """``with stream_bound():`` looks torch's current stream up once; the launches inside use it without asking again.
+    """``with stream_bound():`` looks torch's current stream up once; the launches that this thread makes inside use it without asking again.
     Nesting rebinds (a graph capture inside a step launches on the capture's stream)."""
 
     def __enter__(self):
-        self.previous = _bound_stream[0]
-        _bound_stream[0] = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        self.previous = _bound.stream
+        _bound.stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
         return self
 
     def __exit__(self, *exc):
-        _bound_stream[0] = self.previous
+        _bound.stream = self.previous
         return False
 
 
@@ -140,7 +144,7 @@ def _packed(function, pack, name: str):
 
 def stream_address() -> int:
     """:func:`stream_ptr` as a number, without the objects on the way there."""
-    bound = _bound_stream[0]
+    bound = _bound.stream
     return (bound.value or 0) if bound is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
