@@ -203,11 +203,13 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     capacity = held[-1] if held else 0
     held = (layers, requests, kv_heads, capacity) if layered else (requests, kv_heads, capacity)
     _check_tally(tally, held, what)
+    heavy, where, to_heavy, to_where = weights.data_ptr(), positions.data_ptr(), to_weights.data_ptr(), to_positions.data_ptr()
     if to is not tally:
         _check_tally(to, held, what)
-        apart = abs(to_weights.data_ptr() - weights.data_ptr()), abs(to_positions.data_ptr() - positions.data_ptr())
-        if apart != (0, 0) and min(apart) < 4 * weights.numel():
-            raise KernelError(f"{what}: the new tally takes the place of all of the old one, or of none of it")
+        if to_heavy != heavy or to_where != where:  # then beside it
+            size = 4 * layers * requests * kv_heads * capacity
+            if -size < to_heavy - heavy < size or -size < to_where - where < size:
+                raise KernelError(f"{what}: the new tally takes the place of all of the old one, or of none of it")
     longest = _check_table(what, block_table, requests, page_size, longest, capacity)
     _check_vector(what, "lengths", lengths, requests)
     _check_vector(what, "newest", newest, requests)
@@ -217,12 +219,12 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
     device = cache.device
     left = torch.empty_like(lengths)
     if requests == 0 or layers == 0 or kv_heads == 0 or longest == 0:
-        if to_weights.data_ptr() != weights.data_ptr():  # nobody has slots
+        if to_heavy != heavy:  # nobody has slots
             to_weights.zero_(), to_positions.fill_(-1)
         return left.zero_() if longest == 0 else left.copy_(lengths.clamp(0, min(keep, longest)))
     stream = stream_address()
     memory, owner = scratch(device, stream, _scratch_size("evict", "hb_evict_scratch", 0, layers, requests, kv_heads, longest, keep))
     check(entry("evict", "hb_evict", "piiiiipippiippppiiiipppip", packed=True)(
-        cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, weights.data_ptr(),
-        positions.data_ptr(), to_weights.data_ptr(), to_positions.data_ptr(), capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), sm_count(device), stream), what)
+        cache.data_ptr(), layers, pages, kv_heads, page_size, record, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(), newest.data_ptr(), requests, longest, heavy,
+        where, to_heavy, to_where, capacity, keep, first, recent, left.data_ptr(), memory, status_word(device).data_ptr(), sm_count(device), stream), what)
     return left
