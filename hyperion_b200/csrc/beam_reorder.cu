@@ -5,7 +5,7 @@
 // reads what all of them are to have and writes it only then, so no thread reads what another writes and nothing is kept elsewhere in between.  A parent that several beams have is read from memory
 // once (they follow one another), and a beam that is its own parent is neither read nor written.
 //
-// Bound by memory: 16 groups of 8 beams, 28 layers of part-filled pages and 4 of states, 84.4 us for the 502 MB that distinct parents and changed beams come to (5.9 TB/s, 0.91 of a copy's rate).  One group of four beams 2.6 us.
+// Bound by memory: 16 groups of 8 beams, 28 layers of part-filled pages and 4 of states, 84.9 us for the 502 MB that distinct parents and changed beams come to (5.9 TB/s, 0.90 of a copy's rate).  One group of four beams 2.6 us.
 #include "common.cuh"
 
 namespace {

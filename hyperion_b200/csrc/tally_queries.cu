@@ -19,7 +19,7 @@
 //
 // Measured: three prompts of up to 2,047 tokens, 32 heads over 8 of 128, 123 us (both walks' products 0.6 PFLOP/s), of which either walk takes some 60.  In the loop a tile of 128 x 128 takes an SM
 // 950 to 1,150 clocks: 576 of them are its products, 730 its exponentials on the special function unit (11 of 16 pairs), some 700 its instructions; blocks of two halves with a buffer each do not quite keep them all
-// busy, and starts and ends of blocks cost another 15 %.  The last 32 of 8,192 tokens, 28 heads over 4: 18.5 us, three kernels' starts and trips to memory.  (With mma.sync and registers in place of tensor memory 890 and 49 us.)
+// busy, and starts and ends of blocks cost another 15 %.  The last 32 of 8,192 tokens, 28 heads over 4: 18.6 us, three kernels' starts and trips to memory.  (With mma.sync and registers in place of tensor memory 890 and 49 us.)
 //
 // Slots beyond a request's length may hold anything: their scores are not looked at.  Every wait is bounded; one that runs out sets HB_STATUS_WAIT_EXPIRED and the block leaves, once the copies and products that it
 // has on their way are done.
